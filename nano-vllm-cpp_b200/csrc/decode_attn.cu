@@ -171,6 +171,7 @@ __global__ void __launch_bounds__(kGroupThreads, F::kGroups) decode_cluster_kern
             waited = true;
         };
         auto push = [&](int h, int quad, const float4& o, float m, float l) {
+            if (F::kScores && quad == 0) p.ws_ml[(static_cast<size_t>(pair) * p.num_splits + rank) * p.group + h] = make_float2(m, l);
             if (n == 1) {
                 write_quad(out + h * kHeadDim + 4 * quad, scaled(o, 1.0f / l));   // (rounded as write_merged does)
                 return;

@@ -1,4 +1,4 @@
-// Device code of paged decode attention on tensor cores (F16 / BF16 queries, head_dim 128; 16-bit, int8 or e4m3 cache), shared
+// Device code of paged decode attention on tensor cores (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 or 4-bit cache), shared
 // by the decode kernels (decode_attn.cu) and the mixed prefill + decode kernel (prefill_attn_tc.cu).
 //
 // The op is HBM-bound: every K and V row of every context is read once.  A group of four warps takes a range of the keys of one
@@ -21,6 +21,8 @@
 
 #include "nvk_internal.cuh"
 
+#include <type_traits>
+
 namespace nvk {
 namespace dec {
 
@@ -33,7 +35,7 @@ constexpr int kMergeWarps = 8;         // warps that merge the parts of one (seq
 
 struct DecodeParams {
     const void* q; const void* k_cache; const void* v_cache;
-    const __half* k_scale; const __half* v_scale;      // 8-bit caches
+    const __half* k_scale; const __half* v_scale;      // 8-bit caches: a scale; 4-bit ones: a pair (step, low) in the queries' type, one 32-bit word
     IndexArray context_lens; IndexArray block_tables;
     void* out; float* ws_o; float2* ws_ml;             // partial results: [sequence][KV head][split][group][128] and (maximum, sum)
     int64_t max_blocks, num_cache_blocks;
@@ -44,6 +46,7 @@ struct DecodeParams {
     int chunk_major;                                   // decode_split_kernel's grid: all sequences' first chunks, then all second ones, ...
     int split_shift;                                   // clusters: log2 of num_splits
     int beside;                                        // waits at its end (pdl_wait_beside)
+    float* scores;                                     // where they are kept (F::kScores): [sequence][KV head][max_blocks * block_size][group], times log2(e)
     FastDiv by_block, by_kv_heads;
     float scale_log2;
 };
@@ -91,9 +94,9 @@ struct SoftmaxState {
         for (int i = 0; i < 8; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f; }
         m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f;
     }
-    // Scores of a tile: rescale where a maximum moves (a handful of tiles of a sequence; the branch is warp-uniform).  `extra`: further
-    // columns that are scaled along.
-    __device__ __forceinline__ void raise_max(const float (&sc)[4], float* extra) {
+    // Scores of a tile: rescale where a maximum moves (a handful of tiles of a sequence; the branch is warp-uniform).  `extra`: N further
+    // values that are scaled along, of heads 2t and 2t + 1 in turn.
+    template <int N = 4> __device__ __forceinline__ void raise_max(const float (&sc)[4], float* extra) {
         float top[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
         if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
             float c[2];
@@ -108,7 +111,10 @@ struct SoftmaxState {
             }
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) { o[mt][0] *= c[0]; o[mt][1] *= c[1]; o[mt][2] *= c[0]; o[mt][3] *= c[1]; }
-            if (extra != nullptr) { extra[0] *= c[0]; extra[1] *= c[1]; extra[2] *= c[0]; extra[3] *= c[1]; }
+            if (extra != nullptr) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) extra[i] *= c[i & 1];
+            }
         }
     }
 };
@@ -122,14 +128,40 @@ __device__ __forceinline__ void mask_scores(float (&sc)[4], int g, int valid) {
     }
 }
 
+// Scores that are kept: the warp's tiles are every fourth one, and a lane's place moves on with them.
+struct ScoreOut {
+    float* at;                                         // key g of the warp's next tile, head 2t
+    __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int token, int lane) {
+        const int64_t keys = p.max_blocks * p.block_size;
+        at = p.scores + ((static_cast<int64_t>(b) * p.num_kv_heads + kvh) * keys + token + (lane >> 2)) * p.group + 2 * (lane & 3);
+    }
+    __device__ __forceinline__ void put(const DecodeParams& p, const float (&sc)[4], int valid, int lane) {
+        const int g = lane >> 2, h = 2 * (lane & 3), group = p.group;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (g + 8 * i < valid && h < group) {
+                float* to = at + 8 * i * group;
+                if ((group & 1) == 0) {
+                    *reinterpret_cast<float2*>(to) = make_float2(sc[2 * i], sc[2 * i + 1]);
+                } else {
+                    to[0] = sc[2 * i];
+                    if (h + 1 < group) to[1] = sc[2 * i + 1];
+                }
+            }
+        }
+        at += kGroupWarps * kTileTokens * group;
+    }
+};
+
 // 16-bit cache.  K and V tiles of 16 x 256 bytes, XOR-swizzled by row; S^T = K Q^T as mma.sync m16n8k16: the 16 keys are the rows,
 // the (zero padded) query heads the 8 columns; O^T = V^T P^T with V^T taken straight from the row-major V tile by ldmatrix.trans and
 // P^T from S^T by two 8 x 8 transposes.  (Heads as the 16 rows need no transpose but twice the MMAs, half of them on padding, in a
 // chain twice as long.)  Even and odd k-steps have accumulators of their own: a step is a serial chain that few warps hide.
 // Measured: 37 sequences of up to 2048 keys 34.8 -> 33.7 us; 100 int8 ones of up to 4096, where the step is closer to the bound, 97 -> 89.
 // 8 warps per SM x 3 stages of 8 KiB: 128 KiB in flight.
-template <typename T>
+template <typename T, bool SCORES = false>
 struct Cache16 {
+    static constexpr bool kScores = SCORES;
     static constexpr int kGroups = 2;   // resident per SM
     static constexpr int kRowBytes = kHeadDim * 2;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
@@ -138,6 +170,7 @@ struct Cache16 {
     static constexpr int kPartStride = kHeadDim + 8;
 
     SoftmaxState s;
+    ScoreOut kept;       // (SCORES)
     uint32_t qa[8][2];   // head g of the 8-column B tile; zero from head G on
 
     __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
@@ -185,6 +218,7 @@ struct Cache16 {
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[i] = (s0[i] + s1[i]) * p.scale_log2;
         mask_scores(sc, lane >> 2, valid);
+        if constexpr (SCORES) kept.put(p, sc, valid, lane);
         s.raise_max(sc, nullptr);
         const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
@@ -197,6 +231,7 @@ struct Cache16 {
             mma_16816<T>(s.o[mt], a0, a1, a2, a3, pb0, pb1);
         }
     }
+    __device__ __forceinline__ void finish() {}   // (after the last tile, by the whole warp)
     // The warp's unnormalised output of head 2t + h.
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
 #pragma unroll
@@ -243,6 +278,7 @@ template <bool FP8> __device__ __forceinline__ uint32_t widen_pair_hi(uint32_t x
 // once, probabilities are <= 1.  12 warps per SM x 4 stages of 4.1 KiB: 148 KiB in flight.
 template <typename T, bool FP8>
 struct Cache8 {
+    static constexpr bool kScores = false;
     static constexpr int kGroups = 3;
     static constexpr int kRowBytes = kHeadDim;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
@@ -359,11 +395,185 @@ struct Cache8 {
         constexpr uint32_t kOnes = 0x3C003C00u;   // {1.0, 1.0}
         if (!FP8) mma_16816<__half>(osum, kOnes, kOnes, kOnes, kOnes, pb0, pb1);
     }
+    __device__ __forceinline__ void finish() {}
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
         const float off = kOffset * osum[h];
 #pragma unroll
         for (int i = 0; i < 8; i += 2)
             *reinterpret_cast<float4*>(row + 16 * g + 2 * i) = make_float4(s.o[i][h] - off, s.o[i][2 + h] - off, s.o[i + 1][h] - off, s.o[i + 1][2 + h] - off);
+    }
+};
+
+// 4-bit cache: per token and KV head 64 bytes of K, 64 of V (numbers n from 0 to 15, element 2i in the low half of byte i) and for each a
+// pair (step, low) in the queries' type; an element is low + step n.  The MMA operands are made from the nibbles in registers, in the queries'
+// type: a nibble moved into the top of the mantissa of 1.0 is 1 + n / 16 exactly (a shift and one three-input logic operation a pair), so
+//   q . x         = 16 step (q . (1 + n / 16)) + (low - 16 step) sum(q)
+//   sum_k p_k x_k = 16 sum_k p'_k (1 + n_k / 16) - 23.5 sum_k p'_k + sum_k p_k (low_k + 7.5 step_k),   p'_k = p_k step_k rounded to 16 bits
+// Queries and nibbles are exact, sums are fp32; p' is the one rounding to 16 bits (as with the other caches), and the middle of the range goes
+// in the fp32 sum at the right, so that what the rounding touches is no larger than the values' spread.  sum(p') comes from an MMA against
+// a row of ones, i.e. from exactly the p' that the others used.
+// As in Cache8 the order in which a contraction runs is free: of key row g lane t takes the 16-byte piece t, whose word w has the k-steps
+// 2w and 2w + 1 (register pair j: elements j and j + 4 of the word; the query fragment is loaded the same way).  Of V lane (g, t) takes 8 bytes,
+// d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; halves of two keys' words side by side, a nibble of both is one register, and
+// accumulator rows g / g + 8 of d-tile i hold d = 16 g + 2 i (+ 1).  The two rows of a 128-byte line of V are swizzled by the line's number,
+// so that these reads are conflict free.
+template <typename T> struct Nibbles;   // pair j of a word: nibble j of both halves -> 1 + n / 16
+template <> struct Nibbles<__nv_bfloat16> {   // mantissa bits 3 to 6
+    template <int J> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
+        constexpr int kLeft = 3 - 4 * J;
+        return ((kLeft > 0 ? x << (kLeft > 0 ? kLeft : 0) : x >> (kLeft > 0 ? 0 : -kLeft)) & 0x00780078u) | 0x3F803F80u;
+    }
+};
+template <> struct Nibbles<__half> {          // mantissa bits 6 to 9
+    template <int J> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
+        constexpr int kLeft = 6 - 4 * J;
+        return ((kLeft > 0 ? x << (kLeft > 0 ? kLeft : 0) : x >> (kLeft > 0 ? 0 : -kLeft)) & 0x03C003C0u) | 0x3C003C00u;
+    }
+};
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+template <typename T, bool SCORES = false>
+struct Cache4 {
+    static constexpr bool kScores = SCORES;
+    static constexpr int kGroups = 3;
+    static constexpr int kRowBytes = kHeadDim / 2;
+    static constexpr int kTileBytes = kTileTokens * kRowBytes;
+    static constexpr int kParamBytes = 2 * kTileTokens * 4;   // (step, low) of (K | V, token)
+    static constexpr int kStageBytes = 2 * kTileBytes + kParamBytes;
+    static constexpr int kStages = 6;
+    static constexpr int kPartStride = kHeadDim + 4;
+
+    SoftmaxState s;
+    ScoreOut kept;       // (SCORES)
+    float more[6];       // 0..3: sum(p') from the ones MMA; 4, 5: sum(p (low + 7.5 step)) of heads 2t, 2t + 1 over the lane's keys
+    float q_sum[2];
+    uint32_t qa[8][2];   // k-step 2 w + e: elements 32 t + 8 w + 2 e + {0, 4 | 1, 5}
+
+    __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        const bool live = g < p.group;
+        const uint4* row = reinterpret_cast<const uint4*>(
+            static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.num_heads + kvh * p.group + (live ? g : 0)) * kHeadDim) + 4 * t;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const uint4 v = live ? row[w] : make_uint4(0u, 0u, 0u, 0u);
+            qa[2 * w][0] = __byte_perm(v.x, v.z, 0x5410);
+            qa[2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
+            qa[2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
+            qa[2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<T>(qa[2 * w + (e >> 1)][e & 1]);
+                sum += f.x + f.y;
+            }
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+        q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+#pragma unroll
+        for (int i = 0; i < 6; ++i) more[i] = 0.0f;
+        s.reset();
+    }
+    static __device__ __forceinline__ void issue(const DecodeParams& p, int kvh, int64_t row0, int valid, uint32_t stage, int lane) {
+        const size_t stride = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
+        const int c = lane & 3, rq = lane >> 2;   // 16-byte piece c of rows rq, rq + 8
+        const size_t base = static_cast<size_t>(row0) * stride + static_cast<size_t>(kvh) * kRowBytes + c * 16;
+        const unsigned char* kc = static_cast<const unsigned char*>(p.k_cache) + base;
+        const unsigned char* vc = static_cast<const unsigned char*>(p.v_cache) + base;
+        const uint32_t vpiece = (((rq & 1) << 2) + c) ^ (((rq >> 1) & 3) << 1);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 8 * i + rq;
+            const int bytes = r < valid ? 16 : 0;
+            const size_t src = bytes ? r * stride : 0;
+            cp_async16(stage + r * kRowBytes + c * 16, kc + src, bytes);
+            cp_async16(stage + kTileBytes + (r >> 1) * 128 + vpiece * 16, vc + src, bytes);
+        }
+        const int tr = lane & 15;                 // lanes 0-15 K, lanes 16-31 V
+        const int pbytes = tr < valid ? 4 : 0;
+        const size_t at = pbytes ? (static_cast<size_t>(row0) + tr) * p.num_kv_heads + kvh : 0;
+        cp_async4(stage + 2 * kTileBytes + lane * 4, reinterpret_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + at, pbytes);
+    }
+    __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int /*kvh*/, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+            uint32_t w0[4], w1[4];
+            lds32x4(stage + g * kRowBytes + t * 16, w0);
+            lds32x4(stage + (g + 8) * kRowBytes + t * 16, w1);
+            using N = Nibbles<T>;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                mma_16816<T>(s0, N::template pair<0>(w0[w]), N::template pair<0>(w1[w]), N::template pair<1>(w0[w]), N::template pair<1>(w1[w]), qa[2 * w][0],
+                             qa[2 * w][1]);
+                mma_16816<T>(s1, N::template pair<2>(w0[w]), N::template pair<2>(w1[w]), N::template pair<3>(w0[w]), N::template pair<3>(w1[w]), qa[2 * w + 1][0],
+                             qa[2 * w + 1][1]);
+            }
+        }
+        float2 kp[2], vp[2];                      // (step, low) of keys g and g + 8
+        {
+            uint32_t w[4];
+            const uint32_t at = stage + 2 * kTileBytes + g * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[i]) : "r"(at + i * 32));
+#pragma unroll
+            for (int i = 0; i < 2; ++i) { kp[i] = unpack2<T>(w[i]); vp[i] = unpack2<T>(w[2 + i]); }
+        }
+        float sc[4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float step16 = 16.0f * kp[i].x * p.scale_log2, low16 = fmaf(kp[i].x, -16.0f, kp[i].y) * p.scale_log2;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(s0[2 * i + h] + s1[2 * i + h], step16, low16 * q_sum[h]);
+        }
+        mask_scores(sc, g, valid);
+        if constexpr (SCORES) kept.put(p, sc, valid, lane);
+        s.template raise_max<6>(sc, more);
+        const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
+        s.l[0] += p0 + p2;
+        s.l[1] += p1 + p3;
+        const float mid0 = fmaf(vp[0].x, 7.5f, vp[0].y), mid1 = fmaf(vp[1].x, 7.5f, vp[1].y);
+        more[4] = fmaf(p0, mid0, fmaf(p2, mid1, more[4]));
+        more[5] = fmaf(p1, mid0, fmaf(p3, mid1, more[5]));
+        const uint32_t pb0 = transpose_8x8(ElemTraits<T>::pack2(p0 * vp[0].x, p1 * vp[0].x));
+        const uint32_t pb1 = transpose_8x8(ElemTraits<T>::pack2(p2 * vp[1].x, p3 * vp[1].x));
+        // V rows 2t, 2t + 1 (line t) and 2t + 8, 2t + 9 (line t + 4), words 2g and 2g + 1: half of piece g / 2
+        const uint32_t v_at = stage + kTileBytes + t * 128 + (g & 1) * 8, even = ((g >> 1) ^ (t << 1)) << 4;
+        uint2 x[4];
+        auto lds64 = [](uint32_t addr, uint2& v) { asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr)); };
+        lds64(v_at + even, x[0]);
+        lds64(v_at + (even ^ 64), x[1]);
+        lds64(v_at + 512 + even, x[2]);
+        lds64(v_at + 512 + (even ^ 64), x[3]);
+        auto four = [&](uint32_t k01, uint32_t k89, int i) {   // d-tiles i and i + 1 of two keys' halves side by side
+            using N = Nibbles<T>;
+            mma_16816<T>(s.o[i], N::template pair<0>(k01), N::template pair<1>(k01), N::template pair<0>(k89), N::template pair<1>(k89), pb0, pb1);
+            mma_16816<T>(s.o[i + 1], N::template pair<2>(k01), N::template pair<3>(k01), N::template pair<2>(k89), N::template pair<3>(k89), pb0, pb1);
+        };
+        four(__byte_perm(x[0].x, x[1].x, 0x5410), __byte_perm(x[2].x, x[3].x, 0x5410), 0);
+        four(__byte_perm(x[0].x, x[1].x, 0x7632), __byte_perm(x[2].x, x[3].x, 0x7632), 2);
+        four(__byte_perm(x[0].y, x[1].y, 0x5410), __byte_perm(x[2].y, x[3].y, 0x5410), 4);
+        four(__byte_perm(x[0].y, x[1].y, 0x7632), __byte_perm(x[2].y, x[3].y, 0x7632), 6);
+        constexpr uint32_t kOnes = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
+        mma_16816<T>(*reinterpret_cast<float (*)[4]>(more), kOnes, kOnes, kOnes, kOnes, pb0, pb1);
+    }
+    __device__ __forceinline__ void finish() {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) more[4 + h] += __shfl_xor_sync(0xffffffffu, more[4 + h], x);
+        }
+    }
+    __device__ __forceinline__ void write_part(float* row, int h, int g) const {
+        const float off = fmaf(more[h], -23.5f, more[4 + h]);
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            *reinterpret_cast<float4*>(row + 16 * g + 2 * i) = make_float4(fmaf(s.o[i][h], 16.0f, off), fmaf(s.o[i][2 + h], 16.0f, off),
+                                                                           fmaf(s.o[i + 1][h], 16.0f, off), fmaf(s.o[i + 1][2 + h], 16.0f, off));
     }
 };
 
@@ -423,6 +633,7 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
 
     F st;
     st.start(p, b, kvh, lane);
+    if constexpr (F::kScores) st.kept.start(p, b, kvh, t0 + warp * kTileTokens, lane);
     uint32_t cstage = ring;
     int left = t1 - t0 - warp * kTileTokens;   // keys from this warp's tile on
     for (int j = 0; j < my_tiles; ++j) {
@@ -436,6 +647,7 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
     }
     cp_async_wait<0>();
     __syncwarp();                              // this warp's ring is idle from here on
+    st.finish();
     const int g = lane >> 2, t = lane & 3;
     auto& part = sm.warps[warp].part;
 #pragma unroll
@@ -509,8 +721,9 @@ __device__ __forceinline__ void run_split(const DecodeParams& p, int b, int kvh,
             write_quad(out + h * kHeadDim + 4 * quad, scaled(o, 1.0f / l));   // (rounded as write_merged does)
         } else {
             reinterpret_cast<float4*>(p.ws_o + (part * p.group + h) * kHeadDim)[quad] = o;
-            if (quad == 0) p.ws_ml[part * p.group + h] = make_float2(m, l);
+            if (!F::kScores && quad == 0) p.ws_ml[part * p.group + h] = make_float2(m, l);
         }
+        if (F::kScores && quad == 0) p.ws_ml[part * p.group + h] = make_float2(m, l);   // (the weights of the keys need them, however many parts there are)
     });
 }
 
