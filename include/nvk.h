@@ -166,6 +166,84 @@ int nvk_decode_attention_paged_fp8(const void* query, const void* k_cache, const
                                    int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * 4-bit KV cache.  NO COUNTERPART IN THE REFERENCE.  Per token and KV head 64 bytes of K and 64 of V, and for each a pair of the keys' type (3.76 times
+ * less than a 16-bit cache):
+ *   k_cache, v_cache   bytes [cache_rows, num_kv_heads, head_dim / 2], two numbers n from 0 to 15 each: element 2i in the low half of byte i
+ *   k_params, v_params [cache_rows, num_kv_heads, 2] of `dtype`: (step, low) of the head vector; an element is low + step * n
+ * A vector x is stored as low = min x, step = (max x - min x) / 15 (in fp32, rounded to the type), n = min(15, floor((x - low) / step + 1/2)), the
+ * quotient being the exact one; n = 0 where step is 0.  A vector whose range is not finite (it holds an infinity or a NaN, or spans more than fp32
+ * can hold) gets a pair of NaN and reads as NaN.
+ * F16 / BF16 and head_dim 128 only (NVK_ERR_UNSUPPORTED otherwise).  Every tensor but the params starts on a 16-byte boundary, the params on a
+ * 4-byte one.
+ *
+ * nvk_store_kvcache_int4: key, value [num_tokens, num_kv_heads, 128]; slot_mapping int32 / int64; tokens with a slot < 0 or >= cache_rows are skipped
+ * (two tokens of a call with the same slot: undefined which one is stored).  num_tokens 0 does nothing.
+ *
+ * nvk_gather_kvcache_int4: the keys and values of whole contexts as dense 16-bit rows, for a prefill over cached prefixes: row cu_seqlens_k[s] + i of
+ * key / value [total_k, num_kv_heads, 128] is key i of sequence s, low + step * n rounded to `dtype`; then nvk_prefill_attention_varlen with those rows
+ * and the same cu_seqlens_k.  cu_seqlens_k [num_seqs + 1] ascending from 0, block_tables [num_seqs, max_blocks].  Rows behind the last sequence and
+ * rows whose table entry is outside the cache or the table are zeros; sequences are cut off at total_k.
+ *
+ * nvk_decode_attention_paged_int4: the semantics of nvk_decode_attention_paged over the elements as they are (low + step * n is not rounded); at most
+ * 8 query heads per KV head, block_size a multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes).
+ */
+int nvk_store_kvcache_int4(const void* key, const void* value, void* k_cache, void* v_cache, void* k_params, void* v_params,
+                           const void* slot_mapping, int slot_dtype, int64_t num_tokens, int num_kv_heads, int head_dim, int64_t cache_rows,
+                           int dtype, void* stream);
+int nvk_gather_kvcache_int4(const void* k_cache, const void* v_cache, const void* k_params, const void* v_params, const void* cu_seqlens_k,
+                            int cu_seqlens_k_dtype, const void* block_tables, int block_tables_dtype, int64_t num_seqs, int64_t total_k,
+                            int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int head_dim, int block_size, void* key, void* value,
+                            int dtype, void* stream);
+int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, const void* v_cache, const void* k_params, const void* v_params,
+                                    const void* context_lens, int context_lens_dtype, const void* block_tables, int block_tables_dtype,
+                                    int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads, int num_kv_heads,
+                                    int head_dim, int block_size, float scale, void* output, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/*
+ * Eviction from a cache by accumulated attention weight.  NO COUNTERPART IN THE REFERENCE.  Decode steps add up, for every key of a KV head, the
+ * attention weights that the head's queries give it; when a context has outgrown its budget the keys with the least go, each KV head's own.
+ * Both calls take a 16-bit cache (k_params and v_params NULL) or a 4-bit one; F16 / BF16, head_dim 128.
+ *
+ * nvk_decode_attention_paged_weights: nvk_decode_attention_paged (or _int4), and
+ *   new_key_weights[row, j, k] = key_weights[row, j, k] + sum over query heads h of KV head j of softmax(scale * q[b, h] . K)[k],  k < context_lens[b]
+ *   key_weights, new_key_weights   fp32 [num_weight_rows, num_kv_heads, weight_row_keys], weight_row_keys >= max_blocks * block_size; key_weights may
+ *                                  be NULL (zeros) and may be new_key_weights (in place); otherwise the two do not overlap
+ *   weight_rows                    [batch] int32 / int64, the row of each sequence (a sequence keeps its row while its place in the batch changes), or
+ *                                  NULL: sequence b has row b.  A row < 0 or >= num_weight_rows: nothing is added up (padding).  No two sequences
+ *                                  of a call share a row.
+ * Weights of keys from context_lens[b] on are left as they are.  Sums are fp32, each key's in the order of the heads: bit for bit the same in every
+ * run.  The workspace (nvk_decode_attention_weights_workspace_bytes, 16-byte aligned, required) holds the step's scores; its size covers every call with no
+ * more sequences and no wider tables.  At most 8 query heads per KV head, block_size a multiple of 16.
+ *
+ * nvk_evict_kvcache: of a context of n > budget keys, for each KV head, stay the first `sinks`, the last `recent`, and of those between the ones of the
+ * largest weights, `budget` in all (of equal weights the key that comes first; NaN is less than any other).  They close up in their order: key i of
+ * those that stay goes to position i of the sequence in new_block_tables, its weight to new_key_weights[row, j, i]; the rest of that row of weights is
+ * set to zero.  new_context_lens[b] = min(n, budget) (dtype of context_lens, not the same memory).  Contexts of up to `budget` keys stay whole, and are
+ * copied where the new blocks are others.
+ *   new_block_tables [batch, new_max_blocks]: the same tensor as block_tables (in place: what lies behind position `budget` is left as it is, and the
+ *   caller frees those blocks), or tables of blocks that are in no context of the call.  Blocks that are written must belong to one sequence of the call
+ *   only: a cached prefix that sequences share is evicted into other blocks.  Rows whose old table entry is outside the cache are written as zeros,
+ *   rows whose new one is are not written.  new_key_weights: the same as key_weights, or not overlapping with it.
+ *   A sequence whose weight row is < 0 or >= num_weight_rows is left alone: nothing moves, new_context_lens[b] = n.
+ *   0 <= sinks, 0 <= recent, sinks + recent <= budget, budget >= 1; new_max_blocks * block_size >= budget, or new_max_blocks >= max_blocks.
+ */
+size_t nvk_decode_attention_weights_workspace_bytes(int64_t batch, int num_heads, int num_kv_heads, int head_dim, int64_t max_blocks,
+                                                    int block_size);
+int nvk_decode_attention_paged_weights(const void* query, const void* k_cache, const void* v_cache, const void* k_params, const void* v_params,
+                                       const void* context_lens, int context_lens_dtype, const void* block_tables, int block_tables_dtype,
+                                       int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads, int num_kv_heads,
+                                       int head_dim, int block_size, float scale, const float* key_weights, const void* weight_rows,
+                                       int weight_rows_dtype, int64_t num_weight_rows, int64_t weight_row_keys, float* new_key_weights,
+                                       void* output, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int nvk_evict_kvcache(void* k_cache, void* v_cache, void* k_params, void* v_params, const float* key_weights, const void* weight_rows,
+                      int weight_rows_dtype, int64_t num_weight_rows, int64_t weight_row_keys, const void* context_lens, int context_lens_dtype,
+                      const void* block_tables, int block_tables_dtype, int64_t batch, int64_t max_blocks, int64_t num_cache_blocks,
+                      float* new_key_weights, const void* new_block_tables, int new_block_tables_dtype, int64_t new_max_blocks,
+                      void* new_context_lens, int num_kv_heads, int head_dim, int block_size, int64_t budget, int64_t sinks, int64_t recent,
+                      int dtype, void* stream);
+
+/*
  * Same computation as nvk_decode_attention_paged for callers that cannot provide a workspace and
  * must not allocate device memory.  (No counterpart in the reference: its decode entry point simply
  * has no scratch.)  Typical callers: a wrapper with the reference's launch_decode_attention_paged

@@ -37,6 +37,8 @@ EXPORTED_SYMBOLS = (
     "nvk_tp_row_linear_allreduce_add_rmsnorm_inprocess", "nvk_gemm_status",
     "nvk_tp_allreduce_signal_bytes", "nvk_tp_allreduce_multimem", "nvk_tp_allreduce_add_rmsnorm_multimem",
     "nvk_store_kvcache_fp8", "nvk_decode_attention_paged_fp8",
+    "nvk_store_kvcache_int4", "nvk_gather_kvcache_int4", "nvk_decode_attention_paged_int4",
+    "nvk_decode_attention_weights_workspace_bytes", "nvk_decode_attention_paged_weights", "nvk_evict_kvcache",
 )
 
 _lib = None
@@ -62,6 +64,8 @@ def lib() -> ctypes.CDLL:
         L.nvk_decode_attention_workspace_bytes.restype = ctypes.c_size_t
         L.nvk_decode_attention_workspace_bytes.argtypes = [
             ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int]
+        L.nvk_decode_attention_weights_workspace_bytes.restype = ctypes.c_size_t
+        L.nvk_decode_attention_weights_workspace_bytes.argtypes = L.nvk_decode_attention_workspace_bytes.argtypes
         L.nvk_decode_attention_static_scratch_bytes.restype = ctypes.c_size_t
         _lib = L
     return _lib
@@ -175,6 +179,60 @@ def launch_decode_attention_paged_fp8(query, k_cache, v_cache, k_scale, v_scale,
     launch_count += (_binding or _load_binding()).decode_fp8(
         query, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale,
         output, workspace)
+
+
+def store_kvcache_int4(key, value, k_cache, v_cache, k_params, v_params, slot_mapping) -> None:
+    """Quantising scatter into 4-bit caches (uint8 [..., Hkv, D / 2]) + (step, low) pairs of the keys' type [..., Hkv, 2]
+    (``nvk_store_kvcache_int4``)."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).store_int4(key, value, k_cache, v_cache, k_params, v_params, slot_mapping)
+
+
+def gather_kvcache_int4(k_cache, v_cache, k_params, v_params, cu_seqlens_k, block_tables, num_kv_heads, head_dim, block_size, key,
+                        value) -> None:
+    """Whole contexts of a 4-bit cache as dense 16-bit rows, sequence after sequence (``nvk_gather_kvcache_int4``): what
+    :func:`launch_prefill_attention_dense` then attends over.  Rows of ``key`` / ``value`` behind the last sequence become zeros."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).gather_int4(
+        k_cache, v_cache, k_params, v_params, cu_seqlens_k, block_tables, num_kv_heads, head_dim, block_size, key, value)
+
+
+def launch_decode_attention_paged_int4(query, k_cache, v_cache, k_params, v_params, context_lens, block_tables,
+                                       num_kv_heads, head_dim, block_size, scale, output, workspace=None) -> None:
+    """Paged decode attention over a 4-bit cache (``nvk_decode_attention_paged_int4``), with the optional split-K workspace
+    of :func:`launch_decode_attention_paged`."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).decode_int4(
+        query, k_cache, v_cache, k_params, v_params, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale,
+        output, workspace)
+
+
+def decode_attention_weights_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_blocks, block_size) -> int:
+    return int(lib().nvk_decode_attention_weights_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_blocks, block_size))
+
+
+def launch_decode_attention_paged_weights(query, k_cache, v_cache, k_params, v_params, context_lens, block_tables, num_kv_heads,
+                                          head_dim, block_size, scale, key_weights, weight_rows, new_key_weights, output,
+                                          workspace) -> None:
+    """Paged decode attention that adds up every key's attention weights (``nvk_decode_attention_paged_weights``):
+    ``new_key_weights = key_weights +`` the sum over the query heads of each KV head, fp32 [rows, Hkv, keys].  ``k_params`` and
+    ``v_params`` None: a 16-bit cache; ``key_weights`` None: zeros (it may also be ``new_key_weights``); ``weight_rows`` None:
+    sequence b has row b.  ``workspace``: uint8, ``decode_attention_weights_workspace_bytes`` bytes."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).decode_weights(
+        query, k_cache, v_cache, k_params, v_params, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale,
+        key_weights, weight_rows, new_key_weights, output, workspace)
+
+
+def evict_kvcache(k_cache, v_cache, k_params, v_params, key_weights, weight_rows, context_lens, block_tables, new_key_weights,
+                  new_block_tables, new_context_lens, num_kv_heads, head_dim, block_size, budget, sinks, recent) -> None:
+    """Eviction by accumulated attention weight (``nvk_evict_kvcache``): of every sequence and KV head the first ``sinks`` keys, the
+    last ``recent`` and the heaviest between them stay, ``budget`` in all, and close up in the blocks of ``new_block_tables``
+    (which may be ``block_tables``), their weights in ``new_key_weights`` (which may be ``key_weights``)."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).evict(
+        k_cache, v_cache, k_params, v_params, key_weights, weight_rows, context_lens, block_tables, new_key_weights, new_block_tables,
+        new_context_lens, num_kv_heads, head_dim, block_size, budget, sinks, recent)
 
 
 def _prefill(query, key, value, k_cache, v_cache, cu_q, cu_k, block_tables, num_kv_heads, head_dim,

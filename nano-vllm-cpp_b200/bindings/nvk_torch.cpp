@@ -214,6 +214,140 @@ template <bool FP8> long store8(PyObject* const* a) {
     return 1;
 }
 
+// ---- 4-bit caches ----
+void check_bytes(const char* name, const at::Tensor& t) {
+    if (t.element_size() != 1) raise(PyExc_ValueError, "%s must have one-byte elements", name);
+}
+// The params of a cache of `rows` head vectors, in the type of its keys.
+void check_params(const char* name, const at::Tensor& t, at::ScalarType type, int64_t vectors) {
+    if (t.scalar_type() != type) raise(PyExc_ValueError, "%s must have the type of the keys", name);
+    if (t.numel() != 2 * vectors) raise(PyExc_ValueError, "%s must have two elements for every head vector of the cache", name);
+}
+// Rows of 4-bit caches of `hkv` heads of `d` elements; caches and params agree.
+int64_t rows4(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& kp, const at::Tensor& vp, at::ScalarType type, int64_t hkv, int64_t d) {
+    check_bytes("k_cache", kc);
+    check_bytes("v_cache", vc);
+    if (d <= 0 || d % 2 != 0 || hkv <= 0) raise(PyExc_ValueError, "%s", "num_kv_heads must be positive and head_dim even");
+    const int64_t row = hkv * (d / 2);
+    if (kc.numel() % row != 0 || kc.numel() != vc.numel()) raise(PyExc_ValueError, "%s", "k_cache does not contain an integer number of cache rows");
+    check_params("k_params", kp, type, kc.numel() / row * hkv);
+    check_params("v_params", vp, type, kc.numel() / row * hkv);
+    return kc.numel() / row;
+}
+
+// (key, value, k_cache, v_cache, k_params, v_params, slot_mapping)
+long store_int4(PyObject* const* a) {
+    const at::Tensor &key = cuda("key", a[0]), &value = cuda("value", a[1]), &kc = cuda("k_cache", a[2]), &vc = cuda("v_cache", a[3]),
+                     &kp = cuda("k_params", a[4]), &vp = cuda("v_params", a[5]), &slots = cuda("slot_mapping", a[6]);
+    if (key.dim() != 3) raise(PyExc_ValueError, "key must be rank-3 for %s store", "the int4");
+    if (!key.sizes().equals(value.sizes()) || key.scalar_type() != value.scalar_type())
+        raise(PyExc_ValueError, "%s", "key and value must have the same shape and dtype");
+    if (slots.numel() != key.size(0)) raise(PyExc_ValueError, "%s", "slot_mapping must have an element for every token");
+    const Index index("slot_mapping", &slots);
+    const int64_t hkv = key.size(1), d = key.size(2), rows = rows4(kc, vc, kp, vp, key.scalar_type(), hkv, d);
+    if (slots.numel() == 0) return 0;
+    launch(nvk_store_kvcache_int4, ptr(key), ptr(value), ptr(kc), ptr(vc), ptr(kp), ptr(vp), index.p, index.dtype, slots.numel(), static_cast<int>(hkv),
+           static_cast<int>(d), rows, code(key), stream());
+    return 1;
+}
+
+// (k_cache, v_cache, k_params, v_params, cu_seqlens_k, block_tables, num_kv_heads, head_dim, block_size, key, value)
+long gather_int4(PyObject* const* a) {
+    const at::Tensor &kc = cuda("k_cache", a[0]), &vc = cuda("v_cache", a[1]), &kp = cuda("k_params", a[2]), &vp = cuda("v_params", a[3]),
+                     &cu = cuda("cu_seqlens_k", a[4]), &bt = cuda("block_tables", a[5]), &key = cuda("key", a[9]), &value = cuda("value", a[10]);
+    const int64_t hkv = integer(a[6]), d = integer(a[7]), bs = integer(a[8]);
+    const Index starts("cu_seqlens_k", &cu), tables("block_tables", &bt);
+    if (bs <= 0) raise(PyExc_ValueError, "%s", "block_size must be positive");
+    const int64_t blocks = rows4(kc, vc, kp, vp, key.scalar_type(), hkv, d) / bs;
+    if (!key.sizes().equals(value.sizes()) || key.scalar_type() != value.scalar_type() || key.dim() != 3 || key.size(1) != hkv || key.size(2) != d)
+        raise(PyExc_ValueError, "%s", "key and value must be [total_k, num_kv_heads, head_dim] of one dtype");
+    if (cu.numel() < 2 || bt.dim() != 2 || bt.size(0) != cu.numel() - 1)
+        raise(PyExc_ValueError, "%s", "block_tables must have a row for every sequence of cu_seqlens_k");
+    if (key.size(0) == 0) return 0;
+    launch(nvk_gather_kvcache_int4, ptr(kc), ptr(vc), ptr(kp), ptr(vp), starts.p, starts.dtype, tables.p, tables.dtype, cu.numel() - 1, key.size(0),
+           bt.size(1), blocks, static_cast<int>(hkv), static_cast<int>(d), static_cast<int>(bs), ptr(key), ptr(value), code(key), stream());
+    return 1;
+}
+
+// Sequences of a decode call: as many contexts, tables and outputs as queries.
+void check_rows(const Decode& x) {
+    if (x.ctx.numel() != x.batch || x.bt.dim() != 2 || x.bt.size(0) != x.batch)
+        raise(PyExc_ValueError, "%s", "context_lens and block_tables must have a row for every query");
+    if (x.q.dim() != 3 || x.q.size(2) != x.d || !x.out.sizes().equals(x.q.sizes()) || x.out.scalar_type() != x.q.scalar_type())
+        raise(PyExc_ValueError, "%s", "query must be [batch, num_heads, head_dim], output of its shape and dtype");
+}
+
+// (query, k_cache, v_cache, k_params, v_params, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale, output, workspace)
+long decode_int4(PyObject* const* a) {
+    const Decode x(a[0], a[1], a[2], a[5], a[6], a[11], a[7], a[8], a[9], a[10]);
+    const at::Tensor &kp = cuda("k_params", a[3]), &vp = cuda("v_params", a[4]);
+    const at::Tensor* ws = optional_cuda("workspace", a[12]);
+    check_rows(x);
+    const int64_t blocks = rows4(x.kc, x.vc, kp, vp, x.q.scalar_type(), x.hkv, x.d) / x.bs;
+    launch(nvk_decode_attention_paged_int4, ptr(x.q), ptr(x.kc), ptr(x.vc), ptr(kp), ptr(vp), x.lens.p, x.lens.dtype, x.tables.p, x.tables.dtype, x.batch,
+           x.max_blocks, blocks, static_cast<int>(x.heads), static_cast<int>(x.hkv), static_cast<int>(x.d), static_cast<int>(x.bs), x.scale, ptr(x.out),
+           code(x.q), ptr(ws), bytes(ws), stream());
+    return x.launches(ws);
+}
+
+// Weights of keys [rows, hkv, keys], fp32.
+const at::Tensor& weights_of(const char* name, PyObject* o, int64_t hkv) {
+    const at::Tensor& t = cuda(name, o);
+    if (t.scalar_type() != at::kFloat || t.dim() != 3 || t.size(1) != hkv) raise(PyExc_ValueError, "%s must be float32 [rows, num_kv_heads, keys]", name);
+    return t;
+}
+
+// (query, k_cache, v_cache, k_params, v_params, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale, key_weights, weight_rows,
+//  new_key_weights, output, workspace)
+long decode_weights(PyObject* const* a) {
+    const Decode x(a[0], a[1], a[2], a[5], a[6], a[14], a[7], a[8], a[9], a[10]);
+    const at::Tensor *kp = optional_cuda("k_params", a[3]), *vp = optional_cuda("v_params", a[4]), *rows = optional_cuda("weight_rows", a[12]);
+    const at::Tensor &to = weights_of("new_key_weights", a[13], x.hkv), &ws = cuda("workspace", a[15]);
+    const at::Tensor* from = a[11] == Py_None ? nullptr : &weights_of("key_weights", a[11], x.hkv);
+    check_rows(x);
+    if (from != nullptr && !from->sizes().equals(to.sizes())) raise(PyExc_ValueError, "%s", "key_weights and new_key_weights must have the same shape");
+    if (rows != nullptr && rows->numel() != x.batch) raise(PyExc_ValueError, "%s", "weight_rows must have an element for every query");
+    if ((kp == nullptr) != (vp == nullptr)) raise(PyExc_ValueError, "%s", "k_params and v_params go together");
+    const Index index("weight_rows", rows);
+    int64_t blocks = x.blocks;
+    if (kp != nullptr) {
+        blocks = rows4(x.kc, x.vc, *kp, *vp, x.q.scalar_type(), x.hkv, x.d) / x.bs;
+    } else if (x.kc.scalar_type() != x.q.scalar_type() || x.vc.scalar_type() != x.q.scalar_type() || x.kc.numel() != x.vc.numel()) {
+        raise(PyExc_ValueError, "%s", "k_cache and v_cache must have the dtype of the query and the same size");
+    }
+    launch(nvk_decode_attention_paged_weights, ptr(x.q), ptr(x.kc), ptr(x.vc), ptr(kp), ptr(vp), x.lens.p, x.lens.dtype, x.tables.p, x.tables.dtype, x.batch,
+           x.max_blocks, blocks, static_cast<int>(x.heads), static_cast<int>(x.hkv), static_cast<int>(x.d), static_cast<int>(x.bs), x.scale,
+           static_cast<const float*>(ptr(from)), index.p, index.dtype, to.size(0), to.size(2), static_cast<float*>(ptr(to)), ptr(x.out), code(x.q), ptr(ws),
+           ws.nbytes(), stream());
+    return x.launches(&ws) + 1;
+}
+
+// (k_cache, v_cache, k_params, v_params, key_weights, weight_rows, context_lens, block_tables, new_key_weights, new_block_tables, new_context_lens,
+//  num_kv_heads, head_dim, block_size, budget, sinks, recent)
+long evict(PyObject* const* a) {
+    const at::Tensor &kc = cuda("k_cache", a[0]), &vc = cuda("v_cache", a[1]), &ctx = cuda("context_lens", a[6]), &bt = cuda("block_tables", a[7]),
+                     &new_bt = cuda("new_block_tables", a[9]), &new_ctx = cuda("new_context_lens", a[10]);
+    const at::Tensor *kp = optional_cuda("k_params", a[2]), *vp = optional_cuda("v_params", a[3]), *rows = optional_cuda("weight_rows", a[5]);
+    const int64_t hkv = integer(a[11]), d = integer(a[12]), bs = integer(a[13]);
+    const at::Tensor &from = weights_of("key_weights", a[4], hkv), &to = weights_of("new_key_weights", a[8], hkv);
+    const Index lens("context_lens", &ctx), tables("block_tables", &bt), new_tables("new_block_tables", &new_bt), index("weight_rows", rows);
+    if (!from.sizes().equals(to.sizes())) raise(PyExc_ValueError, "%s", "key_weights and new_key_weights must have the same shape");
+    if ((kp == nullptr) != (vp == nullptr)) raise(PyExc_ValueError, "%s", "k_params and v_params go together");
+    if (bs <= 0) raise(PyExc_ValueError, "%s", "block_size must be positive");
+    const int64_t batch = ctx.numel();
+    if (bt.dim() != 2 || new_bt.dim() != 2 || bt.size(0) != batch || new_bt.size(0) != batch || (rows != nullptr && rows->numel() != batch))
+        raise(PyExc_ValueError, "%s", "block_tables, new_block_tables and weight_rows must have a row for every context length");
+    if (new_ctx.scalar_type() != ctx.scalar_type() || new_ctx.numel() != batch) raise(PyExc_ValueError, "%s", "new_context_lens must be like context_lens");
+    if (kp == nullptr && (kc.scalar_type() != vc.scalar_type() || kc.numel() != vc.numel())) raise(PyExc_ValueError, "%s", "k_cache and v_cache must be alike");
+    const int64_t blocks = kp != nullptr ? rows4(kc, vc, *kp, *vp, kp->scalar_type(), hkv, d) / bs : cache_blocks(kc, bs, hkv, d);
+    if (batch == 0) return 0;
+    launch(nvk_evict_kvcache, ptr(kc), ptr(vc), ptr(kp), ptr(vp), static_cast<const float*>(ptr(from)), index.p, index.dtype, to.size(0), to.size(2), lens.p,
+           lens.dtype, tables.p, tables.dtype, batch, bt.size(1), blocks, static_cast<float*>(ptr(to)), new_tables.p, new_tables.dtype, new_bt.size(1),
+           ptr(new_ctx), static_cast<int>(hkv), static_cast<int>(d), static_cast<int>(bs), integer(a[14]), integer(a[15]), integer(a[16]),
+           code(kp != nullptr ? *kp : kc), stream());
+    return 1;
+}
+
 // (query, key, value, k_cache, v_cache, cu_q, cu_k, block_tables, num_kv_heads, head_dim, block_size, scale, output, max_seqlen_q)
 long prefill(PyObject* const* a) {
     const at::Tensor &q = cuda("query", a[0]), &out = cuda("output", a[12]);
@@ -300,6 +434,11 @@ PyMethodDef methods[] = {
     method<decode8<true>, 13>("decode_fp8"),
     method<store8<false>, 7>("store_int8"),
     method<store8<true>, 7>("store_fp8"),
+    method<store_int4, 7>("store_int4"),
+    method<gather_int4, 11>("gather_int4"),
+    method<decode_int4, 13>("decode_int4"),
+    method<decode_weights, 16>("decode_weights"),
+    method<evict, 17>("evict"),
     method<prefill, 14>("prefill"),
     method<mixed_step, 19>("mixed_step"),
     method<linear, 3>("linear"),

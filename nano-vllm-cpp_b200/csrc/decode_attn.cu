@@ -409,8 +409,9 @@ int check_grid(const DecodeArgs& a, const dec::DecodeParams& p) {   // of decode
     return NVK_OK;
 }
 
+// `scores`, `ml`: where they are kept (F::kScores), and the (maximum, sum) of every part; *plan: how the step was shared out.
 template <class F, typename T>
-int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale) {
+int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, float* scores = nullptr, float2* ml = nullptr, DecodeParams* plan = nullptr) {
     constexpr int kSmem = static_cast<int>(sizeof(GroupSmem<F>));
     static std::atomic<bool> attr_done[64] = {};  // per device; the attribute calls are idempotent
     int device = 0;
@@ -426,6 +427,11 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale) 
     const int rc = decode_plan(a, F::kGroups, &p, &cluster);
     if (rc != NVK_OK) return rc;
     p.k_scale = static_cast<const __half*>(k_scale); p.v_scale = static_cast<const __half*>(v_scale);
+    if constexpr (F::kScores) {
+        p.scores = scores;
+        p.ws_ml = ml;
+        *plan = p;
+    }
     if (cluster > 0) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.num_kv_heads * cluster));
@@ -521,6 +527,106 @@ int launch_decode_int8_mma(const DecodeInt8Args& x) {
                                         : launch_typed<Cache8<__half, true>, __half>(x.base, x.k_scale, x.v_scale);
     return x.base.dtype == NVK_BF16 ? launch_typed<Cache8<bf, false>, bf>(x.base, x.k_scale, x.v_scale)
                                     : launch_typed<Cache8<__half, false>, __half>(x.base, x.k_scale, x.v_scale);
+}
+
+bool decode_int4_supported(const DecodeArgs& a, const void* k_params, const void* v_params) {
+    return shape_supported(a) && aligned_to(a.q, 16) && aligned_to(k_params, 4) && aligned_to(v_params, 4);
+}
+
+int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_params) {
+    return a.dtype == NVK_BF16 ? launch_typed<Cache4<__nv_bfloat16>, __nv_bfloat16>(a, k_params, v_params)
+                               : launch_typed<Cache4<__half>, __half>(a, k_params, v_params);
+}
+
+// ---- the weights of the keys -----------------------------------------------------------------------------------------------
+namespace {
+
+constexpr int kWeightThreads = 256;
+constexpr int kWeightKeys = 1024;   // of a block
+
+// new[row, kvh, k] = old[row, kvh, k] + sum over the group's heads of exp2(score - M) / L, the score as the decode kernel left it (fp32) and (M, L) of
+// the whole context from its parts.
+__global__ void __launch_bounds__(kWeightThreads) key_weights_kernel(const __grid_constant__ DecodeParams p, const KeyWeights w, int chunks) {
+    __shared__ float2 s_ml[kMaxGroup];   // (M, 1 / L)
+    pdl_wait_then_release();
+    const int pair = blockIdx.x / chunks, first = (blockIdx.x - pair * chunks) * kWeightKeys;
+    const int b = static_cast<int>(p.by_kv_heads.div(pair)), kvh = pair - b * p.num_kv_heads;
+    const int ctx = clamped_context(p, b);
+    if (first >= ctx) return;
+    const int64_t row = w.rows != nullptr ? w.rows[b] : b;
+    if (row < 0 || row >= w.num_rows) return;
+    const int len = range_len(p, ctx), parts = (ctx + len - 1) / len;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp < p.group) {
+        const float2* ml = p.ws_ml + static_cast<size_t>(pair) * p.num_splits * p.group + warp;
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml[i * p.group].x);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        for (int i = lane; i < parts; i += 32) l = fmaf(fast_exp2(ml[i * p.group].x - m), ml[i * p.group].y, l);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        if (lane == 0) s_ml[warp] = make_float2(m, 1.0f / l);
+    }
+    __syncthreads();
+    const float* scores = p.scores + static_cast<int64_t>(pair) * p.max_blocks * p.block_size * p.group;
+    const int64_t at = (row * p.num_kv_heads + kvh) * w.row_keys;
+    for (int k = first + threadIdx.x; k < min(ctx, first + kWeightKeys); k += kWeightThreads) {
+        float sum = 0.0f;
+        for (int h = 0; h < p.group; ++h) sum = fmaf(fast_exp2(scores[static_cast<int64_t>(k) * p.group + h] - s_ml[h].x), s_ml[h].y, sum);
+        w.new_weights[at + k] = (w.old_weights != nullptr ? w.old_weights[at + k] : 0.0f) + sum;
+    }
+}
+
+// Workspace of a step: the scores, the parts' (maximum, sum), then the parts of the decode kernels.  It grows with the batch and with the tables' width.
+struct WeightSpace { size_t scores, ml, total; };
+WeightSpace weight_space(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size) {
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const int64_t pairs = batch * num_kv_heads, max_tokens = max_blocks * block_size;
+    const int group = num_heads / num_kv_heads;
+    const int64_t parts = std::max(most_parts(pairs, max_tokens), pairs * std::max<int64_t>(kMaxCluster, (max_tokens + 2047) / 2048));
+    WeightSpace s{};
+    s.scores = up(static_cast<size_t>(batch) * num_heads * max_tokens * sizeof(float));
+    s.ml = up(static_cast<size_t>(parts) * group * sizeof(float2));
+    s.total = s.scores + s.ml + part_bytes(static_cast<size_t>(parts), group);
+    return s;
+}
+
+template <class F, typename T>
+int launch_weights_typed(const DecodeArgs& a, const void* k_params, const void* v_params, const KeyWeights& w) {
+    const WeightSpace space = weight_space(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size);
+    unsigned char* base = static_cast<unsigned char*>(a.workspace);
+    DecodeArgs d = a;
+    d.workspace = base + space.scores + space.ml;
+    d.workspace_bytes = space.total - space.scores - space.ml;
+    const int64_t chunks = (a.max_blocks * a.block_size + kWeightKeys - 1) / kWeightKeys, blocks = a.batch * a.num_kv_heads * chunks;
+    if (blocks > 0x7fffffffLL) return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): batch or block table too large");
+    DecodeParams plan{};
+    int cluster = 0, rc = decode_plan(d, F::kGroups, &plan, &cluster);
+    if (rc != NVK_OK) return rc;
+    if (part_bytes(static_cast<size_t>(a.batch) * a.num_kv_heads * plan.num_splits, plan.group) > space.total - space.scores - space.ml)
+        return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): %d parts to a context", plan.num_splits);
+    rc = launch_typed<F, T>(d, k_params, v_params, reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + space.scores), &plan);
+    if (rc != NVK_OK) return rc;
+    const cudaError_t e = launch_pdl(key_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWeightThreads), 0, a.stream, plan, w, static_cast<int>(chunks));
+    if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "key_weights_kernel launch: %s", cudaGetErrorString(e));
+    return check_launch("key_weights_kernel launch");
+}
+
+}  // namespace
+
+size_t decode_weights_workspace_bytes(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size) {
+    if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || max_blocks <= 0 || block_size <= 0) return 0;
+    return weight_space(batch, num_heads, num_kv_heads, max_blocks, block_size).total;
+}
+
+int launch_decode_weights(const DecodeArgs& a, const void* k_params, const void* v_params, const KeyWeights& w) {
+    using bf = __nv_bfloat16;
+    if (k_params != nullptr)
+        return a.dtype == NVK_BF16 ? launch_weights_typed<Cache4<bf, true>, bf>(a, k_params, v_params, w)
+                                   : launch_weights_typed<Cache4<__half, true>, __half>(a, k_params, v_params, w);
+    return a.dtype == NVK_BF16 ? launch_weights_typed<Cache16<bf, true>, bf>(a, nullptr, nullptr, w)
+                               : launch_weights_typed<Cache16<__half, true>, __half>(a, nullptr, nullptr, w);
 }
 
 int launch_decode_mma(const DecodeArgs& a) {

@@ -32,6 +32,26 @@ namespace {
 bool is_compute_dtype(int dtype) { return dtype == NVK_F16 || dtype == NVK_BF16 || dtype == NVK_F32; }
 bool is_index_dtype(int dtype) { return dtype == NVK_I32 || dtype == NVK_I64; }
 IndexArray index_array(const void* p, int dtype) { return IndexArray(p, dtype == NVK_I64 ? 1 : 0); }
+
+// What the calls over a 4-bit cache have in common: its types and its shape.
+int check_int4(const char* what, int dtype, int num_kv_heads, int head_dim) {
+    if (dtype != NVK_F16 && dtype != NVK_BF16) return fail(NVK_ERR_UNSUPPORTED, "%s: needs F16 or BF16", what);
+    if (num_kv_heads <= 0 || head_dim <= 0) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: sizes must be positive", what);
+    if (head_dim != 128) return fail(NVK_ERR_UNSUPPORTED, "%s: head_dim must be 128 (got %d)", what, head_dim);
+    return NVK_OK;
+}
+int check_decode_sizes(int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads, int num_kv_heads, int head_dim, int block_size) {
+    if (batch < 0 || max_blocks <= 0 || num_cache_blocks <= 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "attention dimensions must be positive");
+    if (num_heads % num_kv_heads != 0) return fail(NVK_ERR_INVALID_ARGUMENT, "num_heads must be divisible by num_kv_heads");
+    return NVK_OK;
+}
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+int64_t index_bytes(int dtype) { return dtype == NVK_I64 ? 8 : 4; }
+
 int launch_prefill(const PrefillArgs& a) {
     if (prefill_tc_supported(a) && !prefill_takes_tiles(a)) return launch_prefill_tc(a);
     if (prefill_mma_supported(a)) return launch_prefill_mma(a);
@@ -225,6 +245,139 @@ int nvk_decode_attention_paged_fp8(const void* query, const void* k_cache, const
         if (!aligned_to(workspace, 16)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (fp8): workspace must be 16-byte aligned");
     }
     return launch_decode_int8_mma(a);
+}
+
+int nvk_store_kvcache_int4(const void* key, const void* value, void* k_cache, void* v_cache, void* k_params, void* v_params,
+                           const void* slot_mapping, int slot_dtype, int64_t num_tokens, int num_kv_heads, int head_dim, int64_t cache_rows,
+                           int dtype, void* stream) {
+    if (!key || !value || !k_cache || !v_cache || !k_params || !v_params || !slot_mapping)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_int4: every tensor must be defined");
+    if (const int rc = check_int4("store_kvcache_int4", dtype, num_kv_heads, head_dim); rc != NVK_OK) return rc;
+    if (!is_index_dtype(slot_dtype)) return fail(NVK_ERR_INVALID_ARGUMENT, "slot_mapping must be int32 or int64");
+    if (num_tokens < 0 || cache_rows <= 0) return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_int4: sizes must be positive");
+    if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_params, 4) ||
+        !aligned_to(v_params, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_int4: key, value and the caches must be 16-byte aligned, the params 4-byte aligned");
+    if (num_tokens == 0) return NVK_OK;
+    return launch_store_int4(key, value, k_cache, v_cache, k_params, v_params, index_array(slot_mapping, slot_dtype), num_tokens, num_kv_heads, cache_rows,
+                             dtype, static_cast<cudaStream_t>(stream));
+}
+
+int nvk_gather_kvcache_int4(const void* k_cache, const void* v_cache, const void* k_params, const void* v_params, const void* cu_seqlens_k,
+                            int cu_seqlens_k_dtype, const void* block_tables, int block_tables_dtype, int64_t num_seqs, int64_t total_k,
+                            int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int head_dim, int block_size, void* key, void* value,
+                            int dtype, void* stream) {
+    if (!k_cache || !v_cache || !k_params || !v_params || !cu_seqlens_k || !block_tables || !key || !value)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_int4: every tensor must be defined");
+    if (const int rc = check_int4("gather_kvcache_int4", dtype, num_kv_heads, head_dim); rc != NVK_OK) return rc;
+    if (!is_index_dtype(cu_seqlens_k_dtype) || !is_index_dtype(block_tables_dtype))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "cu_seqlens_k and block_tables must be int32 or int64");
+    if (num_seqs <= 0 || total_k < 0 || max_blocks <= 0 || num_cache_blocks <= 0 || block_size <= 0)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_int4: sizes must be positive");
+    if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_params, 4) ||
+        !aligned_to(v_params, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_int4: key, value and the caches must be 16-byte aligned, the params 4-byte aligned");
+    if (total_k == 0) return NVK_OK;
+    return launch_gather_int4(k_cache, v_cache, k_params, v_params, index_array(cu_seqlens_k, cu_seqlens_k_dtype), index_array(block_tables, block_tables_dtype),
+                              num_seqs, total_k, max_blocks, num_cache_blocks, num_kv_heads, block_size, key, value, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, const void* v_cache, const void* k_params, const void* v_params,
+                                    const void* context_lens, int context_lens_dtype, const void* block_tables, int block_tables_dtype,
+                                    int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads, int num_kv_heads,
+                                    int head_dim, int block_size, float scale, void* output, int dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    if (!query || !k_cache || !v_cache || !k_params || !v_params || !context_lens || !block_tables || !output)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (int4) requires KV cache, params, context_lens, and block_tables");
+    if (!is_index_dtype(context_lens_dtype) || !is_index_dtype(block_tables_dtype))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "context_lens and block_tables must be int32 or int64");
+    if (const int rc = check_decode_sizes(batch, max_blocks, num_cache_blocks, num_heads, num_kv_heads, head_dim, block_size); rc != NVK_OK) return rc;
+    if (batch == 0) return NVK_OK;
+    const DecodeArgs a{query, k_cache, v_cache, index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype), output, batch,
+                       max_blocks, num_cache_blocks, num_heads, num_kv_heads, head_dim, block_size, scale, dtype, workspace, workspace_bytes,
+                       static_cast<cudaStream_t>(stream)};
+    if (!decode_int4_supported(a, k_params, v_params))
+        return fail(NVK_ERR_UNSUPPORTED, "decode attention (int4): F16 / BF16 queries, head_dim 128, at most 8 query heads per KV head, block_size a multiple "
+                                         "of 16; query and caches 16-byte aligned, params 4-byte and output 8-byte aligned");
+    if (workspace != nullptr) {
+        const size_t need = decode_mma_workspace_needed(batch, num_heads, num_kv_heads, head_dim, max_blocks, block_size);
+        if (workspace_bytes < need)
+            return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (int4): workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+        if (!aligned_to(workspace, 16)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (int4): workspace must be 16-byte aligned");
+    }
+    return launch_decode_int4(a, k_params, v_params);
+}
+
+size_t nvk_decode_attention_weights_workspace_bytes(int64_t batch, int num_heads, int num_kv_heads, int head_dim, int64_t max_blocks, int block_size) {
+    return head_dim > 0 ? decode_weights_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size) : 0;
+}
+
+int nvk_decode_attention_paged_weights(const void* query, const void* k_cache, const void* v_cache, const void* k_params, const void* v_params,
+                                       const void* context_lens, int context_lens_dtype, const void* block_tables, int block_tables_dtype,
+                                       int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads, int num_kv_heads,
+                                       int head_dim, int block_size, float scale, const float* key_weights, const void* weight_rows,
+                                       int weight_rows_dtype, int64_t num_weight_rows, int64_t weight_row_keys, float* new_key_weights,
+                                       void* output, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!query || !k_cache || !v_cache || !context_lens || !block_tables || !new_key_weights || !output)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights) requires KV cache, context_lens, block_tables, new_key_weights and output");
+    if ((k_params == nullptr) != (v_params == nullptr)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): k_params and v_params go together");
+    if (!is_index_dtype(context_lens_dtype) || !is_index_dtype(block_tables_dtype) || (weight_rows && !is_index_dtype(weight_rows_dtype)))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "context_lens, block_tables and weight_rows must be int32 or int64");
+    if (const int rc = check_decode_sizes(batch, max_blocks, num_cache_blocks, num_heads, num_kv_heads, head_dim, block_size); rc != NVK_OK) return rc;
+    if (num_weight_rows <= 0 || weight_row_keys <= 0 || weight_row_keys / block_size < max_blocks)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): a row of weights has to hold max_blocks * block_size keys");
+    if (!weight_rows && num_weight_rows < batch)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): without weight_rows there has to be a row of weights for every sequence");
+    if (batch == 0) return NVK_OK;
+    const DecodeArgs a{query, k_cache, v_cache, index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype), output, batch,
+                       max_blocks, num_cache_blocks, num_heads, num_kv_heads, head_dim, block_size, scale, dtype, workspace, workspace_bytes,
+                       static_cast<cudaStream_t>(stream)};
+    if (k_params ? !decode_int4_supported(a, k_params, v_params) : !decode_mma_supported(a))
+        return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): F16 / BF16 queries, head_dim 128, at most 8 query heads per KV head, block_size a "
+                                         "multiple of 16; caches (4-bit ones: query too) 16-byte aligned, params 4-byte and output 8-byte aligned");
+    if (!aligned_to(key_weights, 4) || !aligned_to(new_key_weights, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): weights must be 4-byte aligned");
+    const size_t need = decode_weights_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size);
+    if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): a 16-byte aligned workspace of %zu bytes is needed "
+                                              "(nvk_decode_attention_weights_workspace_bytes)", need);
+    return launch_decode_weights(a, k_params, v_params,
+                                 KeyWeights{key_weights, new_key_weights, index_array(weight_rows, weight_rows_dtype), num_weight_rows, weight_row_keys});
+}
+
+int nvk_evict_kvcache(void* k_cache, void* v_cache, void* k_params, void* v_params, const float* key_weights, const void* weight_rows,
+                      int weight_rows_dtype, int64_t num_weight_rows, int64_t weight_row_keys, const void* context_lens, int context_lens_dtype,
+                      const void* block_tables, int block_tables_dtype, int64_t batch, int64_t max_blocks, int64_t num_cache_blocks,
+                      float* new_key_weights, const void* new_block_tables, int new_block_tables_dtype, int64_t new_max_blocks,
+                      void* new_context_lens, int num_kv_heads, int head_dim, int block_size, int64_t budget, int64_t sinks, int64_t recent,
+                      int dtype, void* stream) {
+    if (!k_cache || !v_cache || !key_weights || !context_lens || !block_tables || !new_key_weights || !new_block_tables || !new_context_lens)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: the caches, weights, context lengths and block tables must be defined");
+    if ((k_params == nullptr) != (v_params == nullptr)) return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: k_params and v_params go together");
+    if (!is_index_dtype(context_lens_dtype) || !is_index_dtype(block_tables_dtype) || !is_index_dtype(new_block_tables_dtype) ||
+        (weight_rows && !is_index_dtype(weight_rows_dtype)))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "context_lens, block_tables, new_block_tables and weight_rows must be int32 or int64");
+    if (const int rc = check_int4("evict_kvcache", dtype, num_kv_heads, head_dim); rc != NVK_OK) return rc;
+    if (batch < 0 || max_blocks <= 0 || new_max_blocks <= 0 || num_cache_blocks <= 0 || block_size <= 0)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: sizes must be positive");
+    if (sinks < 0 || recent < 0 || budget <= 0 || sinks > budget || recent > budget - sinks)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: budget must be positive, sinks and recent not negative and no more than it together");
+    if (num_weight_rows <= 0 || weight_row_keys <= 0 || weight_row_keys / block_size < max_blocks)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: a row of weights has to hold max_blocks * block_size keys");
+    if (!weight_rows && num_weight_rows < batch)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: without weight_rows there has to be a row of weights for every sequence");
+    if (new_max_blocks < max_blocks && new_max_blocks < (budget + block_size - 1) / block_size)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: new_block_tables has to hold the budget, or as many blocks as block_tables");
+    if (!aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_params, 4) || !aligned_to(v_params, 4) || !aligned_to(key_weights, 4) ||
+        !aligned_to(new_key_weights, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: the caches must be 16-byte aligned, params and weights 4-byte aligned");
+    if (batch == 0) return NVK_OK;
+    if (overlap(new_context_lens, batch * index_bytes(context_lens_dtype), context_lens, batch * index_bytes(context_lens_dtype)))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: new_context_lens must not be context_lens");
+    return launch_evict(EvictArgs{k_cache, v_cache, k_params, v_params, key_weights, new_key_weights, index_array(weight_rows, weight_rows_dtype),
+                                  index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype),
+                                  index_array(new_block_tables, new_block_tables_dtype), new_context_lens, batch, num_weight_rows, weight_row_keys, max_blocks,
+                                  new_max_blocks, num_cache_blocks, budget, sinks, recent, num_kv_heads, block_size, static_cast<cudaStream_t>(stream)});
 }
 
 int nvk_prefill_attention_varlen(const void* query, const void* key, const void* value, const void* k_cache,

@@ -165,6 +165,32 @@ int launch_decode_int8_mma(const DecodeInt8Args& a);
 int launch_store_fp8(const void* key, const void* value, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                      const int32_t* slot_mapping, int64_t num_tokens, int num_kv_heads, int head_dim, int64_t cache_rows,
                      int dtype, cudaStream_t stream);
+// 4-bit KV cache (kv_int4.cu; tensor-core decode in decode_attn.cu); `k_params`, `v_params`: (step, low) pairs of the queries' type
+int launch_store_int4(const void* key, const void* value, void* k_cache, void* v_cache, void* k_params, void* v_params, const IndexArray& slots,
+                      int64_t num_tokens, int num_kv_heads, int64_t cache_rows, int dtype, cudaStream_t stream);
+int launch_gather_int4(const void* k_cache, const void* v_cache, const void* k_params, const void* v_params, const IndexArray& cu, const IndexArray& tables,
+                       int64_t num_seqs, int64_t total, int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int block_size, void* key,
+                       void* value, int dtype, cudaStream_t stream);
+bool decode_int4_supported(const DecodeArgs& a, const void* k_params, const void* v_params);
+int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_params);
+// Decode that adds up the weights of every key (decode_attn.cu), and the eviction that goes by them (evict.cu).  A 16-bit cache has no params.
+struct KeyWeights {
+    const float* old_weights; float* new_weights;   // [num_rows, Hkv, row_keys]; old: may be null (zeros) or the new ones themselves
+    IndexArray rows;                                // of the sequences; none: sequence b has row b
+    int64_t num_rows, row_keys;
+};
+size_t decode_weights_workspace_bytes(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size);
+int launch_decode_weights(const DecodeArgs& a, const void* k_params, const void* v_params, const KeyWeights& w);
+struct EvictArgs {
+    void* k_cache; void* v_cache; void* k_params; void* v_params;
+    const float* weights; float* new_weights; IndexArray rows;
+    IndexArray context_lens; IndexArray block_tables; IndexArray new_tables;
+    void* new_lens;
+    int64_t batch, num_rows, row_keys, max_blocks, new_max_blocks, num_cache_blocks, budget, sinks, recent;
+    int num_kv_heads, block_size;
+    cudaStream_t stream;
+};
+int launch_evict(const EvictArgs& a);
 bool prefill_mma_supported(const PrefillArgs& a);
 int launch_prefill_mma(const PrefillArgs& a);
 bool prefill_takes_tiles(const PrefillArgs& a);   // launch_prefill_mma is quicker than launch_prefill_tc, by sizes that the host knows
