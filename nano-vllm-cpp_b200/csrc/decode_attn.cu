@@ -530,7 +530,8 @@ int launch_decode_int8_mma(const DecodeInt8Args& x) {
 }
 
 bool decode_int4_supported(const DecodeArgs& a, const void* k_params, const void* v_params) {
-    return shape_supported(a) && aligned_to(a.q, 16) && aligned_to(k_params, 4) && aligned_to(v_params, 4);
+    // (rows of heads are counted in 32 bits: 292 GB of cache)
+    return shape_supported(a) && a.num_cache_blocks <= ((1LL << 31) - 1) / a.block_size / a.num_kv_heads && aligned_to(a.q, 16) && aligned_to(k_params, 4) && aligned_to(v_params, 4);
 }
 
 int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_params) {

@@ -21,8 +21,6 @@
 
 #include "nvk_internal.cuh"
 
-#include <type_traits>
-
 namespace nvk {
 namespace dec {
 
@@ -94,9 +92,9 @@ struct SoftmaxState {
         for (int i = 0; i < 8; ++i) { o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f; }
         m[0] = m[1] = -INFINITY; l[0] = l[1] = 0.0f;
     }
-    // Scores of a tile: rescale where a maximum moves (a handful of tiles of a sequence; the branch is warp-uniform).  `extra`: N further
-    // values that are scaled along, of heads 2t and 2t + 1 in turn.
-    template <int N = 4> __device__ __forceinline__ void raise_max(const float (&sc)[4], float* extra) {
+    // Scores of a tile: rescale where a maximum moves (a handful of tiles of a sequence; the branch is warp-uniform).  `extra`: further
+    // columns that are scaled along.
+    __device__ __forceinline__ void raise_max(const float (&sc)[4], float* extra) {
         float top[2] = {fmaxf(sc[0], sc[2]), fmaxf(sc[1], sc[3])};
         if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
             float c[2];
@@ -111,10 +109,7 @@ struct SoftmaxState {
             }
 #pragma unroll
             for (int mt = 0; mt < 8; ++mt) { o[mt][0] *= c[0]; o[mt][1] *= c[1]; o[mt][2] *= c[0]; o[mt][3] *= c[1]; }
-            if (extra != nullptr) {
-#pragma unroll
-                for (int i = 0; i < N; ++i) extra[i] *= c[i & 1];
-            }
+            if (extra != nullptr) { extra[0] *= c[0]; extra[1] *= c[1]; extra[2] *= c[0]; extra[3] *= c[1]; }
         }
     }
 };
@@ -135,12 +130,12 @@ struct ScoreOut {
         const int64_t keys = p.max_blocks * p.block_size;
         at = p.scores + ((static_cast<int64_t>(b) * p.num_kv_heads + kvh) * keys + token + (lane >> 2)) * p.group + 2 * (lane & 3);
     }
-    __device__ __forceinline__ void put(const DecodeParams& p, const float (&sc)[4], int valid, int lane) {
-        const int g = lane >> 2, h = 2 * (lane & 3), group = p.group;
+    __device__ __forceinline__ void put16(const float (&sc)[4], int row0, int valid, int lane, int group) const {
+        const int g = lane >> 2, h = 2 * (lane & 3);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            if (g + 8 * i < valid && h < group) {
-                float* to = at + 8 * i * group;
+            if (row0 + g + 8 * i < valid && h < group) {
+                float* to = at + (row0 + 8 * i) * group;
                 if ((group & 1) == 0) {
                     *reinterpret_cast<float2*>(to) = make_float2(sc[2 * i], sc[2 * i + 1]);
                 } else {
@@ -149,7 +144,15 @@ struct ScoreOut {
                 }
             }
         }
-        at += kGroupWarps * kTileTokens * group;
+    }
+    __device__ __forceinline__ void put(const DecodeParams& p, const float (&sc)[4], int valid, int lane) {   // tiles of 16 keys
+        put16(sc, 0, valid, lane, p.group);
+        at += kGroupWarps * 16 * p.group;
+    }
+    __device__ __forceinline__ void put(const DecodeParams& p, const float (&sa)[4], const float (&sb)[4], int valid, int lane) {   // of 32
+        put16(sa, 0, valid, lane, p.group);
+        put16(sb, 16, valid, lane, p.group);
+        at += kGroupWarps * 32 * p.group;
     }
 };
 
@@ -162,6 +165,7 @@ struct ScoreOut {
 template <typename T, bool SCORES = false>
 struct Cache16 {
     static constexpr bool kScores = SCORES;
+    static constexpr bool kOwnLoop = false;
     static constexpr int kGroups = 2;   // resident per SM
     static constexpr int kRowBytes = kHeadDim * 2;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
@@ -279,6 +283,7 @@ template <bool FP8> __device__ __forceinline__ uint32_t widen_pair_hi(uint32_t x
 template <typename T, bool FP8>
 struct Cache8 {
     static constexpr bool kScores = false;
+    static constexpr bool kOwnLoop = false;
     static constexpr int kGroups = 3;
     static constexpr int kRowBytes = kHeadDim;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
@@ -405,50 +410,48 @@ struct Cache8 {
 };
 
 // 4-bit cache: per token and KV head 64 bytes of K, 64 of V (numbers n from 0 to 15, element 2i in the low half of byte i) and for each a
-// pair (step, low) in the queries' type; an element is low + step n.  The MMA operands are made from the nibbles in registers, in the queries'
-// type: a nibble moved into the top of the mantissa of 1.0 is 1 + n / 16 exactly (a shift and one three-input logic operation a pair), so
-//   q . x         = 16 step (q . (1 + n / 16)) + (low - 16 step) sum(q)
-//   sum_k p_k x_k = 16 sum_k p'_k (1 + n_k / 16) - 23.5 sum_k p'_k + sum_k p_k (low_k + 7.5 step_k),   p'_k = p_k step_k rounded to 16 bits
-// Queries and nibbles are exact, sums are fp32; p' is the one rounding to 16 bits (as with the other caches), and the middle of the range goes
-// in the fp32 sum at the right, so that what the rounding touches is no larger than the values' spread.  sum(p') comes from an MMA against
-// a row of ones, i.e. from exactly the p' that the others used.
+// pair (step, low) in the queries' type; an element is low + step n.  The MMA operands are made from the nibbles in registers: a nibble in bits 0 to 3
+// of an f16 is the subnormal number n 2^-24, in bits 4 to 7 it is 16 n 2^-24, exactly, so that a word of eight nibbles gives its four registers for one shift
+// and four ANDs, whatever the queries' type.  Queries are brought to f16 by a power of two (exact but for elements 2^-25 of the largest),
+// those that meet a number times 16 divided by it; sums are fp32:
+//   q . x         = step 2^24 (q . n 2^-24) + low sum(q)
+//   sum_k p_k x_k = 2^E (2^24 sum_k p'_k n_k 2^-24 - 7.5 sum_k p'_k) + sum_k p_k (low_k + 7.5 step_k),   p'_k = p_k step_k 2^-E rounded to f16
+// p' is the one rounding to 16 bits (as with the other caches); the middle of the range goes in the fp32 sum at the right, so that what the rounding touches is no
+// larger than the values' spread.  sum(p') comes from an MMA against a row of ones, i.e. from exactly the p' that the others used.  2^E is the largest
+// step so far, rounded down to a power of two: p' <= 2, and held to 2^-25 of that; the sums are rescaled where it grows, as where a maximum does.
 // As in Cache8 the order in which a contraction runs is free: of key row g lane t takes the 16-byte piece t, whose word w has the k-steps
-// 2w and 2w + 1 (register pair j: elements j and j + 4 of the word; the query fragment is loaded the same way).  Of V lane (g, t) takes 8 bytes,
-// d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; halves of two keys' words side by side, a nibble of both is one register, and
-// accumulator rows g / g + 8 of d-tile i hold d = 16 g + 2 i (+ 1).  The two rows of a 128-byte line of V are swizzled by the line's number,
-// so that these reads are conflict free.
-template <typename T> struct Nibbles;   // pair j of a word: nibble j of both halves -> 1 + n / 16
-template <> struct Nibbles<__nv_bfloat16> {   // mantissa bits 3 to 6
-    template <int J> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
-        constexpr int kLeft = 3 - 4 * J;
-        return ((kLeft > 0 ? x << (kLeft > 0 ? kLeft : 0) : x >> (kLeft > 0 ? 0 : -kLeft)) & 0x00780078u) | 0x3F803F80u;
-    }
-};
-template <> struct Nibbles<__half> {          // mantissa bits 6 to 9
-    template <int J> static __device__ __forceinline__ uint32_t pair(uint32_t x) {
-        constexpr int kLeft = 6 - 4 * J;
-        return ((kLeft > 0 ? x << (kLeft > 0 ? kLeft : 0) : x >> (kLeft > 0 ? 0 : -kLeft)) & 0x03C003C0u) | 0x3C003C00u;
-    }
-};
+// 2w and 2w + 1 (registers: elements {0, 4}, {1, 5}; {2, 6}, {3, 7}; the query fragment is loaded the same way).  Of V lane (g, t) takes 8 bytes,
+// d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; with halves of two keys' words side by side the same masks give both keys' numbers, and accumulator
+// rows g / g + 8 of d-tile i hold d = 16 g + 2 i and d = 16 g + 2 i + 1 (times 16).  The two rows of a 128-byte line of V are swizzled by the line's number, so
+// that these reads are conflict free.
+// A warp takes 32 keys at a time, two chains of 16: the arithmetic of a tile is one long chain, and three warps to a scheduler do not hide it.  The cache
+// rows of its next 16 tiles are worked out by the lanes, one half of a tile each, while the ids of the 16 after them are on their way.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src)); }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src)); }
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // -126 <= e <= 127
 
 template <typename T, bool SCORES = false>
 struct Cache4 {
     static constexpr bool kScores = SCORES;
+    static constexpr bool kOwnLoop = true;
     static constexpr int kGroups = 3;
     static constexpr int kRowBytes = kHeadDim / 2;
-    static constexpr int kTileBytes = kTileTokens * kRowBytes;
-    static constexpr int kParamBytes = 2 * kTileTokens * 4;   // (step, low) of (K | V, token)
-    static constexpr int kStageBytes = 2 * kTileBytes + kParamBytes;
-    static constexpr int kStages = 6;
+    static constexpr int kKeys = 32;                          // of a stage
+    static constexpr int kTileBytes = kKeys * kRowBytes;
+    static constexpr int kStageBytes = 2 * kTileBytes + 2 * kKeys * 4;   // K, V, (step, low) of K and of V
+    static constexpr int kStages = 3;
     static constexpr int kPartStride = kHeadDim + 4;
+    static constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u, kNone = 0xffffffffu;
 
     SoftmaxState s;
     ScoreOut kept;       // (SCORES)
-    float more[6];       // 0..3: sum(p') from the ones MMA; 4, 5: sum(p (low + 7.5 step)) of heads 2t, 2t + 1 over the lane's keys
-    float q_sum[2];
+    float ones[4];       // sum(p')
+    float mid[2];        // sum(p (low + 7.5 step)) of heads 2t, 2t + 1 over the lane's keys
+    float q_sum[2], step_scale;
+    int v_exp;           // E
     uint32_t qa[8][2];   // k-step 2 w + e: elements 32 t + 8 w + 2 e + {0, 4 | 1, 5}
 
     __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
@@ -456,93 +459,105 @@ struct Cache4 {
         const bool live = g < p.group;
         const uint4* row = reinterpret_cast<const uint4*>(
             static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.num_heads + kvh * p.group + (live ? g : 0)) * kHeadDim) + 4 * t;
-        float sum = 0.0f;
+        float sum = 0.0f, top = 0.0f;
+        uint4 v[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) v[w] = live ? row[w] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const uint4 v = live ? row[w] : make_uint4(0u, 0u, 0u, 0u);
-            qa[2 * w][0] = __byte_perm(v.x, v.z, 0x5410);
-            qa[2 * w][1] = __byte_perm(v.x, v.z, 0x7632);
-            qa[2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);
-            qa[2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+            const uint32_t e[4] = {v[w].x, v[w].y, v[w].z, v[w].w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2<T>(qa[2 * w + (e >> 1)][e & 1]);
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2<T>(e[i]);
                 sum += f.x + f.y;
+                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        // the largest to [2^14, 2^15); (infinities and NaN stay what they are)
+        const int up = top > 0.0f && top < INFINITY ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 100) : 0;
+        const float even = power_of_two(up), odd = even * 0.0625f;
+        step_scale = p.scale_log2 * 0x1p24f * power_of_two(-up);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 e01 = unpack2<T>(v[w].x), e23 = unpack2<T>(v[w].y), e45 = unpack2<T>(v[w].z), e67 = unpack2<T>(v[w].w);
+            qa[2 * w][0] = ElemTraits<__half>::pack2(e01.x * even, e45.x * even);
+            qa[2 * w][1] = ElemTraits<__half>::pack2(e01.y * odd, e45.y * odd);
+            qa[2 * w + 1][0] = ElemTraits<__half>::pack2(e23.x * even, e67.x * even);
+            qa[2 * w + 1][1] = ElemTraits<__half>::pack2(e23.y * odd, e67.y * odd);
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t);
-        q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
-#pragma unroll
-        for (int i = 0; i < 6; ++i) more[i] = 0.0f;
+        q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t) * p.scale_log2;
+        q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * p.scale_log2;
+        ones[0] = ones[1] = ones[2] = ones[3] = mid[0] = mid[1] = 0.0f;
+        v_exp = -126;
         s.reset();
     }
-    static __device__ __forceinline__ void issue(const DecodeParams& p, int kvh, int64_t row0, int valid, uint32_t stage, int lane) {
-        const size_t stride = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
-        const int c = lane & 3, rq = lane >> 2;   // 16-byte piece c of rows rq, rq + 8
-        const size_t base = static_cast<size_t>(row0) * stride + static_cast<size_t>(kvh) * kRowBytes + c * 16;
-        const unsigned char* kc = static_cast<const unsigned char*>(p.k_cache) + base;
-        const unsigned char* vc = static_cast<const unsigned char*>(p.v_cache) + base;
-        const uint32_t vpiece = (((rq & 1) << 2) + c) ^ (((rq >> 1) & 3) << 1);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = 8 * i + rq;
-            const int bytes = r < valid ? 16 : 0;
-            const size_t src = bytes ? r * stride : 0;
-            cp_async16(stage + r * kRowBytes + c * 16, kc + src, bytes);
-            cp_async16(stage + kTileBytes + (r >> 1) * 128 + vpiece * 16, vc + src, bytes);
-        }
-        const int tr = lane & 15;                 // lanes 0-15 K, lanes 16-31 V
-        const int pbytes = tr < valid ? 4 : 0;
-        const size_t at = pbytes ? (static_cast<size_t>(row0) + tr) * p.num_kv_heads + kvh : 0;
-        cp_async4(stage + 2 * kTileBytes + lane * 4, reinterpret_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + at, pbytes);
-    }
-    __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int /*kvh*/, int lane) {
+
+    // Scores of 16 keys, rows `row0` on of a stage; their (step, low) of V.
+    __device__ __forceinline__ void score(uint32_t stage, int row0, int valid, int lane, float (&sc)[4], float2 (&vp)[2]) const {
         const int g = lane >> 2, t = lane & 3;
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-        {
-            uint32_t w0[4], w1[4];
-            lds32x4(stage + g * kRowBytes + t * 16, w0);
-            lds32x4(stage + (g + 8) * kRowBytes + t * 16, w1);
-            using N = Nibbles<T>;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t w0[4], w1[4], w[4];
+        lds32x4(stage + (row0 + g) * kRowBytes + t * 16, w0);
+        lds32x4(stage + (row0 + g + 8) * kRowBytes + t * 16, w1);
+        const uint32_t at = stage + 2 * kTileBytes + (row0 + g) * 4;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                mma_16816<T>(s0, N::template pair<0>(w0[w]), N::template pair<0>(w1[w]), N::template pair<1>(w0[w]), N::template pair<1>(w1[w]), qa[2 * w][0],
-                             qa[2 * w][1]);
-                mma_16816<T>(s1, N::template pair<2>(w0[w]), N::template pair<2>(w1[w]), N::template pair<3>(w0[w]), N::template pair<3>(w1[w]), qa[2 * w + 1][0],
-                             qa[2 * w + 1][1]);
-            }
+        for (int i = 0; i < 4; ++i) asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[i]) : "r"(at + (i & 1) * 32 + (i >> 1) * kKeys * 4));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t x0 = w0[i] >> 8, x1 = w1[i] >> 8;
+            mma_16816<__half>(acc, w0[i] & kLow, w1[i] & kLow, w0[i] & kHigh, w1[i] & kHigh, qa[2 * i][0], qa[2 * i][1]);
+            mma_16816<__half>(acc, x0 & kLow, x1 & kLow, x0 & kHigh, x1 & kHigh, qa[2 * i + 1][0], qa[2 * i + 1][1]);
         }
-        float2 kp[2], vp[2];                      // (step, low) of keys g and g + 8
-        {
-            uint32_t w[4];
-            const uint32_t at = stage + 2 * kTileBytes + g * 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[i]) : "r"(at + i * 32));
-#pragma unroll
-            for (int i = 0; i < 2; ++i) { kp[i] = unpack2<T>(w[i]); vp[i] = unpack2<T>(w[2 + i]); }
-        }
-        float sc[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float step16 = 16.0f * kp[i].x * p.scale_log2, low16 = fmaf(kp[i].x, -16.0f, kp[i].y) * p.scale_log2;
+            const float2 kp = unpack2<T>(w[i]);
+            vp[i] = unpack2<T>(w[2 + i]);
+            const float step = kp.x * step_scale;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(s0[2 * i + h] + s1[2 * i + h], step16, low16 * q_sum[h]);
+            for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(acc[2 * i + h], step, kp.y * q_sum[h]);
         }
         mask_scores(sc, g, valid);
-        if constexpr (SCORES) kept.put(p, sc, valid, lane);
-        s.template raise_max<6>(sc, more);
+    }
+    // Where a maximum or the largest step grows.
+    __device__ __forceinline__ void raise(float top0, float top1, float top_step) {
+        float top[2] = {top0, top1}, c[2];
+#pragma unroll
+        for (int x = 1; x < 32; x *= 2) top_step = fmaxf(top_step, __shfl_xor_sync(0xffffffffu, top_step, x));
+        const int e = min(max(v_exp, static_cast<int>(__float_as_uint(top_step) >> 23) - 127), 126);
+        const float down = power_of_two(max(v_exp - e, -126));   // (2^-126 or less: what was there is no longer seen beside what is coming)
+        v_exp = e;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
+            const float m_new = fmaxf(s.m[h], top[h]);
+            c[h] = s.m[h] == m_new ? 1.0f : fast_exp2(s.m[h] - m_new);
+            s.l[h] *= c[h];
+            mid[h] *= c[h];
+            s.m[h] = m_new;
+            c[h] *= down;
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) { s.o[mt][0] *= c[0]; s.o[mt][1] *= c[1]; s.o[mt][2] *= c[0]; s.o[mt][3] *= c[1]; }
+        ones[0] *= c[0]; ones[1] *= c[1]; ones[2] *= c[0]; ones[3] *= c[1];
+    }
+    // What 16 keys add to the sums.
+    __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], const float2 (&vp)[2], float down, int lane) {
+        const int g = lane >> 2, t = lane & 3;
         const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
-        const float mid0 = fmaf(vp[0].x, 7.5f, vp[0].y), mid1 = fmaf(vp[1].x, 7.5f, vp[1].y);
-        more[4] = fmaf(p0, mid0, fmaf(p2, mid1, more[4]));
-        more[5] = fmaf(p1, mid0, fmaf(p3, mid1, more[5]));
-        const uint32_t pb0 = transpose_8x8(ElemTraits<T>::pack2(p0 * vp[0].x, p1 * vp[0].x));
-        const uint32_t pb1 = transpose_8x8(ElemTraits<T>::pack2(p2 * vp[1].x, p3 * vp[1].x));
+        const float mid0 = fmaf(vp[0].x, 7.5f, vp[0].y), mid1 = fmaf(vp[1].x, 7.5f, vp[1].y), st0 = vp[0].x * down, st1 = vp[1].x * down;
+        mid[0] = fmaf(p0, mid0, fmaf(p2, mid1, mid[0]));
+        mid[1] = fmaf(p1, mid0, fmaf(p3, mid1, mid[1]));
+        const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * st0, p1 * st0));
+        const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * st1, p3 * st1));
         // V rows 2t, 2t + 1 (line t) and 2t + 8, 2t + 9 (line t + 4), words 2g and 2g + 1: half of piece g / 2
-        const uint32_t v_at = stage + kTileBytes + t * 128 + (g & 1) * 8, even = ((g >> 1) ^ (t << 1)) << 4;
+        const uint32_t v_at = stage + kTileBytes + row0 * kRowBytes + t * 128 + (g & 1) * 8, even = ((g >> 1) ^ (t << 1)) << 4;
         uint2 x[4];
         auto lds64 = [](uint32_t addr, uint2& v) { asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr)); };
         lds64(v_at + even, x[0]);
@@ -550,30 +565,129 @@ struct Cache4 {
         lds64(v_at + 512 + even, x[2]);
         lds64(v_at + 512 + (even ^ 64), x[3]);
         auto four = [&](uint32_t k01, uint32_t k89, int i) {   // d-tiles i and i + 1 of two keys' halves side by side
-            using N = Nibbles<T>;
-            mma_16816<T>(s.o[i], N::template pair<0>(k01), N::template pair<1>(k01), N::template pair<0>(k89), N::template pair<1>(k89), pb0, pb1);
-            mma_16816<T>(s.o[i + 1], N::template pair<2>(k01), N::template pair<3>(k01), N::template pair<2>(k89), N::template pair<3>(k89), pb0, pb1);
+            mma_16816<__half>(s.o[i], k01 & kLow, k01 & kHigh, k89 & kLow, k89 & kHigh, pb0, pb1);
+            k01 >>= 8;
+            k89 >>= 8;
+            mma_16816<__half>(s.o[i + 1], k01 & kLow, k01 & kHigh, k89 & kLow, k89 & kHigh, pb0, pb1);
         };
         four(__byte_perm(x[0].x, x[1].x, 0x5410), __byte_perm(x[2].x, x[3].x, 0x5410), 0);
         four(__byte_perm(x[0].x, x[1].x, 0x7632), __byte_perm(x[2].x, x[3].x, 0x7632), 2);
         four(__byte_perm(x[0].y, x[1].y, 0x5410), __byte_perm(x[2].y, x[3].y, 0x5410), 4);
         four(__byte_perm(x[0].y, x[1].y, 0x7632), __byte_perm(x[2].y, x[3].y, 0x7632), 6);
-        constexpr uint32_t kOnes = std::is_same<T, __half>::value ? 0x3C003C00u : 0x3F803F80u;
-        mma_16816<T>(*reinterpret_cast<float (*)[4]>(more), kOnes, kOnes, kOnes, kOnes, pb0, pb1);
+        constexpr uint32_t kOnes = 0x3c003c00u;
+        mma_16816<__half>(ones, kOnes, kOnes, kOnes, kOnes, pb0, pb1);
+    }
+    // 32 keys, of which `valid` (more than none) are there.
+    __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int lane) {
+        float sa[4], sb[4];
+        float2 va[2], vb[2];
+        score(stage, 0, valid, lane, sa, va);
+        score(stage, 16, valid - 16, lane, sb, vb);
+        if constexpr (SCORES) kept.put(p, sa, sb, valid, lane);
+        const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
+        const float top_step = fmaxf(fmaxf(fabsf(va[0].x), fabsf(va[1].x)), fmaxf(fabsf(vb[0].x), fabsf(vb[1].x)));
+        if (__any_sync(0xffffffffu, top0 > s.m[0] || top1 > s.m[1] || static_cast<int>(__float_as_uint(top_step) >> 23) - 127 > v_exp))
+            raise(top0, top1, top_step);
+        const float down = power_of_two(-v_exp);
+        add(stage, 0, sa, va, down, lane);
+        add(stage, 16, sb, vb, down, lane);
+    }
+
+    // Keys [t0, t1): this warp's tiles of 32, every fourth one.
+    __device__ __forceinline__ void run(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, uint32_t ring, int warp, int lane) {
+        const int tiles = (t1 - t0 + kKeys - 1) / kKeys, mine = tiles > warp ? (tiles - warp + kGroupWarps - 1) / kGroupWarps : 0;
+        const int bs = p.block_size, first = t0 + warp * kKeys;
+        constexpr int kStride = kGroupWarps * kKeys;
+        // Lane 2i + h: half h of tile i of a window of 16 tiles, the place of its first row among all head vectors of the cache.
+        auto token_of = [&](int window) { return first + (window * 16 + (lane >> 1)) * kStride + (lane & 1) * 16; };
+        auto load = [&](int window) {
+            const int token = token_of(window);
+            const int blk = static_cast<int>(p.by_block.div(token < t1 ? token : 0));
+            return p.block_tables.raw(b * p.max_blocks + blk, token < t1);
+        };
+        auto unit_of = [&](int window, IndexArray::Raw raw) {
+            const int token = token_of(window), off = token - static_cast<int>(p.by_block.div(token < t1 ? token : 0)) * bs;
+            const int64_t id = p.block_tables.value(raw);
+            return token < t1 && id >= 0 && id < p.num_cache_blocks ? (static_cast<uint32_t>(id) * bs + off) * p.num_kv_heads + kvh : kNone;
+        };
+        uint32_t units;
+        {   // the first window from the ids that came with the context, if they reach that far
+            const int token = token_of(0), at = static_cast<int>(p.by_block.div(token < t1 ? token : t0)) - id_base;
+            IndexArray::Raw raw{__shfl_sync(0xffffffffu, raw_ids.lo, at), __shfl_sync(0xffffffffu, raw_ids.hi, at)};
+            if (__any_sync(0xffffffffu, at >= 32)) raw = load(0);
+            units = unit_of(0, raw);
+        }
+        IndexArray::Raw next = load(1);
+        const int r = lane >> 2, c = lane & 3;
+        const size_t row_bytes = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
+        const unsigned char* k_at = static_cast<const unsigned char*>(p.k_cache) + r * row_bytes + c * 16;
+        const unsigned char* v_at = static_cast<const unsigned char*>(p.v_cache) + r * row_bytes + c * 16;
+        const uint32_t* par_at = reinterpret_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + static_cast<size_t>(lane & 15) * p.num_kv_heads;
+        const uint32_t k_to = r * kRowBytes + c * 16, v_to = kTileBytes + (r >> 1) * 128 + (((((r & 1) << 2) + c) ^ (((r >> 1) & 3) << 1)) << 4);
+        const uint32_t par_to = 2 * kTileBytes + (lane & 15) * 4 + (lane >> 4) * kKeys * 4;
+        int issued = 0, left = t1 - first;        // keys from the next tile on
+        uint32_t istage = ring;
+        auto issue = [&]() {
+            if (issued < mine) {
+                if ((issued & 15) == 0 && issued > 0) {
+                    units = unit_of(issued >> 4, next);
+                    next = load((issued >> 4) + 1);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t unit = __shfl_sync(0xffffffffu, units, 2 * (issued & 15) + h), stage = istage + h * 16 * kRowBytes;
+                    const int valid = unit == kNone ? 0 : left - 16 * h;
+                    const size_t at = static_cast<size_t>(unit) * kRowBytes;
+                    if (valid >= 16) {
+                        cp_async16(stage + k_to, k_at + at);
+                        cp_async16(stage + k_to + 8 * kRowBytes, k_at + at + 8 * row_bytes);
+                        cp_async16(stage + v_to, v_at + at);
+                        cp_async16(stage + v_to + 8 * kRowBytes, v_at + at + 8 * row_bytes);
+                        cp_async4(istage + h * 64 + par_to, par_at + unit);
+                    } else {   // what is not there reads as zeros (stale cache contents, even NaN, never reach the arithmetic)
+                        const bool r0 = r < valid, r1 = r + 8 < valid, rp = (lane & 15) < valid;
+                        nvk::cp_async16(stage + k_to, r0 ? k_at + at : p.k_cache, r0 ? 16 : 0);
+                        nvk::cp_async16(stage + k_to + 8 * kRowBytes, r1 ? k_at + at + 8 * row_bytes : p.k_cache, r1 ? 16 : 0);
+                        nvk::cp_async16(stage + v_to, r0 ? v_at + at : p.v_cache, r0 ? 16 : 0);
+                        nvk::cp_async16(stage + v_to + 8 * kRowBytes, r1 ? v_at + at + 8 * row_bytes : p.v_cache, r1 ? 16 : 0);
+                        cp_async4(istage + h * 64 + par_to, rp ? static_cast<const void*>(par_at + unit) : p.k_scale, rp ? 4 : 0);
+                    }
+                }
+                ++issued;
+                left -= kStride;
+                istage = istage == ring + (kStages - 1) * kStageBytes ? ring : istage + kStageBytes;
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) issue();
+        start(p, b, kvh, lane);
+        if constexpr (SCORES) kept.start(p, b, kvh, first, lane);
+        uint32_t cstage = ring;
+        int here = t1 - first;
+        for (int j = 0; j < mine; ++j) {
+            issue();
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            step(p, cstage, here, lane);
+            __syncwarp();   // the stage is refilled by other lanes' copies
+            cstage = cstage == ring + (kStages - 1) * kStageBytes ? ring : cstage + kStageBytes;
+            here -= kStride;
+        }
     }
     __device__ __forceinline__ void finish() {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int x = 4; x < 32; x *= 2) more[4 + h] += __shfl_xor_sync(0xffffffffu, more[4 + h], x);
+            for (int x = 4; x < 32; x *= 2) mid[h] += __shfl_xor_sync(0xffffffffu, mid[h], x);
         }
     }
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
-        const float off = fmaf(more[h], -23.5f, more[4 + h]);
+        const float up = power_of_two(v_exp), off = fmaf(ones[h] * -7.5f, up, mid[h]);
+        auto even = [&](int i) { return fmaf(s.o[i][h] * 0x1p24f, up, off); };
+        auto odd = [&](int i) { return fmaf(s.o[i][2 + h] * 0x1p20f, up, off); };
 #pragma unroll
-        for (int i = 0; i < 8; i += 2)
-            *reinterpret_cast<float4*>(row + 16 * g + 2 * i) = make_float4(fmaf(s.o[i][h], 16.0f, off), fmaf(s.o[i][2 + h], 16.0f, off),
-                                                                           fmaf(s.o[i + 1][h], 16.0f, off), fmaf(s.o[i + 1][2 + h], 16.0f, off));
+        for (int i = 0; i < 8; i += 2) *reinterpret_cast<float4*>(row + 16 * g + 2 * i) = make_float4(even(i), odd(i), even(i + 1), odd(i + 1));
     }
 };
 
@@ -589,15 +703,11 @@ struct alignas(128) GroupSmem {
     } warps[kGroupWarps];
 };
 
-// Keys [t0, t1) of sequence b (t0 < t1), one KV head.  sink(h, quad, o, m, l) takes elements 4 quad .. 4 quad + 3 of head h: unnormalised
-// output, maximum and sum.  `tid`: 0..127 inside the group, `bar_id`: its named barrier; all its threads call it.  `raw_ids`: block
-// table entries `id_base` + lane as loaded.  The four warps' parts come together in one trip over all heads, after one barrier (a warp writes
-// its part over its own ring; before, two barriers and a loop over the heads, a trip each).
-template <class F, class Sink>
-__device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, GroupSmem<F>& sm,
-                                             int tid, int bar_id, Sink sink) {
-    const int bs = p.block_size, warp = tid >> 5, lane = tid & 31;
-    const uint32_t ring = smem_u32(sm.warps[warp].ring);
+// The warp's tiles of keys [t0, t1), every fourth one, through its ring.
+template <class F>
+__device__ __forceinline__ void stream_tiles(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, uint32_t ring, int warp,
+                                             int lane, F& st) {
+    const int bs = p.block_size;
     const int num_tiles = (t1 - t0 + kTileTokens - 1) / kTileTokens;
     const int my_tiles = num_tiles > warp ? (num_tiles - warp + kGroupWarps - 1) / kGroupWarps : 0;
     // The issuing end: this warp's next tile begins at row `off` of table entry `blk`.  Lane i holds the cache block of entry
@@ -631,7 +741,6 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
 #pragma unroll
     for (int s = 0; s < F::kStages - 1; ++s) issue();
 
-    F st;
     st.start(p, b, kvh, lane);
     if constexpr (F::kScores) st.kept.start(p, b, kvh, t0 + warp * kTileTokens, lane);
     uint32_t cstage = ring;
@@ -645,6 +754,20 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
         cstage = cstage == ring + (F::kStages - 1) * F::kStageBytes ? ring : cstage + F::kStageBytes;
         left -= kGroupWarps * kTileTokens;
     }
+}
+
+// Keys [t0, t1) of sequence b (t0 < t1), one KV head.  sink(h, quad, o, m, l) takes elements 4 quad .. 4 quad + 3 of head h: unnormalised
+// output, maximum and sum.  `tid`: 0..127 inside the group, `bar_id`: its named barrier; all its threads call it.  `raw_ids`: block
+// table entries `id_base` + lane as loaded.  The four warps' parts come together in one trip over all heads, after one barrier (a warp writes
+// its part over its own ring; before, two barriers and a loop over the heads, a trip each).
+template <class F, class Sink>
+__device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, GroupSmem<F>& sm,
+                                             int tid, int bar_id, Sink sink) {
+    const int warp = tid >> 5, lane = tid & 31;
+    const uint32_t ring = smem_u32(sm.warps[warp].ring);
+    F st;
+    if constexpr (F::kOwnLoop) st.run(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane);
+    else stream_tiles(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane, st);
     cp_async_wait<0>();
     __syncwarp();                              // this warp's ring is idle from here on
     st.finish();
