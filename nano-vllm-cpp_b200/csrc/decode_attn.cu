@@ -87,7 +87,7 @@ __device__ __forceinline__ void st_cluster2(uint32_t addr, uint32_t rank, float 
 }
 
 template <class F, typename T>
-__global__ void __launch_bounds__(kGroupThreads, F::kGroups) decode_split_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kGroupThreads, F::kSplitBlocks) decode_split_kernel(const __grid_constant__ DecodeParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     if (p.beside) pdl_start_beside();
     else pdl_wait_then_release();

@@ -167,6 +167,7 @@ struct Cache16 {
     static constexpr bool kScores = SCORES;
     static constexpr bool kOwnLoop = false;
     static constexpr int kGroups = 2;   // resident per SM
+    static constexpr int kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim * 2;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
     static constexpr int kStageBytes = 2 * kTileBytes;
@@ -284,7 +285,7 @@ template <typename T, bool FP8>
 struct Cache8 {
     static constexpr bool kScores = false;
     static constexpr bool kOwnLoop = false;
-    static constexpr int kGroups = 3;
+    static constexpr int kGroups = 3, kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
     static constexpr int kScaleBytes = 2 * kTileTokens * 4;   // one 32-bit word per (K | V, token): the word that holds its fp16 scale
@@ -437,7 +438,8 @@ template <typename T, bool SCORES = false>
 struct Cache4 {
     static constexpr bool kScores = SCORES;
     static constexpr bool kOwnLoop = true;
-    static constexpr int kGroups = 3;
+    static constexpr int kGroups = 3;                         // resident per SM, by which a step is shared out, as with the 8-bit caches
+    static constexpr int kSplitBlocks = 4;                    // in chunks: the registers are there, and the chains are what a warp waits for
     static constexpr int kRowBytes = kHeadDim / 2;
     static constexpr int kKeys = 32;                          // of a stage
     static constexpr int kTileBytes = kKeys * kRowBytes;
@@ -593,6 +595,18 @@ struct Cache4 {
         add(stage, 16, sb, vb, down, lane);
     }
 
+    // One multiplication with a 64-bit sum: the ALU is the busiest pipe here.
+    static __device__ __forceinline__ const void* row_at(uint32_t unit, const unsigned char* base) {
+        uint64_t at;
+        asm("mad.wide.u32 %0, %1, %2, %3;\n" : "=l"(at) : "r"(unit), "n"(kRowBytes), "l"(base));
+        return reinterpret_cast<const void*>(at);
+    }
+    static __device__ __forceinline__ const void* word_at(uint32_t unit, const uint32_t* base) {
+        uint64_t at;
+        asm("mad.wide.u32 %0, %1, 4, %2;\n" : "=l"(at) : "r"(unit), "l"(base));
+        return reinterpret_cast<const void*>(at);
+    }
+
     // Keys [t0, t1): this warp's tiles of 32, every fourth one.
     __device__ __forceinline__ void run(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, uint32_t ring, int warp, int lane) {
         const int tiles = (t1 - t0 + kKeys - 1) / kKeys, mine = tiles > warp ? (tiles - warp + kGroupWarps - 1) / kGroupWarps : 0;
@@ -622,6 +636,7 @@ struct Cache4 {
         const size_t row_bytes = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
         const unsigned char* k_at = static_cast<const unsigned char*>(p.k_cache) + r * row_bytes + c * 16;
         const unsigned char* v_at = static_cast<const unsigned char*>(p.v_cache) + r * row_bytes + c * 16;
+        const unsigned char *k8_at = k_at + 8 * row_bytes, *v8_at = v_at + 8 * row_bytes;
         const uint32_t* par_at = reinterpret_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + static_cast<size_t>(lane & 15) * p.num_kv_heads;
         const uint32_t k_to = r * kRowBytes + c * 16, v_to = kTileBytes + (r >> 1) * 128 + (((((r & 1) << 2) + c) ^ (((r >> 1) & 3) << 1)) << 4);
         const uint32_t par_to = 2 * kTileBytes + (lane & 15) * 4 + (lane >> 4) * kKeys * 4;
@@ -637,20 +652,19 @@ struct Cache4 {
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t unit = __shfl_sync(0xffffffffu, units, 2 * (issued & 15) + h), stage = istage + h * 16 * kRowBytes;
                     const int valid = unit == kNone ? 0 : left - 16 * h;
-                    const size_t at = static_cast<size_t>(unit) * kRowBytes;
                     if (valid >= 16) {
-                        cp_async16(stage + k_to, k_at + at);
-                        cp_async16(stage + k_to + 8 * kRowBytes, k_at + at + 8 * row_bytes);
-                        cp_async16(stage + v_to, v_at + at);
-                        cp_async16(stage + v_to + 8 * kRowBytes, v_at + at + 8 * row_bytes);
-                        cp_async4(istage + h * 64 + par_to, par_at + unit);
+                        cp_async16(stage + k_to, row_at(unit, k_at));
+                        cp_async16(stage + k_to + 8 * kRowBytes, row_at(unit, k8_at));
+                        cp_async16(stage + v_to, row_at(unit, v_at));
+                        cp_async16(stage + v_to + 8 * kRowBytes, row_at(unit, v8_at));
+                        cp_async4(istage + h * 64 + par_to, word_at(unit, par_at));
                     } else {   // what is not there reads as zeros (stale cache contents, even NaN, never reach the arithmetic)
                         const bool r0 = r < valid, r1 = r + 8 < valid, rp = (lane & 15) < valid;
-                        nvk::cp_async16(stage + k_to, r0 ? k_at + at : p.k_cache, r0 ? 16 : 0);
-                        nvk::cp_async16(stage + k_to + 8 * kRowBytes, r1 ? k_at + at + 8 * row_bytes : p.k_cache, r1 ? 16 : 0);
-                        nvk::cp_async16(stage + v_to, r0 ? v_at + at : p.v_cache, r0 ? 16 : 0);
-                        nvk::cp_async16(stage + v_to + 8 * kRowBytes, r1 ? v_at + at + 8 * row_bytes : p.v_cache, r1 ? 16 : 0);
-                        cp_async4(istage + h * 64 + par_to, rp ? static_cast<const void*>(par_at + unit) : p.k_scale, rp ? 4 : 0);
+                        nvk::cp_async16(stage + k_to, r0 ? row_at(unit, k_at) : p.k_cache, r0 ? 16 : 0);
+                        nvk::cp_async16(stage + k_to + 8 * kRowBytes, r1 ? row_at(unit, k8_at) : p.k_cache, r1 ? 16 : 0);
+                        nvk::cp_async16(stage + v_to, r0 ? row_at(unit, v_at) : p.v_cache, r0 ? 16 : 0);
+                        nvk::cp_async16(stage + v_to + 8 * kRowBytes, r1 ? row_at(unit, v8_at) : p.v_cache, r1 ? 16 : 0);
+                        cp_async4(istage + h * 64 + par_to, rp ? word_at(unit, par_at) : p.k_scale, rp ? 4 : 0);
                     }
                 }
                 ++issued;
