@@ -427,8 +427,12 @@ struct Cache8 {
 // that these reads are conflict free.
 // A warp takes 32 keys at a time, two chains of 16: the arithmetic of a tile is one long chain, and three warps to a scheduler do not hide it.  The cache
 // rows of its next 16 tiles are worked out by the lanes, one half of a tile each, while the ids of the 16 after them are on their way.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src)); }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(src)); }
+template <int AT> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;\n" ::"r"(dst), "l"(src), "n"(AT));
+}
+template <int AT> __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0+%2], [%1], 4;\n" ::"r"(dst), "l"(src), "n"(AT));
+}
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
@@ -453,7 +457,7 @@ struct Cache4 {
     float ones[4];       // sum(p')
     float mid[2];        // sum(p (low + 7.5 step)) of heads 2t, 2t + 1 over the lane's keys
     float q_sum[2], step_scale;
-    int v_exp;           // E
+    float v_down;        // 2^-E
     uint32_t qa[8][2];   // k-step 2 w + e: elements 32 t + 8 w + 2 e + {0, 4 | 1, 5}
 
     __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
@@ -494,20 +498,20 @@ struct Cache4 {
         q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t) * p.scale_log2;
         q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * p.scale_log2;
         ones[0] = ones[1] = ones[2] = ones[3] = mid[0] = mid[1] = 0.0f;
-        v_exp = -126;
+        v_down = 0x1p126f;
         s.reset();
     }
-
+    static __device__ __forceinline__ void lds64(uint32_t addr, uint2& v) { asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr)); }
     // Scores of 16 keys, rows `row0` on of a stage; their (step, low) of V.
-    __device__ __forceinline__ void score(uint32_t stage, int row0, int valid, int lane, float (&sc)[4], float2 (&vp)[2]) const {
+    __device__ __forceinline__ void score(uint32_t stage, int row0, int lane, float (&sc)[4], float2 (&vp)[2]) const {
         const int g = lane >> 2, t = lane & 3;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w0[4], w1[4], w[4];
+        uint32_t w0[4], w1[4];
+        uint2 w[2];
         lds32x4(stage + (row0 + g) * kRowBytes + t * 16, w0);
         lds32x4(stage + (row0 + g + 8) * kRowBytes + t * 16, w1);
-        const uint32_t at = stage + 2 * kTileBytes + (row0 + g) * 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[i]) : "r"(at + (i & 1) * 32 + (i >> 1) * kKeys * 4));
+        for (int i = 0; i < 2; ++i) lds64(stage + 2 * kTileBytes + (row0 + g + 8 * i) * 8, w[i]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t x0 = w0[i] >> 8, x1 = w1[i] >> 8;
@@ -516,22 +520,22 @@ struct Cache4 {
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const float2 kp = unpack2<T>(w[i]);
-            vp[i] = unpack2<T>(w[2 + i]);
+            const float2 kp = unpack2<T>(w[i].x);
+            vp[i] = unpack2<T>(w[i].y);
             const float step = kp.x * step_scale;
 #pragma unroll
             for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(acc[2 * i + h], step, kp.y * q_sum[h]);
         }
-        mask_scores(sc, g, valid);
     }
+    __device__ __forceinline__ int exponent() const { return 127 - static_cast<int>(__float_as_uint(v_down) >> 23); }   // E
     // Where a maximum or the largest step grows.
     __device__ __forceinline__ void raise(float top0, float top1, float top_step) {
         float top[2] = {top0, top1}, c[2];
 #pragma unroll
         for (int x = 1; x < 32; x *= 2) top_step = fmaxf(top_step, __shfl_xor_sync(0xffffffffu, top_step, x));
-        const int e = min(max(v_exp, static_cast<int>(__float_as_uint(top_step) >> 23) - 127), 126);
-        const float down = power_of_two(max(v_exp - e, -126));   // (2^-126 or less: what was there is no longer seen beside what is coming)
-        v_exp = e;
+        const int was = exponent(), e = min(max(was, static_cast<int>(__float_as_uint(top_step) >> 23) - 127), 126);
+        const float down = power_of_two(max(was - e, -126));   // (2^-126 or less: what was there is no longer seen beside what is coming)
+        v_down = power_of_two(-e);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -548,12 +552,12 @@ struct Cache4 {
         ones[0] *= c[0]; ones[1] *= c[1]; ones[2] *= c[0]; ones[3] *= c[1];
     }
     // What 16 keys add to the sums.
-    __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], const float2 (&vp)[2], float down, int lane) {
+    __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], const float2 (&vp)[2], int lane) {
         const int g = lane >> 2, t = lane & 3;
         const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
-        const float mid0 = fmaf(vp[0].x, 7.5f, vp[0].y), mid1 = fmaf(vp[1].x, 7.5f, vp[1].y), st0 = vp[0].x * down, st1 = vp[1].x * down;
+        const float mid0 = fmaf(vp[0].x, 7.5f, vp[0].y), mid1 = fmaf(vp[1].x, 7.5f, vp[1].y), st0 = vp[0].x * v_down, st1 = vp[1].x * v_down;
         mid[0] = fmaf(p0, mid0, fmaf(p2, mid1, mid[0]));
         mid[1] = fmaf(p1, mid0, fmaf(p3, mid1, mid[1]));
         const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * st0, p1 * st0));
@@ -561,7 +565,6 @@ struct Cache4 {
         // V rows 2t, 2t + 1 (line t) and 2t + 8, 2t + 9 (line t + 4), words 2g and 2g + 1: half of piece g / 2
         const uint32_t v_at = stage + kTileBytes + row0 * kRowBytes + t * 128 + (g & 1) * 8, even = ((g >> 1) ^ (t << 1)) << 4;
         uint2 x[4];
-        auto lds64 = [](uint32_t addr, uint2& v) { asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr)); };
         lds64(v_at + even, x[0]);
         lds64(v_at + (even ^ 64), x[1]);
         lds64(v_at + 512 + even, x[2]);
@@ -583,18 +586,19 @@ struct Cache4 {
     __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int lane) {
         float sa[4], sb[4];
         float2 va[2], vb[2];
-        score(stage, 0, valid, lane, sa, va);
-        score(stage, 16, valid - 16, lane, sb, vb);
+        score(stage, 0, lane, sa, va);
+        score(stage, 16, lane, sb, vb);
+        if (valid < kKeys) {
+            mask_scores(sa, lane >> 2, valid);
+            mask_scores(sb, lane >> 2, valid - 16);
+        }
         if constexpr (SCORES) kept.put(p, sa, sb, valid, lane);
         const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
         const float top_step = fmaxf(fmaxf(fabsf(va[0].x), fabsf(va[1].x)), fmaxf(fabsf(vb[0].x), fabsf(vb[1].x)));
-        if (__any_sync(0xffffffffu, top0 > s.m[0] || top1 > s.m[1] || static_cast<int>(__float_as_uint(top_step) >> 23) - 127 > v_exp))
-            raise(top0, top1, top_step);
-        const float down = power_of_two(-v_exp);
-        add(stage, 0, sa, va, down, lane);
-        add(stage, 16, sb, vb, down, lane);
+        if (__any_sync(0xffffffffu, top0 > s.m[0] || top1 > s.m[1] || top_step * v_down >= 2.0f)) raise(top0, top1, top_step);
+        add(stage, 0, sa, va, lane);
+        add(stage, 16, sb, vb, lane);
     }
-
     // One multiplication with a 64-bit sum: the ALU is the busiest pipe here.
     static __device__ __forceinline__ const void* row_at(uint32_t unit, const unsigned char* base) {
         uint64_t at;
@@ -639,7 +643,7 @@ struct Cache4 {
         const unsigned char *k8_at = k_at + 8 * row_bytes, *v8_at = v_at + 8 * row_bytes;
         const uint32_t* par_at = reinterpret_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + static_cast<size_t>(lane & 15) * p.num_kv_heads;
         const uint32_t k_to = r * kRowBytes + c * 16, v_to = kTileBytes + (r >> 1) * 128 + (((((r & 1) << 2) + c) ^ (((r >> 1) & 3) << 1)) << 4);
-        const uint32_t par_to = 2 * kTileBytes + (lane & 15) * 4 + (lane >> 4) * kKeys * 4;
+        const uint32_t par_to = 2 * kTileBytes + (lane & 15) * 8 + (lane >> 4) * 4;
         int issued = 0, left = t1 - first;        // keys from the next tile on
         uint32_t istage = ring;
         auto issue = [&]() {
@@ -648,23 +652,31 @@ struct Cache4 {
                     units = unit_of(issued >> 4, next);
                     next = load((issued >> 4) + 1);
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t unit = __shfl_sync(0xffffffffu, units, 2 * (issued & 15) + h), stage = istage + h * 16 * kRowBytes;
-                    const int valid = unit == kNone ? 0 : left - 16 * h;
-                    if (valid >= 16) {
-                        cp_async16(stage + k_to, row_at(unit, k_at));
-                        cp_async16(stage + k_to + 8 * kRowBytes, row_at(unit, k8_at));
-                        cp_async16(stage + v_to, row_at(unit, v_at));
-                        cp_async16(stage + v_to + 8 * kRowBytes, row_at(unit, v8_at));
-                        cp_async4(istage + h * 64 + par_to, word_at(unit, par_at));
-                    } else {   // what is not there reads as zeros (stale cache contents, even NaN, never reach the arithmetic)
+                const uint32_t u0 = __shfl_sync(0xffffffffu, units, 2 * issued), u1 = __shfl_sync(0xffffffffu, units, 2 * issued + 1);
+                const uint32_t k_dst = istage + k_to, v_dst = istage + v_to, par_dst = istage + par_to;
+                constexpr int kHalf = 16 * kRowBytes, kRow8 = 8 * kRowBytes;
+                if (left >= kKeys && max(u0, u1) != kNone) {
+                    cp_async16<0>(k_dst, row_at(u0, k_at));
+                    cp_async16<kRow8>(k_dst, row_at(u0, k8_at));
+                    cp_async16<kHalf>(k_dst, row_at(u1, k_at));
+                    cp_async16<kHalf + kRow8>(k_dst, row_at(u1, k8_at));
+                    cp_async16<0>(v_dst, row_at(u0, v_at));
+                    cp_async16<kRow8>(v_dst, row_at(u0, v8_at));
+                    cp_async16<kHalf>(v_dst, row_at(u1, v_at));
+                    cp_async16<kHalf + kRow8>(v_dst, row_at(u1, v8_at));
+                    cp_async4<0>(par_dst, word_at(u0, par_at));
+                    cp_async4<128>(par_dst, word_at(u1, par_at));
+                } else {   // what is not there reads as zeros (stale cache contents, even NaN, never reach the arithmetic)
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t unit = h == 0 ? u0 : u1;
+                        const int valid = unit == kNone ? 0 : left - 16 * h;
                         const bool r0 = r < valid, r1 = r + 8 < valid, rp = (lane & 15) < valid;
-                        nvk::cp_async16(stage + k_to, r0 ? row_at(unit, k_at) : p.k_cache, r0 ? 16 : 0);
-                        nvk::cp_async16(stage + k_to + 8 * kRowBytes, r1 ? row_at(unit, k8_at) : p.k_cache, r1 ? 16 : 0);
-                        nvk::cp_async16(stage + v_to, r0 ? row_at(unit, v_at) : p.v_cache, r0 ? 16 : 0);
-                        nvk::cp_async16(stage + v_to + 8 * kRowBytes, r1 ? row_at(unit, v8_at) : p.v_cache, r1 ? 16 : 0);
-                        cp_async4(istage + h * 64 + par_to, rp ? word_at(unit, par_at) : p.k_scale, rp ? 4 : 0);
+                        nvk::cp_async16(k_dst + h * kHalf, r0 ? row_at(unit, k_at) : p.k_cache, r0 ? 16 : 0);
+                        nvk::cp_async16(k_dst + h * kHalf + kRow8, r1 ? row_at(unit, k8_at) : p.k_cache, r1 ? 16 : 0);
+                        nvk::cp_async16(v_dst + h * kHalf, r0 ? row_at(unit, v_at) : p.v_cache, r0 ? 16 : 0);
+                        nvk::cp_async16(v_dst + h * kHalf + kRow8, r1 ? row_at(unit, v8_at) : p.v_cache, r1 ? 16 : 0);
+                        dec::cp_async4(par_dst + h * 128, rp ? word_at(unit, par_at) : p.k_scale, rp ? 4 : 0);
                     }
                 }
                 ++issued;
@@ -697,7 +709,7 @@ struct Cache4 {
         }
     }
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
-        const float up = power_of_two(v_exp), off = fmaf(ones[h] * -7.5f, up, mid[h]);
+        const float up = power_of_two(exponent()), off = fmaf(ones[h] * -7.5f, up, mid[h]);
         auto even = [&](int i) { return fmaf(s.o[i][h] * 0x1p24f, up, off); };
         auto odd = [&](int i) { return fmaf(s.o[i][2 + h] * 0x1p20f, up, off); };
 #pragma unroll
