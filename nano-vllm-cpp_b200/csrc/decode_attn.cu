@@ -323,10 +323,23 @@ size_t part_bytes(size_t parts, int group) { return parts * group * (kHeadDim * 
 size_t part_count(const Splits& s, int64_t batch, int num_kv_heads) {   // (the cluster kernel itself needs none: the mixed step does)
     return s.count > 1 ? static_cast<size_t>(batch) * num_kv_heads * s.count : 0;
 }
-Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size, int groups, bool have_workspace) {
+// 4-bit caches are shared out like 8-bit ones (a key costs as much arithmetic, and that is what bounds both), but for what four blocks to an SM and a block's
+// fixed part, five tiles' worth, change: whole contexts up to 2048 keys from 250 pairs on, up to 4096 at a time beyond three waves' worth of SMs, the
+// longest first.  us, spread from 0.05 / 0.5: 320 pairs of 2048 keys 25.6 / 27.8 -> 22.7 / 25.2, 512 of 8192 76.0 / 99.0 -> 72.7 / 91.7, 1600 of 8192
+// 208 / 299 -> 207 / 271; but 200 of 2048 17.2 / 22.8, whole 19.2 / 21.5, and 320 of 8192 54.1 / 70.3, by 4096 60.5 / 68.5.
+int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
+    if (max_tokens <= 2048) return max_tokens > 768 && pairs >= 250 ? static_cast<int>(max_tokens) : 0;
+    return max_tokens > 4096 && max_tokens <= 8192 && pairs >= 3 * kSmCount ? 4096 : 0;
+}
+Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size, int groups, bool have_workspace, bool four_bits = false) {
     Splits s{cluster_size(batch, num_kv_heads, max_blocks, block_size, groups, have_workspace), 0, 0};
     if (s.cluster > 0) { s.count = s.cluster; return s; }
     const int64_t max_tokens = max_blocks * block_size;
+    if (const int chunk = four_bits ? chunk_tokens4(batch * num_kv_heads, max_tokens) : 0; chunk > 0) {
+        s.chunk = static_cast<int>((chunk + block_size - 1) / block_size) * block_size;
+        s.count = static_cast<int>((max_tokens + s.chunk - 1) / s.chunk);
+        return s;
+    }
     if (max_blocks > 1 && halves(batch * num_kv_heads, max_tokens, groups)) {
         s.chunk = static_cast<int>((max_blocks + 1) / 2 * block_size);
         s.cluster = s.count = 2;
@@ -348,7 +361,7 @@ Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max
 
 // Kernel parameters of a decode call from host-known sizes only, for kernels with `groups` resident groups per SM; returns in
 // *cluster the cluster size, 0 = chunks.
-int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster) {
+int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster, bool four_bits) {
     DecodeParams p{};
     p.q = a.q; p.k_cache = a.k_cache; p.v_cache = a.v_cache;
     p.context_lens = a.context_lens; p.block_tables = a.block_tables; p.out = a.out;
@@ -359,7 +372,7 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     p.beside = a.beside ? 1 : 0;
     if (a.batch * a.num_heads * kMaxCluster >= (1LL << 31) || a.max_blocks * a.block_size >= (1LL << 31) - kTileTokens * kMaxCluster)
         return fail(NVK_ERR_UNSUPPORTED, "decode attention: batch or block table too large");
-    const Splits s = choose_splits(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size, groups, a.workspace != nullptr);
+    const Splits s = choose_splits(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size, groups, a.workspace != nullptr, four_bits);
     *cluster = s.cluster;
     p.per_seq = s.chunk == 0 ? 1 : 0;
     while ((1 << p.split_shift) < s.cluster) ++p.split_shift;
@@ -369,7 +382,7 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     p.num_splits = s.count;
     // More than one wave of blocks: the long contexts first, so that the last blocks to start are short.  Contexts in a few chunks as well:
     // 38 / 44 sequences of 500 / 2000 to 4096 keys, 8 KV heads, 65.4 / 90.1 -> 58.7 / 85.9 us a call (whole 59.8 / 84.7).
-    p.longest_first = s.chunk > 0 && (s.count == 1 || a.max_blocks * a.block_size <= 4096) && a.batch * a.num_kv_heads > static_cast<int64_t>(kSmCount) * groups &&
+    p.longest_first = s.chunk > 0 && (s.count == 1 || a.max_blocks * a.block_size <= 4096 || (four_bits && s.chunk >= 4096)) && a.batch * a.num_kv_heads > static_cast<int64_t>(kSmCount) * groups &&
                       a.batch <= kMaxSorted && a.max_blocks * a.block_size >= kMinSortedTokens;
     // Contexts shorter than the table leave chunks without keys, whose blocks exit at once.  With sequence after sequence they lie between
     // the blocks with work, and these pile up on the SMs where the empty ones were quickest gone; chunk after chunk the ones with
@@ -424,7 +437,7 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     }
     DecodeParams p{};
     int cluster = 0;
-    const int rc = decode_plan(a, F::kGroups, &p, &cluster);
+    const int rc = decode_plan(a, F::kGroups, &p, &cluster, F::kFourBits);
     if (rc != NVK_OK) return rc;
     p.k_scale = static_cast<const __half*>(k_scale); p.v_scale = static_cast<const __half*>(v_scale);
     if constexpr (F::kScores) {
@@ -603,7 +616,7 @@ int launch_weights_typed(const DecodeArgs& a, const void* k_params, const void* 
     const int64_t chunks = (a.max_blocks * a.block_size + kWeightKeys - 1) / kWeightKeys, blocks = a.batch * a.num_kv_heads * chunks;
     if (blocks > 0x7fffffffLL) return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): batch or block table too large");
     DecodeParams plan{};
-    int cluster = 0, rc = decode_plan(d, F::kGroups, &plan, &cluster);
+    int cluster = 0, rc = decode_plan(d, F::kGroups, &plan, &cluster, F::kFourBits);
     if (rc != NVK_OK) return rc;
     if (part_bytes(static_cast<size_t>(a.batch) * a.num_kv_heads * plan.num_splits, plan.group) > space.total - space.scores - space.ml)
         return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): %d parts to a context", plan.num_splits);

@@ -21,6 +21,8 @@
 
 #include "nvk_internal.cuh"
 
+#include <type_traits>
+
 namespace nvk {
 namespace dec {
 
@@ -165,7 +167,7 @@ struct ScoreOut {
 template <typename T, bool SCORES = false>
 struct Cache16 {
     static constexpr bool kScores = SCORES;
-    static constexpr bool kOwnLoop = false;
+    static constexpr bool kFourBits = false;
     static constexpr int kGroups = 2;   // resident per SM
     static constexpr int kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim * 2;
@@ -284,7 +286,7 @@ template <bool FP8> __device__ __forceinline__ uint32_t widen_pair_hi(uint32_t x
 template <typename T, bool FP8>
 struct Cache8 {
     static constexpr bool kScores = false;
-    static constexpr bool kOwnLoop = false;
+    static constexpr bool kFourBits = false;
     static constexpr int kGroups = 3, kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
@@ -417,9 +419,9 @@ struct Cache8 {
 // those that meet a number times 16 divided by it; sums are fp32:
 //   q . x         = step 2^24 (q . n 2^-24) + low sum(q)
 //   sum_k p_k x_k = 2^E (2^24 sum_k p'_k n_k 2^-24 - 7.5 sum_k p'_k) + sum_k p_k (low_k + 7.5 step_k),   p'_k = p_k step_k 2^-E rounded to f16
-// p' is the one rounding to 16 bits (as with the other caches); the middle of the range goes in the fp32 sum at the right, so that what the rounding touches is no
-// larger than the values' spread.  sum(p') comes from an MMA against a row of ones, i.e. from exactly the p' that the others used.  2^E is the largest
-// step so far, rounded down to a power of two: p' <= 2, and held to 2^-25 of that; the sums are rescaled where it grows, as where a maximum does.
+// p' is the one rounding to 16 bits (as with the other caches).  With F16 results the middle of the range goes in the fp32 sum at the right, so that what the
+// rounding touches is no larger than the values' spread, and sum(p') comes from an MMA against a row of ones, i.e. from exactly the p' that the others used;
+// a BF16 result is rounded to an eighth of p''s precision, and the 7.5 and the MMA are left out.  2^E is the largest step so far, rounded down to a power of two: p' <= 2, and held to 2^-25 of that; the sums are rescaled where it grows, as where a maximum does.
 // As in Cache8 the order in which a contraction runs is free: of key row g lane t takes the 16-byte piece t, whose word w has the k-steps
 // 2w and 2w + 1 (registers: elements {0, 4}, {1, 5}; {2, 6}, {3, 7}; the query fragment is loaded the same way).  Of V lane (g, t) takes 8 bytes,
 // d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; with halves of two keys' words side by side the same masks give both keys' numbers, and accumulator
@@ -441,7 +443,7 @@ __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(st
 template <typename T, bool SCORES = false>
 struct Cache4 {
     static constexpr bool kScores = SCORES;
-    static constexpr bool kOwnLoop = true;
+    static constexpr bool kFourBits = true;
     static constexpr int kGroups = 3;                         // resident per SM, by which a step is shared out, as with the 8-bit caches
     static constexpr int kSplitBlocks = 4;                    // in chunks: the registers are there, and the chains are what a warp waits for
     static constexpr int kRowBytes = kHeadDim / 2;
@@ -450,6 +452,7 @@ struct Cache4 {
     static constexpr int kStageBytes = 2 * kTileBytes + 2 * kKeys * 4;   // K, V, (step, low) of K and of V
     static constexpr int kStages = 3;
     static constexpr int kPartStride = kHeadDim + 4;
+    static constexpr bool kCentred = std::is_same<T, __half>::value;
     static constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u, kNone = 0xffffffffu;
 
     SoftmaxState s;
@@ -557,7 +560,7 @@ struct Cache4 {
         const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
-        const float mid0 = fmaf(vp[0].x, 7.5f, vp[0].y), mid1 = fmaf(vp[1].x, 7.5f, vp[1].y), st0 = vp[0].x * v_down, st1 = vp[1].x * v_down;
+        const float mid0 = kCentred ? fmaf(vp[0].x, 7.5f, vp[0].y) : vp[0].y, mid1 = kCentred ? fmaf(vp[1].x, 7.5f, vp[1].y) : vp[1].y, st0 = vp[0].x * v_down, st1 = vp[1].x * v_down;
         mid[0] = fmaf(p0, mid0, fmaf(p2, mid1, mid[0]));
         mid[1] = fmaf(p1, mid0, fmaf(p3, mid1, mid[1]));
         const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * st0, p1 * st0));
@@ -580,7 +583,7 @@ struct Cache4 {
         four(__byte_perm(x[0].y, x[1].y, 0x5410), __byte_perm(x[2].y, x[3].y, 0x5410), 4);
         four(__byte_perm(x[0].y, x[1].y, 0x7632), __byte_perm(x[2].y, x[3].y, 0x7632), 6);
         constexpr uint32_t kOnes = 0x3c003c00u;
-        mma_16816<__half>(ones, kOnes, kOnes, kOnes, kOnes, pb0, pb1);
+        if (kCentred) mma_16816<__half>(ones, kOnes, kOnes, kOnes, kOnes, pb0, pb1);
     }
     // 32 keys, of which `valid` (more than none) are there.
     __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int lane) {
@@ -709,7 +712,7 @@ struct Cache4 {
         }
     }
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
-        const float up = power_of_two(exponent()), off = fmaf(ones[h] * -7.5f, up, mid[h]);
+        const float up = power_of_two(exponent()), off = kCentred ? fmaf(ones[h] * -7.5f, up, mid[h]) : mid[h];
         auto even = [&](int i) { return fmaf(s.o[i][h] * 0x1p24f, up, off); };
         auto odd = [&](int i) { return fmaf(s.o[i][2 + h] * 0x1p20f, up, off); };
 #pragma unroll
@@ -792,7 +795,7 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
     const int warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = smem_u32(sm.warps[warp].ring);
     F st;
-    if constexpr (F::kOwnLoop) st.run(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane);
+    if constexpr (F::kFourBits) st.run(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane);
     else stream_tiles(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane, st);
     cp_async_wait<0>();
     __syncwarp();                              // this warp's ring is idle from here on

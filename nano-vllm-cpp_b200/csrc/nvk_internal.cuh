@@ -141,7 +141,7 @@ size_t decode_mma_workspace_bytes(int64_t batch, int num_heads, int num_kv_heads
 int check_decode_mma(const DecodeArgs& a);
 int launch_decode_mma(const DecodeArgs& a);
 namespace dec { struct DecodeParams; }
-int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster);
+int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster, bool four_bits = false);
 int launch_decode_merge(const dec::DecodeParams& p, int dtype, cudaStream_t stream);
 // Fused all-reduce launchers (tp_allreduce.cu); `pushed`: the other ranks' slices were already pushed by the GEMM
 // that produced the addend (gemm_fused.cu), the kernel starts with the reduction.
