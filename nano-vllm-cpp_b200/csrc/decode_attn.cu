@@ -556,39 +556,78 @@ int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_
 namespace {
 
 constexpr int kWeightThreads = 256;
-constexpr int kWeightKeys = 1024;   // of a block
+constexpr int kWeightEach = 4;      // keys of a thread
+constexpr int kWeightKeys = kWeightThreads * kWeightEach;
 
 // new[row, kvh, k] = old[row, kvh, k] + sum over the group's heads of exp2(score - M) / L, the score as the decode kernel left it (fp32) and (M, L) of
-// the whole context from its parts.
+// the whole context from its parts.  G: heads of a group, 0: any number.  What is read of the keys is on its way before the parts are brought together.
+template <int G>
 __global__ void __launch_bounds__(kWeightThreads) key_weights_kernel(const __grid_constant__ DecodeParams p, const KeyWeights w, int chunks) {
     __shared__ float2 s_ml[kMaxGroup];   // (M, 1 / L)
     pdl_wait_then_release();
     const int pair = blockIdx.x / chunks, first = (blockIdx.x - pair * chunks) * kWeightKeys;
     const int b = static_cast<int>(p.by_kv_heads.div(pair)), kvh = pair - b * p.num_kv_heads;
-    const int ctx = clamped_context(p, b);
-    if (first >= ctx) return;
+    const IndexArray::Raw raw_ctx = p.context_lens.raw(b);
     const int64_t row = w.rows != nullptr ? w.rows[b] : b;
-    if (row < 0 || row >= w.num_rows) return;
+    const int ctx = clamped_context(p, raw_ctx);
+    if (first >= ctx || row < 0 || row >= w.num_rows) return;
+    const int group = G > 0 ? G : p.group;
+    const float* scores = p.scores + static_cast<int64_t>(pair) * p.max_blocks * p.block_size * group;
+    const int64_t at = (row * p.num_kv_heads + kvh) * w.row_keys;
+    float sc[kWeightEach][G > 0 ? G : kMaxGroup], old[kWeightEach];
+#pragma unroll
+    for (int i = 0; i < kWeightEach; ++i) {
+        const int k = first + i * kWeightThreads + static_cast<int>(threadIdx.x);
+        const float* from = scores + static_cast<int64_t>(k) * group;
+        old[i] = k < ctx && w.old_weights != nullptr ? w.old_weights[at + k] : 0.0f;
+        if (k < ctx) {
+            if constexpr (G == 2) {
+                const float2 v = *reinterpret_cast<const float2*>(from);
+                sc[i][0] = v.x; sc[i][1] = v.y;
+            } else if constexpr (G == 4 || G == 8) {
+#pragma unroll
+                for (int h = 0; h < G; h += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(from + h);
+                    sc[i][h] = v.x; sc[i][h + 1] = v.y; sc[i][h + 2] = v.z; sc[i][h + 3] = v.w;
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < kMaxGroup; ++h)
+                    if (h < group) sc[i][G > 0 ? 0 : h] = from[h];
+            }
+        }
+    }
     const int len = range_len(p, ctx), parts = (ctx + len - 1) / len;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp < p.group) {
-        const float2* ml = p.ws_ml + static_cast<size_t>(pair) * p.num_splits * p.group + warp;
+    if (warp < group) {
+        const float2* ml = p.ws_ml + static_cast<size_t>(pair) * p.num_splits * group + warp;
         float m = -INFINITY, l = 0.0f;
-        for (int i = lane; i < parts; i += 32) m = fmaxf(m, ml[i * p.group].x);
+        for (int i = lane; i < parts; i += 32) {   // (one trip for up to 32 parts)
+            const float2 v = ml[i * group];
+            const float top = fmaxf(m, v.x);
+            l = l * fast_exp2(m - top) + v.y * fast_exp2(v.x - top);
+            m = top;
+        }
+        float top = m;
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        for (int i = lane; i < parts; i += 32) l = fmaf(fast_exp2(ml[i * p.group].x - m), ml[i * p.group].y, l);
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        l = lane < parts ? l * fast_exp2(m - top) : 0.0f;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        if (lane == 0) s_ml[warp] = make_float2(m, 1.0f / l);
+        if (lane == 0) s_ml[warp] = make_float2(top, 1.0f / l);
     }
     __syncthreads();
-    const float* scores = p.scores + static_cast<int64_t>(pair) * p.max_blocks * p.block_size * p.group;
-    const int64_t at = (row * p.num_kv_heads + kvh) * w.row_keys;
-    for (int k = first + threadIdx.x; k < min(ctx, first + kWeightKeys); k += kWeightThreads) {
+    float2 ml[G > 0 ? G : kMaxGroup];
+#pragma unroll
+    for (int h = 0; h < (G > 0 ? G : kMaxGroup); ++h) ml[h] = s_ml[h < group ? h : 0];
+#pragma unroll
+    for (int i = 0; i < kWeightEach; ++i) {
+        const int k = first + i * kWeightThreads + static_cast<int>(threadIdx.x);
         float sum = 0.0f;
-        for (int h = 0; h < p.group; ++h) sum = fmaf(fast_exp2(scores[static_cast<int64_t>(k) * p.group + h] - s_ml[h].x), s_ml[h].y, sum);
-        w.new_weights[at + k] = (w.old_weights != nullptr ? w.old_weights[at + k] : 0.0f) + sum;
+#pragma unroll
+        for (int h = 0; h < (G > 0 ? G : kMaxGroup); ++h)
+            if (h < group) sum = fmaf(fast_exp2(sc[i][h] - ml[h].x), ml[h].y, sum);
+        if (k < ctx) w.new_weights[at + k] = old[i] + sum;
     }
 }
 
@@ -622,7 +661,10 @@ int launch_weights_typed(const DecodeArgs& a, const void* k_params, const void* 
         return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): %d parts to a context", plan.num_splits);
     rc = launch_typed<F, T>(d, k_params, v_params, reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + space.scores), &plan);
     if (rc != NVK_OK) return rc;
-    const cudaError_t e = launch_pdl(key_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWeightThreads), 0, a.stream, plan, w, static_cast<int>(chunks));
+    const int group = a.num_heads / a.num_kv_heads;
+    const auto kernel = group == 1 ? key_weights_kernel<1> : group == 2 ? key_weights_kernel<2> : group == 4 ? key_weights_kernel<4>
+                        : group == 8 ? key_weights_kernel<8> : key_weights_kernel<0>;
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWeightThreads), 0, a.stream, plan, w, static_cast<int>(chunks));
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "key_weights_kernel launch: %s", cudaGetErrorString(e));
     return check_launch("key_weights_kernel launch");
 }

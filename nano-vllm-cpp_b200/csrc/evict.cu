@@ -3,20 +3,34 @@
 // Of every (sequence, KV head) the first `sinks` keys stay, the last `recent`, and of those between the ones of the largest weights, `budget` in all
 // (of equal weights the key that comes first; NaN counts as the least).  What stays closes up, in its order, its weights with it.
 //
-// One block has a (sequence, KV head).  The weight that just stays is found by its bits, eight at a time from the top: a histogram of the keys that
-// agree so far, and a scan from the largest class down.  Then the keys are taken in order, a tile at a time: who stays goes to the place that the number of
-// those before it gives.  A key never moves up, and a tile's rows are all read before any is written, so that the same blocks can be source and
-// destination.
+// HBM-bound: the weights are read, the rows of what stays are read and written.  Where there are few (sequence, KV head) pairs several blocks share one: each
+// finds for itself who stays (weights are a small part of what is read, and come from L2; histograms added up through distributed shared memory took 10 us
+// more a pass), and moves the rows of its share of the tiles.  A block
+//   1  reads the weights as whole numbers of the same order into shared memory (contexts of up to 16384 keys; longer ones are read again for every step);
+//   2  finds the order that just stays by its bits, 11, 11 and 10 of them from the top: a histogram of the keys that agree so far, and a scan from the largest
+//      class down (weights share exponents: with 8 bits at first the counters of a few classes are the bottleneck);
+//   3  counts what stays in every tile of 128 keys, which gives the place where each tile's keys go;
+//   4  lists the rows of its tiles, old place and new, and moves them, eight 16-byte pieces under way in every thread (a warp alone with the rows of
+//      its tile: 4 sequences of 2000 to 4096 keys, 8 KV heads, 79 us; the last keys all stay, and who has them ends last).
+// Where the new blocks are the old ones (in place) a row may be written where another one has still to be read.  Then a pair's first block does all of it in order:
+// a key never moves up, and a set of rows is read before any of it is written.
 #include "nvk_internal.cuh"
 
+#include <algorithm>
 #include <atomic>
 
 namespace nvk {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kTile = kThreads;           // keys looked at together
+constexpr int kTile = kThreads;           // keys that a block looks at together
+constexpr int kWarpTile = 128;            // keys that a warp looks at together
+constexpr int kMaxTiles = 1024;           // warp tiles counted one by one; of longer contexts several together
+constexpr int kCached = 16384;            // keys whose orders are kept
+constexpr int kList = kWarps * kWarpTile; // rows listed before they are moved
+constexpr int kBins = 2048;
+constexpr int kMaxSplit = 64;             // blocks of a pair
 constexpr int kDim = 128;
 
 struct EvictParams {
@@ -25,8 +39,18 @@ struct EvictParams {
     IndexArray context_lens; IndexArray block_tables; IndexArray new_tables;
     void* new_lens;
     int64_t num_rows, row_keys, max_blocks, new_max_blocks, num_cache_blocks, budget, sinks, recent;
-    int num_kv_heads, block_size;
+    int num_kv_heads, block_size, split;
     FastDiv by_block;
+};
+
+struct Shared {
+    int bins[kBins];
+    int2 tiles[kMaxTiles];                // of every tile, then before it: keys that stay without regard to ties, ties
+    int2 warp[kWarps];
+    int list_from[kList], list_to[kList];
+    uint32_t prefix;
+    int left, listed;
+    uint32_t orders[kCached];
 };
 
 // Weights as whole numbers of the same order; NaN below all.
@@ -35,169 +59,322 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return w != w ? 0u : (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-struct Select { int hist[256]; int warp_sum[kWarps]; uint32_t prefix; int left; };
+// Sums over the threads before a thread's own, and over all.
+__device__ __forceinline__ int2 scan(int2 v, Shared& sm, int2& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int2 upto = v;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        const int x = __shfl_up_sync(0xffffffffu, upto.x, d), y = __shfl_up_sync(0xffffffffu, upto.y, d);
+        if (lane >= d) { upto.x += x; upto.y += y; }
+    }
+    __syncthreads();                      // (what was in sm.warp has been read)
+    if (lane == 31) sm.warp[warp] = upto;
+    __syncthreads();
+    int2 before = make_int2(0, 0);
+    total = make_int2(0, 0);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const int2 t = sm.warp[w];
+        if (w < warp) { before.x += t.x; before.y += t.y; }
+        total.x += t.x; total.y += t.y;
+    }
+    return make_int2(before.x + upto.x - v.x, before.y + upto.y - v.y);
+}
 
-// The `take`-th largest of weights[0 .. n) (1 <= take <= n): its order, and how many of that order are among the `take`.
-__device__ __forceinline__ void nth_largest(const float* weights, int n, int take, Select& sm, uint32_t& order, int& ties) {
+// Of one (sequence, KV head): who stays.  Keys [lo, hi) go by their weight: those above `order` stay, and the first `ties` of that order.
+struct Choice {
+    int n, lo, hi, take, ties;
+    uint32_t order;
+    bool cached;
+    __device__ __forceinline__ uint32_t order_at(const Shared& sm, const float* weights, int pos) const {
+        return cached ? sm.orders[pos] : order_of(weights[pos]);
+    }
+    // (stays without regard to ties, is a tie)
+    __device__ __forceinline__ int2 of(const Shared& sm, const float* weights, int pos) const {
+        if (pos >= n) return make_int2(0, 0);
+        if (pos < lo || pos >= hi) return make_int2(1, 0);
+        if (take == 0) return make_int2(0, 0);
+        const uint32_t o = order_at(sm, weights, pos);
+        return make_int2(o > order, o == order);
+    }
+};
+
+// The `take`-th largest of weights[lo .. hi) (1 <= take <= hi - lo): its order, and how many of that order are among the `take`.
+__device__ __forceinline__ void choose(const float* weights, Choice& c, Shared& sm) {
     const int tid = threadIdx.x;
     uint32_t prefix = 0;
-    int left = take;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) sm.hist[tid] = 0;
+    int left = c.take, known = 0;         // bits of the order that are known
+    c.cached = c.hi <= kCached;
+#pragma unroll 1
+    for (int bits = 11; known < 32; bits = known < 22 ? 11 : 10) {
+        const int shift = 32 - known - bits, bins = 1 << bits;
+        for (int i = tid; i < kBins; i += kThreads) sm.bins[i] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += kThreads) {
-            const uint32_t o = order_of(weights[i]);
-            if (shift == 24 || (o >> (shift + 8)) == prefix) atomicAdd(&sm.hist[(o >> shift) & 255u], 1);
+        auto count = [&](uint32_t o) {
+            if (known == 0 || (o >> (shift + bits)) == prefix) atomicAdd(&sm.bins[(o >> shift) & (bins - 1)], 1);
+        };
+        if (c.cached && known > 0) {
+            for (int pos = c.lo + tid; pos < c.hi; pos += kThreads) count(sm.orders[pos]);
+        } else {
+            constexpr int kAhead = 8;
+            for (int pos0 = c.lo + tid; pos0 < c.hi; pos0 += kAhead * kThreads) {
+                float w[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) w[i] = pos0 + i * kThreads < c.hi ? weights[pos0 + i * kThreads] : 0.0f;
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    const int pos = pos0 + i * kThreads;
+                    if (pos < c.hi) {
+                        const uint32_t o = order_of(w[i]);
+                        if (c.cached) sm.orders[pos] = o;
+                        count(o);
+                    }
+                }
+            }
         }
         __syncthreads();
-        if (tid < 32) {   // eight classes a lane, the largest first
-            int count[8], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += count[i] = sm.hist[255 - (8 * tid + i)];
-            int upto = sum;
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int up = __shfl_up_sync(0xffffffffu, upto, d);
-                if (tid >= d) upto += up;
-            }
-            int before = upto - sum;
-            if (before < left && left <= upto) {   // (one lane)
-                int i = 0;
-                while (i < 7 && before + count[i] < left) before += count[i++];
-                sm.prefix = (prefix << 8) | static_cast<uint32_t>(255 - (8 * tid + i));
-                sm.left = left - before;
-            }
+        constexpr int kEach = kBins / kThreads;   // neighbouring classes of a thread, the largest first
+        static_assert(kEach == 4, "one int4 a thread");
+        const int4 v = reinterpret_cast<const int4*>(sm.bins)[kThreads - 1 - tid];
+        const int number[kEach] = {v.w, v.z, v.y, v.x}, sum = v.x + v.y + v.z + v.w;
+        int2 total;
+        int before = scan(make_int2(sum, 0), sm, total).x;
+        if (before < left && left <= before + sum) {   // (one thread)
+            int i = 0;
+            while (i < kEach - 1 && before + number[i] < left) before += number[i++];
+            sm.prefix = (prefix << bits) | static_cast<uint32_t>(kBins - 1 - (tid * kEach + i));
+            sm.left = left - before;
         }
         __syncthreads();
         prefix = sm.prefix;
         left = sm.left;
-        __syncthreads();
+        known += bits;
     }
-    order = prefix;
-    ties = left;
-}
-
-// Places of the flags before a thread's own, and how many there are in all.
-__device__ __forceinline__ int count_before(bool flag, int* warp_sum, int& total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const unsigned int mask = __ballot_sync(0xffffffffu, flag);
-    __syncthreads();
-    if (lane == 0) warp_sum[warp] = __popc(mask);
-    __syncthreads();
-    const int mine = warp_sum[lane];
-    int upto = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-        const int up = __shfl_up_sync(0xffffffffu, upto, d);
-        if (lane >= d) upto += up;
-    }
-    total = __shfl_sync(0xffffffffu, upto, 31);
-    return __shfl_sync(0xffffffffu, upto - mine, warp) + __popc(mask & ((1u << lane) - 1u));
+    c.order = prefix;
+    c.ties = left;
 }
 
 // Cache row of position `pos`, or -1.
-__device__ __forceinline__ int64_t row_of(const EvictParams& p, const IndexArray& tables, int64_t max_blocks, int b, int pos) {
+__device__ __forceinline__ int row_of(const EvictParams& p, const IndexArray& tables, int64_t max_blocks, int b, int pos) {
     const int blk = static_cast<int>(p.by_block.div(pos));
     if (blk >= max_blocks) return -1;
     const int64_t id = tables[b * max_blocks + blk];
-    return id >= 0 && id < p.num_cache_blocks ? id * p.block_size + (pos - blk * p.block_size) : -1;
+    return id >= 0 && id < p.num_cache_blocks ? static_cast<int>(id) * p.block_size + (pos - blk * p.block_size) : -1;
 }
+
+// Rows of one KV head: PIECES of 16 bytes of a key, as many of its value, and their params.
+template <int PIECES, bool PARAMS>
+struct Mover {
+    static constexpr int kPerRow = 2 * PIECES;
+    const EvictParams& p;
+    const int kvh;
+    __device__ __forceinline__ uint4 load(int from, int c) const {
+        if (from < 0) return make_uint4(0u, 0u, 0u, 0u);
+        const int64_t at = (static_cast<int64_t>(from) * p.num_kv_heads + kvh) * PIECES;
+        return c < PIECES ? static_cast<const uint4*>(p.k_cache)[at + c] : static_cast<const uint4*>(p.v_cache)[at + c - PIECES];
+    }
+    __device__ __forceinline__ void store(int to, int c, const uint4& v) const {
+        if (to < 0) return;
+        const int64_t at = (static_cast<int64_t>(to) * p.num_kv_heads + kvh) * PIECES;
+        (c < PIECES ? static_cast<uint4*>(p.k_cache) + at + c : static_cast<uint4*>(p.v_cache) + at + c - PIECES)[0] = v;
+    }
+    __device__ __forceinline__ uint2 load_params(int from) const {
+        const int64_t at = static_cast<int64_t>(from) * p.num_kv_heads + kvh;
+        return from < 0 ? make_uint2(0u, 0u) : make_uint2(p.k_params[at], p.v_params[at]);
+    }
+    __device__ __forceinline__ void store_params(int to, uint2 v) const {
+        const int64_t at = static_cast<int64_t>(to) * p.num_kv_heads + kvh;
+        if (to >= 0) { p.k_params[at] = v.x; p.v_params[at] = v.y; }
+    }
+    // `count` rows of a list, by `threads` threads of which this is number `id`.  ORDERED: by the whole block, and a set is read before any of it is written.
+    template <bool ORDERED> __device__ __forceinline__ void move(const int* list_from, const int* list_to, int count, int id, int threads) const {
+        constexpr int kSet = ORDERED ? 4 : 8;
+        for (int first = id; first - id < count * kPerRow; first += kSet * threads) {
+            uint4 v[kSet];
+#pragma unroll
+            for (int i = 0; i < kSet; ++i) {
+                const int at = first + i * threads, r = at / kPerRow;
+                if (r < count) v[i] = load(list_from[r], at - r * kPerRow);
+            }
+            if (ORDERED) __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kSet; ++i) {
+                const int at = first + i * threads, r = at / kPerRow;
+                if (r < count) store(list_to[r], at - r * kPerRow, v[i]);
+            }
+        }
+        if (PARAMS) {
+            for (int first = id; first - id < count; first += threads) {
+                uint2 v = make_uint2(0u, 0u);
+                if (first < count) v = load_params(list_from[first]);
+                if (ORDERED) __syncthreads();
+                if (first < count) store_params(list_to[first], v);
+            }
+        }
+    }
+};
 
 // PIECES: 16-byte pieces of a key's (value's) row of one head.
 template <int PIECES, bool PARAMS>
-__global__ void __launch_bounds__(kThreads) evict_kernel(const __grid_constant__ EvictParams p) {
-    __shared__ Select sel;
-    __shared__ int64_t s_from[kTile], s_to[kTile];
+__global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constant__ EvictParams p) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    Shared& sm = *reinterpret_cast<Shared*>(smem);
     pdl_wait_then_release();
-    const int tid = threadIdx.x;
-    const int b = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x - b * p.num_kv_heads;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int pair = blockIdx.x / p.split, rank = blockIdx.x - pair * p.split;
+    const int b = pair / p.num_kv_heads, kvh = pair - b * p.num_kv_heads;
     const int64_t ctx = p.context_lens[b], cap = p.max_blocks * p.block_size;
-    const int n = static_cast<int>(ctx < 0 ? 0 : ctx < cap ? ctx : cap);
+    Choice c{};
+    c.n = static_cast<int>(ctx < 0 ? 0 : ctx < cap ? ctx : cap);
     const int64_t wrow = p.rows != nullptr ? p.rows[b] : b;
-    const bool live = wrow >= 0 && wrow < p.num_rows;
-    const int new_n = live && n > p.budget ? static_cast<int>(p.budget) : n;
-    if (kvh == 0 && tid == 0) {
+    const bool live = wrow >= 0 && wrow < p.num_rows, all = !live || c.n <= p.budget;
+    const int new_n = all ? c.n : static_cast<int>(p.budget);
+    if (kvh == 0 && rank == 0 && tid == 0) {
         if (p.context_lens.wide) static_cast<int64_t*>(p.new_lens)[b] = new_n;
         else static_cast<int32_t*>(p.new_lens)[b] = new_n;
     }
     if (!live) return;
     const float* weights = p.weights + (wrow * p.num_kv_heads + kvh) * p.row_keys;
     float* new_weights = p.new_weights + (wrow * p.num_kv_heads + kvh) * p.row_keys;
-    // Keys [lo, hi) go by their weight: those above `order` stay, and the first `ties` of that order.
-    const bool all = n <= p.budget;
-    const int lo = all ? n : static_cast<int>(p.sinks), hi = all ? n : n - static_cast<int>(p.recent), take = all ? 0 : static_cast<int>(p.budget - p.sinks - p.recent);
-    uint32_t order = 0xffffffffu;
-    int ties = 0;
-    if (take > 0) nth_largest(weights + lo, hi - lo, take, sel, order, ties);
-    int kept = 0, equal = 0;
-    for (int base = 0; base < n; base += kTile) {
-        const int pos = base + tid;
-        const float w = pos < n ? weights[pos] : 0.0f;
-        const bool mid = pos >= lo && pos < hi;
-        const uint32_t o = order_of(w);
-        const bool tie = mid && take > 0 && o == order;
-        int in_tile, ties_in_tile;
-        const int ties_before = equal + count_before(tie, sel.warp_sum, ties_in_tile);
-        equal += ties_in_tile;
-        const bool stays = pos < n && (!mid || (take > 0 && (o > order || (tie && ties_before < ties))));
-        const int to = kept + count_before(stays, sel.warp_sum, in_tile);
-        if (stays) {
-            s_from[to - kept] = row_of(p, p.block_tables, p.max_blocks, b, pos);
-            s_to[to - kept] = row_of(p, p.new_tables, p.new_max_blocks, b, to);
-            new_weights[to] = w;          // (all weights of this tile and of those before have been read)
-        }
-        __syncthreads();
-        // The rows, a set of pieces of every thread at a time: all read before any is written.
-        constexpr int kSet = 8, kPerRow = 2 * PIECES + (PARAMS ? 1 : 0);
-        const size_t stride = static_cast<size_t>(p.num_kv_heads) * PIECES;   // pieces of a cache row
-        for (int first = 0; first < in_tile * kPerRow; first += kSet * kThreads) {
-            uint4 v[kSet];
-#pragma unroll
-            for (int i = 0; i < kSet; ++i) {
-                const int at = first + i * kThreads + tid;
-                v[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (at < in_tile * kPerRow) {
-                    const int r = at / kPerRow, c = at - r * kPerRow;
-                    const int64_t from = s_from[r];
-                    if (from >= 0 && from != s_to[r]) {
-                        if (c < PIECES) v[i] = static_cast<const uint4*>(p.k_cache)[from * stride + kvh * PIECES + c];
-                        else if (c < 2 * PIECES) v[i] = static_cast<const uint4*>(p.v_cache)[from * stride + kvh * PIECES + c - PIECES];
-                        else { v[i].x = p.k_params[from * p.num_kv_heads + kvh]; v[i].y = p.v_params[from * p.num_kv_heads + kvh]; }
-                    }
-                }
+    // In place, if a block is its own successor, or if the weights are: whoever reads a place has to have done so before it is written.
+    bool same = weights == new_weights;
+    for (int i = tid; i < p.new_max_blocks && i < p.max_blocks && static_cast<int64_t>(i) * p.block_size < new_n; i += kThreads)
+        same |= p.new_tables[b * p.new_max_blocks + i] == p.block_tables[b * p.max_blocks + i];
+    const bool ordered = __syncthreads_or(same);
+    if (ordered && rank > 0) return;
+    c.lo = all ? c.n : static_cast<int>(p.sinks);
+    c.hi = all ? c.n : c.n - static_cast<int>(p.recent);
+    c.take = all ? 0 : static_cast<int>(p.budget - p.sinks - p.recent);
+    if (c.take > 0) choose(weights, c, sm);
+    const Mover<PIECES, PARAMS> mover{p, kvh};
+    if (ordered) {
+        int2 at = make_int2(0, 0);         // keys that stay without regard to ties, and ties, so far
+        for (int pos = tid; pos - tid < c.n; pos += kTile) {
+            const float w = pos < c.n ? weights[pos] : 0.0f;
+            const int2 s = c.of(sm, weights, pos);
+            int2 total;
+            const int2 place = scan(s, sm, total);
+            const int ties = at.y + place.y, to = at.x + place.x + min(ties, c.ties), base = at.x + min(at.y, c.ties);
+            if (s.x != 0 || (s.y != 0 && ties < c.ties)) {
+                const int from_row = row_of(p, p.block_tables, p.max_blocks, b, pos), to_row = row_of(p, p.new_tables, p.new_max_blocks, b, to);
+                sm.list_from[to - base] = from_row;
+                sm.list_to[to - base] = from_row != to_row ? to_row : -1;
+                new_weights[to] = w;       // (all weights of this tile and of those before have been read)
             }
+            at.x += total.x; at.y += total.y;
             __syncthreads();
+            mover.template move<true>(sm.list_from, sm.list_to, at.x + min(at.y, c.ties) - base, tid, kThreads);
+            __syncthreads();
+        }
+        for (int64_t i = new_n + tid; i < p.row_keys; i += kThreads) new_weights[i] = 0.0f;
+        return;
+    }
+    // What stays of every tile; of longer contexts of `per` tiles together.
+    const int per = (c.n + kMaxTiles * kWarpTile - 1) / (kMaxTiles * kWarpTile), keys = per * kWarpTile, tiles = c.n > 0 ? (c.n + keys - 1) / keys : 0;
+    constexpr int kEach = kWarpTile / 32;
+    for (int t = warp; t < tiles; t += kWarps) {
+        int2 sum = make_int2(0, 0);
+        for (int pos0 = t * keys; pos0 < min(c.n, (t + 1) * keys); pos0 += kWarpTile) {
+            int2 s[kEach];
 #pragma unroll
-            for (int i = 0; i < kSet; ++i) {
-                const int at = first + i * kThreads + tid;
-                if (at < in_tile * kPerRow) {
-                    const int r = at / kPerRow, c = at - r * kPerRow;
-                    const int64_t to_row = s_to[r];
-                    if (to_row >= 0 && to_row != s_from[r]) {
-                        if (c < PIECES) static_cast<uint4*>(p.k_cache)[to_row * stride + kvh * PIECES + c] = v[i];
-                        else if (c < 2 * PIECES) static_cast<uint4*>(p.v_cache)[to_row * stride + kvh * PIECES + c - PIECES] = v[i];
-                        else { p.k_params[to_row * p.num_kv_heads + kvh] = v[i].x; p.v_params[to_row * p.num_kv_heads + kvh] = v[i].y; }
-                    }
-                }
+            for (int j = 0; j < kEach; ++j) s[j] = c.of(sm, weights, pos0 + 32 * j + lane);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                sum.x += __popc(__ballot_sync(0xffffffffu, s[j].x != 0));
+                sum.y += __popc(__ballot_sync(0xffffffffu, s[j].y != 0));
             }
         }
-        kept += in_tile;
+        if (lane == 0) sm.tiles[t] = sum;
+    }
+    __syncthreads();
+    {   // before every tile
+        constexpr int kOwn = kMaxTiles / kThreads;
+        int2 own[kOwn], sum = make_int2(0, 0), total;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const int t = tid * kOwn + i;
+            own[i] = t < tiles ? sm.tiles[t] : make_int2(0, 0);
+            sum.x += own[i].x; sum.y += own[i].y;
+        }
+        int2 before = scan(sum, sm, total);
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            if (tid * kOwn + i < tiles) sm.tiles[tid * kOwn + i] = before;
+            before.x += own[i].x; before.y += own[i].y;
+        }
+        if (tid == 0) sm.listed = 0;
         __syncthreads();
     }
-    for (int64_t i = new_n + tid; i < p.row_keys; i += kThreads) new_weights[i] = 0.0f;
+    const uint32_t below = (1u << lane) - 1u;
+    for (int t0 = rank; t0 < tiles; t0 += kWarps * p.split) {   // a tile of every warp
+        const int t = t0 + warp * p.split;
+        int2 at = t < tiles ? sm.tiles[t] : make_int2(0, 0);
+        for (int i = 0; i < per; ++i) {
+            const int pos0 = t < tiles ? t * keys + i * kWarpTile : c.n;
+            int2 s[kEach];
+            uint32_t stay[kEach], tie[kEach];
+            const int2 was = at;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) s[j] = c.of(sm, weights, pos0 + 32 * j + lane);
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                stay[j] = __ballot_sync(0xffffffffu, s[j].x != 0);
+                tie[j] = __ballot_sync(0xffffffffu, s[j].y != 0);
+                at.x += __popc(stay[j]); at.y += __popc(tie[j]);
+            }
+            const int base = was.x + min(was.y, c.ties), count = at.x + min(at.y, c.ties) - base;
+            int slot = 0;
+            if (lane == 0 && count > 0) slot = atomicAdd(&sm.listed, count);   // (in whatever order)
+            slot = __shfl_sync(0xffffffffu, slot, 0) - base;
+            int2 here = was;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j) {
+                const int pos = pos0 + 32 * j + lane, ties = here.y + __popc(tie[j] & below), to = here.x + __popc(stay[j] & below) + min(ties, c.ties);
+                if (s[j].x != 0 || (s[j].y != 0 && ties < c.ties)) {
+                    sm.list_from[slot + to] = row_of(p, p.block_tables, p.max_blocks, b, pos);
+                    sm.list_to[slot + to] = row_of(p, p.new_tables, p.new_max_blocks, b, to);
+                    new_weights[to] = weights[pos];
+                }
+                here.x += __popc(stay[j]); here.y += __popc(tie[j]);
+            }
+            __syncthreads();
+            mover.template move<false>(sm.list_from, sm.list_to, sm.listed, tid, kThreads);
+            __syncthreads();
+            if (tid == 0) sm.listed = 0;
+            __syncthreads();
+        }
+    }
+    for (int64_t i = new_n + tid + rank * kThreads; i < p.row_keys; i += p.split * kThreads) new_weights[i] = 0.0f;
+}
+
+template <int PIECES, bool PARAMS>
+cudaError_t launch_typed(const EvictParams& p, unsigned grid, cudaStream_t stream) {
+    static std::atomic<bool> attr_done[64] = {};  // per device; the attribute call is idempotent
+    int device = 0;
+    cudaGetDevice(&device);
+    if (device < 0 || device >= 64 || !attr_done[device]) {
+        const cudaError_t e = cudaFuncSetAttribute(evict_kernel<PIECES, PARAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+        if (e != cudaSuccess) return e;
+        if (device >= 0 && device < 64) attr_done[device] = true;
+    }
+    return launch_pdl(evict_kernel<PIECES, PARAMS>, dim3(grid), dim3(kThreads), sizeof(Shared), stream, p);
 }
 
 }  // namespace
 
 int launch_evict(const EvictArgs& a) {
-    if (a.batch * a.num_kv_heads > 0x7fffffffLL || a.max_blocks * a.block_size >= 0x7fffffffLL - kTile || a.new_max_blocks * a.block_size >= 0x7fffffffLL)
-        return fail(NVK_ERR_UNSUPPORTED, "evict_kvcache: batch or block table too large");
+    if (a.batch * a.num_kv_heads > 0x7fffffffLL || a.max_blocks * a.block_size > (1LL << 30) || a.new_max_blocks * a.block_size > (1LL << 30) ||
+        a.num_cache_blocks > 0x7fffffffLL / a.block_size)
+        return fail(NVK_ERR_UNSUPPORTED, "evict_kvcache: batch, block table or cache too large");
+    // As many blocks to a pair as there are places for, two to an SM, and no more than there are pairs of tiles.
+    const int64_t pairs = a.batch * a.num_kv_heads, most = (a.max_blocks * a.block_size + 2 * kWarpTile - 1) / (2 * kWarpTile);
+    const int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * kSmCount / pairs, most), kMaxSplit)));
     const EvictParams p{a.k_cache, a.v_cache, static_cast<uint32_t*>(a.k_params), static_cast<uint32_t*>(a.v_params), a.weights, a.new_weights, a.rows,
                         a.context_lens, a.block_tables, a.new_tables, a.new_lens, a.num_rows, a.row_keys, a.max_blocks, a.new_max_blocks,
-                        a.num_cache_blocks, a.budget, a.sinks, a.recent, a.num_kv_heads, a.block_size, FastDiv(static_cast<uint32_t>(a.block_size))};
-    const dim3 grid(static_cast<unsigned>(a.batch * a.num_kv_heads)), block(kThreads);
-    const cudaError_t e = a.k_params != nullptr ? launch_pdl(evict_kernel<kDim / 2 / 16, true>, grid, block, 0, a.stream, p)
-                                                : launch_pdl(evict_kernel<kDim * 2 / 16, false>, grid, block, 0, a.stream, p);
+                        a.num_cache_blocks, a.budget, a.sinks, a.recent, a.num_kv_heads, a.block_size, split, FastDiv(static_cast<uint32_t>(a.block_size))};
+    const unsigned grid = static_cast<unsigned>(pairs * split);
+    const cudaError_t e = a.k_params != nullptr ? launch_typed<kDim / 2 / 16, true>(p, grid, a.stream) : launch_typed<kDim * 2 / 16, false>(p, grid, a.stream);
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "evict_kernel launch: %s", cudaGetErrorString(e));
     return check_launch("evict_kernel launch");
 }

@@ -9,6 +9,8 @@
 // range is not finite gets a pair of NaN, and reads as NaN.
 #include "nvk_internal.cuh"
 
+#include <type_traits>
+
 namespace nvk {
 namespace {
 
@@ -43,27 +45,66 @@ template <typename T> __device__ __forceinline__ uint32_t join_highest(uint32_t 
     return as_word(__hmax2_nan(as_pair<T>(__byte_perm(k, v, 0x5410)), as_pair<T>(__byte_perm(k, v, 0x7632))));
 }
 
-// The numbers of eight elements, as a word.  floor(q + 1/2) of the true quotient q = (x - low) / step, without a division: the product with 1 / step,
-// made smaller by more than its error (2^-16; the error is below 15 x 2^-21), rounds to that number or to the one before it, and it is the one after exactly if
-// x >= low + (n + 1/2) step, which fma rounded upwards decides exactly, x being representable.
-__device__ __forceinline__ uint32_t numbers(float (&x)[8], float low, float step) {
-    if (step < 0x1p-100f) {   // (1 / step may not be finite; the elements are small as well, since low's own spacing is no larger than the range)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= 0x1p100f;
-        low *= 0x1p100f;
-        step *= 0x1p100f;
-    }
+// Two floats in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2_up(uint64_t a, uint64_t b, uint64_t c) {   // rounded upwards
+    uint64_t d;
+    asm("fma.rp.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+
+// The numbers of eight elements (pairs of the type, as loaded), as a word.  floor(q + 1/2) of the true quotient q = (x - low) / step, without a division:
+// x / step - low / step - 1/4, each term rounded (off by less than 1/4, since |low| <= 2^11 ranges), rounds to that number or to the one before it, and it is
+// the one after exactly if x >= low + (n + 1/2) step, which fma rounded upwards decides exactly, x being representable.
+// CAREFUL: step is a subnormal number of the type: 1 / step may not be finite (all is multiplied by 2^100 first; elements are small as well, since low's own
+// spacing is no larger than the range), and numbers above 15 come out where it was rounded down.
+template <typename T, bool CAREFUL> __device__ __forceinline__ uint32_t numbers(const uint4& v, float low, float step) {
+    const float scale = CAREFUL && step < 0x1p-100f ? 0x1p100f : 1.0f;
+    if (CAREFUL) { low *= scale; step *= scale; }
     const float inv = __fdiv_rn(1.0f, step);
     constexpr float kMagic = 12582912.0f;   // 1.5 x 2^23: adding it rounds to a whole number, in the low bits of the sum
+    const uint64_t inv2 = pair_of(inv, inv), from = pair_of(fmaf(-low, inv, -0.25f), fmaf(-low, inv, -0.25f)), low2 = pair_of(low, low), step2 = pair_of(step, step);
+    const uint64_t magic = pair_of(kMagic, kMagic), back = pair_of(-kMagic, -kMagic), half = pair_of(0.5f, 0.5f);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t word = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float m = __fadd_rn(__fmaf_rn(__fsub_rn(x[i], low), inv, -0x1p-16f), kMagic);
-        const float border = __fmaf_ru(__fadd_rn(__fsub_rn(m, kMagic), 0.5f), step, low);
-        const uint32_t n = (__float_as_uint(m) & 0x3fu) + (x[i] >= border ? 1u : 0u);
-        word |= min(n, 15u) << (4 * i);     // (above 15 only where step is a subnormal number, rounded down)
+    for (int i = 0; i < 4; ++i) {
+        float2 x = Pair<T>::floats(w[i]);
+        if (CAREFUL) { x.x *= scale; x.y *= scale; }
+        const uint64_t m = add2(fma2(pair_of(x.x, x.y), inv2, from), magic);
+        const float2 border = floats_of(fma2_up(add2(add2(m, back), half), step2, low2)), whole = floats_of(m);
+        // (whole numbers are 12582912 + n as bits too; what the 12582912 leave in the word goes at the end)
+        uint32_t a = __float_as_uint(whole.x), b = __float_as_uint(whole.y);
+        if (CAREFUL) {
+            a = min((a & 0x3fu) + (x.x >= border.x ? 1u : 0u), 15u);
+            b = min((b & 0x3fu) + (x.y >= border.y ? 1u : 0u), 15u);
+        } else {
+            if (x.x >= border.x) word += 1u << (8 * i);
+            if (x.y >= border.y) word += 1u << (8 * i + 4);
+        }
+        word += (a << (8 * i)) + (b << (8 * i + 4));
     }
-    return word;
+    constexpr uint32_t kBits = 0x4b400000u;
+    return CAREFUL ? word : word - (kBits + (kBits << 4) + (kBits << 8));   // (beyond that the shifts leave nothing of them)
 }
 
 // A head vector's share of one lane -> numbers; step and low as stored.
@@ -73,16 +114,9 @@ template <typename T> __device__ __forceinline__ uint32_t quantise(const uint4& 
     step_out = ElemTraits<T>::from_float(fine ? __fdiv_rn(span, 15.0f) : NAN);
     low_out = ElemTraits<T>::from_float(fine ? low : NAN);
     const float step = ElemTraits<T>::to_float(step_out);
-    if (!(step > 0.0f)) return 0u;
-    float x[8];
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = Pair<T>::floats(w[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
-    }
-    return numbers(x, low, step);
+    constexpr float kNormal = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-126f;
+    if (step >= kNormal) return numbers<T, false>(v, low, step);
+    return step > 0.0f ? numbers<T, true>(v, low, step) : 0u;
 }
 
 // One warp quantises two (token, KV head) vectors of K and of V.
@@ -134,26 +168,31 @@ int launch_store_typed(const void* key, const void* value, void* k_cache, void* 
 
 // ---- gather ----------------------------------------------------------------------------------------------------------------
 constexpr int kGatherWarps = 8;
-constexpr int kGatherRows = 32;           // dense rows of a block
+constexpr int kGatherRows = 32;           // dense rows of a block, at most
+constexpr int kGatherAhead = 4;           // head vectors of K and of V that a lane has under way
 
 struct GatherParams {
     const uint32_t* k_cache; const uint32_t* v_cache; const uint32_t* k_params; const uint32_t* v_params;
     void* key; void* value;
     IndexArray cu; IndexArray block_tables;
     int64_t num_seqs, total, max_blocks, num_cache_blocks;
-    int block_size;
+    int block_size, rows;                 // `rows` of a block
     FastDiv by_heads;
 };
 
+// Numbers 2i and 2i + 1 of a word as a pair of the type: in the low bits of a mantissa, the constant above them taken off again, exactly.
+template <typename T> __device__ __forceinline__ typename Pair<T>::type number_pair(uint32_t word, uint32_t upper, int i) {   // upper: word >> 4
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr uint32_t kBits = kHalf ? 0x64006400u : 0x43004300u;   // 1024, 128
+    const uint32_t n = (__byte_perm(word, upper, 0x0400 + 0x0101 * i + (i << 12)) & 0x000f000fu) | kBits;
+    return __hsub2(as_pair<T>(n), as_pair<T>(kBits));
+}
 template <typename T> __device__ __forceinline__ uint4 dequantise(uint32_t word, uint32_t param) {
-    const float2 p = Pair<T>::floats(param);   // (step, low)
+    const uint32_t upper = word >> 4;
+    const auto step = as_pair<T>(__byte_perm(param, 0, 0x1010)), low = as_pair<T>(__byte_perm(param, 0, 0x3232));
     uint32_t out[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        // 2^23 + n, exactly; n is exact, the product too, and low + step n is rounded once to fp32 and once to the type
-        const float n0 = __uint_as_float(((word >> (8 * i)) & 15u) | 0x4b000000u) - 8388608.0f, n1 = __uint_as_float(((word >> (8 * i + 4)) & 15u) | 0x4b000000u) - 8388608.0f;
-        out[i] = ElemTraits<T>::pack2(fmaf(p.x, n0, p.y), fmaf(p.x, n1, p.y));
-    }
+    for (int i = 0; i < 4; ++i) out[i] = as_word(__hfma2(step, number_pair<T>(word, upper, i), low));   // (one rounding)
     return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
@@ -161,9 +200,9 @@ template <typename T>
 __global__ void __launch_bounds__(kGatherWarps * 32) gather_int4_kernel(const __grid_constant__ GatherParams p) {
     __shared__ int64_t s_row[kGatherRows];   // cache row of a dense row; -1: zeros
     pdl_wait_then_release();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kGatherRows;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(kGatherRows), p.total - first));
-    if (threadIdx.x < kGatherRows) {
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * p.rows;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(p.rows), p.total - first));
+    if (threadIdx.x < static_cast<unsigned>(rows)) {
         const int64_t r = first + threadIdx.x;
         int64_t lo = 0, hi = p.num_seqs;     // the last sequence that begins at or before r
         while (hi - lo > 1) {
@@ -180,19 +219,31 @@ __global__ void __launch_bounds__(kGatherWarps * 32) gather_int4_kernel(const __
         s_row[threadIdx.x] = row;
     }
     __syncthreads();
-    const int lane = threadIdx.x & 31, sub = lane % kLanes;
-    const int vectors = rows * static_cast<int>(p.by_heads.d);
-    uint4* key = static_cast<uint4*>(p.key) + first * p.by_heads.d * kLanes;
-    uint4* value = static_cast<uint4*>(p.value) + first * p.by_heads.d * kLanes;
-    for (int i = (threadIdx.x >> 5) * 2 + lane / kLanes; i < vectors; i += kGatherWarps * 2) {
-        const int r = static_cast<int>(p.by_heads.div(i)), head = i - r * static_cast<int>(p.by_heads.d);
-        const int64_t row = s_row[r];
-        const bool there = row >= 0;
-        const int64_t at = there ? row * p.by_heads.d + head : 0;
-        const uint32_t k = there ? p.k_cache[at * kLanes + sub] : 0u, v = there ? p.v_cache[at * kLanes + sub] : 0u;
-        const uint32_t kp = there ? p.k_params[at] : 0u, vp = there ? p.v_params[at] : 0u;
-        key[static_cast<int64_t>(i) * kLanes + sub] = dequantise<T>(k, kp);
-        value[static_cast<int64_t>(i) * kLanes + sub] = dequantise<T>(v, vp);
+    const int lane = threadIdx.x & 31, sub = lane % kLanes, heads = static_cast<int>(p.by_heads.d), vectors = rows * heads;
+    uint4* key = static_cast<uint4*>(p.key) + first * heads * kLanes + sub;
+    uint4* value = static_cast<uint4*>(p.value) + first * heads * kLanes + sub;
+    constexpr int kStride = kGatherWarps * 2;
+    for (int i0 = (threadIdx.x >> 5) * 2 + lane / kLanes; i0 < vectors; i0 += kStride * kGatherAhead) {
+        uint32_t k[kGatherAhead], v[kGatherAhead], kp[kGatherAhead], vp[kGatherAhead];
+#pragma unroll
+        for (int u = 0; u < kGatherAhead; ++u) {
+            const int i = min(i0 + u * kStride, vectors - 1), r = static_cast<int>(p.by_heads.div(i));
+            const int64_t row = s_row[r];
+            const int64_t at = row >= 0 ? row * heads + (i - r * heads) : 0;
+            k[u] = __ldcs(p.k_cache + at * kLanes + sub);
+            v[u] = __ldcs(p.v_cache + at * kLanes + sub);
+            kp[u] = p.k_params[at];
+            vp[u] = p.v_params[at];
+            if (row < 0) k[u] = v[u] = kp[u] = vp[u] = 0u;
+        }
+#pragma unroll
+        for (int u = 0; u < kGatherAhead; ++u) {
+            const int i = i0 + u * kStride;
+            if (i < vectors) {
+                key[static_cast<int64_t>(i) * kLanes] = dequantise<T>(k[u], kp[u]);
+                value[static_cast<int64_t>(i) * kLanes] = dequantise<T>(v[u], vp[u]);
+            }
+        }
     }
 }
 
@@ -207,10 +258,13 @@ int launch_store_int4(const void* key, const void* value, void* k_cache, void* v
 int launch_gather_int4(const void* k_cache, const void* v_cache, const void* k_params, const void* v_params, const IndexArray& cu, const IndexArray& tables,
                        int64_t num_seqs, int64_t total, int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int block_size, void* key,
                        void* value, int dtype, cudaStream_t stream) {
-    const int64_t blocks = (total + kGatherRows - 1) / kGatherRows;
+    // Few rows are spread over the SMs.
+    int rows = kGatherRows;
+    while (rows > 1 && (total + rows - 1) / rows < 4 * kSmCount) rows >>= 1;
+    const int64_t blocks = (total + rows - 1) / rows;
     if (blocks > 0x7fffffffLL || num_kv_heads > 0x7fffffff / kGatherRows) return fail(NVK_ERR_UNSUPPORTED, "gather_kvcache_int4: too many rows");
     const GatherParams p{static_cast<const uint32_t*>(k_cache), static_cast<const uint32_t*>(v_cache), static_cast<const uint32_t*>(k_params),
-                         static_cast<const uint32_t*>(v_params), key, value, cu, tables, num_seqs, total, max_blocks, num_cache_blocks, block_size,
+                         static_cast<const uint32_t*>(v_params), key, value, cu, tables, num_seqs, total, max_blocks, num_cache_blocks, block_size, rows,
                          FastDiv(static_cast<uint32_t>(num_kv_heads))};
     const dim3 grid(static_cast<unsigned>(blocks)), block(kGatherWarps * 32);
     const cudaError_t e = dtype == NVK_BF16 ? launch_pdl(gather_int4_kernel<__nv_bfloat16>, grid, block, 0, stream, p)
