@@ -6,9 +6,11 @@
 // HBM-bound: the weights are read, the rows of what stays are read and written.  Where there are few (sequence, KV head) pairs several blocks share one: each
 // finds for itself who stays (weights are a small part of what is read, and come from L2; histograms added up through distributed shared memory took 10 us
 // more a pass), and moves the rows of its share of the tiles.  A block
-//   1  reads the weights as whole numbers of the same order into shared memory (contexts of up to 16384 keys; longer ones are read again for every step);
+//   1  reads the weights as whole numbers of the same order into shared memory (contexts of up to 16384 keys, 45056 where it is alone on an SM; longer ones are
+//      read again for every step);
 //   2  finds the order that just stays by its bits, 11, 11 and 10 of them from the top: a histogram of the keys that agree so far, and a scan from the largest
-//      class down (weights share exponents: with 8 bits at first the counters of a few classes are the bottleneck);
+//      class down (weights share exponents: with 8 bits at first the counters of a few classes are the bottleneck; sorting out a class of up to 256 keys by
+//      counting, for each, those above it took as long as the two last histograms);
 //   3  counts what stays in every tile of 128 keys, which gives the place where each tile's keys go;
 //   4  lists the rows of its tiles, old place and new, and moves them, eight 16-byte pieces under way in every thread (a warp alone with the rows of
 //      its tile: 4 sequences of 2000 to 4096 keys, 8 KV heads, 79 us; the last keys all stay, and who has them ends last).
@@ -27,7 +29,8 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kTile = kThreads;           // keys that a block looks at together
 constexpr int kWarpTile = 128;            // keys that a warp looks at together
 constexpr int kMaxTiles = 1024;           // warp tiles counted one by one; of longer contexts several together
-constexpr int kCached = 16384;            // keys whose orders are kept
+constexpr int kCached = 16384;            // keys whose orders are kept, two blocks to an SM
+constexpr int kCachedAlone = 45056;       // one block
 constexpr int kList = kWarps * kWarpTile; // rows listed before they are moved
 constexpr int kBins = 2048;
 constexpr int kMaxSplit = 64;             // blocks of a pair
@@ -39,7 +42,7 @@ struct EvictParams {
     IndexArray context_lens; IndexArray block_tables; IndexArray new_tables;
     void* new_lens;
     int64_t num_rows, row_keys, max_blocks, new_max_blocks, num_cache_blocks, budget, sinks, recent;
-    int num_kv_heads, block_size, split;
+    int num_kv_heads, block_size, split, cached;
     FastDiv by_block;
 };
 
@@ -47,11 +50,13 @@ struct Shared {
     int bins[kBins];
     int2 tiles[kMaxTiles];                // of every tile, then before it: keys that stay without regard to ties, ties
     int2 warp[kWarps];
-    int list_from[kList], list_to[kList];
+    int2 list[kList];                     // old row and new one, -1: none
     uint32_t prefix;
     int left, listed;
-    uint32_t orders[kCached];
+    uint32_t orders[1];                   // as many as there is room for
 };
+constexpr size_t shared_bytes(int cached) { return (offsetof(Shared, orders) + cached * sizeof(uint32_t) + 15) / 16 * 16; }
+static_assert(shared_bytes(kCached) <= 113 * 1024 && shared_bytes(kCachedAlone) <= 227 * 1024, "two blocks to an SM, or one");
 
 // Weights as whole numbers of the same order; NaN below all.
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -101,11 +106,11 @@ struct Choice {
 };
 
 // The `take`-th largest of weights[lo .. hi) (1 <= take <= hi - lo): its order, and how many of that order are among the `take`.
-__device__ __forceinline__ void choose(const float* weights, Choice& c, Shared& sm) {
+__device__ __forceinline__ void choose(const float* weights, Choice& c, Shared& sm, int cached) {
     const int tid = threadIdx.x;
     uint32_t prefix = 0;
     int left = c.take, known = 0;         // bits of the order that are known
-    c.cached = c.hi <= kCached;
+    c.cached = c.hi <= cached;
 #pragma unroll 1
     for (int bits = 11; known < 32; bits = known < 22 ? 11 : 10) {
         const int shift = 32 - known - bits, bins = 1 << bits;
@@ -163,53 +168,65 @@ __device__ __forceinline__ int row_of(const EvictParams& p, const IndexArray& ta
     return id >= 0 && id < p.num_cache_blocks ? static_cast<int>(id) * p.block_size + (pos - blk * p.block_size) : -1;
 }
 
-// Rows of one KV head: PIECES of 16 bytes of a key, as many of its value, and their params.
+// Moves rows of one KV head: PIECES of 16 bytes of a key, as many of its value, and their params.  A thread has the same piece of every row that it moves: what is
+// left to do for one is a place in the list, two multiplications and the copy (with pieces dealt out one by one 111 instructions, and 32 sequences of 1000
+// to 8192 keys, 8 KV heads, took 119 us).
 template <int PIECES, bool PARAMS>
 struct Mover {
-    static constexpr int kPerRow = 2 * PIECES;
+    static constexpr int kPerRow = 2 * PIECES, kRows = kThreads / kPerRow;   // pieces of a row, rows moved together
     const EvictParams& p;
     const int kvh;
-    __device__ __forceinline__ uint4 load(int from, int c) const {
-        if (from < 0) return make_uint4(0u, 0u, 0u, 0u);
-        const int64_t at = (static_cast<int64_t>(from) * p.num_kv_heads + kvh) * PIECES;
-        return c < PIECES ? static_cast<const uint4*>(p.k_cache)[at + c] : static_cast<const uint4*>(p.v_cache)[at + c - PIECES];
+    unsigned char* base;                   // this thread's piece of cache row 0
+    uint32_t stride;                       // bytes of a cache row
+    __device__ __forceinline__ Mover(const EvictParams& params, int head) : p(params), kvh(head), stride(static_cast<uint32_t>(params.num_kv_heads) * PIECES * 16) {
+        const int c = static_cast<int>(threadIdx.x) % kPerRow;
+        base = static_cast<unsigned char*>(c < PIECES ? p.k_cache : p.v_cache) + (static_cast<int64_t>(kvh) * PIECES + c % PIECES) * 16;
     }
-    __device__ __forceinline__ void store(int to, int c, const uint4& v) const {
-        if (to < 0) return;
-        const int64_t at = (static_cast<int64_t>(to) * p.num_kv_heads + kvh) * PIECES;
-        (c < PIECES ? static_cast<uint4*>(p.k_cache) + at + c : static_cast<uint4*>(p.v_cache) + at + c - PIECES)[0] = v;
-    }
-    __device__ __forceinline__ uint2 load_params(int from) const {
-        const int64_t at = static_cast<int64_t>(from) * p.num_kv_heads + kvh;
-        return from < 0 ? make_uint2(0u, 0u) : make_uint2(p.k_params[at], p.v_params[at]);
-    }
-    __device__ __forceinline__ void store_params(int to, uint2 v) const {
-        const int64_t at = static_cast<int64_t>(to) * p.num_kv_heads + kvh;
-        if (to >= 0) { p.k_params[at] = v.x; p.v_params[at] = v.y; }
-    }
-    // `count` rows of a list, by `threads` threads of which this is number `id`.  ORDERED: by the whole block, and a set is read before any of it is written.
-    template <bool ORDERED> __device__ __forceinline__ void move(const int* list_from, const int* list_to, int count, int id, int threads) const {
-        constexpr int kSet = ORDERED ? 4 : 8;
-        for (int first = id; first - id < count * kPerRow; first += kSet * threads) {
-            uint4 v[kSet];
+    __device__ __forceinline__ uint4* at(int row) const { return reinterpret_cast<uint4*>(base + static_cast<uint64_t>(static_cast<uint32_t>(row)) * stride); }
+    template <int N> struct Set { uint4 v[N]; int to[N]; };
+    template <int N> __device__ __forceinline__ void load(Set<N>& set, const int2* list, int count, int r0) const {
 #pragma unroll
-            for (int i = 0; i < kSet; ++i) {
-                const int at = first + i * threads, r = at / kPerRow;
-                if (r < count) v[i] = load(list_from[r], at - r * kPerRow);
+        for (int i = 0; i < N; ++i) {
+            const int r = r0 + i * kRows;
+            const int2 row = r < count ? list[r] : make_int2(-1, -1);
+            set.to[i] = row.y;
+            set.v[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (row.x >= 0) set.v[i] = *at(row.x);
+        }
+    }
+    template <int N> __device__ __forceinline__ void store(const Set<N>& set) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (set.to[i] >= 0) *at(set.to[i]) = set.v[i];
+    }
+    // `count` rows of the list, by the whole block.  ORDERED: a set is read before any of it is written; otherwise the next set is on its way meanwhile.
+    template <bool ORDERED> __device__ __forceinline__ void move(const int2* list, int count) const {
+        const int first = static_cast<int>(threadIdx.x) / kPerRow;
+        if constexpr (ORDERED) {
+            Set<8> set;
+            for (int r0 = first; r0 - first < count; r0 += 8 * kRows) {   // (all threads take the same number of trips)
+                load(set, list, count, r0);
+                __syncthreads();
+                store(set);
             }
-            if (ORDERED) __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kSet; ++i) {
-                const int at = first + i * threads, r = at / kPerRow;
-                if (r < count) store(list_to[r], at - r * kPerRow, v[i]);
+        } else {
+            Set<4> a, b;
+            load(a, list, count, first);
+            for (int r0 = first; r0 < count; r0 += 8 * kRows) {
+                load(b, list, count, r0 + 4 * kRows);
+                store(a);
+                load(a, list, count, r0 + 8 * kRows);
+                store(b);
             }
         }
         if (PARAMS) {
-            for (int first = id; first - id < count; first += threads) {
-                uint2 v = make_uint2(0u, 0u);
-                if (first < count) v = load_params(list_from[first]);
+            for (int r0 = 0; r0 < count; r0 += kThreads) {
+                const int r = r0 + static_cast<int>(threadIdx.x);
+                const int2 row = r < count ? list[r] : make_int2(-1, -1);
+                const int64_t from = static_cast<int64_t>(row.x) * p.num_kv_heads + kvh, to = static_cast<int64_t>(row.y) * p.num_kv_heads + kvh;
+                const uint32_t k = row.x >= 0 ? p.k_params[from] : 0u, v = row.x >= 0 ? p.v_params[from] : 0u;
                 if (ORDERED) __syncthreads();
-                if (first < count) store_params(list_to[first], v);
+                if (row.y >= 0) { p.k_params[to] = k; p.v_params[to] = v; }
             }
         }
     }
@@ -224,6 +241,9 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int pair = blockIdx.x / p.split, rank = blockIdx.x - pair * p.split;
     const int b = pair / p.num_kv_heads, kvh = pair - b * p.num_kv_heads;
+    // (the first blocks' ids come with the context length)
+    const bool there = tid < p.new_max_blocks && tid < p.max_blocks;
+    const int64_t new_id = there ? p.new_tables[b * p.new_max_blocks + tid] : 0, old_id = there ? p.block_tables[b * p.max_blocks + tid] : 0;
     const int64_t ctx = p.context_lens[b], cap = p.max_blocks * p.block_size;
     Choice c{};
     c.n = static_cast<int>(ctx < 0 ? 0 : ctx < cap ? ctx : cap);
@@ -238,16 +258,16 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
     const float* weights = p.weights + (wrow * p.num_kv_heads + kvh) * p.row_keys;
     float* new_weights = p.new_weights + (wrow * p.num_kv_heads + kvh) * p.row_keys;
     // In place, if a block is its own successor, or if the weights are: whoever reads a place has to have done so before it is written.
-    bool same = weights == new_weights;
-    for (int i = tid; i < p.new_max_blocks && i < p.max_blocks && static_cast<int64_t>(i) * p.block_size < new_n; i += kThreads)
+    bool same = weights == new_weights || (there && static_cast<int64_t>(tid) * p.block_size < new_n && new_id == old_id);
+    for (int i = tid + kThreads; i < p.new_max_blocks && i < p.max_blocks && static_cast<int64_t>(i) * p.block_size < new_n; i += kThreads)
         same |= p.new_tables[b * p.new_max_blocks + i] == p.block_tables[b * p.max_blocks + i];
     const bool ordered = __syncthreads_or(same);
     if (ordered && rank > 0) return;
     c.lo = all ? c.n : static_cast<int>(p.sinks);
     c.hi = all ? c.n : c.n - static_cast<int>(p.recent);
     c.take = all ? 0 : static_cast<int>(p.budget - p.sinks - p.recent);
-    if (c.take > 0) choose(weights, c, sm);
-    const Mover<PIECES, PARAMS> mover{p, kvh};
+    if (c.take > 0) choose(weights, c, sm, p.cached);
+    const Mover<PIECES, PARAMS> mover(p, kvh);
     if (ordered) {
         int2 at = make_int2(0, 0);         // keys that stay without regard to ties, and ties, so far
         for (int pos = tid; pos - tid < c.n; pos += kTile) {
@@ -258,13 +278,12 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
             const int ties = at.y + place.y, to = at.x + place.x + min(ties, c.ties), base = at.x + min(at.y, c.ties);
             if (s.x != 0 || (s.y != 0 && ties < c.ties)) {
                 const int from_row = row_of(p, p.block_tables, p.max_blocks, b, pos), to_row = row_of(p, p.new_tables, p.new_max_blocks, b, to);
-                sm.list_from[to - base] = from_row;
-                sm.list_to[to - base] = from_row != to_row ? to_row : -1;
+                sm.list[to - base] = make_int2(from_row, from_row != to_row ? to_row : -1);
                 new_weights[to] = w;       // (all weights of this tile and of those before have been read)
             }
             at.x += total.x; at.y += total.y;
             __syncthreads();
-            mover.template move<true>(sm.list_from, sm.list_to, at.x + min(at.y, c.ties) - base, tid, kThreads);
+            mover.template move<true>(sm.list, at.x + min(at.y, c.ties) - base);
             __syncthreads();
         }
         for (int64_t i = new_n + tid; i < p.row_keys; i += kThreads) new_weights[i] = 0.0f;
@@ -332,14 +351,13 @@ __global__ void __launch_bounds__(kThreads, 2) evict_kernel(const __grid_constan
             for (int j = 0; j < kEach; ++j) {
                 const int pos = pos0 + 32 * j + lane, ties = here.y + __popc(tie[j] & below), to = here.x + __popc(stay[j] & below) + min(ties, c.ties);
                 if (s[j].x != 0 || (s[j].y != 0 && ties < c.ties)) {
-                    sm.list_from[slot + to] = row_of(p, p.block_tables, p.max_blocks, b, pos);
-                    sm.list_to[slot + to] = row_of(p, p.new_tables, p.new_max_blocks, b, to);
+                    sm.list[slot + to] = make_int2(row_of(p, p.block_tables, p.max_blocks, b, pos), row_of(p, p.new_tables, p.new_max_blocks, b, to));
                     new_weights[to] = weights[pos];
                 }
                 here.x += __popc(stay[j]); here.y += __popc(tie[j]);
             }
             __syncthreads();
-            mover.template move<false>(sm.list_from, sm.list_to, sm.listed, tid, kThreads);
+            mover.template move<false>(sm.list, sm.listed);
             __syncthreads();
             if (tid == 0) sm.listed = 0;
             __syncthreads();
@@ -354,11 +372,11 @@ cudaError_t launch_typed(const EvictParams& p, unsigned grid, cudaStream_t strea
     int device = 0;
     cudaGetDevice(&device);
     if (device < 0 || device >= 64 || !attr_done[device]) {
-        const cudaError_t e = cudaFuncSetAttribute(evict_kernel<PIECES, PARAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(Shared));
+        const cudaError_t e = cudaFuncSetAttribute(evict_kernel<PIECES, PARAMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_bytes(kCachedAlone));
         if (e != cudaSuccess) return e;
         if (device >= 0 && device < 64) attr_done[device] = true;
     }
-    return launch_pdl(evict_kernel<PIECES, PARAMS>, dim3(grid), dim3(kThreads), sizeof(Shared), stream, p);
+    return launch_pdl(evict_kernel<PIECES, PARAMS>, dim3(grid), dim3(kThreads), shared_bytes(p.cached), stream, p);
 }
 
 }  // namespace
@@ -367,12 +385,15 @@ int launch_evict(const EvictArgs& a) {
     if (a.batch * a.num_kv_heads > 0x7fffffffLL || a.max_blocks * a.block_size > (1LL << 30) || a.new_max_blocks * a.block_size > (1LL << 30) ||
         a.num_cache_blocks > 0x7fffffffLL / a.block_size)
         return fail(NVK_ERR_UNSUPPORTED, "evict_kvcache: batch, block table or cache too large");
-    // As many blocks to a pair as there are places for, two to an SM, and no more than there are pairs of tiles.
-    const int64_t pairs = a.batch * a.num_kv_heads, most = (a.max_blocks * a.block_size + 2 * kWarpTile - 1) / (2 * kWarpTile);
-    const int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * kSmCount / pairs, most), kMaxSplit)));
+    // As many blocks to a pair as there are places for, two to an SM, and no more than there are pairs of tiles; one to an SM where that lets few pairs of long
+    // contexts keep their orders.
+    const int64_t pairs = a.batch * a.num_kv_heads, tokens = a.max_blocks * a.block_size, most = (tokens + 2 * kWarpTile - 1) / (2 * kWarpTile);
+    const bool alone = tokens > kCached && 2 * pairs <= kSmCount;
+    const int cached = alone ? kCachedAlone : kCached;
+    const int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((alone ? 1 : 2) * kSmCount / pairs, most), kMaxSplit)));
     const EvictParams p{a.k_cache, a.v_cache, static_cast<uint32_t*>(a.k_params), static_cast<uint32_t*>(a.v_params), a.weights, a.new_weights, a.rows,
                         a.context_lens, a.block_tables, a.new_tables, a.new_lens, a.num_rows, a.row_keys, a.max_blocks, a.new_max_blocks,
-                        a.num_cache_blocks, a.budget, a.sinks, a.recent, a.num_kv_heads, a.block_size, split, FastDiv(static_cast<uint32_t>(a.block_size))};
+                        a.num_cache_blocks, a.budget, a.sinks, a.recent, a.num_kv_heads, a.block_size, split, cached, FastDiv(static_cast<uint32_t>(a.block_size))};
     const unsigned grid = static_cast<unsigned>(pairs * split);
     const cudaError_t e = a.k_params != nullptr ? launch_typed<kDim / 2 / 16, true>(p, grid, a.stream) : launch_typed<kDim * 2 / 16, false>(p, grid, a.stream);
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "evict_kernel launch: %s", cudaGetErrorString(e));
