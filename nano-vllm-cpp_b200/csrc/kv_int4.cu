@@ -15,7 +15,7 @@ namespace nvk {
 namespace {
 
 constexpr int kDim = 128;
-constexpr int kLanes = kDim / 8;          // lanes to a head vector: eight elements, 16 bytes, each
+constexpr int kLanes = kDim / 8;          // 16-byte pieces (eight elements) of a head vector
 constexpr int kStoreWarps = 8;
 
 template <typename T> struct Pair;
@@ -80,7 +80,8 @@ __device__ __forceinline__ uint64_t fma2_up(uint64_t a, uint64_t b, uint64_t c) 
 template <typename T, bool CAREFUL> __device__ __forceinline__ uint32_t numbers(const uint4& v, float low, float step) {
     const float scale = CAREFUL && step < 0x1p-100f ? 0x1p100f : 1.0f;
     if (CAREFUL) { low *= scale; step *= scale; }
-    const float inv = __fdiv_rn(1.0f, step);
+    float inv;                              // (to within one unit in its last place)
+    asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(inv) : "f"(step));
     constexpr float kMagic = 12582912.0f;   // 1.5 x 2^23: adding it rounds to a whole number, in the low bits of the sum
     const uint64_t inv2 = pair_of(inv, inv), from = pair_of(fmaf(-low, inv, -0.25f), fmaf(-low, inv, -0.25f)), low2 = pair_of(low, low), step2 = pair_of(step, step);
     const uint64_t magic = pair_of(kMagic, kMagic), back = pair_of(-kMagic, -kMagic), half = pair_of(0.5f, 0.5f);
@@ -107,48 +108,66 @@ template <typename T, bool CAREFUL> __device__ __forceinline__ uint32_t numbers(
     return CAREFUL ? word : word - (kBits + (kBits << 4) + (kBits << 8));   // (beyond that the shifts leave nothing of them)
 }
 
-// A head vector's share of one lane -> numbers; step and low as stored.
-template <typename T> __device__ __forceinline__ uint32_t quantise(const uint4& v, float low, float high, T& step_out, T& low_out) {
+// x / 15, correctly rounded: a quotient from the rounded reciprocal, and one step with its exact remainder (Markstein, Computation of elementary functions on the
+// IBM RISC System/6000 processor, 1990); small numbers, whose remainders may not be exact, are divided.
+__device__ __forceinline__ float fifteenth(float x) {
+    constexpr float kInv = 1.0f / 15.0f;
+    const float q = __fmul_rn(x, kInv);
+    return x >= 0x1p-100f ? __fmaf_rn(__fmaf_rn(-q, 15.0f, x), kInv, q) : __fdiv_rn(x, 15.0f);
+}
+// What is stored of a head vector beside its numbers: a pair (step, low).
+template <typename T> __device__ __forceinline__ uint32_t params_of(float low, float high) {
     const float span = __fsub_rn(high, low);
-    const bool fine = fabsf(span) < INFINITY;
-    step_out = ElemTraits<T>::from_float(fine ? __fdiv_rn(span, 15.0f) : NAN);
-    low_out = ElemTraits<T>::from_float(fine ? low : NAN);
-    const float step = ElemTraits<T>::to_float(step_out);
+    return fabsf(span) < INFINITY ? ElemTraits<T>::pack2(fifteenth(span), low) : ElemTraits<T>::pack2(NAN, NAN);
+}
+// A lane's two pieces of a head vector -> numbers.
+template <typename T> __device__ __forceinline__ uint2 quantise(const uint4 (&v)[2], uint32_t params) {
     constexpr float kNormal = std::is_same<T, __half>::value ? 0x1p-14f : 0x1p-126f;
-    if (step >= kNormal) return numbers<T, false>(v, low, step);
-    return step > 0.0f ? numbers<T, true>(v, low, step) : 0u;
+    const float2 p = Pair<T>::floats(params);
+    if (p.x >= kNormal) return make_uint2(numbers<T, false>(v[0], p.y, p.x), numbers<T, false>(v[1], p.y, p.x));
+    return p.x > 0.0f ? make_uint2(numbers<T, true>(v[0], p.y, p.x), numbers<T, true>(v[1], p.y, p.x)) : make_uint2(0u, 0u);
 }
 
-// One warp quantises two (token, KV head) vectors of K and of V.
+// One warp quantises four (token, KV head) vectors of K and of V, eight lanes to a vector, each with its pieces `sub` and `sub` + 8: what is done once for a vector
+// is as much as what is done for eight elements (with 16 lanes to a vector 310 instructions a warp for 1024 elements, and 36864 tokens of 8 heads took
+// 53 us; by 8 lanes 1.5 times as many for twice the elements).
+constexpr int kStoreLanes = 8, kStoreVectors = 32 / kStoreLanes;
 template <typename T>
 __global__ void __launch_bounds__(kStoreWarps * 32)
 store_int4_kernel(const T* __restrict__ key, const T* __restrict__ value, uint32_t* __restrict__ k_cache, uint32_t* __restrict__ v_cache,
                   uint32_t* __restrict__ k_params, uint32_t* __restrict__ v_params, const IndexArray slot_mapping, uint32_t total, const FastDiv by_heads,
                   int64_t cache_rows) {
     pdl_wait_then_release();
-    const uint32_t lane = threadIdx.x & 31u, sub = lane % kLanes;
-    uint32_t work = (blockIdx.x * kStoreWarps + (threadIdx.x >> 5)) * 2 + lane / kLanes;   // (token, head)
+    const uint32_t lane = threadIdx.x & 31u, sub = lane % kStoreLanes;
+    uint32_t work = (blockIdx.x * kStoreWarps + (threadIdx.x >> 5)) * kStoreVectors + lane / kStoreLanes;   // (token, head)
     if (work >= total) work = total - 1;   // lanes past the end repeat the last vector: the shuffles stay full-warp
     const uint32_t token = by_heads.div(work), head = work - token * by_heads.d;
-    const size_t src = static_cast<size_t>(work) * kDim + sub * 8;
-    const uint4 kv = __ldcs(reinterpret_cast<const uint4*>(key + src));
-    const uint4 vv = __ldcs(reinterpret_cast<const uint4*>(value + src));
-    const int64_t slot = slot_mapping[token];
-    uint32_t lo = join_lowest<T>(lowest2<T>(kv), lowest2<T>(vv)), hi = join_highest<T>(highest2<T>(kv), highest2<T>(vv));
+    const uint4* k_src = reinterpret_cast<const uint4*>(key) + static_cast<size_t>(work) * kLanes + sub;
+    const uint4* v_src = reinterpret_cast<const uint4*>(value) + static_cast<size_t>(work) * kLanes + sub;
+    const uint4 kv[2] = {__ldcs(k_src), __ldcs(k_src + kStoreLanes)}, vv[2] = {__ldcs(v_src), __ldcs(v_src + kStoreLanes)};
+    const IndexArray::Raw raw_slot = slot_mapping.raw(token);
+    auto both = [](uint32_t a, uint32_t b, bool low) { return as_word(low ? __hmin2_nan(as_pair<T>(a), as_pair<T>(b)) : __hmax2_nan(as_pair<T>(a), as_pair<T>(b))); };
+    uint32_t lo = join_lowest<T>(both(lowest2<T>(kv[0]), lowest2<T>(kv[1]), true), both(lowest2<T>(vv[0]), lowest2<T>(vv[1]), true));
+    uint32_t hi = join_highest<T>(both(highest2<T>(kv[0]), highest2<T>(kv[1]), false), both(highest2<T>(vv[0]), highest2<T>(vv[1]), false));
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
-        lo = as_word(__hmin2_nan(as_pair<T>(lo), as_pair<T>(__shfl_xor_sync(0xffffffffu, lo, o))));
-        hi = as_word(__hmax2_nan(as_pair<T>(hi), as_pair<T>(__shfl_xor_sync(0xffffffffu, hi, o))));
+    for (int o = kStoreLanes / 2; o > 0; o >>= 1) {
+        lo = both(lo, __shfl_xor_sync(0xffffffffu, lo, o), true);
+        hi = both(hi, __shfl_xor_sync(0xffffffffu, hi, o), false);
     }
+    const int64_t slot = slot_mapping.value(raw_slot);
     if (slot < 0 || slot >= cache_rows) return;
     const float2 low = Pair<T>::floats(lo), high = Pair<T>::floats(hi);
     const size_t row = static_cast<size_t>(slot) * by_heads.d + head;
-    union { T e[2]; uint32_t w; } kp, vp;
-    k_cache[row * kLanes + sub] = quantise<T>(kv, low.x, high.x, kp.e[0], kp.e[1]);
-    v_cache[row * kLanes + sub] = quantise<T>(vv, low.y, high.y, vp.e[0], vp.e[1]);
+    const uint32_t kp = params_of<T>(low.x, high.x), vp = params_of<T>(low.y, high.y);
+    const uint2 k = quantise<T>(kv, kp), v = quantise<T>(vv, vp);
+    uint32_t *k_dst = k_cache + row * kLanes + sub, *v_dst = v_cache + row * kLanes + sub;
+    k_dst[0] = k.x;
+    k_dst[kStoreLanes] = k.y;
+    v_dst[0] = v.x;
+    v_dst[kStoreLanes] = v.y;
     if (sub == 0) {
-        k_params[row] = kp.w;
-        v_params[row] = vp.w;
+        k_params[row] = kp;
+        v_params[row] = vp;
     }
 }
 
@@ -157,7 +176,8 @@ int launch_store_typed(const void* key, const void* value, void* k_cache, void* 
                        int64_t num_tokens, int num_kv_heads, int64_t cache_rows, cudaStream_t stream) {
     const int64_t work = num_tokens * num_kv_heads;
     if (work >= 0x7fffffffLL) return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_int4: too many tokens");
-    const int64_t blocks = (work + 2 * kStoreWarps - 1) / (2 * kStoreWarps);
+    constexpr int kPerBlock = kStoreVectors * kStoreWarps;
+    const int64_t blocks = (work + kPerBlock - 1) / kPerBlock;
     const cudaError_t e = launch_pdl(store_int4_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(kStoreWarps * 32), 0, stream, static_cast<const T*>(key),
                                      static_cast<const T*>(value), static_cast<uint32_t*>(k_cache), static_cast<uint32_t*>(v_cache),
                                      static_cast<uint32_t*>(k_params), static_cast<uint32_t*>(v_params), slots, static_cast<uint32_t>(work),
