@@ -94,7 +94,12 @@ __global__ void __launch_bounds__(kGroupThreads, F::kSplitBlocks) decode_split_k
     const int rank = p.chunk_major ? blockIdx.y : blockIdx.z, split = p.chunk_major ? blockIdx.z : blockIdx.y;
     const int b = p.longest_first ? sequence_of_rank(p, rank, *reinterpret_cast<SortScratch*>(smem)) : rank;
     if (p.longest_first) __syncthreads();   // (the ring takes the scratch's place)
-    run_split<F, T>(p, b, blockIdx.x, split, *reinterpret_cast<GroupSmem<F>*>(smem), threadIdx.x, 1);
+    if constexpr (F::kScores) {
+        __shared__ float2 s_heads[kMaxGroup];
+        run_split<F, T>(p, b, blockIdx.x, split, *reinterpret_cast<GroupSmem<F>*>(smem), threadIdx.x, 1, s_heads);
+    } else {
+        run_split<F, T>(p, b, blockIdx.x, split, *reinterpret_cast<GroupSmem<F>*>(smem), threadIdx.x, 1);
+    }
     if (p.beside) pdl_wait_beside();
 }
 
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(kGroupThreads, F::kGroups) decode_cluster_kern
             waited = true;
         };
         auto push = [&](int h, int quad, const float4& o, float m, float l) {
-            if (F::kScores && quad == 0) p.ws_ml[(static_cast<size_t>(pair) * p.num_splits + rank) * p.group + h] = make_float2(m, l);
+            if (F::kScores && n == 1 && quad == 0) s_ml[h] = make_float2(m, l);
             if (n == 1) {
                 write_quad(out + h * kHeadDim + 4 * quad, scaled(o, 1.0f / l));   // (rounded as write_merged does)
                 return;
@@ -209,6 +214,18 @@ __global__ void __launch_bounds__(kGroupThreads, F::kGroups) decode_cluster_kern
                 if (ctx == 0) acc = nothing_merged();
                 write_merged<T>(out + h * kHeadDim, acc, quad);
             }
+        }
+        if constexpr (F::kScores) {
+            __shared__ float2 s_heads[kMaxGroup];
+            if (n == 1) __syncthreads();
+            if (tid < p.group) {
+                float m = -INFINITY, l = 0.0f;
+                for (int r = 0; r < n; ++r) m = fmaxf(m, s_ml[r * p.group + tid].x);
+                for (int r = 0; r < n; ++r) l = fmaf(fast_exp2(s_ml[r * p.group + tid].x - m), s_ml[r * p.group + tid].y, l);
+                s_heads[tid] = make_float2(m, 1.0f / l);
+            }
+            __syncthreads();
+            if (t0 < t1) add_key_weights(p, b, kvh, t0, t1, s_heads, tid);
         }
     }
     if (p.beside) pdl_wait_beside();
@@ -422,9 +439,10 @@ int check_grid(const DecodeArgs& a, const dec::DecodeParams& p) {   // of decode
     return NVK_OK;
 }
 
-// `scores`, `ml`: where they are kept (F::kScores), and the (maximum, sum) of every part; *plan: how the step was shared out.
+// `scores`, `ml`, `weights`: where they are kept (F::kScores), the (maximum, sum) of every part, and what becomes of them; *plan: how the step was shared out.
 template <class F, typename T>
-int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, float* scores = nullptr, float2* ml = nullptr, DecodeParams* plan = nullptr) {
+int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, float* scores = nullptr, float2* ml = nullptr, const KeyWeights* weights = nullptr,
+                 DecodeParams* plan = nullptr) {
     constexpr int kSmem = static_cast<int>(sizeof(GroupSmem<F>));
     static std::atomic<bool> attr_done[64] = {};  // per device; the attribute calls are idempotent
     int device = 0;
@@ -443,6 +461,7 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     if constexpr (F::kScores) {
         p.scores = scores;
         p.ws_ml = ml;
+        p.weights = *weights;
         *plan = p;
     }
     if (cluster > 0) {
@@ -560,9 +579,10 @@ constexpr int kWeightEach = 4;      // keys of a thread
 constexpr int kWeightKeys = kWeightThreads * kWeightEach;
 
 // new[row, kvh, k] = old[row, kvh, k] + sum over the group's heads of exp2(score - M) / L, the score as the decode kernel left it (fp32) and (M, L) of
-// the whole context from its parts.  G: heads of a group, 0: any number.  What is read of the keys is on its way before the parts are brought together.
+// the whole context from its parts: for contexts in chunks.  G: heads of a group, 0: any number.  What is read of the keys is on its way before the parts are brought together.
 template <int G>
-__global__ void __launch_bounds__(kWeightThreads) key_weights_kernel(const __grid_constant__ DecodeParams p, const KeyWeights w, int chunks) {
+__global__ void __launch_bounds__(kWeightThreads) key_weights_kernel(const __grid_constant__ DecodeParams p, int chunks) {
+    const KeyWeights& w = p.weights;
     __shared__ float2 s_ml[kMaxGroup];   // (M, 1 / L)
     pdl_wait_then_release();
     const int pair = blockIdx.x / chunks, first = (blockIdx.x - pair * chunks) * kWeightKeys;
@@ -659,12 +679,12 @@ int launch_weights_typed(const DecodeArgs& a, const void* k_params, const void* 
     if (rc != NVK_OK) return rc;
     if (part_bytes(static_cast<size_t>(a.batch) * a.num_kv_heads * plan.num_splits, plan.group) > space.total - space.scores - space.ml)
         return fail(NVK_ERR_UNSUPPORTED, "decode attention (weights): %d parts to a context", plan.num_splits);
-    rc = launch_typed<F, T>(d, k_params, v_params, reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + space.scores), &plan);
-    if (rc != NVK_OK) return rc;
+    rc = launch_typed<F, T>(d, k_params, v_params, reinterpret_cast<float*>(base), reinterpret_cast<float2*>(base + space.scores), &w, &plan);
+    if (rc != NVK_OK || cluster > 0 || plan.num_splits == 1) return rc;   // (where a block has the whole context, or its cluster, it has added the weights itself)
     const int group = a.num_heads / a.num_kv_heads;
     const auto kernel = group == 1 ? key_weights_kernel<1> : group == 2 ? key_weights_kernel<2> : group == 4 ? key_weights_kernel<4>
                         : group == 8 ? key_weights_kernel<8> : key_weights_kernel<0>;
-    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWeightThreads), 0, a.stream, plan, w, static_cast<int>(chunks));
+    const cudaError_t e = launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kWeightThreads), 0, a.stream, plan, static_cast<int>(chunks));
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "key_weights_kernel launch: %s", cudaGetErrorString(e));
     return check_launch("key_weights_kernel launch");
 }
