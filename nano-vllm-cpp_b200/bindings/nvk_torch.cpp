@@ -10,10 +10,12 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/nvk.h"
 
@@ -214,6 +216,13 @@ template <bool FP8> long store8(PyObject* const* a) {
     return 1;
 }
 
+// All on the device that the call runs on.
+void check_here(std::initializer_list<const at::Tensor*> tensors) {
+    const auto device = c10::cuda::current_device();
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && t->device().index() != device) raise(PyExc_ValueError, "%s", "every tensor must live on the current CUDA device");
+}
+
 // ---- 4-bit caches ----
 void check_bytes(const char* name, const at::Tensor& t) {
     if (t.element_size() != 1) raise(PyExc_ValueError, "%s must have one-byte elements", name);
@@ -244,6 +253,7 @@ long store_int4(PyObject* const* a) {
         raise(PyExc_ValueError, "%s", "key and value must have the same shape and dtype");
     if (slots.numel() != key.size(0)) raise(PyExc_ValueError, "%s", "slot_mapping must have an element for every token");
     const Index index("slot_mapping", &slots);
+    check_here({&key, &value, &kc, &vc, &kp, &vp, &slots});
     const int64_t hkv = key.size(1), d = key.size(2), rows = rows4(kc, vc, kp, vp, key.scalar_type(), hkv, d);
     if (slots.numel() == 0) return 0;
     launch(nvk_store_kvcache_int4, ptr(key), ptr(value), ptr(kc), ptr(vc), ptr(kp), ptr(vp), index.p, index.dtype, slots.numel(), static_cast<int>(hkv),
@@ -255,6 +265,7 @@ long store_int4(PyObject* const* a) {
 long gather_int4(PyObject* const* a) {
     const at::Tensor &kc = cuda("k_cache", a[0]), &vc = cuda("v_cache", a[1]), &kp = cuda("k_params", a[2]), &vp = cuda("v_params", a[3]),
                      &cu = cuda("cu_seqlens_k", a[4]), &bt = cuda("block_tables", a[5]), &key = cuda("key", a[9]), &value = cuda("value", a[10]);
+    check_here({&kc, &vc, &kp, &vp, &cu, &bt, &key, &value});
     const int64_t hkv = integer(a[6]), d = integer(a[7]), bs = integer(a[8]);
     const Index starts("cu_seqlens_k", &cu), tables("block_tables", &bt);
     if (bs <= 0) raise(PyExc_ValueError, "%s", "block_size must be positive");
@@ -271,6 +282,7 @@ long gather_int4(PyObject* const* a) {
 
 // Sequences of a decode call: as many contexts, tables and outputs as queries.
 void check_rows(const Decode& x) {
+    check_here({&x.q, &x.kc, &x.vc, &x.ctx, &x.bt, &x.out});
     if (x.ctx.numel() != x.batch || x.bt.dim() != 2 || x.bt.size(0) != x.batch)
         raise(PyExc_ValueError, "%s", "context_lens and block_tables must have a row for every query");
     if (x.q.dim() != 3 || x.q.size(2) != x.d || !x.out.sizes().equals(x.q.sizes()) || x.out.scalar_type() != x.q.scalar_type())
@@ -283,6 +295,7 @@ long decode_int4(PyObject* const* a) {
     const at::Tensor &kp = cuda("k_params", a[3]), &vp = cuda("v_params", a[4]);
     const at::Tensor* ws = optional_cuda("workspace", a[12]);
     check_rows(x);
+    check_here({&kp, &vp, ws});
     const int64_t blocks = rows4(x.kc, x.vc, kp, vp, x.q.scalar_type(), x.hkv, x.d) / x.bs;
     launch(nvk_decode_attention_paged_int4, ptr(x.q), ptr(x.kc), ptr(x.vc), ptr(kp), ptr(vp), x.lens.p, x.lens.dtype, x.tables.p, x.tables.dtype, x.batch,
            x.max_blocks, blocks, static_cast<int>(x.heads), static_cast<int>(x.hkv), static_cast<int>(x.d), static_cast<int>(x.bs), x.scale, ptr(x.out),
@@ -305,6 +318,7 @@ long decode_weights(PyObject* const* a) {
     const at::Tensor &to = weights_of("new_key_weights", a[13], x.hkv), &ws = cuda("workspace", a[15]);
     const at::Tensor* from = a[11] == Py_None ? nullptr : &weights_of("key_weights", a[11], x.hkv);
     check_rows(x);
+    check_here({kp, vp, rows, &to, &ws, from});
     if (from != nullptr && !from->sizes().equals(to.sizes())) raise(PyExc_ValueError, "%s", "key_weights and new_key_weights must have the same shape");
     if (rows != nullptr && rows->numel() != x.batch) raise(PyExc_ValueError, "%s", "weight_rows must have an element for every query");
     if ((kp == nullptr) != (vp == nullptr)) raise(PyExc_ValueError, "%s", "k_params and v_params go together");
@@ -330,6 +344,7 @@ long evict(PyObject* const* a) {
     const at::Tensor *kp = optional_cuda("k_params", a[2]), *vp = optional_cuda("v_params", a[3]), *rows = optional_cuda("weight_rows", a[5]);
     const int64_t hkv = integer(a[11]), d = integer(a[12]), bs = integer(a[13]);
     const at::Tensor &from = weights_of("key_weights", a[4], hkv), &to = weights_of("new_key_weights", a[8], hkv);
+    check_here({&kc, &vc, kp, vp, &from, &to, rows, &ctx, &bt, &new_bt, &new_ctx});
     const Index lens("context_lens", &ctx), tables("block_tables", &bt), new_tables("new_block_tables", &new_bt), index("weight_rows", rows);
     if (!from.sizes().equals(to.sizes())) raise(PyExc_ValueError, "%s", "key_weights and new_key_weights must have the same shape");
     if ((kp == nullptr) != (vp == nullptr)) raise(PyExc_ValueError, "%s", "k_params and v_params go together");

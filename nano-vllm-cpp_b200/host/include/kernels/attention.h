@@ -1,6 +1,7 @@
 // Attention operators (signatures of include/kernels/attention.h:7-56 of the reference).
 #pragma once
 
+#include "utils/cuda_allocator.h"
 #include "utils/tensor.h"
 
 namespace nano_vllm {
@@ -39,6 +40,21 @@ void launch_decode_attention_paged_int8(const Tensor& query, const Tensor& k_cac
                                         const Tensor& k_scale, const Tensor& v_scale, const Tensor& context_lens,
                                         const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size,
                                         float scale, Tensor& output, cudaStream_t stream = nullptr);
+
+// Decode attention over a 4-bit cache (store_kvcache_int4); split-K scratch is taken from `allocator`.
+void launch_decode_attention_paged_int4(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                                        const Tensor& k_params, const Tensor& v_params, const Tensor& context_lens,
+                                        const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size,
+                                        float scale, Tensor& output, DeviceAllocator& allocator, cudaStream_t stream = nullptr);
+
+// Decode attention that adds every key's attention weights to new_key_weights = key_weights + .. (float32 [rows, Hkv, keys]; key_weights undefined: zeros, or
+// the same tensor).  Undefined k_params / v_params: a 16-bit cache; undefined weight_rows: sequence b has row b.
+void launch_decode_attention_paged_weights(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                                           const Tensor& k_params, const Tensor& v_params, const Tensor& context_lens,
+                                           const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size,
+                                           float scale, const Tensor& key_weights, const Tensor& weight_rows,
+                                           Tensor& new_key_weights, Tensor& output, DeviceAllocator& allocator,
+                                           cudaStream_t stream = nullptr);
 
 // The tensor-core prefill kernel bounds every internal wait; a launch whose wait ran out leaves rows unwritten and
 // records the fact on the device.  This call synchronises `stream`, and throws std::runtime_error if any prefill launch

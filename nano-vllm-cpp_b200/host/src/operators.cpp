@@ -169,6 +169,115 @@ void store_kvcache_int8(const Tensor& key, const Tensor& value, Tensor& k_cache,
                                                head_dim, rows, code(key.dtype()), stream));
 }
 
+// ---- 4-bit cache, eviction --------------------------------------------------------------------------
+namespace {
+
+// Caches and params of a 4-bit cache agree with one another and with `type`; its rows.
+int64_t int4_rows(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params, ScalarType type, int heads, int head_dim) {
+    ensure_cuda_tensor("k_cache", k_cache);
+    ensure_cuda_tensor("v_cache", v_cache);
+    ensure_cuda_tensor("k_params", k_params);
+    ensure_cuda_tensor("v_params", v_params);
+    ensure_same_device("k_cache", k_cache, "v_cache", v_cache);
+    ensure_same_device("k_cache", k_cache, "k_params", k_params);
+    ensure_same_device("k_cache", k_cache, "v_params", v_params);
+    if (k_cache.dtype() != ScalarType::kInt8 || v_cache.dtype() != ScalarType::kInt8)
+        throw std::invalid_argument("4-bit caches must be byte (int8) tensors");
+    if (type != ScalarType::kFloat16 && type != ScalarType::kBFloat16) throw std::invalid_argument("a 4-bit cache needs float16 or bfloat16");
+    if (k_params.dtype() != type || v_params.dtype() != type) throw std::invalid_argument("k_params and v_params must have the type of the keys");
+    if (head_dim != 128) throw std::invalid_argument("a 4-bit cache needs head_dim 128");
+    const int64_t row = static_cast<int64_t>(heads) * (head_dim / 2), rows = cache_rows_from_tensor("k_cache", k_cache, row);
+    if (cache_rows_from_tensor("v_cache", v_cache, row) != rows) throw std::invalid_argument("k_cache and v_cache must contain the same number of slots");
+    if (static_cast<int64_t>(k_params.numel()) != 2 * rows * heads || static_cast<int64_t>(v_params.numel()) != 2 * rows * heads)
+        throw std::invalid_argument("k_params and v_params must hold a pair per cache row and KV head");
+    return rows;
+}
+
+void ensure_rows(const char* name, const Tensor& t, int64_t rows) {
+    if (t.sizes().empty() || t.sizes()[0] != rows) throw std::invalid_argument(std::string(name) + " must have a row for every sequence");
+}
+
+}  // namespace
+
+void store_kvcache_int4(const Tensor& key, const Tensor& value, Tensor& k_cache, Tensor& v_cache, Tensor& k_params,
+                        Tensor& v_params, const Tensor& slot_mapping, cudaStream_t stream) {
+    ensure_cuda_tensor("key", key);
+    ensure_cuda_tensor("value", value);
+    ensure_same_dtype("key", key, "value", value);
+    ensure_same_shape("key", key, "value", value);
+    ensure_same_device("key", key, "value", value);
+    const IndexRef slots = index_data("slot_mapping", slot_mapping);
+    ensure_same_device("key", key, "slot_mapping", slot_mapping);
+    if (key.dim() != 3 || key.sizes()[0] != static_cast<int64_t>(slot_mapping.numel()))
+        throw std::invalid_argument("key must be [tokens, num_kv_heads, head_dim] with a slot for every token");
+    const int heads = static_cast<int>(key.sizes()[1]), head_dim = static_cast<int>(key.sizes()[2]);
+    const int64_t rows = int4_rows(k_cache, v_cache, k_params, v_params, key.dtype(), heads, head_dim);
+    ensure_same_device("key", key, "k_cache", k_cache);
+    throw_on_nvk_status(nvk_store_kvcache_int4(key.data(), value.data(), k_cache.data(), v_cache.data(), k_params.data(), v_params.data(), slots.ptr, slots.dtype,
+                                               key.sizes()[0], heads, head_dim, rows, code(key.dtype()), stream));
+}
+
+void gather_kvcache_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params,
+                         const Tensor& cu_seqlens_k, const Tensor& block_tables, int num_kv_heads, int head_dim,
+                         int block_size, Tensor& key, Tensor& value, cudaStream_t stream) {
+    ensure_cuda_tensor("key", key);
+    ensure_cuda_tensor("value", value);
+    ensure_same_dtype("key", key, "value", value);
+    ensure_same_shape("key", key, "value", value);
+    const IndexRef starts = index_data("cu_seqlens_k", cu_seqlens_k), tables = index_data("block_tables", block_tables);
+    const int64_t rows = int4_rows(k_cache, v_cache, k_params, v_params, key.dtype(), num_kv_heads, head_dim);
+    ensure_same_device("key", key, "k_cache", k_cache);
+    if (key.dim() != 3 || key.sizes()[1] != num_kv_heads || key.sizes()[2] != head_dim)
+        throw std::invalid_argument("key must be [total_k, num_kv_heads, head_dim]");
+    const int64_t seqs = static_cast<int64_t>(cu_seqlens_k.numel()) - 1;
+    if (block_tables.dim() != 2 || block_size <= 0) throw std::invalid_argument("block_tables must be [num_seqs, max_blocks], block_size positive");
+    ensure_rows("block_tables", block_tables, seqs);
+    throw_on_nvk_status(nvk_gather_kvcache_int4(k_cache.data(), v_cache.data(), k_params.data(), v_params.data(), starts.ptr, starts.dtype, tables.ptr,
+                                                tables.dtype, seqs, key.sizes()[0], block_tables.sizes()[1], rows / block_size, num_kv_heads, head_dim,
+                                                block_size, key.data(), value.data(), code(key.dtype()), stream));
+}
+
+void evict_kvcache(Tensor& k_cache, Tensor& v_cache, Tensor& k_params, Tensor& v_params, const Tensor& key_weights,
+                   const Tensor& weight_rows, const Tensor& context_lens, const Tensor& block_tables, Tensor& new_key_weights,
+                   const Tensor& new_block_tables, Tensor& new_context_lens, int num_kv_heads, int head_dim, int block_size,
+                   int64_t budget, int64_t sinks, int64_t recent, cudaStream_t stream) {
+    const bool four = k_params.defined() || v_params.defined();
+    if (num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0) throw std::invalid_argument("attention dimensions must be positive");
+    int64_t blocks = 0;
+    if (four) {
+        blocks = int4_rows(k_cache, v_cache, k_params, v_params, k_params.defined() ? k_params.dtype() : v_params.dtype(), num_kv_heads, head_dim) / block_size;
+    } else {
+        ensure_cuda_tensor("k_cache", k_cache);
+        ensure_cuda_tensor("v_cache", v_cache);
+        ensure_same_dtype("k_cache", k_cache, "v_cache", v_cache);
+        if (k_cache.numel() != v_cache.numel()) throw std::invalid_argument("k_cache and v_cache must contain the same number of slots");
+        blocks = cache_blocks(k_cache, block_size, num_kv_heads, head_dim);
+    }
+    ensure_cuda_tensor("key_weights", key_weights);
+    ensure_cuda_tensor("new_key_weights", new_key_weights);
+    ensure_same_shape("key_weights", key_weights, "new_key_weights", new_key_weights);
+    if (key_weights.dtype() != ScalarType::kFloat32 || new_key_weights.dtype() != ScalarType::kFloat32 || key_weights.dim() != 3 ||
+        key_weights.sizes()[1] != num_kv_heads)
+        throw std::invalid_argument("key_weights and new_key_weights must be float32 [rows, num_kv_heads, keys]");
+    const IndexRef lens = index_data("context_lens", context_lens), tables = index_data("block_tables", block_tables),
+                   new_tables = index_data("new_block_tables", new_block_tables), new_lens = index_data("new_context_lens", new_context_lens);
+    const IndexRef rows = weight_rows.defined() ? index_data("weight_rows", weight_rows) : IndexRef{nullptr, NVK_I32};
+    const int64_t batch = static_cast<int64_t>(context_lens.numel());
+    if (new_lens.dtype != lens.dtype || static_cast<int64_t>(new_context_lens.numel()) != batch)
+        throw std::invalid_argument("new_context_lens must be like context_lens");
+    if (block_tables.dim() != 2 || new_block_tables.dim() != 2) throw std::invalid_argument("block tables must be [batch, max_blocks]");
+    ensure_rows("block_tables", block_tables, batch);
+    ensure_rows("new_block_tables", new_block_tables, batch);
+    if (weight_rows.defined()) ensure_rows("weight_rows", weight_rows, batch);
+    for (const Tensor* t : {&key_weights, static_cast<const Tensor*>(&new_key_weights), &context_lens, &block_tables, &new_block_tables})
+        ensure_same_device("k_cache", k_cache, "every other tensor", *t);
+    throw_on_nvk_status(nvk_evict_kvcache(k_cache.data(), v_cache.data(), four ? k_params.data() : nullptr, four ? v_params.data() : nullptr,
+                                          key_weights.data_as<float>(), rows.ptr, rows.dtype, key_weights.sizes()[0], key_weights.sizes()[2], lens.ptr,
+                                          lens.dtype, tables.ptr, tables.dtype, batch, block_tables.sizes()[1], blocks, new_key_weights.data_as<float>(),
+                                          new_tables.ptr, new_tables.dtype, new_block_tables.sizes()[1], new_context_lens.data(), num_kv_heads, head_dim,
+                                          block_size, budget, sinks, recent, code(four ? k_params.dtype() : k_cache.dtype()), stream));
+}
+
 // ---- fused decode prologue ---------------------------------------------------------------------------
 void fused_split_norm_rope_store(const Tensor& qkv, const Tensor& positions, const Tensor& q_norm_weight,
                                  const Tensor& k_norm_weight, float norm_eps, const Tensor& cos_sin_cache,
@@ -287,6 +396,84 @@ void launch_decode_attention_paged_int8(const Tensor& query, const Tensor& k_cac
     throw_on_nvk_status(nvk_decode_attention_paged_int8(
         query.data(), k_cache.data(), v_cache.data(), k_scale.data(), v_scale.data(), lens.ptr, lens.dtype, tables.ptr,
         tables.dtype, batch, max_blocks, blocks, heads, num_kv_heads, head_dim, block_size, scale, output.data(), code(query.dtype()), nullptr, 0, stream));
+}
+
+namespace {
+
+// The tensors that a decode step over a 16-bit or 4-bit cache has.
+struct Step {
+    IndexRef lens, tables;
+    int64_t batch, max_blocks, blocks;
+    int heads;
+    Step(const Tensor& query, const Tensor& output, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params, bool four,
+         const Tensor& context_lens, const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size)
+        : lens(index_data("context_lens", context_lens)), tables(index_data("block_tables", block_tables)) {
+        check_qo(query, output);
+        if (num_kv_heads <= 0 || head_dim <= 0 || block_size <= 0) throw std::invalid_argument("attention dimensions must be positive");
+        batch = query.sizes()[0];
+        heads = static_cast<int>(query.sizes()[1]);
+        if (query.sizes()[2] != head_dim) throw std::invalid_argument("query head_dim does not match head_dim");
+        if (block_tables.dim() != 2) throw std::invalid_argument("block_tables must be [batch, max_blocks]");
+        ensure_rows("block_tables", block_tables, batch);
+        if (static_cast<int64_t>(context_lens.numel()) != batch) throw std::invalid_argument("context_lens must hold one entry per sequence");
+        max_blocks = block_tables.sizes()[1];
+        if (four) {
+            blocks = int4_rows(k_cache, v_cache, k_params, v_params, query.dtype(), num_kv_heads, head_dim) / block_size;
+        } else {
+            ensure_cuda_tensor("k_cache", k_cache);
+            ensure_cuda_tensor("v_cache", v_cache);
+            ensure_same_dtype("query", query, "k_cache", k_cache);
+            ensure_same_dtype("query", query, "v_cache", v_cache);
+            if (k_cache.numel() != v_cache.numel()) throw std::invalid_argument("k_cache and v_cache must contain the same number of slots");
+            blocks = cache_blocks(k_cache, block_size, num_kv_heads, head_dim);
+        }
+        ensure_same_device("query", query, "k_cache", k_cache);
+        ensure_same_device("query", query, "context_lens", context_lens);
+        ensure_same_device("query", query, "block_tables", block_tables);
+    }
+};
+
+}  // namespace
+
+void launch_decode_attention_paged_int4(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                                        const Tensor& k_params, const Tensor& v_params, const Tensor& context_lens,
+                                        const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size,
+                                        float scale, Tensor& output, DeviceAllocator& allocator, cudaStream_t stream) {
+    const Step s(query, output, k_cache, v_cache, k_params, v_params, true, context_lens, block_tables, num_kv_heads, head_dim, block_size);
+    const size_t need = nvk::decode_mma_workspace_needed(s.batch, s.heads, num_kv_heads, head_dim, s.max_blocks, block_size);
+    Memory::Ptr scratch = need > 0 ? allocator.allocate(need, query.device()) : nullptr;
+    throw_on_nvk_status(nvk_decode_attention_paged_int4(query.data(), k_cache.data(), v_cache.data(), k_params.data(), v_params.data(), s.lens.ptr, s.lens.dtype,
+                                                        s.tables.ptr, s.tables.dtype, s.batch, s.max_blocks, s.blocks, s.heads, num_kv_heads, head_dim,
+                                                        block_size, scale, output.data(), code(query.dtype()), scratch ? scratch->data() : nullptr, need, stream));
+}
+
+void launch_decode_attention_paged_weights(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                                           const Tensor& k_params, const Tensor& v_params, const Tensor& context_lens,
+                                           const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size,
+                                           float scale, const Tensor& key_weights, const Tensor& weight_rows,
+                                           Tensor& new_key_weights, Tensor& output, DeviceAllocator& allocator,
+                                           cudaStream_t stream) {
+    const bool four = k_params.defined() || v_params.defined();
+    const Step s(query, output, k_cache, v_cache, k_params, v_params, four, context_lens, block_tables, num_kv_heads, head_dim, block_size);
+    ensure_cuda_tensor("new_key_weights", new_key_weights);
+    if (new_key_weights.dtype() != ScalarType::kFloat32 || new_key_weights.dim() != 3 || new_key_weights.sizes()[1] != num_kv_heads)
+        throw std::invalid_argument("new_key_weights must be float32 [rows, num_kv_heads, keys]");
+    if (key_weights.defined()) {
+        ensure_cuda_tensor("key_weights", key_weights);
+        ensure_same_dtype("key_weights", key_weights, "new_key_weights", new_key_weights);
+        ensure_same_shape("key_weights", key_weights, "new_key_weights", new_key_weights);
+        ensure_same_device("query", query, "key_weights", key_weights);
+    }
+    ensure_same_device("query", query, "new_key_weights", new_key_weights);
+    const IndexRef rows = weight_rows.defined() ? index_data("weight_rows", weight_rows) : IndexRef{nullptr, NVK_I32};
+    if (weight_rows.defined()) ensure_rows("weight_rows", weight_rows, s.batch);
+    const size_t need = nvk_decode_attention_weights_workspace_bytes(s.batch, s.heads, num_kv_heads, head_dim, s.max_blocks, block_size);
+    Memory::Ptr scratch = need > 0 ? allocator.allocate(need, query.device()) : nullptr;
+    throw_on_nvk_status(nvk_decode_attention_paged_weights(
+        query.data(), k_cache.data(), v_cache.data(), four ? k_params.data() : nullptr, four ? v_params.data() : nullptr, s.lens.ptr, s.lens.dtype, s.tables.ptr,
+        s.tables.dtype, s.batch, s.max_blocks, s.blocks, s.heads, num_kv_heads, head_dim, block_size, scale,
+        key_weights.defined() ? key_weights.data_as<float>() : nullptr, rows.ptr, rows.dtype, new_key_weights.sizes()[0], new_key_weights.sizes()[2],
+        new_key_weights.data_as<float>(), output.data(), code(query.dtype()), scratch ? scratch->data() : nullptr, need, stream));
 }
 
 // ---- prefill ------------------------------------------------------------------------------------------

@@ -73,7 +73,7 @@ TransformerAttention::TransformerAttention(int num_heads, int num_kv_heads, int 
 
 bool TransformerAttention::fused_eligible(const Tensor& qkv) const {
     const Context& ctx = get_context();
-    return !ctx.is_prefill && !attn_.is_int8() && has_qk_norm() && ctx.slot_mapping.defined() && is_half_type(qkv.dtype());
+    return !ctx.is_prefill && !attn_.is_quantised() && has_qk_norm() && ctx.slot_mapping.defined() && is_half_type(qkv.dtype());
 }
 
 Tensor TransformerAttention::forward(const Tensor& positions, const Tensor& qkv, DeviceAllocator& allocator,
