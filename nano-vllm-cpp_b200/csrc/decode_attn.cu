@@ -38,13 +38,13 @@ constexpr int kClusterTokens = 512;
 constexpr int kMaxSorted = 512;
 constexpr int kMinSortedTokens = 1024;   // tables of fewer keys: a block lasts hardly longer than the 1 us that this takes
 struct SortScratch { int count[128]; unsigned char cls[kMaxSorted]; };
-__device__ __forceinline__ int sequence_of_rank(const DecodeParams& p, int rank, SortScratch& sm) {
-    static_assert(kGroupThreads == 128, "one thread per class");
+template <int THREADS> __device__ __forceinline__ int sequence_of_rank(const DecodeParams& p, int rank, SortScratch& sm) {
+    static_assert(THREADS >= 128, "a thread per class");
     const int tid = threadIdx.x, lane = tid & 31;
     const int shift = max(0, 25 - __clz(static_cast<int>(p.max_blocks * p.block_size)));   // the longest context there can be is in class 127 at most
-    sm.count[tid] = 0;
+    if (tid < 128) sm.count[tid] = 0;
     __syncthreads();
-    for (int i = tid; i < p.batch; i += kGroupThreads) {
+    for (int i = tid; i < p.batch; i += THREADS) {
         const int c = 127 - (clamped_context(p, i) >> shift);
         sm.cls[i] = static_cast<unsigned char>(c);
         atomicAdd(&sm.count[c], 1);
@@ -87,12 +87,12 @@ __device__ __forceinline__ void st_cluster2(uint32_t addr, uint32_t rank, float 
 }
 
 template <class F, typename T>
-__global__ void __launch_bounds__(kGroupThreads, F::kSplitBlocks) decode_split_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(F::kWarps * 32, F::kSplitBlocks) decode_split_kernel(const __grid_constant__ DecodeParams p) {
     extern __shared__ __align__(128) unsigned char smem[];
     if (p.beside) pdl_start_beside();
     else pdl_wait_then_release();
     const int rank = p.chunk_major ? blockIdx.y : blockIdx.z, split = p.chunk_major ? blockIdx.z : blockIdx.y;
-    const int b = p.longest_first ? sequence_of_rank(p, rank, *reinterpret_cast<SortScratch*>(smem)) : rank;
+    const int b = p.longest_first ? sequence_of_rank<F::kWarps * 32>(p, rank, *reinterpret_cast<SortScratch*>(smem)) : rank;
     if (p.longest_first) __syncthreads();   // (the ring takes the scratch's place)
     if constexpr (F::kScores) {
         __shared__ float2 s_heads[kMaxGroup];
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kGroupThreads, F::kGroups) decode_cluster_kern
                 s_heads[tid] = make_float2(m, 1.0f / l);
             }
             __syncthreads();
-            if (t0 < t1) add_key_weights(p, b, kvh, t0, t1, s_heads, tid);
+            if (t0 < t1) add_key_weights<kGroupThreads>(p, b, kvh, t0, t1, s_heads, tid);
         }
     }
     if (p.beside) pdl_wait_beside();
@@ -340,12 +340,17 @@ size_t part_bytes(size_t parts, int group) { return parts * group * (kHeadDim * 
 size_t part_count(const Splits& s, int64_t batch, int num_kv_heads) {   // (the cluster kernel itself needs none: the mixed step does)
     return s.count > 1 ? static_cast<size_t>(batch) * num_kv_heads * s.count : 0;
 }
-// 4-bit caches are shared out like 8-bit ones (a key costs as much arithmetic, and that is what bounds both), but for what four blocks to an SM and a block's
-// fixed part, five tiles' worth, change: whole contexts up to 2048 keys from 250 pairs on, up to 4096 at a time beyond three waves' worth of SMs, the
-// longest first.  us, spread from 0.05 / 0.5: 320 pairs of 2048 keys 25.6 / 27.8 -> 22.7 / 25.2, 512 of 8192 76.0 / 99.0 -> 72.7 / 91.7, 1600 of 8192
-// 208 / 299 -> 207 / 271; but 200 of 2048 17.2 / 22.8, whole 19.2 / 21.5, and 320 of 8192 54.1 / 70.3, by 4096 60.5 / 68.5.
+// 4-bit caches are shared out like 8-bit ones (a key costs as much arithmetic, and that is what bounds both), but for what more warps to an SM and a block's
+// fixed part, five tiles' worth, change.  us, spread from 0.05 / 0.5 to all of the table:
+//   * tables of 1536 to 2048 keys beyond the clusters of four, up to 320 pairs: whole contexts by blocks of eight warps, with more pairs than SMs the longest first
+//     (120 pairs of 2048 14.9 / 16.4 -> 12.6 / 12.8, 160 16.1 / 17.9 -> 14.4 / 17.9, 256 21.2 / 21.6 -> 18.5 / 20.9, 320 24.9 / 26.7 -> 21.3 / 26.8);
+//   * tables of 768 to 2048 keys, 250 pairs and more: whole contexts (320 pairs of 2048 by four warps 25.6 / 27.8 -> 22.7 / 25.2);
+//   * tables of 4096 to 8192 keys beyond three waves' worth of SMs: 4096 keys at a time, the longest first (512 of 8192 76.0 / 99.0 -> 72.7 / 91.7, 1600
+//     208 / 299 -> 207 / 271; but 320 54.1 / 70.3 -> 60.5 / 68.5).
+// Whole contexts of 4096 keys by eight warps gain 7 to 12 % over even spreads of 256 to 320 pairs, but leave one long context to a block for twice as long.
+bool eight_warps(int64_t pairs, int64_t max_tokens) { return max_tokens > 1536 && max_tokens <= 2048 && pairs <= 320; }
 int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
-    if (max_tokens <= 2048) return max_tokens > 768 && pairs >= 250 ? static_cast<int>(max_tokens) : 0;
+    if (max_tokens <= 2048) return (max_tokens > 768 && pairs >= 250) || eight_warps(pairs, max_tokens) ? static_cast<int>(max_tokens) : 0;
     return max_tokens > 4096 && max_tokens <= 8192 && pairs >= 3 * kSmCount ? 4096 : 0;
 }
 Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size, int groups, bool have_workspace, bool four_bits = false) {
@@ -399,7 +404,8 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     p.num_splits = s.count;
     // More than one wave of blocks: the long contexts first, so that the last blocks to start are short.  Contexts in a few chunks as well:
     // 38 / 44 sequences of 500 / 2000 to 4096 keys, 8 KV heads, 65.4 / 90.1 -> 58.7 / 85.9 us a call (whole 59.8 / 84.7).
-    p.longest_first = s.chunk > 0 && (s.count == 1 || a.max_blocks * a.block_size <= 4096 || (four_bits && s.chunk >= 4096)) && a.batch * a.num_kv_heads > static_cast<int64_t>(kSmCount) * groups &&
+    p.longest_first = s.chunk > 0 && (s.count == 1 || a.max_blocks * a.block_size <= 4096 || (four_bits && s.chunk >= 4096)) &&
+                      a.batch * a.num_kv_heads > static_cast<int64_t>(kSmCount) * (four_bits && eight_warps(a.batch * a.num_kv_heads, a.max_blocks * a.block_size) ? 1 : groups) &&
                       a.batch <= kMaxSorted && a.max_blocks * a.block_size >= kMinSortedTokens;
     // Contexts shorter than the table leave chunks without keys, whose blocks exit at once.  With sequence after sequence they lie between
     // the blocks with work, and these pile up on the SMs where the empty ones were quickest gone; chunk after chunk the ones with
@@ -450,6 +456,10 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     if (device >= 0 && device < 64 && !attr_done[device]) {
         cudaError_t e = cudaFuncSetAttribute(decode_split_kernel<F, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_cluster_kernel<F, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if constexpr (F::kFourBits) {
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(decode_split_kernel<typename F::Eight, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(GroupSmem<typename F::Eight>));
+        }
         if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "decode attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
         attr_done[device] = true;
     }
@@ -484,7 +494,13 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     if (const int rc1 = check_grid(a, p); rc1 != NVK_OK) return rc1;
     const unsigned batch = static_cast<unsigned>(a.batch), splits = static_cast<unsigned>(p.num_splits);
     const dim3 grid = p.chunk_major ? dim3(a.num_kv_heads, batch, splits) : dim3(a.num_kv_heads, splits, batch);
-    const cudaError_t e = launch_pdl(decode_split_kernel<F, T>, grid, dim3(kGroupThreads), kSmem, a.stream, p);
+    cudaError_t e = cudaSuccess;
+    bool eight = false;
+    if constexpr (F::kFourBits) {
+        eight = splits == 1 && eight_warps(a.batch * a.num_kv_heads, a.max_blocks * a.block_size);
+        if (eight) e = launch_pdl(decode_split_kernel<typename F::Eight, T>, grid, dim3(F::Eight::kWarps * 32), sizeof(GroupSmem<typename F::Eight>), a.stream, p);
+    }
+    if (!eight) e = launch_pdl(decode_split_kernel<F, T>, grid, dim3(kGroupThreads), kSmem, a.stream, p);
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "decode_split_kernel launch: %s", cudaGetErrorString(e));
     const int rc2 = check_launch("decode_split_kernel launch");
     return rc2 != NVK_OK ? rc2 : launch_merge_typed<T>(p, a.stream);

@@ -1,7 +1,7 @@
 // Device code of paged decode attention on tensor cores (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 or 4-bit cache), shared
 // by the decode kernels (decode_attn.cu) and the mixed prefill + decode kernel (prefill_attn_tc.cu).
 //
-// The op is HBM-bound: every K and V row of every context is read once.  A group of four warps takes a range of the keys of one
+// The op is HBM-bound: every K and V row of every context is read once.  A group of four warps (over a 4-bit cache also of eight) takes a range of the keys of one
 // (sequence, KV head); the G = Hq / Hkv <= 8 query heads of the KV head are the columns of the MMA tile, so a K / V row is read once
 // per KV head.  Each warp streams every fourth tile of 16 keys through a private ring of cp.async stages (no barrier in the main
 // loop); at the end the four warps merge through shared memory.
@@ -152,10 +152,10 @@ struct ScoreOut {
         put16(sc, 0, valid, lane, p.group);
         at += kGroupWarps * 16 * p.group;
     }
-    __device__ __forceinline__ void put(const DecodeParams& p, const float (&sa)[4], const float (&sb)[4], int valid, int lane) {   // of 32
+    __device__ __forceinline__ void put(const DecodeParams& p, const float (&sa)[4], const float (&sb)[4], int valid, int lane, int warps) {   // of 32
         put16(sa, 0, valid, lane, p.group);
         put16(sb, 16, valid, lane, p.group);
-        at += kGroupWarps * 32 * p.group;
+        at += warps * 32 * p.group;
     }
 };
 
@@ -169,6 +169,7 @@ template <typename T, bool SCORES = false>
 struct Cache16 {
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = false;
+    static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 2;   // resident per SM
     static constexpr int kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim * 2;
@@ -288,6 +289,7 @@ template <typename T, bool FP8>
 struct Cache8 {
     static constexpr bool kScores = false;
     static constexpr bool kFourBits = false;
+    static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 3, kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim;
     static constexpr int kTileBytes = kTileTokens * kRowBytes;
@@ -441,12 +443,14 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }   // -126 <= e <= 127
 
-template <typename T, bool SCORES = false>
+template <typename T, bool SCORES = false, int WARPS = kGroupWarps>
 struct Cache4 {
+    using Eight = Cache4<T, SCORES, 8>;                       // eight warps to a block
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = true;
+    static constexpr int kWarps = WARPS;
     static constexpr int kGroups = 3;                         // resident per SM, by which a step is shared out, as with the 8-bit caches
-    static constexpr int kSplitBlocks = 4;                    // in chunks: the registers are there, and the chains are what a warp waits for
+    static constexpr int kSplitBlocks = 16 / WARPS;           // in chunks: the registers are there, and the chains are what a warp waits for
     static constexpr int kRowBytes = kHeadDim / 2;
     static constexpr int kKeys = 32;                          // of a stage
     static constexpr int kTileBytes = kKeys * kRowBytes;
@@ -596,7 +600,7 @@ struct Cache4 {
             mask_scores(sa, lane >> 2, valid);
             mask_scores(sb, lane >> 2, valid - 16);
         }
-        if constexpr (SCORES) kept.put(p, sa, sb, valid, lane);
+        if constexpr (SCORES) kept.put(p, sa, sb, valid, lane, WARPS);
         const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
         const float top_step = fmaxf(fmaxf(fabsf(va[0].x), fabsf(va[1].x)), fmaxf(fabsf(vb[0].x), fabsf(vb[1].x)));
         if (__any_sync(0xffffffffu, top0 > s.m[0] || top1 > s.m[1] || top_step * v_down >= 2.0f)) raise(top0, top1, top_step);
@@ -615,11 +619,11 @@ struct Cache4 {
         return reinterpret_cast<const void*>(at);
     }
 
-    // Keys [t0, t1): this warp's tiles of 32, every fourth one.
+    // Keys [t0, t1): this warp's tiles of 32, every WARPS-th one.
     __device__ __forceinline__ void run(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, uint32_t ring, int warp, int lane) {
-        const int tiles = (t1 - t0 + kKeys - 1) / kKeys, mine = tiles > warp ? (tiles - warp + kGroupWarps - 1) / kGroupWarps : 0;
+        const int tiles = (t1 - t0 + kKeys - 1) / kKeys, mine = tiles > warp ? (tiles - warp + WARPS - 1) / WARPS : 0;
         const int bs = p.block_size, first = t0 + warp * kKeys;
-        constexpr int kStride = kGroupWarps * kKeys;
+        constexpr int kStride = WARPS * kKeys;
         // Lane 2i + h: half h of tile i of a window of 16 tiles, the place of its first row among all head vectors of the cache.
         auto token_of = [&](int window) { return first + (window * 16 + (lane >> 1)) * kStride + (lane & 1) * 16; };
         auto load = [&](int window) {
@@ -730,7 +734,7 @@ struct alignas(128) GroupSmem {
             float o[kMaxGroup * F::kPartStride];       // head 2 t + h in row 4 h + t: the lanes of a store hit different banks
             float2 ml[kMaxGroup];
         } part;
-    } warps[kGroupWarps];
+    } warps[F::kWarps];
 };
 
 // The warp's tiles of keys [t0, t1), every fourth one, through its ring.
@@ -813,12 +817,12 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
             st.write_part(part.o + (4 * h + t) * F::kPartStride, h, g);
         }
     }
-    group_sync(bar_id, kGroupThreads);
-    for (int h = warp; h < p.group; h += kGroupWarps) {
-        float4 o[kGroupWarps];
-        float2 ml[kGroupWarps];
+    group_sync(bar_id, F::kWarps * 32);
+    for (int h = warp; h < p.group; h += F::kWarps) {
+        float4 o[F::kWarps];
+        float2 ml[F::kWarps];
 #pragma unroll
-        for (int w = 0; w < kGroupWarps; ++w) {
+        for (int w = 0; w < F::kWarps; ++w) {
             const auto& from = sm.warps[w].part;
             ml[w] = from.ml[h];
             o[w] = *reinterpret_cast<const float4*>(from.o + (4 * (h & 1) + (h >> 1)) * F::kPartStride + 4 * lane);
@@ -826,9 +830,9 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
         float mx = ml[0].x, sum = 0.0f;
         float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 1; w < kGroupWarps; ++w) mx = fmaxf(mx, ml[w].x);
+        for (int w = 1; w < F::kWarps; ++w) mx = fmaxf(mx, ml[w].x);
 #pragma unroll
-        for (int w = 0; w < kGroupWarps; ++w) {
+        for (int w = 0; w < F::kWarps; ++w) {
             const float f = fast_exp2(ml[w].x - mx);   // 0 for a warp without a tile
             total.x = fmaf(f, o[w].x, total.x); total.y = fmaf(f, o[w].y, total.y); total.z = fmaf(f, o[w].z, total.z); total.w = fmaf(f, o[w].w, total.w);
             sum = fmaf(f, ml[w].y, sum);
@@ -844,6 +848,7 @@ __device__ __forceinline__ float4 scaled(const float4& v, float f) { return make
 
 // Keys [t0, t1) of (b, kvh): new = old + sum over the heads of exp2(score - M) / L, with (M, 1 / L) of the whole context in `ml`.  By the block that has these keys'
 // scores, which come back from L2: a kernel of its own after it took 9 us of 105 for 64 sequences of 500 to 4096 keys, 32 / 8 heads.
+template <int THREADS>
 __device__ __forceinline__ void add_key_weights(const DecodeParams& p, int b, int kvh, int t0, int t1, const float2* ml, int tid) {
     const KeyWeights& w = p.weights;
     const int64_t row = w.rows != nullptr ? w.rows[b] : b;
@@ -856,11 +861,11 @@ __device__ __forceinline__ void add_key_weights(const DecodeParams& p, int b, in
     for (int h = 0; h < kMaxGroup; ++h) heads[h] = h < group ? ml[h] : make_float2(0.0f, 0.0f);
     constexpr int kAhead = 4;
     auto trip = [&](auto load, auto count) {   // `count` heads of a key by load(key, to)
-        for (int k0 = t0 + tid; k0 < t1; k0 += kAhead * kGroupThreads) {
+        for (int k0 = t0 + tid; k0 < t1; k0 += kAhead * THREADS) {
             float sc[kAhead][count.value], old[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i) {
-                const int k = min(k0 + i * kGroupThreads, t1 - 1);
+                const int k = min(k0 + i * THREADS, t1 - 1);
                 load(scores + static_cast<int64_t>(k) * group, sc[i]);
                 old[i] = w.old_weights != nullptr ? w.old_weights[at + k] : 0.0f;
             }
@@ -870,7 +875,7 @@ __device__ __forceinline__ void add_key_weights(const DecodeParams& p, int b, in
 #pragma unroll
                 for (int h = 0; h < count.value; ++h)
                     if (h < group) sum = fmaf(fast_exp2(sc[i][h] - heads[h].x), heads[h].y, sum);
-                if (k0 + i * kGroupThreads < t1) w.new_weights[at + k0 + i * kGroupThreads] = old[i] + sum;
+                if (k0 + i * THREADS < t1) w.new_weights[at + k0 + i * THREADS] = old[i] + sum;
             }
         }
     };
@@ -914,7 +919,7 @@ __device__ __forceinline__ void run_split(const DecodeParams& p, int b, int kvh,
     T* out = static_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.num_heads + kvh * p.group) * kHeadDim;
     if (t0 >= t1) {
         if (ctx == 0 && split == 0) {
-            for (int i = tid; i < p.group * kHeadDim; i += kGroupThreads) out[i] = ElemTraits<T>::from_float(0.0f);
+            for (int i = tid; i < p.group * kHeadDim; i += F::kWarps * 32) out[i] = ElemTraits<T>::from_float(0.0f);
         }
         return;
     }
@@ -933,8 +938,8 @@ __device__ __forceinline__ void run_split(const DecodeParams& p, int b, int kvh,
     });
     if constexpr (F::kScores) {
         if (p.num_splits == 1) {
-            group_sync(bar_id, kGroupThreads);
-            add_key_weights(p, b, kvh, t0, t1, heads, tid);
+            group_sync(bar_id, F::kWarps * 32);
+            add_key_weights<F::kWarps * 32>(p, b, kvh, t0, t1, heads, tid);
         }
     }
 }

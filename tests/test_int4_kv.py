@@ -328,3 +328,35 @@ def test_wrong_tensors_are_refused():
         with pytest.raises(ValueError):
             lib.launch_decode_attention_paged_int4(*a.values())
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,longest", [(120, 2000), (200, 2048), (300, 1700), (460, 900), (60, 8000)])
+def test_decode_of_many_contexts_however_they_are_shared_out(batch, longest):
+    """Blocks of four and of eight warps, whole contexts in order of length, long chunks: what comes out is within the roundings of what single calls give, and
+    the same in a second run."""
+    import torch
+    rng = np.random.default_rng(batch)
+    bs, dtype = 256, "bfloat16"
+    hkv = 8 if longest > 4096 else 1
+    hq = 4 * hkv
+    lens = [1 + (i * 7919) % longest for i in range(batch)]
+    lens[batch // 2] = longest
+    width = -(-longest // bs)
+    blocks = 40
+    (kc, kp, _, _), (vc, vp, vv, spread) = _cache(rng, blocks * bs, hkv, dtype)
+    tables = np.stack([rng.permutation(blocks)[:width] for _ in range(batch)])         # (contexts may share blocks)
+    q = _dev(_typed(rng, (batch, hq, D), dtype), dtype)
+    lib, dt = nvk(), torch.int32
+    ctx, bt = to_dev(np.array(lens), dt), to_dev(tables, dt)
+    ws = torch.empty(max(16, lib.decode_attention_workspace_bytes(batch, hq, hkv, D, width, bs)), dtype=torch.uint8, device="cuda")
+    out, again, single = (torch.full_like(q, float("nan")) for _ in range(3))
+    for to in (out, again):
+        lib.launch_decode_attention_paged_int4(q, kc, vc, kp, vp, ctx, bt, hkv, D, bs, 0.088, to, ws)
+    for i in range(0, batch, 37):
+        lib.launch_decode_attention_paged_int4(q[i:i + 1], kc, vc, kp, vp, ctx[i:i + 1], bt[i:i + 1], hkv, D, bs, 0.088, single[i:i + 1])
+    torch.cuda.synchronize()
+    assert torch.equal(out, again) and not torch.isnan(out).any()
+    # both round p' to f16 (2^-11 of at most 15 steps each way) and the result to bf16 (half a step each)
+    most = 2 * 2.0 ** -11 * 15 * float(spread.max()) / 7.5 + 2 * 2.0 ** -8 * float(np.abs(vv).max())
+    assert (single[::37].float() - out[::37].float()).abs().max().item() <= most
