@@ -333,7 +333,7 @@ long decode_weights(PyObject* const* a) {
            x.max_blocks, blocks, static_cast<int>(x.heads), static_cast<int>(x.hkv), static_cast<int>(x.d), static_cast<int>(x.bs), x.scale,
            static_cast<const float*>(ptr(from)), index.p, index.dtype, to.size(0), to.size(2), static_cast<float*>(ptr(to)), ptr(x.out), code(x.q), ptr(ws),
            ws.nbytes(), stream());
-    return x.launches(&ws) + 1;
+    return x.launches(&ws);
 }
 
 // (k_cache, v_cache, k_params, v_params, key_weights, weight_rows, context_lens, block_tables, new_key_weights, new_block_tables, new_context_lens,
