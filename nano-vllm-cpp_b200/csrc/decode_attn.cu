@@ -537,7 +537,7 @@ size_t decode_mma_workspace_needed(int64_t batch, int num_heads, int num_kv_head
     if (batch <= 0 || num_heads <= 0 || num_kv_heads <= 0 || max_blocks <= 0 || block_size <= 0) return 0;
     size_t need = chunk_scratch_bytes(batch, num_heads, num_kv_heads, head_dim, max_blocks, block_size);
     const struct { int groups; bool four_bits; } formats[] = {{Cache16<__half>::kGroups, false}, {Cache8<__half, false>::kGroups, false}, {Cache4<__half>::kGroups, true}};
-    for (const auto& f : formats) {   // (the third has never needed more than the second: tables of up to 12288 keys, up to 4096 sequences)
+    for (const auto& f : formats) {   // (the third has not needed more than the others in any size tried: tables of up to 131072 keys, up to 4096 sequences)
         const Splits s = choose_splits(batch, num_heads, num_kv_heads, max_blocks, block_size, f.groups, true, f.four_bits);
         const size_t n = part_bytes(part_count(s, batch, num_kv_heads), (num_heads + num_kv_heads - 1) / num_kv_heads);
         if (n > need) need = n;

@@ -50,6 +50,11 @@ bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
     const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
     return x < y + b_bytes && y < x + a_bytes;
 }
+// Two arrays of `rows` x `heads` x `keys` weights that are neither the same nor apart.
+bool weights_overlap(const float* old_weights, const float* new_weights, int64_t rows, int heads, int64_t keys) {
+    const int64_t bytes = rows * heads * keys * static_cast<int64_t>(sizeof(float));
+    return old_weights != nullptr && old_weights != new_weights && overlap(old_weights, bytes, new_weights, bytes);
+}
 int64_t index_bytes(int dtype) { return dtype == NVK_I64 ? 8 : 4; }
 
 int launch_prefill(const PrefillArgs& a) {
@@ -337,6 +342,8 @@ int nvk_decode_attention_paged_weights(const void* query, const void* k_cache, c
                                          "multiple of 16; caches (4-bit ones: query too) 16-byte aligned, params 4-byte and output 8-byte aligned");
     if (!aligned_to(key_weights, 4) || !aligned_to(new_key_weights, 4))
         return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): weights must be 4-byte aligned");
+    if (weights_overlap(key_weights, new_key_weights, num_weight_rows, num_kv_heads, weight_row_keys))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): new_key_weights must be key_weights or not overlap with it");
     const size_t need = decode_weights_workspace_bytes(batch, num_heads, num_kv_heads, max_blocks, block_size);
     if (workspace == nullptr || workspace_bytes < need || !aligned_to(workspace, 16))
         return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (weights): a 16-byte aligned workspace of %zu bytes is needed "
@@ -374,6 +381,8 @@ int nvk_evict_kvcache(void* k_cache, void* v_cache, void* k_params, void* v_para
     if (batch == 0) return NVK_OK;
     if (overlap(new_context_lens, batch * index_bytes(context_lens_dtype), context_lens, batch * index_bytes(context_lens_dtype)))
         return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: new_context_lens must not be context_lens");
+    if (weights_overlap(key_weights, new_key_weights, num_weight_rows, num_kv_heads, weight_row_keys))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "evict_kvcache: new_key_weights must be key_weights or not overlap with it");
     return launch_evict(EvictArgs{k_cache, v_cache, k_params, v_params, key_weights, new_key_weights, index_array(weight_rows, weight_rows_dtype),
                                   index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype),
                                   index_array(new_block_tables, new_block_tables_dtype), new_context_lens, batch, num_weight_rows, weight_row_keys, max_blocks,

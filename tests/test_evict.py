@@ -59,6 +59,15 @@ def test_evict_refuses(built, change, code, word):   # noqa: F811
     assert rc == code and (rc == 0 or word in said), said
 
 
+@pytest.mark.parametrize("shift", [4, 64, -64])
+def test_weights_that_overlap_in_part_are_refused(built, shift):   # noqa: F811
+    """The same memory is in place, other memory is other memory; anything between would be read by one block after another has written it."""
+    base = 1 << 20
+    for name, args, new in (("nvk_decode_attention_paged_weights", _weights_args, "new"), ("nvk_evict_kvcache", _evict_args, "new")):
+        rc, said = _call(built, name, *args(old=ctypes.c_void_p(base), **{new: ctypes.c_void_p(base + shift)}))
+        assert rc == 1 and "overlap" in said, (name, said)
+
+
 def test_a_workspace_covers_fewer_sequences_and_narrower_tables(built):   # noqa: F811
     rng = np.random.default_rng(1)
     size = built.decode_attention_weights_workspace_bytes
@@ -410,3 +419,122 @@ def test_wrong_tensors_are_refused_here_too():
         with pytest.raises(ValueError):
             lib.evict_kvcache(*a.values())
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,batch,longest,place", [("bfloat16", 160, 2048, True), ("float16", 120, 1700, False)])
+def test_weights_of_whole_contexts_by_blocks_of_eight_warps(dtype, batch, longest, place):
+    """Enough pairs beyond the clusters of four, tables of 1537 to 2048 keys: every context is one block's of eight warps, which adds the weights itself."""
+    import torch
+    rng = np.random.default_rng(batch)
+    hq, hkv, bs, blocks, width = 4, 1, 16, 130, -(-longest // 16)
+    (kc, kp, k_all, _), (vc, vp, v_all, spread) = _cache(rng, blocks * bs, hkv, dtype)
+    lens = [1 + (i * 7919) % longest for i in range(batch)]
+    lens[0], lens[1], lens[batch // 2] = 0, 1, longest
+    tables = np.stack([rng.permutation(blocks)[:width] for _ in range(batch)])
+    keys, scale, u = width * bs, 0.088, ref.HALF_STEP[dtype]
+    old = np.float32(np.exp(rng.standard_normal((batch, hkv, keys)))) / 100
+    q = _typed(rng, (batch, hq, D), dtype)
+    lib, dev = nvk(), to_dev(old)
+    new = dev if place else torch.full_like(dev, 7.0)
+    out = torch.full((batch, hq, D), float("nan"), dtype=getattr(torch, dtype), device="cuda")
+    ws = torch.empty(lib.decode_attention_weights_workspace_bytes(batch, hq, hkv, D, width, bs), dtype=torch.uint8, device="cuda").fill_(255)
+    lib.launch_decode_attention_paged_weights(_dev(q, dtype), kc, vc, kp, vp, to_dev(np.array(lens), torch.int32), to_dev(tables, torch.int32), hkv, D, bs, scale,
+                                              dev, None, new, out, ws)
+    torch.cuda.synchronize()
+    got, got_out = new.double().cpu().numpy(), out.double().cpu().numpy()
+    for i in sorted({0, 1, batch // 2, *range(0, batch, 13)}):
+        n = lens[i]
+        at = ref.places(tables[i], n, bs, blocks)
+        k, v = ref.context(k_all, at), ref.context(v_all, at)
+        want, p = ref.attend(q[i], k, v, scale)
+        e = ref.score_error(q[i], np.abs(k_all).max() + 15.5, scale) + 2.0 ** -20
+        around = p @ ref.context(spread, at)[:, 0]
+        assert (np.abs(got_out[i] - want) <= u * around + u * np.abs(want) + 2 * e * (np.abs(v_all).max() + 1)).all(), i
+        # a probability is off by 2 e of itself, and by 2^-18 (the sum: 32 additions in a lane and at most 16 that merge lanes and warps, 48 2^-24; exp2 and
+        # 1 / the sum: 2^-21 together); what is added up by an addition for each head
+        add = p.sum(0)
+        assert (np.abs(got[i, 0, :n] - (old[i, 0, :n] + add)) <= (2 * e + 2.0 ** -18) * add + 4 * 2.0 ** -24 * (old[i, 0, :n] + add) + 1e-30).all(), i
+        assert np.array_equal(got[i, 0, n:], old[i, 0, n:] if place else np.full(keys - n, 7.0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["same", "int4"])
+def test_cache_rows_beyond_32_bits_of_offset(kv):
+    """Caches of more than 4 GiB: what a context reads, stores and keeps in its last blocks is what it would in its first ones."""
+    import torch
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("24 GB of device memory")
+    rng = np.random.default_rng(5)
+    hkv, hq, bs, dtype, n = 8, 32, 256, "bfloat16", 700
+    row_bytes = hkv * (64 if kv == "int4" else 2 * D)
+    blocks = (1 << 32) // (row_bytes * bs) + 8
+    lib, dt, bf = nvk(), torch.int32, torch.bfloat16
+    k, v = (_dev(_typed(rng, (n, hkv, D), dtype), dtype) for _ in range(2))
+    q = _dev(_typed(rng, (1, hq, D), dtype), dtype)
+    results = []
+    for count in (8, blocks):
+        width = 64 if kv == "int4" else D
+        cache = [torch.empty((count * bs, hkv, width), dtype=torch.uint8 if kv == "int4" else bf, device="cuda") for _ in range(2)]
+        cache += [torch.empty((count * bs, hkv, 2), dtype=bf, device="cuda") for _ in range(2)] if kv == "int4" else [None, None]
+        table, fresh = [count - 1, count - 4, count - 2], [count - 6, count - 3, count - 5]
+        slots, bt, nt = to_dev(ref.places(table, n, bs, count), torch.int64), to_dev(np.array([table]), dt), to_dev(np.array([fresh]), dt)
+        if kv == "int4":
+            lib.store_kvcache_int4(k, v, *cache, slots)
+        else:
+            lib.store_kvcache(k, v, *cache[:2], slots)
+        ctx, lens = torch.full((1,), n, dtype=dt, device="cuda"), torch.zeros(1, dtype=dt, device="cuda")
+        w, nw = torch.zeros((1, hkv, 3 * bs), device="cuda"), torch.zeros((1, hkv, 3 * bs), device="cuda")
+        ws = torch.empty(lib.decode_attention_weights_workspace_bytes(1, hq, hkv, D, 3, bs), dtype=torch.uint8, device="cuda")
+        first, second = torch.empty_like(q), torch.empty_like(q)
+        lib.launch_decode_attention_paged_weights(q, *cache, ctx, bt, hkv, D, bs, 0.088, None, None, w, first, ws)
+        lib.evict_kvcache(*cache, w, None, ctx, bt, nw, nt, lens, hkv, D, bs, 300, 4, 32)
+        lib.launch_decode_attention_paged_weights(q, *cache, lens, nt, hkv, D, bs, 0.088, None, None, w, second, ws)
+        got = [first, second, w, nw, lens]
+        if kv == "int4":
+            dense = [torch.empty((300, hkv, D), dtype=bf, device="cuda") for _ in range(2)]
+            lib.gather_kvcache_int4(*cache, to_dev(np.array([0, 300]), dt), nt, hkv, D, bs, *dense)
+            got += dense
+        torch.cuda.synchronize()
+        results.append([x.clone() for x in got])
+        del cache
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and not torch.isnan(results[0][1]).any()
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once_do_not_touch_each_other():
+    """Two streams, each with its own cache, weights and workspace: forty rounds of steps and evictions in place give what they give one after the other."""
+    import torch
+    rng = np.random.default_rng(9)
+    hq, hkv, bs, dtype, width, b = 8, 2, 16, "bfloat16", 40, 12
+    lib, dt, bf = nvk(), torch.int32, torch.bfloat16
+
+    def state(seed):
+        r = np.random.default_rng(seed)
+        blocks = b * width
+        (kc, kp, _, _), (vc, vp, _, _) = _cache(r, blocks * bs, hkv, dtype)
+        tables = to_dev(r.permutation(blocks).reshape(b, width), dt)
+        q = _dev(_typed(r, (b, hq, D), dtype), dtype)
+        return dict(cache=[kc, vc, kp, vp], bt=tables, q=q, ctx=to_dev(np.array([600 - 40 * i for i in range(b)]), dt), out=torch.empty((40, b, hq, D), dtype=bf, device="cuda"),
+                    w=torch.zeros((b, hkv, width * bs), device="cuda"), lens=torch.zeros(b, dtype=dt, device="cuda"),
+                    ws=torch.empty(lib.decode_attention_weights_workspace_bytes(b, hq, hkv, D, width, bs), dtype=torch.uint8, device="cuda"))
+
+    def round_of(s, i):
+        lib.launch_decode_attention_paged_weights(s["q"], *s["cache"], s["ctx"], s["bt"], hkv, D, bs, 0.088, s["w"], None, s["w"], s["out"][i], s["ws"])
+        lib.evict_kvcache(*s["cache"], s["w"], None, s["ctx"], s["bt"], s["w"], s["bt"], s["lens"], hkv, D, bs, 590 - 10 * i, 4, 32)
+        s["ctx"].copy_(s["lens"])
+
+    alone, at_once = [state(1), state(2)], [state(1), state(2)]
+    for s in alone:
+        for i in range(40):
+            round_of(s, i)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(40):
+        for s, stream in zip(at_once, streams):
+            with torch.cuda.stream(stream):
+                round_of(s, i)
+    torch.cuda.synchronize()
+    for x, y in zip(alone, at_once):
+        assert torch.equal(x["out"], y["out"]) and torch.equal(x["w"], y["w"]) and torch.equal(x["ctx"], y["ctx"])
+        assert all(torch.equal(a, c) for a, c in zip(x["cache"], y["cache"])) and not torch.isnan(x["out"]).any()
