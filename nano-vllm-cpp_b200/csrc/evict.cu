@@ -385,12 +385,17 @@ int launch_evict(const EvictArgs& a) {
     if (a.batch * a.num_kv_heads > 0x7fffffffLL || a.max_blocks * a.block_size > (1LL << 30) || a.new_max_blocks * a.block_size > (1LL << 30) ||
         a.num_cache_blocks > 0x7fffffffLL / a.block_size)
         return fail(NVK_ERR_UNSUPPORTED, "evict_kvcache: batch, block table or cache too large");
-    // As many blocks to a pair as there are places for, two to an SM, and no more than there are pairs of tiles; one to an SM where that lets few pairs of long
-    // contexts keep their orders.
+    // As many blocks to a pair as there are places for, and no more than there are pairs of tiles.  Two to an SM, where there is enough to do: the second block
+    // costs some 3 us, whatever there is.  One to an SM up to 300000 keys of all pairs' tables, 150000 with more than half as many pairs as SMs (which then have one
+    // block each), 100000 where rows are 4-bit ones (us, one / two to an SM, a third of the keys kept: 16-bit 16 pairs of 4096 12.7 / 15.7, 64 of 1024 11.1 / 13.6,
+    // 72 of 4096 29.2 / 30.0, 144 of 1024 16.2 / 17.6, but 40 of 8192 36.7 / 34.2, 64 of 6000 38.2 / 36.6, 88 of 3000 31.7 / 27.5; 4-bit 48 of 2048 17.4 / 20.3, 24
+    // of 4096 17.7 / 20.9, but 40 of 4096 26.4 / 25.1, 144 of 2048 35.3 / 31.8), and where that lets few pairs of long contexts keep their orders.  More blocks than
+    // places do not even out contexts of different lengths (256 pairs of 1000 to 8192 keys: one block each 107.2, two 108.9, four 110.6, eight 137.9).
     const int64_t pairs = a.batch * a.num_kv_heads, tokens = a.max_blocks * a.block_size, most = (tokens + 2 * kWarpTile - 1) / (2 * kWarpTile);
     const bool alone = tokens > kCached && 2 * pairs <= kSmCount;
+    const bool single = alone || pairs * tokens <= (a.k_params != nullptr ? 100000 : 2 * pairs <= kSmCount ? 300000 : 150000);
     const int cached = alone ? kCachedAlone : kCached;
-    const int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((alone ? 1 : 2) * kSmCount / pairs, most), kMaxSplit)));
+    const int split = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>((single ? 1 : 2) * kSmCount / pairs, most), kMaxSplit)));
     const EvictParams p{a.k_cache, a.v_cache, static_cast<uint32_t*>(a.k_params), static_cast<uint32_t*>(a.v_params), a.weights, a.new_weights, a.rows,
                         a.context_lens, a.block_tables, a.new_tables, a.new_lens, a.num_rows, a.row_keys, a.max_blocks, a.new_max_blocks,
                         a.num_cache_blocks, a.budget, a.sinks, a.recent, a.num_kv_heads, a.block_size, split, cached, FastDiv(static_cast<uint32_t>(a.block_size))};
