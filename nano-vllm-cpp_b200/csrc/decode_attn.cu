@@ -1,16 +1,18 @@
-// Paged-KV decode attention for sm_100a (F16 / BF16 queries, head_dim 128; 16-bit, int8 and e4m3 caches).
+// Paged-KV decode attention for sm_100a (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 and 4-bit caches), and the same with the weights of the
+// keys added up.
 //
 // Replaces decode_paged_attention_kernel and decode_paged_attention_int8_kernel (src/kernels/attention.cu:313-405, :746-842 of the
 // reference: one warp per (sequence, query head), every KV row re-read by each query head of its group, 8 dependent shuffles per
 // key) and the FlashAttention-2 call it can dlopen (src/kernels/flash_attn.cpp:302-431).
 //
-// The op is HBM-bound; decode_body.cuh has the arithmetic and the ways to share out the keys.  What each kernel here adds:
-//   decode_split_kernel    one four-warp block per (KV head, chunk, sequence), two per SM (three for 8-bit caches).  The grid is fixed
+// The op is HBM-bound (over a 4-bit cache bound by issue); decode_body.cuh has the arithmetic and the ways to share out the keys.  What each kernel here adds:
+//   decode_split_kernel    one four-warp block per (KV head, chunk, sequence), two per SM (three for 8-bit caches, four for 4-bit ones, or two of eight warps).  The grid is fixed
 //                          from host-known sizes: nothing depends on host knowledge of context_lens (CUDA-graph safe); blocks
 //                          whose chunk lies beyond the context exit at once.
 //   decode_merge_kernel    merges the chunks of long contexts; launched only where the table can hold more than one.
 //   decode_cluster_kernel  small steps: a cluster of blocks per (sequence, KV head) takes equal ranges of the context, beyond them two blocks the halves
 //                          of the table's row; merged in the same launch.
+//   key_weights_kernel     where contexts are in chunks, adds what each key got to its row of weights; the other kernels do that themselves.
 // Which one is taken depends on the table's WIDTH, not on the contexts: one short sequence in a wide table takes chunks and a merge.
 #include "decode_body.cuh"
 

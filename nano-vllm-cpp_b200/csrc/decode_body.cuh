@@ -430,6 +430,8 @@ struct Cache8 {
 // d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; with halves of two keys' words side by side the same masks give both keys' numbers, and accumulator
 // rows g / g + 8 of d-tile i hold d = 16 g + 2 i and d = 16 g + 2 i + 1 (times 16).  The two rows of a 128-byte line of V are swizzled by the line's number, so
 // that these reads are conflict free.
+// A quarter of the bytes, for as many MMAs: the step is bound by issue (64 sequences of 500 to 4096 keys, 32 / 8 heads, 46.3 us where the bytes take 24.6: issue
+// slots 52 % busy, the ALU pipe 51 %, tensor 24 %, DRAM 45 %; per warp and 32 keys some 570 cycles of a scheduler, of which the MMAs and the masks take most).
 // A warp takes 32 keys at a time, two chains of 16: the arithmetic of a tile is one long chain, and three warps to a scheduler do not hide it.  The cache
 // rows of its next 16 tiles are worked out by the lanes, one half of a tile each, while the ids of the 16 after them are on their way.
 template <int AT> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {

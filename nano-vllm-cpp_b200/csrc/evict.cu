@@ -3,7 +3,8 @@
 // Of every (sequence, KV head) the first `sinks` keys stay, the last `recent`, and of those between the ones of the largest weights, `budget` in all
 // (of equal weights the key that comes first; NaN counts as the least).  What stays closes up, in its order, its weights with it.
 //
-// HBM-bound: the weights are read, the rows of what stays are read and written.  Where there are few (sequence, KV head) pairs several blocks share one: each
+// HBM-bound: the weights are read, the rows of what stays are read and written (32 sequences of 1000 to 8192 keys, 8 KV heads, 2048 of them kept, 524 MB: 107 us,
+// 4.9 TB/s; SMs are busy for 77 % of that, since 256 pairs are two blocks for some SMs and one for others).  Where there are few (sequence, KV head) pairs several blocks share one: each
 // finds for itself who stays (weights are a small part of what is read, and come from L2; histograms added up through distributed shared memory took 10 us
 // more a pass), and moves the rows of its share of the tiles.  A block
 //   1  reads the weights as whole numbers of the same order into shared memory (contexts of up to 16384 keys, 45056 where it is alone on an SM; longer ones are

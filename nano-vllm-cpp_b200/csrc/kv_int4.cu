@@ -7,6 +7,9 @@
 // two to a byte (element 2i in the low half of byte i), and the pair (step, low) in the type itself: x stands for low + step n, off by half a step
 // at most (and by 15 / 2 of what the rounding of step took off it at the top).  low is an element of x, so that it needs no rounding.  A vector whose
 // range is not finite gets a pair of NaN, and reads as NaN.
+//
+// The store should be HBM-bound (of an element two bytes are read and half a one is written) but is bound by issue: 36864 tokens of 8 heads, 192 MB, take 37.5 us, 5.1
+// TB/s, with 80 % of the issue slots busy and DRAM at half.  The gather writes 3.8 times what it reads: 43008 rows of 8 heads, 223 MB, take 39 us, 5.7 TB/s.
 #include "nvk_internal.cuh"
 
 #include <type_traits>
