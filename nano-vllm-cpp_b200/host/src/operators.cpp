@@ -269,8 +269,10 @@ void evict_kvcache(Tensor& k_cache, Tensor& v_cache, Tensor& k_params, Tensor& v
     ensure_rows("block_tables", block_tables, batch);
     ensure_rows("new_block_tables", new_block_tables, batch);
     if (weight_rows.defined()) ensure_rows("weight_rows", weight_rows, batch);
-    for (const Tensor* t : {&key_weights, static_cast<const Tensor*>(&new_key_weights), &context_lens, &block_tables, &new_block_tables})
+    for (const Tensor* t : {&key_weights, static_cast<const Tensor*>(&new_key_weights), &context_lens, &block_tables, &new_block_tables,
+                            static_cast<const Tensor*>(&new_context_lens)})
         ensure_same_device("k_cache", k_cache, "every other tensor", *t);
+    if (weight_rows.defined()) ensure_same_device("k_cache", k_cache, "weight_rows", weight_rows);
     throw_on_nvk_status(nvk_evict_kvcache(k_cache.data(), v_cache.data(), four ? k_params.data() : nullptr, four ? v_params.data() : nullptr,
                                           key_weights.data_as<float>(), rows.ptr, rows.dtype, key_weights.sizes()[0], key_weights.sizes()[2], lens.ptr,
                                           lens.dtype, tables.ptr, tables.dtype, batch, block_tables.sizes()[1], blocks, new_key_weights.data_as<float>(),

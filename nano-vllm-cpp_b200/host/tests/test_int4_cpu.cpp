@@ -92,6 +92,20 @@ TEST_CASE(evict_refuses) {
     CHECK_THROWS(evict(c.weights, c.lens, new_lens32, 8, 8), std::invalid_argument);        // more kept than the budget
 }
 
+TEST_CASE(evict_refuses_tensors_of_another_device) {
+    Case c;
+    Tensor new_lens = borrowed({1}, ScalarType::kInt32), rows = borrowed({1}, ScalarType::kInt32);
+    auto elsewhere = [](uintptr_t at) {
+        return Tensor::from_memory(Memory::make_borrowed(reinterpret_cast<void*>(at), 4, Device{DeviceType::kCUDA, 1}), {1}, ScalarType::kInt32);
+    };
+    Tensor far_lens = elsewhere(0x90000000), far_rows = elsewhere(0x91000000);
+    auto evict = [&](const Tensor& row_of, Tensor& to) {
+        evict_kvcache(c.k_cache, c.v_cache, c.params, c.params, c.weights, row_of, c.lens, c.tables, c.weights, c.tables, to, 2, 128, 16, 8, 1, 2);
+    };
+    CHECK_THROWS(evict(c.none, far_lens), std::invalid_argument);
+    CHECK_THROWS(evict(far_rows, new_lens), std::invalid_argument);
+}
+
 TEST_CASE(layer_refuses) {
     Case c;
     Attention attention(4, 2, 128, 16), narrow(4, 2, 64, 16);
