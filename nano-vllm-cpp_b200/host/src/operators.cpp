@@ -227,6 +227,9 @@ void gather_kvcache_int4(const Tensor& k_cache, const Tensor& v_cache, const Ten
     const IndexRef starts = index_data("cu_seqlens_k", cu_seqlens_k), tables = index_data("block_tables", block_tables);
     const int64_t rows = int4_rows(k_cache, v_cache, k_params, v_params, key.dtype(), num_kv_heads, head_dim);
     ensure_same_device("key", key, "k_cache", k_cache);
+    ensure_same_device("key", key, "value", value);
+    ensure_same_device("key", key, "cu_seqlens_k", cu_seqlens_k);
+    ensure_same_device("key", key, "block_tables", block_tables);
     if (key.dim() != 3 || key.sizes()[1] != num_kv_heads || key.sizes()[2] != head_dim)
         throw std::invalid_argument("key must be [total_k, num_kv_heads, head_dim]");
     const int64_t seqs = static_cast<int64_t>(cu_seqlens_k.numel()) - 1;
@@ -250,6 +253,7 @@ void evict_kvcache(Tensor& k_cache, Tensor& v_cache, Tensor& k_params, Tensor& v
         ensure_cuda_tensor("k_cache", k_cache);
         ensure_cuda_tensor("v_cache", v_cache);
         ensure_same_dtype("k_cache", k_cache, "v_cache", v_cache);
+        ensure_same_device("k_cache", k_cache, "v_cache", v_cache);
         if (k_cache.numel() != v_cache.numel()) throw std::invalid_argument("k_cache and v_cache must contain the same number of slots");
         blocks = cache_blocks(k_cache, block_size, num_kv_heads, head_dim);
     }
@@ -430,6 +434,7 @@ struct Step {
             blocks = cache_blocks(k_cache, block_size, num_kv_heads, head_dim);
         }
         ensure_same_device("query", query, "k_cache", k_cache);
+        ensure_same_device("query", query, "v_cache", v_cache);
         ensure_same_device("query", query, "context_lens", context_lens);
         ensure_same_device("query", query, "block_tables", block_tables);
     }
@@ -468,7 +473,10 @@ void launch_decode_attention_paged_weights(const Tensor& query, const Tensor& k_
     }
     ensure_same_device("query", query, "new_key_weights", new_key_weights);
     const IndexRef rows = weight_rows.defined() ? index_data("weight_rows", weight_rows) : IndexRef{nullptr, NVK_I32};
-    if (weight_rows.defined()) ensure_rows("weight_rows", weight_rows, s.batch);
+    if (weight_rows.defined()) {
+        ensure_rows("weight_rows", weight_rows, s.batch);
+        ensure_same_device("query", query, "weight_rows", weight_rows);
+    }
     const size_t need = nvk_decode_attention_weights_workspace_bytes(s.batch, s.heads, num_kv_heads, head_dim, s.max_blocks, block_size);
     Memory::Ptr scratch = need > 0 ? allocator.allocate(need, query.device()) : nullptr;
     throw_on_nvk_status(nvk_decode_attention_paged_weights(

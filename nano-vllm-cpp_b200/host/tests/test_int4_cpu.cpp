@@ -106,6 +106,25 @@ TEST_CASE(evict_refuses_tensors_of_another_device) {
     CHECK_THROWS(evict(far_rows, new_lens), std::invalid_argument);
 }
 
+TEST_CASE(decode_and_gather_refuse_tensors_of_another_device) {
+    Case c;
+    NoAllocator none;
+    auto far = [](const std::vector<int64_t>& sizes, ScalarType type, uintptr_t at) {
+        return Tensor::from_memory(Memory::make_borrowed(reinterpret_cast<void*>(at), compute_numel(sizes) * scalar_type_size(type), Device{DeviceType::kCUDA, 1}),
+                                   sizes, type);
+    };
+    Tensor rows = far({1}, ScalarType::kInt32, 0x92000000), starts = far({2}, ScalarType::kInt32, 0x93000000), tables = far({1, 2}, ScalarType::kInt32, 0x94000000),
+           near_starts = borrowed({2}, ScalarType::kInt32), value = borrowed({3, 2, 128}, ScalarType::kBFloat16), new_lens = borrowed({1}, ScalarType::kInt32),
+           k16 = borrowed({2, 16, 2, 128}, ScalarType::kBFloat16), v16 = far({2, 16, 2, 128}, ScalarType::kBFloat16, 0x95000000);
+    CHECK_THROWS(launch_decode_attention_paged_weights(c.query, c.k_cache, c.v_cache, c.params, c.params, c.lens, c.tables, 2, 128, 16, 1.0f, c.none, rows, c.weights,
+                                                       c.output, none, nullptr), std::invalid_argument);
+    CHECK_THROWS(launch_decode_attention_paged_weights(c.query, k16, v16, c.none, c.none, c.lens, c.tables, 2, 128, 16, 1.0f, c.none, c.none, c.weights, c.output, none,
+                                                       nullptr), std::invalid_argument);
+    CHECK_THROWS(evict_kvcache(k16, v16, c.none, c.none, c.weights, c.none, c.lens, c.tables, c.weights, c.tables, new_lens, 2, 128, 16, 8, 1, 2), std::invalid_argument);
+    CHECK_THROWS(gather_kvcache_int4(c.k_cache, c.v_cache, c.params, c.params, starts, c.tables, 2, 128, 16, c.key, value), std::invalid_argument);
+    CHECK_THROWS(gather_kvcache_int4(c.k_cache, c.v_cache, c.params, c.params, near_starts, tables, 2, 128, 16, c.key, value), std::invalid_argument);
+}
+
 TEST_CASE(layer_refuses) {
     Case c;
     Attention attention(4, 2, 128, 16), narrow(4, 2, 64, 16);
