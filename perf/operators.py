@@ -243,7 +243,7 @@ def _quantise(x):
     """(bytes, (step, low)) of head vectors; in 64 bits, where a value can lie next to the border between two numbers."""
     lo, hi = x.float().amin(-1, keepdim=True), x.float().amax(-1, keepdim=True)
     span = hi - lo
-    step = (span / torch.full_like(span, LEVELS)).to(x.dtype)
+    step = (span / LEVELS).to(x.dtype)
     fine = torch.isfinite(span)
     n = torch.floor((x.double() - lo.double()) / step.double() + 0.5).clamp(max=LEVELS)
     n = torch.where(fine & (step > 0), n, 0.0).to(torch.uint8)
