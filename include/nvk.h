@@ -185,7 +185,8 @@ int nvk_decode_attention_paged_fp8(const void* query, const void* k_cache, const
  * rows whose table entry is outside the cache or the table are zeros; sequences are cut off at total_k.
  *
  * nvk_decode_attention_paged_int4: the semantics of nvk_decode_attention_paged over the elements as they are (low + step * n is not rounded); at most
- * 8 query heads per KV head, block_size a multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes).
+ * 8 query heads per KV head, block_size a multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes).  One rounding to 16 bits: a head's
+ * weight times the step of the value, to f16, off by 2^-11 of itself or 2^-22 of the head's largest such product.
  */
 int nvk_store_kvcache_int4(const void* key, const void* value, void* k_cache, void* v_cache, void* k_params, void* v_params,
                            const void* slot_mapping, int slot_dtype, int64_t num_tokens, int num_kv_heads, int head_dim, int64_t cache_rows,

@@ -424,7 +424,10 @@ struct Cache8 {
 //   sum_k p_k x_k = 2^E (2^24 sum_k p'_k n_k 2^-24 - 7.5 sum_k p'_k) + sum_k p_k (low_k + 7.5 step_k),   p'_k = p_k step_k 2^-E rounded to f16
 // p' is the one rounding to 16 bits (as with the other caches).  With F16 results the middle of the range goes in the fp32 sum at the right, so that what the
 // rounding touches is no larger than the values' spread, and sum(p') comes from an MMA against a row of ones, i.e. from exactly the p' that the others used;
-// a BF16 result is rounded to an eighth of p''s precision, and the 7.5 and the MMA are left out.  2^E is the largest step so far, rounded down to a power of two: p' <= 2, and held to 2^-25 of that; the sums are rescaled where it grows, as where a maximum does.
+// a BF16 result is rounded to an eighth of p''s precision, and the 7.5 and the MMA are left out.  2^E is each head's own and goes by p step: the largest p' is at
+// least 1/8 when E is chosen, and all are held to 2^-22 of the largest or better.  (By the largest step alone, a key that hardly any attention went to could take the others' bits: one
+// whose step was 2^20 times theirs cost them 10 to 20 %.)  E is chosen, and the sums are rescaled, where a score passes the last maximum by 8 or a step reaches 2^(7 + E): p' < 2^15.
+// (At every new maximum, the ranges of 8 to 16 tiles a warp of few long contexts came there at nearly every tile.)
 // As in Cache8 the order in which a contraction runs is free: of key row g lane t takes the 16-byte piece t, whose word w has the k-steps
 // 2w and 2w + 1 (registers: elements {0, 4}, {1, 5}; {2, 6}, {3, 7}; the query fragment is loaded the same way).  Of V lane (g, t) takes 8 bytes,
 // d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; with halves of two keys' words side by side the same masks give both keys' numbers, and accumulator
@@ -460,6 +463,7 @@ struct Cache4 {
     static constexpr int kStages = 3;
     static constexpr int kPartStride = kHeadDim + 4;
     static constexpr bool kCentred = std::is_same<T, __half>::value;
+    static constexpr float kSlack = 8.0f;                     // by so much a score may pass s.m: p <= 2^8
     static constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u, kNone = 0xffffffffu;
 
     SoftmaxState s;
@@ -467,7 +471,8 @@ struct Cache4 {
     float ones[4];       // sum(p')
     float mid[2];        // sum(p (low + 7.5 step)) of heads 2t, 2t + 1 over the lane's keys
     float q_sum[2], step_scale;
-    float v_down;        // 2^-E
+    float down[2];       // 2^-E of heads 2t, 2t + 1
+    float top_part[2];   // the largest log2(p step) so far, p without the maximum taken off
     uint32_t qa[8][2];   // k-step 2 w + e: elements 32 t + 8 w + 2 e + {0, 4 | 1, 5}
 
     __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
@@ -508,7 +513,8 @@ struct Cache4 {
         q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t) * p.scale_log2;
         q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * p.scale_log2;
         ones[0] = ones[1] = ones[2] = ones[3] = mid[0] = mid[1] = 0.0f;
-        v_down = 0x1p126f;
+        down[0] = down[1] = 0x1p126f;
+        top_part[0] = top_part[1] = -INFINITY;
         s.reset();
     }
     static __device__ __forceinline__ void lds64(uint32_t addr, uint2& v) { asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr)); }
@@ -537,25 +543,29 @@ struct Cache4 {
             for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(acc[2 * i + h], step, kp.y * q_sum[h]);
         }
     }
-    __device__ __forceinline__ int exponent() const { return 127 - static_cast<int>(__float_as_uint(v_down) >> 23); }   // E
-    // Where a maximum or the largest step grows.
-    __device__ __forceinline__ void raise(float top0, float top1, float top_step) {
-        float top[2] = {top0, top1}, c[2];
-#pragma unroll
-        for (int x = 1; x < 32; x *= 2) top_step = fmaxf(top_step, __shfl_xor_sync(0xffffffffu, top_step, x));
-        const int was = exponent(), e = min(max(was, static_cast<int>(__float_as_uint(top_step) >> 23) - 127), 126);
-        const float down = power_of_two(max(was - e, -126));   // (2^-126 or less: what was there is no longer seen beside what is coming)
-        v_down = power_of_two(-e);
+    __device__ __forceinline__ int exponent(int h) const { return 127 - static_cast<int>(__float_as_uint(down[h]) >> 23); }   // E
+    // Where a score passes s.m by more than kSlack, or a p' could leave f16.  s.m is then the maximum, and E is chosen again: the largest p' of the tiles that came here is between
+    // 1/8 and 1/4.
+    __device__ __forceinline__ void raise(const float (&sa)[4], const float (&sb)[4], const float2 (&va)[2], const float2 (&vb)[2]) {
+        const float a0 = __log2f(fabsf(va[0].x)), a1 = __log2f(fabsf(va[1].x)), b0 = __log2f(fabsf(vb[0].x)), b1 = __log2f(fabsf(vb[1].x));
+        float c[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+            float top = fmaxf(fmaxf(sa[h], sa[2 + h]), fmaxf(sb[h], sb[2 + h])), part = fmaxf(fmaxf(sa[h] + a0, sa[2 + h] + a1), fmaxf(sb[h] + b0, sb[2 + h] + b1));
 #pragma unroll
-            for (int x = 4; x < 32; x *= 2) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], x));
-            const float m_new = fmaxf(s.m[h], top[h]);
+            for (int x = 4; x < 32; x *= 2) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, x));
+            }
+            const float m_new = fmaxf(s.m[h], top);
+            top_part[h] = fmaxf(top_part[h], part);
+            const int was = exponent(h), e = static_cast<int>(fminf(fmaxf(ceilf(top_part[h] - m_new) + 2.0f, -126.0f), 126.0f));
             c[h] = s.m[h] == m_new ? 1.0f : fast_exp2(s.m[h] - m_new);
             s.l[h] *= c[h];
             mid[h] *= c[h];
             s.m[h] = m_new;
-            c[h] *= down;
+            c[h] *= power_of_two(min(max(was - e, -126), 127));   // (beyond that nothing is seen of what was there, or there was nothing)
+            down[h] = power_of_two(-e);
         }
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) { s.o[mt][0] *= c[0]; s.o[mt][1] *= c[1]; s.o[mt][2] *= c[0]; s.o[mt][3] *= c[1]; }
@@ -567,11 +577,12 @@ struct Cache4 {
         const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
-        const float mid0 = kCentred ? fmaf(vp[0].x, 7.5f, vp[0].y) : vp[0].y, mid1 = kCentred ? fmaf(vp[1].x, 7.5f, vp[1].y) : vp[1].y, st0 = vp[0].x * v_down, st1 = vp[1].x * v_down;
+        const float mid0 = kCentred ? fmaf(vp[0].x, 7.5f, vp[0].y) : vp[0].y, mid1 = kCentred ? fmaf(vp[1].x, 7.5f, vp[1].y) : vp[1].y;
         mid[0] = fmaf(p0, mid0, fmaf(p2, mid1, mid[0]));
         mid[1] = fmaf(p1, mid0, fmaf(p3, mid1, mid[1]));
-        const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * st0, p1 * st0));
-        const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * st1, p3 * st1));
+        // (p first: where it is 0, 2^-E step need not be finite)
+        const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * down[0] * vp[0].x, p1 * down[1] * vp[0].x));
+        const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * down[0] * vp[1].x, p3 * down[1] * vp[1].x));
         // V rows 2t, 2t + 1 (line t) and 2t + 8, 2t + 9 (line t + 4), words 2g and 2g + 1: half of piece g / 2
         const uint32_t v_at = stage + kTileBytes + row0 * kRowBytes + t * 128 + (g & 1) * 8, even = ((g >> 1) ^ (t << 1)) << 4;
         uint2 x[4];
@@ -605,7 +616,7 @@ struct Cache4 {
         if constexpr (SCORES) kept.put(p, sa, sb, valid, lane, WARPS);
         const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
         const float top_step = fmaxf(fmaxf(fabsf(va[0].x), fabsf(va[1].x)), fmaxf(fabsf(vb[0].x), fabsf(vb[1].x)));
-        if (__any_sync(0xffffffffu, top0 > s.m[0] || top1 > s.m[1] || top_step * v_down >= 2.0f)) raise(top0, top1, top_step);
+        if (__any_sync(0xffffffffu, fmaxf(top0 - s.m[0], top1 - s.m[1]) > kSlack || top_step * fmaxf(down[0], down[1]) >= 0x1p7f)) raise(sa, sb, va, vb);
         add(stage, 0, sa, va, lane);
         add(stage, 16, sb, vb, lane);
     }
@@ -719,7 +730,7 @@ struct Cache4 {
         }
     }
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
-        const float up = power_of_two(exponent()), off = kCentred ? fmaf(ones[h] * -7.5f, up, mid[h]) : mid[h];
+        const float up = power_of_two(exponent(h)), off = kCentred ? fmaf(ones[h] * -7.5f, up, mid[h]) : mid[h];
         auto even = [&](int i) { return fmaf(s.o[i][h] * 0x1p24f, up, off); };
         auto odd = [&](int i) { return fmaf(s.o[i][2 + h] * 0x1p20f, up, off); };
 #pragma unroll

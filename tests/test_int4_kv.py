@@ -360,3 +360,31 @@ def test_decode_of_many_contexts_however_they_are_shared_out(batch, longest):
     # both round p' to f16 (2^-11 of at most 15 steps each way) and the result to bf16 (half a step each)
     most = 2 * 2.0 ** -11 * 15 * float(spread.max()) / 7.5 + 2 * 2.0 ** -8 * float(np.abs(vv).max())
     assert (single[::37].float() - out[::37].float()).abs().max().item() <= most
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,power", [("bfloat16", 16), ("bfloat16", 20), ("bfloat16", 60), ("float16", 17)])
+@pytest.mark.parametrize("place", [0, 40, 289])
+def test_a_value_of_a_large_range_without_weight_leaves_the_others_alone(dtype, power, place):
+    """One key whose value spans 2^power times what the others do, and that hardly any of the attention goes to: before, among and after the others."""
+    import torch
+    rng = np.random.default_rng(power)
+    hq, hkv, bs, n, scale = 4, 1, 64, 290, 0.088
+    key, val = _typed(rng, (320, hkv, D), dtype, 0.25), _typed(rng, (320, hkv, D), dtype, 2.0 ** -4)
+    q = _typed(rng, (1, hq, D), dtype)
+    away = -q[0].sum(0)
+    key[place, 0] = ref.to_type(away * (80.0 + power) / scale / np.abs(q[0] @ away).min(), dtype)
+    val[place] = ref.to_type(val[place] * 2.0 ** power, dtype)
+    (kd, kpar), (vd, vpar) = ref.quantise(key, dtype), ref.quantise(val, dtype)
+    k, v = ref.values(kd, kpar)[:n], ref.values(vd, vpar)[:n]
+    want, p = ref.attend(q[0], k, v, scale)
+    assert p[:, place].max() * 2.0 ** power < 2.0 ** -24                  # what the key itself adds
+    out = torch.empty((1, hq, D), dtype=getattr(torch, dtype), device="cuda")
+    nvk().launch_decode_attention_paged_int4(_dev(q, dtype), torch.from_numpy(kd).cuda(), torch.from_numpy(vd).cuda(), _dev(kpar, dtype), _dev(vpar, dtype),
+                                             to_dev(np.array([n]), torch.int32), to_dev(np.arange(5)[None], torch.int32), hkv, D, bs, scale, out)
+    # p' is rounded to f16 (2^-11 of it, or 2^-22 of the largest p step) and multiplied by up to 15, the result is rounded to the type; a score off by e moves
+    # p by 2e of itself.  What a key without weight can do to the sums in fp32 goes by its p step as well.
+    u, step = ref.HALF_STEP[dtype], vpar[:n, 0, 0]
+    e = ref.score_error(q[0], np.abs(np.delete(k, place, 0)).max() + 31 * 0.25, scale) + 2.0 ** -20
+    most = 15 * (2.0 ** -11 * (p @ step) + 2.0 ** -22 * n * (p * step).max(-1))[:, None] + u * np.abs(want) + 2 * e * (p @ np.abs(v[:, 0]) + np.abs(want)) + 2.0 ** -20
+    assert (np.abs(out[0].double().cpu().numpy() - want) <= most).all(), (np.abs(out[0].double().cpu().numpy() - want) / most).max()
