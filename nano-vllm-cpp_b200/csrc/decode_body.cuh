@@ -418,8 +418,8 @@ struct Cache8 {
 // 4-bit cache: per token and KV head 64 bytes of K, 64 of V (numbers n from 0 to 15, element 2i in the low half of byte i) and for each a
 // pair (step, low) in the queries' type; an element is low + step n.  The MMA operands are made from the nibbles in registers: a nibble in bits 0 to 3
 // of an f16 is the subnormal number n 2^-24, in bits 4 to 7 it is 16 n 2^-24, exactly, so that a word of eight nibbles gives its four registers for one shift
-// and four ANDs, whatever the queries' type.  Queries are brought to f16 by a power of two (exact but for elements 2^-25 of the largest),
-// those that meet a number times 16 divided by it; sums are fp32:
+// and four ANDs, whatever the queries' type.  Queries are brought to f16 by a power of two, each head's own (exact but for
+// elements below 2^-24 of the head's largest), those that meet a number times 16 divided by it; sums are fp32:
 //   q . x         = step 2^24 (q . n 2^-24) + low sum(q)
 //   sum_k p_k x_k = 2^E (2^24 sum_k p'_k n_k 2^-24 - 7.5 sum_k p'_k) + sum_k p_k (low_k + 7.5 step_k),   p'_k = p_k step_k 2^-E rounded to f16
 // p' is the one rounding to 16 bits (as with the other caches).  With F16 results the middle of the range goes in the fp32 sum at the right, so that what the
@@ -435,7 +435,7 @@ struct Cache8 {
 // that these reads are conflict free.
 // A quarter of the bytes, for as many MMAs: the step is bound by issue (64 sequences of 500 to 4096 keys, 32 / 8 heads, 46.3 us where the bytes take 24.6: issue
 // slots 52 % busy, the ALU pipe 51 %, tensor 24 %, DRAM 45 %; per warp and 32 keys some 570 cycles of a scheduler, of which the MMAs and the masks take most).
-// A warp takes 32 keys at a time, two chains of 16: the arithmetic of a tile is one long chain, and three warps to a scheduler do not hide it.  The cache
+// A warp takes 32 keys at a time, two chains of 16: the arithmetic of a tile is one long chain, and the four warps of a scheduler (three in clusters) do not hide it.  The cache
 // rows of its next 16 tiles are worked out by the lanes, one half of a tile each, while the ids of the 16 after them are on their way.
 template <int AT> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0+%2], [%1], 16;\n" ::"r"(dst), "l"(src), "n"(AT));
@@ -470,7 +470,7 @@ struct Cache4 {
     ScoreOut kept;       // (SCORES)
     float ones[4];       // sum(p')
     float mid[2];        // sum(p (low + 7.5 step)) of heads 2t, 2t + 1 over the lane's keys
-    float q_sum[2], step_scale;
+    float q_sum[2], step_scale[2];
     float down[2];       // 2^-E of heads 2t, 2t + 1
     float top_part[2];   // the largest log2(p step) so far, p without the maximum taken off
     uint32_t qa[8][2];   // k-step 2 w + e: elements 32 t + 8 w + 2 e + {0, 4 | 1, 5}
@@ -495,11 +495,13 @@ struct Cache4 {
             }
         }
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        // the largest to [2^14, 2^15); (infinities and NaN stay what they are)
+        for (int x = 1; x < 4; x *= 2) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        }
+        // the head's largest to [2^14, 2^15); (infinities and NaN stay what they are)
         const int up = top > 0.0f && top < INFINITY ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 100) : 0;
         const float even = power_of_two(up), odd = even * 0.0625f;
-        step_scale = p.scale_log2 * 0x1p24f * power_of_two(-up);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float2 e01 = unpack2<T>(v[w].x), e23 = unpack2<T>(v[w].y), e45 = unpack2<T>(v[w].z), e67 = unpack2<T>(v[w].w);
@@ -508,10 +510,11 @@ struct Cache4 {
             qa[2 * w + 1][0] = ElemTraits<__half>::pack2(e23.x * even, e67.x * even);
             qa[2 * w + 1][1] = ElemTraits<__half>::pack2(e23.y * odd, e67.y * odd);
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        q_sum[0] = __shfl_sync(0xffffffffu, sum, 8 * t) * p.scale_log2;
-        q_sum[1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4) * p.scale_log2;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            q_sum[h] = __shfl_sync(0xffffffffu, sum, 8 * t + 4 * h) * p.scale_log2;
+            step_scale[h] = p.scale_log2 * 0x1p24f * power_of_two(-__shfl_sync(0xffffffffu, up, 8 * t + 4 * h));
+        }
         ones[0] = ones[1] = ones[2] = ones[3] = mid[0] = mid[1] = 0.0f;
         down[0] = down[1] = 0x1p126f;
         top_part[0] = top_part[1] = -INFINITY;
@@ -538,9 +541,8 @@ struct Cache4 {
         for (int i = 0; i < 2; ++i) {
             const float2 kp = unpack2<T>(w[i].x);
             vp[i] = unpack2<T>(w[i].y);
-            const float step = kp.x * step_scale;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(acc[2 * i + h], step, kp.y * q_sum[h]);
+            for (int h = 0; h < 2; ++h) sc[2 * i + h] = fmaf(acc[2 * i + h], kp.x * step_scale[h], kp.y * q_sum[h]);
         }
     }
     __device__ __forceinline__ int exponent(int h) const { return 127 - static_cast<int>(__float_as_uint(down[h]) >> 23); }   // E

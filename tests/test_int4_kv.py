@@ -388,3 +388,41 @@ def test_a_value_of_a_large_range_without_weight_leaves_the_others_alone(dtype, 
     e = ref.score_error(q[0], np.abs(np.delete(k, place, 0)).max() + 31 * 0.25, scale) + 2.0 ** -20
     most = 15 * (2.0 ** -11 * (p @ step) + 2.0 ** -22 * n * (p * step).max(-1))[:, None] + u * np.abs(want) + 2 * e * (p @ np.abs(v[:, 0]) + np.abs(want)) + 2.0 ** -20
     assert (np.abs(out[0].double().cpu().numpy() - want) <= most).all(), (np.abs(out[0].double().cpu().numpy() - want) / most).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,other", [("bfloat16", "infinite"), ("bfloat16", "large"), ("float16", "infinite"), ("float16", "large")])
+def test_a_query_head_of_other_magnitude_leaves_the_others_alone(dtype, other):
+    """Of a group of four heads one holds an infinity, and another (BF16) elements beyond f16's range; or one is 2^28 (F16: 2^15) times the others."""
+    import torch
+    rng = np.random.default_rng(3)
+    hq, hkv, bs, n, scale = 4, 1, 16, 150, 0.088
+    small = 2.0 ** -12 if dtype == "float16" else 1.0
+    q = _typed(rng, (1, hq, D), dtype, small)
+    key_std = 1.0 / small
+    if other == "infinite":
+        q[0, 2, 77] = np.inf
+        if dtype == "bfloat16":
+            q[0, 0] *= 2.0 ** 18
+            key_std = 2.0 ** -18
+    else:
+        q[0, 2] *= 2.0 ** (15 if dtype == "float16" else 28)
+    key, val = _typed(rng, (160, hkv, D), dtype, key_std), _typed(rng, (160, hkv, D), dtype)
+    (kd, kpar), (vd, vpar) = ref.quantise(key, dtype), ref.quantise(val, dtype)
+    k, v = ref.values(kd, kpar)[:n], ref.values(vd, vpar)[:n]
+    out = torch.empty((1, hq, D), dtype=getattr(torch, dtype), device="cuda")
+    nvk().launch_decode_attention_paged_int4(_dev(q, dtype), torch.from_numpy(kd).cuda(), torch.from_numpy(vd).cuda(), _dev(kpar, dtype), _dev(vpar, dtype),
+                                             to_dev(np.array([n]), torch.int32), to_dev(np.arange(10)[None], torch.int32), hkv, D, bs, scale, out)
+    got, u, step = out[0].double().cpu().numpy(), ref.HALF_STEP[dtype], vpar[:n, 0, 0]
+    for h in range(hq):
+        if h == 2 and other == "infinite":
+            assert np.isnan(got[h]).all()
+            continue
+        want, p = (x[0] for x in ref.attend(q[0, h:h + 1], k, v, scale))
+        # (as above: p' rounded to f16, the result rounded, scores off by e); the large head gives one key everything, by far more than its e
+        e = ref.score_error(q[0, h:h + 1], np.abs(k).max() + 31 * 0.5 * key_std, scale) + 2.0 ** -20
+        if h == 2:
+            top = np.sort(q[0, h] @ k[:, 0].T * scale)
+            assert top[-1] - top[-2] > 4 * e + 200
+            e = 2.0 ** -20
+        assert (np.abs(got[h] - want) <= 15 * 2.0 ** -11 * (p @ step) + u * np.abs(want) + 2 * e * (p @ np.abs(v[:, 0]) + np.abs(want)) + 2.0 ** -20).all(), h
