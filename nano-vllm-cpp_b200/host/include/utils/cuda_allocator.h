@@ -3,8 +3,8 @@
 // DeviceAllocator so that a bump allocator can stand in while a CUDA graph is captured
 // (src/engine/model_runner.cpp:57-100).
 //
-// Unlike the reference's CudaAllocator, the cache here is keyed by (device, bucket) and every entry
-// point takes the lock, so one process can drive several GPUs from one thread per rank.
+// Unlike the reference's CudaAllocator, the cache here is keyed by device and bucket (scratch: by stream as
+// well) and every entry point takes the lock, so one process can drive several GPUs from one thread per rank.
 #pragma once
 
 #include "utils/tensor.h"
@@ -12,7 +12,7 @@
 #include <cstddef>
 #include <map>
 #include <mutex>
-#include <utility>
+#include <tuple>
 #include <vector>
 
 namespace nano_vllm {
@@ -21,18 +21,28 @@ class DeviceAllocator {
 public:
     virtual ~DeviceAllocator() = default;
     virtual Memory::Ptr allocate(size_t bytes, Device device) = 0;
+    // Memory that only work on `stream` uses and that is let go while this work may still be running: scratch of an operator, tensors that a layer
+    // drops when it returns.  What is let go goes to later calls with the same stream only, which its order keeps apart; memory of allocate() goes to anyone,
+    // so that whoever lets it go has to know that nothing uses it any more.  An allocator that does not overload this serves one stream.
+    virtual Memory::Ptr allocate_on(size_t bytes, Device device, cudaStream_t stream) {
+        static_cast<void>(stream);
+        return allocate(bytes, device);
+    }
     virtual void memset_async(void* ptr, int value, size_t bytes, cudaStream_t stream) const = 0;
     virtual void copy_to_device_async(void* dst, const void* src, size_t bytes, cudaStream_t stream) const = 0;
     virtual void copy_to_host_async(void* dst, const void* src, size_t bytes, cudaStream_t stream) const = 0;
     virtual void synchronize_stream(cudaStream_t stream) const = 0;
 };
 
-// Caching cudaMalloc allocator: freed blocks return to a per-(device, bucket) free list.
+// Caching cudaMalloc allocator: freed blocks return to the free list of their device and bucket, scratch to that of its stream too (by the stream's id, which
+// no later stream has again).  Scratch taken during a capture, which the graph uses in every replay, goes to later captures on the same stream only: the graphs that
+// were captured on one stream are replayed one after the other.
 class CudaAllocator final : public DeviceAllocator {
 public:
     static CudaAllocator& instance();
 
     Memory::Ptr allocate(size_t bytes, Device device) override;
+    Memory::Ptr allocate_on(size_t bytes, Device device, cudaStream_t stream) override;
     void memset_async(void* ptr, int value, size_t bytes, cudaStream_t stream) const override;
     void copy_to_device_async(void* dst, const void* src, size_t bytes, cudaStream_t stream) const override;
     void copy_to_host_async(void* dst, const void* src, size_t bytes, cudaStream_t stream) const override;
@@ -43,15 +53,17 @@ public:
 
 private:
     CudaAllocator() = default;
-    static size_t bucket_for(size_t bytes);
-    void recycle(int device_index, size_t bucket, void* ptr);
+    enum Owner { kAnyone, kStream, kCaptures };
+    using Key = std::tuple<int, Owner, unsigned long long, size_t>;   // device, who may have it, the stream, bucket
+    Memory::Ptr take(const Key& key, size_t bytes, Device device);
+    void recycle(const Key& key, void* ptr);
 
     mutable std::mutex mutex_;
-    std::map<std::pair<int, size_t>, std::vector<void*>> free_lists_;
+    std::map<Key, std::vector<void*>> free_lists_;
 };
 
 // Bump allocator over one device range reserved up front: nothing it hands out is ever freed individually, reset()
-// rewinds it.  A CUDA graph is captured with one of these in place of the caching allocator, so that no cudaMalloc runs
+// rewinds it.  It serves one stream.  A CUDA graph is captured with one of these in place of the caching allocator, so that no cudaMalloc runs
 // under capture and a warm-up pass and the capture pass receive identical addresses (the role of ScratchAllocator in
 // src/engine/model_runner.cpp:57-100 of the reference).  Copies and memsets are forwarded to `delegate`.
 class ArenaAllocator final : public DeviceAllocator {

@@ -65,6 +65,8 @@ public:
     Tensor() = default;
 
     static Tensor empty(const std::vector<int64_t>& sizes, ScalarType dtype, Device device, DeviceAllocator& allocator);
+    // For work on `stream` only, which may still run when the tensor is let go (DeviceAllocator::allocate_on).
+    static Tensor scratch(const std::vector<int64_t>& sizes, ScalarType dtype, Device device, DeviceAllocator& allocator, cudaStream_t stream);
     static Tensor zeros(const std::vector<int64_t>& sizes, ScalarType dtype, Device device, DeviceAllocator& allocator,
                         cudaStream_t stream = nullptr);
     static Tensor from_memory(const Memory::Ptr& memory, const std::vector<int64_t>& sizes, ScalarType dtype,

@@ -328,12 +328,12 @@ void decode_common(const Tensor& query, const Tensor& k_cache, const Tensor& v_c
     const int64_t blocks = cache_blocks(k_cache, block_size, num_kv_heads, head_dim);
     if (allocator != nullptr) {
         const size_t need = nvk::decode_mma_workspace_needed(batch, heads, num_kv_heads, head_dim, max_blocks, block_size);
-        Memory::Ptr scratch = need > 0 ? allocator->allocate(need, query.device()) : nullptr;
+        Memory::Ptr scratch = need > 0 ? allocator->allocate_on(need, query.device(), stream) : nullptr;
         throw_on_nvk_status(nvk_decode_attention_paged(query.data(), k_cache.data(), v_cache.data(), lens.ptr, lens.dtype,
                                                        tables.ptr, tables.dtype, batch, max_blocks, blocks, heads,
                                                        num_kv_heads, head_dim, block_size, scale, output.data(),
                                                        code(query.dtype()), scratch ? scratch->data() : nullptr, need, stream));
-        return;   // the scratch block returns to the allocator's cache; stream order keeps it valid for this launch
+        return;   // the scratch goes to later calls on this stream, whose order keeps it valid for this launch
     }
     const size_t need = nvk::decode_mma_workspace_needed(batch, heads, num_kv_heads, head_dim, max_blocks, block_size);
     if (need > 0 && need <= nvk_decode_attention_static_scratch_bytes()) {
@@ -448,7 +448,7 @@ void launch_decode_attention_paged_int4(const Tensor& query, const Tensor& k_cac
                                         float scale, Tensor& output, DeviceAllocator& allocator, cudaStream_t stream) {
     const Step s(query, output, k_cache, v_cache, k_params, v_params, true, context_lens, block_tables, num_kv_heads, head_dim, block_size);
     const size_t need = nvk::decode_mma_workspace_needed(s.batch, s.heads, num_kv_heads, head_dim, s.max_blocks, block_size);
-    Memory::Ptr scratch = need > 0 ? allocator.allocate(need, query.device()) : nullptr;
+    Memory::Ptr scratch = need > 0 ? allocator.allocate_on(need, query.device(), stream) : nullptr;
     throw_on_nvk_status(nvk_decode_attention_paged_int4(query.data(), k_cache.data(), v_cache.data(), k_params.data(), v_params.data(), s.lens.ptr, s.lens.dtype,
                                                         s.tables.ptr, s.tables.dtype, s.batch, s.max_blocks, s.blocks, s.heads, num_kv_heads, head_dim,
                                                         block_size, scale, output.data(), code(query.dtype()), scratch ? scratch->data() : nullptr, need, stream));
@@ -478,7 +478,7 @@ void launch_decode_attention_paged_weights(const Tensor& query, const Tensor& k_
         ensure_same_device("query", query, "weight_rows", weight_rows);
     }
     const size_t need = nvk_decode_attention_weights_workspace_bytes(s.batch, s.heads, num_kv_heads, head_dim, s.max_blocks, block_size);
-    Memory::Ptr scratch = need > 0 ? allocator.allocate(need, query.device()) : nullptr;
+    Memory::Ptr scratch = need > 0 ? allocator.allocate_on(need, query.device(), stream) : nullptr;
     throw_on_nvk_status(nvk_decode_attention_paged_weights(
         query.data(), k_cache.data(), v_cache.data(), four ? k_params.data() : nullptr, four ? v_params.data() : nullptr, s.lens.ptr, s.lens.dtype, s.tables.ptr,
         s.tables.dtype, s.batch, s.max_blocks, s.blocks, s.heads, num_kv_heads, head_dim, block_size, scale,

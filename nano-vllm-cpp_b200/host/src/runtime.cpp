@@ -6,6 +6,7 @@
 
 #include <cuda_runtime_api.h>
 
+#include <cstdint>
 #include <stdexcept>
 #include <string>
 
@@ -44,41 +45,71 @@ CudaAllocator& CudaAllocator::instance() {
     return allocator;
 }
 
+namespace {
+
 // 512-byte granules up to 1 MiB, 2 MiB granules above: few distinct buckets, bounded waste.
-size_t CudaAllocator::bucket_for(size_t bytes) {
+size_t bucket_for(size_t bytes) {
     if (bytes == 0) bytes = 1;
     const size_t granule = bytes <= (size_t(1) << 20) ? 512 : (size_t(2) << 20);
     return (bytes + granule - 1) / granule * granule;
 }
+// Scratch follows the lengths of a step's contexts: powers of two above 1 MiB, so that all of one stream's buckets together are at most four times the largest request.
+size_t scratch_bucket_for(size_t bytes) {
+    if (bytes <= (size_t(1) << 20)) return bucket_for(bytes);
+    size_t bucket = size_t(2) << 20;
+    while (bucket < bytes) bucket *= 2;
+    return bucket;
+}
+
+}  // namespace
 
 Memory::Ptr CudaAllocator::allocate(size_t bytes, Device device) {
     if (device.type != DeviceType::kCUDA) throw std::invalid_argument("CudaAllocator only serves CUDA devices");
-    const size_t bucket = bucket_for(bytes);
+    return take(Key(device.index, kAnyone, 0, bucket_for(bytes)), bytes, device);
+}
+
+Memory::Ptr CudaAllocator::allocate_on(size_t bytes, Device device, cudaStream_t stream) {
+    if (device.type != DeviceType::kCUDA) throw std::invalid_argument("CudaAllocator only serves CUDA devices");
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    throw_if_cuda_error(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
+    const bool captured = capture != cudaStreamCaptureStatusNone;
+    unsigned long long id = reinterpret_cast<uintptr_t>(stream);
+    if (!captured) throw_if_cuda_error(cudaStreamGetId(stream, &id), "cudaStreamGetId");   // (not to be had during a capture)
+    return take(Key(device.index, captured ? kCaptures : kStream, id, scratch_bucket_for(bytes)), bytes, device);
+}
+
+Memory::Ptr CudaAllocator::take(const Key& key, size_t bytes, Device device) {
     void* ptr = nullptr;
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        auto it = free_lists_.find({device.index, bucket});
+        auto it = free_lists_.find(key);
         if (it != free_lists_.end() && !it->second.empty()) {
             ptr = it->second.back();
             it->second.pop_back();
         }
     }
     if (ptr == nullptr) {
-        with_device(device.index, [&] { throw_if_cuda_error(cudaMalloc(&ptr, bucket), "cudaMalloc"); });
+        with_device(device.index, [&] {
+            // (a stream that is being captured may find its list empty: cudaMalloc is allowed then in this mode)
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            throw_if_cuda_error(cudaThreadExchangeStreamCaptureMode(&mode), "cudaThreadExchangeStreamCaptureMode");
+            const cudaError_t status = cudaMalloc(&ptr, std::get<3>(key));
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            throw_if_cuda_error(status, "cudaMalloc");
+        });
     }
-    const int index = device.index;
-    return Memory::make_owned(ptr, bytes, device, [this, index, bucket](void* p) { recycle(index, bucket, p); });
+    return Memory::make_owned(ptr, bytes, device, [this, key](void* p) { recycle(key, p); });
 }
 
-void CudaAllocator::recycle(int device_index, size_t bucket, void* ptr) {
+void CudaAllocator::recycle(const Key& key, void* ptr) {
     std::lock_guard<std::mutex> lock(mutex_);
-    free_lists_[{device_index, bucket}].push_back(ptr);
+    free_lists_[key].push_back(ptr);
 }
 
 void CudaAllocator::trim() {
     std::lock_guard<std::mutex> lock(mutex_);
     for (auto& entry : free_lists_) {
-        const int index = entry.first.first;
+        const int index = std::get<0>(entry.first);
         for (void* ptr : entry.second) {
             with_device(index, [&] { cudaFree(ptr); });
         }

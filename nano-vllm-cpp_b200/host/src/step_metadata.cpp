@@ -173,7 +173,7 @@ ModelInputs StepUploader::upload(const StepArrays& a, cudaStream_t stream) {
     for (int i = 0; i < 7; ++i) {
         if (!pieces[i]->empty()) std::memcpy(host + offsets[i], pieces[i]->data(), pieces[i]->size() * sizeof(int32_t));
     }
-    Tensor packed = Tensor::empty({static_cast<int64_t>(total)}, ScalarType::kInt32, device_, allocator_);
+    Tensor packed = Tensor::scratch({static_cast<int64_t>(total)}, ScalarType::kInt32, device_, allocator_, stream);   // (the next step's replaces it)
     allocator_.copy_to_device_async(packed.data(), host, bytes, stream);
     throw_if_cuda_error(cudaEventRecord(st.done, stream), "cudaEventRecord (metadata staging)");
     st.in_flight = true;

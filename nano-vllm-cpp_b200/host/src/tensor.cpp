@@ -70,6 +70,10 @@ Tensor Tensor::empty(const std::vector<int64_t>& sizes, ScalarType dtype, Device
     return Tensor(std::move(memory), sizes, make_contiguous_strides(sizes), dtype, 0);
 }
 
+Tensor Tensor::scratch(const std::vector<int64_t>& sizes, ScalarType dtype, Device device, DeviceAllocator& allocator, cudaStream_t stream) {
+    return from_memory(allocator.allocate_on(compute_numel(sizes) * scalar_type_size(dtype), device, stream), sizes, dtype);
+}
+
 Tensor Tensor::zeros(const std::vector<int64_t>& sizes, ScalarType dtype, Device device, DeviceAllocator& allocator,
                      cudaStream_t stream) {
     Tensor t = empty(sizes, dtype, device, allocator);

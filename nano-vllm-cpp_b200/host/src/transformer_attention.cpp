@@ -82,7 +82,7 @@ Tensor TransformerAttention::forward(const Tensor& positions, const Tensor& qkv,
     if (qkv.dim() != 2 || qkv.sizes()[1] != static_cast<int64_t>(num_heads_ + 2 * num_kv_heads_) * head_dim_)
         throw std::invalid_argument("qkv must be [rows, (num_heads + 2 * num_kv_heads) * head_dim]");
     const int64_t rows = qkv.sizes()[0];
-    Tensor q = Tensor::empty({rows, num_heads_, head_dim_}, qkv.dtype(), qkv.device(), allocator);
+    Tensor q = Tensor::scratch({rows, num_heads_, head_dim_}, qkv.dtype(), qkv.device(), allocator, stream);
     last_fused_ = fused_eligible(qkv);
     if (last_fused_) {
         const Context& ctx = get_context();
@@ -91,8 +91,8 @@ Tensor TransformerAttention::forward(const Tensor& positions, const Tensor& qkv,
                                     q, stream);
         return attn_.forward_decode_flash_only(q, allocator, stream);
     }
-    Tensor k = Tensor::empty({rows, num_kv_heads_, head_dim_}, qkv.dtype(), qkv.device(), allocator);
-    Tensor v = Tensor::empty({rows, num_kv_heads_, head_dim_}, qkv.dtype(), qkv.device(), allocator);
+    Tensor k = Tensor::scratch({rows, num_kv_heads_, head_dim_}, qkv.dtype(), qkv.device(), allocator, stream);
+    Tensor v = Tensor::scratch({rows, num_kv_heads_, head_dim_}, qkv.dtype(), qkv.device(), allocator, stream);
     split_norm_rope(qkv, positions, q_norm_weight_, k_norm_weight_, norm_eps_, cos_sin_cache_, num_heads_, num_kv_heads_,
                     head_dim_, q, k, v, stream);
     return attn_.forward(q, k, v, allocator, stream);

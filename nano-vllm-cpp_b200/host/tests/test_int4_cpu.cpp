@@ -3,8 +3,10 @@
 #include "check.h"
 
 #include "kernels/attention.h"
+#include "kernels/flash_attn.h"
 #include "kernels/kvcache.h"
 #include "layers/attention.h"
+#include "utils/context.h"
 #include "utils/cuda_allocator.h"
 
 #include <stdexcept>
@@ -140,6 +142,46 @@ TEST_CASE(layer_refuses) {
     CHECK(attention.is_int4() && attention.is_quantised() && !attention.is_int8());
     attention.set_kv_cache(c.key, c.key);
     CHECK(!attention.is_quantised());
+}
+
+namespace {
+
+// Scratch is asked for by stream; the first request ends the call.
+struct Asked {};
+class StreamAllocator final : public NoAllocator {
+public:
+    Memory::Ptr allocate(size_t bytes, Device device) override { return Memory::make_borrowed(reinterpret_cast<void*>(uintptr_t(1) << 40), bytes, device); }
+    Memory::Ptr allocate_on(size_t bytes, Device, cudaStream_t stream) override {
+        last = stream;
+        size = bytes;
+        throw Asked();
+    }
+    cudaStream_t last = nullptr;
+    size_t size = 0;
+};
+
+}  // namespace
+
+TEST_CASE(scratch_belongs_to_the_stream_of_the_call) {
+    Case c;
+    StreamAllocator alloc;
+    const cudaStream_t stream = reinterpret_cast<cudaStream_t>(uintptr_t(0x77));
+    Tensor tables = borrowed({1, 512}, ScalarType::kInt32), weights = borrowed({1, 2, 8192}, ScalarType::kFloat32), full = borrowed({2, 16, 2, 128}, ScalarType::kBFloat16);
+    auto asks = [&](auto call) {
+        alloc.last = nullptr;
+        CHECK_THROWS(call(), Asked);
+        CHECK(alloc.last == stream && alloc.size > 0);
+    };
+    asks([&] { launch_decode_attention_paged_int4(c.query, c.k_cache, c.v_cache, c.params, c.params, c.lens, tables, 2, 128, 16, 1.0f, c.output, alloc, stream); });
+    asks([&] { launch_decode_attention_paged_weights(c.query, c.k_cache, c.v_cache, c.params, c.params, c.lens, tables, 2, 128, 16, 1.0f, c.none, c.none, weights, c.output, alloc, stream); });
+    asks([&] { launch_decode_attention_paged_weights(c.query, full, full, c.none, c.none, c.lens, tables, 2, 128, 16, 1.0f, c.none, c.none, weights, c.output, alloc, stream); });
+    asks([&] { flash_attn_decode_kvcache(c.query, full, full, c.lens, tables, 2, 128, 16, 1.0f, c.output, alloc, stream); });
+    Attention layer(4, 2, 128, 16);
+    layer.set_kv_cache_int4(c.k_cache, c.v_cache, c.params, c.params);
+    const Tensor cu = borrowed({2}, ScalarType::kInt32), q = borrowed({3, 4, 128}, ScalarType::kBFloat16);
+    set_context(true, cu, cu, 3, 20, Tensor(), Tensor(), borrowed({1, 2}, ScalarType::kInt32));
+    asks([&] { layer.forward(q, c.key, c.key, alloc, stream); });
+    reset_context();
 }
 
 int main() { return check::run_all(); }

@@ -146,6 +146,84 @@ TEST_CASE(evict_keeps_the_first_the_last_and_the_heaviest) {
     }
 }
 
+TEST_CASE(scratch_of_one_stream_does_not_go_to_another) {
+    CudaAllocator& alloc = CudaAllocator::instance();
+    cudaStream_t a = nullptr, b = nullptr;
+    throw_if_cuda_error(cudaStreamCreateWithFlags(&a, cudaStreamNonBlocking), "cudaStreamCreate");
+    throw_if_cuda_error(cudaStreamCreateWithFlags(&b, cudaStreamNonBlocking), "cudaStreamCreate");
+    const size_t bytes = 5 << 20;
+    void* first = alloc.allocate_on(bytes, kDev, a)->data();
+    CHECK(alloc.allocate_on(bytes, kDev, b)->data() != first);
+    CHECK(alloc.allocate_on(bytes, kDev, nullptr)->data() != first);
+    CHECK(alloc.allocate(bytes, kDev)->data() != first);
+    CHECK(alloc.allocate_on(bytes - 1000, kDev, a)->data() == first);
+    // a stream that is being captured, with nothing in its list
+    cudaStream_t c = nullptr;
+    throw_if_cuda_error(cudaStreamCreateWithFlags(&c, cudaStreamNonBlocking), "cudaStreamCreate");
+    throw_if_cuda_error(cudaStreamBeginCapture(c, cudaStreamCaptureModeGlobal), "cudaStreamBeginCapture");
+    void* captured = nullptr;
+    {
+        const Memory::Ptr m = alloc.allocate_on(bytes, kDev, c);
+        alloc.memset_async(m->data(), 0, bytes, c);
+        captured = m->data();
+    }
+    CHECK(alloc.allocate_on(bytes, kDev, c)->data() == captured);
+    CHECK(alloc.allocate_on(bytes, kDev, a)->data() == first);   // (the others go on)
+    CHECK(alloc.allocate_on(3 * bytes, kDev, b)->data() != nullptr);
+    cudaGraph_t graph = nullptr;
+    throw_if_cuda_error(cudaStreamEndCapture(c, &graph), "cudaStreamEndCapture");
+    CHECK(alloc.allocate_on(bytes, kDev, c)->data() != captured);   // (the graph's)
+    throw_if_cuda_error(cudaGraphDestroy(graph), "cudaGraphDestroy");
+    for (cudaStream_t s : {a, b, c}) throw_if_cuda_error(cudaStreamDestroy(s), "cudaStreamDestroy");
+}
+
+TEST_CASE(two_streams_that_share_the_allocator_give_what_one_gives) {
+    CudaAllocator& alloc = CudaAllocator::instance();
+    const int batch = 24, width = 128, blocks = 256, keys = width * kBlock;   // chunks and a merge
+    cudaStream_t streams[2];
+    struct Side { Tensor query, k, v, lens, tables; } side[2];
+    for (int i = 0; i < 2; ++i) {
+        throw_if_cuda_error(cudaStreamCreateWithFlags(&streams[i], cudaStreamNonBlocking), "cudaStreamCreate");
+        std::vector<int32_t> lens, tables;
+        for (int b = 0; b < batch; ++b) lens.push_back(1 + static_cast<int32_t>(next_random() % keys));
+        for (int b = 0; b < batch * width; ++b) tables.push_back(static_cast<int32_t>(next_random() % blocks));
+        side[i] = {queries(batch), numbers(blocks * kBlock), numbers(blocks * kBlock), ints({batch}, lens), ints({batch, width}, tables)};
+    }
+    const Tensor none;
+    const int rounds = 20;
+    std::vector<float> out[2][2], sum[2][2];   // [in turn | at once][side]
+    for (int way = 0; way < 2; ++way) {
+        Tensor outs[2], weights[2];
+        for (int i = 0; i < 2; ++i) {
+            outs[i] = Tensor::zeros({batch, kHeads, kDim}, ScalarType::kBFloat16, kDev, alloc);
+            weights[i] = Tensor::zeros({batch, kKvHeads, keys}, ScalarType::kFloat32, kDev, alloc);
+        }
+        throw_if_cuda_error(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+        auto step = [&](int i) {
+            launch_decode_attention_paged_weights(side[i].query, side[i].k, side[i].v, none, none, side[i].lens, side[i].tables, kKvHeads, kDim, kBlock, 0.1f, weights[i], none,
+                                                  weights[i], outs[i], alloc, streams[i]);
+        };
+        if (way == 0) {
+            for (int i = 0; i < 2; ++i) {
+                for (int r = 0; r < rounds; ++r) step(i);
+                alloc.synchronize_stream(streams[i]);
+            }
+        } else {
+            for (int r = 0; r < rounds; ++r) { step(0); step(1); }
+        }
+        throw_if_cuda_error(cudaDeviceSynchronize(), "cudaDeviceSynchronize");
+        for (int i = 0; i < 2; ++i) {
+            out[way][i] = floats(outs[i]);
+            sum[way][i] = download<float>(weights[i]);
+        }
+    }
+    for (int i = 0; i < 2; ++i) {
+        CHECK(out[0][i] == out[1][i]);
+        CHECK(sum[0][i] == sum[1][i]);
+        throw_if_cuda_error(cudaStreamDestroy(streams[i]), "cudaStreamDestroy");
+    }
+}
+
 int main() {
     int count = 0;
     if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
