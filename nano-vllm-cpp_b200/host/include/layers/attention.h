@@ -18,7 +18,8 @@ public:
 
     // 4-bit caches [blocks, block_size, Hkv, 64] (byte tensors, int8) with pairs (step, low) [blocks, block_size, Hkv, 2] in the model's type: new K / V are
     // quantised on store, decode reads them through launch_decode_attention_paged_int4, and a prefill with block tables over the rows that
-    // gather_kvcache_int4 brings out of them (prefix hits, chunks), in memory from the allocator: rows for max_seqlen_k keys of every sequence.
+    // gather_kvcache_int4 brings out of them (prefix hits, chunks), in scratch from the allocator: total_seqlen_k rows where the context has it (StepUploader
+    // sets it), otherwise max_seqlen_k of every sequence.
     void set_kv_cache_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params);
     // From here on decode steps over a 16-bit or a 4-bit cache add every key's attention weights to `key_weights` [rows, Hkv, keys], float32, for
     // evict_kvcache; `rows` [batch] or undefined, as there.  Undefined weights: no longer.

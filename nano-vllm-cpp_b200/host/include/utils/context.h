@@ -16,6 +16,7 @@ struct Context {
     Tensor slot_mapping;   // [tokens] int32, -1 = padding
     Tensor context_lens;   // [batch] int32, decode (includes the token being generated)
     Tensor block_tables;   // [batch, max_blocks] int32, zero padded
+    int64_t total_seqlen_k = 0;   // the last element of cu_seqlens_k, prefill; 0: the host does not know it (not in the reference)
 };
 
 Context& get_context();
@@ -27,7 +28,8 @@ void set_context(bool is_prefill,
                  int max_seqlen_k = 0,
                  const Tensor& slot_mapping = Tensor(),
                  const Tensor& context_lens = Tensor(),
-                 const Tensor& block_tables = Tensor());
+                 const Tensor& block_tables = Tensor(),
+                 int64_t total_seqlen_k = 0);
 void reset_context();
 
 }  // namespace nano_vllm

@@ -147,7 +147,8 @@ Tensor Attention::forward(const Tensor& query, const Tensor& key, const Tensor& 
             if (cu_q == nullptr || cu_k == nullptr) throw std::invalid_argument("prefill attention with block_tables requires cu_seqlens_q and cu_seqlens_k");
             const int64_t seqs = static_cast<int64_t>(cu_k->numel()) - 1;
             const int64_t longest = ctx.max_seqlen_k > 0 ? ctx.max_seqlen_k : ctx.block_tables.sizes().back() * block_size_;
-            Tensor dense_k = Tensor::scratch({seqs * longest, num_kv_heads_, head_dim_}, query.dtype(), query.device(), allocator, stream);
+            const int64_t rows = ctx.total_seqlen_k > 0 ? ctx.total_seqlen_k : seqs * longest;   // (what is behind the last sequence is written as zeros)
+            Tensor dense_k = Tensor::scratch({rows, num_kv_heads_, head_dim_}, query.dtype(), query.device(), allocator, stream);
             Tensor dense_v = Tensor::scratch(dense_k.sizes(), query.dtype(), query.device(), allocator, stream);
             gather_kvcache_int4(k_cache_, v_cache_, k_scale_, v_scale_, *cu_k, ctx.block_tables, num_kv_heads_, head_dim_, block_size_, dense_k, dense_v, stream);
             launch_prefill_attention_dense(query, cu_q, dense_k, dense_v, cu_k, num_kv_heads_, head_dim_, scale_, output, stream, ctx.max_seqlen_q);

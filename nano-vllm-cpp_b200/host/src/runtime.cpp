@@ -195,7 +195,8 @@ Context& get_context() { return t_context; }
 void set_context(const Context& context) { t_context = context; }
 
 void set_context(bool is_prefill, const Tensor& cu_seqlens_q, const Tensor& cu_seqlens_k, int max_seqlen_q,
-                 int max_seqlen_k, const Tensor& slot_mapping, const Tensor& context_lens, const Tensor& block_tables) {
+                 int max_seqlen_k, const Tensor& slot_mapping, const Tensor& context_lens, const Tensor& block_tables,
+                 int64_t total_seqlen_k) {
     Context& c = t_context;
     c.is_prefill = is_prefill;
     c.cu_seqlens_q = cu_seqlens_q;
@@ -205,6 +206,7 @@ void set_context(bool is_prefill, const Tensor& cu_seqlens_q, const Tensor& cu_s
     c.slot_mapping = slot_mapping;
     c.context_lens = context_lens;
     c.block_tables = block_tables;
+    c.total_seqlen_k = total_seqlen_k;
 }
 
 void reset_context() { t_context = Context{}; }

@@ -184,4 +184,23 @@ TEST_CASE(scratch_belongs_to_the_stream_of_the_call) {
     reset_context();
 }
 
+TEST_CASE(a_prefill_takes_rows_for_the_keys_that_there_are) {
+    Case c;
+    StreamAllocator alloc;
+    Attention layer(4, 2, 128, 16);
+    layer.set_kv_cache_int4(c.k_cache, c.v_cache, c.params, c.params);
+    const Tensor cu = borrowed({33}, ScalarType::kInt32), tables = borrowed({32, 2048}, ScalarType::kInt32), q = borrowed({3, 4, 128}, ScalarType::kBFloat16);
+    const size_t row = 2 * 128 * sizeof(uint16_t);
+    auto rows = [&](int longest, int64_t total) {   // one sequence of 32768 keys among 31 of 100
+        set_context(true, cu, cu, 3, longest, Tensor(), Tensor(), tables, total);
+        CHECK_THROWS(layer.forward(q, c.key, c.key, alloc), Asked);
+        reset_context();
+        return static_cast<int64_t>(alloc.size / row);
+    };
+    CHECK_EQ(rows(32768, 32768 + 31 * 100), 32768 + 31 * 100);
+    CHECK_EQ(rows(0, 32768 + 31 * 100), 32768 + 31 * 100);
+    CHECK_EQ(rows(1000, 0), 32 * 1000);     // not known: as many for each as the longest has
+    CHECK_EQ(rows(0, 0), 32 * 2048 * 16);   // or as the table could hold
+}
+
 int main() { return check::run_all(); }

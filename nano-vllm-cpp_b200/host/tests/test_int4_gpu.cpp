@@ -2,6 +2,7 @@
 // which a 4-bit cache holds exactly: step 1, low 0; the layer over it and the layer over a 16-bit cache then attend over the same numbers.
 #include "check.h"
 
+#include "engine/step_metadata.h"
 #include "kernels/attention.h"
 #include "kernels/kvcache.h"
 #include "layers/attention.h"
@@ -222,6 +223,76 @@ TEST_CASE(two_streams_that_share_the_allocator_give_what_one_gives) {
         CHECK(sum[0][i] == sum[1][i]);
         throw_if_cuda_error(cudaStreamDestroy(streams[i]), "cudaStreamDestroy");
     }
+}
+
+namespace {
+
+// CudaAllocator that counts the scratch asked for.
+class CountingAllocator final : public DeviceAllocator {
+public:
+    Memory::Ptr allocate(size_t bytes, Device device) override { return inner.allocate(bytes, device); }
+    Memory::Ptr allocate_on(size_t bytes, Device device, cudaStream_t stream) override {
+        scratch += bytes;
+        return inner.allocate_on(bytes, device, stream);
+    }
+    void memset_async(void* p, int value, size_t bytes, cudaStream_t stream) const override { inner.memset_async(p, value, bytes, stream); }
+    void copy_to_device_async(void* dst, const void* src, size_t bytes, cudaStream_t stream) const override { inner.copy_to_device_async(dst, src, bytes, stream); }
+    void copy_to_host_async(void* dst, const void* src, size_t bytes, cudaStream_t stream) const override { inner.copy_to_host_async(dst, src, bytes, stream); }
+    void synchronize_stream(cudaStream_t stream) const override { inner.synchronize_stream(stream); }
+    CudaAllocator& inner = CudaAllocator::instance();
+    size_t scratch = 0;
+};
+
+}  // namespace
+
+TEST_CASE(chunks_of_prompts_of_unequal_lengths_over_a_4_bit_cache) {
+    // prompts of 500 and of a few tokens, the first ones cached; the second step has a longer chunk of each
+    CountingAllocator alloc;
+    const std::vector<int> lens = {500, 3, 40, 17, 16, 100};
+    Attention four(kHeads, kKvHeads, kDim, kBlock), full(kHeads, kKvHeads, kDim, kBlock);
+    const int blocks = 64;
+    four.set_kv_cache_int4(Tensor::zeros({blocks, kBlock, kKvHeads, kDim / 2}, ScalarType::kInt8, kDev, alloc),
+                           Tensor::zeros({blocks, kBlock, kKvHeads, kDim / 2}, ScalarType::kInt8, kDev, alloc),
+                           Tensor::zeros({blocks, kBlock, kKvHeads, 2}, ScalarType::kBFloat16, kDev, alloc),
+                           Tensor::zeros({blocks, kBlock, kKvHeads, 2}, ScalarType::kBFloat16, kDev, alloc));
+    full.set_kv_cache(Tensor::zeros({blocks, kBlock, kKvHeads, kDim}, ScalarType::kBFloat16, kDev, alloc),
+                      Tensor::zeros({blocks, kBlock, kKvHeads, kDim}, ScalarType::kBFloat16, kDev, alloc));
+    std::vector<int32_t> tokens(500, 1);
+    std::vector<std::vector<int32_t>> tables;
+    std::vector<SequenceView> seqs;
+    int next = 0;
+    for (int n : lens) {
+        std::vector<int32_t> table;
+        for (int i = 0; i < (n + kBlock - 1) / kBlock; ++i) table.push_back(next++ * 37 % blocks);
+        tables.push_back(table);
+    }
+    CHECK(next <= blocks);
+    for (size_t i = 0; i < lens.size(); ++i) {
+        SequenceView s;
+        s.token_ids = tokens.data();
+        s.num_tokens = lens[i];
+        s.block_table = tables[i].data();
+        s.block_table_len = static_cast<int32_t>(tables[i].size());
+        seqs.push_back(s);
+    }
+    StepUploader uploader(alloc, kDev);
+    for (int part = 0; part < 2; ++part) {
+        for (size_t i = 0; i < lens.size(); ++i) {
+            seqs[i].num_computed_tokens = part == 0 ? 0 : (lens[i] + 1) / 3;
+            seqs[i].num_tokens_to_process = part == 0 ? (lens[i] + 1) / 3 : lens[i] - (lens[i] + 1) / 3;
+        }
+        const StepArrays step = build_prefill_arrays(seqs, kBlock);
+        uploader.upload(step);
+        CHECK_EQ(get_context().total_seqlen_k, static_cast<int64_t>(step.cu_seqlens_k.back()));
+        const int rows = static_cast<int>(step.input_ids.size());
+        const Tensor q = queries(rows), k = numbers(rows), v = numbers(rows);
+        alloc.scratch = 0;
+        const Tensor out = four.forward(q, k, v, alloc);
+        if (part == 1) CHECK_EQ(alloc.scratch, static_cast<size_t>(2 * 676 * kKvHeads * kDim * 2));
+        check_close(out, full.forward(q, k, v, alloc));
+    }
+    throw_if_prefill_error();
+    reset_context();
 }
 
 int main() {
