@@ -394,7 +394,8 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     p.block_size = a.block_size;
     p.scale_log2 = a.scale * kLog2e;
     p.beside = a.beside ? 1 : 0;
-    if (a.batch * a.num_heads * kMaxCluster >= (1LL << 31) || a.max_blocks * a.block_size >= (1LL << 31) - kTileTokens * kMaxCluster)
+    const int64_t ahead = four_bits ? Cache4<__half>::kKeysAhead : kTileTokens * kMaxCluster;   // how far numbers of keys go beyond the last one
+    if (a.batch * a.num_heads * kMaxCluster >= (1LL << 31) || a.max_blocks * a.block_size >= (1LL << 31) - ahead)
         return fail(NVK_ERR_UNSUPPORTED, "decode attention: batch or block table too large");
     const Splits s = choose_splits(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size, groups, a.workspace != nullptr, four_bits);
     *cluster = s.cluster;

@@ -458,6 +458,7 @@ struct Cache4 {
     static constexpr int kSplitBlocks = 16 / WARPS;           // in chunks: the registers are there, and the chains are what a warp waits for
     static constexpr int kRowBytes = kHeadDim / 2;
     static constexpr int kKeys = 32;                          // of a stage
+    static constexpr int kKeysAhead = 32 * 8 * kKeys + 16;    // two windows of 16 tiles, of eight warps at most, and a half: how far `run` counts beyond the last key
     static constexpr int kTileBytes = kKeys * kRowBytes;
     static constexpr int kStageBytes = 2 * kTileBytes + 2 * kKeys * 4;   // K, V, (step, low) of K and of V
     static constexpr int kStages = 3;

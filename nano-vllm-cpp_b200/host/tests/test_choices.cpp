@@ -125,4 +125,25 @@ TEST_CASE(decode_workspace_of_the_largest_call_is_enough_for_smaller_ones) {
     }
 }
 
+// Over a 4-bit cache a warp looks up to 32 strides of 256 keys ahead of the last one: their numbers have to stay below 2^31.
+TEST_CASE(a_4_bit_step_refuses_tables_whose_keys_leave_32_bits_ahead_of_the_end) {
+    static char buffer[64] __attribute__((aligned(64)));
+    alignas(16) static unsigned char room[4096];   // (the parameters themselves are not looked at)
+    auto plan = [&](int64_t keys, bool four_bits) {
+        DecodeArgs a{};
+        a.q = a.k_cache = a.v_cache = a.out = buffer;
+        a.context_lens = a.block_tables = IndexArray(buffer, 0);
+        a.batch = 1; a.max_blocks = keys / 16; a.num_cache_blocks = 4096; a.num_heads = 4; a.num_kv_heads = 1; a.head_dim = 128; a.block_size = 16;
+        a.scale = 0.088f; a.dtype = NVK_BF16;
+        int size = 0;
+        return decode_plan(a, 3, reinterpret_cast<dec::DecodeParams*>(room), &size, four_bits);
+    };
+    constexpr int64_t kEnd = int64_t{1} << 31, kAhead = 31 * 256 + 32 + 16;
+    CHECK_EQ(plan(kEnd - 16, true), NVK_ERR_UNSUPPORTED);
+    CHECK_EQ(plan(kEnd - 4096, true), NVK_ERR_UNSUPPORTED);
+    CHECK_EQ(plan(kEnd - kAhead / 16 * 16 + 16, true), NVK_ERR_UNSUPPORTED);
+    CHECK_EQ(plan(kEnd - 16384, true), NVK_OK);
+    CHECK_EQ(plan(kEnd - 4096, false), NVK_OK);
+}
+
 int main() { return check::run_all(); }
