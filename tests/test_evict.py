@@ -538,3 +538,44 @@ def test_calls_on_two_streams_at_once_do_not_touch_each_other():
     for x, y in zip(alone, at_once):
         assert torch.equal(x["out"], y["out"]) and torch.equal(x["w"], y["w"]) and torch.equal(x["ctx"], y["ctx"])
         assert all(torch.equal(a, c) for a, c in zip(x["cache"], y["cache"])) and not torch.isnan(x["out"]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,dtype,hkv,bs,lens,budget,sinks,recent,tables_are,weights_are", [
+    ("same", "bfloat16", 2, 256, [46500], 20000, 4, 256, "same", "same"),                  # more keys than orders are kept of, alone on an SM
+    ("int4", "float16", 1, 16, [45057, 46000], 45056, 0, 0, "same", "same"),
+    ("int4", "bfloat16", 25, 256, [16385, 17000, 16700], 9000, 4, 1000, "same", "same"),   # and by two blocks to an SM
+    ("int4", "bfloat16", 1, 256, [140000], 66000, 4, 128, "other", "other"),               # several tiles counted together
+    ("same", "float16", 1, 256, [133000], 131080, 0, 1, "other", "same"),
+    ("int4", "bfloat16", 2, 256, [140000], 139990, 100, 100, "same", "same"),
+    ("same", "bfloat16", 2, 16, [700, 90, 1, 333], 100, 2, 30, "same", "other"),
+    ("int4", "bfloat16", 2, 16, [700, 90, 1, 333], 100, 2, 30, "other", "same"),
+    ("same", "float16", 2, 16, [700, 90, 1, 333], 100, 2, 30, "first", "same"),            # the first blocks of the old ones, as a narrower table
+    ("int4", "bfloat16", 8, 48, [3000, 2000], 3000, 0, 0, "same", "same"),                 # nothing to do
+])
+def test_evict_in_place_and_of_long_contexts(kv, dtype, hkv, bs, lens, budget, sinks, recent, tables_are, weights_are):
+    import torch
+    rng = np.random.default_rng(budget + hkv)
+    b = len(lens)
+    kept = [min(n, budget) for n in lens]
+    blocks = sum(-(-n // bs) for n in lens) + (sum(-(-n // bs) for n in kept) if tables_are == "other" else 0) + 2
+    shape = (blocks * bs, hkv)
+    if kv == "int4":
+        cache = [torch.randint(0, 256, (*shape, 64), dtype=torch.uint8, device="cuda") for _ in range(2)]
+        cache += [torch.randint(-2 ** 15, 2 ** 15, (*shape, 2), dtype=torch.int16, device="cuda").view(getattr(torch, dtype)) for _ in range(2)]
+    else:
+        cache = [torch.randint(-2 ** 15, 2 ** 15, (*shape, D), dtype=torch.int16, device="cuda").view(getattr(torch, dtype)) for _ in range(2)]
+    tables = _tables(rng, lens, bs, blocks)
+    new_tables = tables if tables_are == "same" else tables[:, :-(-max(kept) // bs)] if tables_are == "first" else _tables(rng, kept, bs, blocks, taken=set(tables.ravel()))
+    w = np.float32(np.exp(2 * rng.standard_normal((b, hkv, tables.shape[1] * bs))))
+    w[:, :, 5::7] = np.float32(0.25)
+    before = [_np(c) for c in cache]
+    want, want_w, want_lens = _evict_reference(before, tables, new_tables, lens, w, list(range(b)), bs, blocks, budget, sinks, recent)
+    weights, bt = to_dev(w), to_dev(tables, torch.int32)
+    new_w, new_lens = weights if weights_are == "same" else torch.full_like(weights, 7.0), torch.full((b,), -5, dtype=torch.int32, device="cuda")
+    nvk().evict_kvcache(*(cache if kv == "int4" else [*cache, None, None]), weights, None, to_dev(np.array(lens), torch.int32), bt, new_w,
+                        bt if tables_are == "same" else to_dev(np.ascontiguousarray(new_tables), torch.int32), new_lens, hkv, D, bs, budget, sinks, recent)
+    torch.cuda.synchronize()
+    assert new_lens.tolist() == want_lens.tolist() and np.array_equal(new_w.cpu().numpy(), want_w)
+    assert weights_are == "same" or np.array_equal(weights.cpu().numpy(), w)
+    assert all(np.array_equal(_np(got), exp) for got, exp in zip(cache, want))
