@@ -177,7 +177,7 @@ int nvk_decode_attention_paged_fp8(const void* query, const void* k_cache, const
  * 4-byte one.
  *
  * nvk_store_kvcache_int4: key, value [num_tokens, num_kv_heads, 128]; slot_mapping int32 / int64; tokens with a slot < 0 or >= cache_rows are skipped
- * (two tokens of a call with the same slot: undefined which one is stored).  num_tokens 0 does nothing.
+ * (two tokens of a call with the same slot: what is stored there is undefined, a mixture of both among it).  num_tokens 0 does nothing.
  *
  * nvk_gather_kvcache_int4: the keys and values of whole contexts as dense 16-bit rows, for a prefill over cached prefixes: row cu_seqlens_k[s] + i of
  * key / value [total_k, num_kv_heads, 128] is key i of sequence s, low + step * n rounded to `dtype`; then nvk_prefill_attention_varlen with those rows

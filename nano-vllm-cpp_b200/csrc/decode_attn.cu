@@ -5,7 +5,7 @@
 // reference: one warp per (sequence, query head), every KV row re-read by each query head of its group, 8 dependent shuffles per
 // key) and the FlashAttention-2 call it can dlopen (src/kernels/flash_attn.cpp:302-431).
 //
-// The op is HBM-bound (over a 4-bit cache bound by issue); decode_body.cuh has the arithmetic and the ways to share out the keys.  What each kernel here adds:
+// The op is HBM-bound (over a 4-bit cache it is not: see Cache4); decode_body.cuh has the arithmetic and the ways to share out the keys.  What each kernel here adds:
 //   decode_split_kernel    one four-warp block per (KV head, chunk, sequence), two per SM (three for 8-bit caches, four for 4-bit ones, or two of eight warps).  The grid is fixed
 //                          from host-known sizes: nothing depends on host knowledge of context_lens (CUDA-graph safe); blocks
 //                          whose chunk lies beyond the context exit at once.
@@ -342,8 +342,8 @@ size_t part_bytes(size_t parts, int group) { return parts * group * (kHeadDim * 
 size_t part_count(const Splits& s, int64_t batch, int num_kv_heads) {   // (the cluster kernel itself needs none: the mixed step does)
     return s.count > 1 ? static_cast<size_t>(batch) * num_kv_heads * s.count : 0;
 }
-// 4-bit caches are shared out like 8-bit ones (a key costs as much arithmetic, and that is what bounds both), but for what more warps to an SM and a block's
-// fixed part, five tiles' worth, change.  us, spread from 0.05 / 0.5 to all of the table:
+// 4-bit caches are shared out like 8-bit ones (a key costs as much arithmetic), by three blocks to an SM although four fit, but for what more warps to an SM and a
+// block's fixed part, five tiles' worth, change; measured at tables of 2048, 4096 and 8192 keys; wider ones were not.  us, spread from 0.05 / 0.5 to all of the table:
 //   * tables of 1536 to 2048 keys beyond the clusters of four, up to 320 pairs: whole contexts by blocks of eight warps, with more pairs than SMs the longest first
 //     (120 pairs of 2048 14.9 / 16.4 -> 12.6 / 12.8, 160 16.1 / 17.9 -> 14.4 / 17.9, 256 21.2 / 21.6 -> 18.5 / 20.9, 320 24.9 / 26.7 -> 21.3 / 26.8);
 //   * tables of 768 to 2048 keys, 250 pairs and more: whole contexts (320 pairs of 2048 by four warps 25.6 / 27.8 -> 22.7 / 25.2);

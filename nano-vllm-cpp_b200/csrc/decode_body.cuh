@@ -433,8 +433,9 @@ struct Cache8 {
 // d = 16 g .. 16 g + 15, of keys 2t, 2t + 1, 2t + 8, 2t + 9; with halves of two keys' words side by side the same masks give both keys' numbers, and accumulator
 // rows g / g + 8 of d-tile i hold d = 16 g + 2 i and d = 16 g + 2 i + 1 (times 16).  The two rows of a 128-byte line of V are swizzled by the line's number, so
 // that these reads are conflict free.
-// A quarter of the bytes, for as many MMAs: the step is bound by issue (64 sequences of 500 to 4096 keys, 32 / 8 heads, 46.3 us where the bytes take 24.6: issue
-// slots 52 % busy, the ALU pipe 51 %, tensor 24 %, DRAM 45 %; per warp and 32 keys some 570 cycles of a scheduler, of which the MMAs and the masks take most).
+// A quarter of the bytes, for as many MMAs: per warp and 32 keys some 570 cycles of a scheduler, of which the MMAs and the masks take most, and 64 sequences of 500 to
+// 4096 keys, 32 / 8 heads, take 46.0 us where the bytes take 24.6.  No unit is near its limit then (issue slots 52 % busy, the ALU pipe 51 %, tensor 25 %, DRAM 47 %): blocks
+// of uneven length leave SMs idle for a fifth of the time, and latency takes the rest.
 // A warp takes 32 keys at a time, two chains of 16: the arithmetic of a tile is one long chain, and the four warps of a scheduler (three in clusters) do not hide it.  The cache
 // rows of its next 16 tiles are worked out by the lanes, one half of a tile each, while the ids of the 16 after them are on their way.
 template <int AT> __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -454,7 +455,7 @@ struct Cache4 {
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = true;
     static constexpr int kWarps = WARPS;
-    static constexpr int kGroups = 3;                         // resident per SM, by which a step is shared out, as with the 8-bit caches
+    static constexpr int kGroups = 3;                         // resident per SM in clusters; a step is shared out by it in chunks too, as with the 8-bit caches
     static constexpr int kSplitBlocks = 16 / WARPS;           // in chunks: the registers are there, and the chains are what a warp waits for
     static constexpr int kRowBytes = kHeadDim / 2;
     static constexpr int kKeys = 32;                          // of a stage

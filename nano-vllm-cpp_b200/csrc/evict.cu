@@ -16,7 +16,7 @@
 //   4  lists the rows of its tiles, old place and new, and moves them, eight 16-byte pieces under way in every thread (a warp alone with the rows of
 //      its tile: 4 sequences of 2000 to 4096 keys, 8 KV heads, 79 us; the last keys all stay, and who has them ends last).
 // Where the new blocks are the old ones (in place) a row may be written where another one has still to be read.  Then a pair's first block does all of it in order:
-// a key never moves up, and a set of rows is read before any of it is written.
+// a key never moves up, and a set of rows is read before any of it is written (4 sequences of 2000 to 4096 keys, 8 KV heads, 1024 kept: 33.6 us instead of 16.9).
 #include "nvk_internal.cuh"
 
 #include <algorithm>
@@ -386,12 +386,13 @@ int launch_evict(const EvictArgs& a) {
     if (a.batch * a.num_kv_heads > 0x7fffffffLL || a.max_blocks * a.block_size > (1LL << 30) || a.new_max_blocks * a.block_size > (1LL << 30) ||
         a.num_cache_blocks > 0x7fffffffLL / a.block_size)
         return fail(NVK_ERR_UNSUPPORTED, "evict_kvcache: batch, block table or cache too large");
-    // As many blocks to a pair as there are places for, and no more than there are pairs of tiles.  Two to an SM, where there is enough to do: the second block
-    // costs some 3 us, whatever there is.  One to an SM up to 300000 keys of all pairs' tables, 150000 with more than half as many pairs as SMs (which then have one
-    // block each), 100000 where rows are 4-bit ones (us, one / two to an SM, a third of the keys kept: 16-bit 16 pairs of 4096 12.7 / 15.7, 64 of 1024 11.1 / 13.6,
-    // 72 of 4096 29.2 / 30.0, 144 of 1024 16.2 / 17.6, but 40 of 8192 36.7 / 34.2, 64 of 6000 38.2 / 36.6, 88 of 3000 31.7 / 27.5; 4-bit 48 of 2048 17.4 / 20.3, 24
-    // of 4096 17.7 / 20.9, but 40 of 4096 26.4 / 25.1, 144 of 2048 35.3 / 31.8), and where that lets few pairs of long contexts keep their orders.  More blocks than
-    // places do not even out contexts of different lengths (256 pairs of 1000 to 8192 keys: one block each 107.2, two 108.9, four 110.6, eight 137.9).
+    // As many blocks to a pair as there are places for, and no more than there are pairs of tiles; more than that do not even out contexts of different lengths
+    // (256 pairs of 1000 to 8192 keys: one block each 107.2 us, two 108.9, four 110.6, eight 137.9).
+    // Two to an SM where there is enough to do, since the second costs some 3 us whatever there is.  One to an SM (us, one / two, a third of the keys kept)
+    //   * up to 300000 keys of all pairs' tables: 16 pairs of 4096 12.7 / 15.7, 64 of 1024 11.1 / 13.6, 72 of 4096 29.2 / 30.0; but 40 of 8192 36.7 / 34.2;
+    //   * up to 150000 with more than half as many pairs as SMs, which then have one block each: 144 of 1024 16.2 / 17.6; but 88 of 3000 31.7 / 27.5;
+    //   * up to 100000 over 4-bit rows: 48 of 2048 17.4 / 20.3, 24 of 4096 17.7 / 20.9; but 40 of 4096 26.4 / 25.1, 144 of 2048 35.3 / 31.8;
+    //   * where that lets few pairs of long contexts keep their orders.
     const int64_t pairs = a.batch * a.num_kv_heads, tokens = a.max_blocks * a.block_size, most = (tokens + 2 * kWarpTile - 1) / (2 * kWarpTile);
     const bool alone = tokens > kCached && 2 * pairs <= kSmCount;
     const bool single = alone || pairs * tokens <= (a.k_params != nullptr ? 100000 : 2 * pairs <= kSmCount ? 300000 : 150000);
