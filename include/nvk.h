@@ -180,7 +180,8 @@ int nvk_decode_attention_paged_fp8(const void* query, const void* k_cache, const
  * (two tokens of a call with the same slot: what is stored there is undefined, a mixture of both among it).  num_tokens 0 does nothing.
  *
  * nvk_gather_kvcache_int4: the keys and values of whole contexts as dense 16-bit rows, for a prefill over cached prefixes: row cu_seqlens_k[s] + i of
- * key / value [total_k, num_kv_heads, 128] is key i of sequence s, low + step * n rounded to `dtype`; then nvk_prefill_attention_varlen with those rows
+ * key / value [total_k, num_kv_heads, 128] is key i of sequence s, low + step * n rounded to `dtype` (to an infinity where the rounded step takes the top of a
+ * vector that spans all of the type's range beyond it); then nvk_prefill_attention_varlen with those rows
  * and the same cu_seqlens_k.  cu_seqlens_k [num_seqs + 1] ascending from 0, block_tables [num_seqs, max_blocks].  Rows behind the last sequence and
  * rows whose table entry is outside the cache or the table are zeros; sequences are cut off at total_k.
  *
