@@ -43,6 +43,7 @@ extern "C" {
 #define NVK_I32 3
 #define NVK_I64 4
 #define NVK_I8 5
+#define NVK_E4M3 6   /* elements of an 8-bit cache */
 
 /* ABI revision of this header. */
 int nvk_abi_version(void);
@@ -201,6 +202,111 @@ int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, cons
                                     int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads, int num_kv_heads,
                                     int head_dim, int block_size, float scale, void* output, int dtype, void* workspace,
                                     size_t workspace_bytes, void* stream);
+
+/*
+ * 8-bit KV cache with one scale for each (cache block, KV head).  NO COUNTERPART IN THE REFERENCE (its int8 cache has an fp16 scale for every token and head).
+ *   k_cache, v_cache   [num_cache_blocks, block_size, num_kv_heads, head_dim] of `cache_dtype`: NVK_I8 or NVK_E4M3
+ *   k_scale, v_scale   fp32 [num_cache_blocks, num_kv_heads]; an element stands for itself times its block's scale
+ * With A the largest absolute value among a block's rows of a head, its scale is the smallest 2^e, at least 2^-126, with A <= 127 * 2^e (int8) or
+ * A <= 448 * 2^e (e4m3), and elements are x / scale, to nearest, ties to even.  (A value next to the largest of F16 or BF16 may be rounded to a number that
+ * stands for more than the type holds: it reads as an infinity from the gather, as that number in decode.)  A block begins with its row 0, whatever it held before.  Rows that join
+ * it later may raise its scale s to s': every row before them becomes round(n * s / s'), so that a block that has grown several times is off by less than one
+ * step of its last scale.  A block that is given an infinity or a NaN gets a scale of NaN and reads as NaN until it begins anew.
+ * F16 / BF16 and head_dim 128 only (NVK_ERR_UNSUPPORTED otherwise).  Caches, rows and query start on 16-byte boundaries, scales on 4-byte ones.
+ *
+ * nvk_store_kvcache_blocks8: the new rows of a step by sequences: rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1 of key / value are the last ones of the
+ * context_lens[s] positions of sequence s (cu_seqlens_q NULL: row s is the last of sequence s; total_q = num_seqs).  key, value [total_q, num_kv_heads, 128], rows
+ * key_row_stride / value_row_stride elements apart (multiples of 8), so that they may be parts of packed projections.  Rows whose position is negative or
+ * beyond the table, or whose table entry is outside the cache, are skipped.  Positions of a sequence are stored in order, the first row of a block
+ * before the others (rows of a block behind the call's last one may be stored again later: they are left as they were, in the old scale).  No two sequences of a call
+ * write to the same block.
+ *
+ * nvk_gather_kvcache_blocks8: the keys and values of whole contexts as dense 16-bit rows, as nvk_gather_kvcache_int4: row cu_seqlens_k[s] + i of key / value
+ * [total_k, num_kv_heads, 128] is key i of sequence s, rounded to `dtype`.  Rows behind the last sequence and rows whose table entry is outside the cache or the
+ * table are zeros.
+ *
+ * nvk_decode_attention_paged_blocks8: the semantics of nvk_decode_attention_paged over the values as they are; at most 8 query heads per KV head, block_size a
+ * multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes).  Two roundings to f16: BF16 queries (elements below 2^-24 of the head's largest),
+ * and a head's weight times the scale of the value, off by 2^-11 of itself or 2^-22 of the head's largest such product.
+ */
+int nvk_store_kvcache_blocks8(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride, void* k_cache, void* v_cache,
+                              float* k_scale, float* v_scale, int cache_dtype, const void* cu_seqlens_q, int cu_seqlens_q_dtype,
+                              const void* context_lens, int context_lens_dtype, const void* block_tables, int block_tables_dtype, int64_t num_seqs,
+                              int64_t total_q, int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int head_dim, int block_size, int dtype,
+                              void* stream);
+int nvk_gather_kvcache_blocks8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int cache_dtype,
+                               const void* cu_seqlens_k, int cu_seqlens_k_dtype, const void* block_tables, int block_tables_dtype, int64_t num_seqs,
+                               int64_t total_k, int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int head_dim, int block_size, void* key,
+                               void* value, int dtype, void* stream);
+int nvk_decode_attention_paged_blocks8(const void* query, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                                       int cache_dtype, const void* context_lens, int context_lens_dtype, const void* block_tables,
+                                       int block_tables_dtype, int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads,
+                                       int num_kv_heads, int head_dim, int block_size, float scale, void* output, int dtype, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/*
+ * The metadata of a step from the lengths of its requests, on the GPU: what the reference's ModelRunner builds on the host (prepare_prefill, prepare_decode,
+ * build_block_tables, src/engine/model_runner.cpp:482-632, :748-769), and the cache blocks that its scheduler hands out before.  A decode loop that is replayed as a CUDA
+ * graph needs no host for either.  Every index tensor of a call has `index_dtype`, I32 or I64.
+ *   Requests have a row each of two tables that the caller keeps from step to step:
+ *     request_lens [num_request_rows]                          tokens in the cache
+ *     request_blocks [num_request_rows, request_max_blocks]    cache blocks, ceil(length / block_size) of them in use
+ *   and share a list of free blocks, free_blocks [num_free_blocks], of which the first free_count[0] are free; the last of them is taken first.
+ *
+ * nvk_step_metadata: request b of the step, in row request_rows[b] (NULL: row b), gets new_lens[b] >= 0 new tokens.  It has a place if its row is one of the
+ * table, its new length is at most min(request_max_blocks, max_blocks) * block_size, and either it needs no new block or the free ones are enough for it and for those
+ * before it that have a row and a length that fits.  Requests with a place take their new blocks in their order, and
+ *     block_tables [batch, max_blocks]   their blocks, zero padded             context_lens [batch]   their new lengths
+ *     cu_seqlens_q, cu_seqlens_k [batch + 1] (each may be NULL)                running sums of new_lens (of all requests) and of context_lens
+ *     positions, slot_mapping [num_tokens] (both NULL if num_tokens is 0)      of token cu_seqlens_q[b] + i: its place in the sequence, and its cache row
+ *   new_request_lens (may be request_lens) and new_free_count (may be free_count) are the tables' new state; request_blocks gets the new blocks.  Where
+ *   a request has no place nothing changes, its context length is 0, its table zeros and its tokens have position 0 and slot -1, which the other calls skip; so have
+ *   tokens from cu_seqlens_q[batch] on (num_tokens may be more than there are: a captured step).  Tokens whose block is not in [0, num_cache_blocks) have slot -1.  A row < 0
+ *   or >= num_request_rows is padding.  No two requests of a call share a row.  Sums of lengths are held at 2^31 - 1.
+ *
+ * nvk_release_blocks: requests that have ended, or are put off: blocks first_blocks[b] (NULL: 0) up to the last in use of row request_rows[b] (NULL: b) go behind the
+ * free ones, request after request, and the row's length becomes 0.  (first_blocks: a cached prefix that others share stays with its owner.)  Ids that
+ * free_blocks has no room for are dropped.  Rows outside the table are skipped; no two requests of a call share a row.
+ *
+ * At most 8192 requests to a call (a step: at least one); block_size >= 1; new_request_lens and new_free_count are the same memory as their old ones or do not overlap with them.
+ */
+int nvk_step_metadata(const void* new_lens, const void* request_rows, const void* request_lens, void* request_blocks, const void* free_blocks,
+                      const void* free_count, int64_t batch, int64_t num_request_rows, int64_t request_max_blocks, int64_t num_free_blocks,
+                      int64_t num_cache_blocks, int block_size, void* block_tables, int64_t max_blocks, void* context_lens, void* cu_seqlens_q,
+                      void* cu_seqlens_k, void* positions, void* slot_mapping, int64_t num_tokens, void* new_request_lens, void* new_free_count,
+                      int index_dtype, void* stream);
+int nvk_release_blocks(const void* request_rows, const void* first_blocks, const void* request_lens, const void* request_blocks, void* free_blocks,
+                       const void* free_count, int64_t batch, int64_t num_request_rows, int64_t request_max_blocks, int64_t num_free_blocks,
+                       int block_size, void* new_request_lens, void* new_free_count, int index_dtype, void* stream);
+
+/*
+ * Rotary positions on query and key heads, where the table of nvk_fused_split_norm_rope_store does not serve: the first rotary_dim elements of a head (even, at most
+ * head_dim; the others are copied), as pairs of halves (interleaved 0: elements i and i + rotary_dim / 2) or of neighbours (1: elements 2i and 2i + 1), at any
+ * position, with any frequencies.  The reference rotates whole heads by halves (src/kernels/split_qkv.cu:62-154).
+ *   (a, b) -> attention_factor * (a cos t - b sin t, b cos t + a sin t),   t = positions[row] * inv_freq[pair]
+ *   query [rows, num_q_heads, head_dim], key [rows, num_kv_heads, head_dim] (NULL: queries alone), rows a row stride (elements) apart, heads contiguous: parts
+ *   of packed projections as they are.  query_out, key_out likewise; each may be its input with the same stride (in place), otherwise it overlaps with no input.
+ *   positions [rows] int32 / int64, any number; inv_freq fp32 [rotary_dim / 2] on the device.  Angles are taken in 64 bits: as exact for position 2^31 as for 1.
+ *   F16, BF16 or F32; head_dim up to 1024.  Widest loads where head_dim, rotary_dim / 2, strides and addresses are multiples of 16 bytes.
+ *
+ * nvk_rotary_inv_freq fills inv_freq (HOST memory, rotary_dim / 2 numbers) and *attention_factor for a context that was stretched by `factor` >= 1 beyond the
+ * original_positions that a model was trained on (theta_i = base^(-2i / rotary_dim)):
+ *   NVK_ROPE_PLAIN    theta_i                        NVK_ROPE_LINEAR   theta_i / factor
+ *   NVK_ROPE_BASE     theta_i of the base base * factor^(rotary_dim / (rotary_dim - 2)), which takes the slowest pair to theta / factor; rotary_dim > 2
+ *   NVK_ROPE_PARTS    (1 - g) theta_i / factor + g theta_i, g = (turns - low_turns) / (high_turns - low_turns) held in [0, 1], turns = original_positions theta_i / 2 pi
+ *   NVK_ROPE_YARN     the same, and *attention_factor = 0.1 ln(factor) + 1 (Peng et al., YaRN, 2023); 1 otherwise
+ */
+#define NVK_ROPE_PLAIN 0
+#define NVK_ROPE_LINEAR 1
+#define NVK_ROPE_BASE 2
+#define NVK_ROPE_PARTS 3
+#define NVK_ROPE_YARN 4
+int nvk_rotary_embedding(const void* query, const void* key, const void* positions, int positions_dtype, const float* inv_freq, float attention_factor,
+                         int64_t rows, int num_q_heads, int num_kv_heads, int head_dim, int rotary_dim, int interleaved, int64_t query_row_stride,
+                         int64_t key_row_stride, void* query_out, void* key_out, int64_t query_out_row_stride, int64_t key_out_row_stride, int dtype,
+                         void* stream);
+int nvk_rotary_inv_freq(float* inv_freq, float* attention_factor, int rotary_dim, double base, int scaling, double factor, double original_positions,
+                        double low_turns, double high_turns);
 
 /*
  * Eviction from a cache by accumulated attention weight.  NO COUNTERPART IN THE REFERENCE.  Decode steps add up, for every key of a KV head, the

@@ -22,7 +22,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libnvk.so")
 BINDING_PATH = os.path.join(HERE, "nvk_torch.so")
 
-F16, BF16, F32, I32, I64, I8 = 0, 1, 2, 3, 4, 5
+F16, BF16, F32, I32, I64, I8, E4M3 = 0, 1, 2, 3, 4, 5, 6
 OK, ERR_INVALID_ARGUMENT, ERR_CUDA, ERR_UNSUPPORTED = 0, 1, 2, 3
 
 EXPORTED_SYMBOLS = (
@@ -38,6 +38,8 @@ EXPORTED_SYMBOLS = (
     "nvk_tp_allreduce_signal_bytes", "nvk_tp_allreduce_multimem", "nvk_tp_allreduce_add_rmsnorm_multimem",
     "nvk_store_kvcache_fp8", "nvk_decode_attention_paged_fp8",
     "nvk_store_kvcache_int4", "nvk_gather_kvcache_int4", "nvk_decode_attention_paged_int4",
+    "nvk_store_kvcache_blocks8", "nvk_gather_kvcache_blocks8", "nvk_decode_attention_paged_blocks8",
+    "nvk_step_metadata", "nvk_release_blocks", "nvk_rotary_embedding", "nvk_rotary_inv_freq",
     "nvk_decode_attention_weights_workspace_bytes", "nvk_decode_attention_paged_weights", "nvk_evict_kvcache",
 )
 
@@ -205,6 +207,83 @@ def launch_decode_attention_paged_int4(query, k_cache, v_cache, k_params, v_para
     launch_count += (_binding or _load_binding()).decode_int4(
         query, k_cache, v_cache, k_params, v_params, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale,
         output, workspace)
+
+
+def store_kvcache_blocks8(key, value, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, context_lens, block_tables) -> None:
+    """Quantising store into 8-bit caches (int8, or float8_e4m3fn / uint8 for e4m3; [blocks, block_size, Hkv, 128]) with one fp32 scale for
+    each cache block and KV head [blocks, Hkv] (``nvk_store_kvcache_blocks8``), by sequences: rows ``cu_seqlens_q[s]`` on are the last of
+    the ``context_lens[s]`` positions of sequence s; ``cu_seqlens_q=None``: one row for every sequence.  ``key`` / ``value`` may be parts
+    of packed rows."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).store_blocks8(
+        key, value, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, context_lens, block_tables)
+
+
+def gather_kvcache_blocks8(k_cache, v_cache, k_scale, v_scale, cu_seqlens_k, block_tables, num_kv_heads, head_dim, block_size, key,
+                           value) -> None:
+    """Whole contexts of such a cache as dense 16-bit rows, sequence after sequence (``nvk_gather_kvcache_blocks8``), for
+    :func:`launch_prefill_attention_dense`.  Rows of ``key`` / ``value`` behind the last sequence become zeros."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).gather_blocks8(
+        k_cache, v_cache, k_scale, v_scale, cu_seqlens_k, block_tables, num_kv_heads, head_dim, block_size, key, value)
+
+
+def launch_decode_attention_paged_blocks8(query, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables,
+                                          num_kv_heads, head_dim, block_size, scale, output, workspace=None) -> None:
+    """Paged decode attention over such a cache (``nvk_decode_attention_paged_blocks8``), with the optional split-K workspace of
+    :func:`launch_decode_attention_paged`."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).decode_blocks8(
+        query, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale,
+        output, workspace)
+
+
+def step_metadata(new_lens, request_rows, request_lens, request_blocks, free_blocks, free_count, block_size, num_cache_blocks,
+                  block_tables, context_lens, cu_seqlens_q, cu_seqlens_k, positions, slot_mapping, new_request_lens=None,
+                  new_free_count=None) -> None:
+    """Block tables, context lengths, cumulative lengths, positions and slots of a step on the GPU, from the lengths of its requests
+    (``nvk_step_metadata``); new cache blocks come from ``free_blocks[:free_count]``, the last first.  Index tensors of one dtype, int32 or int64.
+    ``request_rows`` None: request b has row b of the tables.  ``new_request_lens`` / ``new_free_count`` None: the tables are updated in
+    place.  ``cu_seqlens_q`` and ``cu_seqlens_k`` may be None, ``positions`` and ``slot_mapping`` too."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).step_metadata(
+        new_lens, request_rows, request_lens, request_blocks, free_blocks, free_count, block_size, num_cache_blocks, block_tables,
+        context_lens, cu_seqlens_q, cu_seqlens_k, positions, slot_mapping, request_lens if new_request_lens is None else new_request_lens,
+        free_count if new_free_count is None else new_free_count)
+
+
+def release_blocks(request_rows, first_blocks, request_lens, request_blocks, free_blocks, free_count, block_size,
+                   new_request_lens=None, new_free_count=None) -> None:
+    """The blocks of requests that ended, from ``first_blocks[b]`` on (None: all), behind the free ones (``nvk_release_blocks``); the
+    requests' lengths become 0.  ``request_rows`` None: all rows."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).release_blocks(
+        request_rows, first_blocks, request_lens, request_blocks, free_blocks, free_count, block_size,
+        request_lens if new_request_lens is None else new_request_lens, free_count if new_free_count is None else new_free_count)
+
+
+def rotary_embedding(query, key, positions, inv_freq, interleaved=False, attention_factor=1.0, query_out=None, key_out=None) -> None:
+    """Rotary positions on the first ``2 * len(inv_freq)`` elements of every head (``nvk_rotary_embedding``): pairs of halves, or of
+    neighbours if ``interleaved``; in place where no outputs are given.  ``query`` [rows, Hq, D] and ``key`` [rows, Hkv, D] (or None) may
+    be parts of packed rows."""
+    global launch_count
+    launch_count += (_binding or _load_binding()).rotary_embedding(
+        query, key, positions, inv_freq, interleaved, attention_factor, query if query_out is None else query_out, key if key_out is None else key_out)
+
+
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "base": 2, "parts": 3, "yarn": 4}
+
+
+def rotary_inv_freq(rotary_dim, base=10000.0, scaling="plain", factor=1.0, original_positions=0.0, low_turns=1.0, high_turns=32.0):
+    """(frequencies as a list of ``rotary_dim / 2`` floats, attention factor) for a plain or a stretched context
+    (``nvk_rotary_inv_freq``)."""
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling must be one of {', '.join(ROPE_SCALINGS)}")
+    out, attention_factor = (ctypes.c_float * max(1, int(rotary_dim) // 2))(), ctypes.c_float(1.0)
+    _check(lib().nvk_rotary_inv_freq(out, ctypes.byref(attention_factor), int(rotary_dim), ctypes.c_double(base), ROPE_SCALINGS[scaling],
+                                     ctypes.c_double(factor), ctypes.c_double(original_positions), ctypes.c_double(low_turns),
+                                     ctypes.c_double(high_turns)))
+    return list(out), float(attention_factor.value)
 
 
 def decode_attention_weights_workspace_bytes(batch, num_heads, num_kv_heads, head_dim, max_blocks, block_size) -> int:

@@ -303,6 +303,190 @@ long decode_int4(PyObject* const* a) {
     return x.launches(ws);
 }
 
+// ---- 8-bit caches with scales of blocks ----
+struct Blocks8 {   // caches and scales that agree
+    const at::Tensor &kc, &vc, &ks, &vs;
+    int type;
+    int64_t blocks = 0;
+    Blocks8(PyObject* kc_, PyObject* vc_, PyObject* ks_, PyObject* vs_)
+        : kc(cuda("k_cache", kc_)), vc(cuda("v_cache", vc_)), ks(cuda("k_scale", ks_)), vs(cuda("v_scale", vs_)) {
+        const auto t = kc.scalar_type();
+        if (vc.scalar_type() != t || (t != at::kChar && t != at::kByte && t != at::kFloat8_e4m3fn))
+            raise(PyExc_ValueError, "%s", "k_cache and v_cache must both be int8, or both float8_e4m3fn or uint8");
+        type = t == at::kChar ? NVK_I8 : NVK_E4M3;
+        if (ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat) raise(PyExc_ValueError, "%s", "k_scale and v_scale must be float32");
+    }
+    void sizes(int64_t block_size, int64_t hkv, int64_t d) {
+        if (block_size <= 0 || hkv <= 0 || d <= 0) raise(PyExc_ValueError, "%s", "block_size, num_kv_heads and head_dim must be positive");
+        const int64_t per = block_size * hkv * d;
+        if (kc.numel() % per != 0 || kc.numel() != vc.numel()) raise(PyExc_ValueError, "%s", "k_cache does not contain an integer number of cache blocks");
+        blocks = kc.numel() / per;
+        if (ks.numel() != blocks * hkv || vs.numel() != blocks * hkv)
+            raise(PyExc_ValueError, "%s", "k_scale and v_scale must have an element for every cache block and KV head");
+    }
+};
+
+// Rows [n, heads, head_dim] on CUDA, each of them contiguous: parts of packed rows too.
+const at::Tensor& strided_rows(const char* name, PyObject* o) {
+    const at::Tensor* t = optional(name, o);
+    if (t == nullptr) raise(PyExc_ValueError, "%s must be defined", name);
+    if (!t->is_cuda()) raise(PyExc_ValueError, "%s must live on CUDA", name);
+    if (t->dim() != 3) raise(PyExc_ValueError, "%s must be [rows, heads, head_dim]", name);
+    if ((t->size(2) > 1 && t->stride(2) != 1) || (t->size(1) > 1 && t->stride(1) != t->size(2))) raise(PyExc_ValueError, "%s must have contiguous rows", name);
+    return *t;
+}
+// (of a single row, whatever its stride is called)
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2); }
+
+// (key, value, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, context_lens, block_tables)
+long store_blocks8(PyObject* const* a) {
+    const at::Tensor &key = strided_rows("key", a[0]), &value = strided_rows("value", a[1]), &ctx = cuda("context_lens", a[7]), &bt = cuda("block_tables", a[8]);
+    Blocks8 cache(a[2], a[3], a[4], a[5]);
+    const at::Tensor* cu = optional_cuda("cu_seqlens_q", a[6]);
+    if (!key.sizes().equals(value.sizes()) || key.scalar_type() != value.scalar_type())
+        raise(PyExc_ValueError, "%s", "key and value must have the same shape and dtype");
+    check_here({&key, &value, &cache.kc, &cache.vc, &cache.ks, &cache.vs, cu, &ctx, &bt});
+    const Index starts("cu_seqlens_q", cu), lens("context_lens", &ctx), tables("block_tables", &bt);
+    const int64_t seqs = ctx.numel(), hkv = key.size(1), d = key.size(2);
+    if (bt.dim() != 2 || bt.size(0) != seqs || (cu != nullptr ? cu->numel() != seqs + 1 : key.size(0) != seqs))
+        raise(PyExc_ValueError, "%s", "block_tables must have a row, cu_seqlens_q or key a sequence, for every context length");
+    if (cache.kc.dim() != 4) raise(PyExc_ValueError, "%s", "k_cache must be [blocks, block_size, num_kv_heads, head_dim]");
+    const int64_t bs = cache.kc.size(1);
+    if (!cache.kc.sizes().equals(cache.vc.sizes()) || cache.kc.size(2) != hkv || cache.kc.size(3) != d)
+        raise(PyExc_ValueError, "%s", "k_cache and v_cache must have the heads and the head_dim of key");
+    cache.sizes(bs, hkv, d);
+    launch(nvk_store_kvcache_blocks8, ptr(key), ptr(value), row_stride(key), row_stride(value), ptr(cache.kc), ptr(cache.vc), static_cast<float*>(ptr(cache.ks)),
+           static_cast<float*>(ptr(cache.vs)), cache.type, starts.p, starts.dtype, lens.p, lens.dtype, tables.p, tables.dtype, seqs, key.size(0), bt.size(1),
+           cache.blocks, static_cast<int>(hkv), static_cast<int>(d), static_cast<int>(bs), code(key), stream());
+    return 1;
+}
+
+// (k_cache, v_cache, k_scale, v_scale, cu_seqlens_k, block_tables, num_kv_heads, head_dim, block_size, key, value)
+long gather_blocks8(PyObject* const* a) {
+    Blocks8 cache(a[0], a[1], a[2], a[3]);
+    const at::Tensor &cu = cuda("cu_seqlens_k", a[4]), &bt = cuda("block_tables", a[5]), &key = cuda("key", a[9]), &value = cuda("value", a[10]);
+    check_here({&cache.kc, &cache.vc, &cache.ks, &cache.vs, &cu, &bt, &key, &value});
+    const int64_t hkv = integer(a[6]), d = integer(a[7]), bs = integer(a[8]);
+    const Index starts("cu_seqlens_k", &cu), tables("block_tables", &bt);
+    cache.sizes(bs, hkv, d);
+    if (!key.sizes().equals(value.sizes()) || key.scalar_type() != value.scalar_type() || key.dim() != 3 || key.size(1) != hkv || key.size(2) != d)
+        raise(PyExc_ValueError, "%s", "key and value must be [total_k, num_kv_heads, head_dim] of one dtype");
+    if (cu.numel() < 2 || bt.dim() != 2 || bt.size(0) != cu.numel() - 1)
+        raise(PyExc_ValueError, "%s", "block_tables must have a row for every sequence of cu_seqlens_k");
+    if (key.size(0) == 0) return 0;
+    launch(nvk_gather_kvcache_blocks8, ptr(cache.kc), ptr(cache.vc), static_cast<const float*>(ptr(cache.ks)), static_cast<const float*>(ptr(cache.vs)), cache.type,
+           starts.p, starts.dtype, tables.p, tables.dtype, cu.numel() - 1, key.size(0), bt.size(1), cache.blocks, static_cast<int>(hkv), static_cast<int>(d),
+           static_cast<int>(bs), ptr(key), ptr(value), code(key), stream());
+    return 1;
+}
+
+// (query, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, num_kv_heads, head_dim, block_size, scale, output, workspace)
+long decode_blocks8(PyObject* const* a) {
+    const Decode x(a[0], a[1], a[2], a[5], a[6], a[11], a[7], a[8], a[9], a[10]);
+    Blocks8 cache(a[1], a[2], a[3], a[4]);
+    const at::Tensor* ws = optional_cuda("workspace", a[12]);
+    check_rows(x);
+    check_here({&cache.ks, &cache.vs, ws});
+    cache.sizes(x.bs, x.hkv, x.d);
+    launch(nvk_decode_attention_paged_blocks8, ptr(x.q), ptr(cache.kc), ptr(cache.vc), static_cast<const float*>(ptr(cache.ks)),
+           static_cast<const float*>(ptr(cache.vs)), cache.type, x.lens.p, x.lens.dtype, x.tables.p, x.tables.dtype, x.batch, x.max_blocks, cache.blocks,
+           static_cast<int>(x.heads), static_cast<int>(x.hkv), static_cast<int>(x.d), static_cast<int>(x.bs), x.scale, ptr(x.out), code(x.q), ptr(ws), bytes(ws),
+           stream());
+    return x.launches(ws);
+}
+
+// ---- the metadata of a step ----
+// One width for every index tensor of a call.
+struct Indices {
+    int dtype = -1;
+    template <typename P = void> P* take(const char* name, const at::Tensor* t) {
+        if (t == nullptr) return nullptr;
+        const Index i(name, t);
+        if (dtype >= 0 && i.dtype != dtype) raise(PyExc_ValueError, "%s must have the dtype of the other index tensors", name);
+        dtype = i.dtype;
+        return const_cast<P*>(static_cast<const P*>(i.p));
+    }
+};
+// The tables of requests: lengths, blocks, free blocks and their count, and where the new lengths and the new count go.
+struct Requests {
+    const at::Tensor &lens, &blocks, &free, &count, &new_lens, &new_count;
+    Requests(PyObject* lens_, PyObject* blocks_, PyObject* free_, PyObject* count_, PyObject* new_lens_, PyObject* new_count_)
+        : lens(cuda("request_lens", lens_)), blocks(cuda("request_blocks", blocks_)), free(cuda("free_blocks", free_)), count(cuda("free_count", count_)),
+          new_lens(cuda("new_request_lens", new_lens_)), new_count(cuda("new_free_count", new_count_)) {
+        if (blocks.dim() != 2 || blocks.size(0) != lens.numel() || new_lens.numel() != lens.numel())
+            raise(PyExc_ValueError, "%s", "request_blocks must have a row, new_request_lens an element, for every element of request_lens");
+        if (count.numel() != 1 || new_count.numel() != 1) raise(PyExc_ValueError, "%s", "free_count and new_free_count must have one element");
+    }
+};
+
+// (new_lens, request_rows, request_lens, request_blocks, free_blocks, free_count, block_size, num_cache_blocks, block_tables, context_lens, cu_seqlens_q,
+//  cu_seqlens_k, positions, slot_mapping, new_request_lens, new_free_count)
+long step_metadata(PyObject* const* a) {
+    const at::Tensor &n = cuda("new_lens", a[0]), &bt = cuda("block_tables", a[8]), &ctx = cuda("context_lens", a[9]);
+    const at::Tensor *rows = optional_cuda("request_rows", a[1]), *cu_q = optional_cuda("cu_seqlens_q", a[10]), *cu_k = optional_cuda("cu_seqlens_k", a[11]),
+                     *pos = optional_cuda("positions", a[12]), *slots = optional_cuda("slot_mapping", a[13]);
+    const Requests r(a[2], a[3], a[4], a[5], a[14], a[15]);
+    check_here({&n, rows, &r.lens, &r.blocks, &r.free, &r.count, &bt, &ctx, cu_q, cu_k, pos, slots, &r.new_lens, &r.new_count});
+    const int64_t batch = n.numel();
+    if ((rows != nullptr && rows->numel() != batch) || bt.dim() != 2 || bt.size(0) != batch || ctx.numel() != batch)
+        raise(PyExc_ValueError, "%s", "request_rows, block_tables and context_lens must have a row for every element of new_lens");
+    if ((cu_q != nullptr && cu_q->numel() != batch + 1) || (cu_k != nullptr && cu_k->numel() != batch + 1))
+        raise(PyExc_ValueError, "%s", "cu_seqlens_q and cu_seqlens_k must have one element more than new_lens");
+    if (numel(pos) != numel(slots)) raise(PyExc_ValueError, "%s", "positions and slot_mapping must have the same size");
+    Indices i;
+    const void *pn = i.take("new_lens", &n), *pr = i.take("request_rows", rows), *pl = i.take("request_lens", &r.lens), *pf = i.take("free_blocks", &r.free),
+               *pc = i.take("free_count", &r.count);
+    void *pb = i.take("request_blocks", &r.blocks), *pt = i.take("block_tables", &bt), *px = i.take("context_lens", &ctx), *pq = i.take("cu_seqlens_q", cu_q),
+         *pk = i.take("cu_seqlens_k", cu_k), *pp = i.take("positions", pos), *ps = i.take("slot_mapping", slots), *nl = i.take("new_request_lens", &r.new_lens),
+         *nc = i.take("new_free_count", &r.new_count);
+    const int64_t bs = integer(a[6]), blocks = integer(a[7]);
+    if (batch == 0 || bt.size(1) == 0) raise(PyExc_ValueError, "%s", "new_lens and the rows of block_tables must contain at least one element");
+    if (bs <= 0 || bs > 0x7fffffff) raise(PyExc_ValueError, "%s", "block_size must be positive");
+    launch(nvk_step_metadata, pn, pr, pl, pb, pf, pc, batch, r.lens.numel(), r.blocks.size(1), r.free.numel(), blocks, static_cast<int>(bs), pt, bt.size(1), px, pq,
+           pk, pp, ps, numel(pos), nl, nc, i.dtype, stream());
+    return 1;
+}
+
+// (request_rows, first_blocks, request_lens, request_blocks, free_blocks, free_count, block_size, new_request_lens, new_free_count)
+long release_blocks(PyObject* const* a) {
+    const at::Tensor *rows = optional_cuda("request_rows", a[0]), *first = optional_cuda("first_blocks", a[1]);
+    const Requests r(a[2], a[3], a[4], a[5], a[7], a[8]);
+    check_here({rows, first, &r.lens, &r.blocks, &r.free, &r.count, &r.new_lens, &r.new_count});
+    const int64_t batch = rows != nullptr ? rows->numel() : r.lens.numel();
+    if (first != nullptr && first->numel() != batch) raise(PyExc_ValueError, "%s", "first_blocks must have an element for every request");
+    Indices i;
+    const void *pr = i.take("request_rows", rows), *p1 = i.take("first_blocks", first), *pl = i.take("request_lens", &r.lens), *pb = i.take("request_blocks", &r.blocks),
+               *pc = i.take("free_count", &r.count);
+    void *pf = i.take("free_blocks", &r.free), *nl = i.take("new_request_lens", &r.new_lens), *nc = i.take("new_free_count", &r.new_count);
+    const int64_t bs = integer(a[6]);
+    if (bs <= 0 || bs > 0x7fffffff) raise(PyExc_ValueError, "%s", "block_size must be positive");
+    launch(nvk_release_blocks, pr, p1, pl, pb, pf, pc, batch, r.lens.numel(), r.blocks.size(1), r.free.numel(), static_cast<int>(bs), nl, nc, i.dtype, stream());
+    return 1;
+}
+
+// (query, key, positions, inv_freq, interleaved, attention_factor, query_out, key_out)
+long rotary_embedding(PyObject* const* a) {
+    const at::Tensor &q = strided_rows("query", a[0]), &qo = strided_rows("query_out", a[6]), &pos = cuda("positions", a[2]), &f = cuda("inv_freq", a[3]);
+    const at::Tensor* k = a[1] == Py_None ? nullptr : &strided_rows("key", a[1]);
+    const at::Tensor* ko = a[7] == Py_None ? nullptr : &strided_rows("key_out", a[7]);
+    check_here({&q, k, &pos, &f, &qo, ko});
+    const Index at("positions", &pos);
+    if (f.scalar_type() != at::kFloat) raise(PyExc_ValueError, "%s must be float32", "inv_freq");
+    if ((k == nullptr) != (ko == nullptr)) raise(PyExc_ValueError, "%s", "key and key_out go together");
+    if (!qo.sizes().equals(q.sizes()) || qo.scalar_type() != q.scalar_type() || (k != nullptr && (!ko->sizes().equals(k->sizes()) || ko->scalar_type() != k->scalar_type())))
+        raise(PyExc_ValueError, "%s", "query_out and key_out must have the shapes and the dtype of query and key");
+    if (k != nullptr && (k->size(0) != q.size(0) || k->size(2) != q.size(2) || k->scalar_type() != q.scalar_type()))
+        raise(PyExc_ValueError, "%s", "key must have the rows, the head_dim and the dtype of query");
+    if (pos.numel() != q.size(0)) raise(PyExc_ValueError, "%s", "positions must have an element for every row");
+    const int pairs = PyObject_IsTrue(a[4]);
+    if (pairs < 0) throw Raised{};
+    if (q.size(0) == 0) return 0;
+    launch(nvk_rotary_embedding, ptr(q), ptr(k), at.p, at.dtype, static_cast<const float*>(ptr(f)), real(a[5]), q.size(0), static_cast<int>(q.size(1)),
+           static_cast<int>(k != nullptr ? k->size(1) : 0), static_cast<int>(q.size(2)), static_cast<int>(2 * f.numel()), pairs, row_stride(q),
+           k != nullptr ? row_stride(*k) : 0, ptr(qo), ptr(ko), row_stride(qo), ko != nullptr ? row_stride(*ko) : 0, code(q), stream());
+    return 1;
+}
+
 // Weights of keys [rows, hkv, keys], fp32.
 const at::Tensor& weights_of(const char* name, PyObject* o, int64_t hkv) {
     const at::Tensor& t = cuda(name, o);
@@ -452,6 +636,12 @@ PyMethodDef methods[] = {
     method<store_int4, 7>("store_int4"),
     method<gather_int4, 11>("gather_int4"),
     method<decode_int4, 13>("decode_int4"),
+    method<store_blocks8, 9>("store_blocks8"),
+    method<gather_blocks8, 11>("gather_blocks8"),
+    method<decode_blocks8, 13>("decode_blocks8"),
+    method<step_metadata, 16>("step_metadata"),
+    method<release_blocks, 9>("release_blocks"),
+    method<rotary_embedding, 8>("rotary_embedding"),
     method<decode_weights, 16>("decode_weights"),
     method<evict, 17>("evict"),
     method<prefill, 14>("prefill"),

@@ -470,7 +470,7 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     int cluster = 0;
     const int rc = decode_plan(a, F::kGroups, &p, &cluster, F::kFourBits);
     if (rc != NVK_OK) return rc;
-    p.k_scale = static_cast<const __half*>(k_scale); p.v_scale = static_cast<const __half*>(v_scale);
+    p.k_scale = k_scale; p.v_scale = v_scale;
     if constexpr (F::kScores) {
         p.scores = scores;
         p.ws_ml = ml;
@@ -589,6 +589,16 @@ bool decode_int4_supported(const DecodeArgs& a, const void* k_params, const void
 int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_params) {
     return a.dtype == NVK_BF16 ? launch_typed<Cache4<__nv_bfloat16>, __nv_bfloat16>(a, k_params, v_params)
                                : launch_typed<Cache4<__half>, __half>(a, k_params, v_params);
+}
+
+bool decode_blocks8_supported(const DecodeArgs& a, const float* k_scale, const float* v_scale) {
+    return shape_supported(a) && aligned_to(a.q, 16) && aligned_to(k_scale, 4) && aligned_to(v_scale, 4);
+}
+
+int launch_decode_blocks8(const DecodeArgs& a, const float* k_scale, const float* v_scale, bool fp8) {
+    using bf = __nv_bfloat16;
+    if (a.dtype == NVK_BF16) return fp8 ? launch_typed<CacheBlocks8<bf, true>, bf>(a, k_scale, v_scale) : launch_typed<CacheBlocks8<bf, false>, bf>(a, k_scale, v_scale);
+    return fp8 ? launch_typed<CacheBlocks8<__half, true>, __half>(a, k_scale, v_scale) : launch_typed<CacheBlocks8<__half, false>, __half>(a, k_scale, v_scale);
 }
 
 // ---- the weights of the keys -----------------------------------------------------------------------------------------------

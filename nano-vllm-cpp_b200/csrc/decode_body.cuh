@@ -1,4 +1,5 @@
-// Device code of paged decode attention on tensor cores (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 or 4-bit cache), shared
+// Device code of paged decode attention on tensor cores (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 or 4-bit cache, 8-bit ones with scales for
+// tokens or for blocks), shared
 // by the decode kernels (decode_attn.cu) and the mixed prefill + decode kernel (prefill_attn_tc.cu).
 //
 // The op is HBM-bound: every K and V row of every context is read once.  A group of four warps (over a 4-bit cache also of eight) takes a range of the keys of one
@@ -35,7 +36,8 @@ constexpr int kMergeWarps = 8;         // warps that merge the parts of one (seq
 
 struct DecodeParams {
     const void* q; const void* k_cache; const void* v_cache;
-    const __half* k_scale; const __half* v_scale;      // 8-bit caches: a scale; 4-bit ones: a pair (step, low) in the queries' type, one 32-bit word
+    const void* k_scale; const void* v_scale;          // 8-bit caches: fp16 scales of tokens, or fp32 ones of cache blocks; 4-bit ones: pairs (step, low) in the
+                                                       // queries' type, 32-bit words
     IndexArray context_lens; IndexArray block_tables;
     void* out; float* ws_o; float2* ws_ml;             // partial results: [sequence][KV head][split][group][128] and (maximum, sum)
     int64_t max_blocks, num_cache_blocks;
@@ -169,6 +171,7 @@ template <typename T, bool SCORES = false>
 struct Cache16 {
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = false;
+    static constexpr bool kBlockScales = false;
     static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 2;   // resident per SM
     static constexpr int kSplitBlocks = kGroups;
@@ -289,6 +292,7 @@ template <typename T, bool FP8>
 struct Cache8 {
     static constexpr bool kScores = false;
     static constexpr bool kFourBits = false;
+    static constexpr bool kBlockScales = false;
     static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 3, kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim;
@@ -345,7 +349,7 @@ struct Cache8 {
         const int tr = lane & 15;
         const int sbytes = tr < valid ? 4 : 0;
         const size_t sidx = sbytes ? (static_cast<size_t>(row0) + tr) * p.num_kv_heads + kvh : 0;
-        cp_async4(stage + 2 * kTileBytes + lane * 4, (lane < 16 ? p.k_scale : p.v_scale) + (sidx & ~static_cast<size_t>(1)), sbytes);
+        cp_async4(stage + 2 * kTileBytes + lane * 4, static_cast<const __half*>(lane < 16 ? p.k_scale : p.v_scale) + (sidx & ~static_cast<size_t>(1)), sbytes);
     }
     __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int kvh, int lane) {
         const int g = lane >> 2, t = lane & 3;
@@ -454,6 +458,7 @@ struct Cache4 {
     using Eight = Cache4<T, SCORES, 8>;                       // eight warps to a block
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = true;
+    static constexpr bool kBlockScales = false;
     static constexpr int kWarps = WARPS;
     static constexpr int kGroups = 3;                         // resident per SM in clusters; a step is shared out by it in chunks too, as with the 8-bit caches
     static constexpr int kSplitBlocks = 16 / WARPS;           // in chunks: the registers are there, and the chains are what a warp waits for
@@ -666,7 +671,7 @@ struct Cache4 {
         const unsigned char* k_at = static_cast<const unsigned char*>(p.k_cache) + r * row_bytes + c * 16;
         const unsigned char* v_at = static_cast<const unsigned char*>(p.v_cache) + r * row_bytes + c * 16;
         const unsigned char *k8_at = k_at + 8 * row_bytes, *v8_at = v_at + 8 * row_bytes;
-        const uint32_t* par_at = reinterpret_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + static_cast<size_t>(lane & 15) * p.num_kv_heads;
+        const uint32_t* par_at = static_cast<const uint32_t*>(lane < 16 ? p.k_scale : p.v_scale) + static_cast<size_t>(lane & 15) * p.num_kv_heads;
         const uint32_t k_to = r * kRowBytes + c * 16, v_to = kTileBytes + (r >> 1) * 128 + (((((r & 1) << 2) + c) ^ (((r >> 1) & 3) << 1)) << 4);
         const uint32_t par_to = 2 * kTileBytes + (lane & 15) * 8 + (lane >> 4) * 4;
         int issued = 0, left = t1 - first;        // keys from the next tile on
@@ -742,6 +747,171 @@ struct Cache4 {
     }
 };
 
+// 8-bit cache with one fp32 scale, a power of two, for each (cache block, KV head): kv_blocks8.cu.  Tiles, pieces and the order of the contractions are those of
+// Cache8; a tile of 16 keys lies in one cache block, so that its K and its V have one scale each, two words beside the tile.
+//   * int8: the byte glued under the exponent byte of 1024 as there, and 1152 taken off right away, exactly (one HADD2 for two elements).  Taken off the sums
+//     afterwards, as Cache8 does, it costs the accumulators up to ten bits.
+//   * Queries are brought to f16 by a power of two, each head's own (exact but for elements below 2^-24 of the head's largest), as in Cache4.
+//   * sum_k p_k s_k n_k: p' = p s 2^-E goes to the MMA in f16, exact but for its rounding; E is each head's own, chosen as in Cache4 by the largest product p s so
+//     far, and chosen again, with the sums rescaled, where a score passes the last maximum by 8 or a scale reaches 2^(7 + E).  So p' is rounded by 2^-11 of itself or 2^-22 of the
+//     head's largest, and one block whose scale is far above the others' does not cost them their bits.
+template <typename T, bool FP8>
+struct CacheBlocks8 {
+    static constexpr bool kScores = false;
+    static constexpr bool kFourBits = false;
+    static constexpr bool kBlockScales = true;
+    static constexpr int kWarps = kGroupWarps;
+    static constexpr int kGroups = 3, kSplitBlocks = kGroups;
+    static constexpr int kRowBytes = kHeadDim;
+    static constexpr int kTileBytes = kTileTokens * kRowBytes;
+    static constexpr int kStageBytes = 2 * kTileBytes + 16;   // K, V, the scales of both
+    static constexpr int kStages = 4;
+    static constexpr int kPartStride = kHeadDim + 4;
+    static constexpr float kSlack = 8.0f;                     // by so much a score may pass s.m: p <= 2^8
+
+    SoftmaxState s;
+    float score_scale[2];
+    float down[2];       // 2^-E of heads 2t, 2t + 1
+    float top_part[2];   // the largest log2(p s) so far, p without the maximum taken off
+    uint32_t qa[8][2];   // as in Cache8
+
+    __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        const bool live = g < p.group;
+        const uint2* row = reinterpret_cast<const uint2*>(
+            static_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.num_heads + kvh * p.group + (live ? g : 0)) * kHeadDim) + 4 * t;
+        uint2 v[8];
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) v[ks] = live ? row[16 * (ks >> 2) + (ks & 3)] : make_uint2(0u, 0u);
+        float top = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+            const float2 a = unpack2<T>(v[ks].x), c = unpack2<T>(v[ks].y);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(c.x), fabsf(c.y))));
+        }
+#pragma unroll
+        for (int x = 1; x < 4; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        // the head's largest to [2^14, 2^15); (infinities and NaN stay what they are)
+        const int up = top > 0.0f && top < INFINITY ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 100) : 0;
+        const float by = power_of_two(up);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+            const float2 a = unpack2<T>(v[ks].x), c = unpack2<T>(v[ks].y);
+            qa[ks][0] = ElemTraits<__half>::pack2(a.x * by, a.y * by);
+            qa[ks][1] = ElemTraits<__half>::pack2(c.x * by, c.y * by);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) score_scale[h] = p.scale_log2 * power_of_two(-__shfl_sync(0xffffffffu, up, 8 * t + 4 * h));
+        down[0] = down[1] = 0x1p126f;
+        top_part[0] = top_part[1] = -INFINITY;
+        s.reset();
+    }
+    static __device__ __forceinline__ void issue(const DecodeParams& p, int kvh, int64_t row0, int valid, uint32_t stage, int lane) {
+        const size_t stride = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
+        const int c = lane & 7, rq = lane >> 3;   // 16-byte piece c of rows 4 i + rq; swizzles as in Cache8
+        const size_t base = static_cast<size_t>(row0) * stride + static_cast<size_t>(kvh) * kRowBytes + c * 16;
+        const unsigned char* kc = static_cast<const unsigned char*>(p.k_cache) + base;
+        const unsigned char* vc = static_cast<const unsigned char*>(p.v_cache) + base;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 4 * i + rq;
+            const int bytes = r < valid ? 16 : 0;
+            const size_t src = bytes ? r * stride : 0;
+            nvk::cp_async16(stage + r * kRowBytes + ((c ^ ((r & 1) << 2)) << 4), kc + src, bytes);
+            nvk::cp_async16(stage + kTileBytes + r * kRowBytes + ((c ^ (r & 6)) << 4), vc + src, bytes);
+        }
+    }
+    static __device__ __forceinline__ void issue_scales(const DecodeParams& p, int kvh, int block, uint32_t stage, int lane) {   // (block < 0: zeros)
+        if (lane < 2) {
+            const float* from = static_cast<const float*>(lane == 0 ? p.k_scale : p.v_scale);
+            dec::cp_async4(stage + 2 * kTileBytes + lane * 4, from + static_cast<int64_t>(max(block, 0)) * p.num_kv_heads + kvh, block < 0 ? 0 : 4);
+        }
+    }
+    static __device__ __forceinline__ uint32_t whole(uint32_t glued) {   // two f16, int8: less 1152
+        if constexpr (FP8) return glued;
+        const uint32_t off = 0xe480e480u;   // -1152
+        const __half2 d = __hadd2(*reinterpret_cast<const __half2*>(&glued), *reinterpret_cast<const __half2*>(&off));
+        return *reinterpret_cast<const uint32_t*>(&d);
+    }
+    static __device__ __forceinline__ uint32_t lo2(uint32_t x) { return whole(widen_pair_lo<FP8>(x)); }
+    static __device__ __forceinline__ uint32_t hi2(uint32_t x) { return whole(widen_pair_hi<FP8>(x)); }
+    static constexpr uint32_t kFlip = FP8 ? 0u : 0x80808080u;
+
+    __device__ __forceinline__ int exponent(int h) const { return 127 - static_cast<int>(__float_as_uint(down[h]) >> 23); }   // E
+    // (Cache4::raise; the tile's V has one scale.)
+    __device__ __forceinline__ void raise(const float (&sc)[4], float v_scale) {
+        const float by = __log2f(v_scale);
+        float c[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float top = fmaxf(sc[h], sc[2 + h]);
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float m_new = fmaxf(s.m[h], top);
+            top_part[h] = fmaxf(top_part[h], top + by);
+            const int was = exponent(h), e = static_cast<int>(fminf(fmaxf(ceilf(top_part[h] - m_new) + 2.0f, -126.0f), 126.0f));
+            c[h] = s.m[h] == m_new ? 1.0f : fast_exp2(s.m[h] - m_new);
+            s.l[h] *= c[h];
+            s.m[h] = m_new;
+            c[h] *= power_of_two(min(max(was - e, -126), 127));   // (beyond that nothing is seen of what was there, or there was nothing)
+            down[h] = power_of_two(-e);
+        }
+#pragma unroll
+        for (int mt = 0; mt < 8; ++mt) { s.o[mt][0] *= c[0]; s.o[mt][1] *= c[1]; s.o[mt][2] *= c[0]; s.o[mt][3] *= c[1]; }
+    }
+    __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int /*kvh*/, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        float k_scale, v_scale;
+        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(k_scale), "=f"(v_scale) : "r"(stage + 2 * kTileBytes));
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            uint32_t w0[4], w1[4];
+            lds32x4(stage + g * kRowBytes + (((4 * q + t) ^ ((g & 1) << 2)) << 4), w0);
+            lds32x4(stage + (g + 8) * kRowBytes + (((4 * q + t) ^ ((g & 1) << 2)) << 4), w1);
+#pragma unroll
+            for (int wi = 0; wi < 4; ++wi) {
+                const int ks = 4 * q + wi;
+                const uint32_t x0 = w0[wi] ^ kFlip, x1 = w1[wi] ^ kFlip;
+                mma_16816<__half>(ks & 1 ? s1 : s0, lo2(x0), lo2(x1), hi2(x0), hi2(x1), qa[ks][0], qa[ks][1]);
+            }
+        }
+        const float by[2] = {score_scale[0] * k_scale, score_scale[1] * k_scale};
+        float sc[4] = {(s0[0] + s1[0]) * by[0], (s0[1] + s1[1]) * by[1], (s0[2] + s1[2]) * by[0], (s0[3] + s1[3]) * by[1]};
+        mask_scores(sc, g, valid);
+        const float top0 = fmaxf(sc[0], sc[2]), top1 = fmaxf(sc[1], sc[3]);
+        if (__any_sync(0xffffffffu, fmaxf(top0 - s.m[0], top1 - s.m[1]) > kSlack || v_scale * fmaxf(down[0], down[1]) >= 0x1p7f)) raise(sc, v_scale);
+        const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
+        s.l[0] += p0 + p2;
+        s.l[1] += p1 + p3;
+        const float part[2] = {v_scale * down[0], v_scale * down[1]};
+        const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * part[0], p1 * part[1]));
+        const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * part[0], p3 * part[1]));
+        // output: V rows 2t, 2t+1, 2t+8, 2t+9, piece g (d = 16 g .. 16 g + 15)
+        uint32_t v0[4], v1[4], v2[4], v3[4];
+        const uint32_t vbase = stage + kTileBytes;
+        lds32x4(vbase + (2 * t) * kRowBytes + ((g ^ ((2 * t) & 6)) << 4), v0);
+        lds32x4(vbase + (2 * t + 1) * kRowBytes + ((g ^ ((2 * t + 1) & 6)) << 4), v1);
+        lds32x4(vbase + (2 * t + 8) * kRowBytes + ((g ^ ((2 * t + 8) & 6)) << 4), v2);
+        lds32x4(vbase + (2 * t + 9) * kRowBytes + ((g ^ ((2 * t + 9) & 6)) << 4), v3);
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const uint32_t x0 = v0[a] ^ kFlip, x1 = v1[a] ^ kFlip, x2 = v2[a] ^ kFlip, x3 = v3[a] ^ kFlip;
+            const uint32_t lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);
+            const uint32_t lo23 = __byte_perm(x2, x3, 0x5140), hi23 = __byte_perm(x2, x3, 0x7362);
+            mma_16816<__half>(s.o[2 * a], lo2(lo01), hi2(lo01), lo2(lo23), hi2(lo23), pb0, pb1);
+            mma_16816<__half>(s.o[2 * a + 1], lo2(hi01), hi2(hi01), lo2(hi23), hi2(hi23), pb0, pb1);
+        }
+    }
+    __device__ __forceinline__ void finish() {}
+    __device__ __forceinline__ void write_part(float* row, int h, int g) const {
+        const float up = power_of_two(exponent(h));
+#pragma unroll
+        for (int i = 0; i < 8; i += 2)
+            *reinterpret_cast<float4*>(row + 16 * g + 2 * i) = make_float4(s.o[i][h] * up, s.o[i][2 + h] * up, s.o[i + 1][h] * up, s.o[i + 1][2 + h] * up);
+    }
+};
+
 // ---- a group's range of keys ---------------------------------------------------------------------------------------------
 template <class F>
 struct alignas(128) GroupSmem {
@@ -782,6 +952,7 @@ __device__ __forceinline__ void stream_tiles(const DecodeParams& p, int b, int k
         if (tok < t1) {
             const int phys = __shfl_sync(0xffffffffu, ids, blk - id_base);
             F::issue(p, kvh, phys < 0 ? 0 : static_cast<int64_t>(phys) * bs + off, phys < 0 ? 0 : t1 - tok, istage, lane);
+            if constexpr (F::kBlockScales) F::issue_scales(p, kvh, phys, istage, lane);
             istage = istage == ring + (F::kStages - 1) * F::kStageBytes ? ring : istage + F::kStageBytes;
             tok += kGroupWarps * kTileTokens;
             for (off += kGroupWarps * kTileTokens; off >= bs; off -= bs) ++blk;

@@ -3,6 +3,7 @@
 // src/kernels/kernel_types.cu:24-110) and dispatch to the kernels of this library.
 #include "nvk_internal.cuh"
 
+#include <cmath>
 #include <string>
 
 namespace nvk {
@@ -56,6 +57,27 @@ bool weights_overlap(const float* old_weights, const float* new_weights, int64_t
     return old_weights != nullptr && old_weights != new_weights && overlap(old_weights, bytes, new_weights, bytes);
 }
 int64_t index_bytes(int dtype) { return dtype == NVK_I64 ? 8 : 4; }
+// What the calls over a cache with block scales have in common.
+int check_blocks8(const char* what, int dtype, int cache_dtype, int num_kv_heads, int head_dim) {
+    if (cache_dtype != NVK_I8 && cache_dtype != NVK_E4M3) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: cache elements are int8 or e4m3", what);
+    return check_int4(what, dtype, num_kv_heads, head_dim);
+}
+// Neither the same nor apart.
+bool partly(const void* a, const void* b, int64_t bytes) { return a != b && overlap(a, bytes, b, bytes); }
+// What the calls over the tables of requests have in common.
+int check_requests(const char* what, const void* lens, const void* blocks, const void* free_blocks, const void* count, const void* new_lens, const void* new_count,
+                   int64_t batch, int64_t rows, int64_t row_blocks, int64_t num_free, int block_size, const void* request_rows, int index_dtype) {
+    if (!lens || !blocks || !free_blocks || !count || !new_lens || !new_count) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: lengths, blocks and counts must be defined", what);
+    if (!is_index_dtype(index_dtype)) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: index tensors must be int32 or int64", what);
+    if (batch < 0 || rows <= 0 || row_blocks <= 0 || num_free <= 0 || block_size <= 0) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: sizes must be positive", what);
+    if (!request_rows && rows < batch) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: without request_rows there has to be a row for every request", what);
+    const int64_t wide = index_bytes(index_dtype);
+    for (const void* p : {lens, blocks, free_blocks, count, new_lens, new_count, request_rows})
+        if (!aligned_to(p, static_cast<size_t>(wide))) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: misaligned tensor", what);
+    if (partly(lens, new_lens, rows * wide) || partly(count, new_count, wide))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "%s: new lengths and count are the old ones' memory or do not overlap with it", what);
+    return NVK_OK;
+}
 
 int launch_prefill(const PrefillArgs& a) {
     if (prefill_tc_supported(a) && !prefill_takes_tiles(a)) return launch_prefill_tc(a);
@@ -311,6 +333,188 @@ int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, cons
         if (!aligned_to(workspace, 16)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (int4): workspace must be 16-byte aligned");
     }
     return launch_decode_int4(a, k_params, v_params);
+}
+
+int nvk_store_kvcache_blocks8(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride, void* k_cache, void* v_cache,
+                              float* k_scale, float* v_scale, int cache_dtype, const void* cu_seqlens_q, int cu_seqlens_q_dtype,
+                              const void* context_lens, int context_lens_dtype, const void* block_tables, int block_tables_dtype, int64_t num_seqs,
+                              int64_t total_q, int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int head_dim, int block_size, int dtype,
+                              void* stream) {
+    if (!key || !value || !k_cache || !v_cache || !k_scale || !v_scale || !context_lens || !block_tables)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_blocks8: key, value, caches, scales, context_lens and block_tables must be defined");
+    if (const int rc = check_blocks8("store_kvcache_blocks8", dtype, cache_dtype, num_kv_heads, head_dim); rc != NVK_OK) return rc;
+    if (!is_index_dtype(context_lens_dtype) || !is_index_dtype(block_tables_dtype) || (cu_seqlens_q && !is_index_dtype(cu_seqlens_q_dtype)))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "cu_seqlens_q, context_lens and block_tables must be int32 or int64");
+    if (num_seqs < 0 || total_q < 0 || max_blocks <= 0 || num_cache_blocks <= 0 || block_size <= 0)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_blocks8: sizes must be positive");
+    if (!cu_seqlens_q && total_q != num_seqs)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_blocks8: without cu_seqlens_q there has to be one row for every sequence");
+    const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
+    if (key_row_stride < row || value_row_stride < row || key_row_stride % 8 != 0 || value_row_stride % 8 != 0)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_blocks8: row strides must be multiples of 8 elements, and no less than a row");
+    if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_blocks8: key, value and the caches must be 16-byte aligned, the scales 4-byte aligned");
+    if (num_seqs > (1LL << 30) / num_kv_heads || total_q >= (1LL << 31) - block_size || max_blocks > ((1LL << 31) - 1) / block_size || num_kv_heads > (1 << 24))
+        return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many sequences, tokens, heads or blocks");
+    if (num_seqs == 0 || total_q == 0) return NVK_OK;
+    return launch_store_blocks8(Blocks8StoreArgs{key, value, k_cache, v_cache, k_scale, v_scale, index_array(cu_seqlens_q, cu_seqlens_q_dtype),
+                                                 index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype), num_seqs, total_q,
+                                                 max_blocks, num_cache_blocks, key_row_stride, value_row_stride, num_kv_heads, block_size,
+                                                 cache_dtype == NVK_E4M3, dtype, static_cast<cudaStream_t>(stream)});
+}
+
+int nvk_gather_kvcache_blocks8(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale, int cache_dtype,
+                               const void* cu_seqlens_k, int cu_seqlens_k_dtype, const void* block_tables, int block_tables_dtype, int64_t num_seqs,
+                               int64_t total_k, int64_t max_blocks, int64_t num_cache_blocks, int num_kv_heads, int head_dim, int block_size, void* key,
+                               void* value, int dtype, void* stream) {
+    if (!k_cache || !v_cache || !k_scale || !v_scale || !cu_seqlens_k || !block_tables || !key || !value)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: every tensor must be defined");
+    if (const int rc = check_blocks8("gather_kvcache_blocks8", dtype, cache_dtype, num_kv_heads, head_dim); rc != NVK_OK) return rc;
+    if (!is_index_dtype(cu_seqlens_k_dtype) || !is_index_dtype(block_tables_dtype))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "cu_seqlens_k and block_tables must be int32 or int64");
+    if (num_seqs <= 0 || total_k < 0 || max_blocks <= 0 || num_cache_blocks <= 0 || block_size <= 0)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: sizes must be positive");
+    if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: key, value and the caches must be 16-byte aligned, the scales 4-byte aligned");
+    if (total_k == 0) return NVK_OK;
+    return launch_gather_blocks8(Blocks8GatherArgs{k_cache, v_cache, k_scale, v_scale, index_array(cu_seqlens_k, cu_seqlens_k_dtype),
+                                                   index_array(block_tables, block_tables_dtype), num_seqs, total_k, max_blocks, num_cache_blocks, num_kv_heads,
+                                                   block_size, cache_dtype == NVK_E4M3, key, value, dtype, static_cast<cudaStream_t>(stream)});
+}
+
+int nvk_decode_attention_paged_blocks8(const void* query, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                                       int cache_dtype, const void* context_lens, int context_lens_dtype, const void* block_tables,
+                                       int block_tables_dtype, int64_t batch, int64_t max_blocks, int64_t num_cache_blocks, int num_heads,
+                                       int num_kv_heads, int head_dim, int block_size, float scale, void* output, int dtype, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    if (!query || !k_cache || !v_cache || !k_scale || !v_scale || !context_lens || !block_tables || !output)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8) requires KV cache, scales, context_lens, and block_tables");
+    if (cache_dtype != NVK_I8 && cache_dtype != NVK_E4M3) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): cache elements are int8 or e4m3");
+    if (!is_index_dtype(context_lens_dtype) || !is_index_dtype(block_tables_dtype))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "context_lens and block_tables must be int32 or int64");
+    if (const int rc = check_decode_sizes(batch, max_blocks, num_cache_blocks, num_heads, num_kv_heads, head_dim, block_size); rc != NVK_OK) return rc;
+    if (!std::isfinite(scale)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): scale must be finite");
+    if (batch == 0) return NVK_OK;
+    const DecodeArgs a{query, k_cache, v_cache, index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype), output, batch,
+                       max_blocks, num_cache_blocks, num_heads, num_kv_heads, head_dim, block_size, scale, dtype, workspace, workspace_bytes,
+                       static_cast<cudaStream_t>(stream)};
+    if (!decode_blocks8_supported(a, k_scale, v_scale))
+        return fail(NVK_ERR_UNSUPPORTED, "decode attention (blocks8): F16 / BF16 queries, head_dim 128, at most 8 query heads per KV head, block_size a multiple "
+                                         "of 16; query and caches 16-byte aligned, output 8-byte and scales 4-byte aligned");
+    if (workspace != nullptr) {
+        const size_t need = decode_mma_workspace_needed(batch, num_heads, num_kv_heads, head_dim, max_blocks, block_size);
+        if (workspace_bytes < need)
+            return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): workspace of %zu bytes given, %zu needed", workspace_bytes, need);
+        if (!aligned_to(workspace, 16)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): workspace must be 16-byte aligned");
+    }
+    return launch_decode_blocks8(a, k_scale, v_scale, cache_dtype == NVK_E4M3);
+}
+
+int nvk_step_metadata(const void* new_lens, const void* request_rows, const void* request_lens, void* request_blocks, const void* free_blocks,
+                      const void* free_count, int64_t batch, int64_t num_request_rows, int64_t request_max_blocks, int64_t num_free_blocks,
+                      int64_t num_cache_blocks, int block_size, void* block_tables, int64_t max_blocks, void* context_lens, void* cu_seqlens_q,
+                      void* cu_seqlens_k, void* positions, void* slot_mapping, int64_t num_tokens, void* new_request_lens, void* new_free_count,
+                      int index_dtype, void* stream) {
+    if (!new_lens || !block_tables || !context_lens) return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: new_lens, block_tables and context_lens must be defined");
+    if (const int rc = check_requests("step_metadata", request_lens, request_blocks, free_blocks, free_count, new_request_lens, new_free_count, batch,
+                                      num_request_rows, request_max_blocks, num_free_blocks, block_size, request_rows, index_dtype); rc != NVK_OK)
+        return rc;
+    if (batch == 0 || max_blocks <= 0 || num_cache_blocks <= 0 || num_tokens < 0) return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: sizes must be positive");
+    if (num_tokens > 0 && (!positions || !slot_mapping)) return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: positions and slot_mapping must be defined");
+    for (const void* p : {new_lens, static_cast<const void*>(block_tables), static_cast<const void*>(context_lens), static_cast<const void*>(cu_seqlens_q),
+                          static_cast<const void*>(cu_seqlens_k), static_cast<const void*>(positions), static_cast<const void*>(slot_mapping)})
+        if (!aligned_to(p, static_cast<size_t>(index_bytes(index_dtype)))) return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: misaligned tensor");
+    if (index_dtype == NVK_I32 && num_cache_blocks > ((1LL << 31) - 1) / block_size)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: slots of that many blocks need int64");
+    StepArgs a{};
+    auto index = [&](const void* p) { return index_array(p, index_dtype); };
+    a.new_lens = index(new_lens); a.rows = index(request_rows); a.lens = index(request_lens); a.free_count = index(free_count);
+    a.request_blocks = request_blocks; a.free_blocks = const_cast<void*>(free_blocks);
+    a.block_tables = block_tables; a.context_lens = context_lens; a.cu_q = cu_seqlens_q; a.cu_k = cu_seqlens_k;
+    a.positions = positions; a.slots = slot_mapping; a.new_request_lens = new_request_lens; a.new_free_count = new_free_count;
+    a.batch = batch; a.num_rows = num_request_rows; a.row_blocks = request_max_blocks; a.num_free = num_free_blocks;
+    a.num_cache_blocks = num_cache_blocks; a.max_blocks = max_blocks; a.num_tokens = num_tokens;
+    a.block_size = block_size; a.wide = index_dtype == NVK_I64 ? 1 : 0;
+    a.stream = static_cast<cudaStream_t>(stream);
+    return launch_step_metadata(a);
+}
+
+int nvk_release_blocks(const void* request_rows, const void* first_blocks, const void* request_lens, const void* request_blocks, void* free_blocks,
+                       const void* free_count, int64_t batch, int64_t num_request_rows, int64_t request_max_blocks, int64_t num_free_blocks,
+                       int block_size, void* new_request_lens, void* new_free_count, int index_dtype, void* stream) {
+    if (const int rc = check_requests("release_blocks", request_lens, request_blocks, free_blocks, free_count, new_request_lens, new_free_count, batch,
+                                      num_request_rows, request_max_blocks, num_free_blocks, block_size, request_rows, index_dtype); rc != NVK_OK)
+        return rc;
+    if (!aligned_to(first_blocks, static_cast<size_t>(index_bytes(index_dtype)))) return fail(NVK_ERR_INVALID_ARGUMENT, "release_blocks: misaligned tensor");
+    StepArgs a{};
+    auto index = [&](const void* p) { return index_array(p, index_dtype); };
+    a.rows = index(request_rows); a.first_blocks = index(first_blocks); a.lens = index(request_lens); a.free_count = index(free_count);
+    a.request_blocks = const_cast<void*>(request_blocks); a.free_blocks = free_blocks;
+    a.new_request_lens = new_request_lens; a.new_free_count = new_free_count;
+    a.batch = batch; a.num_rows = num_request_rows; a.row_blocks = request_max_blocks; a.num_free = num_free_blocks;
+    a.block_size = block_size; a.wide = index_dtype == NVK_I64 ? 1 : 0;
+    a.stream = static_cast<cudaStream_t>(stream);
+    return launch_release_blocks(a);
+}
+
+int nvk_rotary_embedding(const void* query, const void* key, const void* positions, int positions_dtype, const float* inv_freq, float attention_factor,
+                         int64_t rows, int num_q_heads, int num_kv_heads, int head_dim, int rotary_dim, int interleaved, int64_t query_row_stride,
+                         int64_t key_row_stride, void* query_out, void* key_out, int64_t query_out_row_stride, int64_t key_out_row_stride, int dtype,
+                         void* stream) {
+    if (!query || !query_out || !positions || !inv_freq) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: query, query_out, positions and inv_freq must be defined");
+    if ((key == nullptr) != (key_out == nullptr)) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: key and key_out go together");
+    if (!is_compute_dtype(dtype)) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: query must be float16, bfloat16, or float32");
+    if (!is_index_dtype(positions_dtype)) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: positions must be int32 or int64");
+    if (rows < 0 || num_q_heads <= 0 || (key && num_kv_heads <= 0) || head_dim <= 0) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: sizes must be positive");
+    if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
+        return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: rotary_dim must be even, positive and at most head_dim");
+    if (head_dim > 1024) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: head_dim must be at most 1024 (got %d)", head_dim);
+    const int64_t size = static_cast<int64_t>(dtype_size(dtype));
+    auto check = [&](const void* in, int64_t in_stride, const void* out, int64_t out_stride, int heads) -> int {
+        const int64_t row = static_cast<int64_t>(heads) * head_dim;
+        if (in_stride < row || out_stride < row) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: a row stride is less than a row");
+        if (!aligned_to(in, static_cast<size_t>(size)) || !aligned_to(out, static_cast<size_t>(size))) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: misaligned tensor");
+        const int64_t last = rows > 0 ? rows - 1 : 0;
+        if ((in != out || in_stride != out_stride) && rows > 0 && overlap(in, (last * in_stride + row) * size, out, (last * out_stride + row) * size))
+            return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: an output is its input, with its stride, or does not overlap with it");
+        return NVK_OK;
+    };
+    if (const int rc = check(query, query_row_stride, query_out, query_out_row_stride, num_q_heads); rc != NVK_OK) return rc;
+    if (key) {
+        if (const int rc = check(key, key_row_stride, key_out, key_out_row_stride, num_kv_heads); rc != NVK_OK) return rc;
+    }
+    if (!aligned_to(positions, static_cast<size_t>(index_bytes(positions_dtype))) || !aligned_to(inv_freq, 4))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: misaligned tensor");
+    if (rows == 0) return NVK_OK;
+    return launch_rotary(RotaryArgs{query, key, query_out, key_out, query_row_stride, key_row_stride, query_out_row_stride, key_out_row_stride,
+                                    index_array(positions, positions_dtype), inv_freq, attention_factor, rows, num_q_heads, num_kv_heads, head_dim, rotary_dim,
+                                    interleaved != 0, dtype, static_cast<cudaStream_t>(stream)});
+}
+
+int nvk_rotary_inv_freq(float* inv_freq, float* attention_factor, int rotary_dim, double base, int scaling, double factor, double original_positions,
+                        double low_turns, double high_turns) {
+    if (!inv_freq || !attention_factor) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_inv_freq: inv_freq and attention_factor must be defined");
+    if (rotary_dim <= 0 || rotary_dim % 2 != 0 || !(base > 0.0) || !std::isfinite(base)) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_inv_freq: rotary_dim must be even, base positive");
+    if (scaling < NVK_ROPE_PLAIN || scaling > NVK_ROPE_YARN) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_inv_freq: no such scaling (%d)", scaling);
+    if (scaling != NVK_ROPE_PLAIN && (!(factor >= 1.0) || !std::isfinite(factor))) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_inv_freq: factor must be at least 1");
+    if (scaling == NVK_ROPE_BASE && rotary_dim <= 2) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_inv_freq: a scaled base needs more than one pair");
+    const bool parts = scaling == NVK_ROPE_PARTS || scaling == NVK_ROPE_YARN;
+    if (parts && (!(original_positions > 0.0) || !(high_turns > low_turns)))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_inv_freq: original_positions must be positive, high_turns above low_turns");
+    if (scaling == NVK_ROPE_BASE) base *= std::pow(factor, static_cast<double>(rotary_dim) / (rotary_dim - 2));
+    for (int i = 0; i < rotary_dim / 2; ++i) {
+        const double theta = std::pow(base, -2.0 * i / rotary_dim);
+        double f = theta;
+        if (scaling == NVK_ROPE_LINEAR) f = theta / factor;
+        if (parts) {
+            const double turns = original_positions * theta / 6.283185307179586;
+            const double g = std::fmin(std::fmax((turns - low_turns) / (high_turns - low_turns), 0.0), 1.0);
+            f = (1.0 - g) * theta / factor + g * theta;
+        }
+        inv_freq[i] = static_cast<float>(f);
+    }
+    *attention_factor = scaling == NVK_ROPE_YARN ? static_cast<float>(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return NVK_OK;
 }
 
 size_t nvk_decode_attention_weights_workspace_bytes(int64_t batch, int num_heads, int num_kv_heads, int head_dim, int64_t max_blocks, int block_size) {

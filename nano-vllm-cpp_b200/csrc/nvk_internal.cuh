@@ -173,6 +173,55 @@ int launch_gather_int4(const void* k_cache, const void* v_cache, const void* k_p
                        void* value, int dtype, cudaStream_t stream);
 bool decode_int4_supported(const DecodeArgs& a, const void* k_params, const void* v_params);
 int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_params);
+// 8-bit KV cache with a scale for each (cache block, KV head) (kv_blocks8.cu; tensor-core decode in decode_attn.cu)
+struct Blocks8StoreArgs {
+    const void* key; const void* value; void* k_cache; void* v_cache; float* k_scale; float* v_scale;
+    IndexArray cu;               // of the new rows; none: one for each sequence
+    IndexArray context_lens; IndexArray block_tables;
+    int64_t num_seqs, total_q, max_blocks, num_cache_blocks, key_stride, value_stride;
+    int num_kv_heads, block_size;
+    bool fp8;                    // e4m3 elements, else int8
+    int dtype;
+    cudaStream_t stream;
+};
+struct Blocks8GatherArgs {
+    const void* k_cache; const void* v_cache; const float* k_scale; const float* v_scale;
+    IndexArray cu; IndexArray block_tables;
+    int64_t num_seqs, total, max_blocks, num_cache_blocks;
+    int num_kv_heads, block_size;
+    bool fp8;
+    void* key; void* value;
+    int dtype;
+    cudaStream_t stream;
+};
+int launch_store_blocks8(const Blocks8StoreArgs& a);
+int launch_gather_blocks8(const Blocks8GatherArgs& a);
+bool decode_blocks8_supported(const DecodeArgs& a, const float* k_scale, const float* v_scale);
+int launch_decode_blocks8(const DecodeArgs& a, const float* k_scale, const float* v_scale, bool fp8);
+// Metadata of a step from its requests' lengths, and blocks given back (step_metadata.cu)
+struct StepArgs {
+    IndexArray new_lens, rows, lens, free_count, first_blocks;   // (new_lens: of a step; first_blocks: of a release)
+    void *request_blocks, *free_blocks;
+    void *block_tables, *context_lens, *cu_q, *cu_k, *positions, *slots, *new_request_lens, *new_free_count;
+    int64_t batch, num_rows, row_blocks, num_free, num_cache_blocks, max_blocks, num_tokens;
+    int block_size, wide;
+    cudaStream_t stream;
+};
+int launch_step_metadata(const StepArgs& a);
+int launch_release_blocks(const StepArgs& a);
+// Rotary positions (rotary.cu); strides are elements from a row to the next
+struct RotaryArgs {
+    const void* query; const void* key; void* query_out; void* key_out;   // no key: queries alone
+    int64_t query_stride, key_stride, query_out_stride, key_out_stride;
+    IndexArray positions; const float* inv_freq;
+    float factor;
+    int64_t rows;
+    int num_q_heads, num_kv_heads, head_dim, rotary_dim;
+    bool interleaved;
+    int dtype;
+    cudaStream_t stream;
+};
+int launch_rotary(const RotaryArgs& a);
 // Decode that adds up the weights of every key (decode_attn.cu), and the eviction that goes by them (evict.cu).  A 16-bit cache has no params.
 struct KeyWeights {
     const float* old_weights; float* new_weights;   // [num_rows, Hkv, row_keys]; old: may be null (zeros) or the new ones themselves

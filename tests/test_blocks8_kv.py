@@ -1,0 +1,570 @@
+"""8-bit paged KV cache with scales of blocks: nvk_store_kvcache_blocks8, nvk_gather_kvcache_blocks8, nvk_decode_attention_paged_blocks8.
+
+The reference has no such cache, so the format is pinned by the 64-bit restatement of its definition in ref_blocks8.py (checked by hand on the CPU): the
+store and the gather bit for bit, the decode within what its roundings allow."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import ref_blocks8 as ref
+from util import entry, nvk
+
+D = 128
+TINY = {"bfloat16": 2.0 ** -134, "float16": 2.0 ** -25}       # half of the smallest number
+
+
+@pytest.fixture(scope="module")
+def built():
+    entry.build()
+    return nvk()
+
+
+# ---- on the CPU --------------------------------------------------------------------------------------------------------------
+def test_scales_by_hand():
+    for kind, top in ref.TOP.items():
+        a = np.array([0.0, top, top * 1.0001, top / 2, top / 2 * 1.0001, 1.0, 2.0 ** -133, np.inf, np.nan, 3.3895313892515355e38])
+        s = ref.scale_for(a, kind)
+        assert s[:5].tolist() == [2.0 ** -126, 1.0, 2.0, 0.5, 1.0] and s[6] == 2.0 ** -126 and np.isnan(s[7:9]).all()
+        assert s[5] == (2.0 ** -6 if kind == "int8" else 2.0 ** -8) and s[9] == (2.0 ** 122 if kind == "int8" else 2.0 ** 120)
+
+
+def test_elements_by_hand():
+    assert ref.nearest([0.5, 1.5, -2.5, 126.5, np.nan], "int8").tolist() == [0, 2, -2, 126, 0]
+    x = ref.nearest([0.0, 1.0625, 1.1875, 2.0 ** -10, 2.0 ** -9, 1.5 * 2.0 ** -9, 447.0, 432.0, -17.0], "e4m3")
+    assert x.tolist() == [0.0, 1.0, 1.25, 0.0, 2.0 ** -9, 2.0 ** -8, 448.0, 448.0, -16.0]   # (432 and -17 lie between two: to the even one)
+
+
+def test_a_block_that_grows():
+    c = ref.Cache(2, 4, 1, "int8")
+    row = lambda v: np.full((1, 1, D), v)
+    c.store(row(127.0), [0, 1], [1], [[1]])
+    assert c.scale[1, 0] == 1.0 and c.data[1, 0, 0, 0] == 127
+    c.store(row(129.0), [0, 1], [2], [[1]])
+    assert c.scale[1, 0] == 2.0 and c.data[1, 0, 0, 0] == 64 and c.data[1, 1, 0, 0] == 64     # 63.5 and 64.5, to even
+    c.store(row(1.0), [0, 1], [3], [[1]])
+    assert c.scale[1, 0] == 2.0 and c.data[1, 2, 0, 0] == 0
+    c.store(row(np.inf), [0, 1], [4], [[1]])
+    assert np.isnan(c.rows([1], 4)).all()
+    c.store(row(3.0), [0, 1], [1], [[1]])                                                     # anew
+    assert c.scale[1, 0] == 2.0 ** -5 and c.rows([1], 1)[0, 0, 0] == 3.0
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_less_than_a_step_off(kind):
+    """However often a block grew: int8 by less than one step, e4m3 by less than twice its half step (or by one step of its smallest numbers)."""
+    rng = np.random.default_rng(5)
+    c = ref.Cache(1, 64, 2, kind)
+    x = rng.standard_normal((64, 2, D)) * 2.0 ** np.linspace(-4, 4, 64)[:, None, None]
+    for i in range(64):
+        c.store(x[i:i + 1], [0, 1], [i + 1], [[0]])
+    step = c.scale[0][:, None]
+    most = step if kind == "int8" else np.maximum(np.abs(x) * 2.0 ** -3, step * 2.0 ** -9)
+    assert (np.abs(c.rows([0], 64) - x) < most).all()
+
+
+def _call(lib, name, *args):
+    rc = getattr(lib.lib(), name)(*args)
+    return rc, lib.lib().nvk_last_error().decode()
+
+
+L, I = ctypes.c_int64, ctypes.c_int
+P, ODD = ctypes.c_void_p(256), ctypes.c_void_p(264)
+
+
+def _store_args(**change):
+    a = dict(key=P, value=P, ks=L(256), vs=L(256), k_cache=P, v_cache=P, k_scale=P, v_scale=P, kind=I(5), cu=P, cu_dtype=I(3), ctx=P, ctx_dtype=I(3), bt=P, bt_dtype=I(4),
+             seqs=L(2), total=L(5), max_blocks=L(3), blocks=L(4), hkv=I(2), d=I(128), bs=I(16), dtype=I(1), stream=None)
+    a.update(change)
+    return a.values()
+
+
+def _gather_args(**change):
+    a = dict(k_cache=P, v_cache=P, k_scale=P, v_scale=P, kind=I(6), cu=P, cu_dtype=I(3), bt=P, bt_dtype=I(4), seqs=L(2), total=L(10), max_blocks=L(2), blocks=L(4),
+             hkv=I(2), d=I(128), bs=I(16), key=P, value=P, dtype=I(0), stream=None)
+    a.update(change)
+    return a.values()
+
+
+def _decode_args(**change):
+    a = dict(q=P, k_cache=P, v_cache=P, k_scale=P, v_scale=P, kind=I(5), ctx=P, ctx_dtype=I(3), bt=P, bt_dtype=I(3), batch=L(2), max_blocks=L(40), blocks=L(4), hq=I(8),
+             hkv=I(2), d=I(128), bs=I(256), scale=ctypes.c_float(1.0), out=P, dtype=I(1), ws=None, ws_bytes=ctypes.c_size_t(0), stream=None)
+    a.update(change)
+    return a.values()
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(key=None), 1, "defined"), (dict(v_scale=None), 1, "defined"), (dict(bt=None), 1, "defined"), (dict(kind=I(1)), 1, "int8 or e4m3"), (dict(dtype=I(2)), 3, "F16 or BF16"),
+    (dict(d=I(64)), 3, "128"), (dict(hkv=I(0)), 1, "positive"), (dict(ctx_dtype=I(5)), 1, "int32 or int64"), (dict(cu_dtype=I(1)), 1, "int32 or int64"),
+    (dict(seqs=L(-1)), 1, "positive"), (dict(blocks=L(0)), 1, "positive"), (dict(bs=I(0)), 1, "positive"), (dict(cu=None), 1, "one row for every"),
+    (dict(ks=L(248)), 1, "strides"), (dict(vs=L(260)), 1, "strides"), (dict(key=ODD), 1, "aligned"), (dict(k_scale=ctypes.c_void_p(258)), 1, "aligned"),
+    (dict(total=L(1 << 31)), 3, "too many"), (dict(max_blocks=L(1 << 30)), 3, "too many"), (dict(seqs=L(1 << 30)), 3, "too many"), (dict(total=L(0)), 0, ""),
+    (dict(seqs=L(0)), 0, "")])
+def test_store_refuses(built, change, code, word):
+    rc, said = _call(built, "nvk_store_kvcache_blocks8", *_store_args(**change))
+    assert rc == code and (rc == 0 or word in said), said
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(cu=None), 1, "defined"), (dict(k_scale=None), 1, "defined"), (dict(kind=I(0)), 1, "int8 or e4m3"), (dict(dtype=I(2)), 3, "F16 or BF16"), (dict(d=I(256)), 3, "128"),
+    (dict(cu_dtype=I(0)), 1, "int32 or int64"), (dict(seqs=L(0)), 1, "positive"), (dict(total=L(-1)), 1, "positive"), (dict(max_blocks=L(0)), 1, "positive"),
+    (dict(value=ODD), 1, "aligned"), (dict(total=L(0)), 0, ""), (dict(total=L(1 << 40)), 3, "too many")])
+def test_gather_refuses(built, change, code, word):
+    rc, said = _call(built, "nvk_gather_kvcache_blocks8", *_gather_args(**change))
+    assert rc == code and (rc == 0 or word in said), said
+
+
+@pytest.mark.parametrize("change,code,word", [
+    (dict(q=None), 1, "requires"), (dict(v_scale=None), 1, "requires"), (dict(kind=I(4)), 1, "int8 or e4m3"), (dict(scale=ctypes.c_float(float("inf"))), 1, "finite"),
+    (dict(scale=ctypes.c_float(float("nan"))), 1, "finite"), (dict(ctx_dtype=I(1)), 1, "int32 or int64"),
+    (dict(batch=L(-1)), 1, "positive"), (dict(hq=I(7)), 1, "divisible"), (dict(dtype=I(2)), 3, "F16 / BF16"), (dict(d=I(64)), 3, "head_dim"),
+    (dict(hq=I(18)), 3, "8 query heads"), (dict(bs=I(24)), 3, "multiple"), (dict(q=ODD), 3, "aligned"), (dict(ws=P, ws_bytes=ctypes.c_size_t(64)), 1, "workspace"),
+    (dict(ws=ODD, ws_bytes=ctypes.c_size_t(1 << 30)), 1, "aligned"), (dict(batch=L(0)), 0, "")])
+def test_decode_refuses(built, change, code, word):
+    rc, said = _call(built, "nvk_decode_attention_paged_blocks8", *_decode_args(**change))
+    assert rc == code and (rc == 0 or word in said), said
+
+
+# ---- on the GPU --------------------------------------------------------------------------------------------------------------
+def _typed(x, dtype):
+    """float64 -> the 16-bit type, on the GPU, and as float64 again."""
+    import torch
+    t = torch.from_numpy(np.ascontiguousarray(x, np.float64)).to(getattr(torch, dtype))
+    return t.cuda(), t.double().numpy()
+
+
+class Both:
+    """K and V caches on the GPU and here."""
+
+    def __init__(self, blocks, bs, hkv, kind, garbage=True):
+        import torch
+        self.kind, self.bs, self.hkv, self.blocks = kind, bs, hkv, blocks
+        self.ref = [ref.Cache(blocks, bs, hkv, kind) for _ in range(2)]
+        self.data, self.scale = [], []
+        for _ in range(2):   # what was there before: anything
+            d = torch.randint(0, 256, (blocks, bs, hkv, D), dtype=torch.uint8, device="cuda") if garbage else torch.zeros((blocks, bs, hkv, D), dtype=torch.uint8, device="cuda")
+            self.data.append(d.view(torch.int8 if kind == "int8" else torch.float8_e4m3fn))
+            self.scale.append(torch.full((blocks, hkv), 2.0 ** 60 if garbage else 0.0, device="cuda"))
+        self.seen = {}       # rows of a block that mean something
+
+    def store(self, x, cu, lens, tables, index="int32", one=False):
+        """x: (k, v) on the GPU and here."""
+        import torch
+        up = lambda v: torch.as_tensor(np.asarray(v), dtype=getattr(torch, index)).cuda()
+        behind = [d.view(torch.uint8).clone() for d in self.data]
+        nvk().store_kvcache_blocks8(x[0][0], x[1][0], *self.data, *self.scale, None if one else up(cu), up(lens), up(tables))
+        for w in range(2):
+            for block in self.ref[w].store(x[w][1], cu, lens, tables):
+                self.seen[block] = 0
+        for s, total in enumerate(lens):
+            for pos in range(max(int(total) - (cu[s + 1] - cu[s]), 0), int(total)):
+                if pos // self.bs < len(tables[s]) and 0 <= tables[s][pos // self.bs] < self.blocks:
+                    self.seen[int(tables[s][pos // self.bs])] = pos % self.bs + 1
+        self.same(behind)
+
+    def same(self, behind):
+        import torch
+        for w in range(2):
+            got, scale = self.data[w].double() if self.kind == "int8" else self.data[w].float().double(), self.scale[w].double().cpu().numpy()
+            got = got.cpu().numpy()
+            for block in range(self.blocks):
+                n = self.seen.get(block, 0)
+                if n:
+                    assert np.array_equal(scale[block], self.ref[w].scale[block], equal_nan=True), (w, block, scale[block], self.ref[w].scale[block])
+                    assert np.array_equal(got[block, :n], self.ref[w].data[block, :n], equal_nan=True), (w, block)
+                # rows behind the last one, and blocks of nobody
+                assert torch.equal(self.data[w].view(torch.uint8)[block, n:], behind[w][block, n:]), (w, block)
+
+
+def _tables(rng, need, width, blocks):
+    perm, out, at = rng.permutation(blocks), np.full((len(need), width), -1, np.int64), 0
+    for i, n in enumerate(need):
+        out[i, :n] = perm[at:at + n]
+        at += n
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("bs,hkv,index", [(16, 1, "int32"), (16, 8, "int64"), (64, 3, "int32"), (256, 2, "int32"), (48, 2, "int64"), (512, 1, "int32"), (8, 5, "int32")])
+def test_store_in_several_steps(kind, dtype, bs, hkv, index):
+    """Prompts, then chunks and single rows that join blocks and raise their scales."""
+    rng = np.random.default_rng(bs + hkv)
+    seqs = 5
+    need = [6] * seqs
+    blocks = sum(need) + 2
+    c = Both(blocks, bs, hkv, kind)
+    tables = _tables(rng, need, 6, blocks)
+    lens = np.zeros(seqs, np.int64)
+    for step in range(7):
+        one = step >= 4
+        new = np.ones(seqs, np.int64) if one else rng.integers(0, bs + 5, seqs)
+        if step == 0:
+            new[:] = [0, 1, bs, bs + 1, 2 * bs + 3]
+        lens = np.minimum(lens + new, 6 * bs)
+        new = np.minimum(new, lens)
+        cu = np.concatenate([[0], np.cumsum(new)]).tolist()
+        x = [_typed(rng.standard_normal((cu[-1], hkv, D)) * 2.0 ** rng.uniform(-2, 1 + step, (cu[-1], 1, 1)), dtype) for _ in range(2)]
+        c.store(x, cu, lens.tolist(), tables.tolist(), index, one)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_store_of_hard_values(kind, dtype):
+    """Zeros, borders between elements and between scales, the largest and the smallest numbers, infinities and NaN, alone and joining a block."""
+    rng = np.random.default_rng(9)
+    tiny, huge = {"bfloat16": (2.0 ** -133, 3.3895313892515355e38), "float16": (2.0 ** -24, 65504.0)}[dtype]
+    top = ref.TOP[kind]
+    vectors = [np.zeros(D), np.full(D, -top), np.full(D, top), np.arange(D) - 64.0, (np.arange(D) - 64) * 0.5, np.full(D, 128.0 if kind == "int8" else 464.0),
+               np.arange(D) % 7 * tiny, -np.arange(D) * 16 * tiny, np.where(np.arange(D) % 2, huge, -huge), np.arange(D) * huge / 200, np.full(D, 2.0 ** -9),
+               np.where(np.arange(D) == 5, np.inf, 1.0), np.where(np.arange(D) == 127, np.nan, 2.0), np.where(np.arange(D) == 0, -np.inf, 0.0), np.full(D, 1.0)]
+    n = len(vectors)
+    # each pair of vectors, one joining the other in a block of its own, as one call and as two
+    pairs = [(a, b) for a in vectors for b in vectors]
+    x = np.asarray(pairs).reshape(-1, 1, D)
+    blocks = len(pairs)
+    tables = np.arange(blocks)[:, None]
+    both = [_typed(x, dtype), _typed(x[::-1], dtype)]
+    c = Both(blocks, 16, 1, kind)
+    c.store(both, list(range(0, 2 * blocks + 1, 2)), [2] * blocks, tables.tolist())
+    c = Both(blocks, 16, 1, kind)
+    for i in range(2):
+        part = [(t.view(blocks, 2, 1, D)[:, i].contiguous(), v.reshape(blocks, 2, 1, D)[:, i]) for t, v in both]
+        c.store(part, list(range(blocks + 1)), [i + 1] * blocks, tables.tolist(), one=i == 1)
+
+
+@pytest.mark.gpu
+def test_store_skips_what_has_no_place():
+    """Negative positions (a request that waits), blocks outside the cache, rows beyond the table, rows behind the last sequence."""
+    rng = np.random.default_rng(10)
+    c = Both(6, 16, 2, "int8")
+    tables = [[0, 1], [2, 99], [-1, 3], [4, 5]]
+    cu, lens = [0, 5, 30, 60, 100], [0, 25, 30, 40]
+    x = [_typed(rng.standard_normal((107, 2, D)), "bfloat16") for _ in range(2)]
+    c.store(x, cu, lens, tables)
+    assert sorted(c.seen) == [2, 3, 4, 5]
+    one = [(t[:4], v[:4]) for t, v in x]
+    c.store(one, [0, 1, 2, 3, 4], [0, -3, 33, 32], tables, one=True)
+
+
+@pytest.mark.gpu
+def test_store_of_packed_rows_and_on_another_stream():
+    import torch
+    rng = np.random.default_rng(11)
+    hq, hkv, n, bs = 4, 2, 70, 16
+    qkv, here = _typed(rng.standard_normal((n, (hq + 2 * hkv) * D)), "bfloat16")
+    parts = [((slice(None), slice((hq + i * hkv) * D, (hq + (i + 1) * hkv) * D))) for i in range(2)]
+    x = [(qkv[p].unflatten(1, (hkv, D)), here[p].reshape(n, hkv, D)) for p in parts]
+    c = Both(8, bs, hkv, "e4m3")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        c.store(x, [0, n], [n], [list(range(7, 2, -1))])
+    one = [(t[-1:], v[-1:]) for t, v in x]
+    c.store(one, [0, 1], [n + 1], [list(range(7, 2, -1))], one=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("bs,hkv,lens,index", [(16, 2, [40, 0, 1, 16], "int32"), (256, 1, [300], "int64"), (48, 3, [1, 47, 48, 49, 200], "int32")])
+def test_gather(kind, dtype, bs, hkv, lens, index):
+    import torch
+    rng = np.random.default_rng(bs)
+    need = [-(-n // bs) for n in lens]
+    blocks, width = sum(need) + 1, max(need) + 1
+    tables = _tables(rng, need, width, blocks)
+    c = Both(blocks, bs, hkv, kind)
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    x = [_typed(rng.standard_normal((cu[-1], hkv, D)) * 2.0 ** rng.uniform(-18, 8, (cu[-1], hkv, 1)), dtype) for _ in range(2)]
+    c.store(x, cu, lens, tables.tolist(), index)
+    tables[-1, 0] = blocks + 5   # (reads as zeros)
+    up = lambda v: torch.as_tensor(np.asarray(v), dtype=getattr(torch, index)).cuda()
+    out = [torch.full((cu[-1] + 3, hkv, D), float("nan"), dtype=getattr(torch, dtype), device="cuda") for _ in range(2)]
+    nvk().gather_kvcache_blocks8(*c.data, *c.scale, up(cu), up(tables), hkv, D, bs, *out)
+    for w in range(2):
+        want = np.concatenate([c.ref[w].rows(tables[s], n) for s, n in enumerate(lens)] + [np.zeros((3, hkv, D))])
+        assert torch.equal(out[w].cpu().double(), torch.from_numpy(want).to(out[w].dtype).double())
+
+
+# How far a decode output can be off.  A score: the query to f16 (2^-25 of the head's largest, whose power of two is taken out first), 128 products summed in fp32 and 8
+# operations more, each addition by 2^-23 of the sum of magnitudes at most (the MMA may cut off instead of rounding).  A weight p by a factor e^(2 score error), its
+# exponential by 2^-20; p s to f16: 2^-11 of itself, or, where it is less than 2^-10 of the head's largest, 2^-22 of that; sums over the keys and the merges: 2^-23 for every one of
+# some 300 operations of a chain, of the sum of magnitudes.
+def _bound(c, table, n, q, scale, dtype):
+    """(the output in 64 bits, how far it may be off)"""
+    k, v = (r.rows(table, n) for r in c.ref)
+    per = q.shape[0] // c.hkv
+    kk, vv = (np.repeat(np.abs(x), per, axis=1) for x in (k, v))          # [n, Hq, D]
+    score = abs(scale) * (136 * 2.0 ** -23 * np.einsum("hd,nhd->nh", np.abs(q), kk).max(0) + 2.0 ** -25 * np.abs(q).max(-1) * kk.sum(-1).max(0))
+    s = np.einsum("hd,nhd->hn", q, np.repeat(k, per, axis=1)) * scale
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    want, mags = (np.einsum("hn,nhd->hd", p, x) for x in (np.repeat(v, per, axis=1), vv))
+    blocks = np.array([table[i // c.bs] if i // c.bs < len(table) else -1 for i in range(n)])
+    steps = np.where(((blocks >= 0) & (blocks < c.blocks))[:, None], c.ref[1].scale[np.clip(blocks, 0, c.blocks - 1)], 0.0)   # [n, Hkv]
+    part = p * np.repeat(steps, per, axis=1).T                               # [Hq, n]
+    most = part.max(-1, keepdims=True)
+    numbers = np.repeat(np.divide(np.abs(v), steps[..., None], out=np.zeros_like(v), where=steps[..., None] > 0), per, axis=1)
+    tail = np.einsum("hn,nhd->hd", np.where(part < most * 2.0 ** -10, most * 2.0 ** -22, 0.0), numbers)
+    weight = 2 * score + 2.0 ** -11 + 2.0 ** -20 + 300 * 2.0 ** -23
+    return want, weight[:, None] * mags * 1.01 + tail + np.abs(want) * ref.HALF_STEP[dtype] + TINY[dtype]
+
+
+def _decode(c, q, lens, tables, index="int32", workspace=True, scale=0.09):
+    import torch
+    up = lambda v: torch.as_tensor(np.asarray(v), dtype=getattr(torch, index)).cuda()
+    out = torch.full_like(q, float("nan"))
+    b, hq = q.shape[:2]
+    bt = up(tables)
+    size = nvk().decode_attention_workspace_bytes(b, hq, c.hkv, D, bt.shape[1], c.bs)
+    ws = torch.full((max(16, size),), 0x7f, dtype=torch.uint8, device="cuda") if workspace else None
+    nvk().launch_decode_attention_paged_blocks8(q, *c.data, *c.scale, up(lens), bt, c.hkv, D, c.bs, scale, out, ws)
+    return out.double().cpu().numpy()
+
+
+def _check_decode(c, q, here, lens, tables, dtype, **more):
+    scale = more.get("scale", 0.09)
+    got = _decode(c, q, lens, tables, **more)
+    for s, n in enumerate(lens):
+        n = max(0, min(int(n), len(tables[s]) * c.bs))
+        if n == 0:
+            assert (got[s] == 0).all()
+            continue
+        want, most = _bound(c, tables[s], n, here[s], scale, dtype)
+        assert (np.abs(got[s] - want) <= most).all(), (s, np.abs(got[s] - want).max(), (np.abs(got[s] - want) / most).max())
+    return got
+
+
+def _filled(rng, kind, dtype, bs, hkv, lens, width=None, spread=1.0, std=1.0):
+    need = [-(-n // bs) for n in lens]
+    blocks = sum(need) + 1
+    tables = _tables(rng, need, width or max(max(need), 1), blocks)
+    c = Both(blocks, bs, hkv, kind)
+    cu = np.concatenate([[0], np.cumsum(lens)]).tolist()
+    x = [_typed(rng.standard_normal((cu[-1], hkv, D)) * std * 2.0 ** rng.uniform(-spread, spread, (cu[-1], 1, 1)), dtype) for _ in range(2)]
+    c.store(x, cu, lens, tables.tolist())
+    return c, tables
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("bs,hq,hkv,lens,width,index", [
+    (16, 32, 8, [1], None, "int32"), (256, 32, 8, [300], None, "int64"), (16, 4, 1, [15, 16, 17, 0, 33], 4, "int32"), (64, 14, 2, [700, 5, 64], 40, "int32"),
+    (256, 8, 8, [1000, 2049, 1], 16, "int64"), (32, 8, 1, [3000], 128, "int32"), (16, 6, 2, [100] * 40, 9, "int32")])
+def test_decode(kind, dtype, bs, hq, hkv, lens, width, index):
+    rng = np.random.default_rng(hq * bs + len(lens))
+    c, tables = _filled(rng, kind, dtype, bs, hkv, lens, width)
+    q, here = _typed(rng.standard_normal((len(lens), hq, D)) * 2.0, dtype)
+    a = _check_decode(c, q, here, lens, tables, dtype, index=index)
+    _check_decode(c, q, here, lens, tables, dtype, index=index, workspace=False)
+    again = _decode(c, q, lens, tables, index=index)
+    assert np.array_equal(a, again)
+    # one way out of the table: a length beyond it
+    long = [n + 10 ** 6 for n in lens[:1]] + lens[1:]
+    if len(tables[0]) == -(-lens[0] // bs) and lens[0] % bs == 0:
+        assert np.array_equal(_decode(c, q, long, tables, index=index), a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_decode_over_scales_far_apart(kind, dtype):
+    """Blocks whose values are 2^16 times the others' must not cost these their bits where hardly any attention goes to them."""
+    rng = np.random.default_rng(21)
+    lens = [640, 640]
+    c, tables = _filled(rng, kind, dtype, 16, 2, lens, spread=0.0)
+    import torch
+    # values of every fifth block far larger, keys of the same blocks turned away from the query
+    q = np.zeros((2, 4, D))
+    q[..., 0] = 8.0
+    for s in range(2):
+        for j, block in enumerate(tables[s]):
+            if j % 5 == 2:
+                for r, w in ((c.ref[1], 1),):
+                    r.scale[block] *= 2.0 ** 14
+                    c.scale[w][int(block)] *= 2.0 ** 14
+                c.ref[0].data[block, :, :, 0] = -100 if kind == "int8" else -96
+                c.data[0].view(torch.uint8)[int(block), :, :, 0] = (256 - 100) if kind == "int8" else int(torch.tensor(-96.0).to(torch.float8_e4m3fn).view(torch.uint8))
+    qd, here = _typed(q, dtype)
+    _check_decode(c, qd, here, lens, tables, dtype, scale=0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -100, 2.0 ** 14, 2.0 ** -60])
+def test_decode_with_queries_and_values_of_any_size(dtype, size):
+    if dtype == "float16" and size < 2.0 ** -30:
+        size = 2.0 ** -22
+    rng = np.random.default_rng(22)
+    lens = [200, 31]
+    c, tables = _filled(rng, "int8", dtype, 16, 2, lens, std=min(size, 2.0 ** 10))
+    q, here = _typed(rng.standard_normal((2, 8, D)) * size, dtype)
+    k = max(np.abs(r.rows(tables[0], 200)).max() for r in c.ref)
+    scale = float(1.0 / (size * k * 8))
+    if scale > float(np.finfo(np.float32).max):   # (no number of the call's type)
+        with pytest.raises(ValueError, match="finite"):
+            _decode(c, q, lens, tables, scale=scale)
+        return
+    _check_decode(c, q, here, lens, tables, dtype, scale=scale)
+
+
+@pytest.mark.gpu
+def test_decode_with_keys_alike_and_long_contexts():
+    """A mean over many keys, whose sums an offset of the elements would swamp."""
+    import torch
+    rng = np.random.default_rng(23)
+    lens, bs = [9000], 256
+    c, tables = _filled(rng, "int8", "float16", bs, 1, lens, width=40, spread=0.0)
+    q, here = _typed(np.zeros((1, 4, D)), "float16")
+    got = _check_decode(c, q, here, lens, tables, "float16")
+    mean = c.ref[1].rows(tables[0], 9000)[:, 0].mean(0)
+    # weights are 1 / 9000 each: f16 holds 2^-11 of p s; the errors of equal weights are alike, and go into all sums alike
+    assert np.abs(got[0] - mean).max() <= np.abs(mean).max() * 2.0 ** -10 + 1e-5
+
+
+@pytest.mark.gpu
+def test_a_block_of_nan_is_one_sequences_and_heads_own():
+    rng = np.random.default_rng(24)
+    lens = [100, 100, 100]
+    c, tables = _filled(rng, "int8", "bfloat16", 16, 2, lens)
+    x = np.ones((3, 2, D))
+    x[1, 1, 7] = np.nan
+    xs = _typed(x, "bfloat16")
+    c.store([xs, xs], [0, 1, 2, 3], [101] * 3, tables.tolist() if tables.shape[1] > 6 else np.pad(tables, ((0, 0), (0, 1))).tolist(), one=True)
+    q, here = _typed(rng.standard_normal((3, 8, D)), "bfloat16")
+    got = _decode(c, q, [101] * 3, tables if tables.shape[1] > 6 else np.pad(tables, ((0, 0), (0, 1))))
+    bad = np.isnan(got)
+    assert bad[1, 4:].all() and not bad[1, :4].any() and not bad[0].any() and not bad[2].any()
+
+
+@pytest.mark.gpu
+def test_blocks_outside_the_cache_read_as_zeros():
+    rng = np.random.default_rng(25)
+    lens = [64]
+    c, tables = _filled(rng, "e4m3", "bfloat16", 16, 1, lens)
+    tables[0, 1], tables[0, 2] = -1, 1 << 20
+    q, here = _typed(rng.standard_normal((1, 4, D)), "bfloat16")
+    _check_decode(c, q, here, lens, tables, "bfloat16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("change,word", [
+    (dict(k_cache="bfloat16"), "both be int8"), (dict(v_cache="uint8"), "both be int8"), (dict(k_scale="float16"), "float32"), (dict(scale_shape=(3, 2)), "every cache block"),
+    (dict(ctx=3), "every context length"), (dict(value=(2, 2, 64)), "same shape"), (dict(key_dim=2), "must be \\[rows")])
+def test_the_binding_refuses(change, word):
+    import torch
+    dt = lambda n, d: getattr(torch, change.get(n, d))
+    kc, vc = torch.zeros(4, 16, 2, D, dtype=dt("k_cache", "int8"), device="cuda"), torch.zeros(4, 16, 2, D, dtype=dt("v_cache", "int8"), device="cuda")
+    ks, vs = torch.zeros(change.get("scale_shape", (4, 2)), dtype=dt("k_scale", "float32"), device="cuda"), torch.zeros(4, 2, device="cuda")
+    key = torch.zeros((2, 2, D) if "key_dim" not in change else (2, 2 * D), dtype=torch.bfloat16, device="cuda")
+    value = torch.zeros(change.get("value", key.shape), dtype=torch.bfloat16, device="cuda")
+    ctx = torch.zeros(change.get("ctx", 2), dtype=torch.int32, device="cuda")
+    bt = torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match=word):
+        nvk().store_kvcache_blocks8(key, value, kc, vc, ks, vs, None, ctx, bt)
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+def test_a_run_of_steps_from_lengths_to_outputs(kind):
+    """Metadata, rotary positions, store, attention: a prefill step, then decode steps replayed as a graph, then a request that ends and one that takes its blocks."""
+    import torch
+    rng = np.random.default_rng(31)
+    hq, hkv, bs, dtype, width, pool = 8, 2, 16, "bfloat16", 8, 40
+    scale = D ** -0.5
+    f = nvk().rotary_inv_freq(64, 10000.0, "yarn", 4.0, 64.0)
+    freq = torch.tensor(f[0], device="cuda")
+    lens, held = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.full((6, width), -1, dtype=torch.int32, device="cuda")
+    free, count = torch.from_numpy(rng.permutation(pool)).int().cuda(), torch.tensor([pool], dtype=torch.int32, device="cuda")
+    c = Both(pool, bs, hkv, kind)
+    book = ref.Requests([0] * 6, held.tolist(), free.tolist(), pool, bs)
+
+    def metadata(batch, tokens):
+        i = lambda *s: torch.full(s, -9, dtype=torch.int32, device="cuda")
+        return i(batch, width), i(batch), i(batch + 1), i(batch + 1), i(tokens), i(tokens)
+
+    def enqueue(new, rows, meta, qkv, q, k):
+        nvk().step_metadata(new, rows, lens, held, free, count, bs, pool, *meta)
+        parts = [qkv[:, a * D:b * D].unflatten(1, (b - a, D)) for a, b in ((0, hq), (hq, hq + hkv), (hq + hkv, hq + 2 * hkv))]
+        nvk().rotary_embedding(parts[0], parts[1], meta[4], freq, False, f[1], q, k)
+        return parts[2]
+
+    def here(qkv, positions):
+        x = qkv.double().cpu().numpy().reshape(len(qkv), -1, D)
+        turned = ref.rotary(x[:, :hq + hkv], positions, freq.double().tolist(), False, f[1])
+        return torch.from_numpy(turned).to(torch.bfloat16).double().numpy(), x[:, hq + hkv:]
+
+    # prefill: 20, 0 and 37 tokens, two rows more than there are
+    new, rows = [20, 0, 37], [4, 0, 2]
+    meta = metadata(3, 59)
+    qkv = torch.from_numpy(rng.standard_normal((59, (hq + 2 * hkv) * D))).to(torch.bfloat16).cuda()
+    q, k = (torch.empty(59, h, D, dtype=torch.bfloat16, device="cuda") for h in (hq, hkv))
+    v = enqueue(torch.tensor(new, dtype=torch.int32, device="cuda"), torch.tensor(rows, dtype=torch.int32, device="cuda"), meta, qkv, q, k)
+    want = book.step(new, rows, width, 59, pool)
+    assert [m.tolist() for m in meta] == list(want)
+    both, v64 = here(qkv, want[4])
+    # (within a step of the type, as other arithmetic may round the other way; what is stored is what the kernel made)
+    assert (np.abs(torch.cat([q, k], 1).double().cpu().numpy() - both) <= np.abs(both) * 2.0 ** -7 + 2.0 ** -16).all()
+    c.store([(k, k.double().cpu().numpy()), (v, v64)], want[2], want[1], want[0])
+    dense = [torch.empty(57, hkv, D, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    nvk().gather_kvcache_blocks8(*c.data, *c.scale, meta[3], meta[0], hkv, D, bs, *dense)
+    out = torch.zeros(57, hq, D, dtype=torch.bfloat16, device="cuda")
+    nvk().launch_prefill_attention_dense(q[:57].contiguous(), meta[2], *dense, meta[3], hkv, D, scale, out)
+    for s, (a, b) in enumerate(((0, 20), (20, 57))):
+        kk, vv = (r.rows(want[0][2 * s], b - a) for r in c.ref)
+        q64 = q.double().cpu().numpy()
+        for i in range(a, b, 7):
+            w, w_abs = ref.attend(q64[i], kk[:i - a + 1], vv[:i - a + 1], scale)
+            assert np.abs(out[i].double().cpu().numpy() - w).max() <= 2.0 ** -7 * np.max(w_abs) + 2.0 ** -8 * np.abs(w).max()
+
+    # decode steps of the two, and padding, as one graph
+    rows = [2, -1, 4]
+    meta = metadata(3, 3)
+    new_t, rows_t = torch.ones(3, dtype=torch.int32, device="cuda"), torch.tensor(rows, dtype=torch.int32, device="cuda")
+    qkv = torch.zeros(3, (hq + 2 * hkv) * D, dtype=torch.bfloat16, device="cuda")
+    q, k = (torch.empty(3, h, D, dtype=torch.bfloat16, device="cuda") for h in (hq, hkv))
+    out = torch.empty_like(q)
+    ws = torch.empty(max(16, nvk().decode_attention_workspace_bytes(3, hq, hkv, D, width, bs)), dtype=torch.uint8, device="cuda")
+
+    def step():
+        v = enqueue(new_t, rows_t, meta, qkv, q, k)
+        nvk().store_kvcache_blocks8(k, v, *c.data, *c.scale, None, meta[1], meta[0])
+        nvk().launch_decode_attention_paged_blocks8(q, *c.data, *c.scale, meta[1], meta[0], hkv, D, bs, scale, out, ws)
+
+    def follow():
+        want = book.step([1, 1, 1], rows, width, 3, pool)
+        assert [m.tolist() for m in meta] == list(want) and count.item() == book.count
+        for w, x in ((0, k), (1, qkv[:, (hq + hkv) * D:].reshape(3, hkv, D))):
+            c.ref[w].store(x.double().cpu().numpy(), [0, 1, 2, 3], want[1], want[0])
+        q64 = q.double().cpu().numpy()
+        for s, n in enumerate(want[1]):
+            o = out[s].double().cpu().numpy()
+            if n == 0:
+                assert (o == 0).all()
+                continue
+            w, most = _bound(c, want[0][s], n, q64[s], scale, dtype)
+            assert (np.abs(o - w) <= most).all()
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    follow()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for i in range(20):
+        qkv.copy_(torch.from_numpy(rng.standard_normal(qkv.shape) * 2.0 ** (i / 6)))
+        graph.replay()
+        torch.cuda.synchronize()
+        follow()
+
+    nvk().release_blocks(torch.tensor([2], dtype=torch.int32, device="cuda"), None, lens, held, free, count, bs)
+    book.release([2], None)
+    assert free.tolist()[:book.count] == book.free[:book.count] and lens.tolist() == book.lens and count.item() == book.count
