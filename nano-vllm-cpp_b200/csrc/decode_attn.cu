@@ -385,7 +385,7 @@ Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max
 
 // Kernel parameters of a decode call from host-known sizes only, for kernels with `groups` resident groups per SM; returns in
 // *cluster the cluster size, 0 = chunks.
-int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster, bool four_bits) {
+int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster, bool four_bits, int64_t ahead) {
     DecodeParams p{};
     p.q = a.q; p.k_cache = a.k_cache; p.v_cache = a.v_cache;
     p.context_lens = a.context_lens; p.block_tables = a.block_tables; p.out = a.out;
@@ -394,7 +394,7 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     p.block_size = a.block_size;
     p.scale_log2 = a.scale * kLog2e;
     p.beside = a.beside ? 1 : 0;
-    const int64_t ahead = four_bits ? Cache4<__half>::kKeysAhead : kTileTokens * kMaxCluster;   // how far numbers of keys go beyond the last one
+    if (ahead == 0) ahead = four_bits ? Cache4<__half>::kKeysAhead : kTileTokens * kMaxCluster;   // how far numbers of keys go beyond the last one
     if (a.batch * a.num_heads * kMaxCluster >= (1LL << 31) || a.max_blocks * a.block_size >= (1LL << 31) - ahead)
         return fail(NVK_ERR_UNSUPPORTED, "decode attention: batch or block table too large");
     const Splits s = choose_splits(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size, groups, a.workspace != nullptr, four_bits);
@@ -468,7 +468,9 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     }
     DecodeParams p{};
     int cluster = 0;
-    const int rc = decode_plan(a, F::kGroups, &p, &cluster, F::kFourBits);
+    int64_t ahead = 0;
+    if constexpr (F::kOwnRun) ahead = F::kKeysAhead;
+    const int rc = decode_plan(a, F::kGroups, &p, &cluster, F::kFourBits, ahead);
     if (rc != NVK_OK) return rc;
     p.k_scale = k_scale; p.v_scale = v_scale;
     if constexpr (F::kScores) {
@@ -592,7 +594,9 @@ int launch_decode_int4(const DecodeArgs& a, const void* k_params, const void* v_
 }
 
 bool decode_blocks8_supported(const DecodeArgs& a, const float* k_scale, const float* v_scale) {
-    return shape_supported(a) && aligned_to(a.q, 16) && aligned_to(k_scale, 4) && aligned_to(v_scale, 4);
+    // (rows of heads are counted in 32 bits: 275 GB of K)
+    return shape_supported(a) && a.num_cache_blocks <= ((1LL << 31) - 1) / a.block_size / a.num_kv_heads && aligned_to(a.q, 16) && aligned_to(k_scale, 4) &&
+           aligned_to(v_scale, 4);
 }
 
 int launch_decode_blocks8(const DecodeArgs& a, const float* k_scale, const float* v_scale, bool fp8) {

@@ -171,7 +171,7 @@ template <typename T, bool SCORES = false>
 struct Cache16 {
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = false;
-    static constexpr bool kBlockScales = false;
+    static constexpr bool kOwnRun = false;              // goes through its keys itself (stream_tiles otherwise)
     static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 2;   // resident per SM
     static constexpr int kSplitBlocks = kGroups;
@@ -292,7 +292,7 @@ template <typename T, bool FP8>
 struct Cache8 {
     static constexpr bool kScores = false;
     static constexpr bool kFourBits = false;
-    static constexpr bool kBlockScales = false;
+    static constexpr bool kOwnRun = false;
     static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 3, kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim;
@@ -458,7 +458,7 @@ struct Cache4 {
     using Eight = Cache4<T, SCORES, 8>;                       // eight warps to a block
     static constexpr bool kScores = SCORES;
     static constexpr bool kFourBits = true;
-    static constexpr bool kBlockScales = false;
+    static constexpr bool kOwnRun = true;
     static constexpr int kWarps = WARPS;
     static constexpr int kGroups = 3;                         // resident per SM in clusters; a step is shared out by it in chunks too, as with the 8-bit caches
     static constexpr int kSplitBlocks = 16 / WARPS;           // in chunks: the registers are there, and the chains are what a warp waits for
@@ -747,10 +747,12 @@ struct Cache4 {
     }
 };
 
-// 8-bit cache with one fp32 scale, a power of two, for each (cache block, KV head): kv_blocks8.cu.  Tiles, pieces and the order of the contractions are those of
-// Cache8; a tile of 16 keys lies in one cache block, so that its K and its V have one scale each, two words beside the tile.
-//   * int8: the byte glued under the exponent byte of 1024 as there, and 1152 taken off right away, exactly (one HADD2 for two elements).  Taken off the sums
-//     afterwards, as Cache8 does, it costs the accumulators up to ten bits.
+// 8-bit cache with one fp32 scale, a power of two, for each (cache block, KV head): kv_blocks8.cu.  A warp takes 32 keys at a time, two chains of 16 as in Cache4, whose way of
+// finding the cache rows this is too; 16 keys lie in one cache block, so that their K and their V have one scale each.  Pieces, swizzles and the order of the contractions
+// are those of Cache8, but for the elements of a word of K: a register has elements {0, 2} or {1, 3}.
+//   * int8, K: the byte with its sign flipped in the low bits of an f16 is the subnormal number (n + 128) 2^-24; 128 sum(q) is taken off the sums afterwards.  (1152 sum(q), as
+//     with Cache8's bytes under the exponent of 1024, would cost them three bits more.)
+//   * int8, V: the byte glued under the exponent byte of 1024, and 1152 taken off right away, exactly (one HADD2 for two elements): sums over thousands of keys have no bits to spare.
 //   * Queries are brought to f16 by a power of two, each head's own (exact but for elements below 2^-24 of the head's largest), as in Cache4.
 //   * sum_k p_k s_k n_k: p' = p s 2^-E goes to the MMA in f16, exact but for its rounding; E is each head's own, chosen as in Cache4 by the largest product p s so
 //     far, and chosen again, with the sums rescaled, where a score passes the last maximum by 8 or a scale reaches 2^(7 + E).  So p' is rounded by 2^-11 of itself or 2^-22 of the
@@ -759,21 +761,24 @@ template <typename T, bool FP8>
 struct CacheBlocks8 {
     static constexpr bool kScores = false;
     static constexpr bool kFourBits = false;
-    static constexpr bool kBlockScales = true;
+    static constexpr bool kOwnRun = true;
     static constexpr int kWarps = kGroupWarps;
     static constexpr int kGroups = 3, kSplitBlocks = kGroups;
     static constexpr int kRowBytes = kHeadDim;
-    static constexpr int kTileBytes = kTileTokens * kRowBytes;
-    static constexpr int kStageBytes = 2 * kTileBytes + 16;   // K, V, the scales of both
-    static constexpr int kStages = 4;
+    static constexpr int kKeys = 32;                          // of a stage
+    static constexpr int kKeysAhead = 32 * kWarps * kKeys + 16;   // two windows of 16 tiles and a half: how far `run` counts beyond the last key
+    static constexpr int kTileBytes = kKeys * kRowBytes;
+    static constexpr int kStageBytes = 2 * kTileBytes + 128;  // K, V, the scales (K, K, V, V) of both halves; (whole 128-byte lines: pieces are found by XOR)
+    static constexpr int kStages = 2;
     static constexpr int kPartStride = kHeadDim + 4;
     static constexpr float kSlack = 8.0f;                     // by so much a score may pass s.m: p <= 2^8
+    static constexpr uint32_t kNone = 0xffffffffu;
 
     SoftmaxState s;
-    float score_scale[2];
+    float score_scale[2], q_off[2];
     float down[2];       // 2^-E of heads 2t, 2t + 1
     float top_part[2];   // the largest log2(p s) so far, p without the maximum taken off
-    uint32_t qa[8][2];   // as in Cache8
+    uint32_t qa[8][2];   // k-step 4 q + w: elements 64 q + 16 t + 4 w + {0, 1 | 2, 3}, int8: {0, 2 | 1, 3}
 
     __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
         const int g = lane >> 2, t = lane & 3;
@@ -794,61 +799,74 @@ struct CacheBlocks8 {
         // the head's largest to [2^14, 2^15); (infinities and NaN stay what they are)
         const int up = top > 0.0f && top < INFINITY ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 100) : 0;
         const float by = power_of_two(up);
+        float sum = 0.0f;   // of the f16-rounded query
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
             const float2 a = unpack2<T>(v[ks].x), c = unpack2<T>(v[ks].y);
-            qa[ks][0] = ElemTraits<__half>::pack2(a.x * by, a.y * by);
-            qa[ks][1] = ElemTraits<__half>::pack2(c.x * by, c.y * by);
+            qa[ks][0] = ElemTraits<__half>::pack2(a.x * by, (FP8 ? a.y : c.x) * by);
+            qa[ks][1] = ElemTraits<__half>::pack2((FP8 ? c.x : a.y) * by, c.y * by);
+            const float2 x = unpack2<__half>(qa[ks][0]), y = unpack2<__half>(qa[ks][1]);
+            sum += (x.x + x.y) + (y.x + y.y);
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) score_scale[h] = p.scale_log2 * power_of_two(-__shfl_sync(0xffffffffu, up, 8 * t + 4 * h));
+        for (int x = 1; x < 4; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            score_scale[h] = p.scale_log2 * power_of_two(-__shfl_sync(0xffffffffu, up, 8 * t + 4 * h));
+            q_off[h] = FP8 ? 0.0f : 128.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * h);
+        }
         down[0] = down[1] = 0x1p126f;
         top_part[0] = top_part[1] = -INFINITY;
         s.reset();
     }
-    static __device__ __forceinline__ void issue(const DecodeParams& p, int kvh, int64_t row0, int valid, uint32_t stage, int lane) {
-        const size_t stride = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
-        const int c = lane & 7, rq = lane >> 3;   // 16-byte piece c of rows 4 i + rq; swizzles as in Cache8
-        const size_t base = static_cast<size_t>(row0) * stride + static_cast<size_t>(kvh) * kRowBytes + c * 16;
-        const unsigned char* kc = static_cast<const unsigned char*>(p.k_cache) + base;
-        const unsigned char* vc = static_cast<const unsigned char*>(p.v_cache) + base;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 4 * i + rq;
-            const int bytes = r < valid ? 16 : 0;
-            const size_t src = bytes ? r * stride : 0;
-            nvk::cp_async16(stage + r * kRowBytes + ((c ^ ((r & 1) << 2)) << 4), kc + src, bytes);
-            nvk::cp_async16(stage + kTileBytes + r * kRowBytes + ((c ^ (r & 6)) << 4), vc + src, bytes);
-        }
-    }
-    static __device__ __forceinline__ void issue_scales(const DecodeParams& p, int kvh, int block, uint32_t stage, int lane) {   // (block < 0: zeros)
-        if (lane < 2) {
-            const float* from = static_cast<const float*>(lane == 0 ? p.k_scale : p.v_scale);
-            dec::cp_async4(stage + 2 * kTileBytes + lane * 4, from + static_cast<int64_t>(max(block, 0)) * p.num_kv_heads + kvh, block < 0 ? 0 : 4);
-        }
-    }
-    static __device__ __forceinline__ uint32_t whole(uint32_t glued) {   // two f16, int8: less 1152
+    // Four elements of K as two registers of an MMA operand.
+    static __device__ __forceinline__ uint32_t k_lo(uint32_t x) { return FP8 ? widen_pair_lo<FP8>(x) : (x ^ 0x00800080u) & 0x00ff00ffu; }
+    static __device__ __forceinline__ uint32_t k_hi(uint32_t x) { return FP8 ? widen_pair_hi<FP8>(x) : ((x >> 8) ^ 0x00800080u) & 0x00ff00ffu; }
+    static __device__ __forceinline__ uint32_t whole(uint32_t glued) {   // two f16 of V, int8: less 1152
         if constexpr (FP8) return glued;
         const uint32_t off = 0xe480e480u;   // -1152
         const __half2 d = __hadd2(*reinterpret_cast<const __half2*>(&glued), *reinterpret_cast<const __half2*>(&off));
         return *reinterpret_cast<const uint32_t*>(&d);
     }
-    static __device__ __forceinline__ uint32_t lo2(uint32_t x) { return whole(widen_pair_lo<FP8>(x)); }
-    static __device__ __forceinline__ uint32_t hi2(uint32_t x) { return whole(widen_pair_hi<FP8>(x)); }
-    static constexpr uint32_t kFlip = FP8 ? 0u : 0x80808080u;
+    static __device__ __forceinline__ uint32_t v_lo(uint32_t x) { return whole(widen_pair_lo<FP8>(x)); }
+    static __device__ __forceinline__ uint32_t v_hi(uint32_t x) { return whole(widen_pair_hi<FP8>(x)); }
 
+    // Scores of 16 keys, rows `row0` on of a stage.
+    __device__ __forceinline__ void score(uint32_t stage, int row0, float k_scale, int lane, float (&sc)[4]) const {
+        const int g = lane >> 2, t = lane & 3;
+        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint32_t at = stage + (row0 + g) * kRowBytes + ((t ^ ((g & 1) << 2)) << 4);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            uint32_t w0[4], w1[4];
+            lds32x4(at ^ (q * 64), w0);
+            lds32x4((at ^ (q * 64)) + 8 * kRowBytes, w1);
+#pragma unroll
+            for (int wi = 0; wi < 4; ++wi) {
+                const int ks = 4 * q + wi;
+                mma_16816<__half>(q ? s1 : s0, k_lo(w0[wi]), k_lo(w1[wi]), k_hi(w0[wi]), k_hi(w1[wi]), qa[ks][0], qa[ks][1]);
+            }
+        }
+        const float by[2] = {score_scale[0] * k_scale, score_scale[1] * k_scale};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[i] = (FP8 ? s0[i] + s1[i] : fmaf(s0[i] + s1[i], 0x1p24f, -q_off[i & 1])) * by[i & 1];
+    }
     __device__ __forceinline__ int exponent(int h) const { return 127 - static_cast<int>(__float_as_uint(down[h]) >> 23); }   // E
-    // (Cache4::raise; the tile's V has one scale.)
-    __device__ __forceinline__ void raise(const float (&sc)[4], float v_scale) {
-        const float by = __log2f(v_scale);
+    // (Cache4::raise; the V of 16 keys has one scale.)
+    __device__ __forceinline__ void raise(const float (&sa)[4], const float (&sb)[4], float va, float vb) {
+        const float a = __log2f(va), b = __log2f(vb);
         float c[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float top = fmaxf(sc[h], sc[2 + h]);
+            const float top_a = fmaxf(sa[h], sa[2 + h]), top_b = fmaxf(sb[h], sb[2 + h]);
+            float top = fmaxf(top_a, top_b), part = fmaxf(top_a + a, top_b + b);
 #pragma unroll
-            for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            for (int x = 4; x < 32; x *= 2) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                part = fmaxf(part, __shfl_xor_sync(0xffffffffu, part, x));
+            }
             const float m_new = fmaxf(s.m[h], top);
-            top_part[h] = fmaxf(top_part[h], top + by);
+            top_part[h] = fmaxf(top_part[h], part);
             const int was = exponent(h), e = static_cast<int>(fminf(fmaxf(ceilf(top_part[h] - m_new) + 2.0f, -126.0f), 126.0f));
             c[h] = s.m[h] == m_new ? 1.0f : fast_exp2(s.m[h] - m_new);
             s.l[h] *= c[h];
@@ -859,48 +877,165 @@ struct CacheBlocks8 {
 #pragma unroll
         for (int mt = 0; mt < 8; ++mt) { s.o[mt][0] *= c[0]; s.o[mt][1] *= c[1]; s.o[mt][2] *= c[0]; s.o[mt][3] *= c[1]; }
     }
-    __device__ __forceinline__ void step(const DecodeParams& p, uint32_t stage, int valid, int /*kvh*/, int lane) {
+    // A key's weight; for F16 results rounded to the 11 bits that the MMA takes of it, so that the sum of the weights is that of the rounded ones and a key that has nearly all of
+    // the attention is not off by its rounding (BF16 results are rounded to an eighth of that).
+    static __device__ __forceinline__ float weight(float x) {
+        const float w = fast_exp2(x);
+        return std::is_same<T, __half>::value ? __uint_as_float((__float_as_uint(w) + 0x1000u) & 0xffffe000u) : w;
+    }
+    // What 16 keys add to the sums.
+    __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], float v_scale, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        float k_scale, v_scale;
-        asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];\n" : "=f"(k_scale), "=f"(v_scale) : "r"(stage + 2 * kTileBytes));
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            uint32_t w0[4], w1[4];
-            lds32x4(stage + g * kRowBytes + (((4 * q + t) ^ ((g & 1) << 2)) << 4), w0);
-            lds32x4(stage + (g + 8) * kRowBytes + (((4 * q + t) ^ ((g & 1) << 2)) << 4), w1);
-#pragma unroll
-            for (int wi = 0; wi < 4; ++wi) {
-                const int ks = 4 * q + wi;
-                const uint32_t x0 = w0[wi] ^ kFlip, x1 = w1[wi] ^ kFlip;
-                mma_16816<__half>(ks & 1 ? s1 : s0, lo2(x0), lo2(x1), hi2(x0), hi2(x1), qa[ks][0], qa[ks][1]);
-            }
-        }
-        const float by[2] = {score_scale[0] * k_scale, score_scale[1] * k_scale};
-        float sc[4] = {(s0[0] + s1[0]) * by[0], (s0[1] + s1[1]) * by[1], (s0[2] + s1[2]) * by[0], (s0[3] + s1[3]) * by[1]};
-        mask_scores(sc, g, valid);
-        const float top0 = fmaxf(sc[0], sc[2]), top1 = fmaxf(sc[1], sc[3]);
-        if (__any_sync(0xffffffffu, fmaxf(top0 - s.m[0], top1 - s.m[1]) > kSlack || v_scale * fmaxf(down[0], down[1]) >= 0x1p7f)) raise(sc, v_scale);
-        const float p0 = fast_exp2(sc[0] - s.m[0]), p1 = fast_exp2(sc[1] - s.m[1]), p2 = fast_exp2(sc[2] - s.m[0]), p3 = fast_exp2(sc[3] - s.m[1]);
+        const float p0 = weight(sc[0] - s.m[0]), p1 = weight(sc[1] - s.m[1]), p2 = weight(sc[2] - s.m[0]), p3 = weight(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
         const float part[2] = {v_scale * down[0], v_scale * down[1]};
         const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * part[0], p1 * part[1]));
         const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * part[0], p3 * part[1]));
-        // output: V rows 2t, 2t+1, 2t+8, 2t+9, piece g (d = 16 g .. 16 g + 15)
+        // V rows 2t, 2t+1, 2t+8, 2t+9, piece g (d = 16 g .. 16 g + 15)
+        const uint32_t at = stage + kTileBytes + (row0 + 2 * t) * kRowBytes + ((g ^ (2 * t)) << 4);
+        constexpr uint32_t kFlip = FP8 ? 0u : 0x80808080u;
         uint32_t v0[4], v1[4], v2[4], v3[4];
-        const uint32_t vbase = stage + kTileBytes;
-        lds32x4(vbase + (2 * t) * kRowBytes + ((g ^ ((2 * t) & 6)) << 4), v0);
-        lds32x4(vbase + (2 * t + 1) * kRowBytes + ((g ^ ((2 * t + 1) & 6)) << 4), v1);
-        lds32x4(vbase + (2 * t + 8) * kRowBytes + ((g ^ ((2 * t + 8) & 6)) << 4), v2);
-        lds32x4(vbase + (2 * t + 9) * kRowBytes + ((g ^ ((2 * t + 9) & 6)) << 4), v3);
+        lds32x4(at, v0);
+        lds32x4(at + kRowBytes, v1);
+        lds32x4(at + 8 * kRowBytes, v2);
+        lds32x4(at + 9 * kRowBytes, v3);
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            const uint32_t x0 = v0[a] ^ kFlip, x1 = v1[a] ^ kFlip, x2 = v2[a] ^ kFlip, x3 = v3[a] ^ kFlip;
-            const uint32_t lo01 = __byte_perm(x0, x1, 0x5140), hi01 = __byte_perm(x0, x1, 0x7362);
-            const uint32_t lo23 = __byte_perm(x2, x3, 0x5140), hi23 = __byte_perm(x2, x3, 0x7362);
-            mma_16816<__half>(s.o[2 * a], lo2(lo01), hi2(lo01), lo2(lo23), hi2(lo23), pb0, pb1);
-            mma_16816<__half>(s.o[2 * a + 1], lo2(hi01), hi2(hi01), lo2(hi23), hi2(hi23), pb0, pb1);
+            const uint32_t lo01 = __byte_perm(v0[a], v1[a], 0x5140) ^ kFlip, hi01 = __byte_perm(v0[a], v1[a], 0x7362) ^ kFlip;
+            const uint32_t lo23 = __byte_perm(v2[a], v3[a], 0x5140) ^ kFlip, hi23 = __byte_perm(v2[a], v3[a], 0x7362) ^ kFlip;
+            mma_16816<__half>(s.o[2 * a], v_lo(lo01), v_hi(lo01), v_lo(lo23), v_hi(lo23), pb0, pb1);
+            mma_16816<__half>(s.o[2 * a + 1], v_lo(hi01), v_hi(hi01), v_lo(hi23), v_hi(hi23), pb0, pb1);
+        }
+    }
+    // 32 keys, of which `valid` (more than none) are there.
+    __device__ __forceinline__ void step(uint32_t stage, int valid, int lane) {
+        float ka, kb, va, vb, sa[4], sb[4];
+        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(ka), "=f"(kb), "=f"(va), "=f"(vb) : "r"(stage + 2 * kTileBytes));
+        score(stage, 0, ka, lane, sa);
+        score(stage, 16, kb, lane, sb);
+        if (valid < kKeys) {
+            mask_scores(sa, lane >> 2, valid);
+            mask_scores(sb, lane >> 2, valid - 16);
+        }
+        const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
+        if (__any_sync(0xffffffffu, fmaxf(top0 - s.m[0], top1 - s.m[1]) > kSlack || fmaxf(va, vb) * fmaxf(down[0], down[1]) >= 0x1p7f)) raise(sa, sb, va, vb);
+        add(stage, 0, sa, va, lane);
+        add(stage, 16, sb, vb, lane);
+    }
+    static __device__ __forceinline__ const void* row_at(uint32_t unit, const unsigned char* base) {
+        uint64_t at;
+        asm("mad.wide.u32 %0, %1, %2, %3;\n" : "=l"(at) : "r"(unit), "n"(kRowBytes), "l"(base));
+        return reinterpret_cast<const void*>(at);
+    }
+    static __device__ __forceinline__ const void* scale_at(uint32_t unit, const float* base) {
+        uint64_t at;
+        asm("mad.wide.u32 %0, %1, 4, %2;\n" : "=l"(at) : "r"(unit), "l"(base));
+        return reinterpret_cast<const void*>(at);
+    }
+
+    // Keys [t0, t1): this warp's tiles of 32, every fourth one.
+    __device__ __forceinline__ void run(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, uint32_t ring, int warp, int lane) {
+        const int tiles = (t1 - t0 + kKeys - 1) / kKeys, mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+        const int bs = p.block_size, first = t0 + warp * kKeys;
+        constexpr int kStride = kWarps * kKeys;
+        // Lane 2i + h: half h of tile i of a window of 16 tiles: its cache block's place among all scales, and the place of its first row among all head vectors of the cache.
+        auto token_of = [&](int window) { return first + (window * 16 + (lane >> 1)) * kStride + (lane & 1) * 16; };
+        auto load = [&](int window) {
+            const int token = token_of(window);
+            const int blk = static_cast<int>(p.by_block.div(token < t1 ? token : 0));
+            return p.block_tables.raw(b * p.max_blocks + blk, token < t1);
+        };
+        uint32_t units, scales;
+        auto take = [&](int window, IndexArray::Raw raw) {
+            const int token = token_of(window), off = token - static_cast<int>(p.by_block.div(token < t1 ? token : 0)) * bs;
+            const int64_t id = p.block_tables.value(raw);
+            const bool there = token < t1 && id >= 0 && id < p.num_cache_blocks;
+            units = there ? (static_cast<uint32_t>(id) * bs + off) * p.num_kv_heads + kvh : kNone;
+            scales = there ? static_cast<uint32_t>(id) * p.num_kv_heads + kvh : 0u;
+        };
+        {   // the first window from the ids that came with the context, if they reach that far
+            const int token = token_of(0), at = static_cast<int>(p.by_block.div(token < t1 ? token : t0)) - id_base;
+            IndexArray::Raw raw{__shfl_sync(0xffffffffu, raw_ids.lo, at), __shfl_sync(0xffffffffu, raw_ids.hi, at)};
+            if (__any_sync(0xffffffffu, at >= 32)) raw = load(0);
+            take(0, raw);
+        }
+        IndexArray::Raw next = load(1);
+        const int r = lane >> 3, c = lane & 7;               // 16-byte piece c of rows 4 i + r
+        const size_t row_bytes = static_cast<size_t>(p.num_kv_heads) * kRowBytes;
+        const unsigned char *k_at[4], *v_at[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            k_at[i] = static_cast<const unsigned char*>(p.k_cache) + (4 * i + r) * row_bytes + c * 16;
+            v_at[i] = static_cast<const unsigned char*>(p.v_cache) + (4 * i + r) * row_bytes + c * 16;
+        }
+        const float* scale_from = static_cast<const float*>((lane & 2) ? p.v_scale : p.k_scale);   // lanes 0 to 3: (K, K, V, V) of halves (0, 1, 0, 1)
+        // Swizzles of row 4 i + r: K piece c ^ ((row & 1) << 2), V piece c ^ (row & 6): for odd i 4 more.
+        const uint32_t k_to = r * kRowBytes + ((c ^ ((r & 1) << 2)) << 4), v_to = kTileBytes + r * kRowBytes + ((c ^ (r & 2)) << 4);
+        int issued = 0, left = t1 - first;                    // keys from the next tile on
+        uint32_t istage = ring;
+        auto issue = [&]() {
+            if (issued < mine) {
+                if ((issued & 15) == 0 && issued > 0) {
+                    take(issued >> 4, next);
+                    next = load((issued >> 4) + 1);
+                }
+                const uint32_t u0 = __shfl_sync(0xffffffffu, units, 2 * issued), u1 = __shfl_sync(0xffffffffu, units, 2 * issued + 1);
+                const uint32_t at = __shfl_sync(0xffffffffu, scales, 2 * issued + (lane & 1));
+                const uint32_t k_dst = istage + k_to, v_dst = istage + v_to, v_odd = v_dst ^ 64, s_dst = istage + 2 * kTileBytes + lane * 4;
+                constexpr int kHalf = 16 * kRowBytes, kRows4 = 4 * kRowBytes;
+                if (left >= kKeys && max(u0, u1) != kNone) {
+                    cp_async16<0>(k_dst, row_at(u0, k_at[0]));
+                    cp_async16<kRows4>(k_dst, row_at(u0, k_at[1]));
+                    cp_async16<2 * kRows4>(k_dst, row_at(u0, k_at[2]));
+                    cp_async16<3 * kRows4>(k_dst, row_at(u0, k_at[3]));
+                    cp_async16<kHalf>(k_dst, row_at(u1, k_at[0]));
+                    cp_async16<kHalf + kRows4>(k_dst, row_at(u1, k_at[1]));
+                    cp_async16<kHalf + 2 * kRows4>(k_dst, row_at(u1, k_at[2]));
+                    cp_async16<kHalf + 3 * kRows4>(k_dst, row_at(u1, k_at[3]));
+                    cp_async16<0>(v_dst, row_at(u0, v_at[0]));
+                    cp_async16<kRows4>(v_odd, row_at(u0, v_at[1]));
+                    cp_async16<2 * kRows4>(v_dst, row_at(u0, v_at[2]));
+                    cp_async16<3 * kRows4>(v_odd, row_at(u0, v_at[3]));
+                    cp_async16<kHalf>(v_dst, row_at(u1, v_at[0]));
+                    cp_async16<kHalf + kRows4>(v_odd, row_at(u1, v_at[1]));
+                    cp_async16<kHalf + 2 * kRows4>(v_dst, row_at(u1, v_at[2]));
+                    cp_async16<kHalf + 3 * kRows4>(v_odd, row_at(u1, v_at[3]));
+                    if (lane < 4) cp_async4<0>(s_dst, scale_at(at, scale_from));
+                } else {   // what is not there reads as zeros (stale cache contents, even NaN, never reach the arithmetic)
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t unit = h == 0 ? u0 : u1;
+                        const int valid = unit == kNone ? 0 : left - 16 * h;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const bool there = 4 * i + r < valid;
+                            nvk::cp_async16(k_dst + h * kHalf + i * kRows4, there ? row_at(unit, k_at[i]) : p.k_cache, there ? 16 : 0);
+                            nvk::cp_async16((i & 1 ? v_odd : v_dst) + h * kHalf + i * kRows4, there ? row_at(unit, v_at[i]) : p.v_cache, there ? 16 : 0);
+                        }
+                    }
+                    const bool there = (lane & 1) == 0 ? u0 != kNone : u1 != kNone;   // (a half beyond the last key has no unit)
+                    if (lane < 4) dec::cp_async4(s_dst, scale_at(at, scale_from), there ? 4 : 0);
+                }
+                ++issued;
+                left -= kStride;
+                istage = istage == ring + (kStages - 1) * kStageBytes ? ring : istage + kStageBytes;
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) issue();
+        start(p, b, kvh, lane);
+        uint32_t cstage = ring;
+        int here = t1 - first;
+        for (int j = 0; j < mine; ++j) {
+            issue();
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            step(cstage, here, lane);
+            __syncwarp();   // the stage is refilled by other lanes' copies
+            cstage = cstage == ring + (kStages - 1) * kStageBytes ? ring : cstage + kStageBytes;
+            here -= kStride;
         }
     }
     __device__ __forceinline__ void finish() {}
@@ -952,7 +1087,6 @@ __device__ __forceinline__ void stream_tiles(const DecodeParams& p, int b, int k
         if (tok < t1) {
             const int phys = __shfl_sync(0xffffffffu, ids, blk - id_base);
             F::issue(p, kvh, phys < 0 ? 0 : static_cast<int64_t>(phys) * bs + off, phys < 0 ? 0 : t1 - tok, istage, lane);
-            if constexpr (F::kBlockScales) F::issue_scales(p, kvh, phys, istage, lane);
             istage = istage == ring + (F::kStages - 1) * F::kStageBytes ? ring : istage + F::kStageBytes;
             tok += kGroupWarps * kTileTokens;
             for (off += kGroupWarps * kTileTokens; off >= bs; off -= bs) ++blk;
@@ -988,7 +1122,7 @@ __device__ __forceinline__ void attend_range(const DecodeParams& p, int b, int k
     const int warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = smem_u32(sm.warps[warp].ring);
     F st;
-    if constexpr (F::kFourBits) st.run(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane);
+    if constexpr (F::kOwnRun) st.run(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane);
     else stream_tiles(p, b, kvh, t0, t1, raw_ids, id_base, ring, warp, lane, st);
     cp_async_wait<0>();
     __syncwarp();                              // this warp's ring is idle from here on
