@@ -448,17 +448,23 @@ int check_grid(const DecodeArgs& a, const dec::DecodeParams& p) {   // of decode
     return NVK_OK;
 }
 
+// The format as decode_cluster_kernel takes it.
+template <class F, class = void> struct InClusters { using type = F; };
+template <class F> struct InClusters<F, std::void_t<typename F::InClusters>> { using type = typename F::InClusters; };
+
 // `scores`, `ml`, `weights`: where they are kept (F::kScores), the (maximum, sum) of every part, and what becomes of them; *plan: how the step was shared out.
 template <class F, typename T>
 int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, float* scores = nullptr, float2* ml = nullptr, const KeyWeights* weights = nullptr,
                  DecodeParams* plan = nullptr) {
+    using C = typename InClusters<F>::type;
+    static_assert(sizeof(GroupSmem<C>) == sizeof(GroupSmem<F>), "one size of shared memory");
     constexpr int kSmem = static_cast<int>(sizeof(GroupSmem<F>));
     static std::atomic<bool> attr_done[64] = {};  // per device; the attribute calls are idempotent
     int device = 0;
     cudaGetDevice(&device);
     if (device >= 0 && device < 64 && !attr_done[device]) {
         cudaError_t e = cudaFuncSetAttribute(decode_split_kernel<F, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_cluster_kernel<F, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_cluster_kernel<C, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if constexpr (F::kFourBits) {
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(decode_split_kernel<typename F::Eight, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(GroupSmem<typename F::Eight>));
@@ -492,7 +498,7 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
         attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 2;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_cluster_kernel<F, T>, p);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, decode_cluster_kernel<C, T>, p);
         if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "decode_cluster_kernel launch: %s", cudaGetErrorString(e));
         return check_launch("decode_cluster_kernel launch");
     }

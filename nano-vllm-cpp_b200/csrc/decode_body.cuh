@@ -757,8 +757,10 @@ struct Cache4 {
 //   * sum_k p_k s_k n_k: p' = p s 2^-E goes to the MMA in f16, exact but for its rounding; E is each head's own, chosen as in Cache4 by the largest product p s so
 //     far, and chosen again, with the sums rescaled, where a score passes the last maximum by 8 or a scale reaches 2^(7 + E).  So p' is rounded by 2^-11 of itself or 2^-22 of the
 //     head's largest, and one block whose scale is far above the others' does not cost them their bits.
-template <typename T, bool FP8>
+// CLUSTERS: for blocks that share a context in a cluster, and may have a few keys each (launches in chunks were 0.5 to 1.5 % slower with that code).
+template <typename T, bool FP8, bool CLUSTERS = false>
 struct CacheBlocks8 {
+    using InClusters = CacheBlocks8<T, FP8, true>;
     static constexpr bool kScores = false;
     static constexpr bool kFourBits = false;
     static constexpr bool kOwnRun = true;
@@ -852,6 +854,10 @@ struct CacheBlocks8 {
         for (int i = 0; i < 4; ++i) sc[i] = (FP8 ? s0[i] + s1[i] : fmaf(s0[i] + s1[i], 0x1p24f, -q_off[i & 1])) * by[i & 1];
     }
     __device__ __forceinline__ int exponent(int h) const { return 127 - static_cast<int>(__float_as_uint(down[h]) >> 23); }   // E
+    __device__ __forceinline__ bool raises(const float (&sa)[4], const float (&sb)[4], float va, float vb) const {
+        const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
+        return fmaxf(top0 - s.m[0], top1 - s.m[1]) > kSlack || fmaxf(va, vb) * fmaxf(down[0], down[1]) >= 0x1p7f;
+    }
     // (Cache4::raise; the V of 16 keys has one scale.)
     __device__ __forceinline__ void raise(const float (&sa)[4], const float (&sb)[4], float va, float vb) {
         const float a = __log2f(va), b = __log2f(vb);
@@ -912,14 +918,21 @@ struct CacheBlocks8 {
     __device__ __forceinline__ void step(uint32_t stage, int valid, int lane) {
         float ka, kb, va, vb, sa[4], sb[4];
         asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(ka), "=f"(kb), "=f"(va), "=f"(vb) : "r"(stage + 2 * kTileBytes));
+        if (CLUSTERS && valid <= 16) {   // (a range's last keys, or all that a warp has of a short one)
+            score(stage, 0, ka, lane, sa);
+            mask_scores(sa, lane >> 2, valid);
+            sb[0] = sb[1] = sb[2] = sb[3] = -INFINITY;
+            if (__any_sync(0xffffffffu, raises(sa, sb, va, 0.0f))) raise(sa, sb, va, 0.0f);
+            add(stage, 0, sa, va, lane);
+            return;
+        }
         score(stage, 0, ka, lane, sa);
         score(stage, 16, kb, lane, sb);
         if (valid < kKeys) {
             mask_scores(sa, lane >> 2, valid);
             mask_scores(sb, lane >> 2, valid - 16);
         }
-        const float top0 = fmaxf(fmaxf(sa[0], sa[2]), fmaxf(sb[0], sb[2])), top1 = fmaxf(fmaxf(sa[1], sa[3]), fmaxf(sb[1], sb[3]));
-        if (__any_sync(0xffffffffu, fmaxf(top0 - s.m[0], top1 - s.m[1]) > kSlack || fmaxf(va, vb) * fmaxf(down[0], down[1]) >= 0x1p7f)) raise(sa, sb, va, vb);
+        if (__any_sync(0xffffffffu, raises(sa, sb, va, vb))) raise(sa, sb, va, vb);
         add(stage, 0, sa, va, lane);
         add(stage, 16, sb, vb, lane);
     }
@@ -936,8 +949,10 @@ struct CacheBlocks8 {
 
     // Keys [t0, t1): this warp's tiles of 32, every fourth one.
     __device__ __forceinline__ void run(const DecodeParams& p, int b, int kvh, int t0, int t1, IndexArray::Raw raw_ids, int id_base, uint32_t ring, int warp, int lane) {
-        const int tiles = (t1 - t0 + kKeys - 1) / kKeys, mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
-        const int bs = p.block_size, first = t0 + warp * kKeys;
+        // Of a range that four warps have in 16 keys each, each takes so many (1 sequence of 300 keys in a cluster of eight blocks, 8 KV heads, 3.83 -> 3.58 us a call).
+        const int span = CLUSTERS && t1 - t0 <= kWarps * 16 ? 16 : kKeys, shift = span == 16 ? 4 : 5;
+        const int tiles = (t1 - t0 + span - 1) >> shift, mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;
+        const int bs = p.block_size, first = t0 + (warp << shift);
         constexpr int kStride = kWarps * kKeys;
         // Lane 2i + h: half h of tile i of a window of 16 tiles: its cache block's place among all scales, and the place of its first row among all head vectors of the cache.
         auto token_of = [&](int window) { return first + (window * 16 + (lane >> 1)) * kStride + (lane & 1) * 16; };
@@ -950,7 +965,7 @@ struct CacheBlocks8 {
         auto take = [&](int window, IndexArray::Raw raw) {
             const int token = token_of(window), off = token - static_cast<int>(p.by_block.div(token < t1 ? token : 0)) * bs;
             const int64_t id = p.block_tables.value(raw);
-            const bool there = token < t1 && id >= 0 && id < p.num_cache_blocks;
+            const bool there = token < t1 && (lane & 1) * 16 < span && id >= 0 && id < p.num_cache_blocks;
             units = there ? (static_cast<uint32_t>(id) * bs + off) * p.num_kv_heads + kvh : kNone;
             scales = there ? static_cast<uint32_t>(id) * p.num_kv_heads + kvh : 0u;
         };
@@ -972,7 +987,8 @@ struct CacheBlocks8 {
         const float* scale_from = static_cast<const float*>((lane & 2) ? p.v_scale : p.k_scale);   // lanes 0 to 3: (K, K, V, V) of halves (0, 1, 0, 1)
         // Swizzles of row 4 i + r: K piece c ^ ((row & 1) << 2), V piece c ^ (row & 6): for odd i 4 more.
         const uint32_t k_to = r * kRowBytes + ((c ^ ((r & 1) << 2)) << 4), v_to = kTileBytes + r * kRowBytes + ((c ^ (r & 2)) << 4);
-        int issued = 0, left = t1 - first;                    // keys from the next tile on
+        const int left_all = span == 16 ? min(t1 - first, 16) : t1 - first;   // (a warp's only tile)
+        int issued = 0, left = left_all;                      // keys from the next tile on
         uint32_t istage = ring;
         auto issue = [&]() {
             if (issued < mine) {
@@ -1027,7 +1043,7 @@ struct CacheBlocks8 {
         for (int i = 0; i < kStages - 1; ++i) issue();
         start(p, b, kvh, lane);
         uint32_t cstage = ring;
-        int here = t1 - first;
+        int here = left_all;
         for (int j = 0; j < mine; ++j) {
             issue();
             cp_async_wait<kStages - 1>();
