@@ -3,263 +3,453 @@
 // the host for every step (src/engine/model_runner.cpp:482-632, :748-769) and its BlockManager hands out.
 //
 // With old length l_b, n_b new tokens and blocks of s tokens, request b needs ceil((l_b + n_b) / s) - ceil(l_b / s) new blocks; the prefix sums of these
-// say which of the free blocks are its own, and whether there are enough.  Two sums over the batch, then every table entry and every token by itself.
+// say which of the free blocks are its own, and whether there are enough.  Sums over the batch, then every table entry and every token by itself.
 //
-// A call is bound by the trips to memory one after the other (row, its length, its blocks) and by the launch: all blocks of one cluster do the sums over the
+// A call is bound by the trips to memory one after the other (row, its length and its blocks) and by the launch: all blocks of one cluster do the sums over the
 // whole batch for themselves, so that nothing is handed over, and share out the table entries and the tokens.  A cluster because lengths and the count of free
-// blocks may be updated in place: each block has read them when the cluster's barrier is passed.
+// blocks may be updated in place: they are when every block has read them.
 #include "nvk_internal.cuh"
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace nvk {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kFewThreads = 256, kManyThreads = 1024;
 constexpr int kMaxBlocks = 16;            // of a cluster (not portable, but there on every B200)
-constexpr int kMaxBatch = 8192;           // 16 bytes of shared memory for each
+constexpr int kMaxBatch = 8192;           // 24 bytes of shared memory for each
+constexpr int kAhead = 2;                 // pieces of table rows that a thread has under way
+constexpr int64_t kWideWork = 2 * kMaxBlocks * kManyThreads;   // pieces of 16 bytes up to which one cluster takes a step
 constexpr uint32_t kMost = 0x7fffffffu;
 
 // Sums of numbers below 2^31, held at 2^31 - 1: lengths come from the device, and no sum of them may wrap round.
 __device__ __forceinline__ uint32_t add_held(uint32_t a, uint32_t b) { return min(a + b, kMost); }
-
-__device__ __forceinline__ void put(void* p, int wide, int64_t i, int64_t v) {
-    if (wide) static_cast<int64_t*>(p)[i] = v;
-    else static_cast<int32_t*>(p)[i] = static_cast<int32_t>(v);
+template <typename E> __device__ __forceinline__ uint32_t held(E v, uint32_t most = kMost) {   // within 0 .. most
+    return v < 0 ? 0u : v > static_cast<E>(most) ? most : static_cast<uint32_t>(v);
 }
 
-// Sums over the threads before this one and, in `total`, over all.  Two numbers at a time.
-struct Two { uint32_t a, b; };
-__device__ __forceinline__ Two scan_block(Two v, Two& total, Two* s_warp) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    Two x = v;
+// Sums of three numbers over the threads before this one and, in `total`, over all.
+struct Three { uint32_t a, b, c; };
+__device__ __forceinline__ Three add_held(Three x, Three y) { return Three{add_held(x.a, y.a), add_held(x.b, y.b), add_held(x.c, y.c)}; }
+__device__ __forceinline__ Three shfl(Three x, int lane) {
+    return Three{__shfl_sync(0xffffffffu, x.a, lane), __shfl_sync(0xffffffffu, x.b, lane), __shfl_sync(0xffffffffu, x.c, lane)};
+}
+__device__ __forceinline__ Three scan_warp(Three x, int lane) {   // with its own
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, x.a, d), b = __shfl_up_sync(0xffffffffu, x.b, d);
-        if (lane >= d) { x.a = add_held(x.a, a); x.b = add_held(x.b, b); }
+        const Three y{__shfl_up_sync(0xffffffffu, x.a, d), __shfl_up_sync(0xffffffffu, x.b, d), __shfl_up_sync(0xffffffffu, x.c, d)};
+        if (lane >= d) x = add_held(x, y);
     }
+    return x;
+}
+__device__ __forceinline__ Three before_in_warp(Three x, int lane) {
+    const Three y = shfl(x, max(lane - 1, 0));
+    return lane > 0 ? y : Three{0u, 0u, 0u};
+}
+template <int WARPS> __device__ __forceinline__ Three scan_block(Three v, Three& total, Three* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Three x = scan_warp(v, lane);
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    Two w = lane < kWarps ? s_warp[lane] : Two{0u, 0u};
-#pragma unroll
-    for (int d = 1; d < kWarps; d *= 2) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, w.a, d), b = __shfl_up_sync(0xffffffffu, w.b, d);
-        if (lane >= d) { w.a = add_held(w.a, a); w.b = add_held(w.b, b); }
-    }
-    total = Two{__shfl_sync(0xffffffffu, w.a, kWarps - 1), __shfl_sync(0xffffffffu, w.b, kWarps - 1)};
-    const uint32_t a = __shfl_sync(0xffffffffu, w.a, max(warp - 1, 0)), b = __shfl_sync(0xffffffffu, w.b, max(warp - 1, 0));
-    Two before{__shfl_up_sync(0xffffffffu, x.a, 1), __shfl_up_sync(0xffffffffu, x.b, 1)};
-    if (lane == 0) before = Two{0u, 0u};
-    if (warp > 0) before = Two{add_held(before.a, a), add_held(before.b, b)};
+    const Three w = scan_warp(lane < WARPS ? s_warp[lane] : Three{0u, 0u, 0u}, lane);
+    total = shfl(w, 31);
+    const Three others = shfl(w, max(warp - 1, 0)), before = before_in_warp(x, lane);
     __syncthreads();                      // (s_warp is used again)
-    return before;
+    return warp > 0 ? add_held(before, others) : before;
 }
 
-// Every block of the cluster has come here, and has read what comes before it in its program.
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
+// All blocks of the cluster arrive when they have read what is updated in place, and gone on from its values; the first one, which writes it, waits at its end.  Nothing that
+// one block writes is read by another, so that the barrier need not wait for anybody's writes (it did for 1 us of the 5 that 256 requests took).
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
 
-// What is known of a request of the step, in shared memory.
+// What is known of the requests of a step, in shared memory.
 struct Request {
     int row;      // of the table of requests; -1: padding
-    int old_len;  // -1: there is no place for it
-    int cu;       // first token
+    int had;      // blocks in use before
+    int used;     // and after; 0: there is no place for it
     int first;    // the first of its new blocks among those of the step
 };
+struct Tokens {
+    int cu;       // the first one
+    int old_len;  // -1: there is no place for it
+};
 
-struct StepParams {
-    IndexArray new_lens, rows, lens, free_blocks, free_count;
-    void *request_blocks, *block_tables, *context_lens, *cu_q, *cu_k, *positions, *slots, *new_lens_out, *new_count;
+template <typename E> struct StepParams {
+    const E *new_lens, *rows, *lens, *free_blocks, *free_count;
+    E *request_blocks, *block_tables, *context_lens, *cu_q, *cu_k, *positions, *slots, *new_lens_out, *new_count;
     int64_t num_rows, row_blocks, num_free, num_cache_blocks, num_tokens;
-    int batch, max_blocks, wide;
+    int batch, max_blocks;
+    int token_pieces;                     // positions and slots are written 16 bytes at a time
+    int wide;                             // many blocks instead of one cluster; what is updated in place is left to commit_step_kernel
     uint32_t capacity;                    // tokens of a request, at most
-    FastDiv by_block, by_width;
+    FastDiv by_block, by_pieces;          // by_pieces: of a table row
 };
 
 __device__ __forceinline__ uint32_t blocks_of(const FastDiv& by_block, uint32_t tokens) { return by_block.div(tokens + by_block.d - 1); }
 
-__global__ void __launch_bounds__(kThreads) step_metadata_kernel(const __grid_constant__ StepParams p) {
-    extern __shared__ Request s_request[];
-    __shared__ Two s_warp[kWarps];
+// V numbers next to each other.
+template <typename E, int V> struct alignas(V * sizeof(E)) Entries { E e[V]; };
+
+template <typename E, int V, int THREADS>
+__global__ void __launch_bounds__(THREADS) step_metadata_kernel(const __grid_constant__ StepParams<E> p) {
+    constexpr int kWarps = THREADS / 32, kTokens = 4;
+    extern __shared__ __align__(16) Request s_request[];
+    Tokens* s_token = reinterpret_cast<Tokens*>(s_request + p.batch);
+    __shared__ Three s_warp[kWarps];
+    __shared__ uint32_t s_tokens, s_taken;
+    __shared__ E s_free[THREADS];         // the blocks that are taken first
+    using Piece = Entries<E, V>;
     pdl_wait_then_release();
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31;
     const bool first_block = blockIdx.x == 0;
-    const int64_t count_in = p.free_count[0];
-    const uint32_t count = static_cast<uint32_t>(min(max(count_in, static_cast<int64_t>(0)), p.num_free));
-    Two base{0u, 0u};                     // tokens, new blocks
-    uint32_t keys = 0, taken = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
+    const int threads = static_cast<int>(gridDim.x) * THREADS, me = static_cast<int>(blockIdx.x) * THREADS + tid;
+    const int pieces = p.batch * static_cast<int>(p.by_pieces.d);
+    // What needs no other number first, then what needs those: two trips to memory before the sums.
+    auto known = [&](E row) { return row >= 0 && row < p.num_rows; };
+    auto row_of = [&](int b) { return p.rows != nullptr ? p.rows[b] : static_cast<E>(b); };
+    const E count_in = p.free_count[0];
+    E row0 = -1, new0 = 0, len0 = 0, free0 = 0, piece_row[kAhead];
+    if (tid < p.batch) {
+        row0 = row_of(tid);
+        new0 = p.new_lens[tid];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) piece_row[u] = me + u * threads < pieces ? row_of(static_cast<int>(p.by_pieces.div(me + u * threads))) : static_cast<E>(-1);
+    if (known(row0)) len0 = p.lens[row0];
+    // The first pieces of the table rows: which of their entries count is seen later.
+    auto load = [&](int i, E row, Piece& to) {
+        const int64_t j = static_cast<int64_t>(i - static_cast<int>(p.by_pieces.div(i)) * static_cast<int>(p.by_pieces.d)) * V;
+        if (j < p.row_blocks) to = *reinterpret_cast<const Piece*>(p.request_blocks + static_cast<int64_t>(row) * p.row_blocks + j);
+    };
+    Piece piece[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+        if (known(piece_row[u])) load(me + u * threads, piece_row[u], piece[u]);
+    const uint32_t count = held(count_in, static_cast<uint32_t>(min(p.num_free, static_cast<int64_t>(kMost))));
+    if (static_cast<uint32_t>(tid) < count) free0 = p.free_blocks[static_cast<int64_t>(count) - 1 - tid];
+    // Where there is a thread for every token: token t is most often request t's only one, in a decode step.  The block that it would then be in, while the sums are taken.
+    const bool single = p.num_tokens <= threads;
+    E guess = -1;
+    if (single && me < p.batch && me < p.num_tokens) {
+        const E row = first_block ? row0 : row_of(me);
+        if (known(row)) {
+            const uint32_t j = p.by_block.div(held(first_block ? len0 : p.lens[row]));
+            if (j < p.row_blocks) guess = p.request_blocks[static_cast<int64_t>(row) * p.row_blocks + j];
+        }
+    }
+    if (tid == 0) s_taken = 0;
+    // The requests, THREADS at a time (up to 32 by one warp, without barriers).
+    Three base{0u, 0u, 0u};               // tokens, new blocks, keys
+    uint32_t taken = 0;
+    auto requests = [&](int b0, auto scan) {
         const int b = b0 + tid;
         const bool there = b < p.batch;
-        int64_t row = -1, n64 = 0;
-        if (there) {
-            row = p.rows != nullptr ? p.rows[b] : b;
-            n64 = p.new_lens[b];
+        E row = row0, n_in = new0, len_in = len0;
+        if (b0 > 0) {
+            row = there ? row_of(b) : static_cast<E>(-1);
+            n_in = there ? p.new_lens[b] : static_cast<E>(0);
+            len_in = known(row) ? p.lens[row] : static_cast<E>(0);
         }
-        const bool known = there && row >= 0 && row < p.num_rows;
-        const int64_t len64 = known ? p.lens[row] : 0;
-        const uint32_t n = static_cast<uint32_t>(min(max(n64, static_cast<int64_t>(0)), static_cast<int64_t>(kMost)));
-        const uint32_t len = static_cast<uint32_t>(min(max(len64, static_cast<int64_t>(0)), static_cast<int64_t>(kMost)));
-        const bool fits = known && len <= p.capacity && n <= p.capacity - len;
-        const uint32_t need = fits ? blocks_of(p.by_block, len + n) - blocks_of(p.by_block, len) : 0;
-        Two total;
-        Two at = scan_block(Two{n, need}, total, s_warp);
-        at = Two{add_held(at.a, base.a), add_held(at.b, base.b)};
+        const bool ours = known(row);
+        const uint32_t len = held(len_in), n = held(n_in);
+        const bool fits = ours && len <= p.capacity && n <= p.capacity - len;
+        const uint32_t had = fits ? blocks_of(p.by_block, len) : 0u, used = fits ? blocks_of(p.by_block, len + n) : 0u, need = used - had;
+        Three total;
+        Three at = add_held(scan(Three{n, need, fits ? len + n : 0u}, total), base);
         const bool placed = fits && (need == 0 || add_held(at.b, need) <= count);
-        if (placed && need > 0) taken = max(taken, add_held(at.b, need));
-        base = Two{add_held(base.a, total.a), add_held(base.b, total.b)};
-        if (there) s_request[b] = Request{known ? static_cast<int>(row) : -1, placed ? static_cast<int>(len) : -1, static_cast<int>(at.a), static_cast<int>(at.b)};
         const uint32_t ctx = placed ? len + n : 0;
-        const Two before = scan_block(Two{ctx, 0u}, total, s_warp);
+        if (placed && need > 0) taken = max(taken, add_held(at.b, need));
+        Three upto = add_held(base, total);
+        if (upto.b > count) {             // not all have a place: the sum of the contexts again
+            Three keys;
+            at.c = add_held(base.c, scan(Three{ctx, 0u, 0u}, keys).a);
+            upto.c = add_held(base.c, keys.a);
+        }
+        base = upto;
+        if (there) {
+            s_request[b] = Request{ours ? static_cast<int>(row) : -1, placed ? static_cast<int>(had) : 0, placed ? static_cast<int>(used) : 0, static_cast<int>(at.b)};
+            s_token[b] = Tokens{static_cast<int>(at.a), placed ? static_cast<int>(len) : -1};
+        }
         if (first_block && there) {       // (outputs of their own: nobody reads them here)
-            put(p.context_lens, p.wide, b, ctx);
-            if (p.cu_q != nullptr) put(p.cu_q, p.wide, b + 1, add_held(at.a, n));
-            if (p.cu_k != nullptr) put(p.cu_k, p.wide, b + 1, add_held(add_held(keys, before.a), ctx));
+            p.context_lens[b] = ctx;
+            if (p.cu_q != nullptr) p.cu_q[b + 1] = add_held(at.a, n);
+            if (p.cu_k != nullptr) p.cu_k[b + 1] = add_held(at.c, ctx);
         }
-        keys = add_held(keys, total.a);
-    }
-    if (first_block && tid == 0) {
-        if (p.cu_q != nullptr) put(p.cu_q, p.wide, 0, 0);
-        if (p.cu_k != nullptr) put(p.cu_k, p.wide, 0, 0);
-    }
-    const uint32_t tokens = base.a;
-    taken = __reduce_max_sync(0xffffffffu, taken);
-    if ((tid & 31) == 0) s_warp[tid >> 5].a = taken;
-    const bool copy = p.new_lens_out != p.lens.ptr;
-    const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads, me = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
-    if (copy) {
-        for (int64_t i = me; i < p.num_rows; i += threads) put(p.new_lens_out, p.wide, i, p.lens[i]);
-    }
-    if (gridDim.x > 1) cluster_sync();
-    else __syncthreads();
-    // From here on lengths and count are no longer read.
-    const IndexArray held(p.request_blocks, p.wide);
-    auto new_block = [&](const Request& r, uint32_t nth) { return p.free_blocks[static_cast<int64_t>(count) - 1 - r.first - nth]; };
-    auto end_of = [&](int b) { return b + 1 < p.batch ? static_cast<uint32_t>(s_request[b + 1].cu) : tokens; };
-    if (first_block) {
-        for (int b = tid; b < p.batch; b += kThreads) {
-            const Request r = s_request[b];
-            if (r.old_len >= 0) put(p.new_lens_out, p.wide, r.row, r.old_len + (end_of(b) - r.cu));
-        }
+    };
+    if (p.batch <= 32) {
         if (tid < 32) {
-            const uint32_t all = __reduce_max_sync(0xffffffffu, tid < kWarps ? s_warp[tid].a : 0u);
-            if (tid == 0) put(p.new_count, p.wide, 0, count - all);
+            requests(0, [&](Three v, Three& total) {
+                const Three x = scan_warp(v, lane);
+                total = shfl(x, 31);
+                return before_in_warp(x, lane);
+            });
         }
+    } else {
+        for (int b0 = 0; b0 < p.batch; b0 += THREADS) requests(b0, [&](Three v, Three& total) { return scan_block<kWarps>(v, total, s_warp); });
     }
+    s_free[tid] = free0;
+    if (tid == 0) {
+        s_tokens = base.a;
+        if (first_block && p.cu_q != nullptr) p.cu_q[0] = 0;
+        if (first_block && p.cu_k != nullptr) p.cu_k[0] = 0;
+    }
+    if (first_block) {
+        if (p.batch > 32) __syncthreads();   // (s_taken is zero)
+        else __syncwarp();
+        if (taken > 0) atomicMax(&s_taken, taken);
+    }
+    if (first_block && p.new_lens_out != p.lens) {   // (whole; the new ones follow)
+        for (int64_t i = tid; i < p.num_rows; i += THREADS) p.new_lens_out[i] = p.lens[i];
+    }
+    if (!p.wide && gridDim.x > 1) cluster_arrive();
+    __syncthreads();
+    // From here on lengths and count are no longer read.
+    const uint32_t tokens = s_tokens;
+    auto new_block = [&](uint32_t i) { return i < THREADS ? s_free[i] : p.free_blocks[static_cast<int64_t>(count) - 1 - i]; };
+    auto end_of = [&](int b) { return b + 1 < p.batch ? static_cast<uint32_t>(s_token[b + 1].cu) : tokens; };
     // Table entries.
-    const int64_t entries = static_cast<int64_t>(p.batch) * p.max_blocks;
-    for (int64_t i = me; i < entries; i += threads) {
-        const int b = static_cast<int>(p.by_width.div(static_cast<uint32_t>(i))), j = static_cast<int>(i - static_cast<int64_t>(b) * p.max_blocks);
-        const Request r = s_request[b];
-        int64_t id = 0;
-        if (r.old_len >= 0) {
-            const uint32_t had = blocks_of(p.by_block, r.old_len), used = blocks_of(p.by_block, r.old_len + (end_of(b) - r.cu));
-            const int64_t at = r.row * p.row_blocks + j;
-            if (j < had) {
-                id = held[at];
-            } else if (j < used) {
-                id = new_block(r, j - had);
-                put(p.request_blocks, p.wide, at, id);
-            }
-        }
-        put(p.block_tables, p.wide, i, id);
-    }
-    // Tokens.
-    for (int64_t t = me; t < p.num_tokens; t += threads) {
-        int64_t pos = 0, slot = -1;
-        if (t < tokens) {
-            // The last request that begins at or before t (those of no tokens begin where the next one does); of single tokens it is request t.
-            int lo = 0, hi = p.batch;
-            if (t < p.batch && s_request[t].cu == t && end_of(static_cast<int>(t)) == t + 1) {
-                lo = static_cast<int>(t);
-            } else {
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (s_request[mid].cu <= t) lo = mid;
-                    else hi = mid;
+    for (int i0 = me; i0 < pieces; i0 += kAhead * threads) {
+        if (i0 != me) {
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int i = i0 + u * threads;
+                if (i < pieces) {
+                    const int row = s_request[p.by_pieces.div(i)].row;
+                    if (row >= 0) load(i, row, piece[u]);
                 }
             }
-            const Request r = s_request[lo];
-            if (r.old_len >= 0) {
-                const uint32_t at = r.old_len + static_cast<uint32_t>(t - r.cu), j = p.by_block.div(at), had = blocks_of(p.by_block, r.old_len);
-                const int64_t id = j < had ? held[r.row * p.row_blocks + j] : new_block(r, j - had);
-                pos = at;
-                if (id >= 0 && id < p.num_cache_blocks) slot = id * p.by_block.d + (at - j * p.by_block.d);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = i0 + u * threads;
+            if (i >= pieces) break;
+            const int b = static_cast<int>(p.by_pieces.div(i)), j0 = (i - b * static_cast<int>(p.by_pieces.d)) * V;
+            const Request r = s_request[b];
+            if (j0 >= r.used) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) piece[u].e[k] = 0;
+            } else if (j0 + V > r.had) {                  // (not all of it was in use)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const int j = j0 + k;
+                    if (j >= r.had) piece[u].e[k] = 0;
+                    if (j >= r.had && j < r.used) {
+                        piece[u].e[k] = new_block(r.first + (j - r.had));
+                        p.request_blocks[r.row * p.row_blocks + j] = piece[u].e[k];
+                    }
+                }
+            }
+            *reinterpret_cast<Piece*>(p.block_tables + static_cast<int64_t>(i) * V) = piece[u];   // (rows are whole pieces)
+        }
+    }
+    // The last request that begins at or before token t (those of no tokens begin where the next one does); of single tokens it is request t.
+    auto request_of = [&](int64_t t) {
+        int lo = 0, hi = p.batch;
+        if (t < p.batch && s_token[t].cu == t && end_of(static_cast<int>(t)) == t + 1) return static_cast<int>(t);
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (s_token[mid].cu <= t) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    auto block_of = [&](const Request& r, uint32_t j) {
+        return static_cast<int64_t>(j < static_cast<uint32_t>(r.had) ? p.request_blocks[r.row * p.row_blocks + j] : new_block(r.first + (j - r.had)));
+    };
+    auto slot_of = [&](int64_t id, uint32_t off) { return id >= 0 && id < p.num_cache_blocks ? static_cast<E>(id * p.by_block.d + off) : static_cast<E>(-1); };
+    if (single) {
+        if (me < p.num_tokens) {
+            E pos = 0, slot = -1;
+            if (static_cast<uint32_t>(me) < tokens) {
+                const int b = request_of(me);
+                const Tokens x = s_token[b];
+                if (x.old_len >= 0) {
+                    const Request r = s_request[b];
+                    const uint32_t at = x.old_len + (me - x.cu), j = p.by_block.div(at);
+                    const bool guessed = b == me && x.cu == me && j < static_cast<uint32_t>(r.had);
+                    pos = static_cast<E>(at);
+                    slot = slot_of(guessed ? static_cast<int64_t>(guess) : block_of(r, j), at - j * p.by_block.d);
+                }
+            }
+            p.positions[me] = pos;
+            p.slots[me] = slot;
+        }
+    } else {
+        // Four next to each other a thread.
+        for (int64_t t0 = static_cast<int64_t>(me) * kTokens; t0 < p.num_tokens; t0 += static_cast<int64_t>(threads) * kTokens) {
+            int lo = t0 < tokens ? request_of(t0) : 0;
+            uint32_t at[kTokens], off[kTokens];
+            int64_t id[kTokens];
+            const Tokens x = s_token[lo];
+            const uint32_t at0 = x.old_len + static_cast<uint32_t>(t0 - x.cu), j0 = p.by_block.div(at0 & kMost), off0 = at0 - j0 * p.by_block.d;
+            if (t0 + kTokens <= tokens && x.old_len >= 0 && end_of(lo) >= t0 + kTokens && off0 + kTokens <= p.by_block.d) {   // all in one block
+                const int64_t one = block_of(s_request[lo], j0);
+#pragma unroll
+                for (int k = 0; k < kTokens; ++k) { at[k] = at0 + k; off[k] = off0 + k; id[k] = one; }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kTokens; ++k) {
+                    const int64_t t = t0 + k;
+                    at[k] = off[k] = 0;
+                    id[k] = -1;
+                    if (t < tokens && t < p.num_tokens) {
+                        while (end_of(lo) <= t) ++lo;     // (t < tokens, where the last one ends)
+                        const Tokens y = s_token[lo];
+                        if (y.old_len >= 0) {
+                            at[k] = y.old_len + static_cast<uint32_t>(t - y.cu);
+                            const uint32_t j = p.by_block.div(at[k]);
+                            off[k] = at[k] - j * p.by_block.d;
+                            id[k] = block_of(s_request[lo], j);
+                        }
+                    }
+                }
+            }
+            constexpr int kPiece = 16 / sizeof(E);
+            if (p.token_pieces && t0 + kTokens <= p.num_tokens) {
+#pragma unroll
+                for (int k0 = 0; k0 < kTokens; k0 += kPiece) {
+                    Entries<E, kPiece> pos, slot;
+#pragma unroll
+                    for (int k = 0; k < kPiece; ++k) {
+                        pos.e[k] = static_cast<E>(at[k0 + k]);
+                        slot.e[k] = slot_of(id[k0 + k], off[k0 + k]);
+                    }
+                    *reinterpret_cast<Entries<E, kPiece>*>(p.positions + t0 + k0) = pos;
+                    *reinterpret_cast<Entries<E, kPiece>*>(p.slots + t0 + k0) = slot;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kTokens; ++k) {
+                    if (t0 + k < p.num_tokens) {
+                        p.positions[t0 + k] = static_cast<E>(at[k]);
+                        p.slots[t0 + k] = slot_of(id[k], off[k]);
+                    }
+                }
             }
         }
-        put(p.positions, p.wide, t, pos);
-        put(p.slots, p.wide, t, slot);
+    }
+    if (first_block) {
+        if (!p.wide && gridDim.x > 1) cluster_wait();
+        if (!p.wide || p.new_lens_out != p.lens) {
+            for (int b = tid; b < p.batch; b += THREADS) {
+                const Tokens x = s_token[b];
+                if (x.old_len >= 0) p.new_lens_out[s_request[b].row] = x.old_len + (end_of(b) - x.cu);
+            }
+        }
+        if (tid == 0 && (!p.wide || p.new_count != p.free_count)) p.new_count[0] = count - s_taken;
     }
 }
 
-struct ReleaseParams {
-    IndexArray rows, first_blocks, lens, request_blocks, free_count;
-    void *free_blocks, *new_lens_out, *new_count;
-    int64_t num_rows, row_blocks, num_free;
-    int batch, wide;
-    uint32_t capacity;
-    FastDiv by_block;
-};
-
-// Blocks first_blocks[b] .. ceil(l_b / s) - 1 of each request behind those that are free already, in the requests' order.
-__global__ void __launch_bounds__(kThreads) release_blocks_kernel(const __grid_constant__ ReleaseParams p) {
-    extern __shared__ Request s_request[];   // row, first of its blocks, how many, where they go
-    __shared__ Two s_warp[kWarps];
+// After the many blocks of a large step: the lengths and the count that are updated in place.  A request with a place has a context length of its new length; what it
+// took is what that needs beyond its old one.  One block, one pass.
+template <typename E> __global__ void __launch_bounds__(kManyThreads) commit_step_kernel(const __grid_constant__ StepParams<E> p) {
+    __shared__ uint32_t s_taken;
     pdl_wait_then_release();
-    const int tid = threadIdx.x;
-    const int64_t count = min(max(p.free_count[0], static_cast<int64_t>(0)), p.num_free);
-    uint32_t base = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += kThreads) {
-        const int b = b0 + tid;
-        const bool there = b < p.batch;
-        const int64_t row = !there ? -1 : p.rows != nullptr ? p.rows[b] : b;
-        const bool known = there && row >= 0 && row < p.num_rows;
-        const int64_t len = known ? min(max(p.lens[row], static_cast<int64_t>(0)), static_cast<int64_t>(p.capacity)) : 0;
-        const int64_t first = known && p.first_blocks != nullptr ? max(p.first_blocks[b], static_cast<int64_t>(0)) : 0;
-        const int64_t held = blocks_of(p.by_block, static_cast<uint32_t>(len));
-        const uint32_t n = first < held ? static_cast<uint32_t>(held - first) : 0;
-        Two total;
-        const Two at = scan_block(Two{n, 0u}, total, s_warp);
-        if (there) s_request[b] = Request{known ? static_cast<int>(row) : -1, n > 0 ? static_cast<int>(first) : 0, static_cast<int>(n), static_cast<int>(add_held(at.a, base))};
-        base = add_held(base, total.a);
-    }
-    const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads, me = static_cast<int64_t>(blockIdx.x) * kThreads + tid;
-    if (p.new_lens_out != p.lens.ptr) {
-        for (int64_t i = me; i < p.num_rows; i += threads) put(p.new_lens_out, p.wide, i, p.lens[i]);
-    }
-    if (gridDim.x > 1) cluster_sync();
-    else __syncthreads();
-    // A warp to a request.
-    for (int b = static_cast<int>(me >> 5); b < p.batch; b += static_cast<int>(threads >> 5)) {
-        const Request r = s_request[b];
-        if (r.row < 0) continue;
-        if ((tid & 31) == 0) put(p.new_lens_out, p.wide, r.row, 0);
-        for (int j = tid & 31; j < r.cu; j += 32) {
-            const int64_t to = count + r.first + j;
-            if (to < p.num_free) put(p.free_blocks, p.wide, to, p.request_blocks[r.row * p.row_blocks + r.old_len + j]);
+    if (threadIdx.x == 0) s_taken = 0;
+    __syncthreads();
+    uint32_t taken = 0;
+    for (int b = threadIdx.x; b < p.batch; b += kManyThreads) {
+        const E row = p.rows != nullptr ? p.rows[b] : static_cast<E>(b);
+        const uint32_t ctx = static_cast<uint32_t>(p.context_lens[b]);
+        if (row >= 0 && row < p.num_rows && ctx > 0) {
+            // (where new lengths are of their own, the first kernel has set them: lens are still the old ones)
+            taken += blocks_of(p.by_block, ctx) - blocks_of(p.by_block, held(p.lens[row]));
+            if (p.new_lens_out == p.lens) p.new_lens_out[row] = ctx;
         }
     }
-    if (me == 0) put(p.new_count, p.wide, 0, min(count + base, p.num_free));
+    taken = __reduce_add_sync(0xffffffffu, taken);
+    if ((threadIdx.x & 31) == 0) atomicAdd(&s_taken, taken);
+    __syncthreads();
+    if (threadIdx.x == 0 && p.new_count == p.free_count)
+        p.new_count[0] = held(p.free_count[0], static_cast<uint32_t>(min(p.num_free, static_cast<int64_t>(kMost)))) - s_taken;
 }
 
-// One cluster of as many blocks as the work is worth: a block for each 4 entries of a thread.
+template <typename E> struct ReleaseParams {
+    const E *rows, *first_blocks, *lens, *request_blocks, *free_count;
+    E *free_blocks, *new_lens_out, *new_count;
+    int64_t num_rows, row_blocks, num_free;
+    int batch;
+    uint32_t capacity;
+    FastDiv by_block, by_chunks;          // by_chunks: of a request's blocks
+};
+
+// Blocks first_blocks[b] .. ceil(l_b / s) - 1 of each request behind those that are free already, in the requests' order.  A warp takes a chunk of a request's.
+constexpr int kChunk = 256;
+template <typename E>
+__global__ void __launch_bounds__(kFewThreads) release_blocks_kernel(const __grid_constant__ ReleaseParams<E> p) {
+    extern __shared__ __align__(16) Request s_request[];   // row, first of its blocks, how many, where they go
+    __shared__ Three s_warp[kFewThreads / 32];
+    pdl_wait_then_release();
+    const int tid = threadIdx.x;
+    const int threads = static_cast<int>(gridDim.x) * kFewThreads, me = static_cast<int>(blockIdx.x) * kFewThreads + tid;
+    const E count_in = p.free_count[0];
+    uint32_t base = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += kFewThreads) {
+        const int b = b0 + tid;
+        const bool there = b < p.batch;
+        const E row = !there ? -1 : p.rows != nullptr ? p.rows[b] : static_cast<E>(b);
+        const bool ours = there && row >= 0 && row < p.num_rows;
+        const uint32_t first = ours && p.first_blocks != nullptr ? held(p.first_blocks[b]) : 0;
+        const uint32_t used = blocks_of(p.by_block, ours ? held(p.lens[row], p.capacity) : 0);
+        const uint32_t n = first < used ? used - first : 0;
+        Three total;
+        const Three at = scan_block<kFewThreads / 32>(Three{n, 0u, 0u}, total, s_warp);
+        if (there) s_request[b] = Request{ours ? static_cast<int>(row) : -1, n > 0 ? static_cast<int>(first) : 0, static_cast<int>(n), static_cast<int>(add_held(at.a, base))};
+        base = add_held(base, total.a);
+    }
+    const int64_t count = held(count_in, static_cast<uint32_t>(min(p.num_free, static_cast<int64_t>(kMost))));
+    if (blockIdx.x == 0 && p.new_lens_out != p.lens) {
+        for (int64_t i = tid; i < p.num_rows; i += kFewThreads) p.new_lens_out[i] = p.lens[i];
+    }
+    if (gridDim.x > 1) cluster_arrive();
+    __syncthreads();
+    const int lane = tid & 31, chunks = static_cast<int>(p.by_chunks.d), units = p.batch * chunks;
+    for (int i = me >> 5; i < units; i += threads >> 5) {
+        const int b = static_cast<int>(p.by_chunks.div(i)), j0 = (i - b * chunks) * kChunk + lane;
+        const Request r = s_request[b];
+        if (r.row < 0) continue;
+        const E* from = p.request_blocks + r.row * p.row_blocks + r.had;
+        E id[kChunk / 32];
+#pragma unroll
+        for (int u = 0; u < kChunk / 32; ++u)
+            if (j0 + u * 32 < r.used) id[u] = from[j0 + u * 32];
+#pragma unroll
+        for (int u = 0; u < kChunk / 32; ++u) {
+            const int64_t to = count + r.first + j0 + u * 32;
+            if (j0 + u * 32 < r.used && to < p.num_free) p.free_blocks[to] = id[u];
+        }
+    }
+    if (blockIdx.x == 0) {
+        if (gridDim.x > 1) cluster_wait();
+        for (int b = tid; b < p.batch; b += kFewThreads) {
+            const int row = s_request[b].row;
+            if (row >= 0) p.new_lens_out[row] = 0;
+        }
+        if (tid == 0) p.new_count[0] = static_cast<E>(min(count + base, p.num_free));
+    }
+}
+
+// One cluster of as many blocks as the work is worth, or, `wide`, so many blocks by themselves.
 template <typename P>
-int launch(const char* what, void (*kernel)(P), const P& p, int64_t work, std::atomic<bool> (&attr_done)[64], cudaStream_t stream) {
+int launch(const char* what, void (*kernel)(P), const P& p, int threads, int64_t blocks_worth, bool wide, std::atomic<bool> (&attr_done)[64], cudaStream_t stream) {
     int device = 0;
     cudaGetDevice(&device);
     if (device >= 0 && device < 64 && !attr_done[device]) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBatch * static_cast<int>(sizeof(Request)));
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxBatch * static_cast<int>(sizeof(Request) + sizeof(Tokens)));
         if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
         attr_done[device] = true;
     }
     int blocks = 1;
-    while (blocks < kMaxBlocks && work > static_cast<int64_t>(blocks) * 4 * kThreads) blocks *= 2;
+    if (wide) blocks = static_cast<int>(std::min<int64_t>(blocks_worth, kSmCount));
+    else while (blocks < kMaxBlocks && blocks_worth > blocks) blocks *= 2;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = p.batch * sizeof(Request);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = p.batch * (sizeof(Request) + sizeof(Tokens));
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -267,44 +457,72 @@ int launch(const char* what, void (*kernel)(P), const P& p, int64_t work, std::a
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = blocks; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = blocks > 1 && !wide ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "%s kernel launch: %s", what, cudaGetErrorString(e));
     return check_launch(what);
+}
+
+template <typename E, int V> int launch_step(const StepArgs& a, uint32_t capacity) {
+    static std::atomic<bool> few_done[64] = {}, many_done[64] = {};
+    auto in = [](const IndexArray& x) { return static_cast<const E*>(x.ptr); };
+    auto out = [](void* x) { return static_cast<E*>(x); };
+    StepParams<E> p{};
+    p.new_lens = in(a.new_lens); p.rows = in(a.rows); p.lens = in(a.lens); p.free_blocks = static_cast<const E*>(a.free_blocks); p.free_count = in(a.free_count);
+    p.request_blocks = out(a.request_blocks); p.block_tables = out(a.block_tables); p.context_lens = out(a.context_lens); p.cu_q = out(a.cu_q); p.cu_k = out(a.cu_k);
+    p.positions = out(a.positions); p.slots = out(a.slots); p.new_lens_out = out(a.new_request_lens); p.new_count = out(a.new_free_count);
+    p.num_rows = a.num_rows; p.row_blocks = a.row_blocks; p.num_free = a.num_free; p.num_cache_blocks = a.num_cache_blocks; p.num_tokens = a.num_tokens;
+    p.batch = static_cast<int>(a.batch); p.max_blocks = static_cast<int>(a.max_blocks);
+    p.capacity = capacity;
+    p.by_block = FastDiv(static_cast<uint32_t>(a.block_size));
+    p.by_pieces = FastDiv(static_cast<uint32_t>(a.max_blocks / V));
+    p.token_pieces = aligned_to(a.positions, 16) && aligned_to(a.slots, 16);
+    const int64_t work = std::max(a.batch * a.max_blocks / V, a.num_tokens / 4);
+    if (a.batch <= kFewThreads && work <= kMaxBlocks * kFewThreads)
+        return launch("step_metadata", step_metadata_kernel<E, V, kFewThreads>, p, kFewThreads, work / kFewThreads + 1, false, few_done, a.stream);
+    p.wide = work > kWideWork;
+    const int rc = launch("step_metadata", step_metadata_kernel<E, V, kManyThreads>, p, kManyThreads, work / kManyThreads + 1, p.wide, many_done, a.stream);
+    if (rc != NVK_OK || !p.wide || (p.new_lens_out != p.lens && p.new_count != p.free_count)) return rc;
+    const cudaError_t e = launch_pdl(commit_step_kernel<E>, dim3(1), dim3(kManyThreads), 0, a.stream, p);
+    if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "commit_step_kernel launch: %s", cudaGetErrorString(e));
+    return check_launch("commit_step_kernel launch");
+}
+
+template <typename E> int launch_release(const StepArgs& a, uint32_t capacity) {
+    static std::atomic<bool> attr_done[64] = {};
+    auto in = [](const IndexArray& x) { return static_cast<const E*>(x.ptr); };
+    ReleaseParams<E> p{};
+    p.rows = in(a.rows); p.first_blocks = in(a.first_blocks); p.lens = in(a.lens); p.request_blocks = static_cast<const E*>(a.request_blocks); p.free_count = in(a.free_count);
+    p.free_blocks = static_cast<E*>(a.free_blocks); p.new_lens_out = static_cast<E*>(a.new_request_lens); p.new_count = static_cast<E*>(a.new_free_count);
+    p.num_rows = a.num_rows; p.row_blocks = a.row_blocks; p.num_free = a.num_free;
+    p.batch = static_cast<int>(a.batch);
+    p.capacity = capacity;
+    p.by_block = FastDiv(static_cast<uint32_t>(a.block_size));
+    p.by_chunks = FastDiv(static_cast<uint32_t>((a.row_blocks + kChunk - 1) / kChunk));
+    return launch("release_blocks", release_blocks_kernel<E>, p, kFewThreads, a.batch * p.by_chunks.d * 32 / kFewThreads + 1, false, attr_done, a.stream);
 }
 
 }  // namespace
 
 int launch_step_metadata(const StepArgs& a) {
     if (a.batch > kMaxBatch) return fail(NVK_ERR_UNSUPPORTED, "step_metadata: at most %d requests (got %lld)", kMaxBatch, static_cast<long long>(a.batch));
-    const int64_t blocks = std::min(a.row_blocks, a.max_blocks), most = (1LL << 31) - 1 - a.block_size;
-    if (a.batch * a.max_blocks > most || a.num_rows > most) return fail(NVK_ERR_UNSUPPORTED, "step_metadata: too many requests or table entries");
-    static std::atomic<bool> attr_done[64] = {};
-    StepParams p{};
-    p.new_lens = a.new_lens; p.rows = a.rows; p.lens = a.lens; p.free_blocks = IndexArray(a.free_blocks, a.wide); p.free_count = a.free_count;
-    p.request_blocks = a.request_blocks; p.block_tables = a.block_tables; p.context_lens = a.context_lens; p.cu_q = a.cu_q; p.cu_k = a.cu_k;
-    p.positions = a.positions; p.slots = a.slots; p.new_lens_out = a.new_request_lens; p.new_count = a.new_free_count;
-    p.num_rows = a.num_rows; p.row_blocks = a.row_blocks; p.num_free = a.num_free; p.num_cache_blocks = a.num_cache_blocks; p.num_tokens = a.num_tokens;
-    p.batch = static_cast<int>(a.batch); p.max_blocks = static_cast<int>(a.max_blocks); p.wide = a.wide;
-    p.capacity = static_cast<uint32_t>(blocks <= most / a.block_size ? blocks * a.block_size : most);
-    p.by_block = FastDiv(static_cast<uint32_t>(a.block_size));
-    p.by_width = FastDiv(static_cast<uint32_t>(a.max_blocks));
-    return launch("step_metadata", step_metadata_kernel, p, std::max(a.batch * a.max_blocks, a.num_tokens), attr_done, a.stream);
+    // (entries are counted in 32 bits, and beyond the last one by as many as all threads take at a time; lengths as well, and beyond the longest by a block)
+    const int64_t blocks = std::min(a.row_blocks, a.max_blocks), most = (1LL << 31) - 1 - a.block_size, ahead = kAhead * kSmCount * kManyThreads;
+    if (a.max_blocks > ((1LL << 31) - ahead) / std::max<int64_t>(a.batch, 1) || a.num_rows > most) return fail(NVK_ERR_UNSUPPORTED, "step_metadata: too many requests or table entries");
+    const uint32_t capacity = static_cast<uint32_t>(blocks <= most / a.block_size ? blocks * a.block_size : most);
+    // Table rows in pieces of 16 bytes where both tables' rows are whole ones.
+    const int v = a.wide ? 2 : 4;
+    const bool pieces = a.max_blocks % v == 0 && a.row_blocks % v == 0 && aligned_to(a.block_tables, 16) && aligned_to(a.request_blocks, 16);
+    if (a.wide) return pieces ? launch_step<int64_t, 2>(a, capacity) : launch_step<int64_t, 1>(a, capacity);
+    return pieces ? launch_step<int32_t, 4>(a, capacity) : launch_step<int32_t, 1>(a, capacity);
 }
 
 int launch_release_blocks(const StepArgs& a) {
     if (a.batch > kMaxBatch) return fail(NVK_ERR_UNSUPPORTED, "release_blocks: at most %d requests (got %lld)", kMaxBatch, static_cast<long long>(a.batch));
     const int64_t most = (1LL << 31) - 1 - a.block_size;
-    if (a.row_blocks > most || a.num_rows > most) return fail(NVK_ERR_UNSUPPORTED, "release_blocks: too many requests or blocks");
-    static std::atomic<bool> attr_done[64] = {};
-    ReleaseParams p{};
-    p.rows = a.rows; p.first_blocks = a.first_blocks; p.lens = a.lens; p.request_blocks = IndexArray(a.request_blocks, a.wide); p.free_count = a.free_count;
-    p.free_blocks = a.free_blocks; p.new_lens_out = a.new_request_lens; p.new_count = a.new_free_count;
-    p.num_rows = a.num_rows; p.row_blocks = a.row_blocks; p.num_free = a.num_free;
-    p.batch = static_cast<int>(a.batch); p.wide = a.wide;
-    p.capacity = static_cast<uint32_t>(a.row_blocks <= most / a.block_size ? a.row_blocks * a.block_size : most);
-    p.by_block = FastDiv(static_cast<uint32_t>(a.block_size));
-    return launch("release_blocks", release_blocks_kernel, p, a.batch * 32, attr_done, a.stream);
+    if (a.row_blocks > ((1LL << 31) - 1) / kMaxBatch * kChunk || a.num_rows > most) return fail(NVK_ERR_UNSUPPORTED, "release_blocks: too many requests or blocks");
+    const uint32_t capacity = static_cast<uint32_t>(a.row_blocks <= most / a.block_size ? a.row_blocks * a.block_size : most);
+    return a.wide ? launch_release<int64_t>(a, capacity) : launch_release<int32_t>(a, capacity);
 }
 
 }  // namespace nvk
