@@ -23,12 +23,23 @@ constexpr int kDim = 128;
 constexpr int kThreads = 256;
 constexpr int kLanes = kDim / 8;          // 16-byte pieces (eight elements) of a 16-bit head vector
 constexpr int kMaxSets = 16;              // (head, K or V) of a block of threads
-constexpr int kPasses = 16;               // pieces of a thread in registers
+constexpr int kPasses = 16;               // pieces of a thread of store_blocks_kernel in registers
+constexpr int kTileRows = kThreads * kPasses / kLanes;   // rows of a head, or of several together, that a block of threads holds
 
-// Absolute values of two elements as whole numbers: they order like the values, infinity and NaN above all.
-__device__ __forceinline__ uint32_t top_of(uint32_t top, uint32_t pair) { return __vmaxu2(top, pair & 0x7fff7fffu); }
-__device__ __forceinline__ uint32_t top_of(uint32_t top, const uint4& v) { return top_of(top_of(top_of(top_of(top, v.x), v.y), v.z), v.w); }
-__device__ __forceinline__ uint32_t halves_top(uint32_t top) { return max(top & 0xffffu, top >> 16); }
+// Two elements of T as one register.
+template <typename T> struct PairOf;
+template <> struct PairOf<__nv_bfloat16> { using type = __nv_bfloat162; };
+template <> struct PairOf<__half> { using type = __half2; };
+template <typename T> __device__ __forceinline__ typename PairOf<T>::type as_pair(uint32_t w) { return *reinterpret_cast<const typename PairOf<T>::type*>(&w); }
+template <typename P> __device__ __forceinline__ uint32_t as_word(P p) { return *reinterpret_cast<const uint32_t*>(&p); }
+
+// The largest absolute values so far of the elements in both halves of a word, NaN if one is.
+template <typename T> __device__ __forceinline__ uint32_t top_of(uint32_t top, uint32_t pair) { return as_word(__hmax2_nan(as_pair<T>(top), __habs2(as_pair<T>(pair)))); }
+template <typename T> __device__ __forceinline__ uint32_t top_of(uint32_t top, const uint4& v) {
+    return top_of<T>(top_of<T>(top_of<T>(top_of<T>(top, v.x), v.y), v.z), v.w);
+}
+// Of both halves, as a whole number: absolute values order like that, infinity and NaN above all.
+__device__ __forceinline__ uint32_t halves_top(uint32_t top) { return max(top & 0x7fffu, (top >> 16) & 0x7fffu); }
 
 template <typename T> __device__ __forceinline__ float2 floats_of(uint32_t w);
 template <> __device__ __forceinline__ float2 floats_of<__nv_bfloat16>(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
@@ -77,10 +88,51 @@ template <bool FP8> __device__ __forceinline__ float4 unpack4(uint32_t w) {
     }
 }
 
-template <typename T, bool FP8> __device__ __forceinline__ uint2 quantise8(const uint4& v, float inv) {
-    const float2 a = floats_of<T>(v.x), b = floats_of<T>(v.y), c = floats_of<T>(v.z), d = floats_of<T>(v.w);
-    return make_uint2(pack4<FP8>(a.x * inv, a.y * inv, b.x * inv, b.y * inv), pack4<FP8>(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
+// Bytes 0 of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410); }
+// Eight elements over the block's scale, `inv` = 1 / scale.  Products with a power of two are exact, and so
+//   * F16 -> e4m3: in f16 (what gets lost below its smallest normal number is far below half of e4m3's smallest);
+//   * F16 -> int8: one fma with 1536, whose spacing is 1, leaves the rounded number in the sum's low byte;
+//   * BF16: the same in fp32 (12582912), two at a time.
+// The f16 forms need `inv` to be a normal f16 number: scales from 2^-15 to 2^14.
+template <typename T, bool FP8> __device__ __forceinline__ uint2 quantise8(const uint4& v, float inv, bool narrow) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (std::is_same<T, __half>::value) {
+        if (narrow) {
+            const __half2 by = __float2half2_rn(inv);
+            uint32_t o[4];
+            if constexpr (FP8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    unsigned short e;
+                    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;\n" : "=h"(e) : "r"(as_word(__hmul2(as_pair<T>(w[i]), by))));
+                    o[i] = e;
+                }
+                return make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+            } else {
+                const uint32_t magic = 0x66006600u;   // 1536
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i] = as_word(__hfma2(as_pair<T>(w[i]), by, as_pair<T>(magic)));
+                return make_uint2(__byte_perm(o[0], o[1], 0x6420), __byte_perm(o[2], o[3], 0x6420));
+            }
+        }
+    }
+    if constexpr (FP8) {
+        const float2 a = floats_of<T>(w[0]), b = floats_of<T>(w[1]), c = floats_of<T>(w[2]), d = floats_of<T>(w[3]);
+        return make_uint2(pack4<FP8>(a.x * inv, a.y * inv, b.x * inv, b.y * inv), pack4<FP8>(c.x * inv, c.y * inv, d.x * inv, d.y * inv));
+    } else {
+        if (inv != inv) return make_uint2(0u, 0u);
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = floats_of<T>(w[i]);
+            asm("{\n\t.reg .b64 x, y, m, d;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 m, {%5, %5};\n\tfma.rn.f32x2 d, x, y, m;\n\tmov.b64 {%0, %1}, d;\n\t}\n"
+                : "=r"(o[2 * i]), "=r"(o[2 * i + 1]) : "f"(f.x), "f"(f.y), "f"(inv), "f"(12582912.0f));
+        }
+        return make_uint2(low_bytes(o[0], o[1], o[2], o[3]), low_bytes(o[4], o[5], o[6], o[7]));
+    }
 }
+__device__ __forceinline__ bool narrow_scale(float scale) { return scale >= 0x1p-15f && scale <= 0x1p14f; }
 
 // Rows [0, rows) of a head in a cache block, elements times `ratio`, by thread t of n.
 template <bool FP8> __device__ __forceinline__ void scale_rows(unsigned char* base, size_t stride, int rows, float ratio, int t, int n) {
@@ -137,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) store_row_kernel(const __grid_consta
             if (id >= 0 && id < p.num_cache_blocks) {
                 float* scale = p.scale[which] + id * p.num_kv_heads + head;
                 const float old = row > 0 ? *scale : 0.0f;
-                const uint32_t top = __reduce_max_sync(0xffffffffu, halves_top(top_of(top_of(0u, v.x), v.y)));
+                const uint32_t top = __reduce_max_sync(0xffffffffu, halves_top(top_of<T>(top_of<T>(0u, v.x), v.y)));
                 const float now = larger(old, scale_for<T, FP8>(top)), inv = __fdiv_rn(1.0f, now);
                 unsigned char* base = p.cache[which] + static_cast<size_t>(id) * p.block_size * row_bytes + head * kDim;
                 const float2 a = floats_of<T>(v.x), b = floats_of<T>(v.y);
@@ -193,22 +245,22 @@ __global__ void __launch_bounds__(kThreads, 2) store_blocks_kernel(const __grid_
     const bool live = set < static_cast<int>(p.by_sets.d);
     const int which = live && set >= p.num_kv_heads ? 1 : 0, head = live ? set - which * p.num_kv_heads : 0;
     const int mine = live ? rows : 0;                                   // (threads without a set go along)
-    const T* src = static_cast<const T*>(p.rows[which]) + (q0 + (first - start)) * p.stride[which] + head * kDim + sub * 8;
-    auto load = [&](int r) { return __ldcs(reinterpret_cast<const uint4*>(src + r * p.stride[which])); };
+    const T* src = static_cast<const T*>(p.rows[which]) + (q0 + (first - start) + rank) * p.stride[which] + head * kDim + sub * 8;
+    const int64_t step = ranks * p.stride[which];
+    auto load = [](const T* at) { return __ldcs(reinterpret_cast<const uint4*>(at)); };
     float* scale = p.scale[which] + id * p.num_kv_heads + head;
     const float old = live && row0 > 0 ? *scale : 0.0f;
     uint4 v[HELD ? kPasses : 1];
     uint32_t top = 0;
     if constexpr (HELD) {
+        const T* at = src;
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int r = rank + i * ranks;
-            v[i] = r < mine ? load(r) : make_uint4(0u, 0u, 0u, 0u);
-        }
+        for (int i = 0; i < kPasses; ++i, at += step) v[i] = rank + i * ranks < mine ? load(at) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) top = top_of(top, v[i]);
+        for (int i = 0; i < kPasses; ++i) top = top_of<T>(top, v[i]);
     } else {
-        for (int r = rank; r < mine; r += ranks) top = top_of(top, load(r));
+        const T* at = src;
+        for (int r = rank; r < mine; r += ranks, at += step) top = top_of<T>(top, *reinterpret_cast<const uint4*>(at));
     }
     top = halves_top(top);
 #pragma unroll
@@ -217,18 +269,18 @@ __global__ void __launch_bounds__(kThreads, 2) store_blocks_kernel(const __grid_
     __syncthreads();
     if (!live) return;
     const float now = larger(old, scale_for<T, FP8>(s_top[in_block])), inv = __fdiv_rn(1.0f, now);
+    const bool narrow = narrow_scale(now);
     const size_t row_bytes = static_cast<size_t>(p.num_kv_heads) * kDim;
     unsigned char* base = p.cache[which] + static_cast<size_t>(id) * p.block_size * row_bytes + head * kDim;
-    unsigned char* dst = base + row0 * row_bytes + sub * 8;
-    auto store = [&](int r, const uint4& x) { *reinterpret_cast<uint2*>(dst + r * row_bytes) = quantise8<T, FP8>(x, inv); };
+    unsigned char* dst = base + (row0 + rank) * row_bytes + sub * 8;
+    const size_t dst_step = ranks * row_bytes;
     if constexpr (HELD) {
 #pragma unroll
-        for (int i = 0; i < kPasses; ++i) {
-            const int r = rank + i * ranks;
-            if (r < rows) store(r, v[i]);
-        }
+        for (int i = 0; i < kPasses; ++i, dst += dst_step)
+            if (rank + i * ranks < rows) *reinterpret_cast<uint2*>(dst) = quantise8<T, FP8>(v[i], inv, narrow);
     } else {
-        for (int r = rank; r < rows; r += ranks) store(r, load(r));
+        const T* at = src;
+        for (int r = rank; r < rows; r += ranks, at += step, dst += dst_step) *reinterpret_cast<uint2*>(dst) = quantise8<T, FP8>(load(at), inv, narrow);
     }
     const bool raised = __float_as_int(old) != __float_as_int(now);
     if (t == 0 && raised) *scale = now;   // (read by this set's threads before the barrier)
@@ -242,23 +294,24 @@ template <typename T, bool FP8> int launch_store_typed(const StoreParams& in, cu
         const int64_t blocks = (static_cast<int64_t>(p.num_seqs) * p.by_sets.d + kThreads / 32 - 1) / (kThreads / 32);
         e = launch_pdl(store_row_kernel<T, FP8>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
     } else {
-        // As many sets to a block of threads as 16 pieces for each thread hold.
+        // As many sets to a block of threads as its registers hold.
         p.sets = 1;
-        while (p.sets < kMaxSets && 2 * p.sets * p.block_size <= kThreads) p.sets *= 2;
+        while (p.sets < kMaxSets && 2 * p.sets * p.block_size <= kTileRows) p.sets *= 2;
         const int64_t units = p.total_q / p.block_size + 2ll * p.num_seqs;
         if (units > 0x7fffffffLL) return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many tokens");
         const dim3 grid(static_cast<unsigned>(units), (p.by_sets.d + p.sets - 1) / p.sets);
         if (grid.y > 65535) return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many heads");
-        e = p.sets * p.block_size <= kThreads ? launch_pdl(store_blocks_kernel<T, FP8, true>, grid, dim3(kThreads), 0, stream, p)
-                                              : launch_pdl(store_blocks_kernel<T, FP8, false>, grid, dim3(kThreads), 0, stream, p);
+        e = p.sets * p.block_size <= kTileRows ? launch_pdl(store_blocks_kernel<T, FP8, true>, grid, dim3(kThreads), 0, stream, p)
+                                               : launch_pdl(store_blocks_kernel<T, FP8, false>, grid, dim3(kThreads), 0, stream, p);
     }
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "store_kvcache_blocks8 kernel launch: %s", cudaGetErrorString(e));
     return check_launch("store_kvcache_blocks8 kernel launch");
 }
 
 // ---- gather ----------------------------------------------------------------------------------------------------------------
-constexpr int kGatherRows = 32;           // dense rows of a block of threads, at most
-constexpr int kGatherAhead = 2;           // head vectors of K and of V that a lane has under way
+constexpr int kGatherRows = 256;          // dense rows of a block of threads, at most
+constexpr int kGatherVectors = 256;       // and of K and of V head vectors, where there are enough of them for two blocks to an SM
+constexpr int kGatherAhead = 4;           // head vectors of K and of V that a lane has under way
 constexpr int kGatherLanes = kDim / 16;   // lanes of a head vector
 
 struct GatherParams {
@@ -266,10 +319,20 @@ struct GatherParams {
     IndexArray cu; IndexArray block_tables;
     int64_t num_seqs, total, max_blocks, num_cache_blocks;
     int block_size, rows;                 // `rows` of a block of threads
-    FastDiv by_heads;
+    FastDiv by_heads, by_block;
 };
 
-template <typename T, bool FP8> __device__ __forceinline__ void dequantise16(const uint4& v, float scale, uint4* out) {
+// 32 bytes next to each other: one store where they lie on such a boundary.
+template <bool WIDE> __device__ __forceinline__ void store32(uint4* out, const uint32_t (&o)[8]) {
+    if constexpr (WIDE) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                     ::"l"(out), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+    } else {
+        out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+}
+template <typename T, bool FP8, bool WIDE> __device__ __forceinline__ void dequantise16(const uint4& v, float scale, uint4* out) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[8];
 #pragma unroll
@@ -278,32 +341,40 @@ template <typename T, bool FP8> __device__ __forceinline__ void dequantise16(con
         o[2 * i] = ElemTraits<T>::pack2(f.x * scale, f.y * scale);
         o[2 * i + 1] = ElemTraits<T>::pack2(f.z * scale, f.w * scale);
     }
-    out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    store32<WIDE>(out, o);
 }
 
-template <typename T, bool FP8>
+template <typename T, bool FP8, bool WIDE>
 __global__ void __launch_bounds__(kThreads) gather_blocks8_kernel(const __grid_constant__ GatherParams p) {
     __shared__ int64_t s_row[kGatherRows];     // cache row of a dense row; -1: zeros
     __shared__ int64_t s_block[kGatherRows];   // its cache block
+    __shared__ int64_t s_cu[kThreads];
     pdl_wait_then_release();
     const int64_t first = static_cast<int64_t>(blockIdx.x) * p.rows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(p.rows), p.total - first));
+    // The last sequence that begins at or before the first row: all threads look, one trip to memory where there are up to kThreads sequences.
+    int64_t seq = -1, base = 0;
+    for (;; base += kThreads) {
+        const int64_t s = base + threadIdx.x, begin = s <= p.num_seqs ? p.cu[s] : 0;
+        s_cu[threadIdx.x] = begin;
+        const int n = __syncthreads_count(s < p.num_seqs && begin <= first);
+        seq += n;
+        if (n < kThreads || base + kThreads >= p.num_seqs) break;
+        __syncthreads();
+    }
+    auto begin_of = [&](int64_t s) { return s >= base && s < base + kThreads ? s_cu[s - base] : p.cu[s]; };
     if (threadIdx.x < static_cast<unsigned>(rows)) {
         const int64_t r = first + threadIdx.x;
-        int64_t lo = 0, hi = p.num_seqs;     // the last sequence that begins at or before r
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) >> 1;
-            if (p.cu[mid] <= r) lo = mid;
-            else hi = mid;
-        }
-        const int64_t pos = r - p.cu[lo];
         int64_t row = -1, at = 0;
-        if (pos >= 0 && r < p.cu[lo + 1] && pos < p.max_blocks * p.block_size) {
-            const int64_t block = p.block_tables[lo * p.max_blocks + pos / p.block_size];
-            if (block >= 0 && block < p.num_cache_blocks) {
-                row = block * p.block_size + pos % p.block_size;
-                at = block;
+        if (seq >= 0) {
+            while (seq + 1 < p.num_seqs && begin_of(seq + 1) <= r) ++seq;
+            const int64_t pos = r - begin_of(seq);
+            if (pos >= 0 && r < begin_of(seq + 1) && pos < p.max_blocks * p.block_size) {
+                const int64_t blk = p.by_block.div(static_cast<uint32_t>(pos)), block = p.block_tables[seq * p.max_blocks + blk];
+                if (block >= 0 && block < p.num_cache_blocks) {
+                    row = block * p.block_size + (pos - blk * p.block_size);
+                    at = block;
+                }
             }
         }
         s_row[threadIdx.x] = row;
@@ -320,6 +391,7 @@ __global__ void __launch_bounds__(kThreads) gather_blocks8_kernel(const __grid_c
         float scale[kGatherAhead][2];
 #pragma unroll
         for (int u = 0; u < kGatherAhead; ++u) {
+            // (loads without branches, so that all are under way at once)
             const int i = min(i0 + u * kStride, vectors - 1), r = static_cast<int>(p.by_heads.div(i)), head = i - r * heads;
             const int64_t row = s_row[r], at = row >= 0 ? row * heads + head : 0, scale_at = s_block[r] * heads + head;
 #pragma unroll
@@ -334,14 +406,15 @@ __global__ void __launch_bounds__(kThreads) gather_blocks8_kernel(const __grid_c
             const int i = i0 + u * kStride;
             if (i < vectors) {
 #pragma unroll
-                for (int w = 0; w < 2; ++w) dequantise16<T, FP8>(v[u][w], scale[u][w], out[w] + static_cast<int64_t>(i) * kLanes);
+                for (int w = 0; w < 2; ++w) dequantise16<T, FP8, WIDE>(v[u][w], scale[u][w], out[w] + static_cast<int64_t>(i) * kLanes);
             }
         }
     }
 }
 
 template <typename T, bool FP8> cudaError_t launch_gather_typed(const GatherParams& p, int64_t blocks, cudaStream_t stream) {
-    return launch_pdl(gather_blocks8_kernel<T, FP8>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
+    const auto kernel = aligned_to(p.out[0], 32) && aligned_to(p.out[1], 32) ? gather_blocks8_kernel<T, FP8, true> : gather_blocks8_kernel<T, FP8, false>;
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
 }
 
 }  // namespace
@@ -364,8 +437,9 @@ int launch_store_blocks8(const Blocks8StoreArgs& a) {
 
 int launch_gather_blocks8(const Blocks8GatherArgs& a) {
     // Few rows are spread over the SMs.
-    int rows = kGatherRows;
-    while (rows > 1 && (a.total + rows - 1) / rows < 4 * kSmCount) rows >>= 1;
+    int rows = kGatherVectors / a.num_kv_heads;
+    while (rows > 1 && (a.total + rows - 1) / rows < 2 * kSmCount) rows >>= 1;
+    if (rows < 1) rows = 1;
     const int64_t blocks = (a.total + rows - 1) / rows;
     if (blocks > 0x7fffffffLL || a.num_kv_heads > 0x7fffffff / kGatherRows) return fail(NVK_ERR_UNSUPPORTED, "gather_kvcache_blocks8: too many rows");
     GatherParams p{};
@@ -375,6 +449,7 @@ int launch_gather_blocks8(const Blocks8GatherArgs& a) {
     p.num_seqs = a.num_seqs; p.total = a.total; p.max_blocks = a.max_blocks; p.num_cache_blocks = a.num_cache_blocks;
     p.block_size = a.block_size; p.rows = rows;
     p.by_heads = FastDiv(static_cast<uint32_t>(a.num_kv_heads));
+    p.by_block = FastDiv(static_cast<uint32_t>(a.block_size));
     using bf = __nv_bfloat16;
     const cudaError_t e = a.dtype == NVK_BF16 ? (a.fp8 ? launch_gather_typed<bf, true>(p, blocks, a.stream) : launch_gather_typed<bf, false>(p, blocks, a.stream))
                                               : (a.fp8 ? launch_gather_typed<__half, true>(p, blocks, a.stream) : launch_gather_typed<__half, false>(p, blocks, a.stream));

@@ -376,6 +376,7 @@ int nvk_gather_kvcache_blocks8(const void* k_cache, const void* v_cache, const f
         return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: sizes must be positive");
     if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
         return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: key, value and the caches must be 16-byte aligned, the scales 4-byte aligned");
+    if (max_blocks > ((1LL << 31) - 1) / block_size) return fail(NVK_ERR_UNSUPPORTED, "gather_kvcache_blocks8: too many blocks");
     if (total_k == 0) return NVK_OK;
     return launch_gather_blocks8(Blocks8GatherArgs{k_cache, v_cache, k_scale, v_scale, index_array(cu_seqlens_k, cu_seqlens_k_dtype),
                                                    index_array(block_tables, block_tables_dtype), num_seqs, total_k, max_blocks, num_cache_blocks, num_kv_heads,
