@@ -355,7 +355,18 @@ int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
     if (max_tokens <= 2048) return (max_tokens > 768 && pairs >= 250) || eight_warps(pairs, max_tokens) ? static_cast<int>(max_tokens) : 0;
     return max_tokens > 4096 && max_tokens <= 8192 && pairs >= 3 * kSmCount ? 4096 : 0;
 }
-Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size, int groups, bool have_workspace, bool four_bits = false) {
+// 8-bit caches with block scales are shared out like the other 8-bit ones, but in shorter chunks where those have chunks of 1024 or 2048 keys: their tiles take half the time, so that
+// a block's range ends sooner and what is left at the end counts for more.  768 keys up to four pairs to an SM, 1024 up to eight, where the workspace has room for the parts (it is sized for
+// the other caches).  us, as above: 64 pairs of 8192 keys 18.7 / 18.5 / 19.1, 19.9 / 21.3 / 30.6 -> 16.0 / 15.9 / 16.7, 17.5 / 23.7 / 29.7; 256 of 2048 12.1 / 14.7 / 16.7, 16.9 /
+// 21.1 / 31.9 -> 10.8 / 12.9 / 14.3, 16.5 / 22.3 / 28.3; 256 of 4096 13.9 / 16.2 / 20.9, 33.5 / 41.0 / 53.4 -> 12.2 / 14.7 / 19.1, 29.6 / 40.8 / 49.4; 800 of 8192 40.2 / 57.5 / 109.4, 154.0 /
+// 209.6 / 263.5 -> 36.7 / 55.4 / 104.9, 148.6 / 204.7 / 260.9; but 2048 of 8192 65.8 / 116.5 / 251.6, 364.6 / 510.0 / 655.4 -> 68.3 / 119.6 / 254.5, 366.2 / 502.0 / 686.5.
+int chunk_of_block_scales(int64_t pairs, int64_t max_tokens, int chunk, int block_size) {
+    if (chunk < 1024 || max_tokens <= chunk || pairs > 8 * kSmCount) return chunk;
+    const int finer = pairs <= 4 * kSmCount ? 768 : 1024;
+    return finer < chunk ? (finer + block_size - 1) / block_size * block_size : chunk;
+}
+Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max_blocks, int block_size, int groups, bool have_workspace, bool four_bits = false,
+                     size_t block_scale_room = 0) {   // block_scale_room: bytes of workspace, of a cache with block scales
     Splits s{cluster_size(batch, num_kv_heads, max_blocks, block_size, groups, have_workspace), 0, 0};
     if (s.cluster > 0) { s.count = s.cluster; return s; }
     const int64_t max_tokens = max_blocks * block_size;
@@ -378,6 +389,12 @@ Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max
         s.chunk *= 2;
         s.count = static_cast<int>((max_tokens + s.chunk - 1) / s.chunk);
     }
+    if (block_scale_room > 0) {
+        Splits finer = s;
+        finer.chunk = chunk_of_block_scales(batch * num_kv_heads, max_tokens, s.chunk, block_size);
+        finer.count = static_cast<int>((max_tokens + finer.chunk - 1) / finer.chunk);
+        if (part_bytes(part_count(finer, batch, num_kv_heads), num_heads / num_kv_heads) <= block_scale_room) return finer;
+    }
     return s;
 }
 
@@ -385,7 +402,7 @@ Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max
 
 // Kernel parameters of a decode call from host-known sizes only, for kernels with `groups` resident groups per SM; returns in
 // *cluster the cluster size, 0 = chunks.
-int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster, bool four_bits, int64_t ahead) {
+int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cluster, bool four_bits, int64_t ahead, bool block_scales) {
     DecodeParams p{};
     p.q = a.q; p.k_cache = a.k_cache; p.v_cache = a.v_cache;
     p.context_lens = a.context_lens; p.block_tables = a.block_tables; p.out = a.out;
@@ -397,7 +414,7 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     if (ahead == 0) ahead = four_bits ? Cache4<__half>::kKeysAhead : kTileTokens * kMaxCluster;   // how far numbers of keys go beyond the last one
     if (a.batch * a.num_heads * kMaxCluster >= (1LL << 31) || a.max_blocks * a.block_size >= (1LL << 31) - ahead)
         return fail(NVK_ERR_UNSUPPORTED, "decode attention: batch or block table too large");
-    const Splits s = choose_splits(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size, groups, a.workspace != nullptr, four_bits);
+    const Splits s = choose_splits(a.batch, a.num_heads, a.num_kv_heads, a.max_blocks, a.block_size, groups, a.workspace != nullptr, four_bits, block_scales ? a.workspace_bytes : 0);
     *cluster = s.cluster;
     p.per_seq = s.chunk == 0 ? 1 : 0;
     while ((1 << p.split_shift) < s.cluster) ++p.split_shift;
@@ -449,8 +466,8 @@ int check_grid(const DecodeArgs& a, const dec::DecodeParams& p) {   // of decode
 }
 
 // The format as decode_cluster_kernel takes it.
-template <class F, class = void> struct InClusters { using type = F; };
-template <class F> struct InClusters<F, std::void_t<typename F::InClusters>> { using type = typename F::InClusters; };
+template <class F, class = void> struct InClusters { static constexpr bool kBlockScales = false; using type = F; };
+template <class F> struct InClusters<F, std::void_t<typename F::InClusters>> { static constexpr bool kBlockScales = true; using type = typename F::InClusters; };
 
 // `scores`, `ml`, `weights`: where they are kept (F::kScores), the (maximum, sum) of every part, and what becomes of them; *plan: how the step was shared out.
 template <class F, typename T>
@@ -476,7 +493,7 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     int cluster = 0;
     int64_t ahead = 0;
     if constexpr (F::kOwnRun) ahead = F::kKeysAhead;
-    const int rc = decode_plan(a, F::kGroups, &p, &cluster, F::kFourBits, ahead);
+    const int rc = decode_plan(a, F::kGroups, &p, &cluster, F::kFourBits, ahead, InClusters<F>::kBlockScales);
     if (rc != NVK_OK) return rc;
     p.k_scale = k_scale; p.v_scale = v_scale;
     if constexpr (F::kScores) {
