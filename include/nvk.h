@@ -226,8 +226,9 @@ int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, cons
  * table are zeros.
  *
  * nvk_decode_attention_paged_blocks8: the semantics of nvk_decode_attention_paged over the values as they are; at most 8 query heads per KV head, block_size a
- * multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes).  Two roundings to f16: BF16 queries (elements below 2^-24 of the head's largest),
- * and a head's weight times the scale of the value, off by 2^-11 of itself or 2^-22 of the head's largest such product.
+ * multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes; where more of it is given a context may be shared out into more parts, whose sums differ
+ * in their last bits).  Query elements are off by 2^-20 (int8) or 2^-25 (e4m3) of their head's largest, and a head's weight times the scale of the value is
+ * rounded to f16: by 2^-11 of itself or 2^-22 of the head's largest such product.  scale must be finite; a query that is not gives NaN.
  */
 int nvk_store_kvcache_blocks8(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride, void* k_cache, void* v_cache,
                               float* k_scale, float* v_scale, int cache_dtype, const void* cu_seqlens_q, int cu_seqlens_q_dtype,

@@ -748,15 +748,26 @@ struct Cache4 {
 };
 
 // 8-bit cache with one fp32 scale, a power of two, for each (cache block, KV head): kv_blocks8.cu.  A warp takes 32 keys at a time, two chains of 16 as in Cache4, whose way of
-// finding the cache rows this is too; 16 keys lie in one cache block, so that their K and their V have one scale each.  Pieces, swizzles and the order of the contractions
-// are those of Cache8, but for the elements of a word of K: a register has elements {0, 2} or {1, 3}.
-//   * int8, K: the byte with its sign flipped in the low bits of an f16 is the subnormal number (n + 128) 2^-24; 128 sum(q) is taken off the sums afterwards.  (1152 sum(q), as
-//     with Cache8's bytes under the exponent of 1024, would cost them three bits more.)
-//   * int8, V: the byte glued under the exponent byte of 1024, and 1152 taken off right away, exactly (one HADD2 for two elements): sums over thousands of keys have no bits to spare.
-//   * Queries are brought to f16 by a power of two, each head's own (exact but for elements below 2^-24 of the head's largest), as in Cache4.
+// finding the cache rows this is too; 16 keys lie in one cache block, so that their K and their V have one scale each.
+//   * int8, K: the bytes go to the integer MMA as they are.  The query is a whole number, 2^14 q2 + 2^7 q1 + q0 with q0 and q1 from 0 to 127, by a power of two of each head's own (its
+//     elements are off by 2^-20 of the head's largest at most), and three MMAs of 32 elements do what two of 16 did in f16, without the three instructions that every word of K took
+//     there.  Sums are exact; they begin at the bits of 1.5 2^23, so that they are numbers of fp32 without a conversion.
+//   * e4m3, K: f16, with the query brought to f16 by a power of two (exact but for elements below 2^-24 of the head's largest), as in Cache4.
+//   * V: ldmatrix with transposed bytes, so that a word has one d of four keys, 4 t to 4 t + 3 for lane t.  The keys of a tile go to the scores' rows in the order that the output's contraction
+//     then asks for: row g has key 4 (g / 2) + (g & 1), row g + 8 the key two after it.  int8: the byte glued under the exponent byte of 1024, and 1152 taken off right
+//     away, exactly (one HADD2 for two elements): sums over thousands of keys have no bits to spare.
 //   * sum_k p_k s_k n_k: p' = p s 2^-E goes to the MMA in f16, exact but for its rounding; E is each head's own, chosen as in Cache4 by the largest product p s so
 //     far, and chosen again, with the sums rescaled, where a score passes the last maximum by 8 or a scale reaches 2^(7 + E).  So p' is rounded by 2^-11 of itself or 2^-22 of the
 //     head's largest, and one block whose scale is far above the others' does not cost them their bits.
+__device__ __forceinline__ void imma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));
+}
+// Two matrices of 16 x 16 bytes, transposed: lane (g, t) gets rows 4 t .. 4 t + 3 of columns g (first word) and g + 8 of each; lane l gives the address of row l & 15 of matrix l >> 4.
+__device__ __forceinline__ void ldmatrix_b8_trans(uint32_t (&w)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+}
 // CLUSTERS: for blocks that share a context in a cluster, and may have a few keys each (launches in chunks were 0.5 to 1.5 % slower with that code).
 template <typename T, bool FP8, bool CLUSTERS = false>
 struct CacheBlocks8 {
@@ -772,15 +783,17 @@ struct CacheBlocks8 {
     static constexpr int kTileBytes = kKeys * kRowBytes;
     static constexpr int kStageBytes = 2 * kTileBytes + 128;  // K, V, the scales (K, K, V, V) of both halves; (whole 128-byte lines: pieces are found by XOR)
     static constexpr int kStages = 2;
-    static constexpr int kPartStride = kHeadDim + 4;
+    static constexpr int kPartStride = kHeadDim + 8;
     static constexpr float kSlack = 8.0f;                     // by so much a score may pass s.m: p <= 2^8
     static constexpr uint32_t kNone = 0xffffffffu;
+    static constexpr int kParts = 3;                          // int8: bytes of a query element
+    static constexpr int kMagic = 0x4b400000;                 // 1.5 2^23: sums of 128 products of bytes stay within 2^21
 
     SoftmaxState s;
-    float score_scale[2], q_off[2];
+    float score_scale[2];
     float down[2];       // 2^-E of heads 2t, 2t + 1
     float top_part[2];   // the largest log2(p s) so far, p without the maximum taken off
-    uint32_t qa[8][2];   // k-step 4 q + w: elements 64 q + 16 t + 4 w + {0, 1 | 2, 3}, int8: {0, 2 | 1, 3}
+    uint32_t qa[FP8 ? 8 : 4 * kParts][2];   // elements 64 q + 16 t + 4 w + ..: e4m3, k-step 4 q + w: {0, 1 | 2, 3}; int8, part i of k-step 2 q + w / 2: {w even | w odd}
 
     __device__ __forceinline__ void start(const DecodeParams& p, int b, int kvh, int lane) {
         const int g = lane >> 2, t = lane & 3;
@@ -790,40 +803,44 @@ struct CacheBlocks8 {
         uint2 v[8];
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) v[ks] = live ? row[16 * (ks >> 2) + (ks & 3)] : make_uint2(0u, 0u);
-        float top = 0.0f;
+        uint32_t bits = 0;   // of the largest absolute value; infinity and NaN above all
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
             const float2 a = unpack2<T>(v[ks].x), c = unpack2<T>(v[ks].y);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(c.x), fabsf(c.y))));
+            bits = max(bits, max(max(__float_as_uint(fabsf(a.x)), __float_as_uint(fabsf(a.y))), max(__float_as_uint(fabsf(c.x)), __float_as_uint(fabsf(c.y)))));
         }
 #pragma unroll
-        for (int x = 1; x < 4; x *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        // the head's largest to [2^14, 2^15); (infinities and NaN stay what they are)
-        const int up = top > 0.0f && top < INFINITY ? min(14 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), 100) : 0;
+        for (int x = 1; x < 4; x *= 2) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, x));
+        const bool finite = bits < 0x7f800000u;
+        // the head's largest to [2^14, 2^15), int8: [2^19, 2^20)
+        const int up = bits > 0 && finite ? min((FP8 ? 14 : 19) - (static_cast<int>(bits >> 23) - 127), 100) : 0;
         const float by = power_of_two(up);
-        float sum = 0.0f;   // of the f16-rounded query
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
             const float2 a = unpack2<T>(v[ks].x), c = unpack2<T>(v[ks].y);
-            qa[ks][0] = ElemTraits<__half>::pack2(a.x * by, (FP8 ? a.y : c.x) * by);
-            qa[ks][1] = ElemTraits<__half>::pack2((FP8 ? c.x : a.y) * by, c.y * by);
-            const float2 x = unpack2<__half>(qa[ks][0]), y = unpack2<__half>(qa[ks][1]);
-            sum += (x.x + x.y) + (y.x + y.y);
-        }
+            if constexpr (FP8) {
+                qa[ks][0] = ElemTraits<__half>::pack2(a.x * by, a.y * by);
+                qa[ks][1] = ElemTraits<__half>::pack2(c.x * by, c.y * by);
+            } else {
+                // whole numbers in the low bits of a sum with 1.5 2^23; seven bits at a time, the last ones with the sign
+                auto number = [&](float f) { return __float_as_int(fmaf(f, by, __int_as_float(kMagic))) - kMagic; };
+                const int x[4] = {number(a.x), number(a.y), number(c.x), number(c.y)};
 #pragma unroll
-        for (int x = 1; x < 4; x *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                for (int i = 0; i < kParts; ++i) {
+                    const uint32_t word = __byte_perm(__byte_perm(x[0] >> (7 * i), x[1] >> (7 * i), 0x0040), __byte_perm(x[2] >> (7 * i), x[3] >> (7 * i), 0x0040), 0x5410);
+                    qa[4 * i + (ks >> 1)][ks & 1] = i < kParts - 1 ? word & 0x7f7f7f7fu : word;
+                }
+            }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            score_scale[h] = p.scale_log2 * power_of_two(-__shfl_sync(0xffffffffu, up, 8 * t + 4 * h));
-            q_off[h] = FP8 ? 0.0f : 128.0f * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * h);
+            const float scale = FP8 || finite ? p.scale_log2 * power_of_two(-up) : __uint_as_float(0x7fc00000u);   // (a query that is not finite: NaN)
+            score_scale[h] = __shfl_sync(0xffffffffu, scale, 8 * t + 4 * h);
         }
         down[0] = down[1] = 0x1p126f;
         top_part[0] = top_part[1] = -INFINITY;
         s.reset();
     }
-    // Four elements of K as two registers of an MMA operand.
-    static __device__ __forceinline__ uint32_t k_lo(uint32_t x) { return FP8 ? widen_pair_lo<FP8>(x) : (x ^ 0x00800080u) & 0x00ff00ffu; }
-    static __device__ __forceinline__ uint32_t k_hi(uint32_t x) { return FP8 ? widen_pair_hi<FP8>(x) : ((x >> 8) ^ 0x00800080u) & 0x00ff00ffu; }
     static __device__ __forceinline__ uint32_t whole(uint32_t glued) {   // two f16 of V, int8: less 1152
         if constexpr (FP8) return glued;
         const uint32_t off = 0xe480e480u;   // -1152
@@ -832,26 +849,53 @@ struct CacheBlocks8 {
     }
     static __device__ __forceinline__ uint32_t v_lo(uint32_t x) { return whole(widen_pair_lo<FP8>(x)); }
     static __device__ __forceinline__ uint32_t v_hi(uint32_t x) { return whole(widen_pair_hi<FP8>(x)); }
+    static __device__ __forceinline__ int key_of(int g) { return 2 * g - (g & 1); }   // of the scores' row g: 4 (g / 2) + (g & 1); two more for row g + 8
+    static __device__ __forceinline__ void mask(float (&sc)[4], int g, int valid) {
+        if (key_of(g) >= valid) sc[0] = sc[1] = -INFINITY;
+        if (key_of(g) + 2 >= valid) sc[2] = sc[3] = -INFINITY;
+    }
 
     // Scores of 16 keys, rows `row0` on of a stage.
     __device__ __forceinline__ void score(uint32_t stage, int row0, float k_scale, int lane, float (&sc)[4]) const {
         const int g = lane >> 2, t = lane & 3;
-        float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t at = stage + (row0 + g) * kRowBytes + ((t ^ ((g & 1) << 2)) << 4);
+        const uint32_t at = stage + (row0 + key_of(g)) * kRowBytes + ((t ^ ((g & 1) << 2)) << 4);
+        uint32_t w0[2][4], w1[2][4];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-            uint32_t w0[4], w1[4];
-            lds32x4(at ^ (q * 64), w0);
-            lds32x4((at ^ (q * 64)) + 8 * kRowBytes, w1);
-#pragma unroll
-            for (int wi = 0; wi < 4; ++wi) {
-                const int ks = 4 * q + wi;
-                mma_16816<__half>(q ? s1 : s0, k_lo(w0[wi]), k_lo(w1[wi]), k_hi(w0[wi]), k_hi(w1[wi]), qa[ks][0], qa[ks][1]);
-            }
+            lds32x4(at ^ (q * 64), w0[q]);
+            lds32x4((at ^ (q * 64)) + 2 * kRowBytes, w1[q]);
         }
         const float by[2] = {score_scale[0] * k_scale, score_scale[1] * k_scale};
+        if constexpr (FP8) {
+            float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = (FP8 ? s0[i] + s1[i] : fmaf(s0[i] + s1[i], 0x1p24f, -q_off[i & 1])) * by[i & 1];
+            for (int q = 0; q < 2; ++q) {
+#pragma unroll
+                for (int wi = 0; wi < 4; ++wi)
+                    mma_16816<__half>(q ? s1 : s0, widen_pair_lo<FP8>(w0[q][wi]), widen_pair_lo<FP8>(w1[q][wi]), widen_pair_hi<FP8>(w0[q][wi]), widen_pair_hi<FP8>(w1[q][wi]),
+                                      qa[4 * q + wi][0], qa[4 * q + wi][1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[i] = (s0[i] + s1[i]) * by[i & 1];
+        } else {
+            const int zero[4] = {kMagic, kMagic, kMagic, kMagic};
+            int x[kParts][4];
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) {
+                const int q = ks >> 1, w = 2 * (ks & 1);
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) {
+                    if (ks == 0) imma_16832(x[i], w0[q][w], w1[q][w], w0[q][w + 1], w1[q][w + 1], qa[4 * i + ks][0], qa[4 * i + ks][1], zero);
+                    else imma_16832(x[i], w0[q][w], w1[q][w], w0[q][w + 1], w1[q][w + 1], qa[4 * i + ks][0], qa[4 * i + ks][1], x[i]);
+                }
+            }
+            constexpr float kTaken = 12582912.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float lo = __int_as_float(x[0][i]) - kTaken, mid = __int_as_float(x[1][i]) - kTaken, hi = __int_as_float(x[2][i]) - kTaken;
+                sc[i] = fmaf(fmaf(hi, 128.0f, mid), 128.0f, lo) * by[i & 1];
+            }
+        }
     }
     __device__ __forceinline__ int exponent(int h) const { return 127 - static_cast<int>(__float_as_uint(down[h]) >> 23); }   // E
     __device__ __forceinline__ bool raises(const float (&sa)[4], const float (&sb)[4], float va, float vb) const {
@@ -891,27 +935,24 @@ struct CacheBlocks8 {
     }
     // What 16 keys add to the sums.
     __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], float v_scale, int lane) {
-        const int g = lane >> 2, t = lane & 3;
         const float p0 = weight(sc[0] - s.m[0]), p1 = weight(sc[1] - s.m[1]), p2 = weight(sc[2] - s.m[0]), p3 = weight(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
         const float part[2] = {v_scale * down[0], v_scale * down[1]};
         const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * part[0], p1 * part[1]));
         const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * part[0], p3 * part[1]));
-        // V rows 2t, 2t+1, 2t+8, 2t+9, piece g (d = 16 g .. 16 g + 15)
-        const uint32_t at = stage + kTileBytes + (row0 + 2 * t) * kRowBytes + ((g ^ (2 * t)) << 4);
+        // V rows of the tile, two d-tiles of 16 at a time
+        const int row = row0 + (lane & 15);
+        const uint32_t at = stage + kTileBytes + row * kRowBytes + (((lane >> 4) ^ (row & 7)) << 4);
         constexpr uint32_t kFlip = FP8 ? 0u : 0x80808080u;
-        uint32_t v0[4], v1[4], v2[4], v3[4];
-        lds32x4(at, v0);
-        lds32x4(at + kRowBytes, v1);
-        lds32x4(at + 8 * kRowBytes, v2);
-        lds32x4(at + 9 * kRowBytes, v3);
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
-            const uint32_t lo01 = __byte_perm(v0[a], v1[a], 0x5140) ^ kFlip, hi01 = __byte_perm(v0[a], v1[a], 0x7362) ^ kFlip;
-            const uint32_t lo23 = __byte_perm(v2[a], v3[a], 0x5140) ^ kFlip, hi23 = __byte_perm(v2[a], v3[a], 0x7362) ^ kFlip;
-            mma_16816<__half>(s.o[2 * a], v_lo(lo01), v_hi(lo01), v_lo(lo23), v_hi(lo23), pb0, pb1);
-            mma_16816<__half>(s.o[2 * a + 1], v_lo(hi01), v_hi(hi01), v_lo(hi23), v_hi(hi23), pb0, pb1);
+            uint32_t v[4];
+            ldmatrix_b8_trans(v, at ^ (a * 32));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] ^= kFlip;
+            mma_16816<__half>(s.o[2 * a], v_lo(v[0]), v_lo(v[1]), v_hi(v[0]), v_hi(v[1]), pb0, pb1);
+            mma_16816<__half>(s.o[2 * a + 1], v_lo(v[2]), v_lo(v[3]), v_hi(v[2]), v_hi(v[3]), pb0, pb1);
         }
     }
     // 32 keys, of which `valid` (more than none) are there.
@@ -920,7 +961,7 @@ struct CacheBlocks8 {
         asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(ka), "=f"(kb), "=f"(va), "=f"(vb) : "r"(stage + 2 * kTileBytes));
         if (CLUSTERS && valid <= 16) {   // (a range's last keys, or all that a warp has of a short one)
             score(stage, 0, ka, lane, sa);
-            mask_scores(sa, lane >> 2, valid);
+            mask(sa, lane >> 2, valid);
             sb[0] = sb[1] = sb[2] = sb[3] = -INFINITY;
             if (__any_sync(0xffffffffu, raises(sa, sb, va, 0.0f))) raise(sa, sb, va, 0.0f);
             add(stage, 0, sa, va, lane);
@@ -929,8 +970,8 @@ struct CacheBlocks8 {
         score(stage, 0, ka, lane, sa);
         score(stage, 16, kb, lane, sb);
         if (valid < kKeys) {
-            mask_scores(sa, lane >> 2, valid);
-            mask_scores(sb, lane >> 2, valid - 16);
+            mask(sa, lane >> 2, valid);
+            mask(sb, lane >> 2, valid - 16);
         }
         if (__any_sync(0xffffffffu, raises(sa, sb, va, vb))) raise(sa, sb, va, vb);
         add(stage, 0, sa, va, lane);
@@ -985,8 +1026,8 @@ struct CacheBlocks8 {
             v_at[i] = static_cast<const unsigned char*>(p.v_cache) + (4 * i + r) * row_bytes + c * 16;
         }
         const float* scale_from = static_cast<const float*>((lane & 2) ? p.v_scale : p.k_scale);   // lanes 0 to 3: (K, K, V, V) of halves (0, 1, 0, 1)
-        // Swizzles of row 4 i + r: K piece c ^ ((row & 1) << 2), V piece c ^ (row & 6): for odd i 4 more.
-        const uint32_t k_to = r * kRowBytes + ((c ^ ((r & 1) << 2)) << 4), v_to = kTileBytes + r * kRowBytes + ((c ^ (r & 2)) << 4);
+        // Swizzles of row 4 i + r, for reads without bank conflicts: K piece c ^ ((row & 1) << 2), V piece c ^ (row & 7), of which odd i have 4 more.
+        const uint32_t k_to = r * kRowBytes + ((c ^ ((r & 1) << 2)) << 4), v_to = kTileBytes + r * kRowBytes + ((c ^ r) << 4);
         const int left_all = span == 16 ? min(t1 - first, 16) : t1 - first;   // (a warp's only tile)
         int issued = 0, left = left_all;                      // keys from the next tile on
         uint32_t istage = ring;
@@ -1058,8 +1099,7 @@ struct CacheBlocks8 {
     __device__ __forceinline__ void write_part(float* row, int h, int g) const {
         const float up = power_of_two(exponent(h));
 #pragma unroll
-        for (int i = 0; i < 8; i += 2)
-            *reinterpret_cast<float4*>(row + 16 * g + 2 * i) = make_float4(s.o[i][h] * up, s.o[i][2 + h] * up, s.o[i + 1][h] * up, s.o[i + 1][2 + h] * up);
+        for (int i = 0; i < 16; ++i) row[8 * i + g] = s.o[i >> 1][(i & 1) * 2 + h] * up;
     }
 };
 

@@ -289,7 +289,7 @@ def test_gather(kind, dtype, bs, hkv, lens, index):
         assert torch.equal(out[w].cpu().double(), torch.from_numpy(want).to(out[w].dtype).double())
 
 
-# How far a decode output can be off.  A score: the query to f16 (2^-25 of the head's largest, whose power of two is taken out first), 128 products summed in fp32 and 8
+# How far a decode output can be off.  A score: the query's elements (by 2^-25 of the head's largest, int8: 2^-20), 128 products summed in fp32 and 8
 # operations more, each addition by 2^-23 of the sum of magnitudes at most (the MMA may cut off instead of rounding).  A weight p by a factor e^(2 score error), its
 # exponential by 2^-20; p s to f16: 2^-11 of itself, or, where it is less than 2^-10 of the head's largest, 2^-22 of that; sums over the keys and the merges: 2^-23 for every one of
 # some 300 operations of a chain, of the sum of magnitudes.
@@ -298,7 +298,7 @@ def _bound(c, table, n, q, scale, dtype):
     k, v = (r.rows(table, n) for r in c.ref)
     per = q.shape[0] // c.hkv
     kk, vv = (np.repeat(np.abs(x), per, axis=1) for x in (k, v))          # [n, Hq, D]
-    score = abs(scale) * (136 * 2.0 ** -23 * np.einsum("hd,nhd->nh", np.abs(q), kk).max(0) + 2.0 ** -25 * np.abs(q).max(-1) * kk.sum(-1).max(0))
+    score = abs(scale) * (136 * 2.0 ** -23 * np.einsum("hd,nhd->nh", np.abs(q), kk).max(0) + (2.0 ** -25 if c.kind == "e4m3" else 2.0 ** -20) * np.abs(q).max(-1) * kk.sum(-1).max(0))
     s = np.einsum("hd,nhd->hn", q, np.repeat(k, per, axis=1)) * scale
     p = np.exp(s - s.max(-1, keepdims=True))
     p /= p.sum(-1, keepdims=True)
