@@ -49,6 +49,27 @@ StepArrays build_prefill_arrays(const std::vector<SequenceView>& seqs, int block
 // to the longest table of the batch.
 StepArrays build_decode_arrays(const std::vector<SequenceView>& seqs, int block_size);
 
+// The same on the device, with the cache blocks handed out there too (not in the reference): for steps that the host does not prepare, such as a decode loop that is replayed as a
+// CUDA graph.  Index tensors of one width, int32 or int64.
+struct RequestTables {           // kept from step to step
+    Tensor lens;                 // [rows] tokens in the cache
+    Tensor blocks;               // [rows, max_blocks] cache blocks, ceil(length / block_size) of them in use
+    Tensor free_blocks;          // free ones, of which the first free_count[0] are free; the last of them is taken first
+    Tensor free_count;           // [1]
+    int block_size = 0;
+    int64_t num_cache_blocks = 0;
+};
+struct DeviceStep {              // what a step is made of; cu_seqlens_* and (both) positions and slot_mapping may be undefined
+    Tensor block_tables;         // [batch, max_blocks], zero padded
+    Tensor context_lens;         // [batch]; 0: the request has no place in this step
+    Tensor cu_seqlens_q, cu_seqlens_k;   // [batch + 1]
+    Tensor positions, slot_mapping;      // [tokens], more of them than there are: position 0, slot -1
+};
+// new_lens[b] tokens for the request in row rows[b] of the tables (undefined: row b), which are updated in place (nvk_step_metadata has the rules).
+void build_step(const Tensor& new_lens, const Tensor& rows, RequestTables& tables, DeviceStep& step, cudaStream_t stream = nullptr);
+// The blocks of requests that ended, from first_blocks[b] on (undefined: all), behind the free ones; rows undefined: all rows.
+void release_blocks(const Tensor& rows, const Tensor& first_blocks, RequestTables& tables, cudaStream_t stream = nullptr);
+
 // KV-cache sizing and per-layer slicing of one [2, L, blocks, block_size, Hkv / tp, D] allocation.
 struct KvCachePlan {
     int num_layers = 0, block_size = 0, local_kv_heads = 0, head_dim = 0;

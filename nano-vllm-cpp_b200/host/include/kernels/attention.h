@@ -47,6 +47,12 @@ void launch_decode_attention_paged_int4(const Tensor& query, const Tensor& k_cac
                                         const Tensor& block_tables, int num_kv_heads, int head_dim, int block_size,
                                         float scale, Tensor& output, DeviceAllocator& allocator, cudaStream_t stream = nullptr);
 
+// Decode attention over an 8-bit cache with block scales (store_kvcache_blocks8); split-K scratch is taken from `allocator`.
+void launch_decode_attention_paged_blocks8(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                                           const Tensor& k_scale, const Tensor& v_scale, const Tensor& context_lens,
+                                           const Tensor& block_tables, float scale, Tensor& output,
+                                           DeviceAllocator& allocator, bool e4m3 = false, cudaStream_t stream = nullptr);
+
 // Decode attention that adds every key's attention weights to new_key_weights = key_weights + .. (float32 [rows, Hkv, keys]; key_weights undefined: zeros, or
 // the same tensor).  Undefined k_params / v_params: a 16-bit cache; undefined weight_rows: sequence b has row b.
 void launch_decode_attention_paged_weights(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,

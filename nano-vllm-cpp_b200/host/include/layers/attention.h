@@ -21,6 +21,10 @@ public:
     // gather_kvcache_int4 brings out of them (prefix hits, chunks), in scratch from the allocator: total_seqlen_k rows where the context has it (StepUploader
     // sets it), otherwise max_seqlen_k of every sequence.
     void set_kv_cache_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params);
+    // 8-bit caches [blocks, block_size, Hkv, 128] (byte tensors, int8; `e4m3`: of e4m3 elements) with one float32 scale for each block and KV head [blocks, Hkv].  The store goes by
+    // sequences, so that the context of every step, a prefill's too, has context_lens and block_tables (build_step gives both); decode reads the cache through
+    // launch_decode_attention_paged_blocks8, and a prefill attends over the rows that gather_kvcache_blocks8 brings out of it, as with a 4-bit cache.
+    void set_kv_cache_blocks8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, bool e4m3 = false);
     // From here on decode steps over a 16-bit or a 4-bit cache add every key's attention weights to `key_weights` [rows, Hkv, keys], float32, for
     // evict_kvcache; `rows` [batch] or undefined, as there.  Undefined weights: no longer.
     void set_key_weights(const Tensor& key_weights, const Tensor& rows = Tensor());
@@ -43,7 +47,8 @@ public:
     Tensor& v_params() { return v_scale_; }
     bool is_int8() const { return is_int8_; }
     bool is_int4() const { return is_int4_; }
-    bool is_quantised() const { return is_int8_ || is_int4_; }
+    bool is_blocks8() const { return is_blocks8_; }
+    bool is_quantised() const { return is_int8_ || is_int4_ || is_blocks8_; }
 
 private:
     void decode(const Tensor& query, Tensor& output, DeviceAllocator& allocator, cudaStream_t stream);
@@ -59,6 +64,8 @@ private:
     Tensor v_scale_;
     bool is_int8_ = false;
     bool is_int4_ = false;
+    bool is_blocks8_ = false;
+    bool is_e4m3_ = false;
     Tensor key_weights_;
     Tensor weight_rows_;
 };

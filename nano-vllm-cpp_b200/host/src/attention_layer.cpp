@@ -53,7 +53,7 @@ void Attention::set_kv_cache(const Tensor& k_cache, const Tensor& v_cache) {
     if (k_cache.sizes() != v_cache.sizes()) throw std::invalid_argument("k_cache and v_cache must have the same shape");
     k_cache_ = k_cache;
     v_cache_ = v_cache;
-    is_int8_ = is_int4_ = false;
+    is_int8_ = is_int4_ = is_blocks8_ = false;
 }
 
 void Attention::set_kv_cache_int8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale) {
@@ -70,7 +70,7 @@ void Attention::set_kv_cache_int8(const Tensor& k_cache, const Tensor& v_cache, 
     k_scale_ = k_scale;
     v_scale_ = v_scale;
     is_int8_ = true;
-    is_int4_ = false;
+    is_int4_ = is_blocks8_ = false;
 }
 
 void Attention::set_kv_cache_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params) {
@@ -89,8 +89,30 @@ void Attention::set_kv_cache_int4(const Tensor& k_cache, const Tensor& v_cache, 
     v_cache_ = v_cache;
     k_scale_ = k_params;
     v_scale_ = v_params;
-    is_int8_ = false;
+    is_int8_ = is_blocks8_ = false;
     is_int4_ = true;
+}
+
+void Attention::set_kv_cache_blocks8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, bool e4m3) {
+    require_cuda_contiguous("k_cache", k_cache);
+    require_cuda_contiguous("v_cache", v_cache);
+    require_cuda_contiguous("k_scale", k_scale);
+    require_cuda_contiguous("v_scale", v_scale);
+    if (k_cache.dtype() != ScalarType::kInt8 || v_cache.dtype() != ScalarType::kInt8)
+        throw std::invalid_argument("8-bit KV cache tensors must be byte (int8) tensors");
+    if (k_scale.dtype() != ScalarType::kFloat32 || v_scale.dtype() != ScalarType::kFloat32)
+        throw std::invalid_argument("8-bit KV cache block scales must be float32");
+    if (head_dim_ != 128) throw std::invalid_argument("an 8-bit KV cache with block scales needs head_dim 128");
+    if (k_cache.dim() != 4 || k_cache.sizes() != v_cache.sizes() || k_cache.sizes()[1] != block_size_ || k_cache.sizes()[2] != num_kv_heads_ ||
+        k_cache.sizes()[3] != head_dim_ || static_cast<int64_t>(k_scale.numel()) != k_cache.sizes()[0] * num_kv_heads_ || k_scale.numel() != v_scale.numel())
+        throw std::invalid_argument("8-bit KV caches must be [blocks, block_size, num_kv_heads, head_dim], with a scale for every block and KV head");
+    k_cache_ = k_cache;
+    v_cache_ = v_cache;
+    k_scale_ = k_scale;
+    v_scale_ = v_scale;
+    is_int8_ = is_int4_ = false;
+    is_blocks8_ = true;
+    is_e4m3_ = e4m3;
 }
 
 void Attention::set_key_weights(const Tensor& key_weights, const Tensor& rows) {
@@ -128,7 +150,12 @@ Tensor Attention::forward(const Tensor& query, const Tensor& key, const Tensor& 
     if (ctx.block_tables.defined()) require_index_tensor("block_tables", ctx.block_tables);
 
     // new K/V go into the cache first: both prefill-with-prefix and decode read them back from it
-    if (k_cache_.defined() && ctx.slot_mapping.defined()) {
+    if (is_blocks8_) {
+        if (!ctx.context_lens.defined() || !ctx.block_tables.defined() || (ctx.is_prefill && !ctx.cu_seqlens_q.defined()))
+            throw std::invalid_argument("an 8-bit cache with block scales requires context_lens, block_tables and, for a prefill, cu_seqlens_q");
+        store_kvcache_blocks8(key, value, k_cache_, v_cache_, k_scale_, v_scale_, ctx.is_prefill ? ctx.cu_seqlens_q : Tensor(), ctx.context_lens, ctx.block_tables,
+                              is_e4m3_, stream);
+    } else if (k_cache_.defined() && ctx.slot_mapping.defined()) {
         if (is_int8_) {
             store_kvcache_int8(key, value, k_cache_, v_cache_, k_scale_, v_scale_, ctx.slot_mapping, stream);
         } else if (is_int4_) {
@@ -143,14 +170,15 @@ Tensor Attention::forward(const Tensor& query, const Tensor& key, const Tensor& 
     if (ctx.is_prefill) {
         const Tensor* cu_q = ctx.cu_seqlens_q.defined() ? &ctx.cu_seqlens_q : nullptr;
         const Tensor* cu_k = ctx.cu_seqlens_k.defined() ? &ctx.cu_seqlens_k : nullptr;
-        if (paged && is_int4_) {
+        if (paged && (is_int4_ || is_blocks8_)) {
             if (cu_q == nullptr || cu_k == nullptr) throw std::invalid_argument("prefill attention with block_tables requires cu_seqlens_q and cu_seqlens_k");
             const int64_t seqs = static_cast<int64_t>(cu_k->numel()) - 1;
             const int64_t longest = ctx.max_seqlen_k > 0 ? ctx.max_seqlen_k : ctx.block_tables.sizes().back() * block_size_;
             const int64_t rows = ctx.total_seqlen_k > 0 ? ctx.total_seqlen_k : seqs * longest;   // (what is behind the last sequence is written as zeros)
             Tensor dense_k = Tensor::scratch({rows, num_kv_heads_, head_dim_}, query.dtype(), query.device(), allocator, stream);
             Tensor dense_v = Tensor::scratch(dense_k.sizes(), query.dtype(), query.device(), allocator, stream);
-            gather_kvcache_int4(k_cache_, v_cache_, k_scale_, v_scale_, *cu_k, ctx.block_tables, num_kv_heads_, head_dim_, block_size_, dense_k, dense_v, stream);
+            if (is_int4_) gather_kvcache_int4(k_cache_, v_cache_, k_scale_, v_scale_, *cu_k, ctx.block_tables, num_kv_heads_, head_dim_, block_size_, dense_k, dense_v, stream);
+            else gather_kvcache_blocks8(k_cache_, v_cache_, k_scale_, v_scale_, *cu_k, ctx.block_tables, dense_k, dense_v, is_e4m3_, stream);
             launch_prefill_attention_dense(query, cu_q, dense_k, dense_v, cu_k, num_kv_heads_, head_dim_, scale_, output, stream, ctx.max_seqlen_q);
         } else if (paged && !is_int8_) {   // an int8 cache is only read by decode: prefill attends over the dense K / V it was given
             if (cu_k == nullptr) throw std::invalid_argument("prefill attention with block_tables requires cu_seqlens_k");
@@ -170,10 +198,12 @@ Tensor Attention::forward(const Tensor& query, const Tensor& key, const Tensor& 
 void Attention::decode(const Tensor& query, Tensor& output, DeviceAllocator& allocator, cudaStream_t stream) {
     const Context& ctx = get_context();
     if (key_weights_.defined()) {
-        if (is_int8_) throw std::invalid_argument("key weights are added up over a 16-bit or a 4-bit cache");
+        if (is_int8_ || is_blocks8_) throw std::invalid_argument("key weights are added up over a 16-bit or a 4-bit cache");
         const Tensor none;
         launch_decode_attention_paged_weights(query, k_cache_, v_cache_, is_int4_ ? k_scale_ : none, is_int4_ ? v_scale_ : none, ctx.context_lens, ctx.block_tables,
                                               num_kv_heads_, head_dim_, block_size_, scale_, key_weights_, weight_rows_, key_weights_, output, allocator, stream);
+    } else if (is_blocks8_) {
+        launch_decode_attention_paged_blocks8(query, k_cache_, v_cache_, k_scale_, v_scale_, ctx.context_lens, ctx.block_tables, scale_, output, allocator, is_e4m3_, stream);
     } else if (is_int8_) {
         launch_decode_attention_paged_int8(query, k_cache_, v_cache_, k_scale_, v_scale_, ctx.context_lens, ctx.block_tables,
                                            num_kv_heads_, head_dim_, block_size_, scale_, output, stream);

@@ -5,13 +5,16 @@
 #include "kernels/attention.h"
 #include "kernels/flash_attn.h"
 #include "kernels/kernel_types.h"
+#include "engine/step_metadata.h"
 #include "kernels/kvcache.h"
+#include "kernels/rotary.h"
 #include "kernels/split_qkv.h"
 
 #include "nvk.h"
 
 #include "../../csrc/decode_sizes.h"
 
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
@@ -240,6 +243,189 @@ void gather_kvcache_int4(const Tensor& k_cache, const Tensor& v_cache, const Ten
                                                 block_size, key.data(), value.data(), code(key.dtype()), stream));
 }
 
+// ---- 8-bit cache with block scales --------------------------------------------------------------------
+namespace {
+
+struct Blocks8 {   // caches and scales that agree
+    int64_t blocks;
+    int block_size, heads, head_dim, type;
+    Blocks8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, bool e4m3) : type(e4m3 ? NVK_E4M3 : NVK_I8) {
+        ensure_cuda_tensor("k_cache", k_cache);
+        ensure_cuda_tensor("v_cache", v_cache);
+        ensure_cuda_tensor("k_scale", k_scale);
+        ensure_cuda_tensor("v_scale", v_scale);
+        ensure_same_device("k_cache", k_cache, "v_cache", v_cache);
+        ensure_same_device("k_cache", k_cache, "k_scale", k_scale);
+        ensure_same_device("k_cache", k_cache, "v_scale", v_scale);
+        ensure_same_shape("k_cache", k_cache, "v_cache", v_cache);
+        if (k_cache.dtype() != ScalarType::kInt8 || v_cache.dtype() != ScalarType::kInt8) throw std::invalid_argument("8-bit caches must be byte (int8) tensors");
+        if (k_cache.dim() != 4) throw std::invalid_argument("k_cache must be [blocks, block_size, num_kv_heads, head_dim]");
+        if (k_scale.dtype() != ScalarType::kFloat32 || v_scale.dtype() != ScalarType::kFloat32) throw std::invalid_argument("k_scale and v_scale must be float32");
+        blocks = k_cache.sizes()[0];
+        block_size = static_cast<int>(k_cache.sizes()[1]);
+        heads = static_cast<int>(k_cache.sizes()[2]);
+        head_dim = static_cast<int>(k_cache.sizes()[3]);
+        if (static_cast<int64_t>(k_scale.numel()) != blocks * heads || k_scale.numel() != v_scale.numel())
+            throw std::invalid_argument("k_scale and v_scale must hold one value per cache block and KV head");
+    }
+};
+
+// Rows [rows, heads, head_dim], or [rows, heads * head_dim] that may be slices of wider ones; the elements from one to the next.
+int64_t packed_rows(const char* name, const Tensor& t, int heads, int head_dim) {
+    const std::string n(name);
+    if (!t.defined()) throw std::invalid_argument(n + " must be defined");
+    if (t.device().type != DeviceType::kCUDA) throw std::invalid_argument(n + " must live on CUDA");
+    const int64_t row = static_cast<int64_t>(heads) * head_dim;
+    if (t.dim() == 3 ? t.sizes()[1] != heads || t.sizes()[2] != head_dim || !t.is_contiguous() : t.dim() != 2 || t.sizes()[1] != row || t.strides()[1] != 1)
+        throw std::invalid_argument(n + " must be [rows, heads, head_dim], or rows of heads * head_dim elements");
+    return t.sizes()[0] > 1 && t.dim() == 2 ? t.strides()[0] : row;
+}
+
+}  // namespace
+
+void store_kvcache_blocks8(const Tensor& key, const Tensor& value, Tensor& k_cache, Tensor& v_cache, Tensor& k_scale,
+                           Tensor& v_scale, const Tensor& cu_seqlens_q, const Tensor& context_lens, const Tensor& block_tables, bool e4m3,
+                           cudaStream_t stream) {
+    const Blocks8 c(k_cache, v_cache, k_scale, v_scale, e4m3);
+    const int64_t key_stride = packed_rows("key", key, c.heads, c.head_dim), value_stride = packed_rows("value", value, c.heads, c.head_dim);
+    ensure_same_dtype("key", key, "value", value);
+    if (key.sizes()[0] != value.sizes()[0]) throw std::invalid_argument("key and value must have the same number of rows");
+    ensure_same_device("key", key, "value", value);
+    ensure_same_device("key", key, "k_cache", k_cache);
+    const IndexRef lens = index_data("context_lens", context_lens), tables = index_data("block_tables", block_tables);
+    const IndexRef starts = cu_seqlens_q.defined() ? index_data("cu_seqlens_q", cu_seqlens_q) : IndexRef{nullptr, NVK_I32};
+    ensure_same_device("key", key, "context_lens", context_lens);
+    ensure_same_device("key", key, "block_tables", block_tables);
+    if (cu_seqlens_q.defined()) ensure_same_device("key", key, "cu_seqlens_q", cu_seqlens_q);
+    const int64_t seqs = static_cast<int64_t>(context_lens.numel());
+    if (cu_seqlens_q.defined() ? static_cast<int64_t>(cu_seqlens_q.numel()) != seqs + 1 : key.sizes()[0] != seqs)
+        throw std::invalid_argument("cu_seqlens_q, or key, must have a sequence for every context length");
+    if (block_tables.dim() != 2) throw std::invalid_argument("block_tables must be [num_seqs, max_blocks]");
+    ensure_rows("block_tables", block_tables, seqs);
+    throw_on_nvk_status(nvk_store_kvcache_blocks8(key.data(), value.data(), key_stride, value_stride, k_cache.data(), v_cache.data(), k_scale.data_as<float>(),
+                                                  v_scale.data_as<float>(), c.type, starts.ptr, starts.dtype, lens.ptr, lens.dtype, tables.ptr, tables.dtype, seqs,
+                                                  key.sizes()[0], block_tables.sizes()[1], c.blocks, c.heads, c.head_dim, c.block_size, code(key.dtype()), stream));
+}
+
+void gather_kvcache_blocks8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale,
+                            const Tensor& cu_seqlens_k, const Tensor& block_tables, Tensor& key, Tensor& value, bool e4m3, cudaStream_t stream) {
+    const Blocks8 c(k_cache, v_cache, k_scale, v_scale, e4m3);
+    ensure_cuda_tensor("key", key);
+    ensure_cuda_tensor("value", value);
+    ensure_same_dtype("key", key, "value", value);
+    ensure_same_shape("key", key, "value", value);
+    const IndexRef starts = index_data("cu_seqlens_k", cu_seqlens_k), tables = index_data("block_tables", block_tables);
+    ensure_same_device("key", key, "k_cache", k_cache);
+    ensure_same_device("key", key, "value", value);
+    ensure_same_device("key", key, "cu_seqlens_k", cu_seqlens_k);
+    ensure_same_device("key", key, "block_tables", block_tables);
+    if (key.dim() != 3 || key.sizes()[1] != c.heads || key.sizes()[2] != c.head_dim) throw std::invalid_argument("key must be [total_k, num_kv_heads, head_dim]");
+    const int64_t seqs = static_cast<int64_t>(cu_seqlens_k.numel()) - 1;
+    if (block_tables.dim() != 2) throw std::invalid_argument("block_tables must be [num_seqs, max_blocks]");
+    ensure_rows("block_tables", block_tables, seqs);
+    throw_on_nvk_status(nvk_gather_kvcache_blocks8(k_cache.data(), v_cache.data(), k_scale.data_as<float>(), v_scale.data_as<float>(), c.type, starts.ptr,
+                                                   starts.dtype, tables.ptr, tables.dtype, seqs, key.sizes()[0], block_tables.sizes()[1], c.blocks, c.heads,
+                                                   c.head_dim, c.block_size, key.data(), value.data(), code(key.dtype()), stream));
+}
+
+// ---- rotary positions ---------------------------------------------------------------------------------
+void rotary_embedding(const Tensor& query, const Tensor& key, const Tensor& positions, const Tensor& inv_freq, int num_q_heads,
+                      int num_kv_heads, int head_dim, bool interleaved, float attention_factor, Tensor& query_out, Tensor& key_out,
+                      cudaStream_t stream) {
+    if (num_q_heads <= 0 || head_dim <= 0) throw std::invalid_argument("attention dimensions must be positive");
+    const int64_t q_stride = packed_rows("query", query, num_q_heads, head_dim), qo_stride = packed_rows("query_out", query_out, num_q_heads, head_dim);
+    const IndexRef pos = index_data("positions", positions);
+    ensure_cuda_tensor("inv_freq", inv_freq);
+    if (inv_freq.dtype() != ScalarType::kFloat32) throw std::invalid_argument("inv_freq must be float32");
+    const int64_t rows = query.sizes()[0];
+    auto alike = [&](const char* name, const Tensor& t) {
+        if (t.sizes()[0] != rows) throw std::invalid_argument(std::string(name) + " must have the rows of query");
+        ensure_same_dtype("query", query, name, t);
+        ensure_same_device("query", query, name, t);
+    };
+    alike("query_out", query_out);
+    if (key.defined() != key_out.defined()) throw std::invalid_argument("key and key_out go together");
+    int64_t k_stride = 0, ko_stride = 0;
+    if (key.defined()) {
+        k_stride = packed_rows("key", key, num_kv_heads, head_dim);
+        ko_stride = packed_rows("key_out", key_out, num_kv_heads, head_dim);
+        alike("key", key);
+        alike("key_out", key_out);
+    }
+    ensure_same_device("query", query, "positions", positions);
+    ensure_same_device("query", query, "inv_freq", inv_freq);
+    if (static_cast<int64_t>(positions.numel()) != rows) throw std::invalid_argument("positions must have an element for every row");
+    throw_on_nvk_status(nvk_rotary_embedding(query.data(), key.defined() ? key.data() : nullptr, pos.ptr, pos.dtype, inv_freq.data_as<float>(), attention_factor, rows,
+                                             num_q_heads, num_kv_heads, head_dim, static_cast<int>(2 * inv_freq.numel()), interleaved ? 1 : 0, q_stride, k_stride,
+                                             query_out.data(), key_out.defined() ? key_out.data() : nullptr, qo_stride, ko_stride, code(query.dtype()), stream));
+}
+
+RotaryFrequencies rotary_inv_freq(int rotary_dim, double base, RopeScaling scaling, double factor, double original_positions, double low_turns,
+                                  double high_turns) {
+    RotaryFrequencies f;
+    f.inv_freq.resize(static_cast<size_t>(rotary_dim > 1 ? rotary_dim / 2 : 1));
+    throw_on_nvk_status(nvk_rotary_inv_freq(f.inv_freq.data(), &f.attention_factor, rotary_dim, base, static_cast<int>(scaling), factor, original_positions, low_turns,
+                                            high_turns));
+    return f;
+}
+
+// ---- metadata of a step on the device -----------------------------------------------------------------
+namespace {
+
+// The tables of requests agree with one another; the width of their elements.
+int check_tables(const RequestTables& t) {
+    const IndexRef lens = index_data("lens", t.lens);
+    struct { const char* name; const Tensor& t; } others[] = {{"blocks", t.blocks}, {"free_blocks", t.free_blocks}, {"free_count", t.free_count}};
+    for (const auto& o : others) {
+        if (index_data(o.name, o.t).dtype != lens.dtype) throw std::invalid_argument(std::string(o.name) + " must have the dtype of the other index tensors");
+        ensure_same_device("lens", t.lens, o.name, o.t);
+    }
+    if (t.blocks.dim() != 2 || t.blocks.sizes()[0] != static_cast<int64_t>(t.lens.numel())) throw std::invalid_argument("blocks must have a row for every length");
+    if (t.free_count.numel() != 1) throw std::invalid_argument("free_count must have one element");
+    return lens.dtype;
+}
+const void* step_index(const char* name, const Tensor& x, const RequestTables& t, int dtype, int64_t elements) {
+    if (index_data(name, x).dtype != dtype) throw std::invalid_argument(std::string(name) + " must have the dtype of the other index tensors");
+    ensure_same_device("lens", t.lens, name, x);
+    if (elements >= 0 && static_cast<int64_t>(x.numel()) != elements) throw std::invalid_argument(std::string(name) + " has the wrong size");
+    return x.data();
+}
+void* step_output(const char* name, const Tensor& x, const RequestTables& t, int dtype, int64_t elements) {
+    return x.defined() ? const_cast<void*>(step_index(name, x, t, dtype, elements)) : nullptr;
+}
+
+}  // namespace
+
+void build_step(const Tensor& new_lens, const Tensor& rows, RequestTables& tables, DeviceStep& step, cudaStream_t stream) {
+    const int dtype = check_tables(tables);
+    const int64_t batch = new_lens.defined() ? static_cast<int64_t>(new_lens.numel()) : 0;
+    const void* n = step_index("new_lens", new_lens, tables, dtype, batch);
+    const void* r = rows.defined() ? step_index("rows", rows, tables, dtype, batch) : nullptr;
+    if (!step.block_tables.defined() || step.block_tables.dim() != 2) throw std::invalid_argument("block_tables must be [batch, max_blocks]");
+    ensure_rows("block_tables", step.block_tables, batch);
+    void* bt = step_output("block_tables", step.block_tables, tables, dtype, -1);
+    if (!step.context_lens.defined()) throw std::invalid_argument("context_lens must be defined");
+    void* ctx = step_output("context_lens", step.context_lens, tables, dtype, batch);
+    void *cu_q = step_output("cu_seqlens_q", step.cu_seqlens_q, tables, dtype, batch + 1), *cu_k = step_output("cu_seqlens_k", step.cu_seqlens_k, tables, dtype, batch + 1);
+    if (step.positions.defined() != step.slot_mapping.defined()) throw std::invalid_argument("positions and slot_mapping go together");
+    const int64_t tokens = step.positions.defined() ? static_cast<int64_t>(step.positions.numel()) : 0;
+    void *pos = step_output("positions", step.positions, tables, dtype, tokens), *slots = step_output("slot_mapping", step.slot_mapping, tables, dtype, tokens);
+    throw_on_nvk_status(nvk_step_metadata(n, r, tables.lens.data(), tables.blocks.data(), tables.free_blocks.data(), tables.free_count.data(), batch,
+                                          static_cast<int64_t>(tables.lens.numel()), tables.blocks.sizes()[1], static_cast<int64_t>(tables.free_blocks.numel()),
+                                          tables.num_cache_blocks, tables.block_size, bt, step.block_tables.sizes()[1], ctx, cu_q, cu_k, pos, slots, tokens,
+                                          tables.lens.data(), tables.free_count.data(), dtype, stream));
+}
+
+void release_blocks(const Tensor& rows, const Tensor& first_blocks, RequestTables& tables, cudaStream_t stream) {
+    const int dtype = check_tables(tables);
+    const int64_t batch = static_cast<int64_t>(rows.defined() ? rows.numel() : tables.lens.numel());
+    const void* r = rows.defined() ? step_index("rows", rows, tables, dtype, batch) : nullptr;
+    const void* f = first_blocks.defined() ? step_index("first_blocks", first_blocks, tables, dtype, batch) : nullptr;
+    throw_on_nvk_status(nvk_release_blocks(r, f, tables.lens.data(), tables.blocks.data(), tables.free_blocks.data(), tables.free_count.data(), batch,
+                                           static_cast<int64_t>(tables.lens.numel()), tables.blocks.sizes()[1], static_cast<int64_t>(tables.free_blocks.numel()),
+                                           tables.block_size, tables.lens.data(), tables.free_count.data(), dtype, stream));
+}
+
 void evict_kvcache(Tensor& k_cache, Tensor& v_cache, Tensor& k_params, Tensor& v_params, const Tensor& key_weights,
                    const Tensor& weight_rows, const Tensor& context_lens, const Tensor& block_tables, Tensor& new_key_weights,
                    const Tensor& new_block_tables, Tensor& new_context_lens, int num_kv_heads, int head_dim, int block_size,
@@ -452,6 +638,33 @@ void launch_decode_attention_paged_int4(const Tensor& query, const Tensor& k_cac
     throw_on_nvk_status(nvk_decode_attention_paged_int4(query.data(), k_cache.data(), v_cache.data(), k_params.data(), v_params.data(), s.lens.ptr, s.lens.dtype,
                                                         s.tables.ptr, s.tables.dtype, s.batch, s.max_blocks, s.blocks, s.heads, num_kv_heads, head_dim,
                                                         block_size, scale, output.data(), code(query.dtype()), scratch ? scratch->data() : nullptr, need, stream));
+}
+
+void launch_decode_attention_paged_blocks8(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
+                                           const Tensor& k_scale, const Tensor& v_scale, const Tensor& context_lens,
+                                           const Tensor& block_tables, float scale, Tensor& output, DeviceAllocator& allocator, bool e4m3,
+                                           cudaStream_t stream) {
+    const Blocks8 c(k_cache, v_cache, k_scale, v_scale, e4m3);
+    check_qo(query, output);
+    const IndexRef lens = index_data("context_lens", context_lens), tables = index_data("block_tables", block_tables);
+    const int64_t batch = query.sizes()[0];
+    const int heads = static_cast<int>(query.sizes()[1]);
+    if (query.sizes()[2] != c.head_dim) throw std::invalid_argument("query head_dim does not match that of the cache");
+    if (heads % c.heads != 0 || heads / c.heads > 8) throw std::invalid_argument("num_heads must be divisible by num_kv_heads, and at most 8 times as many");
+    if (!std::isfinite(scale)) throw std::invalid_argument("scale must be finite");
+    if (block_tables.dim() != 2) throw std::invalid_argument("block_tables must be [batch, max_blocks]");
+    ensure_rows("block_tables", block_tables, batch);
+    if (static_cast<int64_t>(context_lens.numel()) != batch) throw std::invalid_argument("context_lens must hold one entry per sequence");
+    ensure_same_device("query", query, "k_cache", k_cache);
+    ensure_same_device("query", query, "context_lens", context_lens);
+    ensure_same_device("query", query, "block_tables", block_tables);
+    const int64_t max_blocks = block_tables.sizes()[1];
+    // (more than this call needs: with room for them, contexts go into shorter parts)
+    const size_t room = nvk_decode_attention_workspace_bytes(batch, heads, c.heads, c.head_dim, max_blocks, c.block_size);
+    Memory::Ptr scratch = room > 0 ? allocator.allocate_on(room, query.device(), stream) : nullptr;
+    throw_on_nvk_status(nvk_decode_attention_paged_blocks8(query.data(), k_cache.data(), v_cache.data(), k_scale.data_as<float>(), v_scale.data_as<float>(), c.type,
+                                                           lens.ptr, lens.dtype, tables.ptr, tables.dtype, batch, max_blocks, c.blocks, heads, c.heads, c.head_dim,
+                                                           c.block_size, scale, output.data(), code(query.dtype()), scratch ? scratch->data() : nullptr, room, stream));
 }
 
 void launch_decode_attention_paged_weights(const Tensor& query, const Tensor& k_cache, const Tensor& v_cache,
