@@ -360,6 +360,15 @@ int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
 // the other caches).  us, as above: 64 pairs of 8192 keys 18.7 / 18.5 / 19.1, 19.9 / 21.3 / 30.6 -> 16.0 / 15.9 / 16.7, 17.5 / 23.7 / 29.7; 256 of 2048 12.1 / 14.7 / 16.7, 16.9 /
 // 21.1 / 31.9 -> 10.8 / 12.9 / 14.3, 16.5 / 22.3 / 28.3; 256 of 4096 13.9 / 16.2 / 20.9, 33.5 / 41.0 / 53.4 -> 12.2 / 14.7 / 19.1, 29.6 / 40.8 / 49.4; 800 of 8192 40.2 / 57.5 / 109.4, 154.0 /
 // 209.6 / 263.5 -> 36.7 / 55.4 / 104.9, 148.6 / 204.7 / 260.9; but 2048 of 8192 65.8 / 116.5 / 251.6, 364.6 / 510.0 / 655.4 -> 68.3 / 119.6 / 254.5, 366.2 / 502.0 / 686.5.
+// Tables of 1024 to 2048 keys beyond the clusters of four: whole contexts by blocks of eight warps, one to an SM, with more pairs than SMs the longest first; between one and one and a half
+// pairs to an SM, where a second wave of those would be nearly empty, the halves of a table row, which 8-bit caches otherwise have up to 1536 keys.  us with inputs beyond L2: 120 pairs of 2048
+// keys 9.5 / 12.5 / 14.2, 14.8 / 15.6 / 20.5 -> 11.8 / 12.9 / 13.5, 13.5 / 13.8 / 14.2; 256 12.0 / 15.6 / 17.8, 21.0 / 27.9 / 30.2 -> 13.2 / 14.2 / 14.8, 19.2 / 24.3 / 29.6; 256 of
+// 1024 10.6 / 11.9 / 14.4, 15.2 / 19.1 / 22.2 -> 8.7 / 9.2 / 13.2, 14.6 / 17.1 / 19.4; 160 of 2048 10.2 / 13.1 / 14.6, 15.6 / 21.6 / 24.3 -> 10.0 / 13.2 / 15.9, 16.0 / 17.0 / 18.2 (by eight
+// warps 12.5 / 13.6 / 14.2, 14.4 / 20.8 / 27.9); but 384 of 2048 by four warps 18.8 / 21.7 / 28.8, 27.6 / 31.9 / 37.0, by eight 14.0 / 16.7 / 23.1, 28.7 / 35.4 / 43.3.
+bool halves_of_block_scales(int64_t pairs, int64_t max_tokens) { return pairs > kSmCount && 2 * pairs <= 3 * kSmCount && max_tokens >= 1024 && max_tokens <= 2048; }
+bool eight_warps_of_block_scales(int64_t pairs, int64_t max_tokens) {
+    return !halves_of_block_scales(pairs, max_tokens) && max_tokens >= 1024 && max_tokens <= 2048 && pairs <= 320;
+}
 int chunk_of_block_scales(int64_t pairs, int64_t max_tokens, int chunk, int block_size) {
     if (chunk < 1024 || max_tokens <= chunk || pairs > 8 * kSmCount) return chunk;
     const int finer = pairs <= 4 * kSmCount ? 768 : 1024;
@@ -370,12 +379,17 @@ Splits choose_splits(int64_t batch, int num_heads, int num_kv_heads, int64_t max
     Splits s{cluster_size(batch, num_kv_heads, max_blocks, block_size, groups, have_workspace), 0, 0};
     if (s.cluster > 0) { s.count = s.cluster; return s; }
     const int64_t max_tokens = max_blocks * block_size;
+    if (block_scale_room > 0 && eight_warps_of_block_scales(batch * num_kv_heads, max_tokens)) {
+        s.chunk = static_cast<int>(max_tokens);
+        s.count = 1;
+        return s;
+    }
     if (const int chunk = four_bits ? chunk_tokens4(batch * num_kv_heads, max_tokens) : 0; chunk > 0) {
         s.chunk = static_cast<int>((chunk + block_size - 1) / block_size) * block_size;
         s.count = static_cast<int>((max_tokens + s.chunk - 1) / s.chunk);
         return s;
     }
-    if (max_blocks > 1 && halves(batch * num_kv_heads, max_tokens, groups)) {
+    if (max_blocks > 1 && (halves(batch * num_kv_heads, max_tokens, groups) || (block_scale_room > 0 && halves_of_block_scales(batch * num_kv_heads, max_tokens)))) {
         s.chunk = static_cast<int>((max_blocks + 1) / 2 * block_size);
         s.cluster = s.count = 2;
         return s;
@@ -422,10 +436,12 @@ int decode_plan(const DecodeArgs& a, int groups, dec::DecodeParams* out, int* cl
     p.by_kv_heads = FastDiv(static_cast<uint32_t>(a.num_kv_heads));
     p.chunk_tokens = s.chunk;
     p.num_splits = s.count;
+    const int64_t pairs = a.batch * a.num_kv_heads, max_tokens = a.max_blocks * a.block_size;
+    const bool eight = four_bits ? eight_warps(pairs, max_tokens) : block_scales && eight_warps_of_block_scales(pairs, max_tokens);
     // More than one wave of blocks: the long contexts first, so that the last blocks to start are short.  Contexts in a few chunks as well:
     // 38 / 44 sequences of 500 / 2000 to 4096 keys, 8 KV heads, 65.4 / 90.1 -> 58.7 / 85.9 us a call (whole 59.8 / 84.7).
     p.longest_first = s.chunk > 0 && (s.count == 1 || a.max_blocks * a.block_size <= 4096 || (four_bits && s.chunk >= 4096)) &&
-                      a.batch * a.num_kv_heads > static_cast<int64_t>(kSmCount) * (four_bits && eight_warps(a.batch * a.num_kv_heads, a.max_blocks * a.block_size) ? 1 : groups) &&
+                      a.batch * a.num_kv_heads > static_cast<int64_t>(kSmCount) * (eight ? 1 : groups) &&
                       a.batch <= kMaxSorted && a.max_blocks * a.block_size >= kMinSortedTokens;
     // Contexts shorter than the table leave chunks without keys, whose blocks exit at once.  With sequence after sequence they lie between
     // the blocks with work, and these pile up on the SMs where the empty ones were quickest gone; chunk after chunk the ones with
@@ -482,7 +498,7 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     if (device >= 0 && device < 64 && !attr_done[device]) {
         cudaError_t e = cudaFuncSetAttribute(decode_split_kernel<F, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(decode_cluster_kernel<C, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-        if constexpr (F::kFourBits) {
+        if constexpr (F::kFourBits || InClusters<F>::kBlockScales) {
             if (e == cudaSuccess)
                 e = cudaFuncSetAttribute(decode_split_kernel<typename F::Eight, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, sizeof(GroupSmem<typename F::Eight>));
         }
@@ -524,8 +540,8 @@ int launch_typed(const DecodeArgs& a, const void* k_scale, const void* v_scale, 
     const dim3 grid = p.chunk_major ? dim3(a.num_kv_heads, batch, splits) : dim3(a.num_kv_heads, splits, batch);
     cudaError_t e = cudaSuccess;
     bool eight = false;
-    if constexpr (F::kFourBits) {
-        eight = splits == 1 && eight_warps(a.batch * a.num_kv_heads, a.max_blocks * a.block_size);
+    if constexpr (F::kFourBits || InClusters<F>::kBlockScales) {
+        eight = splits == 1 && (F::kFourBits ? eight_warps : eight_warps_of_block_scales)(a.batch * a.num_kv_heads, a.max_blocks * a.block_size);
         if (eight) e = launch_pdl(decode_split_kernel<typename F::Eight, T>, grid, dim3(F::Eight::kWarps * 32), sizeof(GroupSmem<typename F::Eight>), a.stream, p);
     }
     if (!eight) e = launch_pdl(decode_split_kernel<F, T>, grid, dim3(kGroupThreads), kSmem, a.stream, p);

@@ -769,17 +769,19 @@ __device__ __forceinline__ void ldmatrix_b8_trans(uint32_t (&w)[4], uint32_t add
     asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];\n" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
 }
 // CLUSTERS: for blocks that share a context in a cluster, and may have a few keys each (launches in chunks were 0.5 to 1.5 % slower with that code).
-template <typename T, bool FP8, bool CLUSTERS = false>
+template <typename T, bool FP8, bool CLUSTERS = false, int WARPS = kGroupWarps>
 struct CacheBlocks8 {
     using InClusters = CacheBlocks8<T, FP8, true>;
+    using Eight = CacheBlocks8<T, FP8, false, 8>;             // eight warps to a block
     static constexpr bool kScores = false;
     static constexpr bool kFourBits = false;
     static constexpr bool kOwnRun = true;
-    static constexpr int kWarps = kGroupWarps;
-    static constexpr int kGroups = 3, kSplitBlocks = kGroups;
+    static constexpr int kWarps = WARPS;
+    static constexpr int kGroups = 3;                         // resident per SM in clusters and, of four warps, in chunks
+    static constexpr int kSplitBlocks = WARPS == 8 ? 1 : kGroups;
     static constexpr int kRowBytes = kHeadDim;
     static constexpr int kKeys = 32;                          // of a stage
-    static constexpr int kKeysAhead = 32 * kWarps * kKeys + 16;   // two windows of 16 tiles and a half: how far `run` counts beyond the last key
+    static constexpr int kKeysAhead = 32 * 8 * kKeys + 16;   // two windows of 16 tiles and a half: how far `run` counts beyond the last key
     static constexpr int kTileBytes = kKeys * kRowBytes;
     static constexpr int kStageBytes = 2 * kTileBytes + 128;  // K, V, the scales (K, K, V, V) of both halves; (whole 128-byte lines: pieces are found by XOR)
     static constexpr int kStages = 2;

@@ -67,10 +67,10 @@ class Cache:
     def rows(self, table, n):
         """Values of positions 0 .. n - 1 of a sequence; zeros where there is no block."""
         out = np.zeros((n, *self.data.shape[2:]))
-        for i in range(n):
+        for i in range(0, n, self.bs):
             if i // self.bs < len(table) and 0 <= table[i // self.bs] < len(self.data):
                 block = int(table[i // self.bs])
-                out[i] = self.data[block, i % self.bs] * self.scale[block][:, None]
+                out[i:i + self.bs] = self.data[block, :min(self.bs, n - i)] * self.scale[block][:, None]
         return out
 
 

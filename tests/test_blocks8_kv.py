@@ -370,6 +370,28 @@ def test_decode(kind, dtype, bs, hq, hkv, lens, width, index):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [("int8", "bfloat16"), ("e4m3", "float16")])
+@pytest.mark.parametrize("hq,hkv,batch,width,long", [
+    (8, 8, 15, 16, [1024, 900]),          # 120 pairs, 1024-key tables: whole contexts, eight warps
+    (16, 8, 30, 32, [2048, 1]),           # 240 pairs, 2048 keys: the same, the longest first
+    (16, 8, 20, 32, [2048, 1025]),        # 160 pairs: halves of a table row
+    (2, 1, 200, 64, [4096, 769, 768]),    # chunks of 768
+    (8, 8, 90, 128, [3000, 8192]),        # 720 pairs: of 1024, where the workspace has room for them
+    (8, 1, 8, 64, [4096, 4095, 33])])     # clusters of eight
+def test_decode_in_all_ways_of_sharing_out(kind, dtype, hq, hkv, batch, width, long):
+    """Contexts of which a few fill their tables and the others end in their first blocks, none among them."""
+    rng = np.random.default_rng(hq * batch)
+    bs = 64
+    lens = (long + [0, 1, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129] + [int(x) for x in rng.integers(1, 200, batch)])[:batch]
+    rng.shuffle(lens)
+    c, tables = _filled(rng, kind, dtype, bs, hkv, lens, width)
+    q, here = _typed(rng.standard_normal((batch, hq, D)) * 2.0, dtype)
+    got = _check_decode(c, q, here, lens, tables, dtype)
+    assert np.array_equal(got, _decode(c, q, lens, tables))
+    _check_decode(c, q, here, lens, tables, dtype, workspace=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_decode_over_scales_far_apart(kind, dtype):

@@ -199,13 +199,57 @@ def test_blocks_outside_the_cache_give_no_slots():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch,width,tokens", [(8192, 7, 20000), (64, 2048, 70000)])
-def test_the_largest_batch_and_wide_tables(batch, width, tokens):
+@pytest.mark.parametrize("batch,width,tokens", [(8192, 7, 20000), (64, 2048, 70000), (1100, 128, 300000), (8192, 64, 9000)])
+@pytest.mark.parametrize("dtype,apart", [("int64", False), ("int32", True), ("int32", False)])
+def test_the_largest_batch_and_wide_tables(batch, width, tokens, dtype, apart):
+    """Steps of many blocks, twice in a row (what is updated in place follows in a kernel of its own)."""
     rng = np.random.default_rng(7)
-    t = Tables(rng, batch + 1, width, 4, batch * 3, dtype="int64")
-    new = rng.integers(0, 4, batch) if batch > 100 else rng.integers(0, 2000, batch)
-    t.step(new.tolist(), (rng.permutation(batch + 1)[:batch]).tolist(), width, tokens)
-    t.release(rng.permutation(batch + 1)[:batch].tolist(), None)
+    t = Tables(rng, batch + 1, width, 4, batch * 2, dtype=dtype)
+    for _ in range(2):
+        new = rng.integers(0, 4, batch) if batch > 100 else rng.integers(0, 2000, batch)
+        t.step(new.tolist(), (rng.permutation(batch + 1)[:batch]).tolist(), width, tokens, apart)
+    t.release(rng.permutation(batch + 1)[:batch].tolist(), None, apart)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,width", [(5, 8), (300, 16), (2000, 96)])
+def test_tables_and_tokens_at_odd_addresses(batch, width):
+    """Tables, positions and slots that begin off a 16-byte boundary; counts of tokens that are no multiple of four."""
+    import torch
+    rng = np.random.default_rng(batch)
+    t = Tables(rng, batch, width, 16, batch * 2, dtype="int32")
+    odd = lambda *shape: torch.full((1 + int(np.prod(shape)),), -99, dtype=torch.int32, device="cuda")[1:].view(shape)
+    new = rng.integers(0, 40, batch).tolist()
+    tokens = sum(new) + 1
+    held = odd(batch, width)
+    held.copy_(t.held)
+    out = [odd(batch, width), odd(batch), odd(batch + 1), odd(batch + 1), odd(tokens), odd(tokens)]
+    nvk().step_metadata(t.up(new), None, t.lens, held, t.free, t.count, 16, t.pool, *out)
+    want = t.ref.step(new, None, width, tokens, t.pool)
+    assert [o.tolist() for o in out] == list(want)
+    assert held.tolist() == t.ref.held and t.lens.tolist() == t.ref.lens and t.count.tolist() == [t.ref.count]
+
+
+@pytest.mark.gpu
+def test_two_steps_at_once_on_two_streams():
+    """Two sets of tables, one step each, at the same time: nothing is shared between calls."""
+    import torch
+    rng = np.random.default_rng(12)
+    sets = [Tables(rng, 200, 40, 16, 300, dtype="int32") for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in sets]
+    new = [rng.integers(0, 30, 200).tolist() for _ in sets]
+    outs = []
+    for t, n in zip(sets, new):
+        full = lambda *shape: torch.full(shape, -99, dtype=torch.int32, device="cuda")
+        outs.append((t.up(n), [full(200, 40), full(200), full(201), full(201), full(sum(n)), full(sum(n))]))
+    torch.cuda.synchronize()
+    for t, st, (n, out) in zip(sets, streams, outs):
+        with torch.cuda.stream(st):
+            nvk().step_metadata(n, None, t.lens, t.held, t.free, t.count, 16, t.pool, *out)
+    torch.cuda.synchronize()
+    for t, n, (_, out) in zip(sets, new, outs):
+        assert [o.tolist() for o in out] == list(t.ref.step(n, None, 40, sum(n), t.pool))
+        t.same()
 
 
 @pytest.mark.gpu
