@@ -269,7 +269,8 @@ int nvk_decode_attention_paged_blocks8(const void* query, const void* k_cache, c
  * free ones, request after request, and the row's length becomes 0.  (first_blocks: a cached prefix that others share stays with its owner.)  Ids that
  * free_blocks has no room for are dropped.  Rows outside the table are skipped; no two requests of a call share a row.
  *
- * At most 8192 requests to a call (a step: at least one); block_size >= 1; new_request_lens and new_free_count are the same memory as their old ones or do not overlap with them.
+ * At most 8192 requests to a call (a step: at least one); block_size >= 1.  new_request_lens and new_free_count may be the same memory as their old ones; nothing else that is
+ * written may overlap with another tensor of the call (NVK_ERR_INVALID_ARGUMENT).
  */
 int nvk_step_metadata(const void* new_lens, const void* request_rows, const void* request_lens, void* request_blocks, const void* free_blocks,
                       const void* free_count, int64_t batch, int64_t num_request_rows, int64_t request_max_blocks, int64_t num_free_blocks,

@@ -4,6 +4,7 @@
 #include "nvk_internal.cuh"
 
 #include <cmath>
+#include <initializer_list>
 #include <string>
 
 namespace nvk {
@@ -64,12 +65,27 @@ int check_blocks8(const char* what, int dtype, int cache_dtype, int num_kv_heads
 }
 // Neither the same nor apart.
 bool partly(const void* a, const void* b, int64_t bytes) { return a != b && overlap(a, bytes, b, bytes); }
+// Memory that a call writes, or only reads.
+struct Range { const void* at; int64_t bytes; };
+// Whether something that is written overlaps with anything else.
+bool written_twice(std::initializer_list<Range> written, std::initializer_list<Range> read) {
+    for (const Range* a = written.begin(); a != written.end(); ++a) {
+        if (a->at == nullptr || a->bytes <= 0) continue;
+        auto hits = [&](const Range& b) { return b.at != nullptr && b.bytes > 0 && overlap(a->at, a->bytes, b.at, b.bytes); };
+        for (const Range* b = a + 1; b != written.end(); ++b)
+            if (hits(*b)) return true;
+        for (const Range& b : read)
+            if (hits(b)) return true;
+    }
+    return false;
+}
 // What the calls over the tables of requests have in common.
 int check_requests(const char* what, const void* lens, const void* blocks, const void* free_blocks, const void* count, const void* new_lens, const void* new_count,
                    int64_t batch, int64_t rows, int64_t row_blocks, int64_t num_free, int block_size, const void* request_rows, int index_dtype) {
     if (!lens || !blocks || !free_blocks || !count || !new_lens || !new_count) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: lengths, blocks and counts must be defined", what);
     if (!is_index_dtype(index_dtype)) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: index tensors must be int32 or int64", what);
     if (batch < 0 || rows <= 0 || row_blocks <= 0 || num_free <= 0 || block_size <= 0) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: sizes must be positive", what);
+    if (rows > (1LL << 40) / row_blocks || num_free > (1LL << 40)) return fail(NVK_ERR_UNSUPPORTED, "%s: too many requests or blocks", what);
     if (!request_rows && rows < batch) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: without request_rows there has to be a row for every request", what);
     const int64_t wide = index_bytes(index_dtype);
     for (const void* p : {lens, blocks, free_blocks, count, new_lens, new_count, request_rows})
@@ -427,6 +443,16 @@ int nvk_step_metadata(const void* new_lens, const void* request_rows, const void
         if (!aligned_to(p, static_cast<size_t>(index_bytes(index_dtype)))) return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: misaligned tensor");
     if (index_dtype == NVK_I32 && num_cache_blocks > ((1LL << 31) - 1) / block_size)
         return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: slots of that many blocks need int64");
+    if (batch > (1LL << 40) / max_blocks || num_tokens > (1LL << 40) || num_cache_blocks > (1LL << 40)) return fail(NVK_ERR_UNSUPPORTED, "step_metadata: too many requests or table entries");
+    {
+        const int64_t w = index_bytes(index_dtype);
+        const Range lens{request_lens == new_request_lens ? nullptr : request_lens, num_request_rows * w}, count{free_count == new_free_count ? nullptr : free_count, w};
+        if (written_twice({{request_blocks, num_request_rows * request_max_blocks * w}, {block_tables, batch * max_blocks * w}, {context_lens, batch * w},
+                           {cu_seqlens_q, (batch + 1) * w}, {cu_seqlens_k, (batch + 1) * w}, {positions, num_tokens * w}, {slot_mapping, num_tokens * w},
+                           {new_request_lens, num_request_rows * w}, {new_free_count, w}},
+                          {{new_lens, batch * w}, {request_rows, batch * w}, {free_blocks, num_free_blocks * w}, lens, count}))
+            return fail(NVK_ERR_INVALID_ARGUMENT, "step_metadata: an output overlaps with another tensor (lengths and count may be updated in place)");
+    }
     StepArgs a{};
     auto index = [&](const void* p) { return index_array(p, index_dtype); };
     a.new_lens = index(new_lens); a.rows = index(request_rows); a.lens = index(request_lens); a.free_count = index(free_count);
@@ -447,6 +473,13 @@ int nvk_release_blocks(const void* request_rows, const void* first_blocks, const
                                       num_request_rows, request_max_blocks, num_free_blocks, block_size, request_rows, index_dtype); rc != NVK_OK)
         return rc;
     if (!aligned_to(first_blocks, static_cast<size_t>(index_bytes(index_dtype)))) return fail(NVK_ERR_INVALID_ARGUMENT, "release_blocks: misaligned tensor");
+    {
+        const int64_t w = index_bytes(index_dtype);
+        const Range lens{request_lens == new_request_lens ? nullptr : request_lens, num_request_rows * w}, count{free_count == new_free_count ? nullptr : free_count, w};
+        if (written_twice({{free_blocks, num_free_blocks * w}, {new_request_lens, num_request_rows * w}, {new_free_count, w}},
+                          {{request_rows, batch * w}, {first_blocks, batch * w}, {request_blocks, num_request_rows * request_max_blocks * w}, lens, count}))
+            return fail(NVK_ERR_INVALID_ARGUMENT, "release_blocks: an output overlaps with another tensor (lengths and count may be updated in place)");
+    }
     StepArgs a{};
     auto index = [&](const void* p) { return index_array(p, index_dtype); };
     a.rows = index(request_rows); a.first_blocks = index(first_blocks); a.lens = index(request_lens); a.free_count = index(free_count);

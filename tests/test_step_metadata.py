@@ -30,19 +30,21 @@ def test_by_hand():
 
 
 L, I = ctypes.c_int64, ctypes.c_int
-P, Q, ODD = ctypes.c_void_p(4096), ctypes.c_void_p(8192), ctypes.c_void_p(4098)
+P, ODD = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 2)
+AT = [ctypes.c_void_p(i << 40) for i in range(1, 16)]       # (nothing is read there)
+LENS, COUNT, BLOCKS, FREE, NEW, TABLES = AT[0], AT[1], AT[2], AT[3], AT[4], AT[5]
 
 
 def _step_args(**change):
-    a = dict(new=P, rows=None, lens=P, blocks=P, free=P, count=P, batch=L(2), num_rows=L(4), row_blocks=L(8), num_free=L(16), cache=L(64), bs=I(16), tables=P,
-             width=L(8), ctx=P, cu_q=P, cu_k=P, pos=P, slots=P, tokens=L(8), new_lens=P, new_count=P, dtype=I(3), stream=None)
+    a = dict(new=NEW, rows=None, lens=LENS, blocks=BLOCKS, free=FREE, count=COUNT, batch=L(2), num_rows=L(4), row_blocks=L(8), num_free=L(16), cache=L(64), bs=I(16),
+             tables=TABLES, width=L(8), ctx=AT[6], cu_q=AT[7], cu_k=AT[8], pos=AT[9], slots=AT[10], tokens=L(8), new_lens=LENS, new_count=COUNT, dtype=I(3), stream=None)
     a.update(change)
     return a.values()
 
 
 def _release_args(**change):
-    a = dict(rows=P, first=None, lens=P, blocks=P, free=P, count=P, batch=L(2), num_rows=L(4), row_blocks=L(8), num_free=L(16), bs=I(16), new_lens=P,
-             new_count=P, dtype=I(3), stream=None)
+    a = dict(rows=P, first=None, lens=LENS, blocks=BLOCKS, free=FREE, count=COUNT, batch=L(2), num_rows=L(4), row_blocks=L(8), num_free=L(16), bs=I(16), new_lens=LENS,
+             new_count=COUNT, dtype=I(3), stream=None)
     a.update(change)
     return a.values()
 
@@ -56,7 +58,10 @@ def _call(lib, name, *args):
     (dict(new=None), 1, "defined"), (dict(lens=None), 1, "defined"), (dict(tables=None), 1, "defined"), (dict(new_count=None), 1, "defined"),
     (dict(pos=None), 1, "defined"), (dict(dtype=I(1)), 1, "int32 or int64"), (dict(batch=L(-1)), 1, "positive"), (dict(bs=I(0)), 1, "positive"),
     (dict(width=L(0)), 1, "positive"), (dict(tokens=L(-1)), 1, "positive"), (dict(batch=L(5)), 1, "row for every request"), (dict(new=ODD), 1, "misaligned"),
-    (dict(lens=ODD), 1, "misaligned"), (dict(dtype=I(4), new_lens=ctypes.c_void_p(4104)), 1, "overlap"), (dict(new_lens=ctypes.c_void_p(4104)), 1, "overlap"),
+    (dict(lens=ODD), 1, "misaligned"), (dict(dtype=I(4), new_lens=ctypes.c_void_p(LENS.value + 8)), 1, "overlap"), (dict(new_lens=ctypes.c_void_p(LENS.value + 4)), 1, "overlap"),
+    (dict(ctx=LENS), 1, "overlaps"), (dict(ctx=NEW), 1, "overlaps"), (dict(tables=BLOCKS), 1, "overlaps"), (dict(pos=AT[10]), 1, "overlaps"), (dict(rows=P, cu_q=P), 1, "overlaps"),
+    (dict(new_count=FREE), 1, "overlaps"), (dict(new_lens=COUNT), 1, "overlaps"), (dict(slots=FREE), 1, "overlaps"), (dict(width=L(1 << 45)), 3, "too many"),
+    (dict(row_blocks=L(1 << 45)), 3, "too many"), (dict(tokens=L(1 << 45)), 3, "too many"),
     (dict(cache=L(1 << 28)), 1, "int64"), (dict(rows=P, batch=L(8193)), 3, "at most 8192"), (dict(rows=P, batch=L(8192), width=L(1 << 20)), 3, "too many"),
     (dict(batch=L(0)), 1, "positive")])
 def test_step_refuses(built, change, code, word):
@@ -66,7 +71,8 @@ def test_step_refuses(built, change, code, word):
 
 @pytest.mark.parametrize("change,code,word", [
     (dict(lens=None), 1, "defined"), (dict(free=None), 1, "defined"), (dict(dtype=I(0)), 1, "int32 or int64"), (dict(num_rows=L(0)), 1, "positive"),
-    (dict(rows=None, batch=L(5)), 1, "row for every request"), (dict(first=ODD), 1, "misaligned"), (dict(new_lens=ctypes.c_void_p(4100)), 1, "overlap"),
+    (dict(rows=None, batch=L(5)), 1, "row for every request"), (dict(first=ODD), 1, "misaligned"), (dict(new_lens=ctypes.c_void_p(LENS.value + 4)), 1, "overlap"),
+    (dict(free=BLOCKS), 1, "overlaps"), (dict(rows=P, free=P), 1, "overlaps"), (dict(new_count=FREE), 1, "overlaps"), (dict(row_blocks=L(1 << 45)), 3, "too many"),
     (dict(rows=P, batch=L(9000)), 3, "at most 8192"), (dict(batch=L(-1)), 1, "positive")])
 def test_release_refuses(built, change, code, word):
     rc, said = _call(built, "nvk_release_blocks", *_release_args(**change))
@@ -199,7 +205,7 @@ def test_blocks_outside_the_cache_give_no_slots():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("batch,width,tokens", [(8192, 7, 20000), (64, 2048, 70000), (1100, 128, 300000), (8192, 64, 9000)])
+@pytest.mark.parametrize("batch,width,tokens", [(8192, 7, 20000), (64, 2048, 70000), (1100, 128, 300000), (8192, 64, 9000), (8192, 2, 5000)])
 @pytest.mark.parametrize("dtype,apart", [("int64", False), ("int32", True), ("int32", False)])
 def test_the_largest_batch_and_wide_tables(batch, width, tokens, dtype, apart):
     """Steps of many blocks, twice in a row (what is updated in place follows in a kernel of its own)."""
