@@ -318,9 +318,11 @@ struct Blocks8 {   // caches and scales that agree
     }
     void sizes(int64_t block_size, int64_t hkv, int64_t d) {
         if (block_size <= 0 || hkv <= 0 || d <= 0) raise(PyExc_ValueError, "%s", "block_size, num_kv_heads and head_dim must be positive");
-        const int64_t per = block_size * hkv * d;
-        if (kc.numel() % per != 0 || kc.numel() != vc.numel()) raise(PyExc_ValueError, "%s", "k_cache does not contain an integer number of cache blocks");
-        blocks = kc.numel() / per;
+        const int64_t n = kc.numel();
+        const bool fit = block_size <= n && hkv <= n / block_size && d <= n / block_size / hkv;   // (and so their product)
+        const int64_t per = fit ? block_size * hkv * d : 1;
+        if (!fit || n % per != 0 || n != vc.numel()) raise(PyExc_ValueError, "%s", "k_cache does not contain an integer number of cache blocks");
+        blocks = n / per;
         if (ks.numel() != blocks * hkv || vs.numel() != blocks * hkv)
             raise(PyExc_ValueError, "%s", "k_scale and v_scale must have an element for every cache block and KV head");
     }
@@ -478,6 +480,7 @@ long rotary_embedding(PyObject* const* a) {
     if (k != nullptr && (k->size(0) != q.size(0) || k->size(2) != q.size(2) || k->scalar_type() != q.scalar_type()))
         raise(PyExc_ValueError, "%s", "key must have the rows, the head_dim and the dtype of query");
     if (pos.numel() != q.size(0)) raise(PyExc_ValueError, "%s", "positions must have an element for every row");
+    if (2 * f.numel() > q.size(2)) raise(PyExc_ValueError, "%s", "inv_freq must have an element for every pair, at most head_dim / 2");
     const int pairs = PyObject_IsTrue(a[4]);
     if (pairs < 0) throw Raised{};
     if (q.size(0) == 0) return 0;

@@ -503,6 +503,7 @@ int nvk_rotary_embedding(const void* query, const void* key, const void* positio
     if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
         return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: rotary_dim must be even, positive and at most head_dim");
     if (head_dim > 1024) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: head_dim must be at most 1024 (got %d)", head_dim);
+    if (num_q_heads > (1 << 19) || (key && num_kv_heads > (1 << 19))) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: too many heads");
     const int64_t size = static_cast<int64_t>(dtype_size(dtype));
     auto check = [&](const void* in, int64_t in_stride, const void* out, int64_t out_stride, int heads) -> int {
         const int64_t row = static_cast<int64_t>(heads) * head_dim;

@@ -168,7 +168,6 @@ template <typename T, int V> int launch_width(const RotaryParams& in, bool pairs
     p.by_items = FastDiv(static_cast<uint32_t>(p.items));
     p.by_heads = FastDiv(static_cast<uint32_t>(heads));
     p.by_pairs = FastDiv(static_cast<uint32_t>(p.rot / 2));
-    if (static_cast<int64_t>(heads) * p.items > (1 << 28)) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: too many heads");
     // As many rows to a block as its threads have under way at once, once there are blocks enough.
     const int row_items = heads * p.items;
     p.block_rows = 1;

@@ -260,6 +260,7 @@ struct Blocks8 {   // caches and scales that agree
         ensure_same_shape("k_cache", k_cache, "v_cache", v_cache);
         if (k_cache.dtype() != ScalarType::kInt8 || v_cache.dtype() != ScalarType::kInt8) throw std::invalid_argument("8-bit caches must be byte (int8) tensors");
         if (k_cache.dim() != 4) throw std::invalid_argument("k_cache must be [blocks, block_size, num_kv_heads, head_dim]");
+        if (k_cache.numel() == 0) throw std::invalid_argument("k_cache must contain at least one cache block");
         if (k_scale.dtype() != ScalarType::kFloat32 || v_scale.dtype() != ScalarType::kFloat32) throw std::invalid_argument("k_scale and v_scale must be float32");
         blocks = k_cache.sizes()[0];
         block_size = static_cast<int>(k_cache.sizes()[1]);
@@ -355,6 +356,7 @@ void rotary_embedding(const Tensor& query, const Tensor& key, const Tensor& posi
     ensure_same_device("query", query, "positions", positions);
     ensure_same_device("query", query, "inv_freq", inv_freq);
     if (static_cast<int64_t>(positions.numel()) != rows) throw std::invalid_argument("positions must have an element for every row");
+    if (static_cast<int64_t>(inv_freq.numel()) > head_dim / 2) throw std::invalid_argument("inv_freq must have an element for every pair, at most head_dim / 2");
     throw_on_nvk_status(nvk_rotary_embedding(query.data(), key.defined() ? key.data() : nullptr, pos.ptr, pos.dtype, inv_freq.data_as<float>(), attention_factor, rows,
                                              num_q_heads, num_kv_heads, head_dim, static_cast<int>(2 * inv_freq.numel()), interleaved ? 1 : 0, q_stride, k_stride,
                                              query_out.data(), key_out.defined() ? key_out.data() : nullptr, qo_stride, ko_stride, code(query.dtype()), stream));

@@ -490,7 +490,86 @@ def test_the_binding_refuses(change, word):
         nvk().store_kvcache_blocks8(key, value, kc, vc, ks, vs, None, ctx, bt)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("sizes", [(16, 1 << 62, 1 << 10), (1 << 40, 1 << 20, 1 << 10), (1 << 32, 2, D), (16, (1 << 32) + 2, D), (16, 2, (1 << 32) + D)])
+def test_the_binding_refuses_sizes_beyond_the_cache(sizes):
+    import torch
+    bs, hkv, d = sizes
+    kc, ks = torch.zeros(4, 16, 2, D, dtype=torch.int8, device="cuda"), torch.zeros(4, 2, device="cuda")
+    key, cu, bt = torch.zeros(4, 2, D, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(1, 2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        nvk().gather_kvcache_blocks8(kc, kc, ks, ks, cu, bt, hkv, d, bs, key, key.clone())
+    with pytest.raises((ValueError, ZeroDivisionError)):   # (as the other decode calls have it)
+        nvk().launch_decode_attention_paged_blocks8(key[:1].contiguous(), kc, kc, ks, ks, cu[:1], bt, hkv, d, bs, 1.0, key[:1].clone())
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [("int8", "bfloat16"), ("e4m3", "float16")])
+def test_two_streams_and_two_graphs_of_one_workspace(kind, dtype):
+    """Store, gather and decode on two streams at the same time, with a workspace each; then two captured decodes that share one, replayed one after the other."""
+    import torch
+    rng = np.random.default_rng(41)
+    hq, hkv, bs, scale, batch, width = 8, 2, 64, D ** -0.5, 3, 150
+    lens = [[9000, 0, 700], [1, 5000, 64]]
+    streams, work = [torch.cuda.Stream() for _ in range(2)], []
+    for n in lens:
+        c = Both(160, bs, hkv, kind)
+        tables = _tables(rng, [-(-x // bs) for x in n], width, 160)
+        cu = np.concatenate([[0], np.cumsum(n)])
+        rows = [_typed(rng.standard_normal((cu[-1], hkv, D)), dtype) for _ in range(2)]
+        q, q64 = _typed(rng.standard_normal((batch, hq, D)), dtype)
+        for w in range(2):
+            c.ref[w].store(rows[w][1], cu, n, tables)
+        up = lambda v: torch.as_tensor(np.asarray(v), dtype=torch.int32).cuda()
+        ws = torch.empty(max(16, nvk().decode_attention_workspace_bytes(batch, hq, hkv, D, width, bs)), dtype=torch.uint8, device="cuda")
+        work.append(dict(c=c, tables=tables, rows=rows, q=q, q64=q64, cu=up(cu), n=up(n), bt=up(tables), ws=ws, out=torch.full_like(q, float("nan")),
+                         dense=[torch.full_like(r[0], float("nan")) for r in rows]))
+
+    def decode(x, ws):
+        nvk().launch_decode_attention_paged_blocks8(x["q"], *x["c"].data, *x["c"].scale, x["n"], x["bt"], hkv, D, bs, scale, x["out"], ws)
+
+    torch.cuda.synchronize()
+    for s, x in zip(streams, work):
+        with torch.cuda.stream(s):
+            nvk().store_kvcache_blocks8(x["rows"][0][0], x["rows"][1][0], *x["c"].data, *x["c"].scale, x["cu"], x["n"], x["bt"])
+            nvk().gather_kvcache_blocks8(*x["c"].data, *x["c"].scale, x["cu"], x["bt"], hkv, D, bs, *x["dense"])
+            decode(x, x["ws"])
+    torch.cuda.synchronize()
+
+    def check():
+        for n, x in zip(lens, work):
+            for s in range(batch):
+                o = x["out"][s].double().cpu().numpy()
+                if n[s] == 0:
+                    assert (o == 0).all()
+                else:
+                    w, most = _bound(x["c"], x["tables"][s], n[s], x["q64"][s], scale, dtype)
+                    assert (np.abs(o - w) <= most).all()
+
+    check()
+    for x, n in zip(work, lens):
+        at = 0
+        for s in range(batch):
+            for w in range(2):   # (what the block stands for, rounded to the type: a power of two times 8 bits, exact in both)
+                assert np.array_equal(x["dense"][w][at:at + n[s]].double().cpu().numpy(), x["c"].ref[w].rows(x["tables"][s], n[s]))
+            at += n[s]
+    graphs, stream = [], torch.cuda.Stream()
+    for x in work:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            decode(x, work[0]["ws"])
+        graphs.append(g)
+    for x in work:
+        x["out"].fill_(float("nan"))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    check()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 def test_a_run_of_steps_from_lengths_to_outputs(kind):

@@ -48,7 +48,8 @@ P, Q = ctypes.c_void_p(1 << 20), ctypes.c_void_p(1 << 24)
     (dict(rows=L(-1)), 1, "positive"), (dict(hkv=I(0)), 1, "positive"), (dict(rot=I(63)), 1, "even"), (dict(rot=I(130)), 1, "at most head_dim"), (dict(rot=I(0)), 1, "positive"),
     (dict(d=I(1026), rot=I(2), q_stride=L(1 << 16), k_stride=L(1 << 16), qo_stride=L(1 << 16), ko_stride=L(1 << 16)), 3, "1024"), (dict(q_stride=L(1000)), 1, "less than a row"),
     (dict(qo=ctypes.c_void_p((1 << 20) + 64)), 1, "overlap"), (dict(qo=P, qo_stride=L(2048)), 1, "overlap"), (dict(q=ctypes.c_void_p((1 << 20) + 1)), 1, "misaligned"),
-    (dict(f=ctypes.c_void_p(2)), 1, "misaligned"), (dict(rows=L(0)), 0, "")])
+    (dict(f=ctypes.c_void_p(2)), 1, "misaligned"), (dict(rows=L(0)), 0, ""),
+    (dict(hq=I((1 << 19) + 1), q_stride=L(1 << 40), qo_stride=L(1 << 40)), 3, "too many heads"), (dict(hkv=I((1 << 31) - 1), k_stride=L(1 << 40), ko_stride=L(1 << 40)), 3, "too many heads")])
 def test_refuses(built, change, code, word):
     a = dict(q=P, k=ctypes.c_void_p(1 << 22), pos=P, pos_dtype=I(3), f=P, factor=ctypes.c_float(1.0), rows=L(4), hq=I(8), hkv=I(2), d=I(128), rot=I(128), pairs=I(0),
              q_stride=L(1024), k_stride=L(256), qo=Q, ko=ctypes.c_void_p(1 << 25), qo_stride=L(1024), ko_stride=L(256), dtype=I(1), stream=None)
@@ -133,6 +134,31 @@ def test_far_positions(position):
     want = np.concatenate([y[..., :32] * c - y[..., 32:] * s, y[..., 32:] * c + y[..., :32] * s], -1)
     off = 2 * math.pi * abs(position) / (2 * math.pi) * 2.0 ** -52     # two roundings of the turns, in radians
     assert np.abs(out.double().cpu().numpy() - want).max() <= 2 * np.abs(y).max() * (off + 2.0 ** -21 + 2.0 ** -23) + 2.0 ** -23
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("rows,heads,d,rot", [(14300, 1, 1024, 1024), (2400, 2, 1024, 1024), (19000, 1, 128, 128), (3000, 1, 1024, 8)])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_many_rows_of_few_heads(dtype, rows, heads, d, rot, pairs):
+    """As many rows to a block, and as many angles, as there can be; queries alone, and another call of them on a second stream at the same time."""
+    import torch
+    rng = np.random.default_rng(rows)
+    sets, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    f = torch.tensor(nvk().rotary_inv_freq(rot, 10000.0)[0], dtype=torch.float32, device="cuda")
+    for _ in streams:
+        x = torch.from_numpy(rng.standard_normal((rows, heads, d))).to(getattr(torch, dtype)).cuda()
+        sets.append((x, torch.from_numpy(rng.integers(0, 1 << 17, rows)).cuda(), torch.full_like(x, float("nan"))))
+    torch.cuda.synchronize()
+    for s, (x, pos, out) in zip(streams, sets):
+        with torch.cuda.stream(s):
+            nvk().rotary_embedding(x, None, pos, f, pairs, query_out=out)
+    torch.cuda.synchronize()
+    for x, pos, out in sets:
+        y = x.double().cpu().numpy()
+        want = ref.rotary(y, pos.tolist(), f.double().tolist(), pairs, 1.0)
+        assert (np.abs(out.double().cpu().numpy() - want) <= _tolerance(want, np.abs(y).max(), 1.0, dtype)).all()
+        assert torch.equal(out[..., rot:], x[..., rot:])
 
 
 @pytest.mark.gpu
