@@ -5,9 +5,13 @@
 // With old length l_b, n_b new tokens and blocks of s tokens, request b needs ceil((l_b + n_b) / s) - ceil(l_b / s) new blocks; the prefix sums of these
 // say which of the free blocks are its own, and whether there are enough.  Sums over the batch, then every table entry and every token by itself.
 //
-// A call is bound by the trips to memory one after the other (row, its length and its blocks) and by the launch: all blocks of one cluster do the sums over the
-// whole batch for themselves, so that nothing is handed over, and share out the table entries and the tokens.  A cluster because lengths and the count of free
-// blocks may be updated in place: they are when every block has read them.
+// A call is bound by the trips to memory one after the other (row, its length and its blocks) and by the launch.  So every block does the sums over the whole batch for itself, so that
+// nothing is handed over, and the blocks share out the table entries and the tokens.  Lengths and the count of free blocks may be updated in place, when every block has read them.  Where
+// they are, the blocks are one cluster, whose first one writes them behind a barrier, up to four pieces of 16 bytes to a thread; beyond, and wherever the new ones are of their own, there
+// are as many blocks as the work is worth, and what is updated in place follows in a kernel of one block.  us, in a cluster / by many blocks (and that kernel): 256 requests, table rows of 33
+// int32 (8448 pieces) 3.9 / 5.0, 16 of 2304 new tokens, int64 (36864 pieces) 5.7 / 4.9, 1024 with rows of 33 6.2 / 7.1, of 129 (132096) 9.2 / 8.0.  Of their own: 3.7, 4.5, 5.7, 6.7; a
+// decode step of one request 2.7, of 256 (rows of 32) 3.3, 1024 requests of rows of 512 6.4 (2.1 MB written), 8192 of 33 26 us.  Up to 256 requests by blocks of 256 threads (a scan over
+// 1024 takes 1 us more: 256 requests, rows of 33, 4.7), beyond by 1024.
 #include "nvk_internal.cuh"
 
 #include <algorithm>
@@ -21,8 +25,8 @@ constexpr int kFewThreads = 256, kManyThreads = 1024;
 constexpr int kMaxBlocks = 16;            // of a cluster (not portable, but there on every B200)
 constexpr int kMaxBatch = 8192;           // 24 bytes of shared memory for each
 constexpr int kAhead = 2;                 // pieces of table rows that a thread has under way
-constexpr int64_t kWideWork = 2 * kMaxBlocks * kManyThreads;   // pieces of 16 bytes up to which one cluster takes a step
-constexpr uint32_t kMost = 0x7fffffffu;
+constexpr int64_t kClusterPieces = 4;     // of 16 bytes to a thread, up to which one cluster takes a step that updates in place
+constexpr uint32_t kMost = 0x7fffffffu, kNone = 0xffffffffu;
 
 // Sums of numbers below 2^31, held at 2^31 - 1: lengths come from the device, and no sum of them may wrap round.
 __device__ __forceinline__ uint32_t add_held(uint32_t a, uint32_t b) { return min(a + b, kMost); }
@@ -94,8 +98,9 @@ __device__ __forceinline__ uint32_t blocks_of(const FastDiv& by_block, uint32_t 
 template <typename E, int V> struct alignas(V * sizeof(E)) Entries { E e[V]; };
 
 template <typename E, int V, int THREADS>
-__global__ void __launch_bounds__(THREADS) step_metadata_kernel(const __grid_constant__ StepParams<E> p) {
+__global__ void __launch_bounds__(THREADS, 1) step_metadata_kernel(const __grid_constant__ StepParams<E> p) {
     constexpr int kWarps = THREADS / 32, kTokens = 4;
+    constexpr bool kRounds = THREADS > kFewThreads;   // (few threads: where there are no more requests than those)
     extern __shared__ __align__(16) Request s_request[];
     Tokens* s_token = reinterpret_cast<Tokens*>(s_request + p.batch);
     __shared__ Three s_warp[kWarps];
@@ -119,6 +124,13 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const __grid_con
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) piece_row[u] = me + u * threads < pieces ? row_of(static_cast<int>(p.by_pieces.div(me + u * threads))) : static_cast<E>(-1);
     if (known(row0)) len0 = p.lens[row0];
+    // And of the requests that follow, THREADS at a time: two rounds ahead the row and the new tokens, one round ahead the length.
+    E row1 = -1, new1 = 0;
+    auto load_row = [&](int b) {
+        row1 = b < p.batch ? row_of(b) : static_cast<E>(-1);
+        new1 = b < p.batch ? p.new_lens[b] : static_cast<E>(0);
+    };
+    if constexpr (kRounds) load_row(tid + THREADS);
     // The first pieces of the table rows: which of their entries count is seen later.
     auto load = [&](int i, E row, Piece& to) {
         const int64_t j = static_cast<int64_t>(i - static_cast<int>(p.by_pieces.div(i)) * static_cast<int>(p.by_pieces.d)) * V;
@@ -147,11 +159,12 @@ __global__ void __launch_bounds__(THREADS) step_metadata_kernel(const __grid_con
     auto requests = [&](int b0, auto scan) {
         const int b = b0 + tid;
         const bool there = b < p.batch;
-        E row = row0, n_in = new0, len_in = len0;
-        if (b0 > 0) {
-            row = there ? row_of(b) : static_cast<E>(-1);
-            n_in = there ? p.new_lens[b] : static_cast<E>(0);
-            len_in = known(row) ? p.lens[row] : static_cast<E>(0);
+        const E row = row0, n_in = new0, len_in = len0;
+        if (kRounds && b0 + THREADS < p.batch) {
+            row0 = row1;
+            new0 = new1;
+            len0 = known(row0) ? p.lens[row0] : static_cast<E>(0);
+            load_row(b + 2 * THREADS);
         }
         const bool ours = known(row);
         const uint32_t len = held(len_in), n = held(n_in);
@@ -351,15 +364,29 @@ template <typename E> __global__ void __launch_bounds__(kManyThreads) commit_ste
     if (threadIdx.x == 0) s_taken = 0;
     __syncthreads();
     uint32_t taken = 0;
-    for (int b = threadIdx.x; b < p.batch; b += kManyThreads) {
-        const E row = p.rows != nullptr ? p.rows[b] : static_cast<E>(b);
-        const uint32_t ctx = static_cast<uint32_t>(p.context_lens[b]);
-        if (row >= 0 && row < p.num_rows && ctx > 0) {
-            // (where new lengths are of their own, the first kernel has set them: lens are still the old ones)
-            taken += blocks_of(p.by_block, ctx) - blocks_of(p.by_block, held(p.lens[row]));
-            if (p.new_lens_out == p.lens) p.new_lens_out[row] = ctx;
+    // `each` requests of a thread (where new lengths are of their own, the first kernel has set them: lens are still the old ones)
+    auto commit = [&](auto each) {
+        constexpr int kEach = decltype(each)::value;
+        uint32_t ctx[kEach], old[kEach];
+        int row[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int b = threadIdx.x + i * kManyThreads;
+            const E id = b >= p.batch ? static_cast<E>(-1) : p.rows != nullptr ? p.rows[b] : static_cast<E>(b);
+            ctx[i] = b < p.batch ? static_cast<uint32_t>(p.context_lens[b]) : 0u;
+            row[i] = id >= 0 && id < p.num_rows ? static_cast<int>(id) : -1;
         }
-    }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) old[i] = ctx[i] > 0 && row[i] >= 0 ? held(p.lens[row[i]]) : kNone;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (old[i] == kNone) continue;
+            taken += blocks_of(p.by_block, ctx[i]) - blocks_of(p.by_block, old[i]);
+            if (p.new_lens_out == p.lens) p.new_lens_out[row[i]] = ctx[i];
+        }
+    };
+    if (p.batch <= kManyThreads) commit(std::integral_constant<int, 1>());
+    else commit(std::integral_constant<int, kMaxBatch / kManyThreads>());
     taken = __reduce_add_sync(0xffffffffu, taken);
     if ((threadIdx.x & 31) == 0) atomicAdd(&s_taken, taken);
     __syncthreads();
@@ -478,11 +505,12 @@ template <typename E, int V> int launch_step(const StepArgs& a, uint32_t capacit
     p.by_pieces = FastDiv(static_cast<uint32_t>(a.max_blocks / V));
     p.token_pieces = aligned_to(a.positions, 16) && aligned_to(a.slots, 16);
     const int64_t work = std::max(a.batch * a.max_blocks / V, a.num_tokens / 4);
-    if (a.batch <= kFewThreads && work <= kMaxBlocks * kFewThreads)
-        return launch("step_metadata", step_metadata_kernel<E, V, kFewThreads>, p, kFewThreads, work / kFewThreads + 1, false, few_done, a.stream);
-    p.wide = work > kWideWork;
-    const int rc = launch("step_metadata", step_metadata_kernel<E, V, kManyThreads>, p, kManyThreads, work / kManyThreads + 1, p.wide, many_done, a.stream);
-    if (rc != NVK_OK || !p.wide || (p.new_lens_out != p.lens && p.new_count != p.free_count)) return rc;
+    const bool in_place = p.new_lens_out == p.lens || p.new_count == p.free_count;
+    const int threads = a.batch <= kFewThreads ? kFewThreads : kManyThreads;
+    p.wide = in_place ? std::max(work, a.num_tokens * 2 * static_cast<int64_t>(sizeof(E)) / 16) > kClusterPieces * kMaxBlocks * threads : work > threads;
+    const int rc = threads == kFewThreads ? launch("step_metadata", step_metadata_kernel<E, V, kFewThreads>, p, threads, work / threads + 1, p.wide, few_done, a.stream)
+                                          : launch("step_metadata", step_metadata_kernel<E, V, kManyThreads>, p, threads, work / threads + 1, p.wide, many_done, a.stream);
+    if (rc != NVK_OK || !p.wide || !in_place) return rc;
     const cudaError_t e = launch_pdl(commit_step_kernel<E>, dim3(1), dim3(kManyThreads), 0, a.stream, p);
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "commit_step_kernel launch: %s", cudaGetErrorString(e));
     return check_launch("commit_step_kernel launch");
