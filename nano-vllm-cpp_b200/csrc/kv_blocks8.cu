@@ -14,6 +14,7 @@
 // The store goes by sequences, not by slots: rows that share a scale have to come together, and a block of threads finds those of one cache block from the lengths.
 #include "nvk_internal.cuh"
 
+#include <atomic>
 #include <type_traits>
 
 namespace nvk {
@@ -23,8 +24,9 @@ constexpr int kDim = 128;
 constexpr int kThreads = 256;
 constexpr int kLanes = kDim / 8;          // 16-byte pieces (eight elements) of a 16-bit head vector
 constexpr int kMaxSets = 16;              // (head, K or V) of a block of threads
-constexpr int kPasses = 16;               // pieces of a thread of store_blocks_kernel in registers
+constexpr int kPasses = 16;               // pieces of a thread of store_blocks_kernel, in registers or shared memory
 constexpr int kTileRows = kThreads * kPasses / kLanes;   // rows of a head, or of several together, that a block of threads holds
+constexpr int kTileBytes = kThreads * kPasses * 16;      // 64 KiB, three blocks to an SM
 
 // Two elements of T as one register.
 template <typename T> struct PairOf;
@@ -167,7 +169,7 @@ struct StoreParams {
     FastDiv by_block, by_sets;                                       // by_sets: 2 Hkv
 };
 
-// One new row for each sequence: a warp takes one head of K or of V of one, and the whole block of threads the rows of those whose scale it raised.
+// One new row for each sequence (1.4 us for one, 2.7 for 256 of 8 KV heads: latency): a warp takes one head of K or of V of one, and the whole block of threads the rows of those whose scale it raised.
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kThreads) store_row_kernel(const __grid_constant__ StoreParams p) {
     struct Raise { unsigned char* base; int rows; float ratio; };
@@ -212,9 +214,14 @@ __global__ void __launch_bounds__(kThreads) store_row_kernel(const __grid_consta
 
 // Any number of new rows: a block of threads takes those that fall into one cache block, of one or several sets.  Which sequence its unit
 // belongs to: sequence s has the units from floor(cu[s] / block_size) + 2 s on, which are at least as many as the cache blocks that its rows can touch.
-// HELD: a block's rows are few enough to stay in registers between their maximum and their rounding.
-template <typename T, bool FP8, bool HELD>
-__global__ void __launch_bounds__(kThreads, 2) store_blocks_kernel(const __grid_constant__ StoreParams p) {
+// Between their maximum and their rounding the rows wait in shared memory, or in registers; of blocks too large for that they are read again.
+// Bound by HBM: 36864 rows of 8 KV heads of F16, blocks of 256, 39.1 us, 5.8 TB/s of what is read and written.  What a block of threads does is load, wait, round and store, one after the
+// other, so that several of them have to be there to keep the memory busy: three with 64 KiB each on their way by asynchronous copies to shared memory, where registers hold two (43.4 us;
+// blocks that go from task to task and load the next one meanwhile 46.8 and 50.5).  Where there are no more than two to an SM anyway registers take less time: 77 rows 3.3 us instead of 3.8.
+enum StoreRows { kInRegisters, kInShared, kAgain };
+template <typename T, bool FP8, StoreRows ROWS>
+__global__ void __launch_bounds__(kThreads, ROWS == kInShared ? 3 : 2) store_blocks_kernel(const __grid_constant__ StoreParams p) {
+    extern __shared__ __align__(16) uint4 s_rows[];
     __shared__ uint32_t s_top[kMaxSets];
     pdl_wait_then_release();
     const int tid = threadIdx.x, unit = blockIdx.x;
@@ -250,9 +257,21 @@ __global__ void __launch_bounds__(kThreads, 2) store_blocks_kernel(const __grid_
     auto load = [](const T* at) { return __ldcs(reinterpret_cast<const uint4*>(at)); };
     float* scale = p.scale[which] + id * p.num_kv_heads + head;
     const float old = live && row0 > 0 ? *scale : 0.0f;
-    uint4 v[HELD ? kPasses : 1];
+    uint4* held = s_rows + tid;              // this thread's own pieces, kThreads apart (zeros where there is no row)
+    uint4 v[ROWS == kInRegisters ? kPasses : 1];
     uint32_t top = 0;
-    if constexpr (HELD) {
+    if constexpr (ROWS == kInShared) {
+        const T* at = src;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i, at += step) {
+            const bool there = rank + i * ranks < mine;
+            cp_async16(smem_u32(held + i * kThreads), there ? at : static_cast<const T*>(p.rows[which]), there ? 16 : 0);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) top = top_of<T>(top, held[i * kThreads]);
+    } else if constexpr (ROWS == kInRegisters) {
         const T* at = src;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i, at += step) v[i] = rank + i * ranks < mine ? load(at) : make_uint4(0u, 0u, 0u, 0u);
@@ -274,10 +293,10 @@ __global__ void __launch_bounds__(kThreads, 2) store_blocks_kernel(const __grid_
     unsigned char* base = p.cache[which] + static_cast<size_t>(id) * p.block_size * row_bytes + head * kDim;
     unsigned char* dst = base + (row0 + rank) * row_bytes + sub * 8;
     const size_t dst_step = ranks * row_bytes;
-    if constexpr (HELD) {
+    if constexpr (ROWS != kAgain) {
 #pragma unroll
         for (int i = 0; i < kPasses; ++i, dst += dst_step)
-            if (rank + i * ranks < rows) *reinterpret_cast<uint2*>(dst) = quantise8<T, FP8>(v[i], inv, narrow);
+            if (rank + i * ranks < rows) *reinterpret_cast<uint2*>(dst) = quantise8<T, FP8>(ROWS == kInShared ? held[i * kThreads] : v[i], inv, narrow);
     } else {
         const T* at = src;
         for (int r = rank; r < rows; r += ranks, at += step, dst += dst_step) *reinterpret_cast<uint2*>(dst) = quantise8<T, FP8>(load(at), inv, narrow);
@@ -294,15 +313,24 @@ template <typename T, bool FP8> int launch_store_typed(const StoreParams& in, cu
         const int64_t blocks = (static_cast<int64_t>(p.num_seqs) * p.by_sets.d + kThreads / 32 - 1) / (kThreads / 32);
         e = launch_pdl(store_row_kernel<T, FP8>, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream, p);
     } else {
-        // As many sets to a block of threads as its registers hold.
+        static std::atomic<bool> attr_done[64] = {};
+        int device = 0;
+        cudaGetDevice(&device);
+        if (device >= 0 && device < 64 && !attr_done[device]) {
+            e = cudaFuncSetAttribute(store_blocks_kernel<T, FP8, kInShared>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTileBytes);
+            if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "store_kvcache_blocks8: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+            attr_done[device] = true;
+        }
+        // As many sets to a block of threads as it has room for.
         p.sets = 1;
         while (p.sets < kMaxSets && 2 * p.sets * p.block_size <= kTileRows) p.sets *= 2;
         const int64_t units = p.total_q / p.block_size + 2ll * p.num_seqs;
         if (units > 0x7fffffffLL) return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many tokens");
         const dim3 grid(static_cast<unsigned>(units), (p.by_sets.d + p.sets - 1) / p.sets);
         if (grid.y > 65535) return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many heads");
-        e = p.sets * p.block_size <= kTileRows ? launch_pdl(store_blocks_kernel<T, FP8, true>, grid, dim3(kThreads), 0, stream, p)
-                                               : launch_pdl(store_blocks_kernel<T, FP8, false>, grid, dim3(kThreads), 0, stream, p);
+        if (p.sets * p.block_size > kTileRows) e = launch_pdl(store_blocks_kernel<T, FP8, kAgain>, grid, dim3(kThreads), 0, stream, p);
+        else if (units * grid.y <= 2 * kSmCount) e = launch_pdl(store_blocks_kernel<T, FP8, kInRegisters>, grid, dim3(kThreads), 0, stream, p);
+        else e = launch_pdl(store_blocks_kernel<T, FP8, kInShared>, grid, dim3(kThreads), kTileBytes, stream, p);
     }
     if (e != cudaSuccess) return fail(NVK_ERR_CUDA, "store_kvcache_blocks8 kernel launch: %s", cudaGetErrorString(e));
     return check_launch("store_kvcache_blocks8 kernel launch");
@@ -310,7 +338,7 @@ template <typename T, bool FP8> int launch_store_typed(const StoreParams& in, cu
 
 // ---- gather ----------------------------------------------------------------------------------------------------------------
 constexpr int kGatherRows = 256;          // dense rows of a block of threads, at most
-constexpr int kGatherVectors = 256;       // and of K and of V head vectors, where there are enough of them for two blocks to an SM
+constexpr int kGatherVectors = 128;       // and of K and of V head vectors, where there are enough of them for two blocks to an SM
 constexpr int kGatherAhead = 4;           // head vectors of K and of V that a lane has under way
 constexpr int kGatherLanes = kDim / 16;   // lanes of a head vector
 
@@ -344,6 +372,8 @@ template <typename T, bool FP8, bool WIDE> __device__ __forceinline__ void dequa
     store32<WIDE>(out, o);
 }
 
+// Bound by HBM: 43008 rows of 8 KV heads, 42.7 us, 6.2 TB/s.  A lane has four head vectors of K and of V under way by loads without branches, and writes 32 bytes at a time; a block of threads
+// has 128 of each (256: 44.1 us and, at a sixth of the rows, 12.9 instead of 10.2, since the last blocks run alone for longer; 64: 42.9 to 46.7).
 template <typename T, bool FP8, bool WIDE>
 __global__ void __launch_bounds__(kThreads) gather_blocks8_kernel(const __grid_constant__ GatherParams p) {
     __shared__ int64_t s_row[kGatherRows];     // cache row of a dense row; -1: zeros

@@ -210,6 +210,20 @@ def test_store_in_several_steps(kind, dtype, bs, hkv, index):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [("int8", "bfloat16"), ("int8", "float16"), ("e4m3", "bfloat16"), ("e4m3", "float16")])
+@pytest.mark.parametrize("bs,hkv,first,then", [(16, 8, (0, 37, 5000, 16), (5100, 0, 300, 1)), (64, 3, (9000, 700, 1), (63, 10500, 64)), (256, 4, (9000, 255, 1000), (300, 9400, 25)),
+                                               (8, 5, (2600,), (2700,)), (48, 1, (31000, 5), (20, 30100))])
+def test_store_of_many_rows(kind, dtype, bs, hkv, first, then):
+    """More blocks of threads than two to an SM, twice: the second step joins blocks of the first one with larger rows."""
+    rng = np.random.default_rng(bs + hkv)
+    need = [-(-(a + b) // bs) for a, b in zip(first, then)]
+    c, tables, total = Both(sum(need) + 3, bs, hkv, kind), _tables(rng, need, max(need), sum(need) + 3), np.zeros(len(first), np.int64)
+    for size, new in ((1.0, first), (5.0, then)):
+        cu, total = [0, *np.cumsum(new).tolist()], total + np.array(new)
+        c.store([_typed(rng.standard_normal((cu[-1], hkv, D)) * size, dtype) for _ in range(2)], cu, total.tolist(), tables)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 def test_store_of_hard_values(kind, dtype):
