@@ -1,12 +1,12 @@
-// Paged-KV decode attention for sm_100a (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 and 4-bit caches), and the same with the weights of the
-// keys added up.
+// Paged-KV decode attention for sm_100a (F16 / BF16 queries, head_dim 128; 16-bit, int8, e4m3 and 4-bit caches, 8-bit ones with scales of tokens or of blocks), and the same with the
+// weights of the keys added up.
 //
 // Replaces decode_paged_attention_kernel and decode_paged_attention_int8_kernel (src/kernels/attention.cu:313-405, :746-842 of the
 // reference: one warp per (sequence, query head), every KV row re-read by each query head of its group, 8 dependent shuffles per
 // key) and the FlashAttention-2 call it can dlopen (src/kernels/flash_attn.cpp:302-431).
 //
 // The op is HBM-bound (over a 4-bit cache it is not: see Cache4); decode_body.cuh has the arithmetic and the ways to share out the keys.  What each kernel here adds:
-//   decode_split_kernel    one four-warp block per (KV head, chunk, sequence), two per SM (three for 8-bit caches, four for 4-bit ones, or two of eight warps).  The grid is fixed
+//   decode_split_kernel    one four-warp block per (KV head, chunk, sequence), two per SM (three for 8-bit caches, four for 4-bit ones, or two of eight warps; with scales of blocks three, or one of eight).  The grid is fixed
 //                          from host-known sizes: nothing depends on host knowledge of context_lens (CUDA-graph safe); blocks
 //                          whose chunk lies beyond the context exit at once.
 //   decode_merge_kernel    merges the chunks of long contexts; launched only where the table can hold more than one.
