@@ -159,6 +159,17 @@ template <bool FP8> __device__ __forceinline__ void scale_rows(unsigned char* ba
     }
 }
 
+// cp_async16 of what is read once: it gives way first in L2, where the elements that are written stay for the gather or the attention that comes next.  (So do the gather's dense rows, which are
+// too many to stay; together, a store of 36864 rows and a gather of 43008: 83.4 -> 77.8 us.)
+__device__ __forceinline__ uint64_t read_once() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void cp_async16_once(uint32_t dst, const void* src, int src_bytes, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;\n" ::"r"(dst), "l"(src), "r"(src_bytes), "l"(policy) : "memory");
+}
+
 struct StoreParams {
     const void* rows[2]; unsigned char* cache[2]; float* scale[2];   // of K and of V
     int64_t stride[2];                                               // elements from a token to the next
@@ -215,7 +226,7 @@ __global__ void __launch_bounds__(kThreads) store_row_kernel(const __grid_consta
 // Any number of new rows: a block of threads takes those that fall into one cache block, of one or several sets.  Which sequence its unit
 // belongs to: sequence s has the units from floor(cu[s] / block_size) + 2 s on, which are at least as many as the cache blocks that its rows can touch.
 // Between their maximum and their rounding the rows wait in shared memory, or in registers; of blocks too large for that they are read again.
-// Bound by HBM: 36864 rows of 8 KV heads of F16, blocks of 256, 39.1 us, 5.8 TB/s of what is read and written.  What a block of threads does is load, wait, round and store, one after the
+// Bound by HBM: 36864 rows of 8 KV heads of F16, blocks of 256, 41.2 us, 5.5 TB/s of what is read and written (over and over; 39.1 where its input may stay in L2).  What a block of threads does is load, wait, round and store, one after the
 // other, so that several of them have to be there to keep the memory busy: three with 64 KiB each on their way by asynchronous copies to shared memory, where registers hold two (43.4 us;
 // blocks that go from task to task and load the next one meanwhile 46.8 and 50.5).  Where there are no more than two to an SM anyway registers take less time: 77 rows 3.3 us instead of 3.8.
 enum StoreRows { kInRegisters, kInShared, kAgain };
@@ -261,11 +272,12 @@ __global__ void __launch_bounds__(kThreads, ROWS == kInShared ? 3 : 2) store_blo
     uint4 v[ROWS == kInRegisters ? kPasses : 1];
     uint32_t top = 0;
     if constexpr (ROWS == kInShared) {
+        const uint64_t policy = read_once();
         const T* at = src;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i, at += step) {
             const bool there = rank + i * ranks < mine;
-            cp_async16(smem_u32(held + i * kThreads), there ? at : static_cast<const T*>(p.rows[which]), there ? 16 : 0);
+            cp_async16_once(smem_u32(held + i * kThreads), there ? at : static_cast<const T*>(p.rows[which]), there ? 16 : 0, policy);
         }
         cp_async_commit();
         cp_async_wait<0>();
@@ -353,11 +365,11 @@ struct GatherParams {
 // 32 bytes next to each other: one store where they lie on such a boundary.
 template <bool WIDE> __device__ __forceinline__ void store32(uint4* out, const uint32_t (&o)[8]) {
     if constexpr (WIDE) {
-        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+        asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
                      ::"l"(out), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
     } else {
-        out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+        __stcs(out, make_uint4(o[0], o[1], o[2], o[3]));
+        __stcs(out + 1, make_uint4(o[4], o[5], o[6], o[7]));
     }
 }
 template <typename T, bool FP8, bool WIDE> __device__ __forceinline__ void dequantise16(const uint4& v, float scale, uint4* out) {
@@ -372,7 +384,7 @@ template <typename T, bool FP8, bool WIDE> __device__ __forceinline__ void dequa
     store32<WIDE>(out, o);
 }
 
-// Bound by HBM: 43008 rows of 8 KV heads, 42.7 us, 6.2 TB/s.  A lane has four head vectors of K and of V under way by loads without branches, and writes 32 bytes at a time; a block of threads
+// Bound by HBM: 43008 rows of 8 KV heads, 42.6 us, 6.2 TB/s, behind their store some 37.  A lane has four head vectors of K and of V under way by loads without branches, and writes 32 bytes at a time; a block of threads
 // has 128 of each (256: 44.1 us and, at a sixth of the rows, 12.9 instead of 10.2, since the last blocks run alone for longer; 64: 42.9 to 46.7).
 template <typename T, bool FP8, bool WIDE>
 __global__ void __launch_bounds__(kThreads) gather_blocks8_kernel(const __grid_constant__ GatherParams p) {
