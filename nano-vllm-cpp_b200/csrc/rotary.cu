@@ -9,10 +9,10 @@
 // bits, and only their fraction goes on to sincospi in 32: off by 2^-53 of the number of turns, and by 2^-25 of a turn.  A row's angles are worked out once for all its
 // heads: a handful of 64-bit operations for each pair of a row, next to Hq + Hkv times as many elements.
 //
-// Bound by HBM for many rows (every element is read and written once), by the trip to memory and the launch for few.  A thread takes two pieces of V elements of a head,
-// whose V pairs lie in them whole, in either layout: pieces i and rot / 2 + i, or two next to each other.  Two pairs are turned by one instruction (f32x2), three items of a
-// thread are under way at once, in 64 registers: 16384 rows of 32 / 8 heads of 128, BF16, halves, take 54.5 us (6.2 TB/s; one pair at a time 62.7, four items at
-// once 57.0, two 58.1), 4096 rows 12.6, 256 rows 2.5, one row 1.9.
+// Bound by HBM for many rows (every element is read and written once), by the trip to memory and the launch for few.  A thread takes two pieces of V elements of a head, i and rot / 2 + i,
+// which hold V pairs whole in either layout, and the lanes' pieces lie next to each other (pairs of neighbours in two pieces next to each other: 59.2 instead of 53.9 us below, in F32 56.3 instead
+// of 50.5).  Two pairs are turned by one instruction (f32x2), three items of a thread are under way at once, in 64 registers: 16384 rows of 32 / 8 heads of 128, BF16, halves, take 54.9 us
+// (6.1 TB/s; one pair at a time 62.7, four items at once 57.0, two 58.1), neighbours 53.9, 4096 rows 13.1, one row 1.9.
 #include "nvk_internal.cuh"
 
 #include <algorithm>
@@ -75,6 +75,8 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
 template <typename T, int V, bool PAIRS>
 __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
     extern __shared__ __align__(16) float s_cos[];    // [row][pair], times the factor; the sines behind them
+    constexpr bool kApart = !PAIRS || V >= 2;         // an item's pieces lie half of the rotated part from each other (neighbours of one element each: next to each other)
+    constexpr int kEach = PAIRS && V >= 2 ? V / 2 : V;   // from the angles of an item to those of the next
     using P = typename Piece<V * sizeof(T)>::type;
     pdl_wait_then_release();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * p.block_rows;
@@ -88,13 +90,13 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_consta
     auto place_of = [&](int i) {
         const int all = static_cast<int>(p.by_items.div(i)), item = i - all * p.items;
         const int row = static_cast<int>(p.by_heads.div(all)), head = all - row * static_cast<int>(p.by_heads.d);
-        const bool halves = !PAIRS && item < turned;
+        const bool halves = kApart && item < turned;
         Place w;
         w.row = row;
         w.which = head >= p.heads[0] ? 1 : 0;
         w.off = (head - (w.which ? p.heads[0] : 0)) * p.head_dim + (halves ? item * V : item * 2 * V);
         w.second = halves ? half : item * 2 * V + V < p.head_dim ? V : 0;
-        w.angle = item < turned ? row * half + item * V : -1;
+        w.angle = item < turned ? row * half + item * kEach : -1;
         return w;
     };
     auto load = [&](int i, Elems<T, V> (&v)[2]) {
@@ -131,26 +133,36 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_consta
             if (i0 + u * kThreads >= total) break;
             const Place w = place_of(i0 + u * kThreads);
             if (w.angle >= 0) {
-                // (pair k: elements k of both pieces, or 2k and 2k + 1 of the two together)
-                auto a_of = [&](int k) -> T& { return PAIRS ? x[u][2 * k / V].e[2 * k % V] : x[u][0].e[k]; };
-                auto b_of = [&](int k) -> T& { return PAIRS ? x[u][(2 * k + 1) / V].e[(2 * k + 1) % V] : x[u][1].e[k]; };
                 using E = ElemTraits<T>;
-                if constexpr (V >= 2) {
+                // Pairs k and k + 1 of a piece, or of both; where their angles are.
+                auto turn2 = [&](T& a0, T& b0, T& a1, T& b1, int angle) {
+                    const float2 c = *reinterpret_cast<const float2*>(s_cos + angle), s = *reinterpret_cast<const float2*>(s_sin + angle);
+                    const F2 c2 = f2(c.x, c.y), s2 = f2(s.x, s.y), n2 = f2(-s.x, -s.y);
+                    const F2 a = f2(E::to_float(a0), E::to_float(a1)), b = f2(E::to_float(b0), E::to_float(b1));
+                    const float2 first = floats(fma2(a, c2, mul2(b, n2))), other = floats(fma2(b, c2, mul2(a, s2)));
+                    a0 = E::from_float(first.x);
+                    a1 = E::from_float(first.y);
+                    b0 = E::from_float(other.x);
+                    b1 = E::from_float(other.y);
+                };
+                auto turn1 = [&](T& a0, T& b0, int angle) {
+                    const float a = E::to_float(a0), b = E::to_float(b0), c = s_cos[angle], s = s_sin[angle];
+                    a0 = E::from_float(fmaf(a, c, -(b * s)));
+                    b0 = E::from_float(fmaf(b, c, a * s));
+                };
+                if constexpr (!PAIRS && V >= 2) {
 #pragma unroll
-                    for (int k = 0; k < V; k += 2) {
-                        const float2 c = *reinterpret_cast<const float2*>(s_cos + w.angle + k), s = *reinterpret_cast<const float2*>(s_sin + w.angle + k);
-                        const F2 c2 = f2(c.x, c.y), s2 = f2(s.x, s.y), n2 = f2(-s.x, -s.y);
-                        const F2 a = f2(E::to_float(a_of(k)), E::to_float(a_of(k + 1))), b = f2(E::to_float(b_of(k)), E::to_float(b_of(k + 1)));
-                        const float2 first = floats(fma2(a, c2, mul2(b, n2))), other = floats(fma2(b, c2, mul2(a, s2)));
-                        a_of(k) = E::from_float(first.x);
-                        a_of(k + 1) = E::from_float(first.y);
-                        b_of(k) = E::from_float(other.x);
-                        b_of(k + 1) = E::from_float(other.y);
-                    }
+                    for (int k = 0; k < V; k += 2) turn2(x[u][0].e[k], x[u][1].e[k], x[u][0].e[k + 1], x[u][1].e[k + 1], w.angle + k);
+                } else if constexpr (PAIRS && V >= 4) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int k = 0; k < V; k += 4) turn2(x[u][i].e[k], x[u][i].e[k + 1], x[u][i].e[k + 2], x[u][i].e[k + 3], w.angle + i * (half / 2) + k / 2);
+                } else if constexpr (PAIRS && V == 2) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) turn1(x[u][i].e[0], x[u][i].e[1], w.angle + i * (half / 2));
                 } else {
-                    const float a = E::to_float(a_of(0)), b = E::to_float(b_of(0)), c = s_cos[w.angle], s = s_sin[w.angle];
-                    a_of(0) = E::from_float(fmaf(a, c, -(b * s)));
-                    b_of(0) = E::from_float(fmaf(b, c, a * s));
+                    turn1(x[u][0].e[0], x[u][1].e[0], w.angle);
                 }
             }
             T* out = static_cast<T*>(p.out[w.which]) + (row0 + w.row) * p.out_stride[w.which] + w.off;
