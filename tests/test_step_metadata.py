@@ -107,13 +107,17 @@ class Tables:
         full = lambda *shape: t.full(shape, -99, dtype=self.dtype, device="cuda")
         b = len(new)
         out = [full(b, width), full(b), full(b + 1) if sums else None, full(b + 1) if sums else None, full(tokens), full(tokens)]
-        to = (t.full_like(self.lens, -99), t.full_like(self.count, -99)) if apart else (None, None)
+        # apart: True, or "lens" or "count": only those have a tensor of their own to go to
+        to = t.full_like(self.lens, -99) if apart in (True, "lens") else None, t.full_like(self.count, -99) if apart in (True, "count") else None
         before = self.lens.clone(), self.count.clone()
         nvk().step_metadata(self.up(new), None if rows is None else self.up(rows), self.lens, self.held, self.free, self.count, self.bs, self.pool, *out, *to)
         want = self.ref.step(new, rows, width, tokens, self.pool)
-        if apart:
-            assert t.equal(before[0], self.lens) and t.equal(before[1], self.count)
-            self.lens, self.count = to
+        if to[0] is not None:
+            assert t.equal(before[0], self.lens)
+            self.lens = to[0]
+        if to[1] is not None:
+            assert t.equal(before[1], self.count)
+            self.count = to[1]
         for name, got, w in zip(("tables", "ctx", "cu_q", "cu_k", "positions", "slots"), out, want):
             assert got is None or got.tolist() == w, name
         self.same()
@@ -215,6 +219,18 @@ def test_the_largest_batch_and_wide_tables(batch, width, tokens, dtype, apart):
         new = rng.integers(0, 4, batch) if batch > 100 else rng.integers(0, 2000, batch)
         t.step(new.tolist(), (rng.permutation(batch + 1)[:batch]).tolist(), width, tokens, apart)
     t.release(rng.permutation(batch + 1)[:batch].tolist(), None, apart)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,width,tokens", [(7, 9, 30), (250, 40, 600), (90, 2000, 400), (1000, 12, 3000), (1500, 300, 5000)])
+@pytest.mark.parametrize("dtype", ["int64", "int32"])
+@pytest.mark.parametrize("apart", ["lens", "count"])
+def test_only_lengths_or_only_the_count_in_place(batch, width, tokens, dtype, apart):
+    """In one cluster and by many blocks; with blocks for all, then for a few."""
+    rng = np.random.default_rng(batch)
+    t = Tables(rng, batch + 2, width, 4, batch * 2, dtype=dtype)
+    for _ in range(3):
+        t.step(rng.integers(0, 4, batch).tolist(), rng.permutation(batch + 2)[:batch].tolist(), width, tokens, apart)
 
 
 @pytest.mark.gpu
