@@ -65,9 +65,10 @@ template <int WARPS> __device__ __forceinline__ Three scan_block(Three v, Three&
 }
 
 // All blocks of the cluster arrive when they have read what is updated in place, and gone on from its values; the first one, which writes it, waits at its end.  Nothing that
-// one block writes is read by another, so that the barrier need not wait for anybody's writes (it did for 1 us of the 5 that 256 requests took).
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
+// one block writes is read by another, so that the barrier need not wait for anybody's writes (it did for 1 us of the 5 that 256 requests took).  Not the .aligned forms, which a warp
+// has to execute together: its threads come here from loops and branches of their own.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;\n" ::: "memory"); }
 
 // What is known of the requests of a step, in shared memory.
 struct Request {

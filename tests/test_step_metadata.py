@@ -319,3 +319,29 @@ def test_the_binding_refuses(change, word):
     x = {n: torch.zeros(shapes[n], dtype=kind[n], device=device[n]) for n in shapes}
     with pytest.raises(ValueError, match=word):
         nvk().step_metadata(x["new"], None, x["lens"], x["held"], x["free"], x["count"], 16, 64, x["tables"], x["ctx"], x["cu"], None, x["pos"], x["slots"])
+
+
+# ---- the barrier of the cluster ------------------------------------------------------------------------------------------------
+def test_no_barrier_asks_a_warp_to_come_together():
+    """The .aligned forms of the cluster's barrier are undefined where a warp's threads come from loops and branches of their own, as here."""
+    import os
+    import re
+    source = open(os.path.join(os.path.dirname(entry.__file__), "nano-vllm-cpp_b200", "csrc", "step_metadata.cu")).read()
+    forms = re.findall(r"barrier\.cluster\.(?:arrive|wait)[a-z.]*", source)
+    assert len(forms) >= 2 and not any("aligned" in f for f in forms), forms
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("apart", [False, "lens", "count"])
+@pytest.mark.parametrize("batch,rows,width,dtype", [(37, 1003, 13, "int32"), (255, 300, 37, "int64"), (700, 1301, 9, "int32")])
+def test_clusters_with_ragged_work(batch, rows, width, dtype, apart):
+    """Requests, table entries, tokens and rows that leave warps with threads of unequal work before the barrier; steps and releases in turn, in place."""
+    rng = np.random.default_rng(batch)
+    t = Tables(rng, rows, width, 8, 3 * batch, longest=5 * 8, dtype=dtype)
+    for n in range(12):
+        mine = rng.permutation(rows)[:batch]
+        mine[rng.random(batch) < 0.1] = -1
+        new = rng.integers(0, 9, batch) * (rng.random(batch) < 0.7)
+        t.step(new.tolist(), mine.tolist(), width, int(new.sum()) + n, apart)
+        done = rng.permutation(rows)[:int(rng.integers(1, batch))]
+        t.release(done.tolist(), rng.integers(0, 3, len(done)).tolist() if n % 2 else None)
