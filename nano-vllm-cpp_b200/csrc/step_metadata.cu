@@ -64,11 +64,15 @@ template <int WARPS> __device__ __forceinline__ Three scan_block(Three v, Three&
     return warp > 0 ? add_held(before, others) : before;
 }
 
-// All blocks of the cluster arrive when they have read what is updated in place, and gone on from its values; the first one, which writes it, waits at its end.  Nothing that
-// one block writes is read by another, so that the barrier need not wait for anybody's writes (it did for 1 us of the 5 that 256 requests took).  Not the .aligned forms, which a warp
-// has to execute together: its threads come here from loops and branches of their own.
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed;\n" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;\n" ::: "memory"); }
+// All blocks of the cluster arrive when they have read what is updated in place; the first one, which writes it, waits at its end.  The others' reads have to come before its
+// writes, so that they arrive with .release (the wait acquires); they have nothing written by then that this would wait for.  The first block's own arrival orders nothing: what it
+// has written by then nobody of the cluster reads, and to wait for it took 1 us of the 5 of 256 requests; its own reads come before the block's barrier that follows.  Not the .aligned
+// forms, which a warp has to execute together: its threads come here from loops and branches of their own.
+__device__ __forceinline__ void cluster_arrive(bool first_block) {
+    if (first_block) asm volatile("barrier.cluster.arrive.relaxed;\n" ::: "memory");
+    else asm volatile("barrier.cluster.arrive.release;\n" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;\n" ::: "memory"); }
 
 // What is known of the requests of a step, in shared memory.
 struct Request {
@@ -218,7 +222,7 @@ __global__ void __launch_bounds__(THREADS, 1) step_metadata_kernel(const __grid_
     if (first_block && p.new_lens_out != p.lens) {   // (whole; the new ones follow)
         for (int64_t i = tid; i < p.num_rows; i += THREADS) p.new_lens_out[i] = p.lens[i];
     }
-    if (!p.wide && gridDim.x > 1) cluster_arrive();
+    if (!p.wide && gridDim.x > 1) cluster_arrive(first_block);
     __syncthreads();
     // From here on lengths and count are no longer read.
     const uint32_t tokens = s_tokens;
@@ -432,7 +436,7 @@ __global__ void __launch_bounds__(kFewThreads) release_blocks_kernel(const __gri
     if (blockIdx.x == 0 && p.new_lens_out != p.lens) {
         for (int64_t i = tid; i < p.num_rows; i += kFewThreads) p.new_lens_out[i] = p.lens[i];
     }
-    if (gridDim.x > 1) cluster_arrive();
+    if (gridDim.x > 1) cluster_arrive(blockIdx.x == 0);
     __syncthreads();
     const int lane = tid & 31, chunks = static_cast<int>(p.by_chunks.d), units = p.batch * chunks;
     for (int i = me >> 5; i < units; i += threads >> 5) {

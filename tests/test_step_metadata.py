@@ -345,3 +345,35 @@ def test_clusters_with_ragged_work(batch, rows, width, dtype, apart):
         t.step(new.tolist(), mine.tolist(), width, int(new.sum()) + n, apart)
         done = rng.permutation(rows)[:int(rng.integers(1, batch))]
         t.release(done.tolist(), rng.integers(0, 3, len(done)).tolist() if n % 2 else None)
+
+
+def test_reads_of_the_other_blocks_come_before_the_first_ones_writes():
+    """Lengths and count are written in place behind a barrier: whoever reads them has to arrive with release, and the writer to wait with acquire."""
+    import os
+    import re
+    source = open(os.path.join(os.path.dirname(entry.__file__), "nano-vllm-cpp_b200", "csrc", "step_metadata.cu")).read()
+    assert re.search(r"if \(first_block\) asm[^;]*barrier\.cluster\.arrive\.relaxed;[^;]*;\s*else asm[^;]*barrier\.cluster\.arrive\.release;", source)
+    assert "barrier.cluster.wait.acquire;" in source
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["int32", "int64"])
+@pytest.mark.parametrize("batch,width", [(9, 100), (60, 300), (300, 700)])
+def test_many_releases_in_place(batch, width, dtype):
+    """The count and the lengths written by one block of a cluster while the others still work: the same tables over and over, by clusters of 2 to 16 blocks."""
+    import torch
+    rng = np.random.default_rng(width)
+    t = Tables(rng, batch + 3, width, 2, 50, dtype=dtype)
+    done = rng.permutation(batch + 3)[:batch]
+    rows, first = t.up(done), t.up(rng.integers(0, 3, batch))
+    lens, free, count = t.lens.clone(), t.free.clone(), t.count.clone()
+    t.ref.release(done.tolist(), first.tolist())
+    want = t.up(t.ref.lens), t.up(t.ref.free), t.up([t.ref.count])
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(300):
+        t.lens.copy_(lens); t.free.copy_(free); t.count.copy_(count)
+        nvk().release_blocks(rows, first, t.lens, t.held, t.free, t.count, 2)
+        for got, w in zip((t.lens, t.free, t.count), want):
+            wrong += (got != w).sum()
+    assert wrong.item() == 0
+    t.same()
