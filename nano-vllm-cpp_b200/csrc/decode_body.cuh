@@ -933,10 +933,11 @@ struct CacheBlocks8 {
         for (int mt = 0; mt < 8; ++mt) { s.o[mt][0] *= c[0]; s.o[mt][1] *= c[1]; s.o[mt][2] *= c[0]; s.o[mt][3] *= c[1]; }
     }
     // A key's weight; for F16 results rounded to the 11 bits that the MMA takes of it, so that the sum of the weights is that of the rounded ones and a key that has nearly all of
-    // the attention is not off by its rounding (BF16 results are rounded to an eighth of that).
+    // the attention is not off by its rounding (BF16 results are rounded to an eighth of that).  2^13 w + w has 24 bits, what is left of it without 2^13 w the upper 11 of w (ties to
+    // even); sums, and not the bits as whole numbers, so that NaN stays NaN.
     static __device__ __forceinline__ float weight(float x) {
         const float w = fast_exp2(x);
-        return std::is_same<T, __half>::value ? __uint_as_float((__float_as_uint(w) + 0x1000u) & 0xffffe000u) : w;
+        return std::is_same<T, __half>::value ? fmaf(w, -8192.0f, fmaf(w, 8192.0f, w)) : w;
     }
     // What 16 keys add to the sums.
     __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], float v_scale, int lane) {

@@ -683,3 +683,45 @@ def test_a_run_of_steps_from_lengths_to_outputs(kind):
     nvk().release_blocks(torch.tensor([2], dtype=torch.int32, device="cuda"), None, lens, held, free, count, bs)
     book.release([2], None)
     assert free.tolist()[:book.count] == book.free[:book.count] and lens.tolist() == book.lens and count.item() == book.count
+
+
+# ---- values that are not finite, and scales far apart ---------------------------------------------------------------------------
+# Every way of sharing a context out: (Hq, Hkv, sequences, table entries of 64 keys, lengths among them).
+WAYS = {"clusters of eight": (8, 1, 6, 64, [4096, 700, 33]), "clusters, few keys": (8, 2, 4, 5, [300, 1, 20]), "eight warps": (8, 8, 15, 16, [1024, 900, 1]),
+        "eight warps, longest first": (16, 8, 30, 32, [2048, 100, 17]), "halves": (16, 8, 20, 32, [2048, 1025, 31]), "chunks of 768": (2, 1, 200, 64, [4096, 769, 5]),
+        "chunks of 1024": (8, 8, 90, 128, [3000, 1025, 64])}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("which", ["K", "V"])
+def test_a_block_of_nan_reads_as_nan_wherever_it_lies(way, kind, dtype, which):
+    """A scale of NaN, of K alone or of V alone, in a context's first, some or last block: NaN for the sequence and KV head whose it is, and not a bit of the others changes."""
+    rng = np.random.default_rng(len(way))
+    hq, hkv, batch, width, long = WAYS[way]
+    bs, per = 64, hq // hkv
+    lens = (long + [int(x) for x in rng.integers(1, 100, batch)])[:batch]
+    c, tables = _filled(rng, kind, dtype, bs, hkv, lens, width)
+    q, _ = _typed(rng.standard_normal((batch, hq, D)), dtype)
+    before = _decode(c, q, lens, tables)
+    assert np.isfinite(before).all()
+    scale = c.scale["KV".index(which)]
+    for s in range(len(long)):
+        used = -(-lens[s] // bs)
+        for blk in sorted({0, int(rng.integers(0, used)), used - 1}):
+            head = int(rng.integers(0, hkv))
+            block = int(tables[s][blk])
+            was = scale[block, head].clone()
+            scale[block, head] = float("nan")
+            for workspace in (True, False):
+                got = _decode(c, q, lens, tables, workspace=workspace)
+                theirs = np.zeros((batch, hq), bool)
+                theirs[s, head * per:(head + 1) * per] = True
+                assert np.isnan(got[theirs]).all(), (s, blk, head)
+                assert not np.isnan(got[~theirs]).any()
+                if workspace:
+                    assert np.array_equal(got[~theirs], before[~theirs])
+            scale[block, head] = was
+    assert np.array_equal(_decode(c, q, lens, tables), before)
