@@ -228,7 +228,8 @@ int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, cons
  * nvk_decode_attention_paged_blocks8: the semantics of nvk_decode_attention_paged over the values as they are; at most 8 query heads per KV head, block_size a
  * multiple of 16; workspace as there (nvk_decode_attention_workspace_bytes; where more of it is given a context may be shared out into more parts, whose sums differ
  * in their last bits).  Query elements are off by 2^-20 (int8) or 2^-25 (e4m3) of their head's largest, and a head's weight times the scale of the value is
- * rounded to f16: by 2^-11 of itself or 2^-22 of the head's largest such product.  scale must be finite; a query that is not gives NaN.
+ * rounded to f16: by 2^-11 of itself or 2^-22 of the head's largest such product; a weight below 2^-126 of the head's largest is zero.  scale must be finite; a query that is not
+ * gives NaN, and so may a head whose largest query element times scale times the largest key element is beyond fp32.
  */
 int nvk_store_kvcache_blocks8(const void* key, const void* value, int64_t key_row_stride, int64_t value_row_stride, void* k_cache, void* v_cache,
                               float* k_scale, float* v_scale, int cache_dtype, const void* cu_seqlens_q, int cu_seqlens_q_dtype,

@@ -939,12 +939,19 @@ struct CacheBlocks8 {
         const float w = fast_exp2(x);
         return std::is_same<T, __half>::value ? fmaf(w, -8192.0f, fmaf(w, 8192.0f, w)) : w;
     }
+    // s 2^-E for a product with p that must not become 0 times infinity: it passes 2^126 only where every p of its keys is zero, since no p s 2^-E is above 2^8 and no p but
+    // zero below 2^-126.  (Keys that lead all others by 2^126 and have values of nothing, whose s is small; NaN stays NaN.)
+    static __device__ __forceinline__ float at_most(float x) {
+        float y;
+        asm("min.NaN.f32 %0, %1, 0f7E800000;\n" : "=f"(y) : "f"(x));
+        return y;
+    }
     // What 16 keys add to the sums.
     __device__ __forceinline__ void add(uint32_t stage, int row0, const float (&sc)[4], float v_scale, int lane) {
         const float p0 = weight(sc[0] - s.m[0]), p1 = weight(sc[1] - s.m[1]), p2 = weight(sc[2] - s.m[0]), p3 = weight(sc[3] - s.m[1]);
         s.l[0] += p0 + p2;
         s.l[1] += p1 + p3;
-        const float part[2] = {v_scale * down[0], v_scale * down[1]};
+        const float part[2] = {at_most(v_scale * down[0]), at_most(v_scale * down[1])};
         const uint32_t pb0 = transpose_8x8(ElemTraits<__half>::pack2(p0 * part[0], p1 * part[1]));
         const uint32_t pb1 = transpose_8x8(ElemTraits<__half>::pack2(p2 * part[0], p3 * part[1]));
         // V rows of the tile, two d-tiles of 16 at a time

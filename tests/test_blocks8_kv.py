@@ -725,3 +725,40 @@ def test_a_block_of_nan_reads_as_nan_wherever_it_lies(way, kind, dtype, which):
                     assert np.array_equal(got[~theirs], before[~theirs])
             scale[block, head] = was
     assert np.array_equal(_decode(c, q, lens, tables), before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("leader", ["zeros", "outside", "tiny"])
+@pytest.mark.parametrize("lead", [100.0, 131.0, 200.0])
+@pytest.mark.parametrize("at", [0, 1, 6, 39])
+def test_decode_where_all_attention_goes_to_values_of_nothing(kind, dtype, leader, lead, at):
+    """A block whose keys lead all others by 2^lead, with values of zero (a scale of 2^-126), of next to nothing, or outside the cache (a scale of 0): the others' values, of
+    scales that are larger by any factor, come with weights of zero and have to leave nothing behind."""
+    rng = np.random.default_rng(int(lead) + at)
+    bs, hq, hkv, n = 16, 4, 2, 640
+    tables = rng.permutation(42)[:40][None]
+    c = Both(42, bs, hkv, kind)
+    k, v = rng.standard_normal((2, n, hkv, D))
+    mine = slice(at * bs, (at + 1) * bs)
+    k[..., 0] = -16.0
+    k[mine] = 0.0
+    v *= 4000.0
+    v[mine] = 0.0 if leader != "tiny" else 2.0 ** -24 if dtype == "float16" else 2.0 ** -100
+    x = [_typed(k, dtype), _typed(v, dtype)]
+    c.store(x, [0, n], [n], tables.tolist())
+    if leader == "outside":
+        tables[0, at] = -1
+    q = np.zeros((1, hq, D))
+    q[..., 0] = 1.0
+    qd, here = _typed(q, dtype)
+    scale = lead * np.log(2.0) / 16.0
+    want, most = _bound(c, tables[0], n, here[0], scale, dtype)
+    # A weight below 2^-126 of the largest is no number that the exponential gives: it is zero, which takes at most 2^-126 of the sum of magnitudes.  (2^-131 of 4000, as for the lead in between,
+    # is a number of BF16.)
+    most = most + 2.0 ** -126 * np.repeat(np.abs(c.ref[1].rows(tables[0], n)).sum(0), hq // hkv, axis=0)
+    for workspace in (True, False):
+        got = _decode(c, qd, [n], tables, scale=scale, workspace=workspace)[0]
+        assert np.isfinite(got).all()
+        assert (np.abs(got - want) <= most).all()
