@@ -357,8 +357,7 @@ int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
 }
 // 8-bit caches with block scales are shared out like the other 8-bit ones, but in shorter chunks where those have chunks of 1024 or 2048 keys: their tiles take half the time, so that
 // a block's range ends sooner and what is left at the end counts for more.  768 keys up to four pairs to an SM, 1024 up to eight, where the workspace has room for the parts (it is sized for
-// the other caches).  us, as above: 64 pairs of 8192 keys 18.7 / 18.5 / 19.1, 19.9 / 21.3 / 30.6 -> 16.0 / 15.9 / 16.7, 17.5 / 23.7 / 29.7; 256 of 2048 12.1 / 14.7 / 16.7, 16.9 /
-// 21.1 / 31.9 -> 10.8 / 12.9 / 14.3, 16.5 / 22.3 / 28.3; 256 of 4096 13.9 / 16.2 / 20.9, 33.5 / 41.0 / 53.4 -> 12.2 / 14.7 / 19.1, 29.6 / 40.8 / 49.4; 800 of 8192 40.2 / 57.5 / 109.4, 154.0 /
+// the other caches).  us, as above: 64 pairs of 8192 keys 18.7 / 18.5 / 19.1, 19.9 / 21.3 / 30.6 -> 16.0 / 15.9 / 16.7, 17.5 / 23.7 / 29.7; 256 of 4096 13.9 / 16.2 / 20.9, 33.5 / 41.0 / 53.4 -> 12.2 / 14.7 / 19.1, 29.6 / 40.8 / 49.4; 800 of 8192 40.2 / 57.5 / 109.4, 154.0 /
 // 209.6 / 263.5 -> 36.7 / 55.4 / 104.9, 148.6 / 204.7 / 260.9; but 2048 of 8192 65.8 / 116.5 / 251.6, 364.6 / 510.0 / 655.4 -> 68.3 / 119.6 / 254.5, 366.2 / 502.0 / 686.5.
 // Tables of 1024 to 2048 keys beyond the clusters of four: whole contexts by blocks of eight warps, one to an SM, with more pairs than SMs the longest first; between one and one and a half
 // pairs to an SM, where a second wave of those would be nearly empty, the halves of a table row, which 8-bit caches otherwise have up to 1536 keys.  us with inputs beyond L2: 120 pairs of 2048
@@ -366,8 +365,11 @@ int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
 // 1024 10.6 / 11.9 / 14.4, 15.2 / 19.1 / 22.2 -> 8.7 / 9.2 / 13.2, 14.6 / 17.1 / 19.4; 160 of 2048 10.2 / 13.1 / 14.6, 15.6 / 21.6 / 24.3 -> 10.0 / 13.2 / 15.9, 16.0 / 17.0 / 18.2 (by eight
 // warps 12.5 / 13.6 / 14.2, 14.4 / 20.8 / 27.9); but 384 of 2048 by four warps 18.8 / 21.7 / 28.8, 27.6 / 31.9 / 37.0, by eight 14.0 / 16.7 / 23.1, 28.7 / 35.4 / 43.3.
 bool halves_of_block_scales(int64_t pairs, int64_t max_tokens) { return pairs > kSmCount && 2 * pairs <= 3 * kSmCount && max_tokens >= 1024 && max_tokens <= 2048; }
+// From two pairs to an SM on, where tables of up to 1280 keys are whole contexts by four warps anyway, three blocks to an SM, they stay that, for what one context in three that fills its
+// table costs: 296 of 1024 by eight 12.0 / 14.4 / 15.2, 15.9 / 18.6 / 21.0, by four 10.1 / 13.5 / 16.2, 15.9 / 16.7 / 17.3; 320 12.6 / 14.8 / 15.5, 19.9 / 24.5 / 28.4 and 9.8 / 13.4 / 16.3,
+// 16.1 / 16.9 / 17.6; 320 of 1280 12.7 / 15.0 / 16.4, 21.2 / 26.8 / 32.6 and 11.5 / 15.8 / 19.2, 18.7 / 19.7 / 20.8.
 bool eight_warps_of_block_scales(int64_t pairs, int64_t max_tokens) {
-    return !halves_of_block_scales(pairs, max_tokens) && max_tokens >= 1024 && max_tokens <= 2048 && pairs <= 320;
+    return !halves_of_block_scales(pairs, max_tokens) && max_tokens >= 1024 && max_tokens <= 2048 && pairs <= 320 && (pairs < 2 * kSmCount || max_tokens > 1280);
 }
 int chunk_of_block_scales(int64_t pairs, int64_t max_tokens, int chunk, int block_size) {
     if (chunk < 1024 || max_tokens <= chunk || pairs > 8 * kSmCount) return chunk;

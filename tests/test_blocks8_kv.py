@@ -762,3 +762,19 @@ def test_decode_where_all_attention_goes_to_values_of_nothing(kind, dtype, leade
         got = _decode(c, qd, [n], tables, scale=scale, workspace=workspace)[0]
         assert np.isfinite(got).all()
         assert (np.abs(got - want) <= most).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [("int8", "bfloat16"), ("e4m3", "float16")])
+@pytest.mark.parametrize("hq,hkv,batch,width", [(4, 1, 296, 16), (2, 1, 320, 20), (16, 8, 38, 18)])
+def test_whole_contexts_with_and_without_a_workspace(kind, dtype, hq, hkv, batch, width):
+    """Two pairs to an SM and more, tables of 1024 to 1280 keys: whole contexts, in the same order of sums whether a workspace is there or not (contexts of more than 64 keys: shorter ones are
+    dealt to the warps otherwise in clusters)."""
+    rng = np.random.default_rng(batch)
+    bs = 64
+    lens = [int(x) for x in rng.integers(65, 300, batch)]
+    lens[:2] = [width * bs, width * bs - 5]
+    c, tables = _filled(rng, kind, dtype, bs, hkv, lens, width)
+    q, here = _typed(rng.standard_normal((batch, hq, D)) * 2.0, dtype)
+    full = _check_decode(c, q, here, lens, tables, dtype)
+    assert np.array_equal(full, _decode(c, q, lens, tables, workspace=False))
