@@ -79,6 +79,15 @@ bool written_twice(std::initializer_list<Range> written, std::initializer_list<R
     }
     return false;
 }
+// `rows` rows of `row` bytes, `stride` bytes from each to the next.  Whether two such share a byte: told apart by their ends, and with one stride by the columns that they take.
+struct Rows { const void* at; int64_t stride, row, rows; };
+bool rows_overlap(const Rows& a, const Rows& b) {
+    if (a.at == nullptr || b.at == nullptr) return false;
+    if (!overlap(a.at, (a.rows - 1) * a.stride + a.row, b.at, (b.rows - 1) * b.stride + b.row)) return false;
+    if (a.stride != b.stride) return true;
+    const int64_t apart = static_cast<const char*>(b.at) - static_cast<const char*>(a.at), column = (apart % a.stride + a.stride) % a.stride;   // where b's columns begin after a's
+    return column < a.row || column + b.row > a.stride;
+}
 // What the calls over the tables of requests have in common.
 int check_requests(const char* what, const void* lens, const void* blocks, const void* free_blocks, const void* count, const void* new_lens, const void* new_count,
                    int64_t batch, int64_t rows, int64_t row_blocks, int64_t num_free, int block_size, const void* request_rows, int index_dtype) {
@@ -505,22 +514,32 @@ int nvk_rotary_embedding(const void* query, const void* key, const void* positio
     if (head_dim > 1024) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: head_dim must be at most 1024 (got %d)", head_dim);
     if (num_q_heads > (1 << 19) || (key && num_kv_heads > (1 << 19))) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: too many heads");
     const int64_t size = static_cast<int64_t>(dtype_size(dtype));
-    auto check = [&](const void* in, int64_t in_stride, const void* out, int64_t out_stride, int heads) -> int {
-        const int64_t row = static_cast<int64_t>(heads) * head_dim;
-        if (in_stride < row || out_stride < row) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: a row stride is less than a row");
-        if (!aligned_to(in, static_cast<size_t>(size)) || !aligned_to(out, static_cast<size_t>(size))) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: misaligned tensor");
-        const int64_t last = rows > 0 ? rows - 1 : 0;
-        if ((in != out || in_stride != out_stride) && rows > 0 && overlap(in, (last * in_stride + row) * size, out, (last * out_stride + row) * size))
-            return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: an output is its input, with its stride, or does not overlap with it");
+    auto check = [&](const void* at, int64_t stride, int heads) -> int {
+        if (stride < static_cast<int64_t>(heads) * head_dim) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: a row stride is less than a row");
+        if (!aligned_to(at, static_cast<size_t>(size))) return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: misaligned tensor");
+        if (stride > (1LL << 40) || rows > (1LL << 56) / stride) return fail(NVK_ERR_UNSUPPORTED, "rotary_embedding: too many rows");
         return NVK_OK;
     };
-    if (const int rc = check(query, query_row_stride, query_out, query_out_row_stride, num_q_heads); rc != NVK_OK) return rc;
+    if (const int rc = check(query, query_row_stride, num_q_heads); rc != NVK_OK) return rc;
+    if (const int rc = check(query_out, query_out_row_stride, num_q_heads); rc != NVK_OK) return rc;
     if (key) {
-        if (const int rc = check(key, key_row_stride, key_out, key_out_row_stride, num_kv_heads); rc != NVK_OK) return rc;
+        if (const int rc = check(key, key_row_stride, num_kv_heads); rc != NVK_OK) return rc;
+        if (const int rc = check(key_out, key_out_row_stride, num_kv_heads); rc != NVK_OK) return rc;
     }
     if (!aligned_to(positions, static_cast<size_t>(index_bytes(positions_dtype))) || !aligned_to(inv_freq, 4))
         return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: misaligned tensor");
     if (rows == 0) return NVK_OK;
+    {   // an output may be its own input, row for row, and a part of the packed rows that its input is another part of
+        const int64_t q_row = static_cast<int64_t>(num_q_heads) * head_dim * size, k_row = key ? static_cast<int64_t>(num_kv_heads) * head_dim * size : 0;
+        const Rows q{query, query_row_stride * size, q_row, rows}, k{key, key_row_stride * size, k_row, rows};
+        const Rows q_out{query_out, query_out_row_stride * size, q_row, rows}, k_out{key_out, key_out_row_stride * size, k_row, rows};
+        const int64_t positions_bytes = rows * index_bytes(positions_dtype), freq_bytes = rotary_dim / 2 * static_cast<int64_t>(sizeof(float));
+        const Rows pos{positions, positions_bytes, positions_bytes, 1}, freq{inv_freq, freq_bytes, freq_bytes, 1};
+        auto same = [](const Rows& a, const Rows& b) { return a.at == b.at && (a.stride == b.stride || a.rows == 1); };
+        if ((!same(q, q_out) && rows_overlap(q, q_out)) || (!same(k, k_out) && rows_overlap(k, k_out)) || rows_overlap(q_out, k) || rows_overlap(k_out, q) ||
+            rows_overlap(q_out, k_out) || rows_overlap(q_out, pos) || rows_overlap(k_out, pos) || rows_overlap(q_out, freq) || rows_overlap(k_out, freq))
+            return fail(NVK_ERR_INVALID_ARGUMENT, "rotary_embedding: an output is its input, with its stride, or does not overlap with any tensor of the call");
+    }
     return launch_rotary(RotaryArgs{query, key, query_out, key_out, query_row_stride, key_row_stride, query_out_row_stride, key_out_row_stride,
                                     index_array(positions, positions_dtype), inv_freq, attention_factor, rows, num_q_heads, num_kv_heads, head_dim, rotary_dim,
                                     interleaved != 0, dtype, static_cast<cudaStream_t>(stream)});

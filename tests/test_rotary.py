@@ -214,3 +214,62 @@ def test_the_binding_refuses(change, word):
         nvk().rotary_embedding(x["q"], x["key"], x["pos"], x["f"], query_out=x["q_out"], key_out=x["key_out"])
     with pytest.raises(ValueError, match="contiguous rows"):
         nvk().rotary_embedding(torch.zeros(4, 64, 4, device="cuda").transpose(1, 2), None, torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(32, device="cuda"))
+
+
+# ---- tensors of a call that overlap ----------------------------------------------------------------------------------------------
+def _at(n):
+    return ctypes.c_void_p(n)
+
+
+@pytest.mark.parametrize("change", [
+    dict(qo=_at(1 << 22)), dict(qo=_at((1 << 22) + 512)), dict(ko=_at(1 << 20)), dict(ko=_at(1 << 24)), dict(ko=_at((1 << 24) + 6 * 1024)), dict(qo=_at(1 << 26)), dict(ko=_at((1 << 26) - 512)),
+    dict(qo=_at(1 << 27)), dict(ko=_at((1 << 27) - 1024)), dict(q=_at(1 << 25), qo=_at(1 << 25)),
+    # columns of one packed row: queries 0 .. 1023, keys 1024 .. 1279, of 1536
+    dict(q=_at(1 << 20), k=_at((1 << 20) + 2048), qo=_at((1 << 20) + 2048), ko=_at((1 << 20) + 2048), packed=True),
+    dict(q=_at(1 << 20), k=_at((1 << 20) + 2048), qo=_at(1 << 20), ko=_at((1 << 20) + 2040), packed=True),
+    dict(q=_at(1 << 20), k=_at((1 << 20) + 2048), qo=_at((1 << 20) + 1040), ko=_at((1 << 20) + 2048), packed=True),
+    dict(q=_at((1 << 20) + 3072), k=_at((1 << 20) + 3072 + 2048), qo=_at((1 << 20) + 3072), ko=_at((1 << 20) + 2560 + 256), packed=True)])
+def test_refuses_outputs_over_other_tensors(built, change):
+    """Queries' output over the keys, keys' output over the queries or their output, either over positions or frequencies, in whole or in part."""
+    a = dict(q=_at(1 << 20), k=_at(1 << 22), pos=_at(1 << 26), pos_dtype=I(3), f=_at(1 << 27), factor=ctypes.c_float(1.0), rows=L(4), hq=I(8), hkv=I(2), d=I(128), rot=I(128), pairs=I(0),
+             q_stride=L(1024), k_stride=L(256), qo=Q, ko=_at(1 << 25), qo_stride=L(1024), ko_stride=L(256), dtype=I(1), stream=None)
+    change = dict(change)
+    if change.pop("packed", False):
+        a.update(dict.fromkeys(("q_stride", "k_stride", "qo_stride", "ko_stride"), L(1536)))
+    a.update(change)
+    rc = built.lib().nvk_rotary_embedding(*a.values())
+    said = built.lib().nvk_last_error().decode()
+    assert rc == 1 and "overlap" in said, said
+
+
+@pytest.mark.parametrize("change", [dict(rows=L(1 << 50)), dict(q_stride=L(1 << 41)), dict(ko_stride=L(1 << 60))])
+def test_refuses_rows_beyond_memory(built, change):
+    a = dict(q=_at(1 << 20), k=_at(1 << 22), pos=_at(1 << 26), pos_dtype=I(3), f=_at(1 << 27), factor=ctypes.c_float(1.0), rows=L(4), hq=I(8), hkv=I(2), d=I(128), rot=I(128), pairs=I(0),
+             q_stride=L(1024), k_stride=L(256), qo=Q, ko=_at(1 << 25), qo_stride=L(1024), ko_stride=L(256), dtype=I(1), stream=None)
+    a.update(change)
+    assert built.lib().nvk_rotary_embedding(*a.values()) == 3 and "too many rows" in built.lib().nvk_last_error().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 37])
+def test_outputs_beside_their_inputs_in_packed_rows(rows):
+    """Other columns of the same packed rows are no overlap; nor is the queries' output in place with the keys' elsewhere."""
+    import torch
+    rng = np.random.default_rng(rows)
+    hq, hkv, d = 4, 2, 64
+    n = (hq + hkv) * d
+    base = torch.from_numpy(rng.standard_normal((rows, 2 * n + 16))).to(torch.bfloat16).cuda()
+    part = lambda a, heads: base[:, a:a + heads * d].unflatten(1, (heads, d))
+    q, k, qo, ko = part(0, hq), part(hq * d, hkv), part(n + 8, hq), part(n + 8 + hq * d, hkv)
+    pos = torch.from_numpy(rng.integers(0, 1 << 16, rows)).cuda()
+    f = torch.tensor(nvk().rotary_inv_freq(d, 10000.0)[0], device="cuda")
+    apart = torch.empty_like(q.contiguous()), torch.empty_like(k.contiguous())
+    nvk().rotary_embedding(q, k, pos, f, query_out=apart[0], key_out=apart[1])
+    kept = base.clone()
+    nvk().rotary_embedding(q, k, pos, f, query_out=qo, key_out=ko)
+    assert torch.equal(qo, apart[0]) and torch.equal(ko, apart[1])
+    assert torch.equal(base[:, :n + 8], kept[:, :n + 8]) and torch.equal(base[:, 2 * n + 8:], kept[:, 2 * n + 8:])
+    nvk().rotary_embedding(q, k, pos, f, key_out=ko)
+    assert torch.equal(q, apart[0]) and torch.equal(ko, apart[1]) and torch.equal(k, kept[:, hq * d:n].unflatten(1, (hkv, d)))
+    with pytest.raises(ValueError, match="overlap"):
+        nvk().rotary_embedding(q, k, pos, f, query_out=q, key_out=q[:, 1:1 + hkv])
