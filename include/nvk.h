@@ -221,6 +221,8 @@ int nvk_decode_attention_paged_int4(const void* query, const void* k_cache, cons
  * before the others (rows of a block behind the call's last one may be stored again later: they are left as they were, in the old scale).  No two sequences of a call
  * write to the same block.
  *
+ * What one of the three calls writes overlaps with no other tensor of the call (NVK_ERR_INVALID_ARGUMENT), but the output of decode may be the query.
+ *
  * nvk_gather_kvcache_blocks8: the keys and values of whole contexts as dense 16-bit rows, as nvk_gather_kvcache_int4: row cu_seqlens_k[s] + i of key / value
  * [total_k, num_kv_heads, 128] is key i of sequence s, rounded to `dtype`.  Rows behind the last sequence and rows whose table entry is outside the cache or the
  * table are zeros.

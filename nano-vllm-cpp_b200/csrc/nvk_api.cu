@@ -3,6 +3,7 @@
 // src/kernels/kernel_types.cu:24-110) and dispatch to the kernels of this library.
 #include "nvk_internal.cuh"
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <string>
@@ -63,6 +64,7 @@ int check_blocks8(const char* what, int dtype, int cache_dtype, int num_kv_heads
     if (cache_dtype != NVK_I8 && cache_dtype != NVK_E4M3) return fail(NVK_ERR_INVALID_ARGUMENT, "%s: cache elements are int8 or e4m3", what);
     return check_int4(what, dtype, num_kv_heads, head_dim);
 }
+constexpr int64_t kMostBytes = 1LL << 60;   // of a tensor: sizes are held below it before they are multiplied
 // Neither the same nor apart.
 bool partly(const void* a, const void* b, int64_t bytes) { return a != b && overlap(a, bytes, b, bytes); }
 // Memory that a call writes, or only reads.
@@ -382,6 +384,14 @@ int nvk_store_kvcache_blocks8(const void* key, const void* value, int64_t key_ro
     if (num_seqs > (1LL << 30) / num_kv_heads || total_q >= (1LL << 31) - block_size || max_blocks > ((1LL << 31) - 1) / block_size || num_kv_heads > (1 << 24))
         return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many sequences, tokens, heads or blocks");
     if (num_seqs == 0 || total_q == 0) return NVK_OK;
+    if (num_cache_blocks > kMostBytes / row / block_size || num_seqs > kMostBytes / 8 / max_blocks || key_row_stride > kMostBytes / 2 / total_q || value_row_stride > kMostBytes / 2 / total_q)
+        return fail(NVK_ERR_UNSUPPORTED, "store_kvcache_blocks8: too many cache blocks or table entries, or rows too far apart");
+    const int64_t cache = num_cache_blocks * block_size * row, scales = num_cache_blocks * num_kv_heads * 4;
+    if (written_twice({{k_cache, cache}, {v_cache, cache}, {k_scale, scales}, {v_scale, scales}},
+                      {{key, ((total_q - 1) * key_row_stride + row) * 2}, {value, ((total_q - 1) * value_row_stride + row) * 2},
+                       {cu_seqlens_q, (num_seqs + 1) * index_bytes(cu_seqlens_q_dtype)}, {context_lens, num_seqs * index_bytes(context_lens_dtype)},
+                       {block_tables, num_seqs * max_blocks * index_bytes(block_tables_dtype)}}))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "store_kvcache_blocks8: a cache or its scales overlap with another tensor");
     return launch_store_blocks8(Blocks8StoreArgs{key, value, k_cache, v_cache, k_scale, v_scale, index_array(cu_seqlens_q, cu_seqlens_q_dtype),
                                                  index_array(context_lens, context_lens_dtype), index_array(block_tables, block_tables_dtype), num_seqs, total_q,
                                                  max_blocks, num_cache_blocks, key_row_stride, value_row_stride, num_kv_heads, block_size,
@@ -402,7 +412,16 @@ int nvk_gather_kvcache_blocks8(const void* k_cache, const void* v_cache, const f
     if (!aligned_to(key, 16) || !aligned_to(value, 16) || !aligned_to(k_cache, 16) || !aligned_to(v_cache, 16) || !aligned_to(k_scale, 4) || !aligned_to(v_scale, 4))
         return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: key, value and the caches must be 16-byte aligned, the scales 4-byte aligned");
     if (max_blocks > ((1LL << 31) - 1) / block_size) return fail(NVK_ERR_UNSUPPORTED, "gather_kvcache_blocks8: too many blocks");
+    const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
     if (total_k == 0) return NVK_OK;
+    if (total_k > (1LL << 38) || total_k > kMostBytes / 2 / row) return fail(NVK_ERR_UNSUPPORTED, "gather_kvcache_blocks8: too many rows");
+    if (num_cache_blocks > kMostBytes / row / block_size || num_seqs > kMostBytes / 8 / max_blocks)
+        return fail(NVK_ERR_UNSUPPORTED, "gather_kvcache_blocks8: too many cache blocks or table entries");
+    const int64_t cache = num_cache_blocks * block_size * row, scales = num_cache_blocks * num_kv_heads * 4;
+    if (written_twice({{key, total_k * row * 2}, {value, total_k * row * 2}},
+                      {{k_cache, cache}, {v_cache, cache}, {k_scale, scales}, {v_scale, scales}, {cu_seqlens_k, (num_seqs + 1) * index_bytes(cu_seqlens_k_dtype)},
+                       {block_tables, num_seqs * max_blocks * index_bytes(block_tables_dtype)}}))
+        return fail(NVK_ERR_INVALID_ARGUMENT, "gather_kvcache_blocks8: key or value overlaps with another tensor");
     return launch_gather_blocks8(Blocks8GatherArgs{k_cache, v_cache, k_scale, v_scale, index_array(cu_seqlens_k, cu_seqlens_k_dtype),
                                                    index_array(block_tables, block_tables_dtype), num_seqs, total_k, max_blocks, num_cache_blocks, num_kv_heads,
                                                    block_size, cache_dtype == NVK_E4M3, key, value, dtype, static_cast<cudaStream_t>(stream)});
@@ -432,6 +451,14 @@ int nvk_decode_attention_paged_blocks8(const void* query, const void* k_cache, c
         if (workspace_bytes < need)
             return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): workspace of %zu bytes given, %zu needed", workspace_bytes, need);
         if (!aligned_to(workspace, 16)) return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): workspace must be 16-byte aligned");
+    }
+    if (batch < (1LL << 28) / num_heads) {   // (the launch refuses more; the output may be the query: a head's is written when all have read it)
+        const int64_t rows = batch * num_heads * head_dim * 2, room = static_cast<int64_t>(std::min<size_t>(workspace_bytes, kMostBytes)), cache = num_cache_blocks * block_size * num_kv_heads * head_dim, scales = num_cache_blocks * num_kv_heads * 4;
+        const Range lens{context_lens, batch * index_bytes(context_lens_dtype)}, tables{block_tables, batch * max_blocks * index_bytes(block_tables_dtype)};
+        const Range q{query, query == output ? 0 : rows};
+        if (written_twice({{output, rows}, {workspace, room}}, {q, {k_cache, cache}, {v_cache, cache}, {k_scale, scales}, {v_scale, scales}, lens, tables}) ||
+            (workspace != nullptr && overlap(workspace, room, query, rows)))
+            return fail(NVK_ERR_INVALID_ARGUMENT, "decode attention (blocks8): output or workspace overlaps with another tensor");
     }
     return launch_decode_blocks8(a, k_scale, v_scale, cache_dtype == NVK_E4M3);
 }

@@ -778,3 +778,85 @@ def test_whole_contexts_with_and_without_a_workspace(kind, dtype, hq, hkv, batch
     q, here = _typed(rng.standard_normal((batch, hq, D)) * 2.0, dtype)
     full = _check_decode(c, q, here, lens, tables, dtype)
     assert np.array_equal(full, _decode(c, q, lens, tables, workspace=False))
+
+
+# ---- tensors of a call that overlap, on the CPU -----------------------------------------------------------------------------------
+AT = {name: ctypes.c_void_p((i + 1) << 40) for i, name in enumerate(("key", "value", "k_cache", "v_cache", "k_scale", "v_scale", "cu", "ctx", "bt", "q", "out", "ws"))}   # (nothing is read there)
+
+
+def _apart(args, **change):
+    """The call's arguments with every tensor at a place of its own, then the change."""
+    a = dict(args)
+    a.update({n: p for n, p in AT.items() if n in a and a[n] is not None})
+    a.update(change)
+    return a.values()
+
+
+def _named(build, names):
+    return dict(zip(names, build()))
+
+
+STORE = "key value ks vs k_cache v_cache k_scale v_scale kind cu cu_dtype ctx ctx_dtype bt bt_dtype seqs total max_blocks blocks hkv d bs dtype stream".split()
+GATHER = "k_cache v_cache k_scale v_scale kind cu cu_dtype bt bt_dtype seqs total max_blocks blocks hkv d bs key value dtype stream".split()
+DECODE = "q k_cache v_cache k_scale v_scale kind ctx ctx_dtype bt bt_dtype batch max_blocks blocks hq hkv d bs scale out dtype ws ws_bytes stream".split()
+
+
+def _by(name, more=0):
+    return ctypes.c_void_p(AT[name].value + more)
+
+
+@pytest.mark.parametrize("change", [
+    dict(v_cache=_by("k_cache")), dict(v_cache=_by("k_cache", 4 * 16 * 256 - 16)), dict(v_scale=_by("k_scale", 28)), dict(k_scale=_by("k_cache", 64)), dict(key=_by("v_cache", 32)),
+    dict(value=_by("k_cache", 4 * 16 * 256 - 16)), dict(cu=_by("k_scale", 4)), dict(ctx=_by("v_scale")), dict(bt=_by("k_cache", 8)), dict(k_cache=_by("key", 4 * 512 + 496)),
+    dict(ks=L(1024), k_cache=_by("key", 4 * 2048))])
+def test_store_refuses_caches_over_other_tensors(built, change):
+    rc, said = _call(built, "nvk_store_kvcache_blocks8", *_apart(_named(_store_args, STORE), **change))
+    assert rc == 1 and "overlap" in said, said
+
+
+@pytest.mark.parametrize("change", [
+    dict(value=_by("key")), dict(value=_by("key", 10 * 512 - 16)), dict(key=_by("k_cache", 16)), dict(value=_by("v_scale")), dict(cu=_by("key", 4)), dict(bt=_by("value", 10 * 512 - 8))])
+def test_gather_refuses_rows_over_other_tensors(built, change):
+    rc, said = _call(built, "nvk_gather_kvcache_blocks8", *_apart(_named(_gather_args, GATHER), **change))
+    assert rc == 1 and "overlap" in said, said
+
+
+@pytest.mark.parametrize("change", [
+    dict(out=_by("k_cache", 256)), dict(out=_by("q", 8)), dict(out=_by("v_scale", 8)), dict(ctx=_by("out", 4)), dict(bt=_by("out")), dict(ws=AT["ws"], ws_bytes=ctypes.c_size_t(1 << 41)),
+    dict(ws=AT["ws"], ws_bytes=ctypes.c_size_t(1 << 30), q=_by("ws", 1024)), dict(ws=AT["ws"], ws_bytes=ctypes.c_size_t(1 << 30), out=_by("ws", 1024), bt=_by("ws", 1 << 31))])
+def test_decode_refuses_outputs_over_other_tensors(built, change):
+    change = dict(change)
+    if change.get("ws_bytes") is not None and change["ws_bytes"].value == 1 << 41:   # (a workspace that reaches to the tables)
+        change["bt"] = _by("ws", (1 << 40) + 64)
+    rc, said = _call(built, "nvk_decode_attention_paged_blocks8", *_apart(_named(_decode_args, DECODE), **change))
+    assert rc == 1 and "overlap" in said, said
+
+
+@pytest.mark.parametrize("call,change", [
+    ("nvk_store_kvcache_blocks8", dict(blocks=L(1 << 50))), ("nvk_store_kvcache_blocks8", dict(ks=L(1 << 60))), ("nvk_store_kvcache_blocks8", dict(seqs=L(1 << 29), max_blocks=L(1 << 30), bs=I(1))),
+    ("nvk_gather_kvcache_blocks8", dict(blocks=L(1 << 50))), ("nvk_gather_kvcache_blocks8", dict(seqs=L(1 << 40), max_blocks=L(1 << 26)))])
+def test_sizes_beyond_memory_are_refused(built, call, change):
+    names, build = (STORE, _store_args) if "store" in call else (GATHER, _gather_args)
+    rc, said = _call(built, call, *_apart(_named(build, names), **change))
+    assert rc == 3 and "too many" in said, said
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,dtype", [("int8", "bfloat16"), ("e4m3", "float16")])
+@pytest.mark.parametrize("way", WAYS)
+def test_decode_into_the_query(way, kind, dtype):
+    """The output may be the query itself, however contexts are shared out."""
+    import torch
+    rng = np.random.default_rng(len(way))
+    hq, hkv, batch, width, long = WAYS[way]
+    lens = (long + [int(x) for x in rng.integers(0, 100, batch)])[:batch]
+    c, tables = _filled(rng, kind, dtype, 64, hkv, lens, width)
+    q, _ = _typed(rng.standard_normal((batch, hq, D)), dtype)
+    want = _decode(c, q, lens, tables)
+    up = lambda v: torch.as_tensor(np.asarray(v), dtype=torch.int32).cuda()
+    ws = torch.empty(max(16, nvk().decode_attention_workspace_bytes(batch, hq, hkv, D, width, 64)), dtype=torch.uint8, device="cuda")
+    n, bt = up(lens), up(tables)
+    for _ in range(20):
+        x = q.clone()
+        nvk().launch_decode_attention_paged_blocks8(x, *c.data, *c.scale, n, bt, hkv, D, 64, 0.09, x, ws)
+        assert np.array_equal(x.double().cpu().numpy(), want)
