@@ -292,7 +292,8 @@ int nvk_release_blocks(const void* request_rows, const void* first_blocks, const
  *   query [rows, num_q_heads, head_dim], key [rows, num_kv_heads, head_dim] (NULL: queries alone), rows a row stride (elements) apart, heads contiguous: parts
  *   of packed projections as they are.  query_out, key_out likewise; each may be its input with the same stride (in place), otherwise an
  *   output overlaps with no tensor of the call (NVK_ERR_INVALID_ARGUMENT; parts of packed rows of one stride are told apart by their columns).
- *   positions [rows] int32 / int64, any number; inv_freq fp32 [rotary_dim / 2] on the device.  Angles are taken in 64 bits: as exact for position 2^31 as for 1.
+ *   positions [rows] int32 / int64, any number; inv_freq fp32 [rotary_dim / 2] on the device.  Angles are off by 2^-26 of a turn before sine and cosine, for position
+ *   2^53 as for 1.
  *   F16, BF16 or F32; head_dim up to 1024.  Widest loads where head_dim, rotary_dim / 2, strides and addresses are multiples of 16 bytes.
  *
  * nvk_rotary_inv_freq fills inv_freq (HOST memory, rotary_dim / 2 numbers) and *attention_factor for a context that was stretched by `factor` >= 1 beyond the

@@ -5,9 +5,9 @@
 // with pairs (i, i + rot / 2) or (2i, 2i + 1) of the first `rot` elements; the others are copied.  The reference rotates whole heads by halves
 // (src/kernels/split_qkv.cu:62-154).
 //
-// Far out in a long context position * frequency has no bits left for the angle in 32 bits (position 2^20: off by up to 1/16), so the turns are taken in 64
-// bits, and only their fraction goes on to sincospi in 32: off by 2^-53 of the number of turns, and by 2^-25 of a turn.  A row's angles are worked out once for all its
-// heads: a handful of 64-bit operations for each pair of a row, next to Hq + Hkv times as many elements.
+// Far out in a long context position * frequency has no bits left for the angle in 32 bits (position 2^20: off by up to 1/16), nor, further out, in 64 (2^40: by 2^-13 of a turn).  So the
+// turns are taken as the sum of two 64-bit numbers, off by some 2^-104 of themselves, and only their fraction goes on to sincospi in 32: off by 2^-26 of a turn, whatever the position up to
+// 2^53.  A row's angles are worked out once for all its heads: a handful of 64-bit operations for each pair of a row, next to Hq + Hkv times as many elements.
 //
 // Bound by HBM for many rows (every element is read and written once), by the trip to memory and the launch for few.  A thread takes two pieces of V elements of a head, i and rot / 2 + i,
 // which hold V pairs whole in either layout, and the lanes' pieces lie next to each other (pairs of neighbours in two pieces next to each other: 59.2 instead of 53.9 us below, in F32 56.3 instead
@@ -113,9 +113,12 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_consta
     }
     for (int i = threadIdx.x; i < rows * half; i += kThreads) {
         const int r = static_cast<int>(p.by_pairs.div(i)), pair = i - r * half;
-        // (1 / 2 pi rounded to 64 bits: with the product's rounding 2^-52 of the turns)
-        const double turns = static_cast<double>(p.positions[row0 + r]) * (static_cast<double>(p.inv_freq[pair]) * 0.15915494309189535);
-        const float part = static_cast<float>(turns - rint(turns));
+        // Turns as the sum of two numbers of 64 bits: the frequency's turns for a position, then for this one.
+        constexpr double kTurn = 0.15915494309189535, kTurnRest = -9.839338337591243e-18;   // 1 / 2 pi
+        const double f = static_cast<double>(p.inv_freq[pair]), at = static_cast<double>(p.positions[row0 + r]);
+        const double each = f * kTurn, each_rest = fma(f, kTurnRest, fma(f, kTurn, -each));
+        const double turns = at * each, rest = fma(at, each_rest, fma(at, each, -turns));
+        const float part = static_cast<float>((turns - rint(turns)) + rest);
         float s, c;
         sincospif(2.0f * part, &s, &c);
         s_cos[i] = c * p.factor;

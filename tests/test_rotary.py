@@ -273,3 +273,30 @@ def test_outputs_beside_their_inputs_in_packed_rows(rows):
     assert torch.equal(q, apart[0]) and torch.equal(ko, apart[1]) and torch.equal(k, kept[:, hq * d:n].unflatten(1, (hkv, d)))
     with pytest.raises(ValueError, match="overlap"):
         nvk().rotary_embedding(q, k, pos, f, query_out=q, key_out=q[:, 1:1 + hkv])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("position", [1, 2 ** 24 + 1, 2 ** 31 - 1, 2 ** 40 + 12345, -(2 ** 33) - 7, 2 ** 52 + 1, -(2 ** 53) + 1])
+@pytest.mark.parametrize("pairs", [False, True])
+def test_angles_far_out_are_as_exact_as_near(position, pairs):
+    """The same bound at every position up to 2^53, the one of the tests above: 2^-26 of a turn for the fraction in 32 bits and what sincospi and the products add; nothing that grows with
+    the position (2^53 turns to 2^-104 of themselves are off by 2^-51)."""
+    import decimal
+
+    import torch
+    rng = np.random.default_rng(3)
+    x = torch.from_numpy(rng.standard_normal((1, 3, 64))).float().cuda()
+    f = [1.0, 0.5, 2.0 ** -7, 0.1, 1 / 3, 0.7071, 1.2345e-4, 0.9999] * 4
+    fd = torch.tensor(f, dtype=torch.float32, device="cuda")
+    out = torch.empty_like(x)
+    nvk().rotary_embedding(x, None, torch.tensor([position], device="cuda"), fd, pairs, query_out=out)
+    with decimal.localcontext() as ctx:
+        ctx.prec = 100
+        turn = 2 * decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+        angle = np.array([float((decimal.Decimal(position) * decimal.Decimal(v)).remainder_near(turn)) for v in fd.double().tolist()])
+    c, s = np.cos(angle), np.sin(angle)
+    y = x.double().cpu().numpy()
+    a, b = (y[..., 0::2], y[..., 1::2]) if pairs else (y[..., :32], y[..., 32:])
+    first, second = a * c - b * s, b * c + a * s
+    want = np.stack([first, second], -1).reshape(y.shape) if pairs else np.concatenate([first, second], -1)
+    assert (np.abs(out.double().cpu().numpy() - want) <= _tolerance(want, np.abs(y).max(), 1.0, "float32")).all()
