@@ -34,7 +34,7 @@ struct StepArrays {
     std::vector<int32_t> input_ids, positions;
     std::vector<int32_t> cu_seqlens_q, cu_seqlens_k;   // prefill
     std::vector<int32_t> slot_mapping;
-    std::vector<int32_t> context_lens;                 // decode
+    std::vector<int32_t> context_lens;                 // decode; prefill by sequences
     std::vector<int32_t> block_tables;                 // [num_seqs, max_blocks] zero padded; empty = none
     int64_t max_blocks = 0;
     int max_seqlen_q = 0, max_seqlen_k = 0;
@@ -43,7 +43,11 @@ struct StepArrays {
 // slot = block_table[t / block_size] * block_size + t % block_size for every token of the chunk;
 // cu_seqlens_k counts all keys attended so far; block tables only when some sequence has keys beyond
 // its new tokens (prefix hit or later chunk), exactly as the reference decides (model_runner.cpp:548-551).
-StepArrays build_prefill_arrays(const std::vector<SequenceView>& seqs, int block_size);
+//
+// `by_sequences` (not in the reference): for a cache whose store goes by sequences (Attention::set_kv_cache_blocks8).  Block tables always, and context_lens: how many positions of a sequence
+// there are with its new rows as the last ones.  0, which stores nothing, where all of the chunk is in the cached prefix (a prompt that is cached whole computes its last token again): its
+// rows are there, in blocks that others share and that no second sequence may write to.  A chunk that begins inside the cached prefix and ends behind it is refused.
+StepArrays build_prefill_arrays(const std::vector<SequenceView>& seqs, int block_size, bool by_sequences = false);
 
 // input = last token, position = len - 1, context_len = len, slot of the last token; block tables padded
 // to the longest table of the batch.

@@ -14,7 +14,7 @@ struct Context {
     int max_seqlen_q = 0;
     int max_seqlen_k = 0;
     Tensor slot_mapping;   // [tokens] int32, -1 = padding
-    Tensor context_lens;   // [batch] int32, decode (includes the token being generated)
+    Tensor context_lens;   // [batch] int32, decode (includes the token being generated); a prefill's where the store goes by sequences
     Tensor block_tables;   // [batch, max_blocks] int32, zero padded
     int64_t total_seqlen_k = 0;   // the last element of cu_seqlens_k, prefill; 0: the host does not know it (not in the reference)
 };

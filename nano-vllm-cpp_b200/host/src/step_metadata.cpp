@@ -33,7 +33,7 @@ void fill_block_tables(const std::vector<SequenceView>& seqs, StepArrays& out) {
 
 }  // namespace
 
-StepArrays build_prefill_arrays(const std::vector<SequenceView>& seqs, int block_size) {
+StepArrays build_prefill_arrays(const std::vector<SequenceView>& seqs, int block_size, bool by_sequences) {
     if (seqs.empty()) throw std::invalid_argument("prepare_prefill requires at least one sequence");
     if (block_size <= 0) throw std::invalid_argument("block size must be positive");
     StepArrays out;
@@ -60,12 +60,18 @@ StepArrays build_prefill_arrays(const std::vector<SequenceView>& seqs, int block
             out.slot_mapping.push_back(s.block_table[t / block_size] * block_size + t % block_size);
         }
         const int q_len = end - begin, k_len = end;
+        if (by_sequences) {
+            const bool cached = end <= s.num_cached_tokens;
+            if (!cached && begin < s.num_cached_tokens)
+                throw std::invalid_argument("prepare_prefill: a chunk that is stored by sequences may not begin inside the cached prefix and end behind it");
+            out.context_lens.push_back(cached ? 0 : end);
+        }
         out.cu_seqlens_q.push_back(out.cu_seqlens_q.back() + q_len);
         out.cu_seqlens_k.push_back(out.cu_seqlens_k.back() + k_len);
         out.max_seqlen_q = std::max(out.max_seqlen_q, q_len);
         out.max_seqlen_k = std::max(out.max_seqlen_k, k_len);
     }
-    if (out.cu_seqlens_k.back() > out.cu_seqlens_q.back()) fill_block_tables(seqs, out);
+    if (by_sequences || out.cu_seqlens_k.back() > out.cu_seqlens_q.back()) fill_block_tables(seqs, out);
     return out;
 }
 
@@ -188,7 +194,7 @@ ModelInputs StepUploader::upload(const StepArrays& a, cudaStream_t stream) {
     Tensor tables = a.block_tables.empty() ? Tensor() : view(6, {seqs, a.max_blocks});
     if (a.is_prefill) {
         set_context(true, view(3, {seqs + 1}), view(4, {seqs + 1}), a.max_seqlen_q, a.max_seqlen_k,
-                    view(2, {static_cast<int64_t>(a.slot_mapping.size())}), Tensor(), tables, a.cu_seqlens_k.back());
+                    view(2, {static_cast<int64_t>(a.slot_mapping.size())}), view(5, {seqs}), tables, a.cu_seqlens_k.back());
     } else {
         set_context(false, Tensor(), Tensor(), 0, 0, view(2, {seqs}), view(5, {seqs}), tables);
     }

@@ -153,4 +153,34 @@ TEST_CASE(step_refuses) {
     CHECK_THROWS(release_blocks(wide, none, t), std::invalid_argument);
 }
 
+TEST_CASE(prefill_arrays_by_sequences) {
+    // Blocks of 4: a prompt of 6, one of 8 of which 4 are cached, one that is cached whole, the chunk [5, 7) of one of 9.
+    std::vector<int32_t> tokens(9, 1);
+    auto view = [&](int n, const std::vector<int32_t>& table, int cached, int computed = 0, int chunk = 0) {
+        SequenceView s;
+        s.token_ids = tokens.data();
+        s.num_tokens = n;
+        s.num_cached_tokens = cached;
+        s.num_computed_tokens = computed;
+        s.num_tokens_to_process = chunk;
+        s.block_table = table.data();
+        s.block_table_len = static_cast<int32_t>(table.size());
+        return s;
+    };
+    const std::vector<int32_t> a = {3, 1}, b = {5, 6}, c = {5, 7}, d = {0, 2, 4};
+    const StepArrays x = build_prefill_arrays({view(6, a, 0), view(8, b, 4), view(8, c, 8), view(9, d, 4, 5, 2)}, 4, true);
+    CHECK_EQ(x.cu_seqlens_q, (std::vector<int32_t>{0, 6, 10, 11, 13}));
+    CHECK_EQ(x.cu_seqlens_k, (std::vector<int32_t>{0, 6, 14, 22, 29}));
+    CHECK_EQ(x.context_lens, (std::vector<int32_t>{6, 8, 0, 7}));
+    CHECK_EQ(x.max_blocks, int64_t(3));
+    CHECK_EQ(x.block_tables, (std::vector<int32_t>{3, 1, 0, 5, 6, 0, 5, 7, 0, 0, 2, 4}));
+    // without a cached key too; and nothing of it unless asked for
+    const StepArrays fresh = build_prefill_arrays({view(6, a, 0)}, 4, true), slots = build_prefill_arrays({view(6, a, 0)}, 4);
+    CHECK_EQ(fresh.context_lens, (std::vector<int32_t>{6}));
+    CHECK_EQ(fresh.block_tables, a);
+    CHECK(slots.context_lens.empty() && slots.block_tables.empty());
+    CHECK_THROWS(build_prefill_arrays({view(9, d, 4, 2, 5)}, 4, true), std::invalid_argument);
+    CHECK_EQ(build_prefill_arrays({view(9, d, 4, 2, 5)}, 4).positions.front(), 2);
+}
+
 int main() { return check::run_all(); }

@@ -13,6 +13,7 @@
 
 #include <cuda_runtime_api.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -127,6 +128,65 @@ TEST_CASE(rotary_of_packed_rows) {
             }
         }
     }
+}
+
+TEST_CASE(prompts_and_chunks_of_the_host_path) {
+    // What StepUploader publishes, into the layer: prompts, chunks of them, one behind a cached prefix, one that is cached whole; then decode.
+    CudaAllocator& alloc = CudaAllocator::instance();
+    Attention eight(kHeads, kKvHeads, kDim, kBlock), full(kHeads, kKvHeads, kDim, kBlock);
+    const int blocks = 40;
+    eight.set_kv_cache_blocks8(Tensor::zeros({blocks, kBlock, kKvHeads, kDim}, ScalarType::kInt8, kDev, alloc),
+                               Tensor::zeros({blocks, kBlock, kKvHeads, kDim}, ScalarType::kInt8, kDev, alloc),
+                               Tensor::zeros({blocks, kKvHeads}, ScalarType::kFloat32, kDev, alloc), Tensor::zeros({blocks, kKvHeads}, ScalarType::kFloat32, kDev, alloc));
+    full.set_kv_cache(Tensor::zeros({blocks, kBlock, kKvHeads, kDim}, ScalarType::kBFloat16, kDev, alloc),
+                      Tensor::zeros({blocks, kBlock, kKvHeads, kDim}, ScalarType::kBFloat16, kDev, alloc));
+    std::vector<int32_t> tokens(200, 1);
+    const std::vector<std::vector<int32_t>> tables = {{9, 30, 2}, {17, 4}, {9, 30, 21, 8}, {17, 4}, {11}};   // the third has two blocks of the first, the fourth all of the second
+    const std::vector<int> lens = {48, 32, 61, 32, 1}, cached = {0, 0, 32, 32, 0};
+    auto view = [&](int i, int computed, int chunk) {
+        SequenceView s;
+        s.token_ids = tokens.data();
+        s.num_tokens = lens[i];
+        s.num_cached_tokens = cached[i];
+        s.num_computed_tokens = computed;
+        s.num_tokens_to_process = chunk;
+        s.block_table = tables[i].data();
+        s.block_table_len = static_cast<int32_t>(tables[i].size());
+        return s;
+    };
+    StepUploader uploader(alloc, kDev);
+    const std::vector<std::vector<SequenceView>> steps = {{view(0, 0, 33), view(1, 0, 0), view(4, 0, 0)}, {view(0, 33, 15)}, {view(2, 0, 0), view(3, 0, 0)}};
+    for (const auto& seqs : steps) {
+        const StepArrays step = build_prefill_arrays(seqs, kBlock, true);
+        uploader.upload(step);
+        CHECK(get_context().context_lens.defined() && get_context().block_tables.defined());
+        const int rows = static_cast<int>(step.input_ids.size());
+        const Tensor q = queries(rows), k = numbers(rows), v = numbers(rows);
+        if (&seqs == &steps[2]) {   // the last row of a prompt that is cached whole is the one that is there: nothing of it is stored in the 8-bit cache, so that the 16-bit one must not either
+            const std::vector<uint16_t> k_rows = download<uint16_t>(full.k_cache()), v_rows = download<uint16_t>(full.v_cache());
+            const size_t row = kKvHeads * kDim, from = (4 * kBlock + 15) * row;
+            CHECK_EQ(step.slot_mapping.back(), 4 * kBlock + 15);
+            alloc.copy_to_device_async(static_cast<uint16_t*>(k.data()) + (rows - 1) * row, k_rows.data() + from, row * 2, nullptr);
+            alloc.copy_to_device_async(static_cast<uint16_t*>(v.data()) + (rows - 1) * row, v_rows.data() + from, row * 2, nullptr);
+            alloc.synchronize_stream(nullptr);
+        }
+        const std::vector<int8_t> before = download<int8_t>(eight.k_cache());
+        check_close(eight.forward(q, k, v, alloc), full.forward(q, k, v, alloc));
+        const std::vector<int8_t> after = download<int8_t>(eight.k_cache());
+        if (&seqs == &steps[2]) {
+            for (int block : {9, 30, 17, 4}) {
+                const size_t at = static_cast<size_t>(block) * kBlock * kKvHeads * kDim;
+                CHECK(std::equal(before.begin() + at, before.begin() + at + kBlock * kKvHeads * kDim, after.begin() + at));
+            }
+        }
+    }
+    std::vector<SequenceView> all;
+    for (int i : {0, 2, 4}) all.push_back(view(i, 0, 0));
+    uploader.upload(build_decode_arrays(all, kBlock));
+    const Tensor q = queries(3), k = numbers(3), v = numbers(3);
+    check_close(eight.forward(q, k, v, alloc), full.forward(q, k, v, alloc));
+    throw_if_prefill_error();
+    reset_context();
 }
 
 int main() { return check::run_all(); }
