@@ -23,7 +23,8 @@ public:
     void set_kv_cache_int4(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_params, const Tensor& v_params);
     // 8-bit caches [blocks, block_size, Hkv, 128] (byte tensors, int8; `e4m3`: of e4m3 elements) with one float32 scale for each block and KV head [blocks, Hkv].  The store goes by
     // sequences, so that the context of every step, a prefill's too, has context_lens and block_tables (build_step gives both, and so does build_prefill_arrays with `by_sequences`); decode reads the cache through
-    // launch_decode_attention_paged_blocks8, and a prefill attends over the rows that gather_kvcache_blocks8 brings out of it, as with a 4-bit cache.
+    // launch_decode_attention_paged_blocks8, and a prefill attends over the rows that gather_kvcache_blocks8 brings out of it, as with a 4-bit cache.  Where the
+    // context says that there are only new keys (StepUploader does; after build_step whoever knows it), a prefill attends over the dense K / V it was given.
     void set_kv_cache_blocks8(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale, bool e4m3 = false);
     // From here on decode steps over a 16-bit or a 4-bit cache add every key's attention weights to `key_weights` [rows, Hkv, keys], float32, for
     // evict_kvcache; `rows` [batch] or undefined, as there.  Undefined weights: no longer.

@@ -17,6 +17,7 @@ struct Context {
     Tensor context_lens;   // [batch] int32, decode (includes the token being generated); a prefill's where the store goes by sequences
     Tensor block_tables;   // [batch, max_blocks] int32, zero padded
     int64_t total_seqlen_k = 0;   // the last element of cu_seqlens_k, prefill; 0: the host does not know it (not in the reference)
+    bool only_new_keys = false;   // prefill: the host knows that every sequence's keys are its new ones, none of them cached before (not in the reference)
 };
 
 Context& get_context();
@@ -29,7 +30,8 @@ void set_context(bool is_prefill,
                  const Tensor& slot_mapping = Tensor(),
                  const Tensor& context_lens = Tensor(),
                  const Tensor& block_tables = Tensor(),
-                 int64_t total_seqlen_k = 0);
+                 int64_t total_seqlen_k = 0,
+                 bool only_new_keys = false);
 void reset_context();
 
 }  // namespace nano_vllm

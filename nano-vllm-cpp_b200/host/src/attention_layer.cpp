@@ -170,7 +170,7 @@ Tensor Attention::forward(const Tensor& query, const Tensor& key, const Tensor& 
     if (ctx.is_prefill) {
         const Tensor* cu_q = ctx.cu_seqlens_q.defined() ? &ctx.cu_seqlens_q : nullptr;
         const Tensor* cu_k = ctx.cu_seqlens_k.defined() ? &ctx.cu_seqlens_k : nullptr;
-        if (paged && (is_int4_ || is_blocks8_)) {
+        if (paged && (is_int4_ || is_blocks8_) && !ctx.only_new_keys) {   // (new keys alone are at hand as they are, not rounded)
             if (cu_q == nullptr || cu_k == nullptr) throw std::invalid_argument("prefill attention with block_tables requires cu_seqlens_q and cu_seqlens_k");
             const int64_t seqs = static_cast<int64_t>(cu_k->numel()) - 1;
             const int64_t longest = ctx.max_seqlen_k > 0 ? ctx.max_seqlen_k : ctx.block_tables.sizes().back() * block_size_;
@@ -180,7 +180,7 @@ Tensor Attention::forward(const Tensor& query, const Tensor& key, const Tensor& 
             if (is_int4_) gather_kvcache_int4(k_cache_, v_cache_, k_scale_, v_scale_, *cu_k, ctx.block_tables, num_kv_heads_, head_dim_, block_size_, dense_k, dense_v, stream);
             else gather_kvcache_blocks8(k_cache_, v_cache_, k_scale_, v_scale_, *cu_k, ctx.block_tables, dense_k, dense_v, is_e4m3_, stream);
             launch_prefill_attention_dense(query, cu_q, dense_k, dense_v, cu_k, num_kv_heads_, head_dim_, scale_, output, stream, ctx.max_seqlen_q);
-        } else if (paged && !is_int8_) {   // an int8 cache is only read by decode: prefill attends over the dense K / V it was given
+        } else if (paged && !is_quantised()) {   // an int8 cache is only read by decode: prefill attends over the dense K / V it was given
             if (cu_k == nullptr) throw std::invalid_argument("prefill attention with block_tables requires cu_seqlens_k");
             launch_prefill_attention_paged(query, cu_q, k_cache_, v_cache_, cu_k, ctx.block_tables, num_kv_heads_,
                                            head_dim_, block_size_, scale_, output, stream, ctx.max_seqlen_q);

@@ -196,7 +196,7 @@ void set_context(const Context& context) { t_context = context; }
 
 void set_context(bool is_prefill, const Tensor& cu_seqlens_q, const Tensor& cu_seqlens_k, int max_seqlen_q,
                  int max_seqlen_k, const Tensor& slot_mapping, const Tensor& context_lens, const Tensor& block_tables,
-                 int64_t total_seqlen_k) {
+                 int64_t total_seqlen_k, bool only_new_keys) {
     Context& c = t_context;
     c.is_prefill = is_prefill;
     c.cu_seqlens_q = cu_seqlens_q;
@@ -207,6 +207,7 @@ void set_context(bool is_prefill, const Tensor& cu_seqlens_q, const Tensor& cu_s
     c.context_lens = context_lens;
     c.block_tables = block_tables;
     c.total_seqlen_k = total_seqlen_k;
+    c.only_new_keys = only_new_keys;
 }
 
 void reset_context() { t_context = Context{}; }

@@ -194,7 +194,8 @@ ModelInputs StepUploader::upload(const StepArrays& a, cudaStream_t stream) {
     Tensor tables = a.block_tables.empty() ? Tensor() : view(6, {seqs, a.max_blocks});
     if (a.is_prefill) {
         set_context(true, view(3, {seqs + 1}), view(4, {seqs + 1}), a.max_seqlen_q, a.max_seqlen_k,
-                    view(2, {static_cast<int64_t>(a.slot_mapping.size())}), view(5, {seqs}), tables, a.cu_seqlens_k.back());
+                    view(2, {static_cast<int64_t>(a.slot_mapping.size())}), view(5, {seqs}), tables, a.cu_seqlens_k.back(),
+                    a.cu_seqlens_k.back() == a.cu_seqlens_q.back());   // (no sequence has fewer keys than queries)
     } else {
         set_context(false, Tensor(), Tensor(), 0, 0, view(2, {seqs}), view(5, {seqs}), tables);
     }

@@ -189,4 +189,43 @@ TEST_CASE(prompts_and_chunks_of_the_host_path) {
     reset_context();
 }
 
+TEST_CASE(prompts_without_cached_keys_attend_over_exact_rows) {
+    // Keys and values that no 8-bit element stands for: bit for bit what a layer without a cache gives, where over the cache's rows there would be a difference.
+    CudaAllocator& alloc = CudaAllocator::instance();
+    auto halves = [](int rows) {
+        std::vector<uint16_t> v;
+        for (int i = 0; i < rows * kKvHeads * kDim; ++i) v.push_back(bf16((static_cast<float>(next_random() % 255) - 127.0f) * (i % 3 ? 1.0f : 1.0f / 128)));
+        return upload({rows, kKvHeads, kDim}, ScalarType::kBFloat16, v);
+    };
+    Attention eight(kHeads, kKvHeads, kDim, kBlock), none(kHeads, kKvHeads, kDim, kBlock);
+    eight.set_kv_cache_blocks8(Tensor::zeros({6, kBlock, kKvHeads, kDim}, ScalarType::kInt8, kDev, alloc), Tensor::zeros({6, kBlock, kKvHeads, kDim}, ScalarType::kInt8, kDev, alloc),
+                               Tensor::zeros({6, kKvHeads}, ScalarType::kFloat32, kDev, alloc), Tensor::zeros({6, kKvHeads}, ScalarType::kFloat32, kDev, alloc));
+    const std::vector<int32_t> tokens(40, 1), a = {4, 1, 0}, b = {2};
+    std::vector<SequenceView> seqs(2);
+    seqs[0].token_ids = seqs[1].token_ids = tokens.data();
+    seqs[0].num_tokens = 40; seqs[0].block_table = a.data(); seqs[0].block_table_len = 3;
+    seqs[1].num_tokens = 7; seqs[1].block_table = b.data(); seqs[1].block_table_len = 1;
+    StepUploader uploader(alloc, kDev);
+    uploader.upload(build_prefill_arrays(seqs, kBlock, true));
+    CHECK(get_context().only_new_keys);
+    const Tensor q = queries(47), k = halves(47), v = halves(47);
+    const std::vector<uint16_t> exact = download<uint16_t>(eight.forward(q, k, v, alloc));
+    Context context = get_context();
+    context.only_new_keys = false;
+    set_context(context);
+    const std::vector<uint16_t> rounded = download<uint16_t>(eight.forward(q, k, v, alloc));
+    context.block_tables = Tensor();
+    set_context(context);
+    const std::vector<uint16_t> want = download<uint16_t>(none.forward(q, k, v, alloc));
+    CHECK(exact == want);
+    CHECK(rounded != want);
+    // behind cached keys there is more than the new ones
+    seqs[0].num_computed_tokens = 30;
+    seqs[0].num_tokens_to_process = 10;
+    uploader.upload(build_prefill_arrays({seqs[0]}, kBlock, true));
+    CHECK(!get_context().only_new_keys);
+    reset_context();
+    CHECK(!get_context().only_new_keys);
+}
+
 int main() { return check::run_all(); }
