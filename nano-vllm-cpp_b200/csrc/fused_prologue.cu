@@ -31,24 +31,6 @@ constexpr int kFewWarps = 4;
 // find a place on an SM, and a second wave of them is where fused_prologue_kernel draws level (700 rows of 32 / 8 heads 4.3 us a call in one, 4.35 in the other).
 constexpr int kFewUnits = 9472;
 
-// Packed fp32 pairs (one 64-bit register pair per two values; Blackwell executes f32x2 mul / fma at one issue slot).
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2_make(float lo, float hi) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void f2_split(F2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 template <typename T> __device__ __forceinline__ F2 f2_unpack(uint32_t w);   // two 16-bit elements -> two floats
 template <> __device__ __forceinline__ F2 f2_unpack<__nv_bfloat16>(uint32_t w) {
     return f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));

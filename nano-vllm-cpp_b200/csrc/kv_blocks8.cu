@@ -58,18 +58,6 @@ template <typename T, bool FP8> __device__ __forceinline__ float scale_for(uint3
 // The larger of a block's scale and of what its new rows ask for; (no scale is negative, and NaN is above all others as a whole number).
 __device__ __forceinline__ float larger(float a, float b) { return __int_as_float(max(__float_as_int(a), __float_as_int(b))); }
 
-__device__ __forceinline__ uint32_t pack_s8x4(int e0, int e1, int e2, int e3) {   // bytes {e0, e1, e2, e3}, e0 lowest
-    uint32_t hi, out;
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;\n" : "=r"(hi) : "r"(e3), "r"(e2), "r"(0));
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;\n" : "=r"(out) : "r"(e1), "r"(e0), "r"(hi));
-    return out;
-}
-__device__ __forceinline__ uint32_t pack_e4m3x4(float e0, float e1, float e2, float e3) {
-    unsigned short lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(lo) : "f"(e1), "f"(e0));   // first source -> upper byte
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(e3), "f"(e2));
-    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
-}
 template <bool FP8> __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
     if constexpr (FP8) return pack_e4m3x4(a, b, c, d);
     else return pack_s8x4(__float2int_rn(a), __float2int_rn(b), __float2int_rn(c), __float2int_rn(d));

@@ -119,14 +119,6 @@ __device__ __forceinline__ typename Pair16<T>::type absmax8(const uint4& v) {
     return __hmax2(m, __lowhigh2highlow(m));
 }
 
-// bytes {e0, e1, e2, e3} (e0 lowest) of four integers, each saturated to int8
-__device__ __forceinline__ uint32_t pack_s8x4(int e0, int e1, int e2, int e3) {
-    uint32_t hi, out;
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;\n" : "=r"(hi) : "r"(e3), "r"(e2), "r"(0));
-    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;\n" : "=r"(out) : "r"(e1), "r"(e0), "r"(hi));
-    return out;
-}
-
 template <typename T>
 __device__ __forceinline__ uint2 quantise8(const uint4& v, float inv) {
     using P = Pair16<T>;
@@ -178,12 +170,6 @@ store_int8_packed_kernel(const T* __restrict__ key, const T* __restrict__ value,
 // ---- fp8 (e4m3) cache: the packed kernel with the other element type.  No counterpart in the reference; the format follows
 // its int8 cache: one fp16 scale per (cache row, KV head) = max(absmax / 448, 1e-10), elements = e4m3(x * 448 / max(absmax,
 // 1e-10)) rounded to nearest even from the fp32 product, saturating at +-448.
-__device__ __forceinline__ uint32_t pack_e4m3x4(float e0, float e1, float e2, float e3) {   // bytes {e0, e1, e2, e3}, e0 lowest
-    unsigned short lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(lo) : "f"(e1), "f"(e0));   // first source -> upper byte
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(hi) : "f"(e3), "f"(e2));
-    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
-}
 template <typename T>
 __device__ __forceinline__ uint2 quantise8_e4m3(const uint4& v, float inv) {
     using P = Pair16<T>;

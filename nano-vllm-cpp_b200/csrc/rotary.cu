@@ -48,29 +48,6 @@ template <typename T, int V> union Elems {
     T e[V];
 };
 
-// Two floats in one instruction.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-    F2 d;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(d) : "f"(lo), "f"(hi));
-    return d;
-}
-__device__ __forceinline__ float2 floats(F2 v) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-    F2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-    F2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-
 // V: elements of a piece.  PAIRS: neighbours are pairs.
 template <typename T, int V, bool PAIRS>
 __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
@@ -140,13 +117,15 @@ __global__ void __launch_bounds__(kThreads, 4) rotary_kernel(const __grid_consta
                 // Pairs k and k + 1 of a piece, or of both; where their angles are.
                 auto turn2 = [&](T& a0, T& b0, T& a1, T& b1, int angle) {
                     const float2 c = *reinterpret_cast<const float2*>(s_cos + angle), s = *reinterpret_cast<const float2*>(s_sin + angle);
-                    const F2 c2 = f2(c.x, c.y), s2 = f2(s.x, s.y), n2 = f2(-s.x, -s.y);
-                    const F2 a = f2(E::to_float(a0), E::to_float(a1)), b = f2(E::to_float(b0), E::to_float(b1));
-                    const float2 first = floats(fma2(a, c2, mul2(b, n2))), other = floats(fma2(b, c2, mul2(a, s2)));
-                    a0 = E::from_float(first.x);
-                    a1 = E::from_float(first.y);
-                    b0 = E::from_float(other.x);
-                    b1 = E::from_float(other.y);
+                    const F2 c2 = f2_make(c.x, c.y), s2 = f2_make(s.x, s.y), n2 = f2_make(-s.x, -s.y);
+                    const F2 a = f2_make(E::to_float(a0), E::to_float(a1)), b = f2_make(E::to_float(b0), E::to_float(b1));
+                    float first, second;
+                    f2_split(f2_fma(a, c2, f2_mul(b, n2)), first, second);
+                    a0 = E::from_float(first);
+                    a1 = E::from_float(second);
+                    f2_split(f2_fma(b, c2, f2_mul(a, s2)), first, second);
+                    b0 = E::from_float(first);
+                    b1 = E::from_float(second);
                 };
                 auto turn1 = [&](T& a0, T& b0, int angle) {
                     const float a = E::to_float(a0), b = E::to_float(b0), c = s_cos[angle], s = s_sin[angle];
