@@ -302,6 +302,8 @@ int nvk_release_blocks(const void* request_rows, const void* first_blocks, const
  *   NVK_ROPE_BASE     theta_i of the base base * factor^(rotary_dim / (rotary_dim - 2)), which takes the slowest pair to theta / factor; rotary_dim > 2
  *   NVK_ROPE_PARTS    (1 - g) theta_i / factor + g theta_i, g = (turns - low_turns) / (high_turns - low_turns) held in [0, 1], turns = original_positions theta_i / 2 pi
  *   NVK_ROPE_YARN     the same, and *attention_factor = 0.1 ln(factor) + 1 (Peng et al., YaRN, 2023); 1 otherwise
+ * PARTS and YARN go by the number of turns, as the paper has it.  A model that was stretched by a ramp over the pair's index (between two pairs found from numbers of turns) has other
+ * frequencies between the two: hand its own to nvk_rotary_embedding.
  */
 #define NVK_ROPE_PLAIN 0
 #define NVK_ROPE_LINEAR 1

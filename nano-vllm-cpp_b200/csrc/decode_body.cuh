@@ -761,7 +761,7 @@ struct Cache4 {
 //     head's largest, and one block whose scale is far above the others' does not cost them their bits.
 // Bound by HBM where there is much to do: 256 sequences of 1024 to 8192 keys, 32 / 8 heads, int8, 369 to 390 us by the GPU's own power limit, 6.2 to 6.5 TB/s (e4m3 368; 414 and, after some
 // time at the limit, 478 us with 16 keys at a time and K and V by way of f16 as Cache8 has them: 417 instructions for 16 keys, some 250 now).  256 of 100 to 2048 keys of one KV
-// head: 15.0 us with the cache in L2, 19.2 beyond it, of 10.9: the longest context alone is 12 us of an SM's share.  One of 300 keys: 3.9 us, latency.
+// head: int8 17.3, e4m3 15.0 us with the cache in L2, e4m3 19.2 beyond it, of 10.9: the longest context alone is 12 us of an SM's share.  One of 300 keys: 3.9 us, latency.
 __device__ __forceinline__ void imma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, const int (&c)[4]) {
     asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
                  : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])

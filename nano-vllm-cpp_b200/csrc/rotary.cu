@@ -12,7 +12,9 @@
 // Bound by HBM for many rows (every element is read and written once), by the trip to memory and the launch for few.  A thread takes two pieces of V elements of a head, i and rot / 2 + i,
 // which hold V pairs whole in either layout, and the lanes' pieces lie next to each other (pairs of neighbours in two pieces next to each other: 59.2 instead of 53.9 us below, in F32 56.3 instead
 // of 50.5).  Two pairs are turned by one instruction (f32x2), three items of a thread are under way at once, in 64 registers: 16384 rows of 32 / 8 heads of 128, BF16, halves, take 54.9 us
-// (6.1 TB/s; one pair at a time 62.7, four items at once 57.0, two 58.1), neighbours 53.9, 4096 rows 13.1, one row 1.9.
+// (6.1 TB/s; one pair at a time 62.7, four items at once 57.0, two 58.1), neighbours 53.9, 4096 rows 13.1, one row 1.9.  Where half of the rotated part is no multiple of 16 bytes all of a
+// head goes in the pieces that it allows, what is only copied too: 16384 rows of 32 / 8 heads of 80 with 20 rotated, BF16, 71.9 us (2.9 TB/s; in place, where nothing is copied, 22.8), of 96
+// with 24 82.3 (3.1; 21.6), of 80 with 20 in F32 87.9 (4.8; 36.2).
 #include "nvk_internal.cuh"
 
 #include <algorithm>

@@ -8,9 +8,10 @@
 // A call is bound by the trips to memory one after the other (row, its length and its blocks) and by the launch.  So every block does the sums over the whole batch for itself, so that
 // nothing is handed over, and the blocks share out the table entries and the tokens.  Lengths and the count of free blocks may be updated in place, when every block has read them.  Where
 // they are, the blocks are one cluster, whose first one writes them behind a barrier, up to four pieces of 16 bytes to a thread; beyond, and wherever the new ones are of their own, there
-// are as many blocks as the work is worth, and what is updated in place follows in a kernel of one block.  us, in a cluster / by many blocks (and that kernel): 256 requests, table rows of 33
-// int32 (8448 pieces) 3.9 / 5.0, 16 of 2304 new tokens, int64 (36864 pieces) 5.7 / 4.9, 1024 with rows of 33 6.2 / 7.1, of 129 (132096) 9.2 / 8.0.  Of their own: 3.7, 4.5, 5.7, 6.7; a
-// decode step of one request 2.7, of 256 (rows of 32) 3.3, 1024 requests of rows of 512 6.4 (2.1 MB written), 8192 of 33 26 us.  Up to 256 requests by blocks of 256 threads (a scan over
+// are as many blocks as the work is worth, and what is updated in place follows in a kernel of one block.  us, in a cluster / by many blocks (and that kernel), behind a small copy: 256 requests, table
+// rows of 33 int32 (8448 pieces) 4.1 / 5.2, 16 of 2304 new tokens, int64 (36864 pieces) 5.2 / 5.4, 1024 with rows of 33 6.2 / 7.1, of 129 (132096) 8.1 / 7.2.  Of their own: 3.8, 3.9, 5.9,
+// 6.0; steps one after the other, a decode step of one request 2.8, of 256 (rows of 32) 3.4, 1024 requests of rows of 512 6.5 (2.1 MB written), 8192 of 33 26 us (every block goes through
+// the batch 1024 requests at a time, with two barriers each).  Up to 256 requests by blocks of 256 threads (a scan over
 // 1024 takes 1 us more: 256 requests, rows of 33, 4.7), beyond by 1024.
 #include "nvk_internal.cuh"
 
