@@ -365,8 +365,8 @@ int chunk_tokens4(int64_t pairs, int64_t max_tokens) {   // 0: as with 8 bits
 // 1024 10.6 / 11.9 / 14.4, 15.2 / 19.1 / 22.2 -> 8.7 / 9.2 / 13.2, 14.6 / 17.1 / 19.4; 160 of 2048 10.2 / 13.1 / 14.6, 15.6 / 21.6 / 24.3 -> 10.0 / 13.2 / 15.9, 16.0 / 17.0 / 18.2 (by eight
 // warps 12.5 / 13.6 / 14.2, 14.4 / 20.8 / 27.9); but 384 of 2048 by four warps 18.8 / 21.7 / 28.8, 27.6 / 31.9 / 37.0, by eight 14.0 / 16.7 / 23.1, 28.7 / 35.4 / 43.3.
 bool halves_of_block_scales(int64_t pairs, int64_t max_tokens) { return pairs > kSmCount && 2 * pairs <= 3 * kSmCount && max_tokens >= 1024 && max_tokens <= 2048; }
-// From two pairs to an SM on, where tables of up to 1280 keys are whole contexts by four warps anyway, three blocks to an SM, they stay that, for what one context in three that fills its
-// table costs: 296 of 1024 by eight 12.0 / 14.4 / 15.2, 15.9 / 18.6 / 21.0, by four 10.1 / 13.5 / 16.2, 15.9 / 16.7 / 17.3; 320 12.6 / 14.8 / 15.5, 19.9 / 24.5 / 28.4 and 9.8 / 13.4 / 16.3,
+// From two pairs to an SM on, where tables of up to 1280 keys are whole contexts by four warps anyway, three blocks to an SM, they stay that, which costs
+// something only where a third of the contexts fill their tables: 296 of 1024 by eight 12.0 / 14.4 / 15.2, 15.9 / 18.6 / 21.0, by four 10.1 / 13.5 / 16.2, 15.9 / 16.7 / 17.3; 320 12.6 / 14.8 / 15.5, 19.9 / 24.5 / 28.4 and 9.8 / 13.4 / 16.3,
 // 16.1 / 16.9 / 17.6; 320 of 1280 12.7 / 15.0 / 16.4, 21.2 / 26.8 / 32.6 and 11.5 / 15.8 / 19.2, 18.7 / 19.7 / 20.8.
 bool eight_warps_of_block_scales(int64_t pairs, int64_t max_tokens) {
     return !halves_of_block_scales(pairs, max_tokens) && max_tokens >= 1024 && max_tokens <= 2048 && pairs <= 320 && (pairs < 2 * kSmCount || max_tokens > 1280);

@@ -939,8 +939,8 @@ struct CacheBlocks8 {
         const float w = fast_exp2(x);
         return std::is_same<T, __half>::value ? fmaf(w, -8192.0f, fmaf(w, 8192.0f, w)) : w;
     }
-    // s 2^-E for a product with p that must not become 0 times infinity: it passes 2^126 only where every p of its keys is zero, since no p s 2^-E is above 2^8 and no p but
-    // zero below 2^-126.  (Keys that lead all others by 2^126 and have values of nothing, whose s is small; NaN stays NaN.)
+    // s 2^-E for a product with p that must not become 0 times infinity.  Where it is 2^7 and more, E has just been chosen so that no p s 2^-E of these keys is above 1; so it passes 2^126 only
+    // where every p is zero, there being none between 0 and 2^-126.  (Keys that lead all others by 2^126 and have values of nothing, whose s is small; NaN stays NaN.)
     static __device__ __forceinline__ float at_most(float x) {
         float y;
         asm("min.NaN.f32 %0, %1, 0f7E800000;\n" : "=f"(y) : "f"(x));
